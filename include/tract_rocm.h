@@ -465,6 +465,83 @@ int trocm_quantized_kv_sdpa_eval(const void *q, const void *k_new, const void *v
                                  int64_t n_new, trocm_kivi_cache *k_cache, trocm_kivi_cache *v_cache, void *out,
                                  float scale, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- around attention: norms with the rotation, a prefix that sequences share, scored attention ----------------
+ * Parts of decoders that the reference's graphs spell out in elementary ops (or has no op for): no counterpart to cite
+ * unless a line names one.  F32 and F16; everything between the inputs and the one rounding at the end is f32. */
+
+/* RMS norm of every query head and key head, scaled by a weight per feature, then the rotation by position
+ * (RotateHalf as apply_rope.rs:58-76), q and k in one launch:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight,   out = y * cos + RotateHalf(y) * sin.
+ * q [batch, q_heads, n, head_dim] and k [batch, kv_heads, n, head_dim] with element strides q_strides[4] and
+ * k_strides[4] (NULL: dense; the last must be 1): views into the rows of a fused projection are legal.  Weights
+ * [head_dim] of `dtype` (NULL: ones).  cos and sin: [n, head_dim] rows of `dtype` per batch entry, `cos_sin_batch_stride`
+ * elements apart (0: one set of rows for all).  q_out and k_out dense; each may be its own input where that is dense,
+ * and may overlap no other input.  head_dim even; 64, 128 and 256 with everything aligned to 16 bytes move 16 bytes per lane. */
+int trocm_qk_norm_rope(const void *q, const void *k, const void *q_weight, const void *k_weight, float eps, const void *cos,
+                       const void *sin, int64_t cos_sin_batch_stride, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                       int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides, void *q_out, void *k_out,
+                       void *stream);
+
+/* trocm_qk_norm_rope on q and k_new, then trocm_inplace_kv_sdpa_eval: the whole attention block of a decoder with normed
+ * queries and keys.  q_strides, k_strides and v_strides as above (NULL: dense).  Normed rows go through `rot_scratch`
+ * (16-byte aligned), which must hold round_up(batch * q_heads * n_new * head_dim * elem, 256) + batch * kv_heads * n_new *
+ * head_dim * elem bytes.  Every cache of trocm_inplace_kv_sdpa_eval will do.  Checked before anything is changed. */
+int trocm_inplace_kv_sdpa_eval_norm_rope(const void *q, const void *k_new, const void *v_new, const void *q_weight,
+                                         const void *k_weight, float eps, const void *cos, const void *sin,
+                                         int64_t cos_sin_batch_stride, int dtype, int64_t q_heads, int64_t n_new,
+                                         const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
+                                         trocm_kv_cache *k_cache, trocm_kv_cache *v_cache, void *out, float scale, int causal,
+                                         void *workspace, size_t workspace_bytes, void *rot_scratch, size_t rot_scratch_bytes,
+                                         void *stream);
+
+/* Attention of sequences that share a prefix: sequence b attends to the prefix_len keys of the prefix, which are stored
+ * and read once for all, and to its own lens[b] keys behind them.
+ *   q, out          : [n_seq, q_heads, q_len, head_dim] dense, not overlapping
+ *   prefix_k, _v    : [kv_heads, prefix_len, head_dim], element strides prefix_strides[2] for head and token (NULL: dense)
+ *   k, v            : sequence b's rows at b * kv_strides[0], heads and tokens kv_strides[1], [2] apart; read up to lens[b] only
+ *   lens            : n_seq lengths in HOST memory, read before the call returns; 0 is legal (and with an empty prefix the row is zeros)
+ *   causal          : over a sequence's own keys: key j visible to query i iff j <= i + (lens[b] - q_len); the prefix always is
+ *   workspace       : trocm_sdpa_shared_workspace_bytes, initialised by trocm_sdpa_workspace_init and shared like any other;
+ *                     with a smaller one or NULL the call takes fewer splits or a slow kernel
+ * Fast kernels: head_dim 64 and 128, bases and strides multiples of 16 bytes; anything else up to head_dim 2048 is correct and slow. */
+int trocm_sdpa_shared_workspace_bytes(int64_t n_seq, int64_t q_heads, int64_t q_len, int64_t head_dim, size_t *bytes);
+int trocm_sdpa_shared_prefix(const void *q, int dtype, int64_t n_seq, int64_t q_heads, int64_t kv_heads, int64_t q_len,
+                             int64_t head_dim, const void *prefix_k, const void *prefix_v, int64_t prefix_len,
+                             const int64_t *prefix_strides, const void *k, const void *v, const int64_t *kv_strides,
+                             const int64_t *lens, void *out, float scale, int causal, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/* The same over caches: prefix_k_cache and prefix_v_cache (batch 1, may be empty) and one K and one V cache per sequence (batch 1
+ * each), F32 or F16, ordinary ones.  With k_new and v_new (dense [n_seq, kv_heads, n_new, head_dim]) it is a step: they are
+ * appended to the sequences' caches first, which must all be different; with both NULL it attends to what the caches hold
+ * (n_new is then only the number of queries per sequence).  Everything is checked before any cache changes. */
+int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const void *v_new, int dtype, int64_t q_heads, int64_t n_seq,
+                                      int64_t n_new, const trocm_kv_cache *prefix_k_cache, const trocm_kv_cache *prefix_v_cache,
+                                      trocm_kv_cache *const *k_caches, trocm_kv_cache *const *v_caches, void *out, float scale,
+                                      int causal, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention whose scores go through more than a scale before the softmax: trocm_sdpa with
+ *   s = scale * q.k;   softcap > 0: s = softcap * tanh(s / softcap);   slopes: s -= slopes[head] * |i + kv_len - q_len - j|
+ * and key j visible to query i iff
+ *   (not causal, or j <= i + (kv_len - q_len), or j < prefix_lens[b])
+ *   and, with documents, both tokens are of one document: documents[b][j] == documents[b][i + kv_len - q_len] >= 0.
+ *   slopes      : [q_heads] f32, device memory, or NULL
+ *   documents   : [batch, kv_len] int32, device memory, or NULL; ids in any order, negative ones are padding that nothing sees
+ *                 and whose K and V rows may hold anything; needs kv_len >= q_len
+ *   prefix_lens : [batch] int32, device memory, or NULL; values past kv_len mean all of it; read only when causal
+ * A row that sees nothing is zeros.  K and V rows that some query of the call sees must be finite: a weight of zero times an
+ * infinite value is NaN for the other queries too.  out may not overlap q, k or v.  k, v, strides, scale and workspace as for trocm_sdpa. */
+int trocm_sdpa_scored(const void *q, const void *k, const void *v, void *out, int dtype, int64_t batch, int64_t q_heads,
+                      int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t head_dim, const int64_t *kv_strides, float scale,
+                      float softcap, const float *slopes, const int32_t *documents, const int32_t *prefix_lens, int causal,
+                      void *workspace, size_t workspace_bytes, void *stream);
+/* The same over the valid region of two caches (F32 or F16, ordinary ones: a ring buffer does not keep its tokens in order);
+ * kv_len is their length.  trocm_kv_append_pair before it makes it a step. */
+int trocm_sdpa_cached_scored(const void *q, int q_dtype, int64_t q_heads, int64_t q_len, const trocm_kv_cache *k_cache,
+                             const trocm_kv_cache *v_cache, void *out, float scale, float softcap, const float *slopes,
+                             const int32_t *documents, const int32_t *prefix_lens, int causal, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

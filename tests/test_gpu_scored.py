@@ -1,0 +1,157 @@
+"""Attention with capped scores, distance slopes, documents and prefixes, against 64 bits."""
+import itertools
+
+import numpy as np
+import pytest
+
+import tract_amd as ta
+from tests.attention_ref import assert_within, scored
+from tests.gpu_util import rt  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+F16, F32 = np.float16, np.float32
+
+
+def _rows(rng, shape, dtype, scale=1.0):
+    return (rng.standard_normal(shape, dtype=np.float32) * scale).astype(dtype)
+
+
+def _slopes(hq):
+    return (2.0 ** (-8.0 * (np.arange(hq) + 1) / hq)).astype(F32)
+
+
+def _packed(rng, b, t, docs):
+    ends = np.sort(rng.integers(0, t, (b, docs - 1)), axis=1)
+    return np.stack([np.searchsorted(e, np.arange(t), side="right") for e in ends]).astype(np.int32)
+
+
+def _check(dtype, b, hq, hkv, n, t, d, cap=0.0, slopes=None, documents=None, prefix_lens=None, causal=True, scale=None, seed=0, big=4.0):
+    rng = np.random.default_rng(seed)
+    q, k, v = _rows(rng, (b, hq, n, d), dtype, big), _rows(rng, (b, hkv, t, d), dtype), _rows(rng, (b, hkv, t, d), dtype)
+    op = ta.ScoredSdpa(scale, cap, causal)
+    rules = dict(slopes=slopes, documents=documents, prefix_lens=prefix_lens)
+    got = op.eval(q, k, v, **rules).to_numpy()
+    assert_within(got, *scored(q, k, v, scale, cap, causal=causal, **rules))
+    return got
+
+
+SHAPES = [(1, 4, 1, 1, 1, 64), (2, 8, 2, 1, 300, 128), (1, 14, 2, 3, 65, 64), (1, 4, 4, 33, 33, 128), (2, 4, 2, 70, 201, 64),
+          (1, 8, 1, 129, 129, 128), (1, 3, 1, 5, 40, 96), (1, 2, 2, 4, 11, 8), (1, 2, 1, 300, 300, 64), (1, 32, 1, 1, 1000, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("rules", list(itertools.product([False, True], repeat=4)), ids=lambda r: "".join("csdp"[i] if x else "-" for i, x in enumerate(r)))
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_every_rule_and_shape(rt, dtype, rules, shape):
+    b, hq, hkv, n, t, d = shape
+    cap, slopes, documents, prefix = rules
+    rng = np.random.default_rng(9)
+    _check(dtype, *shape, cap=15.0 if cap else 0.0, slopes=_slopes(hq) if slopes else None, documents=_packed(rng, b, t, 4) if documents else None,
+           prefix_lens=rng.integers(0, t, b, endpoint=True).astype(np.int32) if prefix else None)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("b,hq,hkv,n,t,d", [(1, 8, 2, 500, 500, 128), (1, 4, 2, 260, 1300, 64), (2, 2, 2, 700, 700, 64), (3, 16, 2, 1, 5000, 128), (1, 6, 1, 11, 3000, 128),
+                                            (1, 7, 1, 640, 641, 64)])
+def test_longer(rt, dtype, b, hq, hkv, n, t, d):
+    rng = np.random.default_rng(10)
+    _check(dtype, b, hq, hkv, n, t, d, cap=30.0)
+    _check(dtype, b, hq, hkv, n, t, d, slopes=_slopes(hq), documents=_packed(rng, b, t, 7))
+    _check(dtype, b, hq, hkv, n, t, d, cap=20.0, prefix_lens=np.array([t // 3] * b, np.int32))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n", [1, 9, 150])
+def test_not_causal_and_scales(rt, dtype, n):
+    rng = np.random.default_rng(11)
+    _check(dtype, 2, 4, 2, n, 190, 64, cap=5.0, causal=False)
+    _check(dtype, 2, 4, 2, n, 190, 64, slopes=_slopes(4), documents=_packed(rng, 2, 190, 3), causal=False, scale=0.02)
+    _check(dtype, 2, 4, 2, n, 190, 64, cap=5.0, causal=False, scale=-0.1)
+    _check(dtype, 2, 4, 2, n, 190, 64, causal=False, scale=0.0)
+    _check(dtype, 1, 4, 2, n, n, 128, cap=1e4)       # hardly a cap at all
+    _check(dtype, 1, 4, 2, n, n, 128, cap=0.01)      # hardly a score left
+    _check(dtype, 1, 4, 2, n, n, 128, cap=50.0, big=60.0)   # scores far beyond the cap
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128, 48])
+@pytest.mark.parametrize("n", [2, 100, 400])
+def test_documents_in_any_order_padding_and_empty_rows(rt, dtype, d, n):
+    rng = np.random.default_rng(12)
+    t = n + 37
+    ids = rng.integers(0, 5, (2, t)).astype(np.int32)      # interleaved
+    ids[0, t // 2 :] = -1                                    # padding: nobody sees it, it sees nobody
+    ids[1, -1] = 77                                          # a document whose only token is the last one
+    q, k, v = _rows(rng, (2, 4, n, d), dtype), _rows(rng, (2, 2, t, d), dtype), _rows(rng, (2, 2, t, d), dtype)
+    want = scored(q, k, v, documents=ids, cap=10.0)
+    k[0, :, t // 2 :], v[0, :, t // 2 :] = np.nan, np.inf    # ... whatever it holds
+    got = ta.ScoredSdpa(softcap=10.0).eval(q, k, v, documents=ids).to_numpy()
+    assert_within(got, *want)
+    empty = ids[0, t - n :] < 0
+    assert not got[0][:, empty].any()
+    assert np.array_equal(got[1, :, -1], np.repeat(v[1, :, -1], 2, axis=0))
+    all_padding = np.full((2, t), -3, np.int32)
+    assert not ta.ScoredSdpa().eval(q, k, v, documents=all_padding).to_numpy().any()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_fewer_keys_than_queries(rt, dtype):
+    """Rows before the first key see nothing; a prefix shows them what it holds."""
+    got = _check(dtype, 1, 4, 2, 50, 20, 64, cap=9.0)
+    assert not got[:, :, :30].any()
+    _check(dtype, 2, 4, 2, 50, 20, 64, prefix_lens=np.array([3, 900], np.int32))
+    _check(dtype, 1, 4, 2, 200, 64, 128, slopes=_slopes(4))
+    q = np.ones((1, 2, 3, 64), dtype)
+    none = np.zeros((1, 1, 0, 64), dtype)
+    assert not ta.ScoredSdpa(softcap=1.0).eval(q, none, none).to_numpy().any()
+
+
+@pytest.mark.parametrize("dtype,b,hq,hkv,d", [(F16, 2, 8, 2, 128), (F32, 1, 4, 2, 64), (F16, 1, 14, 2, 64)])
+def test_session_over_caches(rt, dtype, b, hq, hkv, d):
+    """A prompt, a chunk, single tokens: over the caches as over the tensors they hold; the plain call where no rule is given."""
+    rng = np.random.default_rng(13)
+    kc, vc = ta.InPlaceKvCache(2), ta.InPlaceKvCache(2)
+    whole_k, whole_v = (np.zeros((b, hkv, 0, d), dtype) for _ in range(2))
+    op = ta.ScoredSdpa(softcap=25.0)
+    slopes = _slopes(hq)
+    for n in (130, 40, 1, 1, 5, 1):
+        q = _rows(rng, (b, hq, n, d), dtype, 3.0)
+        kn, vn = (_rows(rng, (b, hkv, n, d), dtype) for _ in range(2))
+        kc.push(kn), vc.push(vn)
+        whole_k, whole_v = np.concatenate([whole_k, kn], axis=2), np.concatenate([whole_v, vn], axis=2)
+        dq = ta.DeviceTensor.from_numpy(q)
+        got = op.eval_cached(dq, kc, vc, slopes=slopes).to_numpy()
+        assert_within(got, *scored(q, whole_k, whole_v, cap=25.0, slopes=slopes))
+        plain = ta.ScoredSdpa().eval_cached(dq, kc, vc).to_numpy()
+        assert_within(plain, *scored(q, whole_k, whole_v))
+
+
+def test_calls_queued_behind_each_other_and_refusals(rt):
+    rng = np.random.default_rng(14)
+    q, k, v = _rows(rng, (1, 8, 1, 128), F16, 4.0), _rows(rng, (1, 2, 4000, 128), F16), _rows(rng, (1, 2, 4000, 128), F16)
+    dq, dk, dv = (ta.DeviceTensor.from_numpy(t) for t in (q, k, v))
+    stream, op = ta.Stream(), ta.ScoredSdpa(softcap=20.0)
+    outs = [op.eval(dq, dk, dv, stream=stream) for _ in range(20)]   # one workspace, one stream
+    first = outs[0].to_numpy(stream)
+    assert_within(first, *scored(q, k, v, cap=20.0))
+    assert all(o.to_numpy(stream).tobytes() == first.tobytes() for o in outs)
+    with pytest.raises(ta.TractRocmError, match="softcap"):
+        ta.ScoredSdpa(softcap=-1.0).eval(dq, dk, dv)
+    with pytest.raises(ta.TractRocmError, match="softcap"):
+        ta.ScoredSdpa(softcap=float("nan")).eval(dq, dk, dv)
+    with pytest.raises(ta.TractRocmError, match="slopes"):
+        op.eval(dq, dk, dv, slopes=np.zeros(4, F32))
+    with pytest.raises(ta.TractRocmError, match="documents"):
+        op.eval(dq, dk, dv, documents=np.zeros((1, 3999), np.int32))
+    with pytest.raises(ta.TractRocmError, match="out overlaps"):
+        op.eval(dq, dk, dv, out=dq)
+    with pytest.raises(ta.TractRocmError, match="documents need"):
+        op.eval(np.zeros((1, 2, 4, 64), F16), np.zeros((1, 2, 3, 64), F16), np.zeros((1, 2, 3, 64), F16), documents=np.zeros((1, 3), np.int32))
+    ring = [ta.WindowKvCache(2, 8) for _ in range(2)]
+    quant = [ta.InPlaceKvCache(2, ta.Q8_0) for _ in range(2)]
+    for c in ring + quant:
+        c.push(_rows(rng, (1, 2, 4, 128), F16))
+    with pytest.raises(ta.TractRocmError, match="in order"):
+        op.eval_cached(dq, *ring)
+    with pytest.raises(ta.TractRocmError, match="block-quantised"):
+        op.eval_cached(dq, *quant)

@@ -104,6 +104,16 @@ SIGNATURES = {
     "trocm_kivi_cache_clone": [_vp, C.POINTER(_vp), _vp],
     "trocm_quantized_kv_sdpa_eval": [_vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _vp, _f, _vp, _sz, _vp],
     "trocm_sdpa_decode_ragged": [_vp, _i, _i64, _i64, C.POINTER(_vp), C.POINTER(_vp), _vp, _f, _vp, _sz, _vp],
+    "trocm_qk_norm_rope": [_vp, _vp, _vp, _vp, _f, _vp, _vp, _i64, _i, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _vp, _vp, _vp],
+    "trocm_inplace_kv_sdpa_eval_norm_rope": [_vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _i64, _i, _i64, _i64, _pi64, _pi64, _pi64, _vp, _vp, _vp,
+                                             _f, _i, _vp, _sz, _vp, _sz, _vp],
+    "trocm_sdpa_shared_workspace_bytes": [_i64, _i64, _i64, _i64, C.POINTER(_sz)],
+    "trocm_sdpa_shared_prefix": [_vp, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _pi64, _vp, _vp, _pi64, _pi64, _vp, _f, _i, _vp,
+                                 _sz, _vp],
+    "trocm_inplace_kv_sdpa_eval_shared": [_vp, _vp, _vp, _i, _i64, _i64, _i64, _vp, _vp, C.POINTER(_vp), C.POINTER(_vp), _vp, _f, _i, _vp,
+                                          _sz, _vp],
+    "trocm_sdpa_scored": [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _f, _f, _vp, _vp, _vp, _i, _vp, _sz, _vp],
+    "trocm_sdpa_cached_scored": [_vp, _i, _i64, _i64, _vp, _vp, _vp, _f, _f, _vp, _vp, _vp, _i, _vp, _sz, _vp],
 }
 _RESTYPES = {"trocm_last_error": C.c_char_p}
 

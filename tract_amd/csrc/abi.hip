@@ -1,6 +1,7 @@
 // Host side of libtract_rocm.so: the C ABI declared in include/tract_rocm.h.
 // Runtime context, error convention, device memory, the in-place capacity-doubling KV
 // cache and the dispatch of attention calls to the kernels.
+#include <algorithm>
 #include <atomic>
 #include <stdarg.h>
 #include <stdio.h>
@@ -9,6 +10,7 @@
 #include <math.h>
 #include <iterator>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -1663,6 +1665,304 @@ int trocm_inplace_kv_sdpa_eval_ragged_rope(const void *q, const void *k_new, con
     TROCM_NOT_NULL(sin);
     return ragged_common(q, k_new, v_new, dtype, q_heads, n_seq, k_caches, v_caches, out, scale, workspace, workspace_bytes,
                          stream, cos, sin, rot_scratch, rot_scratch_bytes);
+}
+
+// ---- around attention: norms with the rotation, a shared prefix, scored attention ------------------------------------
+
+// Bytes from the first to one past the last element of a [B, H, n, D] view with element strides st (D contiguous).
+static size_t view_bytes(int64_t B, int64_t H, int64_t n, int64_t D, const int64_t *st, size_t es) {
+    return B && H && n && D ? (size_t)((B - 1) * st[0] + (H - 1) * st[1] + (n - 1) * st[2] + D) * es : 0;
+}
+
+static int norm_rope_check(const char *what, const void *q, const void *k, float eps, const void *cos, const void *sin, int64_t cs_stride_b, int dtype,
+                           int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides) {
+    TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "%s: dtype must be F32 or F16", what);
+    TROCM_REQUIRE(batch >= 0 && q_heads >= 0 && kv_heads >= 0 && n >= 0 && head_dim >= 0, "%s: negative dimension", what);
+    TROCM_REQUIRE(head_dim % 2 == 0, "%s: the head dimension must be even (got %lld)", what, (long long)head_dim);
+    TROCM_REQUIRE(head_dim < (1 << 24) && n < (1ll << 31) && q_heads + kv_heads <= 65535 && batch < (1ll << 31) && batch * n < (1ll << 31), "%s: tensor too large", what);
+    TROCM_REQUIRE(eps >= 0.0f, "%s: eps must be >= 0", what);
+    TROCM_REQUIRE(cs_stride_b == 0 || cs_stride_b >= n * head_dim, "%s: cos / sin rows of one sequence overlap the next one's (batch stride %lld < %lld)",
+                  what, (long long)cs_stride_b, (long long)(n * head_dim));
+    for (const int64_t *st : {q_strides, k_strides}) {
+        if (!st) continue;
+        TROCM_REQUIRE(st[0] >= 0 && st[1] >= 0 && st[2] >= 0, "%s: negative strides are not supported", what);
+        TROCM_REQUIRE(st[3] == 1, "%s: the features of a head must be contiguous (stride %lld)", what, (long long)st[3]);
+    }
+    if (batch * n * head_dim == 0 || q_heads + kv_heads == 0) return 0;
+    TROCM_REQUIRE(q != nullptr || q_heads == 0, "unexpected null pointer argument: q");
+    TROCM_REQUIRE(k != nullptr || kv_heads == 0, "unexpected null pointer argument: k");
+    TROCM_NOT_NULL(cos);
+    TROCM_NOT_NULL(sin);
+    return 0;
+}
+
+int trocm_qk_norm_rope(const void *q, const void *k, const void *q_weight, const void *k_weight, float eps, const void *cos,
+                       const void *sin, int64_t cos_sin_batch_stride, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                       int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides, void *q_out, void *k_out,
+                       void *stream) {
+    if (norm_rope_check("qk_norm_rope", q, k, eps, cos, sin, cos_sin_batch_stride, dtype, batch, q_heads, kv_heads, n, head_dim, q_strides, k_strides)) return 1;
+    if (batch * n * head_dim == 0 || q_heads + kv_heads == 0) return 0;
+    TROCM_REQUIRE(q_out != nullptr || q_heads == 0, "unexpected null pointer argument: q_out");
+    TROCM_REQUIRE(k_out != nullptr || kv_heads == 0, "unexpected null pointer argument: k_out");
+    QkNormRopeArgs a;
+    a.x[0] = q, a.x[1] = k, a.w[0] = q_weight, a.w[1] = k_weight, a.y[0] = q_out, a.y[1] = k_out;
+    a.H[0] = q_heads, a.H[1] = kv_heads;
+    a.cos = cos, a.sin = sin, a.cs_stride_b = cos_sin_batch_stride, a.dtype = dtype;
+    a.B = batch, a.n = n, a.D = head_dim, a.eps = eps;
+    const size_t es = elem_bytes(dtype), cs_bytes = (size_t)((batch - 1) * cos_sin_batch_stride + n * head_dim) * es;
+    size_t in[2], out[2];
+    bool dense[2];
+    for (int i = 0; i < 2; i++) {
+        const int64_t st[3] = {a.H[i] * n * head_dim, n * head_dim, head_dim}, *given = i ? k_strides : q_strides;
+        dense[i] = true;
+        for (int d = 0; d < 3; d++) {
+            a.xs[i][d] = given ? given[d] : st[d];
+            dense[i] = dense[i] && a.xs[i][d] == st[d];
+        }
+        in[i] = view_bytes(batch, a.H[i], n, head_dim, a.xs[i], es), out[i] = (size_t)batch * a.H[i] * n * head_dim * es;
+    }
+    for (int i = 0; i < 2; i++) {   // what one row's workgroup writes, another may not still have to read
+        if (!out[i]) continue;
+        for (int j = 0; j < 2; j++)
+            TROCM_REQUIRE(!in[j] || !ranges_meet(a.y[i], out[i], a.x[j], in[j]) || (i == j && dense[i] && a.y[i] == a.x[i]),
+                          "qk_norm_rope: an output may overlap no input but its own, dense and at the same place");
+        for (const void *other : {cos, sin}) TROCM_REQUIRE(!ranges_meet(a.y[i], out[i], other, cs_bytes), "qk_norm_rope: an output overlaps cos or sin");
+        for (const void *other : {q_weight, k_weight})
+            TROCM_REQUIRE(!other || !ranges_meet(a.y[i], out[i], other, (size_t)head_dim * es), "qk_norm_rope: an output overlaps a weight");
+    }
+    TROCM_REQUIRE(!out[0] || !out[1] || !ranges_meet(q_out, out[0], k_out, out[1]), "qk_norm_rope: q_out and k_out overlap");
+    hipStream_t s;
+    if (resolve_stream(stream, &s)) return 1;
+    return launch_qk_norm_rope(a, s);
+}
+
+int trocm_inplace_kv_sdpa_eval_norm_rope(const void *q, const void *k_new, const void *v_new, const void *q_weight,
+                                         const void *k_weight, float eps, const void *cos, const void *sin,
+                                         int64_t cos_sin_batch_stride, int dtype, int64_t q_heads, int64_t n_new,
+                                         const int64_t *q_strides, const int64_t *k_strides, const int64_t *v_strides,
+                                         trocm_kv_cache *kc, trocm_kv_cache *vc, void *out, float scale, int causal,
+                                         void *workspace, size_t workspace_bytes, void *rot_scratch, size_t rot_scratch_bytes,
+                                         void *stream) {
+    const char *what = "inplace_kv_sdpa_norm_rope";
+    if (inplace_eval_check(what, q, k_new, v_new, out, dtype, q_heads, n_new, kc, vc)) return 1;
+    if (norm_rope_check(what, q, k_new, eps, cos, sin, cos_sin_batch_stride, dtype, kc->B, q_heads, kc->H, n_new, kc->D, q_strides, k_strides)) return 1;
+    TROCM_REQUIRE(n_new >= 1, "%s: no new token", what);
+    if (v_strides)
+        for (int i = 0; i < 4; i++) TROCM_REQUIRE(v_strides[i] >= 0, "append: negative source strides are not supported");
+    const size_t es = elem_bytes(dtype);
+    const size_t q_bytes = (size_t)kc->B * q_heads * n_new * kc->D * es, k_bytes = (size_t)kc->B * kc->H * n_new * kc->D * es;
+    const size_t q_room = (q_bytes + 255) & ~(size_t)255;
+    TROCM_REQUIRE(rot_scratch != nullptr && rot_scratch_bytes >= q_room + k_bytes, "%s: rot_scratch must hold %zu bytes (%zu given)", what,
+                  q_room + k_bytes, rot_scratch_bytes);
+    TROCM_REQUIRE((uintptr_t)rot_scratch % 16 == 0, "rot_scratch must be 16-byte aligned");
+    void *q_rot = rot_scratch, *k_rot = (char *)rot_scratch + q_room;
+    hipStream_t s;
+    if (resolve_stream(stream, &s)) return 1;
+    const int64_t dense[4] = {kc->H * n_new * kc->D, n_new * kc->D, kc->D, 1};
+    bool v_dense = true;
+    for (int i = 0; i < 4 && v_strides; i++) v_dense = v_dense && v_strides[i] == dense[i];
+    const int64_t *vs = v_strides ? v_strides : dense;
+    if (!v_dense) TROCM_REQUIRE(!ranges_meet(rot_scratch, q_room + k_bytes, v_new, view_bytes(kc->B, kc->H, n_new, 1, vs, es) + (size_t)((kc->D - 1) * vs[3]) * es),
+                                "%s: rot_scratch overlaps v_new", what);
+    else TROCM_REQUIRE(!ranges_meet(rot_scratch, q_room + k_bytes, v_new, k_bytes), "%s: rot_scratch overlaps v_new", what);
+    TROCM_REQUIRE(!ranges_meet(rot_scratch, q_room + k_bytes, out, q_bytes), "%s: rot_scratch overlaps out", what);
+    // room for the new tokens first: a call that finds no memory has changed nothing
+    if (equalise_capacities(kc, vc, s) || append_prepare(kc, k_rot, dtype, dense, n_new, s) || append_prepare(vc, v_new, dtype, vs, n_new, s)) return 1;
+    if (trocm_qk_norm_rope(q, k_new, q_weight, k_weight, eps, cos, sin, cos_sin_batch_stride, dtype, kc->B, q_heads, kc->H, n_new, kc->D, q_strides,
+                           k_strides, q_rot, k_rot, stream)) return 1;
+    if (v_dense)
+        return trocm_inplace_kv_sdpa_eval(q_rot, k_rot, v_new, dtype, q_heads, n_new, nullptr, kc, vc, out, scale, causal, workspace, workspace_bytes, stream);
+    if (trocm_kv_append(kc, k_rot, dtype, dense, n_new, stream) || trocm_kv_append(vc, v_new, dtype, vs, n_new, stream)) return 1;
+    return trocm_sdpa_cached(q_rot, dtype, q_heads, n_new, kc, vc, out, scale, causal, workspace, workspace_bytes, stream);
+}
+
+int trocm_sdpa_shared_workspace_bytes(int64_t n_seq, int64_t q_heads, int64_t q_len, int64_t head_dim, size_t *bytes) {
+    TROCM_NOT_NULL(bytes);
+    TROCM_REQUIRE(n_seq >= 0 && q_heads >= 0 && q_len >= 0 && head_dim >= 0, "workspace_bytes: negative dimension");
+    *bytes = sdpa_shared_workspace_bytes(n_seq, q_heads, q_len, head_dim);
+    return 0;
+}
+
+int trocm_sdpa_shared_prefix(const void *q, int dtype, int64_t n_seq, int64_t q_heads, int64_t kv_heads, int64_t q_len,
+                             int64_t head_dim, const void *prefix_k, const void *prefix_v, int64_t prefix_len,
+                             const int64_t *prefix_strides, const void *k, const void *v, const int64_t *kv_strides,
+                             const int64_t *lens, void *out, float scale, int causal, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+    TROCM_NOT_NULL(q);
+    TROCM_NOT_NULL(out);
+    TROCM_NOT_NULL(lens);
+    TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "shared prefix: dtype must be F32 or F16");
+    TROCM_REQUIRE(n_seq >= 0 && q_heads >= 0 && kv_heads >= 1 && q_len >= 0 && head_dim >= 0 && prefix_len >= 0, "shared prefix: negative dimension");
+    TROCM_REQUIRE(q_heads % kv_heads == 0, "Q heads (%lld) must be a multiple of K/V heads (%lld)", (long long)q_heads, (long long)kv_heads);
+    TROCM_REQUIRE(n_seq < (1 << 24) && q_heads < (1 << 24) && q_len < (1 << 24) && prefix_len < (1ll << 30), "shared prefix: tensor too large");
+    const size_t es = elem_bytes(dtype), q_bytes = (size_t)n_seq * q_heads * q_len * head_dim * es;
+    int64_t longest = 0;
+    for (int64_t i = 0; i < n_seq; i++) {
+        TROCM_REQUIRE(lens[i] >= 0 && lens[i] < (1ll << 30), "shared prefix: length %lld of sequence %lld", (long long)lens[i], (long long)i);
+        longest = lens[i] > longest ? lens[i] : longest;
+    }
+    SdpaRowsArgs a;
+    memset(&a, 0, sizeof(a));
+    a.p_stride_h = prefix_len * head_dim, a.p_stride_t = head_dim;
+    if (prefix_strides) {
+        TROCM_REQUIRE(prefix_strides[0] >= 0 && prefix_strides[1] >= 0, "shared prefix: negative K/V strides");
+        a.p_stride_h = prefix_strides[0], a.p_stride_t = prefix_strides[1];
+    }
+    if (prefix_len) {
+        TROCM_NOT_NULL(prefix_k);
+        TROCM_NOT_NULL(prefix_v);
+        const size_t n = (size_t)((kv_heads - 1) * a.p_stride_h + (prefix_len - 1) * a.p_stride_t + head_dim) * es;
+        TROCM_REQUIRE(!ranges_meet(out, q_bytes, prefix_k, n) && !ranges_meet(out, q_bytes, prefix_v, n), "shared prefix: out overlaps the prefix");
+    }
+    if (longest) {
+        TROCM_NOT_NULL(k);
+        TROCM_NOT_NULL(v);
+        TROCM_NOT_NULL(kv_strides);
+        for (int i = 0; i < 3; i++) TROCM_REQUIRE(kv_strides[i] >= 0, "shared prefix: negative K/V strides");
+        a.stride_b = kv_strides[0], a.stride_h = kv_strides[1], a.stride_t = kv_strides[2];
+        const size_t n = view_bytes(n_seq, kv_heads, longest, head_dim, kv_strides, es);
+        TROCM_REQUIRE(!ranges_meet(out, q_bytes, k, n) && !ranges_meet(out, q_bytes, v, n), "shared prefix: out overlaps k or v");
+    }
+    TROCM_REQUIRE(q_bytes == 0 || !ranges_meet(out, q_bytes, q, q_bytes), "shared prefix: out overlaps q");
+    hipStream_t s;
+    if (resolve_stream(stream, &s)) return 1;
+    a.q = q, a.out = out, a.dtype = dtype;
+    a.B = n_seq, a.Hq = q_heads, a.Hkv = kv_heads, a.Sq = q_len, a.D = head_dim;
+    a.pk = prefix_k, a.pv = prefix_v, a.P = prefix_len;
+    a.k = k, a.v = v, a.lens = lens;
+    a.scale = isnan(scale) ? 1.0f / sqrtf((float)head_dim) : scale;
+    a.causal = causal != 0;
+    a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+    return launch_sdpa_rows(a, s);
+}
+
+int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const void *v_new, int dtype, int64_t q_heads, int64_t n_seq,
+                                      int64_t n_new, const trocm_kv_cache *pk, const trocm_kv_cache *pv,
+                                      trocm_kv_cache *const *k_caches, trocm_kv_cache *const *v_caches, void *out, float scale,
+                                      int causal, void *workspace, size_t workspace_bytes, void *stream) {
+    TROCM_NOT_NULL(q);
+    TROCM_NOT_NULL(out);
+    TROCM_NOT_NULL(pk);
+    TROCM_NOT_NULL(pv);
+    TROCM_NOT_NULL(k_caches);
+    TROCM_NOT_NULL(v_caches);
+    TROCM_REQUIRE((k_new == nullptr) == (v_new == nullptr), "shared prefix: k_new and v_new come together or not at all");
+    TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "shared prefix: dtype must be F32 or F16");
+    TROCM_REQUIRE(n_seq >= 1 && n_seq < (1 << 24), "shared prefix: n_seq must be >= 1");
+    TROCM_REQUIRE(n_new >= 1 && n_new < (1 << 24), "shared prefix: n_new must be >= 1");
+    TROCM_REQUIRE(pk->fmt == dtype && pv->fmt == dtype, "shared prefix: the caches must hold the queries' type (F32 or F16, not block-quantised)");
+    TROCM_REQUIRE(pk->B == 1 && pv->B == 1 && pk->H == pv->H && pk->D == pv->D && pk->window == 0 && pv->window == 0,
+                  "shared prefix: the prefix must be two ordinary caches of batch 1 and one shape");
+    TROCM_REQUIRE(pk->len == pv->len && (pk->len == 0 || pk->pitch == pv->pitch), "K/V lengths and capacities of the prefix must match");
+    TROCM_REQUIRE(q_heads >= 1 && q_heads % pk->H == 0, "Q heads (%lld) must be a multiple of K/V heads (%lld)", (long long)q_heads, (long long)pk->H);
+    const bool step = k_new != nullptr;
+    TROCM_REQUIRE(pk->len < (1ll << 30), "shared prefix: tensor too large");
+    const size_t es = elem_bytes(dtype), q_bytes = (size_t)n_seq * q_heads * n_new * pk->D * es, new_bytes = (size_t)n_seq * pk->H * n_new * pk->D * es;
+    TROCM_REQUIRE(!ranges_meet(out, q_bytes, q, q_bytes), "shared prefix: out overlaps q");
+    TROCM_REQUIRE(!step || (!ranges_meet(out, q_bytes, k_new, new_bytes) && !ranges_meet(out, q_bytes, v_new, new_bytes)), "shared prefix: out overlaps the new rows");
+    std::unique_ptr<const trocm_kv_cache *[]> all(new (std::nothrow) const trocm_kv_cache *[(size_t)(2 * n_seq + 2)]);
+    std::unique_ptr<SdpaRowsSeq[]> seqs(new (std::nothrow) SdpaRowsSeq[(size_t)n_seq]);
+    TROCM_REQUIRE(all && seqs, "out of host memory");
+    size_t n_all = 0;
+    all[n_all++] = pk;
+    if (pv != pk) all[n_all++] = pv;
+    for (int64_t i = 0; i < n_seq; i++) {
+        const trocm_kv_cache *kc = k_caches[i], *vc = v_caches[i];
+        TROCM_NOT_NULL(kc);
+        TROCM_NOT_NULL(vc);
+        for (const trocm_kv_cache *c : {kc, vc})
+            TROCM_REQUIRE(c->fmt == dtype && c->B == 1 && c->H == pk->H && c->D == pk->D && c->window == 0,
+                          "shared prefix: caches differ in format or shape from the prefix, or are ring buffers (sequence %lld)", (long long)i);
+        TROCM_REQUIRE(kc->len == vc->len, "K/V lengths must match (sequence %lld)", (long long)i);
+        TROCM_REQUIRE(kc->len + n_new < (1ll << 30), "shared prefix: tensor too large");
+        all[n_all++] = kc, all[n_all++] = vc;
+    }
+    if (step) {   // two sequences that append to one cache would write each other's rows
+        std::sort(all.get(), all.get() + n_all);
+        for (size_t i = 1; i < n_all; i++) TROCM_REQUIRE(all[i] != all[i - 1], "shared prefix: a step appends to caches that are all different, also from the prefix");
+    }
+    hipStream_t s;
+    if (resolve_stream(stream, &s)) return 1;
+    const int64_t dense[4] = {pk->H * n_new * pk->D, n_new * pk->D, pk->D, 1};
+    for (int64_t i = 0; i < n_seq; i++) {   // growth first, for every sequence
+        if (equalise_capacities(k_caches[i], v_caches[i], s)) return 1;
+        if (step && (append_prepare(k_caches[i], k_new, dtype, dense, n_new, s) || append_prepare(v_caches[i], v_new, dtype, dense, n_new, s))) return 1;
+    }
+    for (int64_t i = 0; i < n_seq; i++) seqs[(size_t)i] = SdpaRowsSeq{k_caches[i]->data, v_caches[i]->data, k_caches[i]->pitch * pk->D, k_caches[i]->len};
+    SdpaRowsArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = q, a.out = out, a.dtype = dtype;
+    a.B = n_seq, a.Hq = q_heads, a.Hkv = pk->H, a.Sq = n_new, a.D = pk->D;
+    a.pk = pk->data, a.pv = pv->data, a.P = pk->len, a.p_stride_h = pk->pitch * pk->D, a.p_stride_t = pk->D;
+    a.stride_t = pk->D, a.seqs = seqs.get();
+    a.scale = isnan(scale) ? 1.0f / sqrtf((float)pk->D) : scale;
+    a.causal = causal != 0;
+    a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+    if (step) {
+        if (launch_append_rows(a, k_new, v_new, s)) return 1;
+        for (int64_t i = 0; i < n_seq; i++) {
+            k_caches[i]->len += n_new, v_caches[i]->len += n_new;
+            seqs[(size_t)i].len += n_new;
+        }
+    }
+    return launch_sdpa_rows(a, s);
+}
+
+static int scored_check(float softcap, const int32_t *documents, int64_t q_len, int64_t kv_len) {
+    TROCM_REQUIRE(softcap >= 0.0f && softcap <= 3.0e38f, "sdpa_scored: softcap must be >= 0 (0: none)");
+    TROCM_REQUIRE(documents == nullptr || kv_len >= q_len, "sdpa_scored: documents need kv_len >= q_len (%lld < %lld)", (long long)kv_len, (long long)q_len);
+    TROCM_REQUIRE(q_len >= 0 && q_len < (1 << 24) && kv_len >= 0 && kv_len < (1ll << 30), "sdpa_scored: q_len or kv_len negative or too large");
+    return 0;
+}
+
+int trocm_sdpa_scored(const void *q, const void *k, const void *v, void *out, int dtype, int64_t batch, int64_t q_heads,
+                      int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t head_dim, const int64_t *kv_strides, float scale,
+                      float softcap, const float *slopes, const int32_t *documents, const int32_t *prefix_lens, int causal,
+                      void *workspace, size_t workspace_bytes, void *stream) {
+    TROCM_NOT_NULL(q);
+    TROCM_NOT_NULL(out);
+    TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "sdpa_scored: dtype must be F32 or F16");
+    TROCM_REQUIRE(batch >= 0 && q_heads >= 0 && kv_heads >= 1 && head_dim >= 0, "sdpa_scored: negative dimension");
+    TROCM_REQUIRE(batch < (1 << 24) && q_heads < (1 << 24), "sdpa_scored: tensor too large");
+    TROCM_REQUIRE(q_heads % kv_heads == 0, "Q heads (%lld) must be a multiple of K/V heads (%lld)", (long long)q_heads, (long long)kv_heads);
+    if (scored_check(softcap, documents, q_len, kv_len)) return 1;
+    SdpaRowsArgs a;
+    memset(&a, 0, sizeof(a));
+    a.stride_t = head_dim, a.stride_h = kv_len * head_dim, a.stride_b = kv_heads * kv_len * head_dim;
+    if (kv_strides) {
+        for (int i = 0; i < 3; i++) TROCM_REQUIRE(kv_strides[i] >= 0, "sdpa_scored: negative K/V strides");
+        a.stride_b = kv_strides[0], a.stride_h = kv_strides[1], a.stride_t = kv_strides[2];
+    }
+    const size_t es = elem_bytes(dtype), q_bytes = (size_t)batch * q_heads * q_len * head_dim * es;
+    if (kv_len) {
+        TROCM_NOT_NULL(k);
+        TROCM_NOT_NULL(v);
+        const int64_t st[3] = {a.stride_b, a.stride_h, a.stride_t};
+        const size_t n = view_bytes(batch, kv_heads, kv_len, head_dim, st, es);
+        TROCM_REQUIRE(n == 0 || q_bytes == 0 || (!ranges_meet(out, q_bytes, k, n) && !ranges_meet(out, q_bytes, v, n)), "sdpa_scored: out overlaps k or v");
+    }
+    TROCM_REQUIRE(q_bytes == 0 || !ranges_meet(out, q_bytes, q, q_bytes), "sdpa_scored: out overlaps q");
+    hipStream_t s;
+    if (resolve_stream(stream, &s)) return 1;
+    a.q = q, a.out = out, a.dtype = dtype;
+    a.B = batch, a.Hq = q_heads, a.Hkv = kv_heads, a.Sq = q_len, a.D = head_dim;
+    a.k = k, a.v = v, a.Sk = kv_len;
+    a.scale = isnan(scale) ? 1.0f / sqrtf((float)head_dim) : scale;
+    a.softcap = softcap, a.slopes = slopes, a.documents = documents, a.prefix_lens = causal ? prefix_lens : nullptr, a.causal = causal != 0;
+    a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+    return launch_sdpa_rows(a, s);
+}
+
+int trocm_sdpa_cached_scored(const void *q, int q_dtype, int64_t q_heads, int64_t q_len, const trocm_kv_cache *kc,
+                             const trocm_kv_cache *vc, void *out, float scale, float softcap, const float *slopes,
+                             const int32_t *documents, const int32_t *prefix_lens, int causal, void *workspace,
+                             size_t workspace_bytes, void *stream) {
+    if (sdpa_cached_check(q, q_dtype, q_heads, kc, vc, out)) return 1;
+    TROCM_REQUIRE(kc->fmt == q_dtype, "sdpa_cached_scored: the caches must hold the queries' type (F32 or F16, not block-quantised)");
+    TROCM_REQUIRE(kc->window == 0 && vc->window == 0, "sdpa_cached_scored: a sliding-window cache does not keep its tokens in order");
+    const int64_t st[3] = {kc->H * kc->pitch * kc->D, kc->pitch * kc->D, kc->D};
+    return trocm_sdpa_scored(q, kc->data, vc->data, out, q_dtype, kc->B, q_heads, kc->H, q_len, kc->len, kc->D, st, scale, softcap, slopes, documents,
+                             prefix_lens, causal, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

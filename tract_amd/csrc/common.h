@@ -244,6 +244,49 @@ int launch_sdpa_decode_ragged(const void *q, void *out, int q_dtype, int kv_fmt,
                               size_t workspace_bytes, const void *k_new, const void *v_new, hipStream_t s,
                               const void *rope_cos = nullptr, const void *rope_sin = nullptr);
 
+// RMS norm per head and rotation of queries (index 0) and keys (1) in one pass (qk_norm_rope.hip).
+struct QkNormRopeArgs {
+    const void *x[2], *w[2];   // w: [D] of dtype, NULL: ones
+    void *y[2];                // dense [B, H, n, D]
+    int64_t xs[2][3];          // element strides of batch, head, token
+    int64_t H[2];
+    const void *cos, *sin;     // [n, D] rows, batch entries cs_stride_b elements apart (0: the same rows)
+    int64_t cs_stride_b;
+    int dtype;
+    int64_t B, n, D;
+    float eps;
+};
+int launch_qk_norm_rope(const QkNormRopeArgs &a, hipStream_t s);
+
+// Attention over a shared prefix and own keys, and over scored keys (sdpa_rows.hip).  Strides in elements, head_dim contiguous.
+struct SdpaRowsSeq {
+    const void *k, *v;     // rows of kv head 0
+    int64_t stride_h, len;
+};
+struct SdpaRowsArgs {
+    const void *q;         // [B, Hq, Sq, D] dense
+    void *out;
+    int dtype;
+    int64_t B, Hq, Hkv, Sq, D;
+    const void *pk, *pv;   // shared prefix: P keys (0: none)
+    int64_t P, p_stride_h, p_stride_t;
+    const void *k, *v;     // own keys of sequence b: at b * stride_b, Sk of them (lens == NULL) or lens[b] (host) ...
+    int64_t stride_b, stride_h, stride_t, Sk;
+    const int64_t *lens;
+    const SdpaRowsSeq *seqs;   // ... or an entry each (host; stride_t is theirs too)
+    float scale, softcap;      // softcap 0: none
+    int causal;            // over the own keys: key j visible to query i iff j <= i + len - Sq, or j < prefix_lens[b]
+    const float *slopes;           // device [Hq] or NULL: score -= slope * |i + len - Sq - j|
+    const int32_t *documents;      // device [B, Sk] or NULL: visible only if both tokens' ids are equal and not negative
+    const int32_t *prefix_lens;    // device [B] or NULL
+    void *workspace;
+    size_t workspace_bytes;
+};
+int launch_sdpa_rows(const SdpaRowsArgs &a, hipStream_t s);
+size_t sdpa_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Sq, int64_t D);
+// k_new, v_new dense [B, Hkv, Sq, D] behind the rows of `seqs` (whose lengths do not count them yet).
+int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_new, hipStream_t s);
+
 // Workspace layout: [arrival counters][partials ...]; a ragged launch keeps its plan (work items and
 // per-sequence slot ranges) between the two, so that the counters stay zero for whichever launch comes next:
 // [arrival counters][plan][partials ...].

@@ -286,6 +286,27 @@ class WindowKvCache(InPlaceKvCache):
 _NAN = float("nan")
 
 
+def _strides4(st):
+    """Element strides [batch, heads, tokens, features] for the ABI (None: dense)."""
+    return None if st is None else _I64x4(*st)
+
+
+def _cos_sin_batch(cos, sin, batch, n, head_dim) -> int:
+    """Batch entries (1 or `batch`) of cos and sin rows [1 or batch, 1, n, head_dim]."""
+    shape = cos.shape
+    if sin.shape != shape:
+        raise TractRocmError("cos and sin must have the same shape")
+    if len(shape) != 4 or shape[1] != 1 or shape[2] != n or shape[3] != head_dim or shape[0] not in (1, batch):
+        raise TractRocmError(f"cos / sin of shape {tuple(shape)} are not [1 or {batch}, 1, {n}, {head_dim}]")
+    return shape[0]
+
+
+def _check_norm_weights(q_weight, k_weight, head_dim) -> None:
+    for w in (q_weight, k_weight):
+        if w is not None and w.shape != (head_dim,):
+            raise TractRocmError(f"a norm's weight must be [{head_dim}], found {tuple(w.shape)}")
+
+
 def _scale_arg(scale) -> float:
     return _NAN if scale is None else float(scale)
 
@@ -528,6 +549,42 @@ class InPlaceKvSdpaState:
         call("trocm_inplace_kv_sdpa_eval_rope", q.ptr, k_new.ptr, v_new.ptr, cos.ptr, sin.ptr, 0 if cb[0] == 1 else Sq * D,
              _code(dtype), Hq, Sq, self.k.handle, self.v.handle, out.ptr, _scale_arg(self.scale), int(self.causal),
              ws.buf.ptr, ws.nbytes, rot.ptr, rot.nbytes, _sh(stream))
+        return out
+
+    def eval_norm_rope_into(self, q: DeviceTensor, k_new: DeviceTensor, v_new: DeviceTensor, q_weight, k_weight, eps: float,
+                            cos: DeviceTensor, sin: DeviceTensor, out: DeviceTensor | None = None, stream=None, q_strides=None,
+                            k_strides=None, v_strides=None) -> DeviceTensor:
+        """RMS norm of every head of Q and K_new and their rotation (QkNormRope), then `eval`.  Rank 4; strides in elements,
+        None for dense (the shapes stay [batch, heads, n_new, head_dim])."""
+        dtype = q.dtype
+        if any(t is not None and not _same(t.dtype, dtype) for t in (k_new, v_new, q_weight, k_weight, cos, sin)):
+            raise TractRocmError("Q, K_new, V_new, weights, cos and sin must share a datum type")
+        if len(q.shape) != 4 or k_new.shape != v_new.shape:
+            raise TractRocmError("Q, K_new and V_new must be of rank 4, K_new and V_new of one shape")
+        B, Hq, Sq, D = q.shape
+        Hkv = k_new.shape[1]
+        if k_new.shape != (B, Hkv, Sq, D):
+            raise TractRocmError(f"K_new {k_new.shape} does not match Q {q.shape}")
+        cb = _cos_sin_batch(cos, sin, B, Sq, D)
+        _check_norm_weights(q_weight, k_weight, D)
+        for c in (self.k, self.v):
+            if c._h is None:
+                c._create(k_new.shape, dtype)
+            c._check_push_shape(k_new.shape)
+        if out is None:
+            out = DeviceTensor(q.shape, dtype)
+        elif tuple(out.shape) != q.shape or not _same(out.dtype, dtype):
+            raise TractRocmError("out must have Q's shape and datum type")
+        ws = self._workspace(B, Hq, Sq, D, stream)
+        es = dtype.itemsize
+        need = ((B * Hq * Sq * D * es + 255) & ~255) + B * Hkv * Sq * D * es
+        rot = getattr(self, "_rot", None)
+        if rot is None or rot.nbytes < need:
+            rot = self._rot = DeviceTensor((need,), np.uint8)
+        call("trocm_inplace_kv_sdpa_eval_norm_rope", q.ptr, k_new.ptr, v_new.ptr, None if q_weight is None else q_weight.ptr,
+             None if k_weight is None else k_weight.ptr, eps, cos.ptr, sin.ptr, 0 if cb == 1 else Sq * D, _code(dtype), Hq, Sq,
+             _strides4(q_strides), _strides4(k_strides), _strides4(v_strides), self.k.handle, self.v.handle, out.ptr,
+             _scale_arg(self.scale), int(self.causal), ws.buf.ptr, ws.nbytes, rot.ptr, rot.nbytes, _sh(stream))
         return out
 
     def attend(self, q: DeviceTensor, stream=None, out: DeviceTensor | None = None) -> DeviceTensor:

@@ -167,8 +167,17 @@ class Workspace:
         call("trocm_sdpa_workspace_bytes", batch, q_heads, q_len, head_dim, C.byref(n))
         return n.value
 
-    def __init__(self, batch: int, q_heads: int, q_len: int, head_dim: int, stream=None):
-        self.nbytes = Workspace.bytes_for(batch, q_heads, q_len, head_dim)
+    @staticmethod
+    @functools.lru_cache(maxsize=1024)
+    def shared_bytes_for(n_seq: int, q_heads: int, q_len: int, head_dim: int) -> int:
+        """What attention over a shared prefix asks for."""
+        n = C.c_size_t()
+        call("trocm_sdpa_shared_workspace_bytes", n_seq, q_heads, q_len, head_dim, C.byref(n))
+        return n.value
+
+    def __init__(self, batch: int, q_heads: int, q_len: int, head_dim: int, stream=None, nbytes: int | None = None):
+        """`nbytes`: the size where it is not that of Sdpa for this shape."""
+        self.nbytes = Workspace.bytes_for(batch, q_heads, q_len, head_dim) if nbytes is None else nbytes
         self.buf = DeviceTensor((self.nbytes,), np.uint8)
         call("trocm_sdpa_workspace_init", self.buf.ptr, self.nbytes, _sh(stream))
         call("trocm_stream_sync", _sh(stream))

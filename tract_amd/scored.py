@@ -1,0 +1,195 @@
+"""Operators around a decoder's attention that the reference's graphs spell out in elementary ops, as single calls:
+
+* ``QkNormRope``        RMS norm of every query and key head and their rotation (ApplyRope,
+  transformers/src/ops/apply_rope.rs:169-176) in one pass
+* ``SharedPrefixSdpa``  attention of sequences that share a prefix, which is read once for all of them;
+  ``inplace_kv_sdpa_eval_shared`` is the same over caches, with the append of a step
+* ``ScoredSdpa``        Sdpa (transformers/src/ops/sdpa.rs:83-89) whose scores are capped by a tanh, fall with the distance,
+  stay inside documents or see a prefix
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from ._lib import TractRocmError, call
+from .ops import _as_device, _canon4, _check_norm_weights, _code, _cos_sin_batch, _same, _scale_arg, _strides4, _I64x3
+from .runtime import DeviceTensor, Workspace, _sh
+
+_I32 = np.dtype(np.int32)
+_F32 = np.dtype(np.float32)
+
+
+def _optr(t):
+    return None if t is None else t.ptr
+
+
+def _output(out, shape, dtype):
+    if out is None:
+        return DeviceTensor(shape, dtype)
+    if out.shape != shape or not _same(out.dtype, dtype):
+        raise TractRocmError("out must have Q's shape and datum type")
+    return out
+
+
+class QkNormRope:
+    """y = x * rsqrt(mean(x^2) + eps) * weight, then y * cos + RotateHalf(y) * sin, for every head of Q and K."""
+
+    def __init__(self, eps: float = 1e-6):
+        self.eps = float(eps)
+
+    def name(self) -> str:
+        return "QkNormRope"
+
+    def is_stateless(self) -> bool:
+        return True
+
+    def output_facts(self, q_shape, k_shape, *_):
+        return tuple(q_shape), tuple(k_shape)
+
+    def eval(self, q, k, q_weight, k_weight, cos, sin, stream=None, q_strides=None, k_strides=None, q_out=None, k_out=None):
+        """Q [batch, q_heads, n, head_dim], K [batch, kv_heads, n, head_dim], weights [head_dim] or None, Cos and Sin
+        [1 or batch, 1, n, head_dim].  Strides: of views, in elements (None: dense).  Returns (q, k), dense."""
+        if not isinstance(q, DeviceTensor):
+            q, k, cos, sin = (_as_device(t, stream) for t in (q, k, cos, sin))
+            q_weight, k_weight = (None if w is None else _as_device(w, stream) for w in (q_weight, k_weight))
+        dtype, shape, k_shape = q.dtype, q.shape, k.shape
+        for t in (k, q_weight, k_weight, cos, sin):
+            if t is not None and not _same(t.dtype, dtype):
+                raise TractRocmError("Q, K, weights, cos and sin must share a datum type")
+        if len(shape) != 4 or len(k_shape) != 4 or k_shape[0] != shape[0] or k_shape[2:] != shape[2:]:
+            raise TractRocmError(f"Q {shape} and K {k_shape} must be [batch, heads, n, head_dim] and differ in heads only")
+        b, hq, n, d = shape
+        cb = _cos_sin_batch(cos, sin, b, n, d)
+        _check_norm_weights(q_weight, k_weight, d)
+        q_out, k_out = _output(q_out, shape, dtype), _output(k_out, k_shape, dtype)
+        call("trocm_qk_norm_rope", q.ptr, k.ptr, _optr(q_weight), _optr(k_weight), self.eps, cos.ptr, sin.ptr, 0 if cb == 1 else n * d,
+             _code(dtype), b, hq, k_shape[1], n, d, _strides4(q_strides), _strides4(k_strides), q_out.ptr, k_out.ptr,
+             None if stream is None else _sh(stream))
+        return q_out, k_out
+
+
+class SharedPrefixSdpa:
+    """Attention of n_seq sequences over one prefix and over their own keys behind it."""
+
+    def __init__(self, scale=None, is_causal: bool = True):
+        self.scale, self.is_causal = scale, bool(is_causal)
+        self._ws = None
+
+    def _workspace(self, n, hq, sq, d, stream):
+        need = Workspace.shared_bytes_for(n, hq, sq, d)
+        if self._ws is None or self._ws.nbytes < need:
+            self._ws = Workspace(n, hq, sq, d, stream, nbytes=need)
+        return self._ws
+
+    def eval(self, q, prefix_k, prefix_v, k, v, lens, stream=None, out=None, prefix_len=None) -> DeviceTensor:
+        """Q [n_seq, q_heads, q_len, head_dim]; prefix K and V [1, kv_heads, room, head_dim] of which `prefix_len` tokens (None:
+        all) count; K and V [n_seq, kv_heads, room, head_dim] of which sequence i's first lens[i] tokens count."""
+        q, prefix_k, prefix_v, k, v = (_as_device(t, stream) for t in (q, prefix_k, prefix_v, k, v))
+        dtype = q.dtype
+        for t in (prefix_k, prefix_v, k, v):
+            if not _same(t.dtype, dtype):
+                raise TractRocmError("Q, K and V must share a datum type")
+        if len(q.shape) != 4 or len(k.shape) != 4 or len(prefix_k.shape) != 4 or k.shape != v.shape or prefix_k.shape != prefix_v.shape:
+            raise TractRocmError("shared prefix: inputs must be of rank 4, K and V of one shape")
+        n, hq, sq, d = q.shape
+        _, hkv, room, _ = k.shape
+        p = prefix_k.shape[2] if prefix_len is None else int(prefix_len)
+        if k.shape != (n, hkv, room, d) or prefix_k.shape != (1, hkv, prefix_k.shape[2], d) or not 0 <= p <= prefix_k.shape[2]:
+            raise TractRocmError(f"shared prefix: Q {q.shape}, prefix {prefix_k.shape} and K {k.shape} do not match")
+        if len(lens) != n or (n and not 0 <= min(lens) <= max(lens) <= room):
+            raise TractRocmError(f"shared prefix: lens must be {n} lengths of 0..={room}")
+        out = _output(out, q.shape, dtype)
+        ws = self._workspace(n, hq, sq, d, stream)
+        call("trocm_sdpa_shared_prefix", q.ptr, _code(dtype), n, hq, hkv, sq, d, prefix_k.ptr, prefix_v.ptr, p,
+             (C.c_int64 * 2)(prefix_k.shape[2] * d, d), k.ptr, v.ptr, _I64x3(hkv * room * d, room * d, d), (C.c_int64 * n)(*lens), out.ptr,
+             _scale_arg(self.scale), int(self.is_causal), ws.buf.ptr, ws.nbytes, None if stream is None else _sh(stream))
+        return out
+
+
+def inplace_kv_sdpa_eval_shared(q: DeviceTensor, k_new, v_new, prefix_k, prefix_v, k_caches, v_caches, scale=None, causal: bool = True,
+                                workspace: Workspace | None = None, stream=None, out: DeviceTensor | None = None) -> DeviceTensor:
+    """One step of `n_seq` sequences that share a prefix: append k_new[i], v_new[i] ([n_seq, Hkv, n_new, D]) to sequence i's
+    caches, then attend q[i] ([n_seq, Hq, n_new, D]) over the prefix caches and over its own.  With k_new and v_new None:
+    attend to what is there.  A sequence's caches may be new; the prefix caches must have been pushed to."""
+    n, hq, sq, d = q.shape
+    if len(k_caches) != n or len(v_caches) != n:
+        raise TractRocmError("shared prefix: one K and one V cache per sequence expected")
+    if prefix_k.handle is None or prefix_v.handle is None:
+        raise TractRocmError("empty kv-cache")
+    hkv = prefix_k._shape[1]
+    if k_new is not None or v_new is not None:
+        if k_new is None or v_new is None or k_new.shape != (n, hkv, sq, d) or v_new.shape != k_new.shape:
+            raise TractRocmError("shared prefix: k_new / v_new must be [n_seq, kv_heads, n_new, head_dim]")
+        if not _same(k_new.dtype, q.dtype) or not _same(v_new.dtype, q.dtype):
+            raise TractRocmError("Q, K_new and V_new must share a datum type")
+    for c in (*k_caches, *v_caches):
+        if c._h is None:
+            c._create((1, hkv, 0, d), q.dtype)
+    out = _output(out, q.shape, q.dtype)
+    ws = workspace or Workspace(n, hq, sq, d, stream, nbytes=Workspace.shared_bytes_for(n, hq, sq, d))
+    ks = (C.c_void_p * n)(*[c._h for c in k_caches])
+    vs = (C.c_void_p * n)(*[c._h for c in v_caches])
+    call("trocm_inplace_kv_sdpa_eval_shared", q.ptr, _optr(k_new), _optr(v_new), _code(q.dtype), hq, n, sq, prefix_k.handle, prefix_v.handle,
+         ks, vs, out.ptr, _scale_arg(scale), int(causal), ws.ptr, ws.nbytes, _sh(stream))
+    return out
+
+
+class ScoredSdpa:
+    """Sdpa whose scores are capped (softcap * tanh(s / softcap)), lose a slope per head times the distance, stay inside packed
+    documents and, where causal, also see the first prefix_lens[b] keys."""
+
+    def __init__(self, scale=None, softcap: float = 0.0, is_causal: bool = True):
+        self.scale, self.softcap, self.is_causal = scale, float(softcap), bool(is_causal)
+        self._ws = self._ws_key = None
+
+    def name(self) -> str:
+        return "ScoredSdpa"
+
+    def _workspace(self, b, hq, sq, d, stream):
+        if self._ws is None or self._ws_key != (b, hq, d) or self._ws.nbytes < Workspace.bytes_for(b, hq, sq, d):
+            self._ws, self._ws_key = Workspace(b, hq, sq, d, stream), (b, hq, d)
+        return self._ws
+
+    @staticmethod
+    def _rules(slopes, documents, prefix_lens, b, hq, sk, stream):
+        slopes, documents, prefix_lens = (None if t is None else _as_device(t, stream) for t in (slopes, documents, prefix_lens))
+        if slopes is not None and (slopes.shape != (hq,) or not _same(slopes.dtype, _F32)):
+            raise TractRocmError(f"slopes must be f32 of shape [{hq}]")
+        if documents is not None and (documents.shape != (b, sk) or not _same(documents.dtype, _I32)):
+            raise TractRocmError(f"documents must be int32 of shape [{b}, {sk}]")
+        if prefix_lens is not None and (prefix_lens.shape != (b,) or not _same(prefix_lens.dtype, _I32)):
+            raise TractRocmError(f"prefix_lens must be int32 of shape [{b}]")
+        return slopes, documents, prefix_lens
+
+    def eval(self, q, k, v, slopes=None, documents=None, prefix_lens=None, stream=None, out=None) -> DeviceTensor:
+        """Q, K, V of rank 3 or 4; slopes f32 [q_heads], documents int32 [batch, kv_len], prefix_lens int32 [batch]."""
+        q, k, v = (_as_device(t, stream) for t in (q, k, v))
+        if not (_same(k.dtype, q.dtype) and _same(v.dtype, q.dtype)):
+            raise TractRocmError("Q, K and V must share a datum type")
+        b, hq, sq, d = _canon4(q.shape)
+        _, hkv, sk, _ = _canon4(k.shape)
+        if _canon4(k.shape) != (b, hkv, sk, d) or k.shape != v.shape:
+            raise TractRocmError("K/V shape mismatch")
+        slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, sk, stream)
+        out = _output(out, q.shape, q.dtype)
+        ws = self._workspace(b, hq, sq, d, stream)
+        call("trocm_sdpa_scored", q.ptr, k.ptr, v.ptr, out.ptr, _code(q.dtype), b, hq, hkv, sq, sk, d, None, _scale_arg(self.scale), self.softcap,
+             _optr(slopes), _optr(documents), _optr(prefix_lens), int(self.is_causal), ws.buf.ptr, ws.nbytes, None if stream is None else _sh(stream))
+        return out
+
+    def eval_cached(self, q: DeviceTensor, k_cache, v_cache, slopes=None, documents=None, prefix_lens=None, stream=None, out=None) -> DeviceTensor:
+        """Q over the valid region of two InPlaceKvCaches (kv_len is their length)."""
+        if k_cache.handle is None or v_cache.handle is None:
+            raise TractRocmError("empty kv-cache")
+        b, hq, sq, d = _canon4(q.shape)
+        cb, _, _, cd = _canon4(k_cache._shape)
+        if (b, d) != (cb, cd):
+            raise TractRocmError(f"Q {q.shape} does not match the cache's {k_cache._shape}")
+        slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, k_cache.len(), stream)
+        out = _output(out, q.shape, q.dtype)
+        ws = self._workspace(b, hq, sq, d, stream)
+        call("trocm_sdpa_cached_scored", q.ptr, _code(q.dtype), hq, sq, k_cache.handle, v_cache.handle, out.ptr, _scale_arg(self.scale), self.softcap,
+             _optr(slopes), _optr(documents), _optr(prefix_lens), int(self.is_causal), ws.ptr, ws.nbytes, _sh(stream))
+        return out
