@@ -95,6 +95,17 @@ def test_documents_in_any_order_padding_and_empty_rows(rt, dtype, d, n):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,n,t", [(64, 600, 600), (128, 300, 900)])
+def test_packed_documents_with_a_tail_of_padding(rt, dtype, d, n, t):
+    """Rows of padding beside rows of a document whose keys fill whole tiles: the ones see nothing, the others all of it."""
+    ids = np.repeat(np.arange(6, dtype=np.int32), t // 6)[None].repeat(2, axis=0)
+    ids[0, t - 77 :] = -1
+    ids[1, 50:90] = -7
+    got = _check(dtype, 2, 6, 2, n, t, d, documents=ids, slopes=_slopes(6))
+    assert not got[0, :, n - 77 :].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 def test_fewer_keys_than_queries(rt, dtype):
     """Rows before the first key see nothing; a prefix shows them what it holds."""
     got = _check(dtype, 1, 4, 2, 50, 20, 64, cap=9.0)
