@@ -23,7 +23,7 @@ def attend(q, keys, values, dtype, scale=None, cap=0.0, bias=None, sees=None):
 
     The bound, per element, with A = sum_j w_j |v_j|: a score of D products is off by at most D + 8 half steps of 32 bits
     on the sum of the products' sizes, and by a few on its own size (scale, change of base, difference from the maximum);
-    the cap only shrinks that but has an error of its own of at most 4e-7 of the cap.  e^ds - 1 <= 2 ds counts twice,
+    the cap only shrinks that but has an error of its own of at most 4e-7 of the cap (caps of up to 512) or of the score.  e^ds - 1 <= 2 ds counts twice,
     for the weight and for the sum it is divided by.  f16: a weight is rounded to f16 before the product with V (half a
     step in the numerator; the sum is over the same values or not: another).  Sums of T terms in f32: T half steps at
     most, numerator and sum.  Then half a step of the result's type."""
@@ -39,7 +39,7 @@ def attend(q, keys, values, dtype, scale=None, cap=0.0, bias=None, sees=None):
     ds = (d + 8) * U32 * (np.abs(q) @ np.abs(safe_k).T) * abs(scale)
     if cap:
         s = cap * np.tanh(s / cap)
-        ds = ds + 4e-7 * cap
+        ds = ds + 4e-7 * (cap if cap <= 512 else np.abs(s))
     if bias is not None:
         s = s + bias
         ds = ds + 2 * U32 * np.abs(bias)

@@ -69,6 +69,8 @@ def test_not_causal_and_scales(rt, dtype, n):
     _check(dtype, 2, 4, 2, n, 190, 64, cap=5.0, causal=False, scale=-0.1)
     _check(dtype, 2, 4, 2, n, 190, 64, causal=False, scale=0.0)
     _check(dtype, 1, 4, 2, n, n, 128, cap=1e4)       # hardly a cap at all
+    _check(dtype, 1, 4, 2, n, n, 128, cap=512.0)
+    _check(dtype, 1, 4, 2, n, n, 64, cap=1e20, scale=0.02)
     _check(dtype, 1, 4, 2, n, n, 128, cap=0.01)      # hardly a score left
     _check(dtype, 1, 4, 2, n, n, 128, cap=50.0, big=60.0)   # scores far beyond the cap
 

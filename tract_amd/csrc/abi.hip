@@ -1909,7 +1909,7 @@ int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const vo
 }
 
 static int scored_check(float softcap, const int32_t *documents, int64_t q_len, int64_t kv_len) {
-    TROCM_REQUIRE(softcap >= 0.0f && softcap <= 3.0e38f, "sdpa_scored: softcap must be >= 0 (0: none)");
+    TROCM_REQUIRE(softcap == 0.0f || (softcap >= 1e-30f && softcap <= 1e30f), "sdpa_scored: softcap must be 0 (none) or in 1e-30..1e30");
     TROCM_REQUIRE(documents == nullptr || kv_len >= q_len, "sdpa_scored: documents need kv_len >= q_len (%lld < %lld)", (long long)kv_len, (long long)q_len);
     TROCM_REQUIRE(q_len >= 0 && q_len < (1 << 24) && kv_len >= 0 && kv_len < (1ll << 30), "sdpa_scored: q_len or kv_len negative or too large");
     return 0;
@@ -1950,7 +1950,8 @@ int trocm_sdpa_scored(const void *q, const void *k, const void *v, void *out, in
     a.scale = isnan(scale) ? 1.0f / sqrtf((float)head_dim) : scale;
     a.softcap = softcap, a.slopes = slopes, a.documents = documents, a.prefix_lens = causal ? prefix_lens : nullptr, a.causal = causal != 0;
     a.workspace = workspace, a.workspace_bytes = workspace_bytes;
-    return launch_sdpa_rows(a, s);
+    const int rc = a.B && a.Hq && a.Sq && a.D ? launch_sdpa_scored_prompt(a, s) : 0;
+    return rc != 2 ? rc : launch_sdpa_rows(a, s);
 }
 
 int trocm_sdpa_cached_scored(const void *q, int q_dtype, int64_t q_heads, int64_t q_len, const trocm_kv_cache *kc,

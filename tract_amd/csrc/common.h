@@ -283,6 +283,10 @@ struct SdpaRowsArgs {
     size_t workspace_bytes;
 };
 int launch_sdpa_rows(const SdpaRowsArgs &a, hipStream_t s);
+// tanh as 1 - 2 / (e^2x + 1) is off by about 1e-7, times the cap: up to this cap less than a f16 weight's own rounding.
+constexpr float kFastTanhCap = 512.0f;
+// f16 prompts of scored attention (sdpa_scored.hip); 2 = not covered.
+int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s);
 size_t sdpa_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Sq, int64_t D);
 // k_new, v_new dense [B, Hkv, Sq, D] behind the rows of `seqs` (whose lengths do not count them yet).
 int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_new, hipStream_t s);

@@ -88,11 +88,9 @@ __device__ __forceinline__ OwnKeys own_keys(const RowsDev &p, int b, int kvh) {
     return o;
 }
 
-// tanh for the f32 rows: the library's, accurate to an ulp or two near zero.  For f16 rows 1 - 2 / (e^2x + 1), whose absolute
-// error of 1e-7 times the cap is far below what the rounding of the weights to f16 leaves.
-template <typename T>
-__device__ __forceinline__ float cap_tanh(float x) {
-    if constexpr (std::is_same<T, float>::value) return tanhf(x);
+// tanh for f32 rows and for large caps: the library's, accurate to an ulp or two near zero.  For f16 rows under a cap of up to
+// kFastTanhCap 1 - 2 / (e^2x + 1).
+__device__ __forceinline__ float fast_tanh(float x) {
     return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.0f * kLog2e)) + 1.0f);
 }
 
@@ -136,7 +134,7 @@ __global__ __launch_bounds__(kAnyThreads) void sdpa_rows_any_kernel(RowsCall cal
 #pragma unroll 1
                 for (int d = 0; d < D; d++) dot = __builtin_fmaf(lds_q[d], widen(k[d]), dot);
                 s = dot * p.scale;
-                if (p.cap > 0.0f) s = p.cap * cap_tanh<T>(s / p.cap);
+                if (p.cap > 0.0f) s = p.cap * tanhf(s / p.cap);
                 if (src && p.slopes) s -= slope * (float)abs(at - j);
                 s *= kLog2e;
             }
@@ -210,7 +208,7 @@ __device__ __forceinline__ void wave_sync() {
 constexpr int kListMax = 4096;   // key tiles of a range that documents are looked up for
 
 // Places of the key tiles [t_begin, t_end) that hold a token of a document in [dmin, dmax]; bit 15: all of the tile's tokens are of
-// document `one`, that of every row (-1: the rows differ, or one is padding).  All threads; returns how many.
+// document `one`, that of every row but padding (-1: they differ).  All threads; returns how many.
 __device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, int t_begin, int t_end, int dmin, int dmax, int one, uint16_t *list, int *counts) {
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     int n = 0;
@@ -304,6 +302,7 @@ __global__ __launch_bounds__(kThreads, RB == 1 && sizeof(T) == 2 ? 2 : 1) void s
         if constexpr (SCORED) {
             slope[rb] = p.slopes ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
             doc[rb] = p.docs ? p.docs[(int64_t)b * p.Sk + at[rb]] : 0;
+            if (doc[rb] < 0) lim[rb] = -1;   // padding sees nothing
         }
     }
     const int *docs = SCORED && p.docs ? p.docs + (int64_t)b * p.Sk : nullptr;
@@ -312,16 +311,12 @@ __global__ __launch_bounds__(kThreads, RB == 1 && sizeof(T) == 2 ? 2 : 1) void s
     if constexpr (SCORED) {
         if (docs && n_tiles > 0 && n_tiles <= kListMax) {
             int dmin = INT_MAX, dmax = -1;
-            bool same = true;
 #pragma unroll
-            for (int rb = 0; rb < RB; rb++) {
+            for (int rb = 0; rb < RB; rb++)
                 if (doc[rb] >= 0) dmin = min(dmin, doc[rb]), dmax = max(dmax, doc[rb]);
-                else same = false;
-            }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) dmin = min(dmin, __shfl_xor(dmin, d, 64)), dmax = max(dmax, __shfl_xor(dmax, d, 64));
-            same = __builtin_amdgcn_ballot_w64(!same) == 0 && dmin == dmax;
-            n_tiles = list_document_tiles(docs, n_keys, t_begin, t_end, dmin, dmax, same ? dmin : -1, s_list, s_counts);
+            n_tiles = list_document_tiles(docs, n_keys, t_begin, t_end, dmin, dmax, dmin == dmax ? dmin : -1, s_list, s_counts);
             listed = true;
         }
     }
@@ -415,23 +410,26 @@ __global__ __launch_bounds__(kThreads, RB == 1 && sizeof(T) == 2 ? 2 : 1) void s
         for (int rb = 0; rb < RB; rb++) {
             if (rb > 0 && rb >= n_rb) break;
             if constexpr (SCORED) {
-                if (p.cap > 0.0f) {
+                if (H16 && p.cap > 0.0f && p.cap <= kFastTanhCap) {
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[rb][r] = cap_log2 * cap_tanh<T>(s[rb][r] * to_cap);
+                    for (int r = 0; r < 16; r++) s[rb][r] = cap_log2 * fast_tanh(s[rb][r] * to_cap);
+                } else if (p.cap > 0.0f) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[rb][r] = cap_log2 * tanhf(s[rb][r] * to_cap);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; r++) s[rb][r] *= to_log2;
                 }
                 if (p.slopes) {
-                    const int d0 = at[rb] - k_lo - 4 * hb;
+                    const float d0 = (float)(at[rb] - k_lo - 4 * hb);
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[rb][r] = __builtin_fmaf(-slope[rb], (float)abs(d0 - (8 * (r >> 2) + (r & 3))), s[rb][r]);
+                    for (int r = 0; r < 16; r++) s[rb][r] = __builtin_fmaf(-slope[rb], fabsf(d0 - (float)(8 * (r >> 2) + (r & 3))), s[rb][r]);
                 }
                 if (by_id) {
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         const int c = 8 * (r >> 2) + (r & 3), even = __builtin_amdgcn_readlane(id_tile, c), odd = __builtin_amdgcn_readlane(id_tile, c + 4), id = hb ? odd : even;
-                        s[rb][r] = id == doc[rb] && id >= 0 ? s[rb][r] : -INFINITY;
+                        s[rb][r] = id == doc[rb] ? s[rb][r] : -INFINITY;
                     }
                 }
             } else {

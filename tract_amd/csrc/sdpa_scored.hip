@@ -1,0 +1,381 @@
+// Prompts whose scores are capped, biased by distance, or cut into documents: f16, head sizes 64 and 128.
+//
+//   s = scale q.k;   s = cap tanh(s / cap);   s -= slope |i - j|;   softmax over the visible j;   out = P V
+//
+// The rows of a kv head are (query, head of the group), heads fastest, so that a workgroup of 4 waves x 32 rows covers few
+// queries and its causal frontier is short.  S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs: every softmax scalar of a row
+// sits in one lane.  A tile of 64 keys is staged into LDS once for the four waves, double buffered, its loads issued two
+// tiles ahead: one barrier per tile.  Two workgroups (head size 64: three) share a compute unit without knowing of each
+// other, so that one's softmax runs beside the other's MFMAs.
+//
+// What bounds it: the vector ALU.  Per score the cap costs two quarter-rate instructions (exp2, rcp) beside the softmax's own
+// exp2: 48 cycles of a SIMD per 64 scores, with the rest of the score's arithmetic about 72, where its share of the MFMAs is 32.
+#include <hip/hip_fp16.h>
+#include <limits.h>
+#include <string.h>
+#include "common.h"
+
+namespace trocm {
+namespace {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kTile = 64, kRows = 32 * kWaves;
+constexpr int kListMax = 4096;   // key tiles that documents are looked up for
+
+struct ScoredDev {
+    const char *q;
+    _Float16 *out;
+    const char *k, *v;
+    int64_t stride_b, stride_h, stride_t;   // bytes
+    int B, Hq, Hkv, Sq, G, Sk, row_tiles, splits, tiles;   // tiles: of a range of keys
+    float scale, cap;
+    int causal;
+    const float *slopes;
+    const int *docs, *prefix_lens;
+    float *part_o, *part_ml;   // as in sdpa_rows.hip
+    int64_t part_rows;
+};
+
+__device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *lds_ptr) {   // (see sdpa_rows.hip)
+    typedef __attribute__((address_space(3))) short4_t *lds_v4_ptr;
+    short4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_ptr)(uintptr_t)(uint32_t)(uintptr_t)lds_ptr);
+    return __builtin_bit_cast(half4_t, r);
+}
+
+template <int D, bool CAP, bool SLOPES, bool DOCS>
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel(ScoredDev p) {
+    constexpr int KS = D / 16, DB = D / 32;
+    constexpr int KROW = D + 8, VROW = D + 16;        // halves per row in LDS (bank spread of the two kinds of reads)
+    constexpr int PPR = D / 8, RPI = kThreads / PPR, NL = kTile / RPI;   // 16-byte pieces per row, rows per load of the workgroup, loads per tile and tensor
+    constexpr int K_TILE = kTile * KROW, V_TILE = kTile * VROW, OROW = D + 8;
+    static_assert(kWaves * 32 * OROW <= 2 * V_TILE, "the output goes through the V buffers");
+    __shared__ __attribute__((aligned(16))) _Float16 lds_k[2][K_TILE], lds_v[2][V_TILE];
+    __shared__ uint16_t s_list[DOCS ? kListMax : 1];
+    __shared__ int s_counts[kWaves], s_range[2][kWaves];
+    __shared__ __attribute__((aligned(16))) int s_ids[2][DOCS ? kTile : 4];   // documents of the staged tiles' tokens
+
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
+    int id = blockIdx.x;
+    const int kvh = id % p.Hkv;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
+    id /= p.Hkv;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int b = id % p.B, rt = p.row_tiles - 1 - id / p.B;   // (the longest first)
+    const int seq_rows = p.Sq * p.G, row0 = rt * kRows, off = p.Sk - p.Sq;
+
+    const int my_row = row0 + 32 * w + l32, r = min(my_row, seq_rows - 1), i = r / p.G, g = r - i * p.G;
+    const int64_t out_row = ((int64_t)b * p.Hq + kvh * p.G + g) * p.Sq + i;
+    const int at = i + off;
+    int lim = p.Sk - 1, n_vis = p.Sk;
+    if (p.causal) {
+        const int pre = p.prefix_lens ? p.prefix_lens[b] : 0;
+        lim = min(lim, max(at, pre - 1));
+        n_vis = max(0, min(p.Sk, max((min(row0 + kRows, seq_rows) - 1) / p.G + off + 1, pre)));
+    }
+    const int wave_lim = __builtin_amdgcn_readfirstlane(p.causal ? max((min(row0 + 32 * w + 32, seq_rows) - 1) / p.G + off, p.prefix_lens ? p.prefix_lens[b] - 1 : -1) : p.Sk - 1);
+    const bool wave_has_rows = row0 + 32 * w < seq_rows;
+    const int t_begin = split * p.tiles, t_end = min((n_vis + kTile - 1) / kTile, t_begin + p.tiles);
+    int n_tiles = max(0, t_end - t_begin);
+
+    const float slope = SLOPES ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
+    const int *docs = DOCS ? p.docs + (int64_t)b * p.Sk : nullptr;
+    const int doc = DOCS ? docs[at] : 0;
+    if (DOCS && doc < 0) lim = -1;   // padding sees nothing
+    bool listed = false;
+    if constexpr (DOCS) {
+        // The tiles with a token of the documents of these rows (a smallest and a largest id: ids in any order are fine), and of them
+        // those whose tokens are all of the rows' one document, which need no look at the ids.
+        if (n_tiles <= kListMax) {
+            int dmin = doc >= 0 ? doc : INT_MAX, dmax = doc;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) dmin = min(dmin, __shfl_xor(dmin, d, 64)), dmax = max(dmax, __shfl_xor(dmax, d, 64));
+            if (lane == 0) s_range[0][w] = dmin, s_range[1][w] = dmax;
+            __syncthreads();
+            dmin = INT_MAX, dmax = -1;
+#pragma unroll
+            for (int x = 0; x < kWaves; x++) dmin = min(dmin, s_range[0][x]), dmax = max(dmax, s_range[1][x]);
+            const int one_doc = dmin == dmax ? dmin : -1;
+            int n = 0;
+            for (int t0 = t_begin; t0 < t_end; t0 += kThreads) {
+                const int t = t0 + tid;
+                int lo = INT_MAX, hi = -1, neg = 0;
+                if (t < t_end) {
+                    const int first = t * kTile, last = min(first + kTile, p.Sk);
+#pragma unroll 8
+                    for (int j = first; j < last; j++) {
+                        const int x = docs[j];
+                        neg |= x;
+                        lo = min(lo, x < 0 ? INT_MAX : x), hi = max(hi, x);
+                    }
+                }
+                const bool active = hi >= dmin && lo <= dmax;
+                const uint64_t mask = __builtin_amdgcn_ballot_w64(active);
+                if (lane == 0) s_counts[w] = __popcll(mask);
+                __syncthreads();
+                int place = n;
+                for (int x = 0; x < kWaves; x++) {
+                    if (x < w) place += s_counts[x];
+                    n += s_counts[x];
+                }
+                if (active) s_list[place + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)((t - t_begin) | (lo == hi && lo == one_doc && neg >= 0 ? 0x8000 : 0));
+                __syncthreads();
+            }
+            n_tiles = n;
+            listed = true;
+        }
+    }
+    float *part_ml = p.part_ml + (int64_t)split * 2 * p.part_rows;
+    if (n_tiles == 0 && p.splits > 1) {   // nothing to add: a maximum of -inf says so
+        if (hb == 0 && my_row < seq_rows) part_ml[out_row] = -INFINITY;
+        return;
+    }
+
+    auto entry = [&](int n) -> int { return DOCS && listed ? __builtin_amdgcn_readfirstlane(s_list[n]) : n; };
+    auto tile_lo = [&](int e) -> int { return (t_begin + (DOCS ? e & 0x7fff : e)) * kTile; };
+
+    const char *kb = p.k + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h, *vb = p.v + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h;
+    const int key0 = tid / PPR, ch = tid % PPR;
+    u32x4 kpre[NL], vpre[NL];
+    int id_pre = 0;   // documents: of this tile's token `lane`
+    auto prefetch = [&](int n) {
+        const int k_lo = tile_lo(entry(n)), most = p.Sk - 1 - k_lo;   // (rows past the last key repeat it)
+        const char *tk = kb + (int64_t)k_lo * p.stride_t, *tv = vb + (int64_t)k_lo * p.stride_t;
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            const uint32_t o = (uint32_t)min(key0 + j * RPI, most) * (uint32_t)p.stride_t + ch * 16;   // (rows of at most 2^25 bytes)
+            kpre[j] = *reinterpret_cast<const u32x4 *>(tk + o);
+            vpre[j] = *reinterpret_cast<const u32x4 *>(tv + o);
+        }
+        if (DOCS) id_pre = docs[k_lo + min(lane, most)];
+    };
+    auto stage = [&](int buf) {
+        if (DOCS) {
+            if (tid < kTile) s_ids[buf][tid] = id_pre;
+            const uint64_t padding = __builtin_amdgcn_ballot_w64(id_pre < 0);
+            if (padding != 0) {   // values of padding may hold anything
+#pragma unroll
+                for (int j = 0; j < NL; j++)
+                    if ((padding >> (key0 + j * RPI)) & 1) vpre[j] = u32x4{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            *reinterpret_cast<u32x4 *>(&lds_k[buf][(key0 + j * RPI) * KROW + ch * 8]) = kpre[j];
+            *reinterpret_cast<u32x4 *>(&lds_v[buf][(key0 + j * RPI) * VROW + ch * 8]) = vpre[j];
+        }
+    };
+
+    float m_run = -INFINITY, l_run = 0.0f;
+    float16_t o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int x = 0; x < 16; x++) o[db][x] = 0.0f;
+    // the cap in the log2 domain: cap log2e tanh(x) = A - 2 A / (e^2x + 1), x = s scale / cap
+    const float to_log2 = p.scale * kLog2e, cap_a = p.cap * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
+
+    half8_t qf[KS];
+    if (n_tiles > 0) prefetch(0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = *reinterpret_cast<const half8_t *>(p.q + out_row * (2 * D) + 32 * ks + 16 * hb);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));   // settled here, not by a wait in the loop that would take the prefetch in too
+    if (n_tiles > 0) {
+        stage(0);
+        if (n_tiles > 1) prefetch(1);
+    }
+    for (int n = 0; n < n_tiles; n++) {
+        __syncthreads();   // tile n is in LDS; every wave is done with the buffers about to be overwritten
+        const int buf = n & 1, e = entry(n), k_lo = tile_lo(e);
+        if (wave_has_rows && k_lo <= wave_lim) {
+            float16_t s[2];
+#pragma unroll
+            for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) s[kb2][x] = 0.0f;
+            const _Float16 *ksrc = &lds_k[buf][l32 * KROW + 8 * hb];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int kb2 = 0; kb2 < 2; kb2++)
+                    s[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t *>(ksrc + 32 * kb2 * KROW + 16 * ks), qf[ks], s[kb2], 0, 0, 0);
+
+            // this lane's keys: k_lo + 4 hb + c, c = 32 kb2 + 8 (x / 4) + x % 4
+            float d0 = (float)(at - k_lo - 4 * hb);
+            // (asked for once the products are there: all 32 distances computed beside the MFMAs spill registers; of the group of four
+            // at hand, so that what is subtracted are inline constants)
+            if constexpr (SLOPES) asm volatile("" : "+v"(d0), "+v"(s[1]));
+#pragma unroll
+            for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    if constexpr (CAP)
+                        s[kb2][x] = __builtin_fmaf(-2.0f * cap_a, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kb2][x] * cap_k) + 1.0f), cap_a);
+                    else
+                        s[kb2][x] *= to_log2;
+                }
+            if constexpr (DOCS) {
+                if (!(listed && (e & 0x8000))) {
+#pragma unroll
+                    for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                        for (int x = 0; x < 16; x += 4) {
+                            const int4 four = *reinterpret_cast<const int4 *>(&s_ids[buf][32 * kb2 + 2 * x + 4 * hb]);
+                            s[kb2][x] = four.x == doc ? s[kb2][x] : -INFINITY;
+                            s[kb2][x + 1] = four.y == doc ? s[kb2][x + 1] : -INFINITY;
+                            s[kb2][x + 2] = four.z == doc ? s[kb2][x + 2] : -INFINITY;
+                            s[kb2][x + 3] = four.w == doc ? s[kb2][x + 3] : -INFINITY;
+                        }
+                }
+            }
+            if constexpr (SLOPES) {
+#pragma unroll
+                for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        const float d = (x & 3) == 0 ? d0 : (x & 3) == 1 ? d0 - 1.0f : (x & 3) == 2 ? d0 - 2.0f : (d0 - 2.0f) - 1.0f;
+                        s[kb2][x] = __builtin_fmaf(-slope, fabsf(d), s[kb2][x]);
+                        if ((x & 3) == 3) d0 -= 8.0f;
+                    }
+            }
+            const int last = lim - k_lo - 4 * hb;
+            if (__builtin_amdgcn_ballot_w64(last < 60) != 0) {
+#pragma unroll
+                for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) s[kb2][x] = 32 * kb2 + 8 * (x >> 2) + (x & 3) <= last ? s[kb2][x] : -INFINITY;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb2][x]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            // the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
+            const bool moved = top > m_run + 8.0f;
+            const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
+            m_run = m_new;
+            half8_t pf[4];
+            float sum = 0.0f;
+            const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + x] - ref);
+#pragma unroll
+                for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
+            }
+            l_run = l_run * keep + sum;
+            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) o[db][x] *= keep;
+            }
+            const _Float16 *vsrc = &lds_v[buf][(4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
+#pragma unroll
+            for (int st = 0; st < 4; st++)
+#pragma unroll
+                for (int db = 0; db < DB; db++) {
+                    const half4_t lo = lds_read_tr16(vsrc + 16 * st * VROW + 32 * db), hi = lds_read_tr16(vsrc + (16 * st + 8) * VROW + 32 * db);
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[st], o[db], 0, 0, 0);
+                }
+        }
+        if (n + 1 < n_tiles) {   // the next tile to LDS after this one's arithmetic, which covers its loads' latency
+            stage(buf ^ 1);
+            if (n + 2 < n_tiles) prefetch(n + 2);
+        }
+    }
+    l_run += __shfl_xor(l_run, 32, 64);
+
+    if (p.splits > 1) {
+        if (my_row < seq_rows) {
+            float *po = p.part_o + ((int64_t)split * p.part_rows + out_row) * D + 4 * hb;
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) *reinterpret_cast<float4_t *>(po + 32 * db + 8 * x) = float4_t{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
+            part_ml[out_row + (hb ? p.part_rows : 0)] = hb ? l_run : m_run;
+        }
+        return;
+    }
+    // rows to their places in whole lines, through the idle V buffers
+    __syncthreads();
+    if (!wave_has_rows) return;
+    const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+    _Float16 *tr = &lds_v[0][0] + w * 32 * OROW;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            half4_t h4;
+#pragma unroll
+            for (int y = 0; y < 4; y++) h4[y] = (_Float16)(o[db][4 * x + y] * inv);
+            *reinterpret_cast<half4_t *>(tr + l32 * OROW + 32 * db + 8 * x + 4 * hb) = h4;
+        }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int LPR = D / 8, RPS = 64 / LPR;
+#pragma unroll
+    for (int j = 0; j < 32 / RPS; j++) {
+        const int row = j * RPS + lane / LPR, rr = row0 + 32 * w + row, ii = rr / p.G, gg = rr - ii * p.G;
+        if (rr < seq_rows)
+            *reinterpret_cast<u32x4 *>(p.out + (((int64_t)b * p.Hq + kvh * p.G + gg) * p.Sq + ii) * D + lane % LPR * 8) = *reinterpret_cast<const u32x4 *>(tr + row * OROW + lane % LPR * 8);
+    }
+}
+
+template <int D>
+void launch_of(const ScoredDev &p, int64_t grid, hipStream_t s) {
+    const bool cap = p.cap > 0.0f, slopes = p.slopes != nullptr, docs = p.docs != nullptr;
+    const dim3 g((unsigned)grid), t(kThreads);
+    if (docs) {
+        if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, true, true>), g, t, 0, s, p);
+        else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, false, true>), g, t, 0, s, p);
+        else if (slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, false, true, true>), g, t, 0, s, p);
+        else hipLaunchKernelGGL((sdpa_scored_kernel<D, false, false, true>), g, t, 0, s, p);
+    } else {
+        if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, true, false>), g, t, 0, s, p);
+        else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, false, false>), g, t, 0, s, p);
+        else if (slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, false, true, false>), g, t, 0, s, p);
+        else hipLaunchKernelGGL((sdpa_scored_kernel<D, false, false, false>), g, t, 0, s, p);
+    }
+}
+
+}  // namespace
+
+// 0 done, 1 failed, 2 not covered (the kernels of sdpa_rows.hip take it).
+int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
+    if (a.dtype != TROCM_F16 || (a.D != 64 && a.D != 128) || a.P || a.lens || a.seqs || a.Sk == 0 || a.softcap > kFastTanhCap) return 2;
+    auto aligned = [](const void *x) { return (uintptr_t)x % 16 == 0; };
+    const int64_t G = a.Hq / a.Hkv, rows = a.Sq * G;
+    if (!aligned(a.q) || !aligned(a.out) || !aligned(a.k) || !aligned(a.v) || a.stride_b % 8 || a.stride_h % 8 || a.stride_t % 8 || a.stride_t * 2 > (1 << 25)) return 2;
+    if (rows >= (1 << 30)) return 2;
+    const int64_t row_tiles = (rows + kRows - 1) / kRows, grid = a.B * a.Hkv * row_tiles;
+    if (rows <= 32 || grid < num_compute_units() / 2 || grid >= (1ll << 31)) return 2;
+    ScoredDev p;
+    memset(&p, 0, sizeof(p));
+    p.q = (const char *)a.q, p.out = (_Float16 *)a.out, p.k = (const char *)a.k, p.v = (const char *)a.v;
+    p.stride_b = a.stride_b * 2, p.stride_h = a.stride_h * 2, p.stride_t = a.stride_t * 2;
+    p.B = (int)a.B, p.Hq = (int)a.Hq, p.Hkv = (int)a.Hkv, p.Sq = (int)a.Sq, p.G = (int)G, p.Sk = (int)a.Sk, p.row_tiles = (int)row_tiles;
+    p.splits = 1, p.tiles = (int)((a.Sk + kTile - 1) / kTile);
+    p.scale = a.scale, p.cap = a.softcap, p.causal = a.causal;
+    p.slopes = a.slopes, p.docs = a.documents, p.prefix_lens = a.prefix_lens;
+    p.part_rows = a.B * a.Hq * a.Sq;
+    if (a.D == 64) launch_of<64>(p, grid, s);
+    else launch_of<128>(p, grid, s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail("sdpa_scored launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+}  // namespace trocm
