@@ -22,6 +22,7 @@ namespace {
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -36,6 +37,22 @@ struct SeqTable { uint32_t w[kSeqWords]; };
 // The table of a launch where its arguments lie (its kernel's one argument is a RowsCall): a word at a computed place is a scalar
 // load.  Asked of the argument itself, the compiler copied all of it to every lane's scratch first.
 typedef const __attribute__((address_space(4))) uint32_t *TableWords;
+
+// n / d for 0 <= n < 2^31 as a product: mul = floor(2^(31 + l) / d) + 1, l = ceil(log2 d).  (A division by a number that only the launch
+// knows is some 40 dependent instructions; a workgroup with one tile to read spent a third of its time on five of them.)
+struct FastDiv {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ int by(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+FastDiv fast_div(int64_t d) {
+    FastDiv f;
+    uint32_t l = 0;
+    if (d < 1) d = 1;
+    while ((1ll << l) < d) l++;
+    f.d = (uint32_t)d, f.shift = 31 + l;
+    f.mul = (uint32_t)(((unsigned __int128)1 << f.shift) / (uint64_t)d + 1);
+    return f;
+}
 
 struct RowsDev {
     const char *q;
@@ -58,7 +75,9 @@ struct RowsDev {
     // partials [splits][B * Hq * Sq][D], then [splits][2][B * Hq * Sq]
     float *part_o, *part_ml;
     int64_t part_rows;
+    int *counters;              // != NULL: the last workgroup of a unit joins its parts; else a launch after this one
     int splits;                 // p_splits + own_splits; 1: no partials, rows go to `out`
+    FastDiv by_g, by_sq, by_p_row_tiles, by_own_splits, by_own_row_tiles;
 };
 
 struct RowsCall { RowsDev p; SeqTable tab; };
@@ -68,6 +87,12 @@ __device__ __forceinline__ TableWords table_words(size_t at = offsetof(RowsCall,
 
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(_Float16 x) { return (float)x; }
+
+// 16 bytes of device memory.  Pointers that come out of a table are generic ones to the compiler, whose loads go by the LDS's
+// counter too: every wait for LDS would wait for the tile in flight.
+__device__ __forceinline__ u32x4 load16(const char *base, uint32_t off) {
+    return *(const __attribute__((address_space(1))) u32x4 *)(base + off);
+}
 
 struct OwnKeys { const char *k, *v; int len; };
 
@@ -207,383 +232,682 @@ __device__ __forceinline__ void wave_sync() {
 
 constexpr int kListMax = 4096;   // key tiles of a range that documents are looked up for
 
+// Partial results for whichever workgroup joins them: written through to where every compute unit sees them once they complete.
+__device__ __forceinline__ void put(float *at, float x) { __hip_atomic_store(at, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get(const float *at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void put2(float *at, float2_t x) { __hip_atomic_store(reinterpret_cast<uint64_t *>(at), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float2_t get2(const float *at) { return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)); }
+
+// What a workgroup has to do: rows [row0, row_end) of a kv head over key tiles [t_begin, t_end) of one set of keys.
+struct RowsWork {
+    const char *k, *v;
+    int64_t st;              // bytes between tokens
+    int kvh, b;              // b: whose own keys (-1: the prefix)
+    int row0, row_end, n_keys, t_begin, t_end, split;
+};
+
+// Where row r of a kv head lies among the q and output rows.
+struct RowPlace { int64_t at; int i, qh; };   // i: its place in the sequence's queries
+__device__ __forceinline__ RowPlace q_row(const RowsDev &p, int kvh, int r) {
+    const int bi = p.by_g.by(r), qh = kvh * p.G + r - bi * p.G, b = p.by_sq.by(bi), i = bi - b * p.Sq;
+    return {((int64_t)b * p.Hq + qh) * p.Sq + i, i, qh};
+}
+
 // Places of the key tiles [t_begin, t_end) that hold a token of a document in [dmin, dmax]; bit 15: all of the tile's tokens are of
-// document `one`, that of every row but padding (-1: they differ).  All threads; returns how many.
+// document `one`, that of every row but padding (-1: they differ).  All threads; returns how many.  A wave looks at two
+// tiles at a time, a token per lane.
 __device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, int t_begin, int t_end, int dmin, int dmax, int one, uint16_t *list, int *counts) {
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    constexpr int PW = 32;   // tiles that a wave looks at before the waves compare
     int n = 0;
-    for (int t0 = t_begin; t0 < t_end; t0 += kThreads) {
-        const int t = t0 + tid;
-        int lo = INT_MAX, hi = -1, neg = 0;
-        if (t < t_end) {
-            const int first = t * kTile, last = min(first + kTile, n_keys);
-            for (int j = first; j < last; j++) {
-                const int id = docs[j];
-                if (id >= 0) lo = min(lo, id), hi = max(hi, id);
-                else neg = 1;
-            }
+    for (int t0 = t_begin; t0 < t_end; t0 += kWaves * PW) {
+        const int first = t0 + w * PW;
+        uint32_t active = 0, whole = 0;
+#pragma unroll
+        for (int x = 0; x < PW; x += 2) {   // (all loads in flight at once)
+            const int j = (first + x) * kTile + lane;
+            const int id = first + x + (lane >> 5) < t_end ? docs[min(j, n_keys - 1)] : -1;
+            const uint64_t in = __builtin_amdgcn_ballot_w64(id >= dmin && id <= dmax && id >= 0), same = __builtin_amdgcn_ballot_w64(id == one && id >= 0);
+            active |= ((uint32_t)in != 0 ? 1u : 0u) << x | ((uint32_t)(in >> 32) != 0 ? 2u : 0u) << x;
+            whole |= ((uint32_t)same == ~0u ? 1u : 0u) << x | ((uint32_t)(same >> 32) == ~0u ? 2u : 0u) << x;
         }
-        const bool active = hi >= dmin && lo <= dmax;
-        const uint64_t mask = __builtin_amdgcn_ballot_w64(active);
-        if (lane == 0) counts[w] = __popcll(mask);
+        if (lane == 0) counts[w] = __popc(active);
         __syncthreads();
         int at = n;
         for (int x = 0; x < kWaves; x++) {
             if (x < w) at += counts[x];
             n += counts[x];
         }
-        if (active) list[at + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)((t - t_begin) | (lo == hi && lo == one && !neg ? 0x8000 : 0));
+        if (lane < PW && ((active >> lane) & 1)) list[at + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane - t_begin) | ((whole >> lane) & 1 ? 0x8000 : 0));
         __syncthreads();
     }
     return n;
 }
 
-template <typename T, int D, int RB, bool SCORED>
-__global__ __launch_bounds__(kThreads, RB == 1 && sizeof(T) == 2 ? 2 : 1) void sdpa_rows_kernel(RowsCall call) {
-    const RowsDev &p = call.p;
+// A tile of 16 or 32 rows, R of them; the four waves take the range's key tiles in turn.
+//   R == 16: 16x16 MFMAs.  K goes straight from memory into fragments (four lanes read 64 consecutive bytes of a key's row), V
+//            through a wave-private LDS tile.
+//   R == 32: 32x32 MFMAs, K and V through a wave-private LDS tile.
+template <typename T, int D, int R, bool SCORED>
+__device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, unsigned char *lds, uint16_t *s_list, int *s_counts) {
     constexpr bool H16 = sizeof(T) == 2;
-    constexpr int MR = 32 * RB, DB = D / 32;
+    constexpr int DB = D / R, NG = 64 / R;        // feature blocks of the output; lane groups (4 or 2), whose lanes hold a row each
+    constexpr int NS = kTile / NG;                // scores of a lane
     constexpr int KROW = H16 ? D + 8 : D + 4;     // elements per K row in LDS: 128-bit reads of 16 rows hit 64 distinct banks
-    constexpr int VROW = H16 ? D + 16 : D + 8;    // f16: the 4 rows of a transposing read sit 8 banks apart; f32: rows 4 apart 32 banks apart
-    constexpr int PRIV = kTile * (KROW + VROW) * (int)sizeof(T);   // a wave's tile
+    constexpr int VROW = H16 ? D + 16 : R == 16 ? D + 4 : D + 8;   // (rows of a read in different banks)
+    constexpr int PRIV = kTile * (VROW + (R == 32 ? KROW : 0)) * (int)sizeof(T);   // a wave's tile
     constexpr int CROW = D + 4;                   // floats per row where waves are joined
     constexpr int LPRW = D * (int)sizeof(T) / 16, RPI = 64 / LPRW, NI = kTile / RPI;   // lanes per key row, rows per load, loads per tile and tensor
-    constexpr int KS = H16 ? D / 16 : D / 8;      // 16-byte pieces of a lane's share of a row
-    static_assert(kWaves * 32 * CROW * 4 + kWaves * 64 * 4 <= kWaves * PRIV, "waves are joined where the tiles were");
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves * PRIV];
-    __shared__ uint16_t s_list[SCORED ? kListMax : 1];
-    __shared__ int s_counts[kWaves];
+    constexpr int KS = D * (int)sizeof(T) / (16 * NG);   // 16-byte pieces of a lane's share of a row
+    static_assert(kWaves * R * CROW * 4 + kWaves * 2 * R * 4 <= kWaves * PRIV, "waves are joined where the tiles were");
+    typedef typename std::conditional<R == 16, float4_t, float16_t>::type Acc;
+    constexpr int NA = R == 16 ? 4 : 16;
 
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
-    int item = blockIdx.x;
-    const int kvh = item % p.Hkv;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
-    item /= p.Hkv;
-    const bool pre = item < p.p_items;
-    int row0, row_end, split, n_keys, n_vis, t_begin, b = 0;
-    const char *kb, *vb;
-    int64_t st;
-    if (pre) {
-        row0 = item % p.p_row_tiles * MR, row_end = min(row0 + MR, p.B * p.Sq * p.G);
-        split = item / p.p_row_tiles;
-        kb = p.pk + (int64_t)kvh * p.p_stride_h, vb = p.pv + (int64_t)kvh * p.p_stride_h, st = p.p_stride_t;
-        n_keys = n_vis = p.P;
-        t_begin = split * p.p_tiles;
-    } else {
-        item -= p.p_items;
-        split = item % p.own_splits, item /= p.own_splits;
-        const int rt = p.own_row_tiles - 1 - item % p.own_row_tiles;   // (the longest first)
-        b = p.seq0 + item / p.own_row_tiles;
-        const OwnKeys own = own_keys(p, b, kvh);
-        kb = own.k, vb = own.v, st = p.stride_t, n_keys = own.len;
-        row0 = b * p.Sq * p.G + rt * MR, row_end = min(row0 + MR, (b + 1) * p.Sq * p.G);
-        n_vis = n_keys;
-        if (p.causal) {
-            n_vis = (row_end - 1) / p.G - b * p.Sq + n_keys - p.Sq + 1;
-            if (SCORED && p.prefix_lens) n_vis = max(n_vis, p.prefix_lens[b]);
-            n_vis = max(0, min(n_vis, n_keys));
-        }
-        t_begin = split * p.own_tiles;
-        split += p.p_splits;
-    }
-    const int t_end = min((n_vis + kTile - 1) / kTile, t_begin + (pre ? p.p_tiles : p.own_tiles));
-    const int n_rb = (row_end - row0 + 31) / 32;
-
-    // this lane's rows: one of each block of 32
-    int lim[RB], at[RB], doc[RB];
-    float slope[RB];
-    int64_t out_row[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-        const int r = min(row0 + 32 * rb + l32, row_end - 1), bi = r / p.G, g = r - bi * p.G, rb_b = bi / p.Sq, i = bi - rb_b * p.Sq;
-        out_row[rb] = ((int64_t)rb_b * p.Hq + kvh * p.G + g) * p.Sq + i;
-        at[rb] = i + n_keys - p.Sq;
-        lim[rb] = n_keys - 1;
-        if (!pre && p.causal) lim[rb] = min(lim[rb], SCORED && p.prefix_lens ? max(at[rb], p.prefix_lens[b] - 1) : at[rb]);
-        if constexpr (SCORED) {
-            slope[rb] = p.slopes ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
-            doc[rb] = p.docs ? p.docs[(int64_t)b * p.Sk + at[rb]] : 0;
-            if (doc[rb] < 0) lim[rb] = -1;   // padding sees nothing
-        }
-    }
-    const int *docs = SCORED && p.docs ? p.docs + (int64_t)b * p.Sk : nullptr;
-    int n_tiles = max(0, t_end - t_begin);
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane / R, lr = lane % R;
+    const bool own = wk.b >= 0;
+    const int n_keys = wk.n_keys;
+    // this lane's row
+    const RowPlace place = q_row(p, wk.kvh, min(wk.row0 + lr, wk.row_end - 1));
+    const int64_t out_row = place.at;
+    const int at = place.i + n_keys - p.Sq;
+    int lim = n_keys - 1, doc = 0;
+    if (own && p.causal) lim = min(lim, SCORED && p.prefix_lens ? max(at, p.prefix_lens[wk.b] - 1) : at);
+    float slope = 0.0f;
+    const int *docs = nullptr;
+    int n_tiles = max(0, wk.t_end - wk.t_begin);
     bool listed = false;
     if constexpr (SCORED) {
-        if (docs && n_tiles > 0 && n_tiles <= kListMax) {
-            int dmin = INT_MAX, dmax = -1;
+        if (p.slopes) slope = p.slopes[place.qh] * kLog2e;
+        if (p.docs) {
+            docs = p.docs + (int64_t)wk.b * p.Sk;
+            doc = docs[at];
+            if (doc < 0) lim = -1;   // padding sees nothing
+            if (n_tiles > 0 && n_tiles <= kListMax) {
+                int dmin = doc >= 0 ? doc : INT_MAX, dmax = doc;
 #pragma unroll
-            for (int rb = 0; rb < RB; rb++)
-                if (doc[rb] >= 0) dmin = min(dmin, doc[rb]), dmax = max(dmax, doc[rb]);
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) dmin = min(dmin, __shfl_xor(dmin, d, 64)), dmax = max(dmax, __shfl_xor(dmax, d, 64));
-            n_tiles = list_document_tiles(docs, n_keys, t_begin, t_end, dmin, dmax, dmin == dmax ? dmin : -1, s_list, s_counts);
-            listed = true;
+                for (int d = 1; d < R; d <<= 1) dmin = min(dmin, __shfl_xor(dmin, d, 64)), dmax = max(dmax, __shfl_xor(dmax, d, 64));
+                n_tiles = list_document_tiles(docs, n_keys, wk.t_begin, wk.t_end, dmin, dmax, dmin == dmax ? dmin : -1, s_list, s_counts);
+                listed = true;
+            }
         }
     }
-    auto part_m = [&](int64_t row) { return p.part_ml + (int64_t)split * 2 * p.part_rows + row; };
+    float *part_ml = p.part_ml + (int64_t)wk.split * 2 * p.part_rows;
     if (n_tiles == 0 && p.splits > 1) {   // nothing to add: a maximum of -inf says so
-        if (w == 0 && hb == 0)
-#pragma unroll
-            for (int rb = 0; rb < RB; rb++)
-                if (row0 + 32 * rb + l32 < row_end) *part_m(out_row[rb]) = -INFINITY;
+        if (w == 0 && grp == 0 && wk.row0 + lr < wk.row_end) put(part_ml + out_row, -INFINITY);
         return;
     }
 
-    u32x4 qf[RB][KS];
+    float m_run = -INFINITY, l_run = 0.0f;
+    Acc o[DB];
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++)
+    for (int db = 0; db < DB; db++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) qf[rb][ks] = *reinterpret_cast<const u32x4 *>(p.q + out_row[rb] * (D * (int)sizeof(T)) + ks * 32 + hb * 16);
+        for (int r = 0; r < NA; r++) o[db][r] = 0.0f;
 
-    float m_run[RB], l_run[RB];
-    float16_t o[RB][DB];
-#pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-        m_run[rb] = -INFINITY, l_run[rb] = 0.0f;
-#pragma unroll
-        for (int db = 0; db < DB; db++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[rb][db][r] = 0.0f;
-    }
-
-    T *lds_k = reinterpret_cast<T *>(lds + w * PRIV), *lds_v = lds_k + kTile * KROW;
+    T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: R == 32)
     const int kr = lane / LPRW, ch = lane % LPRW;
-    u32x4 kpre[NI], vpre[NI];
+    constexpr int NK = R == 16 ? 2 * KS : NI;
+    u32x4 kpre[NK], vpre[NI];
     int id_pre = 0;   // lane%32's token's document
     auto tile_at = [&](int n) -> int {
-        if (SCORED && listed) return t_begin + __builtin_amdgcn_readfirstlane(s_list[n] & 0x7fff);
-        return t_begin + n;
+        if (SCORED && listed) return wk.t_begin + __builtin_amdgcn_readfirstlane(s_list[n] & 0x7fff);
+        return wk.t_begin + n;
     };
-    auto prefetch = [&](int n) {
-        const int k_lo = tile_at(n) * kTile, most = n_keys - 1 - k_lo;   // (rows past the last key repeat it)
-        const char *tk = kb + (int64_t)k_lo * st, *tv = vb + (int64_t)k_lo * st;
+    // (rows past the last key repeat it; rows of at most 2^25 bytes)
+    auto prefetch_k = [&](int n) __attribute__((always_inline)) {
+        const int k_lo = tile_at(n) * kTile, most = n_keys - 1 - k_lo;
+        const char *tk = wk.k + (int64_t)k_lo * wk.st;
+        if constexpr (R == 16) {
 #pragma unroll
-        for (int j = 0; j < NI; j++) {
-            const uint32_t off = (uint32_t)min(j * RPI + kr, most) * (uint32_t)st + ch * 16;
-            kpre[j] = *reinterpret_cast<const u32x4 *>(tk + off);
-            vpre[j] = *reinterpret_cast<const u32x4 *>(tv + off);
+            for (int kb = 0; kb < 2; kb++) {
+                const uint32_t off = (uint32_t)min(16 * kb + lr, most) * (uint32_t)wk.st + grp * 16;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) kpre[kb * KS + ks] = load16(tk, off + ks * 64);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; j++) kpre[j] = load16(tk, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
         }
-        if (SCORED && docs) id_pre = docs[k_lo + min(l32, most)];
+        if (SCORED && docs) id_pre = docs[k_lo + min(lane & 31, most)];
+    };
+    auto prefetch_v = [&](int n) __attribute__((always_inline)) {
+        const int k_lo = tile_at(n) * kTile, most = n_keys - 1 - k_lo;
+        const char *tv = wk.v + (int64_t)k_lo * wk.st;
+#pragma unroll
+        for (int j = 0; j < NI; j++) vpre[j] = load16(tv, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
     };
     const float to_log2 = p.scale * kLog2e, cap_log2 = p.cap * kLog2e, to_cap = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
+    // key of score x of this lane, from the tile's first: groups of four consecutive ones
+    auto key_of = [](int x) { return R == 16 ? 16 * (x >> 2) + (x & 3) : 8 * (x >> 2) + (x & 3); };   // + 4 grp
 
-    if (w < n_tiles) prefetch(w);
+    if (w < n_tiles) prefetch_k(w), prefetch_v(w);
+    u32x4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = load16(p.q + out_row * (D * (int)sizeof(T)), ks * 16 * NG + grp * 16);
     for (int n = w; n < n_tiles; n += kWaves) {
         const int k_lo = tile_at(n) * kTile;
         const bool by_id = SCORED && docs && !(listed && __builtin_amdgcn_readfirstlane(s_list[n] & 0x8000));
         const int id_tile = id_pre;
         const uint32_t padding = SCORED && by_id ? (uint32_t)__builtin_amdgcn_ballot_w64(id_tile < 0) : 0;   // a bit per key of the tile
+
+        // ---- S^T = K Q^T --------------------------------------------------------------------------------------
+        float s[NS];
+        if constexpr (R == 16) {
+            float4_t acc[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[kb][r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) {
+                    if constexpr (H16) {
+                        acc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kpre[kb * KS + ks]), __builtin_bit_cast(half8_t, qf[ks]), acc[kb], 0, 0, 0);
+                    } else {   // (one feature of each group's four at a time)
+                        const float4_t a = __builtin_bit_cast(float4_t, kpre[kb * KS + ks]), c = __builtin_bit_cast(float4_t, qf[ks]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[kb], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+            for (int x = 0; x < NS; x++) s[x] = acc[x >> 2][x & 3];
+            if (n + kWaves < n_tiles) prefetch_k(n + kWaves);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_k + (j * RPI + kr) * KROW + ch * (16 / (int)sizeof(T))) = kpre[j];
+            if (n + kWaves < n_tiles) prefetch_k(n + kWaves);
+            wave_sync();
+            float16_t acc;
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const u32x4 kf = *reinterpret_cast<const u32x4 *>(lds_k + lr * KROW + (ks * 32 + grp * 16) / (int)sizeof(T));
+                if constexpr (H16) {
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, kf), __builtin_bit_cast(half8_t, qf[ks]), acc, 0, 0, 0);
+                } else {
+                    const float4_t a = __builtin_bit_cast(float4_t, kf), c = __builtin_bit_cast(float4_t, qf[ks]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], c[e], acc, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < NS; x++) s[x] = acc[x];
+        }
 #pragma unroll
         for (int j = 0; j < NI; j++) {
-            *reinterpret_cast<u32x4 *>(lds_k + (j * RPI + kr) * KROW + ch * (16 / (int)sizeof(T))) = kpre[j];
             if (by_id && ((padding >> (j * RPI)) >> kr & 1)) vpre[j] = u32x4{0, 0, 0, 0};   // padding may hold anything
             *reinterpret_cast<u32x4 *>(lds_v + (j * RPI + kr) * VROW + ch * (16 / (int)sizeof(T))) = vpre[j];
         }
-        if (n + kWaves < n_tiles) prefetch(n + kWaves);
-        wave_sync();
+        if (n + kWaves < n_tiles) prefetch_v(n + kWaves);
 
-        // ---- S^T = K Q^T: 32 keys x 32 rows each --------------------------------------------------------
-        float16_t s[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[rb][r] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const u32x4 kf = *reinterpret_cast<const u32x4 *>(lds_k + l32 * KROW + (ks * 32 + hb * 16) / (int)sizeof(T));
-#pragma unroll
-            for (int rb = 0; rb < RB; rb++) {
-                if constexpr (H16) {
-                    s[rb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, kf), __builtin_bit_cast(half8_t, qf[rb][ks]), s[rb], 0, 0, 0);
-                } else {   // (one feature of each half's four at a time)
-                    const float4_t a = __builtin_bit_cast(float4_t, kf), c = __builtin_bit_cast(float4_t, qf[rb][ks]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[rb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], c[e], s[rb], 0, 0, 0);
-                }
-            }
-        }
-
-        // ---- softmax of row lane%32 over this lane's 16 keys k_lo + 8 (r / 4) + 4 hb + r % 4 -------------
-        half8_t pf[RB][2];
+        // ---- softmax of this lane's row over its keys k_lo + 4 grp + key_of(x) -----------------------------------
         if constexpr (SCORED) __builtin_amdgcn_sched_barrier(0);   // (V's fragments asked for during the scores' arithmetic spill registers)
+        if constexpr (SCORED) {
+            if (H16 && p.cap > 0.0f && p.cap <= kFastTanhCap) {
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++) {
-            if (rb > 0 && rb >= n_rb) break;
-            if constexpr (SCORED) {
-                if (H16 && p.cap > 0.0f && p.cap <= kFastTanhCap) {
+                for (int x = 0; x < NS; x++) s[x] = cap_log2 * fast_tanh(s[x] * to_cap);
+            } else if (p.cap > 0.0f) {
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[rb][r] = cap_log2 * fast_tanh(s[rb][r] * to_cap);
-                } else if (p.cap > 0.0f) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) s[rb][r] = cap_log2 * tanhf(s[rb][r] * to_cap);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) s[rb][r] *= to_log2;
-                }
-                if (p.slopes) {
-                    const float d0 = (float)(at[rb] - k_lo - 4 * hb);
-#pragma unroll
-                    for (int r = 0; r < 16; r++) s[rb][r] = __builtin_fmaf(-slope[rb], fabsf(d0 - (float)(8 * (r >> 2) + (r & 3))), s[rb][r]);
-                }
-                if (by_id) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int c = 8 * (r >> 2) + (r & 3), even = __builtin_amdgcn_readlane(id_tile, c), odd = __builtin_amdgcn_readlane(id_tile, c + 4), id = hb ? odd : even;
-                        s[rb][r] = id == doc[rb] ? s[rb][r] : -INFINITY;
-                    }
-                }
+                for (int x = 0; x < NS; x++) s[x] = cap_log2 * tanhf(s[x] * to_cap);
             } else {
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[rb][r] *= to_log2;
+                for (int x = 0; x < NS; x++) s[x] *= to_log2;
             }
-            const int last = lim[rb] - k_lo - 4 * hb;
-            if (__builtin_amdgcn_ballot_w64(last < 28) != 0) {
+            if (p.slopes) {
+                const float d0 = (float)(at - k_lo - 4 * grp);
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[rb][r] = 8 * (r >> 2) + (r & 3) <= last ? s[rb][r] : -INFINITY;
+                for (int x = 0; x < NS; x++) s[x] = __builtin_fmaf(-slope, fabsf(d0 - (float)key_of(x)), s[x]);
             }
-            float top = s[rb][0];
+            if (by_id) {
 #pragma unroll
-            for (int r = 1; r < 16; r++) top = fmaxf(top, s[rb][r]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
-            const bool moved = top > m_run[rb] + (H16 ? 8.0f : 0.0f);
-            const float m_new = moved ? top : m_run[rb], ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float keep = moved ? __builtin_amdgcn_exp2f(m_run[rb] - ref) : 1.0f;
-            m_run[rb] = m_new;
-            float sum = 0.0f;
+                for (int x = 0; x < NS; x++) {
+                    int id = __builtin_amdgcn_readlane(id_tile, key_of(x));
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                float e = __builtin_amdgcn_exp2f(s[rb][r] - ref);
-                if constexpr (H16) {   // the product with V takes f16 weights, and the row's sum the same ones
-                    pf[rb][r >> 3][r & 7] = (_Float16)e;
-                    e = (float)pf[rb][r >> 3][r & 7];
+                    for (int y = 1; y < NG; y++) {
+                        const int other = __builtin_amdgcn_readlane(id_tile, key_of(x) + 4 * y);
+                        id = grp == y ? other : id;
+                    }
+                    s[x] = id == doc ? s[x] : -INFINITY;
                 }
-                s[rb][r] = e;
-                sum += e;
             }
-            l_run[rb] = l_run[rb] * keep + sum;
-            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+        } else {
 #pragma unroll
-                for (int db = 0; db < DB; db++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[rb][db][r] *= keep;
-            }
+            for (int x = 0; x < NS; x++) s[x] *= to_log2;
         }
-
-        if constexpr (SCORED) __builtin_amdgcn_sched_barrier(0);
-        // ---- O^T += V^T P^T --------------------------------------------------------------------------------
-        if constexpr (H16) {
-            // this lane as a source of the transposing loads: key (lane%16)/4 of a group of four, features 16 (lane/16 % 2) + 4 (lane%4)
-            const _Float16 *vsrc = reinterpret_cast<const _Float16 *>(lds_v) + (4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const int last = lim - k_lo - 4 * grp;
+        if (__builtin_amdgcn_ballot_w64(last < 28) != 0) {
 #pragma unroll
-            for (int st2 = 0; st2 < 2; st2++)
+            for (int x = 0; x < NS; x++) s[x] = key_of(x) <= last ? s[x] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int x = 1; x < NS; x++) top = fmaxf(top, s[x]);
+#pragma unroll
+        for (int d = R; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
+        const bool moved = top > m_run + (H16 ? 8.0f : 0.0f);
+        const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
+        m_run = m_new;
+        half8_t pf[NS / 8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            float e = __builtin_amdgcn_exp2f(s[x] - ref);
+            if constexpr (H16) {   // the product with V takes f16 weights, and the row's sum the same ones
+                pf[x >> 3][x & 7] = (_Float16)e;
+                e = (float)pf[x >> 3][x & 7];
+            }
+            s[x] = e;
+            sum += e;
+        }
+        l_run = l_run * keep + sum;
+        if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int r = 0; r < NA; r++) o[db][r] *= keep;
+        }
+        if constexpr (SCORED) __builtin_amdgcn_sched_barrier(0);
+
+        // ---- O^T += V^T P^T --------------------------------------------------------------------------------
+        wave_sync();
+        if constexpr (H16) {
+            // this lane as a source of the transposing loads: key (lane%16)/4 of a group of four, features 4 (lane%4) of a block of 16
+            const _Float16 *vsrc = reinterpret_cast<const _Float16 *>(lds_v) + (4 * grp + ((lane & 15) >> 2)) * VROW + (R == 32 ? 16 * ((lane >> 4) & 1) : 0) + 4 * (lane & 3);
+#pragma unroll
+            for (int st = 0; st < NS / 8; st++)
 #pragma unroll
                 for (int db = 0; db < DB; db++) {
-                    const half4_t lo = lds_read_tr16(vsrc + (16 * st2) * VROW + 32 * db);       // keys 16 st2 + 4 hb + 0..3
-                    const half4_t hi = lds_read_tr16(vsrc + (16 * st2 + 8) * VROW + 32 * db);   // ... + 8
+                    // keys 4 grp + 0..3 of the two groups that the lane's weights st are of
+                    const half4_t lo = lds_read_tr16(vsrc + key_of(8 * st) * VROW + R * db), hi = lds_read_tr16(vsrc + key_of(8 * st + 4) * VROW + R * db);
                     const half8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int rb = 0; rb < RB; rb++)
-                        if (rb == 0 || rb < n_rb) o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[rb][st2], o[rb][db], 0, 0, 0);
+                    if constexpr (R == 16) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[st], o[db], 0, 0, 0);
+                    else o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[st], o[db], 0, 0, 0);
                 }
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; r++)
+            for (int x = 0; x < NS; x++)
 #pragma unroll
                 for (int db = 0; db < DB; db++) {
-                    const float a = lds_v[(8 * (r >> 2) + 4 * hb + (r & 3)) * VROW + 32 * db + l32];
-#pragma unroll
-                    for (int rb = 0; rb < RB; rb++)
-                        if (rb == 0 || rb < n_rb) o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[rb][r], o[rb][db], 0, 0, 0);
+                    const float a = lds_v[(key_of(x) + 4 * grp) * VROW + R * db + lr];
+                    if constexpr (R == 16) o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[x], o[db], 0, 0, 0);
+                    else o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[x], o[db], 0, 0, 0);
                 }
         }
         wave_sync();   // (the next tile goes where this one was)
     }
 
-    // ---- the four waves' results joined, a block of 32 rows at a time ------------------------------------------
-    float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + kWaves * 32 * CROW;
+    // ---- the four waves' results joined ------------------------------------------------------------------------
+    float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + kWaves * R * CROW;
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-        if (rb >= n_rb) break;
-        l_run[rb] += __shfl_xor(l_run[rb], 32, 64);
-        __syncthreads();   // tiles, or the block before, are done with
+    for (int d = R; d < 64; d <<= 1) l_run += __shfl_xor(l_run, d, 64);
+    __syncthreads();   // the tiles are done with
 #pragma unroll
-        for (int db = 0; db < DB; db++)
+    for (int db = 0; db < DB; db++)
 #pragma unroll
-            for (int x = 0; x < 4; x++)
-                *reinterpret_cast<float4_t *>(comb + (w * 32 + l32) * CROW + 32 * db + 8 * x + 4 * hb) =
-                    float4_t{o[rb][db][4 * x], o[rb][db][4 * x + 1], o[rb][db][4 * x + 2], o[rb][db][4 * x + 3]};
-        comb_ml[w * 64 + lane] = hb ? l_run[rb] : m_run[rb];
-        __syncthreads();
-        constexpr int TPR = kThreads / 32, PER = D / TPR;   // threads per row, features per thread
-        const int row = tid / TPR, r = row0 + 32 * rb + row;
-        if (r < row_end) {
-            float mm = -INFINITY, l = 0.0f, f[kWaves];
+        for (int x = 0; x < NA / 4; x++)
+            *reinterpret_cast<float4_t *>(comb + (w * R + lr) * CROW + R * db + (R == 32 ? 8 : 16) * x + 4 * grp) = float4_t{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
+    if (grp < 2) comb_ml[(w * 2 + grp) * R + lr] = grp ? l_run : m_run;
+    __syncthreads();
+    constexpr int TPR = kThreads / R, PER = D / TPR;   // threads per row, features per thread
+    const int row = tid / TPR, r = wk.row0 + row;
+    if (r >= wk.row_end) return;
+    float mm = -INFINITY, l = 0.0f, f[kWaves];
 #pragma unroll
-            for (int x = 0; x < kWaves; x++) mm = fmaxf(mm, comb_ml[x * 64 + row]);
-            const float ref = mm == -INFINITY ? 0.0f : mm;
+    for (int x = 0; x < kWaves; x++) mm = fmaxf(mm, comb_ml[x * 2 * R + row]);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-            for (int x = 0; x < kWaves; x++) {
-                f[x] = __builtin_amdgcn_exp2f(comb_ml[x * 64 + row] - ref);
-                l += f[x] * comb_ml[x * 64 + 32 + row];
-            }
-            const int bi = r / p.G, g = r - bi * p.G, rb_b = bi / p.Sq, i = bi - rb_b * p.Sq;
-            const int64_t orow = ((int64_t)rb_b * p.Hq + kvh * p.G + g) * p.Sq + i;
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    for (int x = 0; x < kWaves; x++) {
+        f[x] = __builtin_amdgcn_exp2f(comb_ml[x * 2 * R + row] - ref);
+        l += f[x] * comb_ml[(x * 2 + 1) * R + row];
+    }
+    const int64_t orow = q_row(p, wk.kvh, r).at;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-            for (int e = 0; e < PER; e += 4) {
-                const int d = (tid % TPR) * 4 + e * TPR;   // (16 bytes per thread, threads of a row side by side)
-                float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int e = 0; e < PER; e += 2) {
+        const int d = (tid % TPR) * 2 + e * TPR;   // (8 bytes per thread, threads of a row side by side: a store covers whole lines)
+        float2_t acc = {0.0f, 0.0f};
 #pragma unroll
-                for (int x = 0; x < kWaves; x++) {
-                    const float4_t v = *reinterpret_cast<const float4_t *>(comb + (x * 32 + row) * CROW + d);
+        for (int x = 0; x < kWaves; x++) {
+            const float2_t v = *reinterpret_cast<const float2_t *>(comb + (x * R + row) * CROW + d);
 #pragma unroll
-                    for (int y = 0; y < 4; y++) acc[y] = __builtin_fmaf(f[x], v[y], acc[y]);
-                }
-                if (p.splits == 1) {
-                    T *out = reinterpret_cast<T *>(p.out) + orow * D + d;
-                    struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
-#pragma unroll
-                    for (int y = 0; y < 4; y++) four.e[y] = (T)(acc[y] * inv);
-                    *reinterpret_cast<Four *>(out) = four;
-                } else {
-                    *reinterpret_cast<float4_t *>(p.part_o + ((int64_t)split * p.part_rows + orow) * D + d) = acc;
-                }
-            }
-            if (p.splits > 1 && tid % TPR == 0) {
-                *part_m(orow) = mm;
-                *(part_m(orow) + p.part_rows) = l;
-            }
+            for (int y = 0; y < 2; y++) acc[y] = __builtin_fmaf(f[x], v[y], acc[y]);
         }
+        if (p.splits == 1) {
+            struct alignas(2 * sizeof(T)) Two { T e[2]; } two;
+            two.e[0] = (T)(acc[0] * inv), two.e[1] = (T)(acc[1] * inv);
+            *reinterpret_cast<Two *>(reinterpret_cast<T *>(p.out) + orow * D + d) = two;
+        } else {
+            put2(p.part_o + ((int64_t)wk.split * p.part_rows + orow) * D + d, acc);
+        }
+    }
+    if (p.splits > 1 && tid % TPR == 0) {
+        put(part_ml + orow, mm);
+        put(part_ml + orow + p.part_rows, l);
     }
 }
 
-// The ranges' partial rows -> output rows: D / 4 lanes per row.
+// A tile of 128 f16 rows over a prefix: a tile of 64 keys is staged once for the four waves, 32 rows each (as sdpa_scored.hip has
+// it).  Tiles of [t_begin, t_end) count 64 keys.  Always a part: `splits` > 1.
+constexpr int kTallTile = 64, kTallRows = 128;
+template <int D>
+__device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, unsigned char *lds) {
+    constexpr int KS = D / 16, DB = D / 32, KROW = D + 8, VROW = D + 16;
+    constexpr int PPR = D / 8, RPI = kThreads / PPR, NL = kTallTile / RPI;   // 16-byte pieces per row, rows per load of the workgroup, loads per tile and tensor
+    constexpr int K_TILE = kTallTile * KROW, V_TILE = kTallTile * VROW;
+    _Float16 *lds_k = reinterpret_cast<_Float16 *>(lds), *lds_v = lds_k + 2 * K_TILE;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
+    const int my_row = wk.row0 + 32 * w + l32, n_tiles = wk.t_end - wk.t_begin;
+    const bool wave_has_rows = wk.row0 + 32 * w < wk.row_end;
+    const int64_t out_row = q_row(p, wk.kvh, min(my_row, wk.row_end - 1)).at;
+    const int key0 = tid / PPR, ch = tid % PPR;
+    const uint32_t lane_off = (uint32_t)key0 * (uint32_t)wk.st + ch * 16;
+    u32x4 kpre[NL], vpre[NL];
+    auto prefetch = [&](int n) __attribute__((always_inline)) {
+        const int k_lo = (wk.t_begin + n) * kTallTile, most = wk.n_keys - 1 - k_lo;
+        const char *tk = wk.k + (int64_t)k_lo * wk.st, *tv = wk.v + (int64_t)k_lo * wk.st;
+        if (most >= kTallTile - 1) {   // wave-uniform addresses and one offset per lane
+            uint32_t o = lane_off;
+            asm volatile("" : "+v"(o));   // (stays a 32-bit offset up to the loads)
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                kpre[j] = load16(tk + (int64_t)(j * RPI) * wk.st, o);
+                vpre[j] = load16(tv + (int64_t)(j * RPI) * wk.st, o);
+            }
+        } else {   // rows past the last key repeat it
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const uint32_t o = (uint32_t)min(key0 + j * RPI, most) * (uint32_t)wk.st + ch * 16;
+                kpre[j] = load16(tk, o);
+                vpre[j] = load16(tv, o);
+            }
+        }
+    };
+    auto stage = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            *reinterpret_cast<u32x4 *>(lds_k + buf * K_TILE + (key0 + j * RPI) * KROW + ch * 8) = kpre[j];
+            *reinterpret_cast<u32x4 *>(lds_v + buf * V_TILE + (key0 + j * RPI) * VROW + ch * 8) = vpre[j];
+        }
+    };
+    float m_run = -INFINITY, l_run = 0.0f;
+    float16_t o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int x = 0; x < 16; x++) o[db][x] = 0.0f;
+    const float to_log2 = p.scale * kLog2e;
+    u32x4 qf[KS];
+    prefetch(0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = load16(p.q + out_row * (2 * D), 32 * ks + 16 * hb);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));   // settled here, not by a wait in the loop that would take the prefetch in too
+    stage(0);
+    if (n_tiles > 1) prefetch(1);
+    for (int n = 0; n < n_tiles; n++) {
+        const int buf = n & 1;
+        __syncthreads();   // tile n is in LDS; every wave is done with the buffers about to be overwritten
+        if (wave_has_rows) {
+            float16_t s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) s[kb][x] = 0.0f;
+            const _Float16 *ksrc = lds_k + buf * K_TILE + l32 * KROW + 8 * hb;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t *>(ksrc + 32 * kb * KROW + 16 * ks), __builtin_bit_cast(half8_t, qf[ks]), s[kb], 0, 0, 0);
+            // this lane's keys: 4 hb + c, c = 32 kb + 8 (x / 4) + x % 4
+            const int last = wk.n_keys - 1 - (wk.t_begin + n) * kTallTile - 4 * hb;
+            if (last < 60) {
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) s[kb][x] = 32 * kb + 8 * (x >> 2) + (x & 3) <= last ? s[kb][x] : -INFINITY;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb][x]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * to_log2;   // (scale > 0: the maximum commutes with it)
+            const bool moved = top > m_run + 8.0f;   // (as above)
+            const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
+            m_run = m_new;
+            half8_t pf[4];
+            float sum = 0.0f;
+            const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, -ref));
+#pragma unroll
+                for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
+            }
+            l_run = l_run * keep + sum;
+            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) o[db][x] *= keep;
+            }
+            const _Float16 *vsrc = lds_v + buf * V_TILE + (4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+            for (int st = 0; st < 4; st++)
+#pragma unroll
+                for (int db = 0; db < DB; db++) {
+                    const half4_t lo = lds_read_tr16(vsrc + 16 * st * VROW + 32 * db), hi = lds_read_tr16(vsrc + (16 * st + 8) * VROW + 32 * db);
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[st], o[db], 0, 0, 0);
+                }
+        }
+        if (n + 1 < n_tiles) {   // the next tile to LDS after this one's arithmetic
+            stage(buf ^ 1);
+            if (n + 2 < n_tiles) prefetch(n + 2);
+        }
+    }
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (my_row < wk.row_end) p.part_ml[((int64_t)wk.split * 2 + hb) * p.part_rows + out_row] = hb ? l_run : m_run;
+    // rows to their places in whole lines, through a corner of LDS of the wave's own
+    constexpr int CROW = D + 4, LPR = D / 4, RPS = 64 / LPR;
+    static_assert(kWaves * 32 * CROW * 4 <= 2 * (K_TILE + V_TILE) * 2, "the output goes through the tiles' LDS");
+    float *tr = reinterpret_cast<float *>(lds) + w * 32 * CROW;
+    __syncthreads();
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) *reinterpret_cast<float4_t *>(tr + l32 * CROW + 32 * db + 8 * x + 4 * hb) = float4_t{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
+    wave_sync();
+    float *po = p.part_o + (int64_t)wk.split * p.part_rows * D;
+#pragma unroll 4
+    for (int j = 0; j < 32 / RPS; j++) {
+        const int row = j * RPS + lane / LPR, r = wk.row0 + 32 * w + row;
+        if (r < wk.row_end) *reinterpret_cast<float4_t *>(po + q_row(p, wk.kvh, r).at * D + lane % LPR * 4) = *reinterpret_cast<const float4_t *>(tr + row * CROW + lane % LPR * 4);
+    }
+}
+
+// A row's parts -> its output, by D / 4 lanes of a wave.  Everything that some 8 ranges have is asked for at once: one latency for up to
+// 8 of them.  (At most 64.)
+template <typename T, int D, bool LIVE>   // LIVE: parts that other workgroups of this launch have stored
+__device__ __forceinline__ void join_row(const float *part_o, const float *part_ml, T *out, int64_t row, int64_t rows, int splits) {
+    constexpr int LPR = D / 4, MOST = 64 / LPR, BATCH = 8;
+    const int lr = threadIdx.x % LPR;
+    const float *po = part_o + row * D + 2 * lr;   // this lane's features: two, and two half a row on
+    auto word = [](const float *at) { return LIVE ? get(at) : *at; };
+    auto two = [](const float *at) { return LIVE ? get2(at) : *reinterpret_cast<const float2_t *>(at); };
+    float f[MOST], ls[MOST], l = 0.0f, mm = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < MOST; x++) {
+        const int s = min(x * LPR + lr, splits - 1);
+        f[x] = word(part_ml + (int64_t)s * 2 * rows + row);
+        ls[x] = word(part_ml + ((int64_t)s * 2 + 1) * rows + row);
+    }
+    float2_t v[BATCH][2];
+    auto ask = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int y = 0; y < BATCH; y++) {
+            const float *at = po + (int64_t)min(s0 + y, splits - 1) * rows * D;
+            v[y][0] = two(at), v[y][1] = two(at + D / 2);
+        }
+    };
+    ask(0);
+#pragma unroll
+    for (int x = 0; x < MOST; x++) {
+        if (x * LPR + lr >= splits) f[x] = -INFINITY;
+        mm = fmaxf(mm, f[x]);
+    }
+#pragma unroll
+    for (int w = 1; w < LPR; w <<= 1) mm = fmaxf(mm, __shfl_xor(mm, w, 64));
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+    for (int x = 0; x < MOST; x++) {
+        const bool has = f[x] != -INFINITY;   // (a range without keys for the row has stored nothing else)
+        f[x] = has ? __builtin_amdgcn_exp2f(f[x] - ref) : 0.0f;
+        l += has ? f[x] * ls[x] : 0.0f;
+    }
+#pragma unroll
+    for (int w = 1; w < LPR; w <<= 1) l += __shfl_xor(l, w, 64);
+    float2_t acc[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+    for (int s0 = 0; s0 < splits; s0 += BATCH) {
+#pragma unroll
+        for (int y = 0; y < BATCH; y++) {
+            float g = 0.0f;
+#pragma unroll
+            for (int x = 0; x < MOST; x++) {
+                const float h = __shfl(f[x], (s0 + y) % LPR, LPR);
+                g = (s0 + y) / LPR == x ? h : g;
+            }
+            if (s0 + y >= splits) g = 0.0f;
+#pragma unroll
+            for (int z = 0; z < 2; z++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) acc[z][e] = g != 0.0f ? __builtin_fmaf(g, v[y][z][e], acc[z][e]) : acc[z][e];
+        }
+        if (s0 + BATCH < splits) ask(s0 + BATCH);
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int z = 0; z < 2; z++) {
+        struct alignas(2 * sizeof(T)) Two { T e[2]; } pair;
+        pair.e[0] = (T)(acc[z][0] * inv), pair.e[1] = (T)(acc[z][1] * inv);
+        *reinterpret_cast<Two *>(out + row * D + z * (D / 2) + 2 * lr) = pair;
+    }
+}
+
+// The last workgroup to bring a part of a unit's rows joins them.  A unit is a tile of one sequence's rows (own keys) or, where no
+// sequence has keys of its own, a tile of rows of the prefix; a tile over the prefix holds rows of up to 32 units and brings a
+// part to each.  Counters are zero between launches.
+template <typename T, int D, int PRE, int OWN>
+__device__ __forceinline__ void arrive(const RowsDev &p, const RowsWork &wk, uint32_t *s_done) {
+    const int tid = threadIdx.x, seq_rows = p.Sq * p.G, n_units = p.own_row_tiles ? p.B * p.own_row_tiles : p.p_row_tiles;
+    auto unit_of = [&](int r) {
+        if (!p.own_row_tiles) return r / (PRE ? PRE : 1);
+        const int b = p.by_sq.by(p.by_g.by(r));
+        return b * p.own_row_tiles + (r - b * seq_rows) / OWN;
+    };
+    auto rows_of = [&](int u, int &r0, int &r1) {
+        if (!p.own_row_tiles) {
+            r0 = u * (PRE ? PRE : 1), r1 = min(r0 + (PRE ? PRE : 1), p.B * seq_rows);
+        } else {
+            const int b = p.by_own_row_tiles.by(u);
+            r0 = b * seq_rows + (u - b * p.own_row_tiles) * OWN, r1 = min(r0 + OWN, (b + 1) * seq_rows);
+        }
+    };
+    const int first = unit_of(wk.row0), n = unit_of(wk.row_end - 1) - first + 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
+    __syncthreads();                                     // ... and so have the whole workgroup's
+    if (tid < 64) {
+        bool last = false;
+        if (tid < n) {
+            int r0, r1;
+            rows_of(first + tid, r0, r1);
+            const int parts = p.own_row_tiles ? p.own_splits + (PRE ? p.p_splits * ((r1 - 1) / (PRE ? PRE : 1) - r0 / (PRE ? PRE : 1) + 1) : 0) : p.p_splits;
+            int *counter = p.counters + (int64_t)wk.kvh * n_units + first + tid;
+            last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+            if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        const uint64_t done = __builtin_amdgcn_ballot_w64(last);
+        if (tid == 0) *s_done = (uint32_t)done;   // (n <= 32)
+    }
+    __syncthreads();
+    const uint32_t done = *s_done;
+    if (done == 0) return;
+    int begin, end, unused;
+    rows_of(first, begin, unused), rows_of(first + n - 1, unused, end);
+    constexpr int LPR = D / 4;
+    for (int r = begin + tid / LPR; r < end; r += kThreads / LPR)   // (whole groups of LPR lanes stay or leave)
+        if ((done >> (unit_of(r) - first)) & 1)
+            join_row<T, D, true>(p.part_o, p.part_ml, reinterpret_cast<T *>(p.out), q_row(p, wk.kvh, r).at, p.part_rows, p.splits);
+}
+
+constexpr int rows_lds(int es, int D, int R) {   // rows_body's LDS
+    return kWaves * kTile * ((es == 2 ? D + 16 : R == 16 ? D + 4 : D + 8) + (R == 32 ? (es == 2 ? D + 8 : D + 4) : 0)) * es;
+}
+constexpr int tall_lds(int D) { return 2 * kTallTile * (2 * D + 24) * 2; }
+constexpr int most_of(int a, int b) { return a > b ? a : b; }
+
+// PRE: rows of a tile over the prefix, 128 the tall body (0: there is none); OWN: over own keys.
+template <typename T, int D, int PRE, int OWN, bool SCORED>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 || OWN == 32) ? 1 : 2) void sdpa_rows_kernel(RowsCall call) {
+    const RowsDev &p = call.p;
+    constexpr int ES = sizeof(T);
+    __shared__ __attribute__((aligned(16))) unsigned char lds[most_of(rows_lds(ES, D, OWN), PRE == 128 ? tall_lds(D) : PRE ? rows_lds(ES, D, PRE) : 0)];
+    __shared__ uint16_t s_list[SCORED ? kListMax : 1];
+    __shared__ int s_counts[kWaves];
+    __shared__ uint32_t s_done;
+    int item = blockIdx.y;
+    RowsWork wk;
+    wk.kvh = blockIdx.x;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
+    if (PRE && item < p.p_items) {
+        constexpr int ROWS = PRE ? PRE : 1, TILE = PRE == 128 ? kTallTile : kTile;
+        wk.b = -1;
+        wk.split = p.by_p_row_tiles.by(item);
+        wk.row0 = (item - wk.split * p.p_row_tiles) * ROWS, wk.row_end = min(wk.row0 + ROWS, p.B * p.Sq * p.G);
+        wk.k = p.pk + (int64_t)wk.kvh * p.p_stride_h, wk.v = p.pv + (int64_t)wk.kvh * p.p_stride_h, wk.st = p.p_stride_t;
+        wk.n_keys = p.P;
+        wk.t_begin = wk.split * p.p_tiles, wk.t_end = min((p.P + TILE - 1) / TILE, wk.t_begin + p.p_tiles);
+        if constexpr (PRE == 128) {
+            tall_body<D>(p, wk, lds);
+            return;
+        } else if constexpr (PRE != 0 && PRE != OWN) {
+            rows_body<T, D, PRE, false>(p, wk, lds, nullptr, nullptr);
+            if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
+            return;
+        }
+    } else {
+        if (PRE) item -= p.p_items;
+        const int at = p.by_own_splits.by(item), split = item - at * p.own_splits, b = p.by_own_row_tiles.by(at);
+        const int rt = p.own_row_tiles - 1 - (at - b * p.own_row_tiles);   // (the longest first)
+        wk.b = p.seq0 + b;
+        const OwnKeys own = own_keys(p, wk.b, wk.kvh);
+        wk.k = own.k, wk.v = own.v, wk.st = p.stride_t, wk.n_keys = own.len;
+        wk.row0 = wk.b * p.Sq * p.G + rt * OWN, wk.row_end = min(wk.row0 + OWN, (wk.b + 1) * p.Sq * p.G);
+        int n_vis = own.len;
+        if (p.causal) {
+            n_vis = p.by_g.by(wk.row_end - 1) - wk.b * p.Sq + own.len - p.Sq + 1;
+            if (SCORED && p.prefix_lens) n_vis = max(n_vis, p.prefix_lens[wk.b]);
+            n_vis = max(0, min(n_vis, own.len));
+        }
+        wk.t_begin = split * p.own_tiles, wk.t_end = min((n_vis + kTile - 1) / kTile, wk.t_begin + p.own_tiles);
+        wk.split = p.p_splits + split;
+    }
+    rows_body<T, D, OWN, SCORED>(p, wk, lds, s_list, s_counts);
+    if constexpr (PRE != 128)
+        if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
+}
+
+// The same in a launch of its own: after tall tiles, whose last workgroup would have 128 rows to join.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void sdpa_rows_merge_kernel(const float *__restrict__ part_o, const float *__restrict__ part_ml, T *__restrict__ out, int64_t rows, int splits) {
     constexpr int LPR = D / 4;
-    const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    const int d = threadIdx.x % LPR * 4;
-    if (row >= rows) return;
-    float mm = -INFINITY;
-    for (int s = 0; s < splits; s++) mm = fmaxf(mm, part_ml[(int64_t)s * 2 * rows + row]);
-    float l = 0.0f;
-    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = 0; s < splits; s++) {
-        const float m = part_ml[(int64_t)s * 2 * rows + row];
-        if (m == -INFINITY) continue;   // (a range without keys for the row has stored nothing else)
-        const float f = __builtin_amdgcn_exp2f(m - mm);
-        const float4_t v = *reinterpret_cast<const float4_t *>(part_o + ((int64_t)s * rows + row) * D + d);
-        l += f * part_ml[((int64_t)s * 2 + 1) * rows + row];
-#pragma unroll
-        for (int y = 0; y < 4; y++) acc[y] = __builtin_fmaf(f, v[y], acc[y]);
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
-#pragma unroll
-    for (int y = 0; y < 4; y++) four.e[y] = (T)(acc[y] * inv);
-    *reinterpret_cast<Four *>(out + row * D + d) = four;
+    join_row<T, D, false>(part_o, part_ml, out, min((int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, rows - 1), rows, splits);   // (rows past the last write it again, the same)
 }
 
 int check_launch(const char *what) {
@@ -650,22 +974,24 @@ int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_n
 
 namespace {
 
-template <typename T, int D, int RB, bool SCORED>
+template <typename T, int D, int PRE, int OWN, bool SCORED>
 int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
     RowsDev &p = call.p;
-    const int64_t holds = table_holds(a);
+    const int64_t prefix_items = (int64_t)p.p_splits * p.p_row_tiles, per_seq = (int64_t)p.own_row_tiles * p.own_splits, most = 65535;
+    int64_t holds = table_holds(a);   // sequences of a launch
+    if (per_seq && holds > (most - prefix_items) / per_seq) holds = (most - prefix_items) / per_seq;
+    TROCM_REQUIRE(holds > 0 && prefix_items <= most, "attention: too many workgroups");
     for (int64_t b = 0; b < a.B; b += holds) {   // the prefix, for all rows, with the first sequences' own keys
         const int64_t n = a.B - b < holds ? a.B - b : holds;
         fill_table(a, b, n, call.tab);
         p.seq0 = (int)b;
-        p.p_items = b == 0 ? p.p_splits * p.p_row_tiles : 0;
-        const int64_t grid = a.Hkv * (p.p_items + n * p.own_row_tiles * p.own_splits);
-        if (grid == 0) continue;
-        TROCM_REQUIRE(grid < (1ll << 31), "attention: too many workgroups");
-        hipLaunchKernelGGL((sdpa_rows_kernel<T, D, RB, SCORED>), dim3((unsigned)grid), dim3(kThreads), 0, s, call);
+        p.p_items = b == 0 ? (int)prefix_items : 0;
+        const int64_t items = p.p_items + n * p.own_row_tiles * p.own_splits;
+        if (items == 0) continue;
+        hipLaunchKernelGGL((sdpa_rows_kernel<T, D, PRE, OWN, SCORED>), dim3((unsigned)a.Hkv, (unsigned)items), dim3(kThreads), 0, s, call);
         if (check_launch("sdpa_rows")) return 1;
     }
-    if (p.splits > 1) {
+    if (p.splits > 1 && !p.counters) {
         constexpr int ROWS = 256 / (D / 4);
         hipLaunchKernelGGL((sdpa_rows_merge_kernel<T, D>), dim3((unsigned)((p.part_rows + ROWS - 1) / ROWS)), dim3(256), 0, s, p.part_o, p.part_ml, (T *)p.out, p.part_rows, p.splits);
         if (check_launch("sdpa_rows_merge")) return 1;
@@ -674,17 +1000,26 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
 }
 
 template <typename T, int D>
-int launch_tiles_of(const SdpaRowsArgs &a, RowsCall &call, int rb, bool is_scored, hipStream_t s) {
+int launch_tiles_of(const SdpaRowsArgs &a, RowsCall &call, int pre, int own, bool is_scored, hipStream_t s) {
+    if (is_scored) return own == 16 ? launch_tiles<T, D, 0, 16, true>(a, call, s) : launch_tiles<T, D, 0, 32, true>(a, call, s);
+    if (own == 32) {
+        if constexpr (sizeof(T) == 2)
+            if (pre == 128) return launch_tiles<T, D, 128, 32, false>(a, call, s);
+        return launch_tiles<T, D, 32, 32, false>(a, call, s);
+    }
     if constexpr (sizeof(T) == 2)
-        if (rb == 2) return launch_tiles<T, D, 2, false>(a, call, s);
-    return is_scored ? launch_tiles<T, D, 1, true>(a, call, s) : launch_tiles<T, D, 1, false>(a, call, s);
+        if (pre == 128) return launch_tiles<T, D, 128, 16, false>(a, call, s);
+    return pre == 32 ? launch_tiles<T, D, 32, 16, false>(a, call, s) : launch_tiles<T, D, 16, 16, false>(a, call, s);
 }
+
+// Rounds of a workgroup with `per` tiles of `all`.
+double p_round_of(int64_t per, int64_t all, double step) { return (double)(per < all ? per : all) / step; }
 
 // On the matrix cores: 0 done, 1 failed, 2 not covered.
 int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     const int64_t es = (int64_t)elem_bytes(a.dtype);
     if (a.D != 64 && a.D != 128) return 2;
-    const int64_t G = a.Hq / a.Hkv, rows = a.B * a.Sq * G;
+    const int64_t G = a.Hq / a.Hkv, rows = a.B * a.Sq * G, rows_all = rows * a.Hkv;
     if (rows >= (1ll << 30)) return 2;
     auto aligned = [&](const void *x) { return (uintptr_t)x % 16 == 0; };
     auto strides = [&](int64_t x) { return x * es % 16 == 0; };
@@ -703,31 +1038,67 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     if (!ok || (a.P == 0 && longest == 0)) return 2;
 
     const bool is_scored = a.softcap > 0.0f || a.slopes || a.documents || a.prefix_lens;
-    const int rb = es == 2 && !is_scored && (a.P ? rows : seq_rows) > 32 ? 2 : 1, MR = 32 * rb;
+    const int own = seq_rows <= 16 ? 16 : 32;
+    const int64_t room = a.workspace && aligned(a.workspace) && a.workspace_bytes > kWsCounterBytes + kWsPlanBytes + 256
+                             ? (int64_t)(a.workspace_bytes - kWsCounterBytes - kWsPlanBytes - 256) / ((a.D + 2) * (int64_t)sizeof(float)) / rows_all : 0;
+    const int pre = a.P == 0 ? own : es == 2 && rows > 64 && a.P > kTallTile && room >= 2 && a.scale > 0.0f ? 128 : rows > 16 ? 32 : own;   // (the tall body stores parts only)
     RowsCall call;
     RowsDev &p = call.p;
     fill_rows(a, p);
-    const int64_t p_all = (a.P + kTile - 1) / kTile, own_all = (longest + kTile - 1) / kTile;
-    p.p_row_tiles = a.P ? (int)((rows + MR - 1) / MR) : 0;
-    p.own_row_tiles = longest ? (int)((seq_rows + MR - 1) / MR) : 0;
-    // Ranges: as much work for each workgroup as makes `target` of them in all, a multiple of a tile per wave.
-    const int64_t target = (int64_t)num_compute_units() * (rb == 1 && es == 2 ? 2 : 1);
-    const int64_t work = a.Hkv * (p.p_row_tiles * p_all + p.own_row_tiles * own_tiles_all);
-    int64_t per = ((work + target - 1) / target + kWaves - 1) / kWaves * kWaves;
-    const int64_t room = a.workspace && aligned(a.workspace) && a.workspace_bytes > kWsCounterBytes + kWsPlanBytes + 256
-                             ? (int64_t)(a.workspace_bytes - kWsCounterBytes - kWsPlanBytes - 256) / ((a.D + 2) * (int64_t)sizeof(float)) / p.part_rows : 0;
-    for (;; per *= 2) {
-        p.p_tiles = p.own_tiles = (int)per;
-        p.p_splits = (int)((p_all + per - 1) / per), p.own_splits = (int)((own_all + per - 1) / per);
+    const int64_t p_tile = pre == 128 ? kTallTile : kTile, p_all = (a.P + p_tile - 1) / p_tile, own_all = (longest + kTile - 1) / kTile;
+    p.p_row_tiles = a.P ? (int)((rows + pre - 1) / pre) : 0;
+    p.own_row_tiles = longest ? (int)((seq_rows + own - 1) / own) : 0;
+    // Ranges of keys, by what each choice is expected to take (us).  A workgroup takes `start` and a round of a tile per wave `round`;
+    // all of them together what their tiles take at the rate of memory or of the matrix cores, and `start` times their rounds over the
+    // chip; parts that are joined `join` more each.  (An estimate: it only has to rank the choices.)
+    const bool f32 = es == 4;
+    const double wide = a.D == 128 ? 1.0 : 0.5, cus = num_compute_units();
+    const double own_round = f32 ? (own == 32 ? 3.6 : 2.0) * wide : 0.4 + (own == 32 ? 1.2 : 0.7) * wide;
+    const double own_rate = (f32 ? (own == 32 ? 3.6 : 2.0) : 0.8) * wide / cus / kWaves, pre_rate = pre == 128 ? 1.5 * (0.4 + 0.6 * wide) / cus : (f32 ? (pre == 32 ? 3.6 : 2.0) : pre == 32 ? 1.0 : 0.6) * wide / cus / kWaves;
+    const double pre_round = pre == 128 ? 0.8 + 0.8 * wide : f32 ? (pre == 32 ? 3.6 : 2.0) * wide : 0.4 + (pre == 32 ? 1.2 : 0.7) * wide;
+    const double start = 2.5, slots = cus * (f32 && a.D == 128 && (own == 32 || pre == 32) ? 1 : 2), p_step = pre == 128 ? 1 : kWaves;
+    int64_t p_per = 1, o_per = kWaves;
+    double best = 1e30;
+    for (int64_t op = kWaves;; op = op * 2 > own_all ? (own_all + kWaves - 1) / kWaves * kWaves : op * 2) {
+        int64_t own_wgs = 0;
+        if (a.lens || a.seqs)
+            for (int64_t b = 0; b < a.B; b++) own_wgs += ((a.lens ? a.lens[b] : a.seqs[b].len) + op * kTile - 1) / (op * kTile);
+        else own_wgs = a.B * ((own_all + op - 1) / op);
+        own_wgs *= a.Hkv * p.own_row_tiles;
+        const int64_t own_n = (own_all + op - 1) / op;
+        for (int64_t pp = pre == 128 ? 4 : kWaves;; pp = pp * 2) {
+            const int64_t p_n = (p_all + pp - 1) / pp, p_wgs = a.Hkv * p.p_row_tiles * p_n;
+            const double longest_wg = start + (a.P && p_round_of(pp, p_all, p_step) * pre_round > (double)((op < own_all ? op : own_all) + kWaves - 1) / kWaves * own_round
+                                                   ? p_round_of(pp, p_all, p_step) * pre_round : (longest ? ((op < own_all ? op : own_all) + kWaves - 1) / kWaves * own_round : 0.0));
+            const double all = start * (double)((own_wgs + p_wgs + slots - 1) / slots) + a.Hkv * (p.own_row_tiles * own_tiles_all * own_rate + p.p_row_tiles * p_all * pre_rate);
+            const double parts = (double)(own_n + p_n);
+            const double join = parts > 1 ? (pre == 128 ? 5.0 : 1.5) + parts * (0.1 + rows_all * (a.D + 2) * 8.0 / 4e6) : 0.0;
+            const double t = (longest_wg > all ? longest_wg : all) + join;
+            if (t < best) best = t, p_per = pp, o_per = op;
+            if (pp >= p_all) break;
+        }
+        if (op >= own_all) break;
+    }
+    if (pre == 128 && longest == 0 && p_per > (p_all + 1) / 2) p_per = (p_all + 1) / 2;
+    for (;; p_per *= 2, o_per *= 2) {
+        p.p_tiles = (int)p_per, p.own_tiles = (int)o_per;
+        p.p_splits = (int)((p_all + p_per - 1) / p_per), p.own_splits = (int)((own_all + o_per - 1) / o_per);
         p.splits = p.p_splits + p.own_splits;
         if (p.splits == 1 || (p.splits <= room && p.splits <= 64)) break;
         if (p.p_splits <= 1 && p.own_splits <= 1) return 2;   // (no room to join prefix and own keys in)
     }
+    p.by_g = fast_div(G), p.by_sq = fast_div(a.Sq), p.by_p_row_tiles = fast_div(p.p_row_tiles);
+    p.by_own_splits = fast_div(p.own_splits), p.by_own_row_tiles = fast_div(p.own_row_tiles);
     p.part_o = (float *)((char *)a.workspace + kWsCounterBytes + kWsPlanBytes);
     p.part_ml = p.part_o + (int64_t)p.splits * p.part_rows * a.D;
     if (p.splits == 1) p.part_o = p.part_ml = nullptr;
-    if (a.dtype == TROCM_F16) return a.D == 64 ? launch_tiles_of<_Float16, 64>(a, call, rb, is_scored, s) : launch_tiles_of<_Float16, 128>(a, call, rb, is_scored, s);
-    return a.D == 64 ? launch_tiles_of<float, 64>(a, call, rb, is_scored, s) : launch_tiles_of<float, 128>(a, call, rb, is_scored, s);
+    const int64_t units = a.Hkv * (p.own_row_tiles ? a.B * p.own_row_tiles : p.p_row_tiles);
+    // Joined by the last to arrive where that is at most two rows for a group of D / 4 lanes: 4 x 777 + 40 keys 9.5 -> 8.5 us, but
+    // 16 x 2000 + 600 keys, whose tiles over the prefix hold four rows for each, 13.5 -> 19.3 us.
+    const int64_t joined = a.P ? (rows < pre ? rows : pre) : own;
+    if (p.splits > 1 && pre != 128 && joined * a.D <= 2048 && units <= (int64_t)(kWsCounterBytes / sizeof(int))) p.counters = (int *)a.workspace;
+    if (a.dtype == TROCM_F16) return a.D == 64 ? launch_tiles_of<_Float16, 64>(a, call, pre, own, is_scored, s) : launch_tiles_of<_Float16, 128>(a, call, pre, own, is_scored, s);
+    return a.D == 64 ? launch_tiles_of<float, 64>(a, call, pre, own, is_scored, s) : launch_tiles_of<float, 128>(a, call, pre, own, is_scored, s);
 }
 
 }  // namespace

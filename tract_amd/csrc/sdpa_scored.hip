@@ -103,29 +103,26 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
 #pragma unroll
             for (int x = 0; x < kWaves; x++) dmin = min(dmin, s_range[0][x]), dmax = max(dmax, s_range[1][x]);
             const int one_doc = dmin == dmax ? dmin : -1;
+            // A wave looks at a tile at a time, a token per lane, at 16 of them before the waves compare.
+            constexpr int PW = 16;
             int n = 0;
-            for (int t0 = t_begin; t0 < t_end; t0 += kThreads) {
-                const int t = t0 + tid;
-                int lo = INT_MAX, hi = -1, neg = 0;
-                if (t < t_end) {
-                    const int first = t * kTile, last = min(first + kTile, p.Sk);
-#pragma unroll 8
-                    for (int j = first; j < last; j++) {
-                        const int x = docs[j];
-                        neg |= x;
-                        lo = min(lo, x < 0 ? INT_MAX : x), hi = max(hi, x);
-                    }
+            for (int t0 = t_begin; t0 < t_end; t0 += kWaves * PW) {
+                const int first = t0 + w * PW;
+                uint32_t active = 0, whole = 0;
+#pragma unroll
+                for (int x = 0; x < PW; x++) {   // (all loads in flight at once)
+                    const int id = first + x < t_end ? docs[min((first + x) * kTile + lane, p.Sk - 1)] : -1;
+                    active |= (__builtin_amdgcn_ballot_w64(id >= dmin && id <= dmax && id >= 0) != 0 ? 1u : 0u) << x;
+                    whole |= (__builtin_amdgcn_ballot_w64(id == one_doc && id >= 0) == ~0ull ? 1u : 0u) << x;
                 }
-                const bool active = hi >= dmin && lo <= dmax;
-                const uint64_t mask = __builtin_amdgcn_ballot_w64(active);
-                if (lane == 0) s_counts[w] = __popcll(mask);
+                if (lane == 0) s_counts[w] = __popc(active);
                 __syncthreads();
                 int place = n;
                 for (int x = 0; x < kWaves; x++) {
                     if (x < w) place += s_counts[x];
                     n += s_counts[x];
                 }
-                if (active) s_list[place + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)((t - t_begin) | (lo == hi && lo == one_doc && neg >= 0 ? 0x8000 : 0));
+                if (lane < PW && ((active >> lane) & 1)) s_list[place + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane - t_begin) | ((whole >> lane) & 1 ? 0x8000 : 0));
                 __syncthreads();
             }
             n_tiles = n;
@@ -143,16 +140,27 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
 
     const char *kb = p.k + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h, *vb = p.v + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h;
     const int key0 = tid / PPR, ch = tid % PPR;
+    const uint32_t lane_off = (uint32_t)key0 * (uint32_t)p.stride_t + ch * 16;
     u32x4 kpre[NL], vpre[NL];
     int id_pre = 0;   // documents: of this tile's token `lane`
     auto prefetch = [&](int n) {
-        const int k_lo = tile_lo(entry(n)), most = p.Sk - 1 - k_lo;   // (rows past the last key repeat it)
+        const int k_lo = tile_lo(entry(n)), most = p.Sk - 1 - k_lo;
         const char *tk = kb + (int64_t)k_lo * p.stride_t, *tv = vb + (int64_t)k_lo * p.stride_t;
+        if (most >= kTile - 1) {   // wave-uniform addresses and one offset per lane
+            uint32_t o = lane_off;
+            asm volatile("" : "+v"(o));   // (stays a 32-bit offset up to the loads)
 #pragma unroll
-        for (int j = 0; j < NL; j++) {
-            const uint32_t o = (uint32_t)min(key0 + j * RPI, most) * (uint32_t)p.stride_t + ch * 16;   // (rows of at most 2^25 bytes)
-            kpre[j] = *reinterpret_cast<const u32x4 *>(tk + o);
-            vpre[j] = *reinterpret_cast<const u32x4 *>(tv + o);
+            for (int j = 0; j < NL; j++) {
+                kpre[j] = *reinterpret_cast<const u32x4 *>(tk + (int64_t)(j * RPI) * p.stride_t + o);
+                vpre[j] = *reinterpret_cast<const u32x4 *>(tv + (int64_t)(j * RPI) * p.stride_t + o);
+            }
+        } else {   // rows past the last key repeat it
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const uint32_t o = (uint32_t)min(key0 + j * RPI, most) * (uint32_t)p.stride_t + ch * 16;   // (rows of at most 2^25 bytes)
+                kpre[j] = *reinterpret_cast<const u32x4 *>(tk + o);
+                vpre[j] = *reinterpret_cast<const u32x4 *>(tv + o);
+            }
         }
         if (DOCS) id_pre = docs[k_lo + min(lane, most)];
     };
