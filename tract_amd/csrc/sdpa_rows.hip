@@ -61,7 +61,7 @@ struct RowsDev {
     // shared prefix
     const char *pk, *pv;
     int64_t p_stride_h, p_stride_t;   // bytes
-    int P, p_items, p_splits, p_row_tiles, p_tiles;   // p_items: of this launch; p_tiles, own_tiles: key tiles of a range
+    int P, p_items, p_splits, p_row_tiles;   // p_items: of this launch
     // own keys: regular (one base, strides) or a table entry per sequence
     const char *k, *v;
     int64_t stride_b, stride_h, stride_t;
@@ -77,7 +77,7 @@ struct RowsDev {
     int64_t part_rows;
     int *counters;              // != NULL: the last workgroup of a unit joins its parts; else a launch after this one
     int splits;                 // p_splits + own_splits; 1: no partials, rows go to `out`
-    FastDiv by_g, by_sq, by_p_row_tiles, by_own_splits, by_own_row_tiles;
+    FastDiv by_g, by_sq, by_p_row_tiles, by_own_splits, by_own_row_tiles, by_own_tiles;   // own_tiles: key tiles of a part, about
 };
 
 struct RowsCall { RowsDev p; SeqTable tab; };
@@ -239,12 +239,14 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void put2(float *at, float2_t x) { __hip_atomic_store(reinterpret_cast<uint64_t *>(at), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float2_t get2(const float *at) { return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)); }
 
-// What a workgroup has to do: rows [row0, row_end) of a kv head over key tiles [t_begin, t_end) of one set of keys.
+// What a workgroup has to do: rows [row0, row_end) of a kv head over its share of the first `tiles` key tiles of one set of keys.  `parts`
+// workgroups share them; part `part` takes groups of `kWaves` tiles (a tall tile: tiles) in turn, so that the parts stream through
+// neighbouring memory together.
 struct RowsWork {
     const char *k, *v;
     int64_t st;              // bytes between tokens
     int kvh, b;              // b: whose own keys (-1: the prefix)
-    int row0, row_end, n_keys, t_begin, t_end, split;
+    int row0, row_end, n_keys, tiles, part, parts, split;   // split: where its partial rows go
 };
 
 // Where row r of a kv head lies among the q and output rows.
@@ -254,24 +256,35 @@ __device__ __forceinline__ RowPlace q_row(const RowsDev &p, int kvh, int r) {
     return {((int64_t)b * p.Hq + qh) * p.Sq + i, i, qh};
 }
 
-// Places of the key tiles [t_begin, t_end) that hold a token of a document in [dmin, dmax]; bit 15: all of the tile's tokens are of
+// Places of the first t_end key tiles that hold a token of a document in [dmin, dmax]; bit 15: all of the tile's tokens are of
 // document `one`, that of every row but padding (-1: they differ).  All threads; returns how many.  A wave looks at two
 // tiles at a time, a token per lane.
-__device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, int t_begin, int t_end, int dmin, int dmax, int one, uint16_t *list, int *counts) {
+__device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, int t_end, int dmin, int dmax, int one, uint16_t *list, int *counts) {
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     constexpr int PW = 32;   // tiles that a wave looks at before the waves compare
+    const int dlow = max(dmin, 0);
     int n = 0;
-    for (int t0 = t_begin; t0 < t_end; t0 += kWaves * PW) {
+    for (int t0 = 0; t0 < t_end; t0 += kWaves * PW) {
         const int first = t0 + w * PW;
+        const uint32_t there = first >= t_end ? 0 : first + PW <= t_end ? ~0u : (1u << (t_end - first)) - 1;
         uint32_t active = 0, whole = 0;
+#pragma unroll 1
+        for (int x0 = 0; x0 < PW; x0 += 16) {   // (eight loads in flight; more of them, or their masks at once, spill scalar registers)
+            int ids[8];
 #pragma unroll
-        for (int x = 0; x < PW; x += 2) {   // (all loads in flight at once)
-            const int j = (first + x) * kTile + lane;
-            const int id = first + x + (lane >> 5) < t_end ? docs[min(j, n_keys - 1)] : -1;
-            const uint64_t in = __builtin_amdgcn_ballot_w64(id >= dmin && id <= dmax && id >= 0), same = __builtin_amdgcn_ballot_w64(id == one && id >= 0);
-            active |= ((uint32_t)in != 0 ? 1u : 0u) << x | ((uint32_t)(in >> 32) != 0 ? 2u : 0u) << x;
-            whole |= ((uint32_t)same == ~0u ? 1u : 0u) << x | ((uint32_t)(same >> 32) == ~0u ? 2u : 0u) << x;
+            for (int x = 0; x < 8; x++) ids[x] = docs[min((first + x0 + 2 * x) * kTile + lane, n_keys - 1)];
+            uint32_t a16 = 0, w16 = 0;
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const uint64_t in = __builtin_amdgcn_ballot_w64(ids[x] >= dlow && ids[x] <= dmax), other = __builtin_amdgcn_ballot_w64(ids[x] != one);
+                a16 |= ((uint32_t)in != 0 ? 1u << 2 * x : 0) | ((uint32_t)(in >> 32) != 0 ? 2u << 2 * x : 0);
+                w16 |= ((uint32_t)other == 0 ? 1u << 2 * x : 0) | ((uint32_t)(other >> 32) == 0 ? 2u << 2 * x : 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            active |= a16 << x0, whole |= w16 << x0;
         }
+        if (one < 0) whole = 0;
+        active &= there;
         if (lane == 0) counts[w] = __popc(active);
         __syncthreads();
         int at = n;
@@ -279,7 +292,7 @@ __device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, 
             if (x < w) at += counts[x];
             n += counts[x];
         }
-        if (lane < PW && ((active >> lane) & 1)) list[at + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane - t_begin) | ((whole >> lane) & 1 ? 0x8000 : 0));
+        if (lane < PW && ((active >> lane) & 1)) list[at + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane) | ((whole >> lane) & 1 ? 0x8000 : 0));
         __syncthreads();
     }
     return n;
@@ -296,7 +309,8 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
     constexpr int NS = kTile / NG;                // scores of a lane
     constexpr int KROW = H16 ? D + 8 : D + 4;     // elements per K row in LDS: 128-bit reads of 16 rows hit 64 distinct banks
     constexpr int VROW = H16 ? D + 16 : R == 16 ? D + 4 : D + 8;   // (rows of a read in different banks)
-    constexpr int PRIV = kTile * (VROW + (R == 32 ? KROW : 0)) * (int)sizeof(T);   // a wave's tile
+    constexpr bool KL = R == 32 || H16;
+    constexpr int PRIV = kTile * (VROW + (KL ? KROW : 0)) * (int)sizeof(T);   // a wave's tile
     constexpr int CROW = D + 4;                   // floats per row where waves are joined
     constexpr int LPRW = D * (int)sizeof(T) / 16, RPI = 64 / LPRW, NI = kTile / RPI;   // lanes per key row, rows per load, loads per tile and tensor
     constexpr int KS = D * (int)sizeof(T) / (16 * NG);   // 16-byte pieces of a lane's share of a row
@@ -315,7 +329,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
     if (own && p.causal) lim = min(lim, SCORED && p.prefix_lens ? max(at, p.prefix_lens[wk.b] - 1) : at);
     float slope = 0.0f;
     const int *docs = nullptr;
-    int n_tiles = max(0, wk.t_end - wk.t_begin);
+    int n_tiles = wk.part < wk.parts ? wk.tiles : 0;   // of all parts; with documents those that are listed
     bool listed = false;
     if constexpr (SCORED) {
         if (p.slopes) slope = p.slopes[place.qh] * kLog2e;
@@ -327,13 +341,14 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
                 int dmin = doc >= 0 ? doc : INT_MAX, dmax = doc;
 #pragma unroll
                 for (int d = 1; d < R; d <<= 1) dmin = min(dmin, __shfl_xor(dmin, d, 64)), dmax = max(dmax, __shfl_xor(dmax, d, 64));
-                n_tiles = list_document_tiles(docs, n_keys, wk.t_begin, wk.t_end, dmin, dmax, dmin == dmax ? dmin : -1, s_list, s_counts);
+                n_tiles = list_document_tiles(docs, n_keys, n_tiles, dmin, dmax, dmin == dmax ? dmin : -1, s_list, s_counts);
                 listed = true;
             }
         }
     }
     float *part_ml = p.part_ml + (int64_t)wk.split * 2 * p.part_rows;
-    if (n_tiles == 0 && p.splits > 1) {   // nothing to add: a maximum of -inf says so
+    const int first = wk.part * kWaves, step = wk.parts * kWaves;
+    if (n_tiles <= first && p.splits > 1) {   // nothing to add: a maximum of -inf says so
         if (w == 0 && grp == 0 && wk.row0 + lr < wk.row_end) put(part_ml + out_row, -INFINITY);
         return;
     }
@@ -347,18 +362,18 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 
     T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: R == 32)
     const int kr = lane / LPRW, ch = lane % LPRW;
-    constexpr int NK = R == 16 ? 2 * KS : NI;
+    constexpr int NK = !KL ? 2 * KS : NI;
     u32x4 kpre[NK], vpre[NI];
     int id_pre = 0;   // lane%32's token's document
     auto tile_at = [&](int n) -> int {
-        if (SCORED && listed) return wk.t_begin + __builtin_amdgcn_readfirstlane(s_list[n] & 0x7fff);
-        return wk.t_begin + n;
+        if (SCORED && listed) return __builtin_amdgcn_readfirstlane(s_list[n] & 0x7fff);
+        return n;
     };
     // (rows past the last key repeat it; rows of at most 2^25 bytes)
     auto prefetch_k = [&](int n) __attribute__((always_inline)) {
         const int k_lo = tile_at(n) * kTile, most = n_keys - 1 - k_lo;
         const char *tk = wk.k + (int64_t)k_lo * wk.st;
-        if constexpr (R == 16) {
+        if constexpr (!KL) {
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
                 const uint32_t off = (uint32_t)min(16 * kb + lr, most) * (uint32_t)wk.st + grp * 16;
@@ -381,11 +396,11 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
     // key of score x of this lane, from the tile's first: groups of four consecutive ones
     auto key_of = [](int x) { return R == 16 ? 16 * (x >> 2) + (x & 3) : 8 * (x >> 2) + (x & 3); };   // + 4 grp
 
-    if (w < n_tiles) prefetch_k(w), prefetch_v(w);
+    if (first + w < n_tiles) prefetch_k(first + w), prefetch_v(first + w);
     u32x4 qf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qf[ks] = load16(p.q + out_row * (D * (int)sizeof(T)), ks * 16 * NG + grp * 16);
-    for (int n = w; n < n_tiles; n += kWaves) {
+    for (int n = first + w; n < n_tiles; n += step) {
         const int k_lo = tile_at(n) * kTile;
         const bool by_id = SCORED && docs && !(listed && __builtin_amdgcn_readfirstlane(s_list[n] & 0x8000));
         const int id_tile = id_pre;
@@ -393,7 +408,32 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 
         // ---- S^T = K Q^T --------------------------------------------------------------------------------------
         float s[NS];
-        if constexpr (R == 16) {
+        if constexpr (R == 16 && KL) {
+#pragma unroll
+            for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_k + (j * RPI + kr) * KROW + ch * (16 / (int)sizeof(T))) = kpre[j];
+            if (n + step < n_tiles) prefetch_k(n + step);
+            wave_sync();
+            float4_t acc[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[kb][r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4 *>(lds_k + (16 * kb + lr) * KROW + (ks * 64 + grp * 16) / (int)sizeof(T));
+                    if constexpr (H16) {
+                        acc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kf), __builtin_bit_cast(half8_t, qf[ks]), acc[kb], 0, 0, 0);
+                    } else {
+                        const float4_t a = __builtin_bit_cast(float4_t, kf), c = __builtin_bit_cast(float4_t, qf[ks]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[kb], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+            for (int x = 0; x < NS; x++) s[x] = acc[x >> 2][x & 3];
+        } else if constexpr (R == 16) {
             float4_t acc[2];
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
@@ -413,11 +453,11 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
                 }
 #pragma unroll
             for (int x = 0; x < NS; x++) s[x] = acc[x >> 2][x & 3];
-            if (n + kWaves < n_tiles) prefetch_k(n + kWaves);
+            if (n + step < n_tiles) prefetch_k(n + step);
         } else {
 #pragma unroll
             for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_k + (j * RPI + kr) * KROW + ch * (16 / (int)sizeof(T))) = kpre[j];
-            if (n + kWaves < n_tiles) prefetch_k(n + kWaves);
+            if (n + step < n_tiles) prefetch_k(n + step);
             wave_sync();
             float16_t acc;
 #pragma unroll
@@ -441,7 +481,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
             if (by_id && ((padding >> (j * RPI)) >> kr & 1)) vpre[j] = u32x4{0, 0, 0, 0};   // padding may hold anything
             *reinterpret_cast<u32x4 *>(lds_v + (j * RPI + kr) * VROW + ch * (16 / (int)sizeof(T))) = vpre[j];
         }
-        if (n + kWaves < n_tiles) prefetch_v(n + kWaves);
+        if (n + step < n_tiles) prefetch_v(n + step);
 
         // ---- softmax of this lane's row over its keys k_lo + 4 grp + key_of(x) -----------------------------------
         if constexpr (SCORED) __builtin_amdgcn_sched_barrier(0);   // (V's fragments asked for during the scores' arithmetic spill registers)
@@ -592,8 +632,8 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 }
 
 // A tile of 128 f16 rows over a prefix: a tile of 64 keys is staged once for the four waves, 32 rows each (as sdpa_scored.hip has
-// it).  Tiles of [t_begin, t_end) count 64 keys.  Always a part: `splits` > 1.
-constexpr int kTallTile = 64, kTallRows = 128;
+// it).  Tiles count 64 keys.  Always a part: `splits` > 1.
+constexpr int kTallTile = 64;
 template <int D>
 __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, unsigned char *lds) {
     constexpr int KS = D / 16, DB = D / 32, KROW = D + 8, VROW = D + 16;
@@ -601,14 +641,14 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
     constexpr int K_TILE = kTallTile * KROW, V_TILE = kTallTile * VROW;
     _Float16 *lds_k = reinterpret_cast<_Float16 *>(lds), *lds_v = lds_k + 2 * K_TILE;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
-    const int my_row = wk.row0 + 32 * w + l32, n_tiles = wk.t_end - wk.t_begin;
+    const int my_row = wk.row0 + 32 * w + l32, n_tiles = (wk.tiles - wk.part + wk.parts - 1) / wk.parts;
     const bool wave_has_rows = wk.row0 + 32 * w < wk.row_end;
     const int64_t out_row = q_row(p, wk.kvh, min(my_row, wk.row_end - 1)).at;
     const int key0 = tid / PPR, ch = tid % PPR;
     const uint32_t lane_off = (uint32_t)key0 * (uint32_t)wk.st + ch * 16;
     u32x4 kpre[NL], vpre[NL];
     auto prefetch = [&](int n) __attribute__((always_inline)) {
-        const int k_lo = (wk.t_begin + n) * kTallTile, most = wk.n_keys - 1 - k_lo;
+        const int k_lo = (wk.part + n * wk.parts) * kTallTile, most = wk.n_keys - 1 - k_lo;
         const char *tk = wk.k + (int64_t)k_lo * wk.st, *tv = wk.v + (int64_t)k_lo * wk.st;
         if (most >= kTallTile - 1) {   // wave-uniform addresses and one offset per lane
             uint32_t o = lane_off;
@@ -665,7 +705,7 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
                 for (int kb = 0; kb < 2; kb++)
                     s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8_t *>(ksrc + 32 * kb * KROW + 16 * ks), __builtin_bit_cast(half8_t, qf[ks]), s[kb], 0, 0, 0);
             // this lane's keys: 4 hb + c, c = 32 kb + 8 (x / 4) + x % 4
-            const int last = wk.n_keys - 1 - (wk.t_begin + n) * kTallTile - 4 * hb;
+            const int last = wk.n_keys - 1 - (wk.part + n * wk.parts) * kTallTile - 4 * hb;
             if (last < 60) {
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
@@ -828,7 +868,8 @@ __device__ __forceinline__ void arrive(const RowsDev &p, const RowsWork &wk, uin
         if (tid < n) {
             int r0, r1;
             rows_of(first + tid, r0, r1);
-            const int parts = p.own_row_tiles ? p.own_splits + (PRE ? p.p_splits * ((r1 - 1) / (PRE ? PRE : 1) - r0 / (PRE ? PRE : 1) + 1) : 0) : p.p_splits;
+            int parts = p.p_splits;
+            if (p.own_row_tiles) parts = p.own_splits + (PRE ? parts * ((r1 - 1) / (PRE ? PRE : 1) - r0 / (PRE ? PRE : 1) + 1) : 0);
             int *counter = p.counters + (int64_t)wk.kvh * n_units + first + tid;
             last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
             if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -848,7 +889,7 @@ __device__ __forceinline__ void arrive(const RowsDev &p, const RowsWork &wk, uin
 }
 
 constexpr int rows_lds(int es, int D, int R) {   // rows_body's LDS
-    return kWaves * kTile * ((es == 2 ? D + 16 : R == 16 ? D + 4 : D + 8) + (R == 32 ? (es == 2 ? D + 8 : D + 4) : 0)) * es;
+    return kWaves * kTile * ((es == 2 ? D + 16 : R == 16 ? D + 4 : D + 8) + (R == 32 || es == 2 ? (es == 2 ? D + 8 : D + 4) : 0)) * es;
 }
 constexpr int tall_lds(int D) { return 2 * kTallTile * (2 * D + 24) * 2; }
 constexpr int most_of(int a, int b) { return a > b ? a : b; }
@@ -863,6 +904,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
     __shared__ int s_counts[kWaves];
     __shared__ uint32_t s_done;
     int item = blockIdx.y;
+    bool there = false;   // the work is done
     RowsWork wk;
     wk.kvh = blockIdx.x;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
     if (PRE && item < p.p_items) {
@@ -872,14 +914,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
         wk.row0 = (item - wk.split * p.p_row_tiles) * ROWS, wk.row_end = min(wk.row0 + ROWS, p.B * p.Sq * p.G);
         wk.k = p.pk + (int64_t)wk.kvh * p.p_stride_h, wk.v = p.pv + (int64_t)wk.kvh * p.p_stride_h, wk.st = p.p_stride_t;
         wk.n_keys = p.P;
-        wk.t_begin = wk.split * p.p_tiles, wk.t_end = min((p.P + TILE - 1) / TILE, wk.t_begin + p.p_tiles);
+        wk.tiles = (p.P + TILE - 1) / TILE, wk.part = wk.split, wk.parts = p.p_splits;
         if constexpr (PRE == 128) {
             tall_body<D>(p, wk, lds);
             return;
         } else if constexpr (PRE != 0 && PRE != OWN) {
             rows_body<T, D, PRE, false>(p, wk, lds, nullptr, nullptr);
-            if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
-            return;
+            there = true;
         }
     } else {
         if (PRE) item -= p.p_items;
@@ -895,10 +936,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
             if (SCORED && p.prefix_lens) n_vis = max(n_vis, p.prefix_lens[wk.b]);
             n_vis = max(0, min(n_vis, own.len));
         }
-        wk.t_begin = split * p.own_tiles, wk.t_end = min((n_vis + kTile - 1) / kTile, wk.t_begin + p.own_tiles);
+        wk.tiles = (n_vis + kTile - 1) / kTile, wk.part = split, wk.parts = min(p.own_splits, max(1, p.by_own_tiles.by(wk.tiles + p.own_tiles - 1)));
         wk.split = p.p_splits + split;
     }
-    rows_body<T, D, OWN, SCORED>(p, wk, lds, s_list, s_counts);
+    if (!there) rows_body<T, D, OWN, SCORED>(p, wk, lds, s_list, s_counts);
     if constexpr (PRE != 128)
         if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
 }
@@ -1001,15 +1042,34 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
 
 template <typename T, int D>
 int launch_tiles_of(const SdpaRowsArgs &a, RowsCall &call, int pre, int own, bool is_scored, hipStream_t s) {
-    if (is_scored) return own == 16 ? launch_tiles<T, D, 0, 16, true>(a, call, s) : launch_tiles<T, D, 0, 32, true>(a, call, s);
-    if (own == 32) {
-        if constexpr (sizeof(T) == 2)
-            if (pre == 128) return launch_tiles<T, D, 128, 32, false>(a, call, s);
-        return launch_tiles<T, D, 32, 32, false>(a, call, s);
-    }
+    if constexpr (sizeof(T) == 2 || D == 128)
+        if (own == 32 && is_scored) return launch_tiles<T, D, 0, 32, true>(a, call, s);
+    if (is_scored) return launch_tiles<T, D, 0, 16, true>(a, call, s);
     if constexpr (sizeof(T) == 2)
-        if (pre == 128) return launch_tiles<T, D, 128, 16, false>(a, call, s);
-    return pre == 32 ? launch_tiles<T, D, 32, 16, false>(a, call, s) : launch_tiles<T, D, 16, 16, false>(a, call, s);
+        if (pre == 128) return own == 32 ? launch_tiles<T, D, 128, 32, false>(a, call, s) : launch_tiles<T, D, 128, 16, false>(a, call, s);
+    if constexpr (sizeof(T) == 2 || D == 128)
+        if (own == 32) return launch_tiles<T, D, 32, 32, false>(a, call, s);
+    if constexpr (sizeof(T) == 2)
+        if (pre == 32) return launch_tiles<T, D, 32, 16, false>(a, call, s);
+    return launch_tiles<T, D, 16, 16, false>(a, call, s);
+}
+
+// Sequences of one length: how many of its `all` key tiles a part of each unit of rows takes.  A workgroup's round of a tile per wave takes
+// `full` us where `target` workgroups share the memory's rate, and no less than `least` where fewer do; no more of them than that, or
+// another turn of all (f16, us, by parts: 4 x 8193 keys x 8 kv heads 1: 109, 2: 61, 4: 37.1, 6: 29.1, 8: 29.5, 16: 30.6; one sequence
+// 8: 18.0, 16: 13.7, 32: 14.7; eight 2: 64.0, 3: 50.3, 4: 51.1, 5: 59.2, 8: 52.3).
+int64_t tiles_of_a_part(int64_t units, int64_t all, int64_t es, int64_t D) {
+    const double kb = (double)(kTile * D * es * 2) / 1024, cus = num_compute_units();
+    const double target = kb < 16 ? 2 * cus : cus, least = es == 4 ? 4.7 * (D == 128 ? 1.0 : 0.55) : 1.85, full = kb < 16 ? 3.05 : 3.05 * kb / 16;
+    int64_t best_n = 1;
+    double best = 1e30;
+    for (int64_t n = 1; n <= 64 && n <= (all + kWaves - 1) / kWaves; n++) {
+        const double wgs = (double)(units * n), turns = (double)(int64_t)((wgs + target - 1) / target), share = full * (wgs < target ? wgs / target : 1.0);
+        const double rounds = (double)((all + kWaves * n - 1) / (kWaves * n));
+        const double t = turns * (2.5 + rounds * (share > least ? share : least)) + (n > 1 ? 1.0 + 0.25 * (double)n : 0.0);
+        if (t < best) best = t, best_n = n;
+    }
+    return (all + best_n - 1) / best_n;
 }
 
 // Rounds of a workgroup with `per` tiles of `all`.
@@ -1038,10 +1098,10 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     if (!ok || (a.P == 0 && longest == 0)) return 2;
 
     const bool is_scored = a.softcap > 0.0f || a.slopes || a.documents || a.prefix_lens;
-    const int own = seq_rows <= 16 ? 16 : 32;
+    const int own = seq_rows <= 16 || (es == 4 && a.D == 64) ? 16 : 32;
     const int64_t room = a.workspace && aligned(a.workspace) && a.workspace_bytes > kWsCounterBytes + kWsPlanBytes + 256
                              ? (int64_t)(a.workspace_bytes - kWsCounterBytes - kWsPlanBytes - 256) / ((a.D + 2) * (int64_t)sizeof(float)) / rows_all : 0;
-    const int pre = a.P == 0 ? own : es == 2 && rows > 64 && a.P > kTallTile && room >= 2 && a.scale > 0.0f ? 128 : rows > 16 ? 32 : own;   // (the tall body stores parts only)
+    const int pre = a.P == 0 || es == 4 ? own : rows > 64 && a.P > kTallTile && room >= 2 && a.scale > 0.0f ? 128 : rows > 16 ? 32 : own;   // (the tall body stores parts only)
     RowsCall call;
     RowsDev &p = call.p;
     fill_rows(a, p);
@@ -1062,7 +1122,7 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     for (int64_t op = kWaves;; op = op * 2 > own_all ? (own_all + kWaves - 1) / kWaves * kWaves : op * 2) {
         int64_t own_wgs = 0;
         if (a.lens || a.seqs)
-            for (int64_t b = 0; b < a.B; b++) own_wgs += ((a.lens ? a.lens[b] : a.seqs[b].len) + op * kTile - 1) / (op * kTile);
+            for (int64_t b = 0; b < a.B; b++) own_wgs += (uint32_t)((uint32_t)((a.lens ? a.lens[b] : a.seqs[b].len) + kTile - 1) / kTile + (uint32_t)op - 1) / (uint32_t)op;
         else own_wgs = a.B * ((own_all + op - 1) / op);
         own_wgs *= a.Hkv * p.own_row_tiles;
         const int64_t own_n = (own_all + op - 1) / op;
@@ -1079,16 +1139,19 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
         }
         if (op >= own_all) break;
     }
+    // (Several tiles of rows per sequence are enough workgroups, of unlike lengths.)
+    if (!a.lens && !a.seqs && p.own_row_tiles == 1) o_per = tiles_of_a_part(a.Hkv * a.B, own_all, es, a.D);
+    if (!a.lens && !a.seqs && p.own_row_tiles > 1 && a.documents) o_per = own_all;   // (how much of its keys a row's document has is not known here)
     if (pre == 128 && longest == 0 && p_per > (p_all + 1) / 2) p_per = (p_all + 1) / 2;
     for (;; p_per *= 2, o_per *= 2) {
-        p.p_tiles = (int)p_per, p.own_tiles = (int)o_per;
+        p.own_tiles = (int)o_per;
         p.p_splits = (int)((p_all + p_per - 1) / p_per), p.own_splits = (int)((own_all + o_per - 1) / o_per);
         p.splits = p.p_splits + p.own_splits;
         if (p.splits == 1 || (p.splits <= room && p.splits <= 64)) break;
         if (p.p_splits <= 1 && p.own_splits <= 1) return 2;   // (no room to join prefix and own keys in)
     }
     p.by_g = fast_div(G), p.by_sq = fast_div(a.Sq), p.by_p_row_tiles = fast_div(p.p_row_tiles);
-    p.by_own_splits = fast_div(p.own_splits), p.by_own_row_tiles = fast_div(p.own_row_tiles);
+    p.by_own_splits = fast_div(p.own_splits), p.by_own_row_tiles = fast_div(p.own_row_tiles), p.by_own_tiles = fast_div(p.own_tiles);
     p.part_o = (float *)((char *)a.workspace + kWsCounterBytes + kWsPlanBytes);
     p.part_ml = p.part_o + (int64_t)p.splits * p.part_rows * a.D;
     if (p.splits == 1) p.part_o = p.part_ml = nullptr;

@@ -35,13 +35,11 @@ struct ScoredDev {
     _Float16 *out;
     const char *k, *v;
     int64_t stride_b, stride_h, stride_t;   // bytes
-    int B, Hq, Hkv, Sq, G, Sk, row_tiles, splits, tiles;   // tiles: of a range of keys
+    int B, Hq, Hkv, Sq, G, Sk, row_tiles;
     float scale, cap;
     int causal;
     const float *slopes;
     const int *docs, *prefix_lens;
-    float *part_o, *part_ml;   // as in sdpa_rows.hip
-    int64_t part_rows;
 };
 
 __device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *lds_ptr) {   // (see sdpa_rows.hip)
@@ -66,12 +64,10 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     int id = blockIdx.x;
     const int kvh = id % p.Hkv;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
     id /= p.Hkv;
-    const int split = id % p.splits;
-    id /= p.splits;
     const int b = id % p.B, rt = p.row_tiles - 1 - id / p.B;   // (the longest first)
     const int seq_rows = p.Sq * p.G, row0 = rt * kRows, off = p.Sk - p.Sq;
 
-    const int my_row = row0 + 32 * w + l32, r = min(my_row, seq_rows - 1), i = r / p.G, g = r - i * p.G;
+    const int r = min(row0 + 32 * w + l32, seq_rows - 1), i = r / p.G, g = r - i * p.G;
     const int64_t out_row = ((int64_t)b * p.Hq + kvh * p.G + g) * p.Sq + i;
     const int at = i + off;
     int lim = p.Sk - 1, n_vis = p.Sk;
@@ -82,8 +78,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     }
     const int wave_lim = __builtin_amdgcn_readfirstlane(p.causal ? max((min(row0 + 32 * w + 32, seq_rows) - 1) / p.G + off, p.prefix_lens ? p.prefix_lens[b] - 1 : -1) : p.Sk - 1);
     const bool wave_has_rows = row0 + 32 * w < seq_rows;
-    const int t_begin = split * p.tiles, t_end = min((n_vis + kTile - 1) / kTile, t_begin + p.tiles);
-    int n_tiles = max(0, t_end - t_begin);
+    const int t_end = (n_vis + kTile - 1) / kTile;
+    int n_tiles = t_end;
 
     const float slope = SLOPES ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
     const int *docs = DOCS ? p.docs + (int64_t)b * p.Sk : nullptr;
@@ -102,19 +98,28 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
             dmin = INT_MAX, dmax = -1;
 #pragma unroll
             for (int x = 0; x < kWaves; x++) dmin = min(dmin, s_range[0][x]), dmax = max(dmax, s_range[1][x]);
-            const int one_doc = dmin == dmax ? dmin : -1;
+            const int one_doc = dmin == dmax ? dmin : INT_MIN, dlow = max(dmin, 0);   // (no tile is whole of what is no document)
             // A wave looks at a tile at a time, a token per lane, at 16 of them before the waves compare.
             constexpr int PW = 16;
             int n = 0;
-            for (int t0 = t_begin; t0 < t_end; t0 += kWaves * PW) {
+            for (int t0 = 0; t0 < t_end; t0 += kWaves * PW) {
                 const int first = t0 + w * PW;
+                const uint32_t there = first >= t_end ? 0 : (1u << min(PW, t_end - first)) - 1;
                 uint32_t active = 0, whole = 0;
+#pragma unroll 1
+                for (int x0 = 0; x0 < PW; x0 += 8) {   // (eight loads in flight; more of them, or their masks at once, spill scalar registers)
+                    int ids[8];
 #pragma unroll
-                for (int x = 0; x < PW; x++) {   // (all loads in flight at once)
-                    const int id = first + x < t_end ? docs[min((first + x) * kTile + lane, p.Sk - 1)] : -1;
-                    active |= (__builtin_amdgcn_ballot_w64(id >= dmin && id <= dmax && id >= 0) != 0 ? 1u : 0u) << x;
-                    whole |= (__builtin_amdgcn_ballot_w64(id == one_doc && id >= 0) == ~0ull ? 1u : 0u) << x;
+                    for (int x = 0; x < 8; x++) ids[x] = docs[min((first + x0 + x) * kTile + lane, p.Sk - 1)];
+                    uint32_t a8 = 0, w8 = 0;
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        a8 |= __builtin_amdgcn_ballot_w64(ids[x] >= dlow && ids[x] <= dmax) != 0 ? 1u << x : 0;
+                        w8 |= __builtin_amdgcn_ballot_w64(ids[x] != one_doc) == 0 ? 1u << x : 0;
+                    }
+                    active |= a8 << x0, whole |= w8 << x0;
                 }
+                active &= there;
                 if (lane == 0) s_counts[w] = __popc(active);
                 __syncthreads();
                 int place = n;
@@ -122,21 +127,15 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
                     if (x < w) place += s_counts[x];
                     n += s_counts[x];
                 }
-                if (lane < PW && ((active >> lane) & 1)) s_list[place + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane - t_begin) | ((whole >> lane) & 1 ? 0x8000 : 0));
+                if (lane < PW && ((active >> lane) & 1)) s_list[place + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane) | (one_doc >= 0 && ((whole >> lane) & 1) ? 0x8000 : 0));
                 __syncthreads();
             }
             n_tiles = n;
             listed = true;
         }
     }
-    float *part_ml = p.part_ml + (int64_t)split * 2 * p.part_rows;
-    if (n_tiles == 0 && p.splits > 1) {   // nothing to add: a maximum of -inf says so
-        if (hb == 0 && my_row < seq_rows) part_ml[out_row] = -INFINITY;
-        return;
-    }
-
     auto entry = [&](int n) -> int { return DOCS && listed ? __builtin_amdgcn_readfirstlane(s_list[n]) : n; };
-    auto tile_lo = [&](int e) -> int { return (t_begin + (DOCS ? e & 0x7fff : e)) * kTile; };
+    auto tile_lo = [&](int e) -> int { return (DOCS ? e & 0x7fff : e) * kTile; };
 
     const char *kb = p.k + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h, *vb = p.v + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h;
     const int key0 = tid / PPR, ch = tid % PPR;
@@ -305,17 +304,6 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     }
     l_run += __shfl_xor(l_run, 32, 64);
 
-    if (p.splits > 1) {
-        if (my_row < seq_rows) {
-            float *po = p.part_o + ((int64_t)split * p.part_rows + out_row) * D + 4 * hb;
-#pragma unroll
-            for (int db = 0; db < DB; db++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) *reinterpret_cast<float4_t *>(po + 32 * db + 8 * x) = float4_t{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
-            part_ml[out_row + (hb ? p.part_rows : 0)] = hb ? l_run : m_run;
-        }
-        return;
-    }
     // rows to their places in whole lines, through the idle V buffers
     __syncthreads();
     if (!wave_has_rows) return;
@@ -375,10 +363,8 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     p.q = (const char *)a.q, p.out = (_Float16 *)a.out, p.k = (const char *)a.k, p.v = (const char *)a.v;
     p.stride_b = a.stride_b * 2, p.stride_h = a.stride_h * 2, p.stride_t = a.stride_t * 2;
     p.B = (int)a.B, p.Hq = (int)a.Hq, p.Hkv = (int)a.Hkv, p.Sq = (int)a.Sq, p.G = (int)G, p.Sk = (int)a.Sk, p.row_tiles = (int)row_tiles;
-    p.splits = 1, p.tiles = (int)((a.Sk + kTile - 1) / kTile);
     p.scale = a.scale, p.cap = a.softcap, p.causal = a.causal;
     p.slopes = a.slopes, p.docs = a.documents, p.prefix_lens = a.prefix_lens;
-    p.part_rows = a.B * a.Hq * a.Sq;
     if (a.D == 64) launch_of<64>(p, grid, s);
     else launch_of<128>(p, grid, s);
     hipError_t e = hipGetLastError();

@@ -10,6 +10,7 @@
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -17,6 +18,7 @@ from ._lib import TractRocmError, call
 from .ops import _as_device, _canon4, _check_norm_weights, _code, _cos_sin_batch, _same, _scale_arg, _strides4, _I64x3
 from .runtime import DeviceTensor, Workspace, _sh
 
+_PI64 = C.c_int64 * 1   # (where a row of lengths begins)
 _I32 = np.dtype(np.int32)
 _F32 = np.dtype(np.float32)
 
@@ -38,6 +40,7 @@ class QkNormRope:
 
     def __init__(self, eps: float = 1e-6):
         self.eps = float(eps)
+        self._key = self._sizes = None
 
     def name(self) -> str:
         return "QkNormRope"
@@ -55,18 +58,25 @@ class QkNormRope:
             q, k, cos, sin = (_as_device(t, stream) for t in (q, k, cos, sin))
             q_weight, k_weight = (None if w is None else _as_device(w, stream) for w in (q_weight, k_weight))
         dtype, shape, k_shape = q.dtype, q.shape, k.shape
-        for t in (k, q_weight, k_weight, cos, sin):
-            if t is not None and not _same(t.dtype, dtype):
-                raise TractRocmError("Q, K, weights, cos and sin must share a datum type")
-        if len(shape) != 4 or len(k_shape) != 4 or k_shape[0] != shape[0] or k_shape[2:] != shape[2:]:
-            raise TractRocmError(f"Q {shape} and K {k_shape} must be [batch, heads, n, head_dim] and differ in heads only")
-        b, hq, n, d = shape
-        cb = _cos_sin_batch(cos, sin, b, n, d)
-        _check_norm_weights(q_weight, k_weight, d)
-        q_out, k_out = _output(q_out, shape, dtype), _output(k_out, k_shape, dtype)
-        call("trocm_qk_norm_rope", q.ptr, k.ptr, _optr(q_weight), _optr(k_weight), self.eps, cos.ptr, sin.ptr, 0 if cb == 1 else n * d,
-             _code(dtype), b, hq, k_shape[1], n, d, _strides4(q_strides), _strides4(k_strides), q_out.ptr, k_out.ptr,
-             None if stream is None else _sh(stream))
+        # (A decode step's call takes the device 3.4 us: shapes and types are looked into where they are not the last call's.)
+        key = (shape, k_shape, cos.shape, sin.shape, q_strides, k_strides, dtype, k.dtype, cos.dtype, sin.dtype,
+               q_weight is None or (q_weight.shape, q_weight.dtype), k_weight is None or (k_weight.shape, k_weight.dtype))
+        if key != self._key:
+            for t in (k, q_weight, k_weight, cos, sin):
+                if t is not None and not _same(t.dtype, dtype):
+                    raise TractRocmError("Q, K, weights, cos and sin must share a datum type")
+            if len(shape) != 4 or len(k_shape) != 4 or k_shape[0] != shape[0] or k_shape[2:] != shape[2:]:
+                raise TractRocmError(f"Q {shape} and K {k_shape} must be [batch, heads, n, head_dim] and differ in heads only")
+            b, hq, n, d = shape
+            cb = _cos_sin_batch(cos, sin, b, n, d)
+            _check_norm_weights(q_weight, k_weight, d)
+            self._key, self._sizes = key, (0 if cb == 1 else n * d, _code(dtype), b, hq, k_shape[1], n, d, _strides4(q_strides), _strides4(k_strides))
+        if q_out is None or q_out.shape != shape or q_out.dtype is not dtype:
+            q_out = _output(q_out, shape, dtype)
+        if k_out is None or k_out.shape != k_shape or k_out.dtype is not dtype:
+            k_out = _output(k_out, k_shape, dtype)
+        call("trocm_qk_norm_rope", q.ptr, k.ptr, None if q_weight is None else q_weight.ptr, None if k_weight is None else k_weight.ptr, self.eps,
+             cos.ptr, sin.ptr, *self._sizes, q_out.ptr, k_out.ptr, None if stream is None else _sh(stream))
         return q_out, k_out
 
 
@@ -75,7 +85,7 @@ class SharedPrefixSdpa:
 
     def __init__(self, scale=None, is_causal: bool = True):
         self.scale, self.is_causal = scale, bool(is_causal)
-        self._ws = None
+        self._ws = self._key = self._sizes = None
 
     def _workspace(self, n, hq, sq, d, stream):
         need = Workspace.shared_bytes_for(n, hq, sq, d)
@@ -86,25 +96,36 @@ class SharedPrefixSdpa:
     def eval(self, q, prefix_k, prefix_v, k, v, lens, stream=None, out=None, prefix_len=None) -> DeviceTensor:
         """Q [n_seq, q_heads, q_len, head_dim]; prefix K and V [1, kv_heads, room, head_dim] of which `prefix_len` tokens (None:
         all) count; K and V [n_seq, kv_heads, room, head_dim] of which sequence i's first lens[i] tokens count."""
-        q, prefix_k, prefix_v, k, v = (_as_device(t, stream) for t in (q, prefix_k, prefix_v, k, v))
-        dtype = q.dtype
-        for t in (prefix_k, prefix_v, k, v):
-            if not _same(t.dtype, dtype):
-                raise TractRocmError("Q, K and V must share a datum type")
-        if len(q.shape) != 4 or len(k.shape) != 4 or len(prefix_k.shape) != 4 or k.shape != v.shape or prefix_k.shape != prefix_v.shape:
-            raise TractRocmError("shared prefix: inputs must be of rank 4, K and V of one shape")
-        n, hq, sq, d = q.shape
-        _, hkv, room, _ = k.shape
-        p = prefix_k.shape[2] if prefix_len is None else int(prefix_len)
-        if k.shape != (n, hkv, room, d) or prefix_k.shape != (1, hkv, prefix_k.shape[2], d) or not 0 <= p <= prefix_k.shape[2]:
-            raise TractRocmError(f"shared prefix: Q {q.shape}, prefix {prefix_k.shape} and K {k.shape} do not match")
-        if len(lens) != n or (n and not 0 <= min(lens) <= max(lens) <= room):
+        if not isinstance(q, DeviceTensor):
+            q, prefix_k, prefix_v, k, v = (_as_device(t, stream) for t in (q, prefix_k, prefix_v, k, v))
+        dtype, shape = q.dtype, q.shape
+        key = (shape, k.shape, v.shape, prefix_k.shape, prefix_v.shape, prefix_len, dtype, k.dtype, v.dtype, prefix_k.dtype, prefix_v.dtype)
+        if key != self._key:   # (the last call's need no second look)
+            for t in (prefix_k, prefix_v, k, v):
+                if not _same(t.dtype, dtype):
+                    raise TractRocmError("Q, K and V must share a datum type")
+            if len(shape) != 4 or len(k.shape) != 4 or len(prefix_k.shape) != 4 or k.shape != v.shape or prefix_k.shape != prefix_v.shape:
+                raise TractRocmError("shared prefix: inputs must be of rank 4, K and V of one shape")
+            n, hq, sq, d = shape
+            _, hkv, room, _ = k.shape
+            p_room = prefix_k.shape[2]
+            p = p_room if prefix_len is None else int(prefix_len)
+            if k.shape != (n, hkv, room, d) or prefix_k.shape != (1, hkv, p_room, d) or not 0 <= p <= p_room:
+                raise TractRocmError(f"shared prefix: Q {shape}, prefix {prefix_k.shape} and K {k.shape} do not match")
+            self._key = key
+            self._sizes = (_code(dtype), n, hq, hkv, sq, d), p, (C.c_int64 * 2)(p_room * d, d), _I64x3(hkv * room * d, room * d, d)
+            self._workspace(n, hq, sq, d, stream)
+        sizes, p, prefix_strides, strides = self._sizes
+        n, room = shape[0], k.shape[2]
+        lens = array("q", lens)
+        if len(lens) != n or (n and max(lens) > room):   # (negative ones are refused below)
             raise TractRocmError(f"shared prefix: lens must be {n} lengths of 0..={room}")
-        out = _output(out, q.shape, dtype)
-        ws = self._workspace(n, hq, sq, d, stream)
-        call("trocm_sdpa_shared_prefix", q.ptr, _code(dtype), n, hq, hkv, sq, d, prefix_k.ptr, prefix_v.ptr, p,
-             (C.c_int64 * 2)(prefix_k.shape[2] * d, d), k.ptr, v.ptr, _I64x3(hkv * room * d, room * d, d), (C.c_int64 * n)(*lens), out.ptr,
-             _scale_arg(self.scale), int(self.is_causal), ws.buf.ptr, ws.nbytes, None if stream is None else _sh(stream))
+        if out is None or out.shape != shape or out.dtype is not dtype:
+            out = _output(out, shape, dtype)
+        ws = self._ws
+        call("trocm_sdpa_shared_prefix", q.ptr, *sizes, prefix_k.ptr, prefix_v.ptr, p, prefix_strides, k.ptr, v.ptr, strides,
+             _PI64.from_buffer(lens) if n else _I64x3(0, 0, 0), out.ptr, _scale_arg(self.scale), int(self.is_causal), ws.buf.ptr, ws.nbytes,
+             None if stream is None else _sh(stream))
         return out
 
 
@@ -142,7 +163,7 @@ class ScoredSdpa:
 
     def __init__(self, scale=None, softcap: float = 0.0, is_causal: bool = True):
         self.scale, self.softcap, self.is_causal = scale, float(softcap), bool(is_causal)
-        self._ws = self._ws_key = None
+        self._ws = self._ws_key = self._key = self._sizes = None
 
     def name(self) -> str:
         return "ScoredSdpa"
@@ -165,18 +186,27 @@ class ScoredSdpa:
 
     def eval(self, q, k, v, slopes=None, documents=None, prefix_lens=None, stream=None, out=None) -> DeviceTensor:
         """Q, K, V of rank 3 or 4; slopes f32 [q_heads], documents int32 [batch, kv_len], prefix_lens int32 [batch]."""
-        q, k, v = (_as_device(t, stream) for t in (q, k, v))
-        if not (_same(k.dtype, q.dtype) and _same(v.dtype, q.dtype)):
-            raise TractRocmError("Q, K and V must share a datum type")
-        b, hq, sq, d = _canon4(q.shape)
-        _, hkv, sk, _ = _canon4(k.shape)
-        if _canon4(k.shape) != (b, hkv, sk, d) or k.shape != v.shape:
-            raise TractRocmError("K/V shape mismatch")
-        slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, sk, stream)
-        out = _output(out, q.shape, q.dtype)
+        if not isinstance(q, DeviceTensor):
+            q, k, v = (_as_device(t, stream) for t in (q, k, v))
+        dtype, shape = q.dtype, q.shape
+        key = (shape, k.shape, v.shape, dtype, k.dtype, v.dtype)
+        if key != self._key:   # (the last call's need no second look)
+            if not (_same(k.dtype, dtype) and _same(v.dtype, dtype)):
+                raise TractRocmError("Q, K and V must share a datum type")
+            b, hq, sq, d = _canon4(shape)
+            _, hkv, sk, _ = _canon4(k.shape)
+            if _canon4(k.shape) != (b, hkv, sk, d) or k.shape != v.shape:
+                raise TractRocmError("K/V shape mismatch")
+            self._key, self._sizes = key, (_code(dtype), b, hq, hkv, sq, sk, d)
+        sizes = self._sizes
+        _, b, hq, _, sq, sk, d = sizes
+        if slopes is not None or documents is not None or prefix_lens is not None:
+            slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, sk, stream)
+        if out is None or out.shape != shape or out.dtype is not dtype:
+            out = _output(out, shape, dtype)
         ws = self._workspace(b, hq, sq, d, stream)
-        call("trocm_sdpa_scored", q.ptr, k.ptr, v.ptr, out.ptr, _code(q.dtype), b, hq, hkv, sq, sk, d, None, _scale_arg(self.scale), self.softcap,
-             _optr(slopes), _optr(documents), _optr(prefix_lens), int(self.is_causal), ws.buf.ptr, ws.nbytes, None if stream is None else _sh(stream))
+        call("trocm_sdpa_scored", q.ptr, k.ptr, v.ptr, out.ptr, *sizes, None, _scale_arg(self.scale), self.softcap, _optr(slopes), _optr(documents),
+             _optr(prefix_lens), int(self.is_causal), ws.buf.ptr, ws.nbytes, None if stream is None else _sh(stream))
         return out
 
     def eval_cached(self, q: DeviceTensor, k_cache, v_cache, slopes=None, documents=None, prefix_lens=None, stream=None, out=None) -> DeviceTensor:
