@@ -357,7 +357,16 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     if (!aligned(a.q) || !aligned(a.out) || !aligned(a.k) || !aligned(a.v) || a.stride_b % 8 || a.stride_h % 8 || a.stride_t % 8 || a.stride_t * 2 > (1 << 25)) return 2;
     if (rows >= (1 << 30)) return 2;
     const int64_t row_tiles = (rows + kRows - 1) / kRows, grid = a.B * a.Hkv * row_tiles;
-    if (rows <= 32 || grid < num_compute_units() / 2 || grid >= (1ll << 31)) return 2;
+    if (rows <= 32 || grid >= (1ll << 31)) return 2;
+    // Few workgroups, or few tiles for each, go faster as tiles of 32 rows whose four waves share the keys (sdpa_rows.hip), which take
+    // about 1.5 times as long per product.  What either takes, in us: a start, then the longest workgroup's tiles of 64 keys, or all
+    // tiles over the chip.  (Capped, 32 heads over 8, D = 128, here | there: 300 queries 10.3 | 10.3; 500 18.7 | 12.8; 1000 32.6 | 31.9;
+    // 2048 64.6 | 86.1; 4096 191 | 295; 500 behind 3000 96.7 | 61.6.  D = 64, 64 heads: 300 10.3 | 8.6; 1000 26.9 | 31.4; 4096 235 | 355.)
+    const double cus = num_compute_units(), wide = a.D == 128 ? 1.0 : 0.62, last = (double)((a.Sk + kTile - 1) / kTile);
+    const double first = a.causal && !a.prefix_lens ? (double)((a.Sk - a.Sq > 0 ? a.Sk - a.Sq : 0) / kTile + 1) : last;
+    const double all = (double)grid * (first + last) / 2 / cus, tall = 4 + (last * 1.8 > all * 1.44 ? last * 1.8 : all * 1.44) * wide;
+    const double flat = 4 + (last * 1.0 > all * 2.3 ? last * 1.0 : all * 2.3) * wide;
+    if (flat < tall) return 2;
     ScoredDev p;
     memset(&p, 0, sizeof(p));
     p.q = (const char *)a.q, p.out = (_Float16 *)a.out, p.k = (const char *)a.k, p.v = (const char *)a.v;
