@@ -14,6 +14,7 @@
 #include <limits.h>
 #include <string.h>
 #include "common.h"
+#include "fast_div.h"
 
 namespace trocm {
 namespace {
@@ -36,6 +37,7 @@ struct ScoredDev {
     const char *k, *v;
     int64_t stride_b, stride_h, stride_t;   // bytes
     int B, Hq, Hkv, Sq, G, Sk, row_tiles;
+    FastDiv by_g;
     float scale, cap;
     int causal;
     const float *slopes;
@@ -61,28 +63,55 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     __shared__ __attribute__((aligned(16))) int s_ids[2][DOCS ? kTile : 4];   // documents of the staged tiles' tokens
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
-    int id = blockIdx.x;
-    const int kvh = id % p.Hkv;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
-    id /= p.Hkv;
-    const int b = id % p.B, rt = p.row_tiles - 1 - id / p.B;   // (the longest first)
+    const int kvh = blockIdx.x;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
+    const int b = blockIdx.y, rt = p.row_tiles - 1 - (int)blockIdx.z;   // (the longest first)
     const int seq_rows = p.Sq * p.G, row0 = rt * kRows, off = p.Sk - p.Sq;
 
-    const int r = min(row0 + 32 * w + l32, seq_rows - 1), i = r / p.G, g = r - i * p.G;
+    const int r = min(row0 + 32 * w + l32, seq_rows - 1), i = p.by_g.by(r), g = r - i * p.G;
     const int64_t out_row = ((int64_t)b * p.Hq + kvh * p.G + g) * p.Sq + i;
     const int at = i + off;
     int lim = p.Sk - 1, n_vis = p.Sk;
     if (p.causal) {
         const int pre = p.prefix_lens ? p.prefix_lens[b] : 0;
         lim = min(lim, max(at, pre - 1));
-        n_vis = max(0, min(p.Sk, max((min(row0 + kRows, seq_rows) - 1) / p.G + off + 1, pre)));
+        n_vis = max(0, min(p.Sk, max(p.by_g.by(min(row0 + kRows, seq_rows) - 1) + off + 1, pre)));
     }
-    const int wave_lim = __builtin_amdgcn_readfirstlane(p.causal ? max((min(row0 + 32 * w + 32, seq_rows) - 1) / p.G + off, p.prefix_lens ? p.prefix_lens[b] - 1 : -1) : p.Sk - 1);
+    const int wave_lim = __builtin_amdgcn_readfirstlane(p.causal ? max(p.by_g.by(min(row0 + 32 * w + 32, seq_rows) - 1) + off, p.prefix_lens ? p.prefix_lens[b] - 1 : -1) : p.Sk - 1);
     const bool wave_has_rows = row0 + 32 * w < seq_rows;
     const int t_end = (n_vis + kTile - 1) / kTile;
     int n_tiles = t_end;
 
-    const float slope = SLOPES ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
+    const char *kb = p.k + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h, *vb = p.v + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h;
+    const int key0 = tid / PPR, ch = tid % PPR;
+    const uint32_t lane_off = (uint32_t)key0 * (uint32_t)p.stride_t + ch * 16;
     const int *docs = DOCS ? p.docs + (int64_t)b * p.Sk : nullptr;
+    u32x4 kpre[NL], vpre[NL];
+    int id_pre = 0;   // documents: of this tile's token `lane`
+    auto prefetch = [&](int k_lo) {
+        const int most = p.Sk - 1 - k_lo;
+        const char *tk = kb + (int64_t)k_lo * p.stride_t, *tv = vb + (int64_t)k_lo * p.stride_t;
+        if (most >= kTile - 1) {   // wave-uniform addresses and one offset per lane
+            uint32_t o = lane_off;
+            asm volatile("" : "+v"(o));   // (stays a 32-bit offset up to the loads)
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                kpre[j] = *reinterpret_cast<const u32x4 *>(tk + (int64_t)(j * RPI) * p.stride_t + o);
+                vpre[j] = *reinterpret_cast<const u32x4 *>(tv + (int64_t)(j * RPI) * p.stride_t + o);
+            }
+        } else {   // rows past the last key repeat it
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const uint32_t o = (uint32_t)min(key0 + j * RPI, most) * (uint32_t)p.stride_t + ch * 16;   // (rows of at most 2^25 bytes)
+                kpre[j] = *reinterpret_cast<const u32x4 *>(tk + o);
+                vpre[j] = *reinterpret_cast<const u32x4 *>(tv + o);
+            }
+        }
+        if (DOCS) id_pre = docs[k_lo + min(lane, most)];
+    };
+    // The last tile first, that of the rows' own tokens: it is asked for before anything is known of the documents.
+    if (n_tiles > 0) prefetch((t_end - 1) * kTile);
+
+    const float slope = SLOPES ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
     const int doc = DOCS ? docs[at] : 0;
     if (DOCS && doc < 0) lim = -1;   // padding sees nothing
     bool listed = false;
@@ -134,35 +163,9 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
             listed = true;
         }
     }
-    auto entry = [&](int n) -> int { return DOCS && listed ? __builtin_amdgcn_readfirstlane(s_list[n]) : n; };
-    auto tile_lo = [&](int e) -> int { return (DOCS ? e & 0x7fff : e) * kTile; };
+    auto entry = [&](int n) -> int { return DOCS && listed ? __builtin_amdgcn_readfirstlane(s_list[n_tiles - 1 - n]) : n_tiles - 1 - n; };
+    auto tile_lo = [&](int e) -> int { return (DOCS && listed ? e & 0x7fff : e) * kTile; };
 
-    const char *kb = p.k + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h, *vb = p.v + (int64_t)b * p.stride_b + (int64_t)kvh * p.stride_h;
-    const int key0 = tid / PPR, ch = tid % PPR;
-    const uint32_t lane_off = (uint32_t)key0 * (uint32_t)p.stride_t + ch * 16;
-    u32x4 kpre[NL], vpre[NL];
-    int id_pre = 0;   // documents: of this tile's token `lane`
-    auto prefetch = [&](int n) {
-        const int k_lo = tile_lo(entry(n)), most = p.Sk - 1 - k_lo;
-        const char *tk = kb + (int64_t)k_lo * p.stride_t, *tv = vb + (int64_t)k_lo * p.stride_t;
-        if (most >= kTile - 1) {   // wave-uniform addresses and one offset per lane
-            uint32_t o = lane_off;
-            asm volatile("" : "+v"(o));   // (stays a 32-bit offset up to the loads)
-#pragma unroll
-            for (int j = 0; j < NL; j++) {
-                kpre[j] = *reinterpret_cast<const u32x4 *>(tk + (int64_t)(j * RPI) * p.stride_t + o);
-                vpre[j] = *reinterpret_cast<const u32x4 *>(tv + (int64_t)(j * RPI) * p.stride_t + o);
-            }
-        } else {   // rows past the last key repeat it
-#pragma unroll
-            for (int j = 0; j < NL; j++) {
-                const uint32_t o = (uint32_t)min(key0 + j * RPI, most) * (uint32_t)p.stride_t + ch * 16;   // (rows of at most 2^25 bytes)
-                kpre[j] = *reinterpret_cast<const u32x4 *>(tk + o);
-                vpre[j] = *reinterpret_cast<const u32x4 *>(tv + o);
-            }
-        }
-        if (DOCS) id_pre = docs[k_lo + min(lane, most)];
-    };
     auto stage = [&](int buf) {
         if (DOCS) {
             if (tid < kTile) s_ids[buf][tid] = id_pre;
@@ -190,14 +193,14 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     const float to_log2 = p.scale * kLog2e, cap_a = p.cap * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
 
     half8_t qf[KS];
-    if (n_tiles > 0) prefetch(0);
+    if (DOCS && n_tiles > 0 && tile_lo(entry(0)) != (t_end - 1) * kTile) prefetch(tile_lo(entry(0)));   // (padding, or a prefix)
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qf[ks] = *reinterpret_cast<const half8_t *>(p.q + out_row * (2 * D) + 32 * ks + 16 * hb);
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));   // settled here, not by a wait in the loop that would take the prefetch in too
     if (n_tiles > 0) {
         stage(0);
-        if (n_tiles > 1) prefetch(1);
+        if (n_tiles > 1) prefetch(tile_lo(entry(1)));
     }
     for (int n = 0; n < n_tiles; n++) {
         __syncthreads();   // tile n is in LDS; every wave is done with the buffers about to be overwritten
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
         }
         if (n + 1 < n_tiles) {   // the next tile to LDS after this one's arithmetic, which covers its loads' latency
             stage(buf ^ 1);
-            if (n + 2 < n_tiles) prefetch(n + 2);
+            if (n + 2 < n_tiles) prefetch(tile_lo(entry(n + 2)));
         }
     }
     l_run += __shfl_xor(l_run, 32, 64);
@@ -324,16 +327,16 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     constexpr int LPR = D / 8, RPS = 64 / LPR;
 #pragma unroll
     for (int j = 0; j < 32 / RPS; j++) {
-        const int row = j * RPS + lane / LPR, rr = row0 + 32 * w + row, ii = rr / p.G, gg = rr - ii * p.G;
+        const int row = j * RPS + lane / LPR, rr = row0 + 32 * w + row, ii = p.by_g.by(rr), gg = rr - ii * p.G;
         if (rr < seq_rows)
             *reinterpret_cast<u32x4 *>(p.out + (((int64_t)b * p.Hq + kvh * p.G + gg) * p.Sq + ii) * D + lane % LPR * 8) = *reinterpret_cast<const u32x4 *>(tr + row * OROW + lane % LPR * 8);
     }
 }
 
 template <int D>
-void launch_of(const ScoredDev &p, int64_t grid, hipStream_t s) {
+void launch_of(const ScoredDev &p, hipStream_t s) {
     const bool cap = p.cap > 0.0f, slopes = p.slopes != nullptr, docs = p.docs != nullptr;
-    const dim3 g((unsigned)grid), t(kThreads);
+    const dim3 g((unsigned)p.Hkv, (unsigned)p.B, (unsigned)p.row_tiles), t(kThreads);
     if (docs) {
         if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, true, true>), g, t, 0, s, p);
         else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, false, true>), g, t, 0, s, p);
@@ -357,7 +360,7 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     if (!aligned(a.q) || !aligned(a.out) || !aligned(a.k) || !aligned(a.v) || a.stride_b % 8 || a.stride_h % 8 || a.stride_t % 8 || a.stride_t * 2 > (1 << 25)) return 2;
     if (rows >= (1 << 30)) return 2;
     const int64_t row_tiles = (rows + kRows - 1) / kRows, grid = a.B * a.Hkv * row_tiles;
-    if (rows <= 32 || grid >= (1ll << 31)) return 2;
+    if (rows <= 32 || a.B > 65535 || row_tiles > 65535) return 2;
     // Few workgroups, or few tiles for each, go faster as tiles of 32 rows whose four waves share the keys (sdpa_rows.hip), which take
     // about 1.5 times as long per product.  What either takes, in us: a start, then the longest workgroup's tiles of 64 keys, or all
     // tiles over the chip.  (Capped, 32 heads over 8, D = 128, here | there: 300 queries 10.3 | 10.3; 500 18.7 | 12.8; 1000 32.6 | 31.9;
@@ -371,11 +374,11 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     memset(&p, 0, sizeof(p));
     p.q = (const char *)a.q, p.out = (_Float16 *)a.out, p.k = (const char *)a.k, p.v = (const char *)a.v;
     p.stride_b = a.stride_b * 2, p.stride_h = a.stride_h * 2, p.stride_t = a.stride_t * 2;
-    p.B = (int)a.B, p.Hq = (int)a.Hq, p.Hkv = (int)a.Hkv, p.Sq = (int)a.Sq, p.G = (int)G, p.Sk = (int)a.Sk, p.row_tiles = (int)row_tiles;
+    p.B = (int)a.B, p.Hq = (int)a.Hq, p.Hkv = (int)a.Hkv, p.Sq = (int)a.Sq, p.G = (int)G, p.Sk = (int)a.Sk, p.row_tiles = (int)row_tiles, p.by_g = fast_div(G);
     p.scale = a.scale, p.cap = a.softcap, p.causal = a.causal;
     p.slopes = a.slopes, p.docs = a.documents, p.prefix_lens = a.prefix_lens;
-    if (a.D == 64) launch_of<64>(p, grid, s);
-    else launch_of<128>(p, grid, s);
+    if (a.D == 64) launch_of<64>(p, s);
+    else launch_of<128>(p, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail("sdpa_scored launch failed: %s", hipGetErrorString(e));
     return 0;
