@@ -60,6 +60,14 @@ def test_longer(rt, dtype, b, hq, hkv, n, t, d):
     _check(dtype, b, hq, hkv, n, t, d, cap=20.0, prefix_lens=np.array([t // 3] * b, np.int32))
 
 
+@pytest.mark.parametrize("b,hq,hkv,n,t,d", [(1, 32, 8, 1000, 1000, 128), (3, 28, 4, 1000, 1040, 64), (1, 64, 8, 777, 800, 64)])
+def test_enough_rows_for_every_compute_unit(rt, b, hq, hkv, n, t, d):
+    """128 rows per workgroup, its tiles taken by one group of waves or by two in turn."""
+    rng = np.random.default_rng(15)
+    _check(F16, b, hq, hkv, n, t, d, cap=30.0)
+    _check(F16, b, hq, hkv, n, t, d, cap=20.0, slopes=_slopes(hq), documents=_packed(rng, b, t, 5), prefix_lens=np.full(b, t // 4, np.int32))
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("n", [1, 9, 150])
 def test_not_causal_and_scales(rt, dtype, n):

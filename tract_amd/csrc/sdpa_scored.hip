@@ -5,7 +5,8 @@
 // The rows of a kv head are (query, head of the group), heads fastest, so that a workgroup of 4 waves x 32 rows covers few
 // queries and its causal frontier is short.  S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs: every softmax scalar of a row
 // sits in one lane.  A tile of 64 keys is staged into LDS once for the four waves, double buffered, its loads issued two
-// tiles ahead: one barrier per tile.  Two workgroups (head size 64: three) share a compute unit without knowing of each
+// tiles ahead: one barrier per tile.  Two groups of four waves may take a workgroup's tiles in turn (NK == 2) and join their rows
+// at the end.  Two workgroups (head size 64: three) share a compute unit without knowing of each
 // other, so that one's softmax runs beside the other's MFMAs.
 //
 // What bounds it: the vector ALU.  Per score the cap costs two quarter-rate instructions (exp2, rcp) beside the softmax's own
@@ -28,7 +29,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kTile = 64, kRows = 32 * kWaves;
+constexpr int kWaves = 4, kTile = 64, kRows = 32 * kWaves;   // waves with rows of their own, of each of NK groups
 constexpr int kListMax = 4096;   // key tiles that documents are looked up for
 
 struct ScoredDev {
@@ -50,21 +51,25 @@ __device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *lds_ptr) {   //
     return __builtin_bit_cast(half4_t, r);
 }
 
-template <int D, bool CAP, bool SLOPES, bool DOCS>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel(ScoredDev p) {
+template <int D, int NK, bool CAP, bool SLOPES, bool DOCS>
+__global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_scored_kernel(ScoredDev p) {
     constexpr int KS = D / 16, DB = D / 32;
     constexpr int KROW = D + 8, VROW = D + 16;        // halves per row in LDS (bank spread of the two kinds of reads)
-    constexpr int PPR = D / 8, RPI = kThreads / PPR, NL = kTile / RPI;   // 16-byte pieces per row, rows per load of the workgroup, loads per tile and tensor
-    constexpr int K_TILE = kTile * KROW, V_TILE = kTile * VROW, OROW = D + 8;
+    constexpr int kThreads = 64 * kWaves;             // of a group
+    constexpr int PPR = D / 8, RPI = kThreads / PPR, NL = kTile / RPI;   // 16-byte pieces per row, rows per load of a group, loads per tile and tensor
+    constexpr int K_TILE = kTile * KROW, V_TILE = kTile * VROW, OROW = D + 8, JROW = D + 4;
     static_assert(kWaves * 32 * OROW <= 2 * V_TILE, "the output goes through the V buffers");
-    __shared__ __attribute__((aligned(16))) _Float16 lds_k[2][K_TILE], lds_v[2][V_TILE];
+    __shared__ __attribute__((aligned(16))) _Float16 lds_all[NK][2 * K_TILE + 2 * V_TILE];
     __shared__ uint16_t s_list[DOCS ? kListMax : 1];
-    __shared__ int s_counts[kWaves], s_range[2][kWaves];
-    __shared__ __attribute__((aligned(16))) int s_ids[2][DOCS ? kTile : 4];   // documents of the staged tiles' tokens
+    __shared__ int s_counts[NK * kWaves], s_range[2][kWaves];
+    __shared__ __attribute__((aligned(16))) int s_ids_all[NK][2][DOCS ? kTile : 4];   // documents of the staged tiles' tokens
 
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / kWaves, w = wave % kWaves;   // group, wave of it
+    const int tid = threadIdx.x % kThreads, lane = tid & 63, hb = lane >> 5, l32 = lane & 31;
     const int kvh = blockIdx.x;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
     const int b = blockIdx.y, rt = p.row_tiles - 1 - (int)blockIdx.z;   // (the longest first)
+    _Float16 (*lds_k)[K_TILE] = reinterpret_cast<_Float16 (*)[K_TILE]>(&lds_all[kg][0]), (*lds_v)[V_TILE] = reinterpret_cast<_Float16 (*)[V_TILE]>(&lds_all[kg][2 * K_TILE]);
+    int (*s_ids)[DOCS ? kTile : 4] = s_ids_all[kg];
     const int seq_rows = p.Sq * p.G, row0 = rt * kRows, off = p.Sk - p.Sq;
 
     const int r = min(row0 + 32 * w + l32, seq_rows - 1), i = p.by_g.by(r), g = r - i * p.G;
@@ -109,7 +114,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
         if (DOCS) id_pre = docs[k_lo + min(lane, most)];
     };
     // The last tile first, that of the rows' own tokens: it is asked for before anything is known of the documents.
-    if (n_tiles > 0) prefetch((t_end - 1) * kTile);
+    const int guess = t_end - 1 - kg;
+    if (guess >= 0) prefetch(guess * kTile);
 
     const float slope = SLOPES ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
     const int doc = DOCS ? docs[at] : 0;
@@ -122,7 +128,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
             int dmin = doc >= 0 ? doc : INT_MAX, dmax = doc;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) dmin = min(dmin, __shfl_xor(dmin, d, 64)), dmax = max(dmax, __shfl_xor(dmax, d, 64));
-            if (lane == 0) s_range[0][w] = dmin, s_range[1][w] = dmax;
+            if (kg == 0 && lane == 0) s_range[0][w] = dmin, s_range[1][w] = dmax;
             __syncthreads();
             dmin = INT_MAX, dmax = -1;
 #pragma unroll
@@ -131,8 +137,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
             // A wave looks at a tile at a time, a token per lane, at 16 of them before the waves compare.
             constexpr int PW = 16;
             int n = 0;
-            for (int t0 = 0; t0 < t_end; t0 += kWaves * PW) {
-                const int first = t0 + w * PW;
+            for (int t0 = 0; t0 < t_end; t0 += NK * kWaves * PW) {
+                const int first = t0 + wave * PW;
                 const uint32_t there = first >= t_end ? 0 : (1u << min(PW, t_end - first)) - 1;
                 uint32_t active = 0, whole = 0;
 #pragma unroll 1
@@ -149,11 +155,11 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
                     active |= a8 << x0, whole |= w8 << x0;
                 }
                 active &= there;
-                if (lane == 0) s_counts[w] = __popc(active);
+                if (lane == 0) s_counts[wave] = __popc(active);
                 __syncthreads();
                 int place = n;
-                for (int x = 0; x < kWaves; x++) {
-                    if (x < w) place += s_counts[x];
+                for (int x = 0; x < NK * kWaves; x++) {
+                    if (x < wave) place += s_counts[x];
                     n += s_counts[x];
                 }
                 if (lane < PW && ((active >> lane) & 1)) s_list[place + __popc(active & ((1u << lane) - 1))] = (uint16_t)((first + lane) | (one_doc >= 0 && ((whole >> lane) & 1) ? 0x8000 : 0));
@@ -193,19 +199,19 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     const float to_log2 = p.scale * kLog2e, cap_a = p.cap * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
 
     half8_t qf[KS];
-    if (DOCS && n_tiles > 0 && tile_lo(entry(0)) != (t_end - 1) * kTile) prefetch(tile_lo(entry(0)));   // (padding, or a prefix)
+    if (DOCS && kg < n_tiles && tile_lo(entry(kg)) != guess * kTile) prefetch(tile_lo(entry(kg)));   // (padding, or a prefix)
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qf[ks] = *reinterpret_cast<const half8_t *>(p.q + out_row * (2 * D) + 32 * ks + 16 * hb);
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));   // settled here, not by a wait in the loop that would take the prefetch in too
-    if (n_tiles > 0) {
+    if (kg < n_tiles) {
         stage(0);
-        if (n_tiles > 1) prefetch(tile_lo(entry(1)));
+        if (kg + NK < n_tiles) prefetch(tile_lo(entry(kg + NK)));
     }
-    for (int n = 0; n < n_tiles; n++) {
+    for (int n = kg, it = 0; n - kg < n_tiles; n += NK, it++) {   // (as many rounds for every group)
         __syncthreads();   // tile n is in LDS; every wave is done with the buffers about to be overwritten
-        const int buf = n & 1, e = entry(n), k_lo = tile_lo(e);
-        if (wave_has_rows && k_lo <= wave_lim) {
+        const int buf = it & 1, e = NK == 1 || n < n_tiles ? entry(n) : 0, k_lo = tile_lo(e);
+        if (wave_has_rows && (NK == 1 || n < n_tiles) && k_lo <= wave_lim) {
             float16_t s[2];
 #pragma unroll
             for (int kb2 = 0; kb2 < 2; kb2++)
@@ -300,18 +306,48 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
                     o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[st], o[db], 0, 0, 0);
                 }
         }
-        if (n + 1 < n_tiles) {   // the next tile to LDS after this one's arithmetic, which covers its loads' latency
+        if (n + NK < n_tiles) {   // the next tile to LDS after this one's arithmetic, which covers its loads' latency
             stage(buf ^ 1);
-            if (n + 2 < n_tiles) prefetch(tile_lo(entry(n + 2)));
+            if (n + 2 * NK < n_tiles) prefetch(tile_lo(entry(n + 2 * NK)));
         }
     }
     l_run += __shfl_xor(l_run, 32, 64);
 
-    // rows to their places in whole lines, through the idle V buffers
-    __syncthreads();
+    if constexpr (NK == 2) {   // the second group's rows join the first's, through the tiles' LDS
+        float *comb = reinterpret_cast<float *>(&lds_all[0][0]) + w * 32 * JROW, *comb_ml = reinterpret_cast<float *>(&lds_all[0][0]) + kWaves * 32 * JROW + w * 64;
+        static_assert(kWaves * (32 * JROW + 64) * 4 <= (int)sizeof(lds_all), "rows are joined where the tiles were");
+        __syncthreads();
+        if (kg == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    *reinterpret_cast<float4_t *>(comb + l32 * JROW + 32 * db + 8 * x + 4 * hb) = float4_t{o[db][4 * x], o[db][4 * x + 1], o[db][4 * x + 2], o[db][4 * x + 3]};
+            comb_ml[lane] = hb ? l_run : m_run;
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m2 = comb_ml[l32], l2 = comb_ml[32 + l32], mm = fmaxf(m_run, m2), ref = mm == -INFINITY ? 0.0f : mm;
+        const float f1 = __builtin_amdgcn_exp2f(m_run - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+        l_run = l_run * f1 + l2 * f2;
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float4_t v = *reinterpret_cast<const float4_t *>(comb + l32 * JROW + 32 * db + 8 * x + 4 * hb);
+#pragma unroll
+                for (int y = 0; y < 4; y++) o[db][4 * x + y] = o[db][4 * x + y] * f1 + v[y] * f2;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (a wave's corner is its own)
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    } else {
+        __syncthreads();
+    }
+    // rows to their places in whole lines, through a corner of LDS of the wave's own
     if (!wave_has_rows) return;
     const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-    _Float16 *tr = &lds_v[0][0] + w * 32 * OROW;
+    _Float16 *tr = NK == 2 ? reinterpret_cast<_Float16 *>(reinterpret_cast<float *>(&lds_all[0][0]) + w * 32 * JROW) : &lds_v[0][0] + w * 32 * OROW;
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
@@ -333,20 +369,20 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void sdpa_scored_kernel
     }
 }
 
-template <int D>
+template <int D, int NK>
 void launch_of(const ScoredDev &p, hipStream_t s) {
     const bool cap = p.cap > 0.0f, slopes = p.slopes != nullptr, docs = p.docs != nullptr;
-    const dim3 g((unsigned)p.Hkv, (unsigned)p.B, (unsigned)p.row_tiles), t(kThreads);
+    const dim3 g((unsigned)p.Hkv, (unsigned)p.B, (unsigned)p.row_tiles), t(64 * kWaves * NK);
     if (docs) {
-        if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, true, true>), g, t, 0, s, p);
-        else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, false, true>), g, t, 0, s, p);
-        else if (slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, false, true, true>), g, t, 0, s, p);
-        else hipLaunchKernelGGL((sdpa_scored_kernel<D, false, false, true>), g, t, 0, s, p);
+        if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, true, true, true>), g, t, 0, s, p);
+        else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, true, false, true>), g, t, 0, s, p);
+        else if (slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, false, true, true>), g, t, 0, s, p);
+        else hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, false, false, true>), g, t, 0, s, p);
     } else {
-        if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, true, false>), g, t, 0, s, p);
-        else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, true, false, false>), g, t, 0, s, p);
-        else if (slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, false, true, false>), g, t, 0, s, p);
-        else hipLaunchKernelGGL((sdpa_scored_kernel<D, false, false, false>), g, t, 0, s, p);
+        if (cap && slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, true, true, false>), g, t, 0, s, p);
+        else if (cap) hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, true, false, false>), g, t, 0, s, p);
+        else if (slopes) hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, false, true, false>), g, t, 0, s, p);
+        else hipLaunchKernelGGL((sdpa_scored_kernel<D, NK, false, false, false>), g, t, 0, s, p);
     }
 }
 
@@ -361,14 +397,18 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     if (rows >= (1 << 30)) return 2;
     const int64_t row_tiles = (rows + kRows - 1) / kRows, grid = a.B * a.Hkv * row_tiles;
     if (rows <= 32 || a.B > 65535 || row_tiles > 65535) return 2;
-    // Few workgroups, or few tiles for each, go faster as tiles of 32 rows whose four waves share the keys (sdpa_rows.hip), which take
-    // about 1.5 times as long per product.  What either takes, in us: a start, then the longest workgroup's tiles of 64 keys, or all
-    // tiles over the chip.  (Capped, 32 heads over 8, D = 128, here | there: 300 queries 10.3 | 10.3; 500 18.7 | 12.8; 1000 32.6 | 31.9;
-    // 2048 64.6 | 86.1; 4096 191 | 295; 500 behind 3000 96.7 | 61.6.  D = 64, 64 heads: 300 10.3 | 8.6; 1000 26.9 | 31.4; 4096 235 | 355.)
+    // Up to two workgroups per compute unit (one, where documents leave them unlike work) take their tiles in two groups of waves.
+    // Fewer tiles still go faster as tiles of 32 rows whose four waves share the keys (sdpa_rows.hip), which take about 1.5 times as long
+    // per product but are four times as many.  What either takes, in us: a start, then the longest workgroup's tiles of 64 keys, or all
+    // tiles over the chip.  (Capped, 32 heads over 8, D = 128, one group | two | there: 300 queries 12.9 | 12.8 | 10.1; 500 18.4 | 16.9 |
+    // 12.5; 1000 32.7 | 28.0 | 31.4; 2048 65.3 | 58.2 | 86.1; 4096 194 | 200 | 295; 500 behind 3000 97.5 | 75.6 | 61.6.  D = 64, 64 heads:
+    // 300 10.2 | 9.6 | 8.4; 1000 26.9 | 25.2 | 30.6; 4096 234 | 288 | 355.)
+    const int nk = grid <= (int64_t)num_compute_units() * (a.documents ? 1 : 2) ? 2 : 1;
     const double cus = num_compute_units(), wide = a.D == 128 ? 1.0 : 0.62, last = (double)((a.Sk + kTile - 1) / kTile);
     const double first = a.causal && !a.prefix_lens ? (double)((a.Sk - a.Sq > 0 ? a.Sk - a.Sq : 0) / kTile + 1) : last;
-    const double all = (double)grid * (first + last) / 2 / cus, tall = 4 + (last * 1.8 > all * 1.44 ? last * 1.8 : all * 1.44) * wide;
-    const double flat = 4 + (last * 1.0 > all * 2.3 ? last * 1.0 : all * 2.3) * wide;
+    const double all = (double)grid * (first + last) / 2 / cus, longest = nk == 2 ? (double)(int64_t)((last + 1) / 2) * 2.75 : last * 1.8;
+    const double tall = 4.0 + (longest > all * 1.44 ? longest : all * 1.44) * wide, each = all * 2.25 + (last - first) * 0.5;
+    const double flat = 4.0 + (last > each ? last : each) * wide;
     if (flat < tall) return 2;
     ScoredDev p;
     memset(&p, 0, sizeof(p));
@@ -377,8 +417,8 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     p.B = (int)a.B, p.Hq = (int)a.Hq, p.Hkv = (int)a.Hkv, p.Sq = (int)a.Sq, p.G = (int)G, p.Sk = (int)a.Sk, p.row_tiles = (int)row_tiles, p.by_g = fast_div(G);
     p.scale = a.scale, p.cap = a.softcap, p.causal = a.causal;
     p.slopes = a.slopes, p.docs = a.documents, p.prefix_lens = a.prefix_lens;
-    if (a.D == 64) launch_of<64>(p, s);
-    else launch_of<128>(p, s);
+    if (a.D == 64) nk == 2 ? launch_of<64, 2>(p, s) : launch_of<64, 1>(p, s);
+    else nk == 2 ? launch_of<128, 2>(p, s) : launch_of<128, 1>(p, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail("sdpa_scored launch failed: %s", hipGetErrorString(e));
     return 0;
