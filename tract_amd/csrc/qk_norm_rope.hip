@@ -3,7 +3,8 @@
 // in f32 from the first square to the last sum, rounded once to the tensor's type.  (ApplyRope on its own rounds every
 // product, as the CPU op does; here nothing stands between the norm and the rotation that a graph could observe.)
 //
-// HBM-bound: a row is read and written once.  A lane holds VW consecutive pairs (i, i + D/2) as two 16-byte pieces, so a
+// HBM-bound: a row is read and written once (2 x 4096 tokens of 32 + 8 heads of 128 features in f16: 36.3 us, of which a plain copy of
+// as many bytes takes 33; a token of a decoding step, 5 us, is the launch's latency).  A lane holds VW consecutive pairs (i, i + D/2) as two 16-byte pieces, so a
 // row takes D / (2 VW) lanes, whose squares are summed by shuffles; rows of the same token that a lane takes one after
 // the other (HPC heads) share its cos and sin pieces, which would otherwise cost as many load instructions as the rows.
 #include <hip/hip_fp16.h>
@@ -14,6 +15,10 @@ namespace trocm {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Rows of which at least this much is read and written go past the caches (non-temporal loads and stores): 168 MB of
+// f16 at 128 features 36.3 us (4.75 TB/s) against 41.1 through them, 82 MB 20.1 against 20.2, 61 MB 15.2 against 12.5, 20 MB 7.0 against 6.0.
+constexpr int64_t kStreamBytes = 80ll << 20;
 
 struct NormRope {
     const void *x[2];        // q, k
@@ -32,7 +37,20 @@ struct NormRope {
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(_Float16 x) { return (float)x; }
 
-template <typename T, int LPR, int HPC>
+template <bool STREAM, typename P>
+__device__ __forceinline__ P load16(const void *a) {
+    if (!STREAM) return *reinterpret_cast<const P *>(a);
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(a));
+    return __builtin_bit_cast(P, v);
+}
+
+template <bool STREAM, typename P>
+__device__ __forceinline__ void store16(void *a, const P &v) {
+    if (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4 *>(a));
+    else *reinterpret_cast<P *>(a) = v;
+}
+
+template <typename T, int LPR, int HPC, bool STREAM>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRope p) {
     constexpr int VW = 16 / sizeof(T), HALF = LPR * VW, D = 2 * HALF;
     struct alignas(16) Piece { T e[VW]; };
@@ -49,8 +67,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRope p) {
 #pragma unroll
     for (int j = 0; j < HPC; j++) {
         const T *row = x + (int64_t)min(h0 + j, H - 1) * p.xs[which][1];
-        a[j] = *reinterpret_cast<const Piece *>(row);
-        c[j] = *reinterpret_cast<const Piece *>(row + HALF);
+        a[j] = load16<STREAM, Piece>(row);
+        c[j] = load16<STREAM, Piece>(row + HALF);
     }
     const int64_t cs = b * p.cs_stride_b + t * D + i;
     const T *cos = reinterpret_cast<const T *>(p.cos) + cs, *sin = reinterpret_cast<const T *>(p.sin) + cs;
@@ -86,8 +104,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRope p) {
         }
         if (live && h0 + j < H) {
             T *row = y + (int64_t)(h0 + j) * p.n * D;
-            *reinterpret_cast<Piece *>(row) = lo;
-            *reinterpret_cast<Piece *>(row + HALF) = hi;
+            store16<STREAM>(row, lo);
+            store16<STREAM>(row + HALF, hi);
         }
     }
 }
@@ -117,23 +135,23 @@ __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(NormRope p) {
     }
 }
 
-template <typename T, int LPR, int HPC>
+template <typename T, int LPR, int HPC, bool STREAM>
 void launch_vec(NormRope p, hipStream_t s) {
     p.q_chunks = (p.H[0] + HPC - 1) / HPC;
     const int threads = p.n_tok * LPR <= 64 ? 64 : 256;   // (a whole number of rows either way)
     const int64_t blocks = (p.n_tok * LPR + threads - 1) / threads;
-    hipLaunchKernelGGL((qk_norm_rope_kernel<T, LPR, HPC>), dim3((unsigned)blocks, (unsigned)(p.q_chunks + (p.H[1] + HPC - 1) / HPC)), dim3(threads), 0, s, p);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<T, LPR, HPC, STREAM>), dim3((unsigned)blocks, (unsigned)(p.q_chunks + (p.H[1] + HPC - 1) / HPC)), dim3(threads), 0, s, p);
 }
 
 template <typename T, int LPR>
 void launch_heads(const NormRope &p, hipStream_t s) {
-    // heads that a lane takes: as many as leave four workgroups per compute unit
-    const int64_t rows = (p.n_tok * LPR + 255) / 256 * (p.H[0] + p.H[1]);
-    const int64_t enough = (int64_t)num_compute_units() * 4;
-    if (rows >= 8 * enough) launch_vec<T, LPR, 8>(p, s);
-    else if (rows >= 4 * enough) launch_vec<T, LPR, 4>(p, s);
-    else if (rows >= 2 * enough) launch_vec<T, LPR, 2>(p, s);
-    else launch_vec<T, LPR, 1>(p, s);
+    // a lane takes two heads where that leaves four workgroups per compute unit: 168 MB of f16 41.1 us, against 44.9 with one head a
+    // lane, 40.9 with four and 42.3 with eight (past the caches 36.3, 36.5 with four, 37.7 with eight); 1000 tokens 5.9 to 6.0 with each
+    const int64_t rows = (p.n_tok * LPR + 255) / 256 * (p.H[0] + p.H[1]), enough = (int64_t)num_compute_units() * 4;
+    const int64_t bytes = 2 * p.n_tok * (p.H[0] + p.H[1]) * p.D * (int64_t)sizeof(T);
+    if (bytes > kStreamBytes) launch_vec<T, LPR, 2, true>(p, s);
+    else if (rows >= 2 * enough) launch_vec<T, LPR, 2, false>(p, s);
+    else launch_vec<T, LPR, 1, false>(p, s);
 }
 
 }  // namespace
