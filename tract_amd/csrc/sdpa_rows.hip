@@ -760,26 +760,24 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
 
 // A row's parts -> its output, by D / 4 lanes of a wave.  Everything that some 8 ranges have is asked for at once: one latency for up to
 // 8 of them.  (At most 64.)
-template <typename T, int D, bool LIVE>   // LIVE: parts that other workgroups of this launch have stored
+template <typename T, int D>
 __device__ __forceinline__ void join_row(const float *part_o, const float *part_ml, T *out, int64_t row, int64_t rows, int splits) {
     constexpr int LPR = D / 4, MOST = 64 / LPR, BATCH = 8;
     const int lr = threadIdx.x % LPR;
     const float *po = part_o + row * D + 2 * lr;   // this lane's features: two, and two half a row on
-    auto word = [](const float *at) { return LIVE ? get(at) : *at; };
-    auto two = [](const float *at) { return LIVE ? get2(at) : *reinterpret_cast<const float2_t *>(at); };
     float f[MOST], ls[MOST], l = 0.0f, mm = -INFINITY;
 #pragma unroll
     for (int x = 0; x < MOST; x++) {
         const int s = min(x * LPR + lr, splits - 1);
-        f[x] = word(part_ml + (int64_t)s * 2 * rows + row);
-        ls[x] = word(part_ml + ((int64_t)s * 2 + 1) * rows + row);
+        f[x] = get(part_ml + (int64_t)s * 2 * rows + row);
+        ls[x] = get(part_ml + ((int64_t)s * 2 + 1) * rows + row);
     }
     float2_t v[BATCH][2];
     auto ask = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
         for (int y = 0; y < BATCH; y++) {
             const float *at = po + (int64_t)min(s0 + y, splits - 1) * rows * D;
-            v[y][0] = two(at), v[y][1] = two(at + D / 2);
+            v[y][0] = get2(at), v[y][1] = get2(at + D / 2);
         }
     };
     ask(0);
@@ -870,7 +868,7 @@ __device__ __forceinline__ void arrive(const RowsDev &p, const RowsWork &wk, uin
     constexpr int LPR = D / 4;
     for (int r = begin + tid / LPR; r < end; r += kThreads / LPR)   // (whole groups of LPR lanes stay or leave)
         if ((done >> (unit_of(r) - first)) & 1)
-            join_row<T, D, true>(p.part_o, p.part_ml, reinterpret_cast<T *>(p.out), q_row(p, wk.kvh, r).at, p.part_rows, p.splits);
+            join_row<T, D>(p.part_o, p.part_ml, reinterpret_cast<T *>(p.out), q_row(p, wk.kvh, r).at, p.part_rows, p.splits);
 }
 
 constexpr int rows_lds(int es, int D, int R) {   // rows_body's LDS
@@ -929,11 +927,54 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
         if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
 }
 
-// The same in a launch of its own: after tall tiles, whose last workgroup would have 128 rows to join.
-template <typename T, int D>
+// The same in a launch of its own: after tall tiles, whose last workgroup would have 128 rows to join.  NG groups of D / 4 lanes take a row's
+// parts in turn, so that all of 8 NG are asked for at once; one group where there are no more than 8.  (f16: 2048 rows of 17 parts,
+// D = 128, the call in one group each 40.6 us, in two 39.7; 12800 rows of 4 parts, D = 64, 25.2 us, in four groups 27.1.)
+template <typename T, int D, int NG>
 __global__ __launch_bounds__(256) void sdpa_rows_merge_kernel(const float *__restrict__ part_o, const float *__restrict__ part_ml, T *__restrict__ out, int64_t rows, int splits) {
-    constexpr int LPR = D / 4;
-    join_row<T, D, false>(part_o, part_ml, out, min((int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, rows - 1), rows, splits);   // (rows past the last write it again, the same)
+    constexpr int LPR = D / 4, LANES = LPR * NG, BATCH = 8;
+    const int lane = threadIdx.x % LANES, grp = lane / LPR, lr = lane % LPR;
+    const int64_t row = min((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, rows - 1);   // (rows past the last write it again, the same)
+    const int mine = min(lane, splits - 1);   // (no more parts than lanes: 64, or 8)
+    float f = part_ml[(int64_t)mine * 2 * rows + row];
+    const float ls = part_ml[((int64_t)mine * 2 + 1) * rows + row];
+    const float *po = part_o + row * D + 4 * lr;
+    float4_t v[BATCH];
+    auto ask = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int y = 0; y < BATCH; y++) v[y] = *reinterpret_cast<const float4_t *>(po + (int64_t)min(s0 + y * NG + grp, splits - 1) * rows * D);
+    };
+    ask(0);
+    if (lane >= splits) f = -INFINITY;
+    float mm = f;
+#pragma unroll
+    for (int w = 1; w < LANES; w <<= 1) mm = fmaxf(mm, __shfl_xor(mm, w, 64));
+    const bool has = f != -INFINITY;   // (a range without keys for the row has stored nothing else)
+    f = has ? __builtin_amdgcn_exp2f(f - mm) : 0.0f;
+    float l = has ? f * ls : 0.0f;
+#pragma unroll
+    for (int w = 1; w < LANES; w <<= 1) l += __shfl_xor(l, w, 64);
+    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < splits; s0 += BATCH * NG) {
+#pragma unroll
+        for (int y = 0; y < BATCH; y++) {
+            const float h = __shfl(f, (s0 + y * NG + grp) % LANES, LANES), g = s0 + y * NG + grp < splits ? h : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] = g != 0.0f ? __builtin_fmaf(g, v[y][e], acc[e]) : acc[e];
+        }
+        if (s0 + BATCH * NG < splits) ask(s0 + BATCH * NG);
+    }
+#pragma unroll
+    for (int w = LPR; w < LANES; w <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], w, 64);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (grp == 0) {
+        struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
+#pragma unroll
+        for (int e = 0; e < 4; e++) four.e[e] = (T)(acc[e] * inv);
+        *reinterpret_cast<Four *>(out + row * D + 4 * lr) = four;
+    }
 }
 
 int check_launch(const char *what) {
@@ -1018,8 +1059,8 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
         if (check_launch("sdpa_rows")) return 1;
     }
     if (p.splits > 1 && !p.counters) {
-        constexpr int ROWS = 256 / (D / 4);
-        hipLaunchKernelGGL((sdpa_rows_merge_kernel<T, D>), dim3((unsigned)((p.part_rows + ROWS - 1) / ROWS)), dim3(256), 0, s, p.part_o, p.part_ml, (T *)p.out, p.part_rows, p.splits);
+        if (p.splits <= 8) hipLaunchKernelGGL((sdpa_rows_merge_kernel<T, D, 1>), dim3((unsigned)((p.part_rows * (D / 4) + 255) / 256)), dim3(256), 0, s, p.part_o, p.part_ml, (T *)p.out, p.part_rows, p.splits);
+        else hipLaunchKernelGGL((sdpa_rows_merge_kernel<T, D, 256 / D>), dim3((unsigned)((p.part_rows + 3) / 4)), dim3(256), 0, s, p.part_o, p.part_ml, (T *)p.out, p.part_rows, p.splits);
         if (check_launch("sdpa_rows_merge")) return 1;
     }
     return 0;
