@@ -1098,8 +1098,28 @@ int64_t tiles_of_a_part(int64_t units, int64_t all, int64_t es, int64_t D) {
     return (all + best_n - 1) / best_n;
 }
 
-// Rounds of a workgroup with `per` tiles of `all`.
-double p_round_of(int64_t per, int64_t all, double step) { return (double)(per < all ? per : all) / step; }
+// What a call is expected to take (us) with `pn` parts of the prefix and `on` of the own keys.  A workgroup takes `start` and a round, a
+// tile for each of its waves, `p_round` or `o_round`.  The call takes the longest workgroup and some more where not all run at once; or
+// what memory needs for the keys and parts, and the last one's tail; or the workgroups' rounds over all that run at once; and the join.  The
+// constants were fitted to 370 measured choices of 42 calls (f16 and f32, 64 and 128 features, 1 to 200 sequences, prefixes of 0 to
+// 30000 keys), of which it picks one within 2 % of the best on average and 17 % at worst.
+struct RowsCost {
+    int64_t kv_heads, units, p_row_tiles, p_all, own_all;   // units: rows' tiles of all sequences, over own keys
+    int pre, own;
+    double o_round, p_round, slots, bytes_us, part_mb;
+    bool merged;   // parts are joined by a launch of their own
+    double rounds(int64_t tiles, int64_t parts) const { return (double)(((uint32_t)(tiles + parts - 1) / (uint32_t)parts + kWaves - 1) / kWaves); }
+    double us(int64_t pn, int64_t on, double own_wgs, double own_rounds) const {
+        const double start = 2.1, parts = (double)(pn + on), wgs_p = (double)(kv_heads * p_row_tiles * pn), all_own = (double)(kv_heads * units * on);
+        const double p_chain = pn ? start + (pre == 128 ? (double)((p_all + pn - 1) / pn) : rounds(p_all, pn)) * p_round : 0.0;
+        const double o_chain = on ? start + rounds(own_all, on) * o_round : 0.0, longest = p_chain > o_chain ? p_chain : o_chain;
+        const double run = longest + (own_wgs + wgs_p > slots ? 0.7 * o_chain : 0.0);
+        const double memory = start + bytes_us + 0.43 * parts * part_mb + 0.24 * longest;
+        const double busy = (own_rounds * o_round + all_own * 2.2 * start + wgs_p * p_chain) / slots + 0.26 * longest;
+        const double most = run > memory ? (run > busy ? run : busy) : (memory > busy ? memory : busy);
+        return most + (parts <= 1 ? 0.0 : merged ? 2.0 + parts * (0.07 + 0.64 * part_mb) : 1.0 + parts * (0.27 + 3.1 * part_mb));
+    }
+};
 
 // On the matrix cores: 0 done, 1 failed, 2 not covered.
 int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
@@ -1134,58 +1154,66 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     const int64_t p_tile = pre == 128 ? kTallTile : kTile, p_all = (a.P + p_tile - 1) / p_tile, own_all = (longest + kTile - 1) / kTile;
     p.p_row_tiles = a.P ? (int)((rows + pre - 1) / pre) : 0;
     p.own_row_tiles = longest ? (int)((seq_rows + own - 1) / own) : 0;
-    // Ranges of keys, by what each choice is expected to take (us).  A workgroup takes `start` and a round of a tile per wave `round`;
-    // all of them together what their tiles take at the rate of memory or of the matrix cores, and `start` times their rounds over the
-    // chip; parts that are joined `join` more each.  (An estimate: it only has to rank the choices.)
-    const bool f32 = es == 4;
+    // Into how many parts the keys go (at most as many as there is room for).
+    const bool f32 = es == 4, uniform = !a.lens && !a.seqs;
     const double wide = a.D == 128 ? 1.0 : 0.5, cus = num_compute_units();
-    const double own_round = f32 ? (own == 32 ? 3.6 : 2.0) * wide : 0.4 + (own == 32 ? 1.2 : 0.7) * wide;
-    const double own_rate = (f32 ? (own == 32 ? 3.6 : 2.0) : 0.8) * wide / cus / kWaves, pre_rate = pre == 128 ? 1.5 * (0.4 + 0.6 * wide) / cus : (f32 ? (pre == 32 ? 3.6 : 2.0) : pre == 32 ? 1.0 : 0.6) * wide / cus / kWaves;
-    const double pre_round = pre == 128 ? 0.8 + 0.8 * wide : f32 ? (pre == 32 ? 3.6 : 2.0) * wide : 0.4 + (pre == 32 ? 1.2 : 0.7) * wide;
-    const double start = 2.5, slots = cus * (f32 && a.D == 128 && (own == 32 || pre == 32) ? 1 : 2), p_step = pre == 128 ? 1 : kWaves;
-    int64_t p_per = 1, o_per = kWaves;
+    auto round_of = [&](int rows_) { return f32 ? (rows_ == 32 ? 4.6 * wide : 4.4 * (0.43 + 0.57 * wide)) : (rows_ == 32 ? 2.0 : 1.26) * (0.35 + 0.65 * wide); };
+    RowsCost cost;
+    cost.kv_heads = a.Hkv, cost.units = a.B * p.own_row_tiles, cost.p_row_tiles = p.p_row_tiles, cost.p_all = p_all, cost.own_all = own_all;
+    cost.pre = pre, cost.own = own, cost.o_round = round_of(own), cost.p_round = pre == 128 ? 2.26 * (0.35 + 0.65 * wide) : round_of(pre);
+    cost.slots = cus * (a.D == 64 ? 3 : f32 && (own == 32 || pre == 32) ? 1 : 2);
+    cost.bytes_us = (double)((own_tiles_all + p_all * (p_tile / kTile)) * kTile * a.Hkv) * (double)(a.D * es * 2) / 5e6;
+    cost.part_mb = (double)rows_all * (double)(a.D + 2) * 4e-6;
+    // Joined by the last to arrive where that is at most two rows for a group of D / 4 lanes: 4 x 777 + 40 keys 9.5 -> 8.5 us, but
+    // 16 x 2000 + 600 keys, whose tiles over the prefix hold four rows for each, 13.5 -> 19.3 us.
+    const int64_t joined = a.P ? (rows < pre ? rows : pre) : own, units = a.Hkv * (p.own_row_tiles ? a.B * p.own_row_tiles : p.p_row_tiles);
+    cost.merged = pre == 128 || joined * a.D > 2048 || units > (int64_t)(kWsCounterBytes / sizeof(int));
+    const int64_t p_most = a.P ? (pre == 128 ? p_all : (p_all + kWaves - 1) / kWaves) : 0, o_most = longest ? (own_all + kWaves - 1) / kWaves : 0;
+    static const int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    const int64_t p_least = pre == 128 && o_most == 0 ? 2 : 1, parts_most = room < 64 ? room : 64;
+    const bool fixed = uniform && longest && (a.documents || p.own_row_tiles == 1);
+    int64_t fixed_n = 1;   // (documents: how much of its keys a row's document has is not known here)
+    if (fixed && p.own_row_tiles == 1) {
+        const int64_t per = tiles_of_a_part(a.Hkv * a.B, own_all, es, a.D);
+        fixed_n = (own_all + per - 1) / per;
+        if (fixed_n > parts_most) fixed_n = parts_most > 1 ? parts_most : 1;
+    }
     double best = 1e30;
-    for (int64_t op = kWaves;; op = op * 2 > own_all ? (own_all + kWaves - 1) / kWaves * kWaves : op * 2) {
-        int64_t own_wgs = 0;
-        if (a.lens || a.seqs)
-            for (int64_t b = 0; b < a.B; b++) own_wgs += (uint32_t)((uint32_t)((a.lens ? a.lens[b] : a.seqs[b].len) + kTile - 1) / kTile + (uint32_t)op - 1) / (uint32_t)op;
-        else own_wgs = a.B * ((own_all + op - 1) / op);
-        own_wgs *= a.Hkv * p.own_row_tiles;
-        const int64_t own_n = (own_all + op - 1) / op;
-        for (int64_t pp = pre == 128 ? 4 : kWaves;; pp = pp * 2) {
-            const int64_t p_n = (p_all + pp - 1) / pp, p_wgs = a.Hkv * p.p_row_tiles * p_n;
-            const double longest_wg = start + (a.P && p_round_of(pp, p_all, p_step) * pre_round > (double)((op < own_all ? op : own_all) + kWaves - 1) / kWaves * own_round
-                                                   ? p_round_of(pp, p_all, p_step) * pre_round : (longest ? ((op < own_all ? op : own_all) + kWaves - 1) / kWaves * own_round : 0.0));
-            const double all = start * (double)((own_wgs + p_wgs + slots - 1) / slots) + a.Hkv * (p.own_row_tiles * own_tiles_all * own_rate + p.p_row_tiles * p_all * pre_rate);
-            const double parts = (double)(own_n + p_n);
-            const double join = parts > 1 ? (pre == 128 ? 5.0 : 1.5) + parts * (0.1 + rows_all * (a.D + 2) * 8.0 / 4e6) : 0.0;
-            const double t = (longest_wg > all ? longest_wg : all) + join;
-            if (t < best) best = t, p_per = pp, o_per = op;
-            if (pp >= p_all) break;
+    for (int x = 0; x < (int)(sizeof(kParts) / sizeof(int)); x++) {
+        if (x && (fixed || kParts[x - 1] >= o_most)) break;
+        const int64_t on = fixed ? fixed_n : kParts[x] < o_most ? kParts[x] : o_most;
+        // tiles of a part; workgroups with something to do, and their rounds
+        const int64_t op = on ? (own_all + on - 1) / on : 1;
+        double own_wgs = 0.0, own_rounds = 0.0;
+        auto add = [&](int64_t tiles, double times) {
+            if (tiles == 0) return;
+            const uint32_t n = (uint32_t)(tiles + op - 1) / (uint32_t)op, parts = n < on ? n : (uint32_t)on;
+            own_wgs += times * parts, own_rounds += times * parts * cost.rounds(tiles, parts);
+        };
+        if (uniform && on) {
+            const int64_t hidden = a.causal && !a.prefix_lens ? (a.Sq - 1) / 2 / kTile : 0;   // of a tile of rows, on average
+            add(own_all > hidden ? own_all - hidden : 1, (double)cost.units);
+        } else if (on) {
+            for (int64_t b = 0; b < a.B; b++) add(((a.lens ? a.lens[b] : a.seqs[b].len) + kTile - 1) / kTile, (double)p.own_row_tiles);
         }
-        if (op >= own_all) break;
+        own_wgs *= a.Hkv, own_rounds *= a.Hkv;
+        for (int y = 0; y < (int)(sizeof(kParts) / sizeof(int)); y++) {
+            if (y && kParts[y - 1] >= p_most) break;
+            const int64_t pn = kParts[y] < p_most ? kParts[y] : p_most;
+            if ((p_most && pn < p_least) || (pn + on > 1 && pn + on > parts_most)) continue;
+            const double t = cost.us(pn, on, own_wgs, own_rounds);
+            if (t < best) best = t, p.p_splits = (int)pn, p.own_splits = (int)on, p.own_tiles = (int)op;
+        }
+        if (own_wgs > 4 * cost.slots) break;   // (more of them would not run sooner)
     }
-    // (Several tiles of rows per sequence are enough workgroups, of unlike lengths.)
-    if (!a.lens && !a.seqs && p.own_row_tiles == 1) o_per = tiles_of_a_part(a.Hkv * a.B, own_all, es, a.D);
-    if (!a.lens && !a.seqs && p.own_row_tiles > 1 && a.documents) o_per = own_all;   // (how much of its keys a row's document has is not known here)
-    if (pre == 128 && longest == 0 && p_per > (p_all + 1) / 2) p_per = (p_all + 1) / 2;
-    for (;; p_per *= 2, o_per *= 2) {
-        p.own_tiles = (int)o_per;
-        p.p_splits = (int)((p_all + p_per - 1) / p_per), p.own_splits = (int)((own_all + o_per - 1) / o_per);
-        p.splits = p.p_splits + p.own_splits;
-        if (p.splits == 1 || (p.splits <= room && p.splits <= 64)) break;
-        if (p.p_splits <= 1 && p.own_splits <= 1) return 2;   // (no room to join prefix and own keys in)
-    }
+    if (best == 1e30) return 2;   // (no room to join prefix and own keys in)
+    p.splits = p.p_splits + p.own_splits;
     p.by_g = fast_div(G), p.by_sq = fast_div(a.Sq), p.by_p_row_tiles = fast_div(p.p_row_tiles);
     p.by_own_splits = fast_div(p.own_splits), p.by_own_row_tiles = fast_div(p.own_row_tiles), p.by_own_tiles = fast_div(p.own_tiles);
     p.part_o = (float *)((char *)a.workspace + kWsCounterBytes + kWsPlanBytes);
     p.part_ml = p.part_o + (int64_t)p.splits * p.part_rows * a.D;
     if (p.splits == 1) p.part_o = p.part_ml = nullptr;
-    const int64_t units = a.Hkv * (p.own_row_tiles ? a.B * p.own_row_tiles : p.p_row_tiles);
-    // Joined by the last to arrive where that is at most two rows for a group of D / 4 lanes: 4 x 777 + 40 keys 9.5 -> 8.5 us, but
-    // 16 x 2000 + 600 keys, whose tiles over the prefix hold four rows for each, 13.5 -> 19.3 us.
-    const int64_t joined = a.P ? (rows < pre ? rows : pre) : own;
-    if (p.splits > 1 && pre != 128 && joined * a.D <= 2048 && units <= (int64_t)(kWsCounterBytes / sizeof(int))) p.counters = (int *)a.workspace;
+    if (p.splits > 1 && !cost.merged) p.counters = (int *)a.workspace;
     if (a.dtype == TROCM_F16) return a.D == 64 ? launch_tiles_of<_Float16, 64>(a, call, pre, own, is_scored, s) : launch_tiles_of<_Float16, 128>(a, call, pre, own, is_scored, s);
     return a.D == 64 ? launch_tiles_of<float, 64>(a, call, pre, own, is_scored, s) : launch_tiles_of<float, 128>(a, call, pre, own, is_scored, s);
 }
