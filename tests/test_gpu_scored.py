@@ -1,11 +1,12 @@
 """Attention with capped scores, distance slopes, documents and prefixes, against 64 bits."""
+import ctypes as C
 import itertools
 
 import numpy as np
 import pytest
 
 import tract_amd as ta
-from tests.attention_ref import assert_within, scored
+from tests.attention_ref import assert_within, scored, shared
 from tests.gpu_util import rt  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -66,6 +67,69 @@ def test_enough_rows_for_every_compute_unit(rt, b, hq, hkv, n, t, d):
     rng = np.random.default_rng(15)
     _check(F16, b, hq, hkv, n, t, d, cap=30.0)
     _check(F16, b, hq, hkv, n, t, d, cap=20.0, slopes=_slopes(hq), documents=_packed(rng, b, t, 5), prefix_lens=np.full(b, t // 4, np.int32))
+
+
+@pytest.mark.parametrize("rules", list(itertools.product([False, True], repeat=3)), ids=lambda r: "".join("csd"[i] if x else "-" for i, x in enumerate(r)))
+@pytest.mark.parametrize("shape", [(1, 32, 8, 1000, 1000, 128), (2, 28, 4, 1000, 1040, 64), (4, 32, 32, 300, 300, 128), (8, 64, 32, 300, 310, 64)], ids=str)
+def test_every_rule_where_rows_fill_the_card(rt, rules, shape):
+    """Head sizes 128 and 64, one group of waves per workgroup and two; keys before the queries, of the first of them none for some rows."""
+    b, hq, hkv, n, t, d = shape
+    cap, slopes, documents = rules
+    _check(F16, *shape, cap=25.0 if cap else 0.0, slopes=_slopes(hq) if slopes else None, documents=_packed(np.random.default_rng(16), b, t, 3) if documents else None)
+
+
+def test_unusual_scales_where_rows_fill_the_card(rt):
+    shape = (1, 32, 8, 1000, 1000, 128)
+    _check(F16, *shape, slopes=_slopes(32), scale=-0.05)
+    _check(F16, *shape, scale=0.0)
+    _check(F16, *shape, cap=10.0, scale=-0.05, slopes=_slopes(32))
+    _check(F16, *shape, cap=1e-9, slopes=_slopes(32))
+    _check(F16, *shape, slopes=_slopes(32), scale=1e-9)
+    _check(F16, 1, 32, 8, 1000, 900, 128, cap=10.0)               # fewer keys than queries
+    _check(F16, 1, 32, 8, 1000, 1000, 128, slopes=_slopes(32), causal=False)
+
+
+@pytest.mark.parametrize("hq,hkv,n", [(64, 8, 1000), (4, 2, 3)])
+def test_documents_over_very_many_keys(rt, hq, hkv, n):
+    """More tiles of keys than are looked up beforehand: some rows of some heads against 64 bits."""
+    rng = np.random.default_rng(17)
+    t, d = 263000, 64
+    q, k = _rows(rng, (1, hq, n, d), F16, 3.0), _rows(rng, (1, hkv, t, d), F16)
+    v = np.ascontiguousarray(k[:, ::-1, ::-1])
+    ids = rng.integers(0, 3, (1, t)).astype(np.int32)
+    ids[0, 1000:1500], ids[0, t - 2] = -1, -1
+    slopes = _slopes(hq) * 1e-4
+    dq, dk, dv, di = (ta.DeviceTensor.from_numpy(x) for x in (q, k, v, ids))
+    got = ta.ScoredSdpa(softcap=20.0).eval(dq, dk, dv, slopes=slopes, documents=di).to_numpy()
+    for h, i in ((0, 0), (hq - 1, n - 1), (hq // 2, n - 2), (hq // 3, n // 2)):
+        end = t - n + i + 1
+        want = scored(q[:, h : h + 1, i : i + 1], *(x[:, h * hkv // hq][:, None, :end] for x in (k, v)), cap=20.0, slopes=slopes[h : h + 1], documents=ids[:, :end])
+        assert_within(got[:, h : h + 1, i : i + 1], *want, what=f"head {h}, row {i}")
+
+
+@pytest.mark.parametrize("dtype,n,d", [(F16, 1, 128), (F16, 70, 64), (F32, 1, 64), (F16, 2, 48)])
+def test_keys_further_apart_than_32_bits(rt, dtype, n, d):
+    """300 keys 2^24 bytes apart; over the same rows as a shared prefix too."""
+    rng = np.random.default_rng(18)
+    es, hq, hkv, t = np.dtype(dtype).itemsize, 4, 2, 300
+    apart = 2**24 // es
+    rows = _rows(rng, (t, 2, hkv, d), dtype)
+    big = ta.DeviceTensor((t * apart,), dtype)
+    for j in range(t):
+        ta._lib.call("trocm_h2d", C.c_void_p(big.ptr.value + j * 2**24), rows[j].ctypes.data_as(C.c_void_p), rows[j].nbytes, None)
+    ta.synchronize()
+    k, v = (np.ascontiguousarray(rows[:, i].transpose(1, 0, 2))[None] for i in range(2))
+    q = _rows(rng, (1, hq, n, d), dtype, 2.0)
+    dq, out = ta.DeviceTensor.from_numpy(q), ta.DeviceTensor(q.shape, dtype)
+    ws = ta.Workspace(1, hq, n, d, nbytes=ta.Workspace.shared_bytes_for(1, hq, n, d))
+    code, v_at = 0 if dtype == F32 else 1, C.c_void_p(big.ptr.value + hkv * d * es)
+    ta._lib.call("trocm_sdpa_scored", dq.ptr, big.ptr, v_at, out.ptr, code, 1, hq, hkv, n, t, d, (C.c_int64 * 3)(0, d, apart), float("nan"), 15.0, None, None, None, 1,
+                 ws.ptr, ws.nbytes, None)
+    assert_within(out.to_numpy(), *scored(q, k, v, cap=15.0))
+    none = ta.DeviceTensor((1, hkv, 1, d), dtype)
+    ta._lib.call("trocm_sdpa_shared_prefix", dq.ptr, code, 1, hq, hkv, n, d, big.ptr, v_at, t, (C.c_int64 * 2)(d, apart), none.ptr, none.ptr,
+                 (C.c_int64 * 3)(hkv * d, d, d), (C.c_int64 * 1)(0), out.ptr, float("nan"), 1, ws.ptr, ws.nbytes, None)
+    assert_within(out.to_numpy(), *shared(q, k[0], v[0], [k[0][:, :0]], [v[0][:, :0]]))
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])

@@ -117,7 +117,10 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
     const int guess = t_end - 1 - kg;
     if (guess >= 0) prefetch(guess * kTile);
 
-    const float slope = SLOPES ? p.slopes[kvh * p.G + g] * kLog2e : 0.0f;
+    // A score in the log2 domain is base + to_log2 s, of s the product with the key or, capped, 1 / (e^2x + 1) with x = scale q.k / cap:
+    // cap log2e tanh(x) = A - 2 A / (e^2x + 1).  The largest score is the smallest s there.  Only weights take the whole sum.
+    const float base = CAP ? p.cap * kLog2e : 0.0f, to_log2 = CAP ? -2.0f * base : p.scale * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
+    const float hidden = CAP ? INFINITY : -INFINITY, slope = SLOPES ? -kLog2e / to_log2 * p.slopes[kvh * p.G + g] : 0.0f;
     const int doc = DOCS ? docs[at] : 0;
     if (DOCS && doc < 0) lim = -1;   // padding sees nothing
     bool listed = false;
@@ -195,9 +198,6 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
     for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int x = 0; x < 16; x++) o[db][x] = 0.0f;
-    // the cap in the log2 domain: cap log2e tanh(x) = A - 2 A / (e^2x + 1), x = s scale / cap
-    const float to_log2 = p.scale * kLog2e, cap_a = p.cap * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
-
     half8_t qf[KS];
     if (DOCS && kg < n_tiles && tile_lo(entry(kg)) != guess * kTile) prefetch(tile_lo(entry(kg)));   // (padding, or a prefix)
 #pragma unroll
@@ -229,15 +229,12 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
             // (asked for once the products are there: all 32 distances computed beside the MFMAs spill registers; of the group of four
             // at hand, so that what is subtracted are inline constants)
             if constexpr (SLOPES) asm volatile("" : "+v"(d0), "+v"(s[1]));
+            if constexpr (CAP) {
 #pragma unroll
-            for (int kb2 = 0; kb2 < 2; kb2++)
+                for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    if constexpr (CAP)
-                        s[kb2][x] = __builtin_fmaf(-2.0f * cap_a, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kb2][x] * cap_k) + 1.0f), cap_a);
-                    else
-                        s[kb2][x] *= to_log2;
-                }
+                    for (int x = 0; x < 16; x++) s[kb2][x] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kb2][x] * cap_k) + 1.0f);
+            }
             if constexpr (DOCS) {
                 if (!(listed && (e & 0x8000))) {
 #pragma unroll
@@ -245,10 +242,10 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
                         for (int x = 0; x < 16; x += 4) {
                             const int4 four = *reinterpret_cast<const int4 *>(&s_ids[buf][32 * kb2 + 2 * x + 4 * hb]);
-                            s[kb2][x] = four.x == doc ? s[kb2][x] : -INFINITY;
-                            s[kb2][x + 1] = four.y == doc ? s[kb2][x + 1] : -INFINITY;
-                            s[kb2][x + 2] = four.z == doc ? s[kb2][x + 2] : -INFINITY;
-                            s[kb2][x + 3] = four.w == doc ? s[kb2][x + 3] : -INFINITY;
+                            s[kb2][x] = four.x == doc ? s[kb2][x] : hidden;
+                            s[kb2][x + 1] = four.y == doc ? s[kb2][x + 1] : hidden;
+                            s[kb2][x + 2] = four.z == doc ? s[kb2][x + 2] : hidden;
+                            s[kb2][x + 3] = four.w == doc ? s[kb2][x + 3] : hidden;
                         }
                 }
             }
@@ -258,7 +255,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
                         const float d = (x & 3) == 0 ? d0 : (x & 3) == 1 ? d0 - 1.0f : (x & 3) == 2 ? d0 - 2.0f : (d0 - 2.0f) - 1.0f;
-                        s[kb2][x] = __builtin_fmaf(-slope, fabsf(d), s[kb2][x]);
+                        s[kb2][x] = __builtin_fmaf(slope, fabsf(d), s[kb2][x]);
                         if ((x & 3) == 3) d0 -= 8.0f;
                     }
             }
@@ -267,14 +264,15 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
                 for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
-                    for (int x = 0; x < 16; x++) s[kb2][x] = 32 * kb2 + 8 * (x >> 2) + (x & 3) <= last ? s[kb2][x] : -INFINITY;
+                    for (int x = 0; x < 16; x++) s[kb2][x] = 32 * kb2 + 8 * (x >> 2) + (x & 3) <= last ? s[kb2][x] : hidden;
             }
             float top = s[0][0];
 #pragma unroll
             for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
-                for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb2][x]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
+                for (int x = 0; x < 16; x++) top = CAP ? fminf(top, s[kb2][x]) : fmaxf(top, s[kb2][x]);
+            const float other = __shfl_xor(top, 32, 64);
+            top = __builtin_fmaf(CAP ? fminf(top, other) : fmaxf(top, other), to_log2, base);
             // the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
             const bool moved = top > m_run + 8.0f;
             const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
@@ -286,7 +284,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
             for (int st = 0; st < 4; st++) {
 #pragma unroll
-                for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + x] - ref);
+                for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, base - ref));
 #pragma unroll
                 for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
             }
@@ -391,6 +389,7 @@ void launch_of(const ScoredDev &p, hipStream_t s) {
 // 0 done, 1 failed, 2 not covered (the kernels of sdpa_rows.hip take it).
 int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     if (a.dtype != TROCM_F16 || (a.D != 64 && a.D != 128) || a.P || a.lens || a.seqs || a.Sk == 0 || a.softcap > kFastTanhCap) return 2;
+    if (a.softcap > 0.0f ? a.softcap < 1e-6f : !(a.scale > 1e-6f)) return 2;   // (slopes are divided by it, and the largest product stands for the largest score)
     auto aligned = [](const void *x) { return (uintptr_t)x % 16 == 0; };
     const int64_t G = a.Hq / a.Hkv, rows = a.Sq * G;
     if (!aligned(a.q) || !aligned(a.out) || !aligned(a.k) || !aligned(a.v) || a.stride_b % 8 || a.stride_h % 8 || a.stride_t % 8 || a.stride_t * 2 > (1 << 25)) return 2;
