@@ -74,9 +74,11 @@ __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(_Float16 x) { return (float)x; }
 
 // 16 bytes of device memory.  Pointers that come out of a table are generic ones to the compiler, whose loads go by the LDS's
-// counter too: every wait for LDS would wait for the tile in flight.
+// counter too: every wait for LDS would wait for the tile in flight.  ONCE: past the caches.
+template <bool ONCE = false>
 __device__ __forceinline__ u32x4 load16(const char *base, uint32_t off) {
-    return *(const __attribute__((address_space(1))) u32x4 *)(base + off);
+    const auto *at = (const __attribute__((address_space(1))) u32x4 *)(base + off);
+    return ONCE ? __builtin_nontemporal_load(at) : *at;
 }
 
 struct OwnKeys { const char *k, *v; int len; };
@@ -287,7 +289,7 @@ __device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, 
 //   R == 16: 16x16 MFMAs.  K goes straight from memory into fragments (four lanes read 64 consecutive bytes of a key's row), V
 //            through a wave-private LDS tile.
 //   R == 32: 32x32 MFMAs, K and V through a wave-private LDS tile.
-template <typename T, int D, int R, bool SCORED>
+template <typename T, int D, int R, bool SCORED, bool ONCE>
 __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, unsigned char *lds, uint16_t *s_list, int *s_counts) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int DB = D / R, NG = 64 / R;        // feature blocks of the output; lane groups (4 or 2), whose lanes hold a row each
@@ -367,7 +369,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < NI; j++) kpre[j] = load16(tk, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
+            for (int j = 0; j < NI; j++) kpre[j] = load16<ONCE>(tk, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
         }
         if (SCORED && docs) id_pre = docs[k_lo + min(lane & 31, most)];
     };
@@ -375,7 +377,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
         const int k_lo = tile_at(n) * kTile, most = n_keys - 1 - k_lo;
         const char *tv = wk.v + (int64_t)k_lo * wk.st;
 #pragma unroll
-        for (int j = 0; j < NI; j++) vpre[j] = load16(tv, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
+        for (int j = 0; j < NI; j++) vpre[j] = load16<ONCE>(tv, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
     };
     const float to_log2 = p.scale * kLog2e, cap_log2 = p.cap * kLog2e, to_cap = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
     // key of score x of this lane, from the tile's first: groups of four consecutive ones
@@ -878,7 +880,7 @@ constexpr int tall_lds(int D) { return 2 * kTallTile * (2 * D + 24) * 2; }
 constexpr int most_of(int a, int b) { return a > b ? a : b; }
 
 // PRE: rows of a tile over the prefix, 128 the tall body (0: there is none); OWN: over own keys.
-template <typename T, int D, int PRE, int OWN, bool SCORED>
+template <typename T, int D, int PRE, int OWN, bool SCORED, bool ONCE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 || OWN == 32) ? 1 : 2) void sdpa_rows_kernel(RowsCall call) {
     const RowsDev &p = call.p;
     constexpr int ES = sizeof(T);
@@ -902,7 +904,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
             tall_body<D>(p, wk, lds);
             return;
         } else if constexpr (PRE != 0 && PRE != OWN) {
-            rows_body<T, D, PRE, false>(p, wk, lds, nullptr, nullptr);
+            rows_body<T, D, PRE, false, false>(p, wk, lds, nullptr, nullptr);
             there = true;
         }
     } else {
@@ -922,7 +924,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
         wk.tiles = (n_vis + kTile - 1) / kTile, wk.part = split, wk.parts = min(p.own_splits, max(1, p.by_own_tiles.by(wk.tiles + p.own_tiles - 1)));
         wk.split = p.p_splits + split;
     }
-    if (!there) rows_body<T, D, OWN, SCORED>(p, wk, lds, s_list, s_counts);
+    if (!there) rows_body<T, D, OWN, SCORED, ONCE>(p, wk, lds, s_list, s_counts);
     if constexpr (PRE != 128)
         if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
 }
@@ -1041,7 +1043,7 @@ int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_n
 
 namespace {
 
-template <typename T, int D, int PRE, int OWN, bool SCORED>
+template <typename T, int D, int PRE, int OWN, bool SCORED, bool ONCE>
 int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
     RowsDev &p = call.p;
     const int64_t prefix_items = (int64_t)p.p_splits * p.p_row_tiles, per_seq = (int64_t)p.own_row_tiles * p.own_splits, most = 65535;
@@ -1055,7 +1057,7 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
         p.p_items = b == 0 ? (int)prefix_items : 0;
         const int64_t items = p.p_items + n * p.own_row_tiles * p.own_splits;
         if (items == 0) continue;
-        hipLaunchKernelGGL((sdpa_rows_kernel<T, D, PRE, OWN, SCORED>), dim3((unsigned)a.Hkv, (unsigned)items), dim3(kThreads), 0, s, call);
+        hipLaunchKernelGGL((sdpa_rows_kernel<T, D, PRE, OWN, SCORED, ONCE>), dim3((unsigned)a.Hkv, (unsigned)items), dim3(kThreads), 0, s, call);
         if (check_launch("sdpa_rows")) return 1;
     }
     if (p.splits > 1 && !p.counters) {
@@ -1066,18 +1068,28 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
     return 0;
 }
 
+// ONCE where it pays, for 16 f16 rows: keys that one workgroup reads, and that are more than the 256 MB behind the L2 caches keep from call to
+// call.  (Through the caches | past them, us: 8 x 8193 keys of 8 x 128 features 50.3 | 45.6, 16 x 6000 73.5 | 64.5, 64 x 8192 + 512
+// 35.7 | 32.3; but 64 x 512 17.3 | 18.2, one sequence of 8193 14.4 | 15.2.  f32 keys, read in pieces of 64 bytes: 16 x 4096 + 600 35.1 | 37.2.)
+template <typename T, int D, int PRE, bool SCORED>
+int launch_tiles_16(const SdpaRowsArgs &a, RowsCall &call, bool once, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (once) return launch_tiles<T, D, PRE, 16, SCORED, true>(a, call, s);
+    return launch_tiles<T, D, PRE, 16, SCORED, false>(a, call, s);
+}
+
 template <typename T, int D>
-int launch_tiles_of(const SdpaRowsArgs &a, RowsCall &call, int pre, int own, bool is_scored, hipStream_t s) {
+int launch_tiles_of(const SdpaRowsArgs &a, RowsCall &call, int pre, int own, bool is_scored, bool once, hipStream_t s) {
     if constexpr (sizeof(T) == 2 || D == 128)
-        if (own == 32 && is_scored) return launch_tiles<T, D, 0, 32, true>(a, call, s);
-    if (is_scored) return launch_tiles<T, D, 0, 16, true>(a, call, s);
+        if (own == 32 && is_scored) return launch_tiles<T, D, 0, 32, true, false>(a, call, s);
+    if (is_scored) return launch_tiles_16<T, D, 0, true>(a, call, once, s);
     if constexpr (sizeof(T) == 2)
-        if (pre == 128) return own == 32 ? launch_tiles<T, D, 128, 32, false>(a, call, s) : launch_tiles<T, D, 128, 16, false>(a, call, s);
+        if (pre == 128) return own == 32 ? launch_tiles<T, D, 128, 32, false, false>(a, call, s) : launch_tiles_16<T, D, 128, false>(a, call, once, s);
     if constexpr (sizeof(T) == 2 || D == 128)
-        if (own == 32) return launch_tiles<T, D, 32, 32, false>(a, call, s);
+        if (own == 32) return launch_tiles<T, D, 32, 32, false, false>(a, call, s);
     if constexpr (sizeof(T) == 2)
-        if (pre == 32) return launch_tiles<T, D, 32, 16, false>(a, call, s);
-    return launch_tiles<T, D, 16, 16, false>(a, call, s);
+        if (pre == 32) return launch_tiles_16<T, D, 32, false>(a, call, once, s);
+    return launch_tiles_16<T, D, 16, false>(a, call, once, s);
 }
 
 // Sequences of one length: how many of its `all` key tiles a part of each unit of rows takes.  A workgroup's round of a tile per wave takes
@@ -1208,14 +1220,15 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     }
     if (best == 1e30) return 2;   // (no room to join prefix and own keys in)
     p.splits = p.p_splits + p.own_splits;
+    const bool once = p.own_row_tiles <= 1 && cost.bytes_us > 20.0;   // (100 MB)
     p.by_g = fast_div(G), p.by_sq = fast_div(a.Sq), p.by_p_row_tiles = fast_div(p.p_row_tiles);
     p.by_own_splits = fast_div(p.own_splits), p.by_own_row_tiles = fast_div(p.own_row_tiles), p.by_own_tiles = fast_div(p.own_tiles);
     p.part_o = (float *)((char *)a.workspace + kWsCounterBytes + kWsPlanBytes);
     p.part_ml = p.part_o + (int64_t)p.splits * p.part_rows * a.D;
     if (p.splits == 1) p.part_o = p.part_ml = nullptr;
     if (p.splits > 1 && !cost.merged) p.counters = (int *)a.workspace;
-    if (a.dtype == TROCM_F16) return a.D == 64 ? launch_tiles_of<_Float16, 64>(a, call, pre, own, is_scored, s) : launch_tiles_of<_Float16, 128>(a, call, pre, own, is_scored, s);
-    return a.D == 64 ? launch_tiles_of<float, 64>(a, call, pre, own, is_scored, s) : launch_tiles_of<float, 128>(a, call, pre, own, is_scored, s);
+    if (a.dtype == TROCM_F16) return a.D == 64 ? launch_tiles_of<_Float16, 64>(a, call, pre, own, is_scored, once, s) : launch_tiles_of<_Float16, 128>(a, call, pre, own, is_scored, once, s);
+    return a.D == 64 ? launch_tiles_of<float, 64>(a, call, pre, own, is_scored, once, s) : launch_tiles_of<float, 128>(a, call, pre, own, is_scored, once, s);
 }
 
 }  // namespace
