@@ -476,7 +476,7 @@ int trocm_quantized_kv_sdpa_eval(const void *q, const void *k_new, const void *v
  * k_strides[4] (NULL: dense; the last must be 1): views into the rows of a fused projection are legal.  Weights
  * [head_dim] of `dtype` (NULL: ones).  cos and sin: [n, head_dim] rows of `dtype` per batch entry, `cos_sin_batch_stride`
  * elements apart (0: one set of rows for all).  q_out and k_out dense; each may be its own input where that is dense,
- * and may overlap no other input.  head_dim even; 64, 128 and 256 with everything aligned to 16 bytes move 16 bytes per lane. */
+ * and may overlap no other input.  batch * n below 2^26; head_dim even; 64, 128 and 256 with everything aligned to 16 bytes move 16 bytes per lane. */
 int trocm_qk_norm_rope(const void *q, const void *k, const void *q_weight, const void *k_weight, float eps, const void *cos,
                        const void *sin, int64_t cos_sin_batch_stride, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
                        int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides, void *q_out, void *k_out,
@@ -526,12 +526,12 @@ int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const vo
  *   (not causal, or j <= i + (kv_len - q_len), or j < prefix_lens[b])
  *   and, with documents, both tokens are of one document: documents[b][j] == documents[b][i + kv_len - q_len] >= 0.
  *   softcap     : 0 (none) or 1e-30..1e30
- *   slopes      : [q_heads] f32, device memory, or NULL
+ *   slopes      : [q_heads] f32, device memory, or NULL; any sign, at most 1e30 in size
  *   documents   : [batch, kv_len] int32, device memory, or NULL; ids in any order, negative ones are padding that nothing sees
  *                 and whose K and V rows may hold anything; needs kv_len >= q_len
  *   prefix_lens : [batch] int32, device memory, or NULL; values past kv_len mean all of it; read only when causal
- * A row that sees nothing is zeros.  K and V rows that some query of the call sees must be finite: a weight of zero times an
- * infinite value is NaN for the other queries too.  out may not overlap q, k or v.  k, v, strides, scale and workspace as for trocm_sdpa. */
+ * A row that sees nothing is zeros.  All K and V rows but those of padding must be finite, seen or not: a weight of zero times an
+ * infinite value is NaN.  out may not overlap q, k or v.  k, v, strides, scale and workspace as for trocm_sdpa. */
 int trocm_sdpa_scored(const void *q, const void *k, const void *v, void *out, int dtype, int64_t batch, int64_t q_heads,
                       int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t head_dim, const int64_t *kv_strides, float scale,
                       float softcap, const float *slopes, const int32_t *documents, const int32_t *prefix_lens, int causal,

@@ -82,6 +82,19 @@ def test_nan_stays_in_its_row(rt):
     assert np.isfinite(got_q[~bad_q]).all() and np.isfinite(got_k[~bad_k]).all()
 
 
+def test_strides_are_read_at_every_call(rt):
+    rng = np.random.default_rng(20)
+    rows = rng.standard_normal((3, 8, 64), dtype=np.float32)
+    cos, sin = (ta.DeviceTensor.from_numpy(rng.standard_normal((1, 1, 3, 64), dtype=np.float32)) for _ in range(2))
+    x, strides, op = ta.DeviceTensor.from_numpy(rows), [3 * 8 * 64, 64, 8 * 64, 1], ta.QkNormRope(1e-6)
+    q, k = (ta.DeviceTensor((1, 4, 3, 64), np.float32, ptr=x.ptr, owner=x) for _ in range(2))
+    want = norm_rope(np.ascontiguousarray(rows[:, :4].transpose(1, 0, 2))[None], None, cos.to_numpy(), sin.to_numpy(), 1e-6)
+    assert_within(op.eval(q, k, None, None, cos, sin, q_strides=strides)[0].to_numpy(), *want)
+    strides[:] = [4 * 3 * 64, 3 * 64, 64, 1]     # the same list: now the buffer's first rows as they lie
+    want = norm_rope(rows.reshape(-1, 64)[:12].reshape(1, 4, 3, 64), None, cos.to_numpy(), sin.to_numpy(), 1e-6)
+    assert_within(op.eval(q, k, None, None, cos, sin, q_strides=strides)[0].to_numpy(), *want)
+
+
 def test_stream_and_refusals(rt):
     rng = np.random.default_rng(5)
     q, k = _rows(rng, (1, 4, 3, 64), F16), _rows(rng, (1, 2, 3, 64), F16)

@@ -89,6 +89,17 @@ def test_unusual_scales_where_rows_fill_the_card(rt):
     _check(F16, 1, 32, 8, 1000, 1000, 128, slopes=_slopes(32), causal=False)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_more_tiles_of_rows_than_one_axis_of_a_grid_has_places(rt, dtype):
+    """Over a few keys, where every row is a row of its own in 64 bits too: those at both ends and about tile 65535 of 16 and of 32 rows."""
+    rng = np.random.default_rng(19)
+    hq, n, t, d = 16, 132000, 20, 64
+    q, k, v = _rows(rng, (1, hq, n, d), dtype), _rows(rng, (1, 1, t, d), dtype), _rows(rng, (1, 1, t, d), dtype)
+    got = ta.ScoredSdpa(softcap=5.0, is_causal=False).eval(q, k, v).to_numpy()
+    at = np.r_[0:40, 65500:65570, 131000:131140, n - 40 : n]
+    assert_within(got[:, :, at], *scored(q[:, :, at], k, v, cap=5.0, causal=False))
+
+
 @pytest.mark.parametrize("hq,hkv,n", [(64, 8, 1000), (4, 2, 3)])
 def test_documents_over_very_many_keys(rt, hq, hkv, n):
     """More tiles of keys than are looked up beforehand: some rows of some heads against 64 bits."""

@@ -26,7 +26,7 @@ def _norm(**kw):
     (dict(dtype=2), "F32 or F16"), (dict(d=63), "must be even"), (dict(eps=-1.0), "eps"), (dict(eps=NAN), "eps"), (dict(q=None), "null pointer"), (dict(cos=None), "cos"),
     (dict(n=-1), "negative"), (dict(qs=I4(1, 1, -1, 1)), "negative strides"), (dict(ks=I4(384, 192, 64, 2)), "contiguous"), (dict(cs=100), "overlap"),
     (dict(qo=A + 64), "overlap"), (dict(qo=B_), "overlap"), (dict(ko=D_), "overlap"), (dict(ko=C_), "cos or sin"), (dict(qo=None), "q_out"),
-    (dict(qo=A, qs=I4(768, 64, 256, 1)), "overlap"), (dict(wq=D_), "weight")])
+    (dict(qo=A, qs=I4(768, 64, 256, 1)), "overlap"), (dict(wq=D_), "weight"), (dict(batch=1 << 13, n=1 << 13), "too large")])
 def test_norm_rope(kw, says):
     assert says in _norm(**kw)
 

@@ -1679,7 +1679,7 @@ static int norm_rope_check(const char *what, const void *q, const void *k, float
     TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "%s: dtype must be F32 or F16", what);
     TROCM_REQUIRE(batch >= 0 && q_heads >= 0 && kv_heads >= 0 && n >= 0 && head_dim >= 0, "%s: negative dimension", what);
     TROCM_REQUIRE(head_dim % 2 == 0, "%s: the head dimension must be even (got %lld)", what, (long long)head_dim);
-    TROCM_REQUIRE(head_dim < (1 << 24) && n < (1ll << 31) && q_heads + kv_heads <= 65535 && batch < (1ll << 31) && batch * n < (1ll << 31), "%s: tensor too large", what);
+    TROCM_REQUIRE(head_dim < (1 << 24) && n < (1ll << 31) && q_heads + kv_heads <= 65535 && batch < (1ll << 31) && batch * n < (1ll << 26), "%s: tensor too large", what);
     TROCM_REQUIRE(eps >= 0.0f, "%s: eps must be >= 0", what);
     TROCM_REQUIRE(cs_stride_b == 0 || cs_stride_b >= n * head_dim, "%s: cos / sin rows of one sequence overlap the next one's (batch stride %lld < %lld)",
                   what, (long long)cs_stride_b, (long long)(n * head_dim));

@@ -174,7 +174,6 @@ int launch_qk_norm_rope(const QkNormRopeArgs &a, hipStream_t s) {
         }
         vec = vec && (uintptr_t)a.x[i] % 16 == 0 && (uintptr_t)a.w[i] % 16 == 0 && (uintptr_t)a.y[i] % 16 == 0;
     }
-    TROCM_REQUIRE(p.n_tok < (1ll << 31) && a.H[0] + a.H[1] <= 65535, "qk_norm_rope: tensor too large");
     const int64_t lanes = vec && a.D % (2 * vw) == 0 ? a.D / (2 * vw) : 0;
     if (a.dtype == TROCM_F16 && lanes == 4) launch_heads<_Float16, 4>(p, s);
     else if (a.dtype == TROCM_F16 && lanes == 8) launch_heads<_Float16, 8>(p, s);

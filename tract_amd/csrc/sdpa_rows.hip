@@ -51,7 +51,7 @@ struct RowsDev {
     const char *k, *v;
     int64_t stride_b, stride_h, stride_t;
     int regular;                // 0: table of entries, 1: table of lengths, 2: every sequence has Sk keys
-    int Sk, own_splits, own_row_tiles, own_tiles, seq0, n_seq;
+    int Sk, own_splits, own_row_tiles, own_tiles, seq0, items;   // items: of this launch
     float scale, cap;
     int causal;
     const float *slopes;        // [Hq]
@@ -888,7 +888,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
     __shared__ uint16_t s_list[SCORED ? kListMax : 1];
     __shared__ int s_counts[kWaves];
     __shared__ uint32_t s_done;
-    int item = blockIdx.y;
+    int item = blockIdx.y + blockIdx.z * gridDim.y;   // (z: a grid's y has 65535 places)
+    if (item >= p.items) return;
     bool there = false;   // the work is done
     RowsWork wk;
     wk.kvh = blockIdx.x;   // (consecutive workgroups go to the 8 XCDs in turn: a kv head's keys meet in few L2 caches)
@@ -1046,7 +1047,7 @@ namespace {
 template <typename T, int D, int PRE, int OWN, bool SCORED, bool ONCE>
 int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
     RowsDev &p = call.p;
-    const int64_t prefix_items = (int64_t)p.p_splits * p.p_row_tiles, per_seq = (int64_t)p.own_row_tiles * p.own_splits, most = 65535;
+    const int64_t prefix_items = (int64_t)p.p_splits * p.p_row_tiles, per_seq = (int64_t)p.own_row_tiles * p.own_splits, most = 1 << 30, in_y = 65535;
     int64_t holds = table_holds(a);   // sequences of a launch
     if (per_seq && holds > (most - prefix_items) / per_seq) holds = (most - prefix_items) / per_seq;
     TROCM_REQUIRE(holds > 0 && prefix_items <= most, "attention: too many workgroups");
@@ -1055,9 +1056,9 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
         fill_table(a, b, n, call.tab);
         p.seq0 = (int)b;
         p.p_items = b == 0 ? (int)prefix_items : 0;
-        const int64_t items = p.p_items + n * p.own_row_tiles * p.own_splits;
-        if (items == 0) continue;
-        hipLaunchKernelGGL((sdpa_rows_kernel<T, D, PRE, OWN, SCORED, ONCE>), dim3((unsigned)a.Hkv, (unsigned)items), dim3(kThreads), 0, s, call);
+        p.items = (int)(p.p_items + n * per_seq);
+        if (p.items == 0) continue;
+        hipLaunchKernelGGL((sdpa_rows_kernel<T, D, PRE, OWN, SCORED, ONCE>), dim3((unsigned)a.Hkv, (unsigned)(p.items < in_y ? p.items : in_y), (unsigned)((p.items + in_y - 1) / in_y)), dim3(kThreads), 0, s, call);
         if (check_launch("sdpa_rows")) return 1;
     }
     if (p.splits > 1 && !p.counters) {
@@ -1241,7 +1242,7 @@ int launch_sdpa_rows(const SdpaRowsArgs &a, hipStream_t s) {
     RowsDev &p = call.p;
     fill_rows(a, p);
     TROCM_REQUIRE(a.D <= kAnyMaxD, "attention: head_dim %lld is above %d", (long long)a.D, kAnyMaxD);
-    TROCM_REQUIRE(a.Hq * a.Sq < (1ll << 31), "attention: too many query rows per sequence");
+    TROCM_REQUIRE(a.Hq * a.Sq < (1ll << 24), "attention: too many query rows per sequence");   // (a launch has fewer than 2^32 threads)
     const int64_t holds = table_holds(a), step = holds < 65535 ? holds : 65535;
     for (int64_t b = 0; b < a.B; b += step) {
         const int64_t n = a.B - b < step ? a.B - b : step;

@@ -59,7 +59,7 @@ class QkNormRope:
             q_weight, k_weight = (None if w is None else _as_device(w, stream) for w in (q_weight, k_weight))
         dtype, shape, k_shape = q.dtype, q.shape, k.shape
         # (A decode step's call takes the device 3.4 us: shapes and types are looked into where they are not the last call's.)
-        key = (shape, k_shape, cos.shape, sin.shape, q_strides, k_strides, dtype, k.dtype, cos.dtype, sin.dtype,
+        key = (shape, k_shape, cos.shape, sin.shape, q_strides and tuple(q_strides), k_strides and tuple(k_strides), dtype, k.dtype, cos.dtype, sin.dtype,
                q_weight is None or (q_weight.shape, q_weight.dtype), k_weight is None or (k_weight.shape, k_weight.dtype))
         if key != self._key:
             for t in (k, q_weight, k_weight, cos, sin):
