@@ -7,9 +7,16 @@
 // has rows.  The formulation is the transposed one of the other MFMA kernels, S^T = K Q^T and O^T = V^T P^T: every softmax
 // scalar of a row sits in one lane.
 //
-// Work item = (kv head, tile of 32 RB rows, range of keys); a workgroup of 4 waves takes one.  The waves take the range's
-// tiles of 32 keys in turn, each with a private K and V tile in LDS and the next one in flight in registers: no barrier in
-// the loop.  Waves are joined through LDS, ranges through the workspace (partial rows of f32: unnormalised O, maximum, sum).
+// Work item = (kv head, tile of 16 or 32 rows, part of the keys); a workgroup of 4 waves takes one.  The waves take the part's
+// tiles of 32 keys in turn, each with private tiles in LDS and the next one in flight in registers: no barrier in the loop.  A long prefix
+// under many rows of f16 takes tiles of 128 rows, whose four waves share each tile of 64 keys.  Waves are joined through LDS, parts
+// through the workspace (partial rows of f32: unnormalised O, maximum, sum), by the last workgroup to arrive or a launch after it.
+//
+// What bounds it, and what it takes (f16, 8 kv heads of 128 features unless said otherwise): HBM where rows are few, 8 x 8193 keys
+// under 4 rows 45.6 us (5.9 TB/s; a copy's rate is 5.2), 16 x 6000 65 us (6.0 TB/s); HBM and the f32 parts behind a prefix, 64 sequences of 64 to 512
+// keys behind 8192 under 4 rows each 32 us for 109 MB and 27 MB of parts written and read, 200 of up to 300 behind 1500 of 64 features
+// under 8 rows each 24 us; the chain of a launch where it is short, 4 x 40 keys behind 777 8.5 us.  f32: 16 sequences of up to 600 keys behind
+// 4096, 32 kv heads of 64 features, 35 us for 146 MB; f32 chunks are bound by the f32 matrix instructions of one wave per SIMD.
 #include <hip/hip_fp16.h>
 #include <limits.h>
 #include <stddef.h>
@@ -286,9 +293,9 @@ __device__ __forceinline__ int list_document_tiles(const int *docs, int n_keys, 
 }
 
 // A tile of 16 or 32 rows, R of them; the four waves take the range's key tiles in turn.
-//   R == 16: 16x16 MFMAs.  K goes straight from memory into fragments (four lanes read 64 consecutive bytes of a key's row), V
-//            through a wave-private LDS tile.
-//   R == 32: 32x32 MFMAs, K and V through a wave-private LDS tile.
+//   R == 16: 16x16 MFMAs; R == 32: 32x32.  V goes through a wave-private LDS tile, and so does K but for 16 rows of f32, where it goes
+//   straight from memory into fragments (four lanes read 64 consecutive bytes of a key's row; the tiles of two workgroups fit a compute
+//   unit's LDS then).  K through LDS | straight: f16, 8 x 8193 keys 52.8 | 60.4 us; f32, 4 x 5000 keys 54.0 | 47.4 us.
 template <typename T, int D, int R, bool SCORED, bool ONCE>
 __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, unsigned char *lds, uint16_t *s_list, int *s_counts) {
     constexpr bool H16 = sizeof(T) == 2;
@@ -1088,7 +1095,7 @@ int launch_tiles_of(const SdpaRowsArgs &a, RowsCall &call, int pre, int own, boo
         if (pre == 128) return own == 32 ? launch_tiles<T, D, 128, 32, false, false>(a, call, s) : launch_tiles_16<T, D, 128, false>(a, call, once, s);
     if constexpr (sizeof(T) == 2 || D == 128)
         if (own == 32) return launch_tiles<T, D, 32, 32, false, false>(a, call, s);
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2 && D == 128)
         if (pre == 32) return launch_tiles_16<T, D, 32, false>(a, call, once, s);
     return launch_tiles_16<T, D, 16, false>(a, call, once, s);
 }
@@ -1114,8 +1121,8 @@ int64_t tiles_of_a_part(int64_t units, int64_t all, int64_t es, int64_t D) {
 // What a call is expected to take (us) with `pn` parts of the prefix and `on` of the own keys.  A workgroup takes `start` and a round, a
 // tile for each of its waves, `p_round` or `o_round`.  The call takes the longest workgroup and some more where not all run at once; or
 // what memory needs for the keys and parts, and the last one's tail; or the workgroups' rounds over all that run at once; and the join.  The
-// constants were fitted to 370 measured choices of 42 calls (f16 and f32, 64 and 128 features, 1 to 200 sequences, prefixes of 0 to
-// 30000 keys), of which it picks one within 2 % of the best on average and 17 % at worst.
+// constants were fitted to 767 measured choices of 46 calls (f16 and f32, 64 and 128 features, 1 to 200 sequences, prefixes of 0 to
+// 30000 keys), of which it picked one within 2 % of the best on average and 15 % at worst.
 struct RowsCost {
     int64_t kv_heads, units, p_row_tiles, p_all, own_all;   // units: rows' tiles of all sequences, over own keys
     int pre, own;
@@ -1157,10 +1164,18 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     if (!ok || (a.P == 0 && longest == 0)) return 2;
 
     const bool is_scored = a.softcap > 0.0f || a.slopes || a.documents || a.prefix_lens;
+    // Rows of a tile over own keys, where a sequence has more than 16 (tiles of 16 | 32, us).  f16: 6 queries of 4 heads a kv head behind 5000 keys
+    // 27.7 | 22.9, 40 behind 8000 36.5 | 27.0, 300 of 64 features 10.0 | 8.5.  f32 of 128 features: 333 behind 1000 in documents 51.4 | 48.6,
+    // without 108 | 118, 500 45.7 | 41.1, 10 behind 8000 41.6 | 35.2; of 64: 900 27.9 | 35.5, 10 behind 8000 23.9 | 28.0.
     const int own = seq_rows <= 16 || (es == 4 && a.D == 64) ? 16 : 32;
     const int64_t room = a.workspace && aligned(a.workspace) && a.workspace_bytes > kWsCounterBytes + kWsPlanBytes + 256
                              ? (int64_t)(a.workspace_bytes - kWsCounterBytes - kWsPlanBytes - 256) / ((a.D + 2) * (int64_t)sizeof(float)) / rows_all : 0;
-    const int pre = a.P == 0 || es == 4 ? own : rows > 64 && a.P > kTallTile && room >= 2 && a.scale > 0.0f ? 128 : rows > 16 ? 32 : own;   // (the tall body stores parts only)
+    // Rows of a tile over the prefix.  f16: 128 from so many rows times keys on; under that 32 at 128 features, 16 at 64.  (16 | 32 | 128 rows,
+    // us, 128 features: 64 rows over 8192 keys 18.8 | 16.1 | 17.9, 256 over 2500 18.8 | 15.0 | 17.5, 256 over 8192 39 | 28.5 | 24.7, 1024 over 700 37 |
+    // 25.1 | 25.7, 1024 over 8192 113 | 82 | 60; 64 features: 40 over 700 7.3 | 9.8 | 10.1, 80 over 4000 10.5 | 14.1 | 11.6, 320 over 700 10.4 | 10.9 |
+    // 10.9, 160 over 4000 13.8 | 15.9 | 12.4, 1600 over 1500 33 | 30 | 24.)  The tall body stores parts only and takes the largest product for the largest score.
+    const bool tall = es == 2 && rows > 32 && a.P > kTallTile && room >= 2 && a.scale > 0.0f && rows * a.P > (a.D == 128 ? 1150000 : 450000);
+    const int pre = a.P == 0 || es == 4 ? own : tall ? 128 : rows > 16 && (a.D == 128 || own == 32) ? 32 : own;
     RowsCall call;
     RowsDev &p = call.p;
     fill_rows(a, p);
@@ -1177,10 +1192,10 @@ int launch_sdpa_rows_tiles(const SdpaRowsArgs &a, hipStream_t s) {
     cost.slots = cus * (a.D == 64 ? 3 : f32 && (own == 32 || pre == 32) ? 1 : 2);
     cost.bytes_us = (double)((own_tiles_all + p_all * (p_tile / kTile)) * kTile * a.Hkv) * (double)(a.D * es * 2) / 5e6;
     cost.part_mb = (double)rows_all * (double)(a.D + 2) * 4e-6;
-    // Joined by the last to arrive where that is at most two rows for a group of D / 4 lanes: 4 x 777 + 40 keys 9.5 -> 8.5 us, but
-    // 16 x 2000 + 600 keys, whose tiles over the prefix hold four rows for each, 13.5 -> 19.3 us.
+    // Joined by the last to arrive where that is at most 16 rows: 4 x 777 + 40 keys 9.5 -> 8.5 us; but 16 x 2000 + 600 keys in tiles of 32 rows
+    // over the prefix 13.5 -> 19.3 us, 10 x 4000 + 50 of 64 features 10.4 -> 14.
     const int64_t joined = a.P ? (rows < pre ? rows : pre) : own, units = a.Hkv * (p.own_row_tiles ? a.B * p.own_row_tiles : p.p_row_tiles);
-    cost.merged = pre == 128 || joined * a.D > 2048 || units > (int64_t)(kWsCounterBytes / sizeof(int));
+    cost.merged = joined > 16 || units > (int64_t)(kWsCounterBytes / sizeof(int));
     const int64_t p_most = a.P ? (pre == 128 ? p_all : (p_all + kWaves - 1) / kWaves) : 0, o_most = longest ? (own_all + kWaves - 1) / kWaves : 0;
     static const int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
     const int64_t p_least = pre == 128 && o_most == 0 ? 2 : 1, parts_most = room < 64 ? room : 64;
