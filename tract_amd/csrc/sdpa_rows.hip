@@ -14,9 +14,9 @@
 //
 // What bounds it, and what it takes (f16, 8 kv heads of 128 features unless said otherwise): HBM where rows are few, 8 x 8193 keys
 // under 4 rows 45.6 us (5.9 TB/s; a copy's rate is 5.2), 16 x 6000 65 us (6.0 TB/s); HBM and the f32 parts behind a prefix, 64 sequences of 64 to 512
-// keys behind 8192 under 4 rows each 32 us for 109 MB and 27 MB of parts written and read, 200 of up to 300 behind 1500 of 64 features
+// keys behind 8192 under 4 rows each 32 us for 118 MB and 28 MB of parts written and read, 200 of up to 300 behind 1500 of 64 features
 // under 8 rows each 24 us; the chain of a launch where it is short, 4 x 40 keys behind 777 8.5 us.  f32: 16 sequences of up to 600 keys behind
-// 4096, 32 kv heads of 64 features, 35 us for 146 MB; f32 chunks are bound by the f32 matrix instructions of one wave per SIMD.
+// 4096, 32 kv heads of 64 features, 35 us for 134 MB; f32 chunks are bound by the f32 matrix instructions of one wave per SIMD.
 #include <hip/hip_fp16.h>
 #include <limits.h>
 #include <stddef.h>
