@@ -16,7 +16,7 @@
 // under 4 rows 45.6 us (5.9 TB/s; a copy's rate is 5.2), 16 x 6000 65 us (6.0 TB/s); HBM and the f32 parts behind a prefix, 64 sequences of 64 to 512
 // keys behind 8192 under 4 rows each 32 us for 118 MB and 28 MB of parts written and read, 200 of up to 300 behind 1500 of 64 features
 // under 8 rows each 24 us; the chain of a launch where it is short, 4 x 40 keys behind 777 8.5 us.  f32: 16 sequences of up to 600 keys behind
-// 4096, 32 kv heads of 64 features, 35 us for 134 MB; f32 chunks are bound by the f32 matrix instructions of one wave per SIMD.
+// 4096, 32 kv heads of 64 features, 31.5 us for 134 MB; f32 chunks are bound by the f32 matrix instructions of one wave per SIMD.
 #include <hip/hip_fp16.h>
 #include <limits.h>
 #include <stddef.h>
@@ -1076,13 +1076,13 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
     return 0;
 }
 
-// ONCE where it pays, for 16 f16 rows: keys that one workgroup reads, and that are more than the 256 MB behind the L2 caches keep from call to
-// call.  (Through the caches | past them, us: 8 x 8193 keys of 8 x 128 features 50.3 | 45.6, 16 x 6000 73.5 | 64.5, 64 x 8192 + 512
-// 35.7 | 32.3; but 64 x 512 17.3 | 18.2, one sequence of 8193 14.4 | 15.2.  f32 keys, read in pieces of 64 bytes: 16 x 4096 + 600 35.1 | 37.2.)
+// ONCE where it pays, for tiles of 16 rows: keys that one workgroup reads, and that are more than the 256 MB behind the L2 caches keep from call
+// to call.  (Through the caches | past them, us: 8 x 8193 keys of 8 x 128 features 50.3 | 45.6, 16 x 6000 73.5 | 65.1, 64 x 8192 + 512 35.7 | 32.1;
+// but 64 x 512 17.3 | 18.2, one sequence of 8193 14.4 | 15.2.  f32, where it is the values alone, since a key's row is read in pieces of 64
+// bytes: 16 x 4096 + 600 35.5 | 31.5, 4 x 5000 capped 38.0 | 35.5; with the keys as well 37.2.)
 template <typename T, int D, int PRE, bool SCORED>
 int launch_tiles_16(const SdpaRowsArgs &a, RowsCall &call, bool once, hipStream_t s) {
-    if constexpr (sizeof(T) == 2)
-        if (once) return launch_tiles<T, D, PRE, 16, SCORED, true>(a, call, s);
+    if (once) return launch_tiles<T, D, PRE, 16, SCORED, true>(a, call, s);
     return launch_tiles<T, D, PRE, 16, SCORED, false>(a, call, s);
 }
 
