@@ -89,6 +89,21 @@ def test_unusual_scales_where_rows_fill_the_card(rt):
     _check(F16, 1, 32, 8, 1000, 1000, 128, slopes=_slopes(32), causal=False)
 
 
+@pytest.mark.parametrize("dtype,b,hq,hkv,t,d", [(F16, 4, 32, 8, 8200, 128), (F16, 7, 16, 8, 8200, 64), (F32, 2, 32, 8, 8200, 128), (F32, 4, 8, 8, 8200, 64)])
+def test_single_tokens_over_more_keys_than_caches_hold(rt, dtype, b, hq, hkv, t, d):
+    rng = np.random.default_rng(22)
+    q, k, v = _rows(rng, (b, hq, 1, d), dtype, 4.0), _rows(rng, (b, hkv, t, d), dtype), _rows(rng, (b, hkv, t, d), dtype)
+    ids = _packed(rng, b, t, 3)
+    device = [ta.DeviceTensor.from_numpy(x) for x in (q, k, v)]
+    for rules in ({}, {"slopes": _slopes(hq) * 1e-2}, {"documents": ids}):
+        got = ta.ScoredSdpa(softcap=30.0).eval(*device, **rules).to_numpy()
+        for i, h in zip(rng.integers(0, b, 8), rng.integers(0, hq, 8)):
+            some = {x: y[i : i + 1] if x == "documents" else y[h : h + 1] for x, y in rules.items()}
+            g = h * hkv // hq
+            want = scored(q[i : i + 1, h : h + 1], k[i : i + 1, g : g + 1], v[i : i + 1, g : g + 1], cap=30.0, **some)
+            assert_within(got[i : i + 1, h : h + 1], *want, what=f"{list(rules)}, batch {i}, head {h}")
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_more_tiles_of_rows_than_one_axis_of_a_grid_has_places(rt, dtype):
     """Over a few keys, where every row is a row of its own in 64 bits too: those at both ends and about tile 65535 of 16 and of 32 rows."""

@@ -59,6 +59,24 @@ def test_many_and_long(rt, dtype, n, hq, hkv, p, longest, d):
     assert_within(got.to_numpy(), *_want(*case, lens))
 
 
+@pytest.mark.parametrize("dtype,n,hq,hkv,p,longest,d", [
+    (F16, 3, 32, 8, 30000, 50, 128), (F16, 10, 32, 8, 27000, 90, 128), (F16, 64, 32, 8, 6000, 700, 128), (F16, 1, 64, 8, 60000, 9, 64), (F16, 40, 64, 8, 6000, 2800, 64),
+    (F32, 3, 32, 8, 15000, 50, 128), (F32, 20, 8, 8, 2000, 900, 64), (F32, 70, 32, 8, 800, 500, 128)])
+def test_more_keys_than_caches_hold(rt, dtype, n, hq, hkv, p, longest, d):
+    """100 MB of keys and more; some heads of some sequences against 64 bits, all of a second call against the first."""
+    rng = np.random.default_rng(21)
+    lens = [int(x) for x in rng.integers(longest // 2, longest, n, endpoint=True)]
+    q, pk, pv, k, v = case = _case(rng, lens, hq, hkv, p, 1, d, dtype)
+    device = [ta.DeviceTensor.from_numpy(t) for t in case]
+    op = ta.SharedPrefixSdpa()
+    got = op.eval(*device, lens).to_numpy()
+    for i, h in zip(rng.integers(0, n, 12), rng.integers(0, hq, 12)):
+        g = h * hkv // hq
+        want = shared(q[i : i + 1, h : h + 1], pk[0, g : g + 1], pv[0, g : g + 1], [k[i, g : g + 1, : lens[i]]], [v[i, g : g + 1, : lens[i]]])
+        assert_within(got[i : i + 1, h : h + 1], *want, what=f"sequence {i}, head {h}")
+    assert op.eval(*device, lens).to_numpy().tobytes() == got.tobytes()
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_not_causal_scale_strides_and_small_workspaces(rt, dtype):
     rng = np.random.default_rng(3)
