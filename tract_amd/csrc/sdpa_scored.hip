@@ -140,25 +140,28 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
             for (int x = 0; x < kWaves; x++) dmin = min(dmin, s_range[0][x]), dmax = max(dmax, s_range[1][x]);
             const int one_doc = dmin == dmax ? dmin : INT_MIN, dlow = max(dmin, 0);   // (no tile is whole of what is no document)
-            // A wave looks at a tile at a time, a token per lane, at 16 of them before the waves compare.
+            // A wave looks at four tiles at a time, four tokens per lane, at 16 of them before the waves compare.
             constexpr int PW = 16;
             int n = 0;
             for (int t0 = 0; t0 < t_end; t0 += NK * kWaves * PW) {
                 const int first = t0 + wave * PW;
                 const uint32_t there = first >= t_end ? 0 : (1u << min(PW, t_end - first)) - 1;
                 uint32_t active = 0, whole = 0;
-#pragma unroll 1
-                for (int x0 = 0; x0 < PW; x0 += 8) {   // (eight loads in flight; more of them, or their masks at once, spill scalar registers)
-                    int ids[8];
+                struct alignas(4) Ids { int e[4]; } ids[PW / 4];
 #pragma unroll
-                    for (int x = 0; x < 8; x++) ids[x] = docs[min((first + x0 + x) * kTile + lane, p.Sk - 1)];
-                    uint32_t a8 = 0, w8 = 0;
+                for (int x = 0; x < PW / 4; x++)   // (past the last token: the last four again, which may only make a tile look at more)
+                    ids[x] = *reinterpret_cast<const Ids *>(docs + min((first + 4 * x) * kTile + 4 * lane, p.Sk - 4));
 #pragma unroll
-                    for (int x = 0; x < 8; x++) {
-                        a8 |= __builtin_amdgcn_ballot_w64(ids[x] >= dlow && ids[x] <= dmax) != 0 ? 1u << x : 0;
-                        w8 |= __builtin_amdgcn_ballot_w64(ids[x] != one_doc) == 0 ? 1u << x : 0;
+                for (int x = 0; x < PW / 4; x++) {
+                    bool in = false, other = false;
+#pragma unroll
+                    for (int y = 0; y < 4; y++) in = in || (ids[x].e[y] >= dlow && ids[x].e[y] <= dmax), other = other || ids[x].e[y] != one_doc;
+                    const uint64_t a = __builtin_amdgcn_ballot_w64(in), o = __builtin_amdgcn_ballot_w64(other);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        active |= ((a >> 16 * y) & 0xffff) != 0 ? 1u << (4 * x + y) : 0;
+                        whole |= ((o >> 16 * y) & 0xffff) == 0 ? 1u << (4 * x + y) : 0;
                     }
-                    active |= a8 << x0, whole |= w8 << x0;
                 }
                 active &= there;
                 if (lane == 0) s_counts[wave] = __popc(active);
@@ -398,7 +401,7 @@ int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     if (!aligned(a.q) || !aligned(a.out) || !aligned(a.k) || !aligned(a.v) || a.stride_b % 8 || a.stride_h % 8 || a.stride_t % 8 || a.stride_t * 2 > (1 << 25)) return 2;
     if (rows >= (1 << 30)) return 2;
     const int64_t row_tiles = (rows + kRows - 1) / kRows, grid = a.B * a.Hkv * row_tiles;
-    if (rows <= 32 || a.B > 65535 || row_tiles > 65535) return 2;
+    if (rows <= 32 || a.B > 65535 || row_tiles > 65535 || (a.documents && a.Sk < 4)) return 2;   // (four documents' ids in a load)
     // Up to two workgroups per compute unit (one, where documents leave them unlike work) take their tiles in two groups of waves.
     // Fewer tiles still go faster as tiles of 32 rows whose four waves share the keys (sdpa_rows.hip), which take about 1.5 times as long
     // per product but are four times as many.  What either takes, in us: a start, then the longest workgroup's tiles of 64 keys, or all
