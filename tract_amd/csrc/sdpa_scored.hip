@@ -12,8 +12,8 @@
 // What bounds it: the sum of a SIMD's vector and matrix streams, which take turns.  4096 queries of 32 heads over 8, 128 features, capped: 189.5 us
 // (725 TFLOP/s of visible products; a large product alone reaches 1176), vector instructions 57 % of the cycles and matrix instructions 33 %.  Per
 // 64 scores the cap takes two of the three exponentials and reciprocals (8 cycles each) and three of the eight other instructions (4).
-// 64 heads of 64 features 219 us.  Two batches of 4096 in 9 documents, 14 heads over 2, 64 features, with slopes: 53 us; there the compute
-// units have unlike shares (on average 27 tiles, 49 at most) and a workgroup's look at the documents takes 3 to 4 us.
+// 64 heads of 64 features 219 us.  Two batches of 4096 in 9 documents, 14 heads over 2, 64 features, with slopes: 52.6 us; there the compute
+// units have unlike shares (on average 27 tiles, 49 at most); in 40 documents, where a workgroup's start and end are most of it, 23.4 us.
 #include <hip/hip_fp16.h>
 #include <limits.h>
 #include <string.h>
@@ -117,14 +117,26 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
         if (DOCS) id_pre = docs[k_lo + min(lane, most)];
     };
     // The last tile first, that of the rows' own tokens: it is asked for before anything is known of the documents.
+    // (So are the queries and the first ids: one latency for all.)
     const int guess = t_end - 1 - kg;
+    constexpr int PW = 16;   // tiles whose ids a wave looks at before the waves compare: four at a time, four tokens per lane
+    struct alignas(4) Ids { int e[4]; } ids[DOCS ? PW / 4 : 1];
+    auto ask_ids = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < PW / 4; x++)   // (past the last token: the last four again, which may only make a tile look at more)
+            ids[x] = *reinterpret_cast<const Ids *>(docs + min((first + 4 * x) * kTile + 4 * lane, p.Sk - 4));
+    };
+    const int doc = DOCS ? docs[at] : 0;
+    if constexpr (DOCS) ask_ids(wave * PW);
     if (guess >= 0) prefetch(guess * kTile);
+    half8_t qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = *reinterpret_cast<const half8_t *>(p.q + out_row * (2 * D) + 32 * ks + 16 * hb);
 
     // A score in the log2 domain is base + to_log2 s, of s the product with the key or, capped, 1 / (e^2x + 1) with x = scale q.k / cap:
     // cap log2e tanh(x) = A - 2 A / (e^2x + 1).  The largest score is the smallest s there.  Only weights take the whole sum.
     const float base = CAP ? p.cap * kLog2e : 0.0f, to_log2 = CAP ? -2.0f * base : p.scale * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
     const float hidden = CAP ? INFINITY : -INFINITY, slope = SLOPES ? -kLog2e / to_log2 * p.slopes[kvh * p.G + g] : 0.0f;
-    const int doc = DOCS ? docs[at] : 0;
     if (DOCS && doc < 0) lim = -1;   // padding sees nothing
     bool listed = false;
     if constexpr (DOCS) {
@@ -140,17 +152,12 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
             for (int x = 0; x < kWaves; x++) dmin = min(dmin, s_range[0][x]), dmax = max(dmax, s_range[1][x]);
             const int one_doc = dmin == dmax ? dmin : INT_MIN, dlow = max(dmin, 0);   // (no tile is whole of what is no document)
-            // A wave looks at four tiles at a time, four tokens per lane, at 16 of them before the waves compare.
-            constexpr int PW = 16;
             int n = 0;
             for (int t0 = 0; t0 < t_end; t0 += NK * kWaves * PW) {
                 const int first = t0 + wave * PW;
                 const uint32_t there = first >= t_end ? 0 : (1u << min(PW, t_end - first)) - 1;
                 uint32_t active = 0, whole = 0;
-                struct alignas(4) Ids { int e[4]; } ids[PW / 4];
-#pragma unroll
-                for (int x = 0; x < PW / 4; x++)   // (past the last token: the last four again, which may only make a tile look at more)
-                    ids[x] = *reinterpret_cast<const Ids *>(docs + min((first + 4 * x) * kTile + 4 * lane, p.Sk - 4));
+                if (t0) ask_ids(first);
 #pragma unroll
                 for (int x = 0; x < PW / 4; x++) {
                     bool in = false, other = false;
@@ -204,10 +211,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
     for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int x = 0; x < 16; x++) o[db][x] = 0.0f;
-    half8_t qf[KS];
     if (DOCS && kg < n_tiles && tile_lo(entry(kg)) != guess * kTile) prefetch(tile_lo(entry(kg)));   // (padding, or a prefix)
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) qf[ks] = *reinterpret_cast<const half8_t *>(p.q + out_row * (2 * D) + 32 * ks + 16 * hb);
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));   // settled here, not by a wait in the loop that would take the prefetch in too
     if (kg < n_tiles) {
