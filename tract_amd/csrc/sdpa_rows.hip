@@ -834,7 +834,7 @@ __device__ __forceinline__ void join_row(const float *part_o, const float *part_
 }
 
 // The last workgroup to bring a part of a unit's rows joins them.  A unit is a tile of one sequence's rows (own keys) or, where no
-// sequence has keys of its own, a tile of rows of the prefix; a tile over the prefix holds rows of up to 32 units and brings a
+// sequence has keys of its own, a tile of rows of the prefix; a tile over the prefix holds rows of up to 16 units and brings a
 // part to each.  Counters are zero between launches.
 template <typename T, int D, int PRE, int OWN>
 __device__ __forceinline__ void arrive(const RowsDev &p, const RowsWork &wk, uint32_t *s_done) {
@@ -867,7 +867,7 @@ __device__ __forceinline__ void arrive(const RowsDev &p, const RowsWork &wk, uin
             if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         const uint64_t done = __builtin_amdgcn_ballot_w64(last);
-        if (tid == 0) *s_done = (uint32_t)done;   // (n <= 32)
+        if (tid == 0) *s_done = (uint32_t)done;   // (n <= 16)
     }
     __syncthreads();
     const uint32_t done = *s_done;
@@ -933,7 +933,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && D == 128 && (PRE == 32 
         wk.split = p.p_splits + split;
     }
     if (!there) rows_body<T, D, OWN, SCORED, ONCE>(p, wk, lds, s_list, s_counts);
-    if constexpr (PRE != 128)
+    if constexpr (PRE <= 16 && OWN == 16)   // (parts of more rows are joined by a launch)
         if (p.counters) arrive<T, D, PRE, OWN>(p, wk, &s_done);
 }
 
@@ -1058,6 +1058,7 @@ int launch_tiles(const SdpaRowsArgs &a, RowsCall &call, hipStream_t s) {
     int64_t holds = table_holds(a);   // sequences of a launch
     if (per_seq && holds > (most - prefix_items) / per_seq) holds = (most - prefix_items) / per_seq;
     TROCM_REQUIRE(holds > 0 && prefix_items <= most, "attention: too many workgroups");
+    TROCM_REQUIRE(!p.counters || (PRE <= 16 && OWN == 16), "attention: parts that nothing joins");
     for (int64_t b = 0; b < a.B; b += holds) {   // the prefix, for all rows, with the first sequences' own keys
         const int64_t n = a.B - b < holds ? a.B - b : holds;
         fill_table(a, b, n, call.tab);
