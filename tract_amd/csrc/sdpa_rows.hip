@@ -706,33 +706,44 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
 #pragma unroll
                     for (int x = 0; x < 16; x++) s[kb][x] = 32 * kb + 8 * (x >> 2) + (x & 3) <= last ? s[kb][x] : -INFINITY;
             }
-            float top = s[0][0];
-#pragma unroll
-            for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb][x]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * to_log2;   // (scale > 0: the maximum commutes with it)
-            const bool moved = top > m_run + 8.0f;   // (as above)
-            const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
-            m_run = m_new;
+            // Weights against the reference that the row has.  Only in the first tile, and where a lane's come to 2^15 or more (f16 ends at 2^16), a
+            // look at the maximum: the reference moves where that is more than 8 above it.
             half8_t pf[4];
-            float sum = 0.0f;
-            const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+            float sum;
+            auto weights = [&]() __attribute__((always_inline)) {
+                const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+                sum = 0.0f;
 #pragma unroll
-            for (int st = 0; st < 4; st++) {
+                for (int st = 0; st < 4; st++) {
 #pragma unroll
-                for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, -ref));
+                    for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, -m_run));
 #pragma unroll
-                for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
+                    for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
+                }
+            };
+            bool look = n == 0;
+            if (!look) {
+                weights();
+                look = __builtin_amdgcn_ballot_w64(!(sum < 32768.0f)) != 0;
             }
-            l_run = l_run * keep + sum;
-            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+            if (look) {
+                float top = s[0][0];
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb][x]);
+                top = fmaxf(top, __shfl_xor(top, 32, 64)) * to_log2;   // (scale > 0: the maximum commutes with it)
+                const bool moved = top > m_run + 8.0f;
+                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                m_run = m_new;
+                l_run *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) o[db][x] *= keep;
+                weights();
             }
+            l_run += sum;
             const _Float16 *vsrc = lds_v + buf * V_TILE + (4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
             for (int st = 0; st < 4; st++)

@@ -33,6 +33,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 4, kTile = 64, kRows = 32 * kWaves;   // waves with rows of their own, of each of NK groups
+constexpr float kNone = -1.7e38f;   // the reference of a row that has seen nothing: finite, so that a hidden score stays at minus infinity against it
 constexpr int kListMax = 4096;   // key tiles that documents are looked up for
 
 struct ScoredDev {
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
         }
     };
 
-    float m_run = -INFINITY, l_run = 0.0f;
+    float m_run = kNone, l_run = 0.0f;
     float16_t o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -276,35 +277,46 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 #pragma unroll
                     for (int x = 0; x < 16; x++) s[kb2][x] = 32 * kb2 + 8 * (x >> 2) + (x & 3) <= last ? s[kb2][x] : hidden;
             }
-            float top = s[0][0];
-#pragma unroll
-            for (int kb2 = 0; kb2 < 2; kb2++)
-#pragma unroll
-                for (int x = 0; x < 16; x++) top = CAP ? fminf(top, s[kb2][x]) : fmaxf(top, s[kb2][x]);
-            const float other = __shfl_xor(top, 32, 64);
-            top = __builtin_fmaf(CAP ? fminf(top, other) : fmaxf(top, other), to_log2, base);
-            // the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
-            const bool moved = top > m_run + 8.0f;
-            const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
-            m_run = m_new;
+            // Weights against the reference that the row has.  Only in the first tile, and where a lane's come to 2^15 or more (f16 ends at 2^16), a
+            // look at the maximum: the reference moves where that is more than 8 above it.
             half8_t pf[4];
-            float sum = 0.0f;
-            const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+            float sum;
+            auto weights = [&]() __attribute__((always_inline)) {
+                const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+                const float from = base - m_run;
+                sum = 0.0f;
 #pragma unroll
-            for (int st = 0; st < 4; st++) {
+                for (int st = 0; st < 4; st++) {
 #pragma unroll
-                for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, base - ref));
+                    for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, from));
 #pragma unroll
-                for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
+                    for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
+                }
+            };
+            bool look = !DOCS && n == kg;   // (documents: weights against no reference come to infinity; asked for by place, the first tile spills scalar registers)
+            if (!look) {
+                weights();
+                look = __builtin_amdgcn_ballot_w64(!(sum < 32768.0f)) != 0;
             }
-            l_run = l_run * keep + sum;
-            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+            if (look) {
+                float top = s[0][0];
+#pragma unroll
+                for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) top = CAP ? fminf(top, s[kb2][x]) : fmaxf(top, s[kb2][x]);
+                const float other = __shfl_xor(top, 32, 64);
+                top = __builtin_fmaf(CAP ? fminf(top, other) : fmaxf(top, other), to_log2, base);
+                const bool moved = top > m_run + 8.0f;
+                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                m_run = m_new;
+                l_run *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) o[db][x] *= keep;
+                weights();
             }
+            l_run += sum;
             const _Float16 *vsrc = &lds_v[buf][(4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
 #pragma unroll
             for (int st = 0; st < 4; st++)
@@ -335,8 +347,8 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
         }
         __syncthreads();
         if (kg == 1) return;
-        const float m2 = comb_ml[l32], l2 = comb_ml[32 + l32], mm = fmaxf(m_run, m2), ref = mm == -INFINITY ? 0.0f : mm;
-        const float f1 = __builtin_amdgcn_exp2f(m_run - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+        const float m2 = comb_ml[l32], l2 = comb_ml[32 + l32], mm = fmaxf(m_run, m2);
+        const float f1 = __builtin_amdgcn_exp2f(m_run - mm), f2 = __builtin_amdgcn_exp2f(m2 - mm);
         l_run = l_run * f1 + l2 * f2;
 #pragma unroll
         for (int db = 0; db < DB; db++)
