@@ -6,6 +6,8 @@
   ``inplace_kv_sdpa_eval_shared`` is the same over caches, with the append of a step
 * ``ScoredSdpa``        Sdpa (transformers/src/ops/sdpa.rs:83-89) whose scores are capped by a tanh, fall with the distance,
   stay inside documents or see a prefix
+
+An object keeps its workspace from call to call: its calls follow each other on one stream.
 """
 from __future__ import annotations
 
