@@ -104,6 +104,27 @@ def test_single_tokens_over_more_keys_than_caches_hold(rt, dtype, b, hq, hkv, t,
             assert_within(got[i : i + 1, h : h + 1], *want, what=f"{list(rules)}, batch {i}, head {h}")
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_whose_maximum_rises_late_and_rows_that_are_not_numbers(rt, d):
+    """Scores that grow along the keys and against them, far apart, all alike; a query row of NaN is the only one that shows it."""
+    rng = np.random.default_rng(23)
+    b, hq, hkv, n = 1, 64, 8, 1000
+    q, k, v = _rows(rng, (b, hq, n, d), F16, 40.0), _rows(rng, (b, hkv, n, d), F16), _rows(rng, (b, hkv, n, d), F16)
+    for growth in (np.linspace(0.02, 1.5, n), np.linspace(1.5, 0.02, n), np.zeros(n), np.where(np.arange(n) % 331 == 330, 3.0, 0.05)):
+        kk = (k * growth[None, None, :, None]).astype(F16)
+        for rules in ({}, {"slopes": _slopes(hq)}, {"documents": _packed(rng, b, n, 4)}):
+            got = ta.ScoredSdpa().eval(q, kk, v, **rules).to_numpy()
+            assert_within(got[:, 3:40:9], *scored(q[:, 3:40:9], kk[:, [3 * hkv // hq, 12 * hkv // hq, 21 * hkv // hq, 30 * hkv // hq, 39 * hkv // hq]],
+                                                  v[:, [3 * hkv // hq, 12 * hkv // hq, 21 * hkv // hq, 30 * hkv // hq, 39 * hkv // hq]],
+                                                  **{x: y[3:40:9] if x == "slopes" else y for x, y in rules.items()}))
+    plain = ta.ScoredSdpa(softcap=30.0).eval(q, k, v).to_numpy()
+    q[0, 5, 700] = np.nan
+    got = ta.ScoredSdpa(softcap=30.0).eval(q, k, v).to_numpy()
+    assert np.isnan(got[0, 5, 700]).all()
+    got[0, 5, 700] = plain[0, 5, 700]
+    assert got.tobytes() == plain.tobytes()
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_more_tiles_of_rows_than_one_axis_of_a_grid_has_places(rt, dtype):
     """Over a few keys, where every row is a row of its own in 64 bits too: those at both ends and about tile 65535 of 16 and of 32 rows."""

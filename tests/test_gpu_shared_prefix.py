@@ -77,6 +77,20 @@ def test_more_keys_than_caches_hold(rt, dtype, n, hq, hkv, p, longest, d):
     assert op.eval(*device, lens).to_numpy().tobytes() == got.tobytes()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefixes_whose_scores_rise_late(rt, d):
+    rng = np.random.default_rng(24)
+    n, hq, hkv, p = 40, 32, 4, 4000
+    lens = [int(x) for x in rng.integers(0, 90, n)]
+    q, pk, pv, k, v = _case(rng, lens, hq, hkv, p, 1, d, F16)
+    q = (q * 15).astype(F16)
+    for growth in (np.linspace(0.02, 1.5, p), np.linspace(1.5, 0.02, p), np.zeros(p), np.where(np.arange(p) % 1331 == 1330, 3.0, 0.05)):
+        kk = (pk * growth[None, None, :, None]).astype(F16)
+        got = ta.SharedPrefixSdpa().eval(q, kk, pv, k, v, lens).to_numpy()
+        some = list(range(0, n, 13))
+        assert_within(got[some], *_want(q[some], kk, pv, [k[i] for i in some], [v[i] for i in some], [lens[i] for i in some]))
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_not_causal_scale_strides_and_small_workspaces(rt, dtype):
     rng = np.random.default_rng(3)
