@@ -12,7 +12,7 @@ import re
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
-SCALARS = {"int": "c_int", "int64_t": "i64", "size_t": "usize", "float": "f32", "uint64_t": "u64", "unsigned": "c_uint",
+SCALARS = {"int": "c_int", "int64_t": "i64", "size_t": "usize", "float": "f32", "uint64_t": "u64", "int32_t": "i32", "unsigned": "c_uint",
            "void": "c_void", "char": "c_char"}
 RUST_KEYWORDS = {"type", "ref", "in", "move", "match", "loop", "mod", "fn", "use", "box"}
 
@@ -41,6 +41,7 @@ def rust_type(ctype: str) -> str:
     toks = re.findall(r"\*|const|[A-Za-z_][A-Za-z0-9_]*", ctype)
     base = [t for t in toks if t not in ("*", "const")]
     assert len(base) == 1, ctype
+    assert base[0] in SCALARS or base[0].startswith("trocm_"), f"no Rust type is known for {ctype}"
     rust = SCALARS.get(base[0], base[0])   # opaque structs keep their names
     stars = [i for i, t in enumerate(toks) if t == "*"]
     if not stars:

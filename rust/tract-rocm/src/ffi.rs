@@ -117,8 +117,8 @@ extern "C" {
     pub fn trocm_sdpa_shared_workspace_bytes(n_seq: i64, q_heads: i64, q_len: i64, head_dim: i64, bytes: *mut usize) -> c_int;
     pub fn trocm_sdpa_shared_prefix(q: *const c_void, dtype: c_int, n_seq: i64, q_heads: i64, kv_heads: i64, q_len: i64, head_dim: i64, prefix_k: *const c_void, prefix_v: *const c_void, prefix_len: i64, prefix_strides: *const i64, k: *const c_void, v: *const c_void, kv_strides: *const i64, lens: *const i64, out: *mut c_void, scale: f32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn trocm_inplace_kv_sdpa_eval_shared(q: *const c_void, k_new: *const c_void, v_new: *const c_void, dtype: c_int, q_heads: i64, n_seq: i64, n_new: i64, prefix_k_cache: *const trocm_kv_cache, prefix_v_cache: *const trocm_kv_cache, k_caches: *const *mut trocm_kv_cache, v_caches: *const *mut trocm_kv_cache, out: *mut c_void, scale: f32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
-    pub fn trocm_sdpa_scored(q: *const c_void, k: *const c_void, v: *const c_void, out: *mut c_void, dtype: c_int, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, kv_strides: *const i64, scale: f32, softcap: f32, slopes: *const f32, documents: *const int32_t, prefix_lens: *const int32_t, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
-    pub fn trocm_sdpa_cached_scored(q: *const c_void, q_dtype: c_int, q_heads: i64, q_len: i64, k_cache: *const trocm_kv_cache, v_cache: *const trocm_kv_cache, out: *mut c_void, scale: f32, softcap: f32, slopes: *const f32, documents: *const int32_t, prefix_lens: *const int32_t, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn trocm_sdpa_scored(q: *const c_void, k: *const c_void, v: *const c_void, out: *mut c_void, dtype: c_int, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, kv_strides: *const i64, scale: f32, softcap: f32, slopes: *const f32, documents: *const i32, prefix_lens: *const i32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn trocm_sdpa_cached_scored(q: *const c_void, q_dtype: c_int, q_heads: i64, q_len: i64, k_cache: *const trocm_kv_cache, v_cache: *const trocm_kv_cache, out: *mut c_void, scale: f32, softcap: f32, slopes: *const f32, documents: *const i32, prefix_lens: *const i32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
 }
 
 /// KO -> an error that carries the library's message.
