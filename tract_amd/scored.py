@@ -136,12 +136,16 @@ def inplace_kv_sdpa_eval_shared(q: DeviceTensor, k_new, v_new, prefix_k, prefix_
     """One step of `n_seq` sequences that share a prefix: append k_new[i], v_new[i] ([n_seq, Hkv, n_new, D]) to sequence i's
     caches, then attend q[i] ([n_seq, Hq, n_new, D]) over the prefix caches and over its own.  With k_new and v_new None:
     attend to what is there.  A sequence's caches may be new; the prefix caches must have been pushed to."""
+    if len(q.shape) != 4:
+        raise TractRocmError("shared prefix: inputs must be of rank 4")
     n, hq, sq, d = q.shape
     if len(k_caches) != n or len(v_caches) != n:
         raise TractRocmError("shared prefix: one K and one V cache per sequence expected")
     if prefix_k.handle is None or prefix_v.handle is None:
         raise TractRocmError("empty kv-cache")
-    hkv = prefix_k._shape[1]
+    _, hkv, _, cached_d = _canon4(prefix_k._shape)
+    if d != cached_d:   # (all sizes of the call are taken from the caches)
+        raise TractRocmError(f"shared prefix: Q {q.shape} is not of the prefix's head size {cached_d}")
     if k_new is not None or v_new is not None:
         if k_new is None or v_new is None or k_new.shape != (n, hkv, sq, d) or v_new.shape != k_new.shape:
             raise TractRocmError("shared prefix: k_new / v_new must be [n_seq, kv_heads, n_new, head_dim]")
