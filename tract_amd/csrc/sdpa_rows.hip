@@ -192,14 +192,16 @@ __global__ __launch_bounds__(kAnyThreads) void sdpa_rows_any_kernel(RowsCall cal
 
 // ---- new rows into the caches of their sequences ---------------------------------------------------------------------
 
-// k_new, v_new dense [B, Hkv, n, D]; entry b's planes take them from its length on.  A 4-byte word per thread.
-__global__ __launch_bounds__(256) void append_rows_kernel(SeqTable, const uint32_t *__restrict__ k_new, const uint32_t *__restrict__ v_new, int seq0, int Hkv,
+// k_new, v_new dense [B, Hkv, n, D]; entry b's planes take them from its length on.  A word per thread: 4 bytes where rows and addresses
+// are whole ones, else 2.
+template <typename W>
+__global__ __launch_bounds__(256) void append_rows_kernel(SeqTable, const W *__restrict__ k_new, const W *__restrict__ v_new, int seq0, int Hkv,
                                                           int words_per_head, int64_t row_bytes) {
     const int kvh = blockIdx.y, b = seq0 + blockIdx.z;
     const TableWords e = table_words(0) + blockIdx.z * kSeqEntry;
     const int64_t sh = (int64_t)((uint64_t)e[4] | ((uint64_t)e[5] << 32)), at = kvh * sh + (int64_t)(int)e[6] * row_bytes;
-    uint32_t *k = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>((uint64_t)e[0] | ((uint64_t)e[1] << 32)) + at);
-    uint32_t *v = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>((uint64_t)e[2] | ((uint64_t)e[3] << 32)) + at);
+    W *k = reinterpret_cast<W *>(reinterpret_cast<char *>((uint64_t)e[0] | ((uint64_t)e[1] << 32)) + at);
+    W *v = reinterpret_cast<W *>(reinterpret_cast<char *>((uint64_t)e[2] | ((uint64_t)e[3] << 32)) + at);
     const int64_t from = ((int64_t)b * Hkv + kvh) * words_per_head;
     for (int i = blockIdx.x * 256 + threadIdx.x; i < words_per_head; i += gridDim.x * 256) {
         k[i] = k_new[from + i];
@@ -1044,7 +1046,9 @@ size_t sdpa_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Sq, int64_t D)
 }
 
 int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_new, hipStream_t s) {
-    const int64_t row_bytes = a.D * (int64_t)elem_bytes(a.dtype), words = a.Sq * row_bytes / 4;
+    const int64_t row_bytes = a.D * (int64_t)elem_bytes(a.dtype);
+    const bool whole = row_bytes % 4 == 0 && (uintptr_t)k_new % 4 == 0 && (uintptr_t)v_new % 4 == 0;   // (f16 rows of an odd size are not)
+    const int64_t words = a.Sq * row_bytes / (whole ? 4 : 2);
     TROCM_REQUIRE(words < (1 << 30), "append: too many new tokens");
     if (words == 0) return 0;
     const int64_t step = table_holds(a);
@@ -1053,8 +1057,9 @@ int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_n
         SeqTable tab;
         fill_table(a, b, n, tab);
         const int64_t blocks = (words + 255) / 256;
-        hipLaunchKernelGGL(append_rows_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), (unsigned)a.Hkv, (unsigned)n), dim3(256), 0, s, tab,
-                           (const uint32_t *)k_new, (const uint32_t *)v_new, (int)b, (int)a.Hkv, (int)words, row_bytes);
+        const dim3 grid((unsigned)(blocks < 64 ? blocks : 64), (unsigned)a.Hkv, (unsigned)n);
+        if (whole) hipLaunchKernelGGL((append_rows_kernel<uint32_t>), grid, dim3(256), 0, s, tab, (const uint32_t *)k_new, (const uint32_t *)v_new, (int)b, (int)a.Hkv, (int)words, row_bytes);
+        else hipLaunchKernelGGL((append_rows_kernel<uint16_t>), grid, dim3(256), 0, s, tab, (const uint16_t *)k_new, (const uint16_t *)v_new, (int)b, (int)a.Hkv, (int)words, row_bytes);
         if (check_launch("append_rows")) return 1;
     }
     return 0;
