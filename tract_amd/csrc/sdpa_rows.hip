@@ -344,8 +344,8 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
     }
     float *part_ml = p.part_ml + (int64_t)wk.split * 2 * p.part_rows;
     const int first = wk.part * kWaves, step = wk.parts * kWaves;
-    if (n_tiles <= first && p.splits > 1) {   // nothing to add: a maximum of -inf says so
-        if (w == 0 && grp == 0 && wk.row0 + lr < wk.row_end) put(part_ml + out_row, -INFINITY);
+    if (n_tiles <= first && p.splits > 1) {   // nothing to add: a maximum of -inf and a sum of 0 say so
+        if (w == 0 && grp < 2 && wk.row0 + lr < wk.row_end) put(part_ml + out_row + (grp ? p.part_rows : 0), grp ? 0.0f : -INFINITY);
         return;
     }
 
@@ -602,7 +602,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
         l += f[x] * comb_ml[(x * 2 + 1) * R + row];
     }
     const int64_t orow = q_row(p, wk.kvh, r).at;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < PER; e += 2) {
         const int d = (tid % TPR) * 2 + e * TPR;   // (8 bytes per thread, threads of a row side by side: a store covers whole lines)
@@ -780,6 +780,10 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
     }
 }
 
+// Whether a part has keys for a row: one without has a maximum of -inf and a sum of 0 (and rows of zeros, or none at all).  Scores that are all
+// NaN raise no maximum either, but their sum is NaN, which has to come out.
+__device__ __forceinline__ bool part_has(float m, float l) { return m != -INFINITY || l != 0.0f; }
+
 // A row's parts -> its output, by D / 4 lanes of a wave.  Everything that some 8 ranges have is asked for at once: one latency for up to
 // 8 of them.  (At most 64.)
 template <typename T, int D>
@@ -805,7 +809,7 @@ __device__ __forceinline__ void join_row(const float *part_o, const float *part_
     ask(0);
 #pragma unroll
     for (int x = 0; x < MOST; x++) {
-        if (x * LPR + lr >= splits) f[x] = -INFINITY;
+        if (x * LPR + lr >= splits) f[x] = -INFINITY, ls[x] = 0.0f;
         mm = fmaxf(mm, f[x]);
     }
 #pragma unroll
@@ -813,7 +817,7 @@ __device__ __forceinline__ void join_row(const float *part_o, const float *part_
     const float ref = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
     for (int x = 0; x < MOST; x++) {
-        const bool has = f[x] != -INFINITY;   // (a range without keys for the row has stored nothing else)
+        const bool has = part_has(f[x], ls[x]);
         f[x] = has ? __builtin_amdgcn_exp2f(f[x] - ref) : 0.0f;
         l += has ? f[x] * ls[x] : 0.0f;
     }
@@ -837,7 +841,7 @@ __device__ __forceinline__ void join_row(const float *part_o, const float *part_
         }
         if (s0 + BATCH < splits) ask(s0 + BATCH);
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (a sum of NaN comes out)
 #pragma unroll
     for (int z = 0; z < 2; z++) {
         struct alignas(2 * sizeof(T)) Two { T e[2]; } pair;
@@ -960,7 +964,7 @@ __global__ __launch_bounds__(256) void sdpa_rows_merge_kernel(const float *__res
     const int64_t row = min((int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, rows - 1);   // (rows past the last write it again, the same)
     const int mine = min(lane, splits - 1);   // (no more parts than lanes: 64, or 8)
     float f = part_ml[(int64_t)mine * 2 * rows + row];
-    const float ls = part_ml[((int64_t)mine * 2 + 1) * rows + row];
+    float ls = part_ml[((int64_t)mine * 2 + 1) * rows + row];
     const float *po = part_o + row * D + 4 * lr;
     float4_t v[BATCH];
     auto ask = [&](int s0) __attribute__((always_inline)) {
@@ -968,12 +972,12 @@ __global__ __launch_bounds__(256) void sdpa_rows_merge_kernel(const float *__res
         for (int y = 0; y < BATCH; y++) v[y] = *reinterpret_cast<const float4_t *>(po + (int64_t)min(s0 + y * NG + grp, splits - 1) * rows * D);
     };
     ask(0);
-    if (lane >= splits) f = -INFINITY;
+    if (lane >= splits) f = -INFINITY, ls = 0.0f;
     float mm = f;
 #pragma unroll
     for (int w = 1; w < LANES; w <<= 1) mm = fmaxf(mm, __shfl_xor(mm, w, 64));
-    const bool has = f != -INFINITY;   // (a range without keys for the row has stored nothing else)
-    f = has ? __builtin_amdgcn_exp2f(f - mm) : 0.0f;
+    const bool has = part_has(f, ls);
+    f = has ? __builtin_amdgcn_exp2f(f - (mm == -INFINITY ? 0.0f : mm)) : 0.0f;
     float l = has ? f * ls : 0.0f;
 #pragma unroll
     for (int w = 1; w < LANES; w <<= 1) l += __shfl_xor(l, w, 64);
@@ -991,7 +995,7 @@ __global__ __launch_bounds__(256) void sdpa_rows_merge_kernel(const float *__res
     for (int w = LPR; w < LANES; w <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], w, 64);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (a sum of NaN comes out)
     if (grp == 0) {
         struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
 #pragma unroll
