@@ -26,7 +26,8 @@ def _only(got, at, want, bound):
 @pytest.mark.parametrize("lens,hq,hkv,p,sq,d", [
     ([3, 0, 40], 14, 2, 777, 1, 64), ([100, 31, 900], 8, 2, 2000, 1, 128),    # tiles of 16 rows, joined by the last to arrive
     ([9, 70] * 20, 32, 2, 4000, 1, 128), ([9, 70] * 20, 64, 2, 4000, 1, 64),  # f16: tiles of 128 rows over the prefix, joined by a launch
-    ([40, 200], 32, 2, 300, 5, 128), ([5, 0], 8, 1, 700, 6, 64)])             # several queries of a sequence
+    ([40, 200], 32, 2, 300, 5, 128), ([5, 0], 8, 1, 700, 6, 64),              # several queries of a sequence
+    ([5, 2, 300], 6, 3, 400, 1, 80), ([2, 600], 4, 2, 0, 2, 48)])             # head sizes without a kernel of their own
 def test_shared_prefix(rt, dtype, lens, hq, hkv, p, sq, d):
     rng = np.random.default_rng(41)
     n, room = len(lens), max(lens)
@@ -43,7 +44,8 @@ def test_shared_prefix(rt, dtype, lens, hq, hkv, p, sq, d):
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("b,hq,hkv,n,t,d", [
     (2, 8, 2, 1, 5000, 128), (1, 4, 1, 1, 9000, 64), (1, 32, 4, 1, 300, 128),    # single tokens, in parts and whole
-    (1, 8, 2, 6, 5000, 128), (1, 4, 2, 40, 6000, 64), (1, 8, 2, 100, 130, 64)])  # a few queries, a chunk, a prompt
+    (1, 8, 2, 6, 5000, 128), (1, 4, 2, 40, 6000, 64), (1, 8, 2, 100, 130, 64),   # a few queries, a chunk, a prompt
+    (1, 6, 2, 3, 700, 96), (2, 2, 1, 1, 40, 48)])                                # head sizes without a kernel of their own
 @pytest.mark.parametrize("cap,documents", [(0.0, False), (20.0, False), (0.0, True)])
 def test_scored(rt, dtype, b, hq, hkv, n, t, d, cap, documents):
     rng = np.random.default_rng(42)

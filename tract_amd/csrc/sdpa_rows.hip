@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kAnyThreads) void sdpa_rows_any_kernel(RowsCall cal
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
             if (lane == 0) lds_red[kWaves + w] = l;
-            lds_p[tid] = sees ? e : -1.0f;   // (what is hidden is not read: it may hold anything)
+            lds_p[tid] = sees ? e : -1.0f;   // (what is hidden is not read: it may hold anything; a weight of NaN is not hidden)
             __syncthreads();
             l_run = l_run * keep + (lds_red[kWaves] + lds_red[kWaves + 1] + lds_red[kWaves + 2] + lds_red[kWaves + 3]);
             m_run = m_new;
@@ -180,14 +180,14 @@ __global__ __launch_bounds__(kAnyThreads) void sdpa_rows_any_kernel(RowsCall cal
                 float acc = lds_o[d] * keep;
 #pragma unroll 1
                 for (int jj = 0; jj < cnt; jj++)
-                    if (lds_p[jj] >= 0.0f) acc = __builtin_fmaf(lds_p[jj], widen(reinterpret_cast<const T *>(vb + (int64_t)(j0 + jj) * st)[d]), acc);
+                    if (!(lds_p[jj] < 0.0f)) acc = __builtin_fmaf(lds_p[jj], widen(reinterpret_cast<const T *>(vb + (int64_t)(j0 + jj) * st)[d]), acc);
                 lds_o[d] = acc;
             }
             __syncthreads();
         }
     }
     T *out = reinterpret_cast<T *>(p.out) + row * D;
-    for (int d = tid; d < D; d += kAnyThreads) out[d] = (T)(l_run > 0.0f ? lds_o[d] / l_run : 0.0f);
+    for (int d = tid; d < D; d += kAnyThreads) out[d] = (T)(l_run == 0.0f ? 0.0f : lds_o[d] / l_run);
 }
 
 // ---- new rows into the caches of their sequences ---------------------------------------------------------------------
