@@ -514,7 +514,7 @@ int trocm_sdpa_shared_prefix(const void *q, int dtype, int64_t n_seq, int64_t q_
 /* The same over caches: prefix_k_cache and prefix_v_cache (batch 1, may be empty) and one K and one V cache per sequence (batch 1
  * each), F32 or F16, ordinary ones.  With k_new and v_new (dense [n_seq, kv_heads, n_new, head_dim]) it is a step: they are
  * appended to the sequences' caches first, which must all be different; with both NULL it attends to what the caches hold
- * (n_new is then only the number of queries per sequence).  Everything is checked before any cache changes. */
+ * (n_new is then only the number of queries per sequence).  A call that fails leaves the lengths and rows of all caches as they were. */
 int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const void *v_new, int dtype, int64_t q_heads, int64_t n_seq,
                                       int64_t n_new, const trocm_kv_cache *prefix_k_cache, const trocm_kv_cache *prefix_v_cache,
                                       trocm_kv_cache *const *k_caches, trocm_kv_cache *const *v_caches, void *out, float scale,

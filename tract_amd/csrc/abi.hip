@@ -1856,7 +1856,8 @@ int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const vo
     TROCM_REQUIRE(pk->len == pv->len && (pk->len == 0 || pk->pitch == pv->pitch), "K/V lengths and capacities of the prefix must match");
     TROCM_REQUIRE(q_heads >= 1 && q_heads % pk->H == 0, "Q heads (%lld) must be a multiple of K/V heads (%lld)", (long long)q_heads, (long long)pk->H);
     const bool step = k_new != nullptr;
-    TROCM_REQUIRE(pk->len < (1ll << 30), "shared prefix: tensor too large");
+    TROCM_REQUIRE(pk->len < (1ll << 30) && pk->H <= 65535, "shared prefix: tensor too large");
+    TROCM_REQUIRE(pk->D <= kRowsMaxD, "shared prefix: head_dim %lld is above %d", (long long)pk->D, kRowsMaxD);
     const size_t es = elem_bytes(dtype), q_bytes = (size_t)n_seq * q_heads * n_new * pk->D * es, new_bytes = (size_t)n_seq * pk->H * n_new * pk->D * es;
     TROCM_REQUIRE(!ranges_meet(out, q_bytes, q, q_bytes), "shared prefix: out overlaps q");
     TROCM_REQUIRE(!step || (!ranges_meet(out, q_bytes, k_new, new_bytes) && !ranges_meet(out, q_bytes, v_new, new_bytes)), "shared prefix: out overlaps the new rows");
@@ -1900,12 +1901,12 @@ int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const vo
     a.workspace = workspace, a.workspace_bytes = workspace_bytes;
     if (step) {
         if (launch_append_rows(a, k_new, v_new, s)) return 1;
-        for (int64_t i = 0; i < n_seq; i++) {
-            k_caches[i]->len += n_new, v_caches[i]->len += n_new;
-            seqs[(size_t)i].len += n_new;
-        }
+        for (int64_t i = 0; i < n_seq; i++) seqs[(size_t)i].len += n_new;
     }
-    return launch_sdpa_rows(a, s);
+    if (launch_sdpa_rows(a, s)) return 1;
+    // (new rows are counted when all of the call is on its way: one that fails can be repeated)
+    for (int64_t i = 0; i < n_seq && step; i++) k_caches[i]->len += n_new, v_caches[i]->len += n_new;
+    return 0;
 }
 
 static int scored_check(float softcap, const int32_t *documents, int64_t q_len, int64_t kv_len) {

@@ -283,6 +283,7 @@ struct SdpaRowsArgs {
     size_t workspace_bytes;
 };
 int launch_sdpa_rows(const SdpaRowsArgs &a, hipStream_t s);
+constexpr int kRowsMaxD = 2048;   // the largest head size that it takes
 // tanh as 1 - 2 / (e^2x + 1) is off by about 1e-7, times the cap: up to this cap less than a f16 weight's own rounding.
 constexpr float kFastTanhCap = 512.0f;
 // f16 prompts of scored attention (sdpa_scored.hip); 2 = not covered.

@@ -115,7 +115,7 @@ __device__ __forceinline__ float fast_tanh(float x) {
 
 // ---- any head size, any alignment: a workgroup per query row -------------------------------------------------------
 
-constexpr int kAnyThreads = 256, kAnyMaxD = 2048;
+constexpr int kAnyThreads = 256, kAnyMaxD = kRowsMaxD;
 
 template <typename T>
 __global__ __launch_bounds__(kAnyThreads) void sdpa_rows_any_kernel(RowsCall call) {
