@@ -47,3 +47,22 @@ def test_more_query_rows_than_a_launch_has(rt):
     q, new = (ta.DeviceTensor.from_numpy(np.ones((1, h, 1, d), F16)) for h in (4, 1))
     ta.inplace_kv_sdpa_eval_shared(q, new, new, *caches[:2], caches[2:3], caches[3:])
     assert [c.len() for c in caches] == [3, 3, 3, 3]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n", [1, 3])
+def test_head_sizes_that_steps_with_norms_do_not_take(rt, dtype, n):
+    rng, d = np.random.default_rng(53), 514
+    op = ta.InPlaceKvSdpa(axis=2, causal=True).state()
+    op.k, op.v = (_pushed(rng, (1, 2, 2, d), dtype) for _ in range(2))
+    before = _state([op.k, op.v])
+    q, new = (ta.DeviceTensor.from_numpy(np.ones((1, h, n, d), dtype)) for h in (4, 2))
+    cs = ta.DeviceTensor.from_numpy(np.ones((1, 1, n, d), dtype))
+    dense = (2 * n * d, n * d, d, 1)
+    for strides in (None, dense, (3 * n * d, n * d, d, 1)):   # (the last: values that are not dense are appended by themselves)
+        with pytest.raises(ta.TractRocmError, match="head_dim 514"):
+            op.eval_norm_rope_into(q, new, new, None, None, 1e-6, cs, cs, v_strides=strides)
+        assert _state([op.k, op.v]) == before
+    with pytest.raises(ta.TractRocmError, match="head_dim 514"):
+        op.eval_into(q, new, new)
+    assert _state([op.k, op.v]) == before

@@ -1325,6 +1325,8 @@ static int inplace_eval_check(const char *what, const void *q, const void *k_new
     TROCM_REQUIRE(q_heads >= 1 && q_heads % kc->H == 0, "Q heads (%lld) must be a multiple of K/V heads (%lld)", (long long)q_heads,
                   (long long)kc->H);
     TROCM_REQUIRE(kc->len + n_new > 0, "empty kv-cache");  // inplace_kv_cache.rs:91
+    // (what the kernel for any shape refuses, which takes every head size that no other does)
+    TROCM_REQUIRE(n_new == 0 || kc->D <= kGenericMaxD, "%s: head_dim %lld not in 1..%d", what, (long long)kc->D, kGenericMaxD);
     return 0;
 }
 

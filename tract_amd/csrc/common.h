@@ -186,6 +186,7 @@ struct SdpaArgs {
     int64_t rope_stride_b;
 };
 int launch_sdpa_generic(const SdpaArgs &a, hipStream_t s);
+constexpr int kGenericMaxD = 512;   // the largest head size that it takes
 // Split-K decode (Sq == 1).  Returns 2 when the shape is not covered by a fast kernel.
 int launch_sdpa_decode(const SdpaArgs &a, hipStream_t s);
 // Split-K decode for 2..32 query heads per kv head (f16): the heads are the rows of MFMA tiles.

@@ -76,7 +76,7 @@ __device__ __forceinline__ KvReader<T> make_reader(const GenericDev &p, const vo
 
 template <typename T>
 __global__ __launch_bounds__(64) void sdpa_generic_kernel(GenericDev p) {
-    __shared__ float lds_q[512];
+    __shared__ float lds_q[kGenericMaxD];
     __shared__ float lds_p[64];
     const int lane = threadIdx.x;
     int64_t row = blockIdx.x;
@@ -157,7 +157,7 @@ int launch_sdpa_generic(const SdpaArgs &a, hipStream_t s) {
     const bool quant = a.kv_fmt == TROCM_Q8_0 || a.kv_fmt == TROCM_Q4_0;
     TROCM_REQUIRE(quant || a.q_dtype == a.kv_fmt, "generic sdpa: Q and K/V must share a dtype");
     TROCM_REQUIRE(!quant || (a.D % 32 == 0 && a.kv_stride_t == a.D), "generic sdpa: quantised K/V needs dense rows and head_dim %% 32 == 0");
-    TROCM_REQUIRE(a.D >= 1 && a.D <= 512, "generic sdpa: head_dim %lld not in 1..512", (long long)a.D);
+    TROCM_REQUIRE(a.D >= 1 && a.D <= kGenericMaxD, "generic sdpa: head_dim %lld not in 1..%d", (long long)a.D, kGenericMaxD);
     int64_t rows = a.B * a.Hq * a.Sq;
     if (rows == 0) return 0;
     TROCM_REQUIRE(rows < (1ll << 31), "generic sdpa: too many query rows");
