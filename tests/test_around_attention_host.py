@@ -11,6 +11,7 @@ F16 = np.dtype(np.float16)
 AT = 1 << 20   # an address that nothing reads
 
 
+
 def _tensor(*shape, dtype=F16):
     return DeviceTensor(shape, dtype, ptr=AT)
 
@@ -24,6 +25,45 @@ def calls(monkeypatch):
     made = []
     monkeypatch.setattr(scored, "call", lambda name, *args: made.append(name))
     return made
+
+
+@pytest.fixture
+def sizes(monkeypatch):
+    """The sizes that a call passes on, by position: (name, [its whole numbers])."""
+    made = []
+    monkeypatch.setattr(scored, "call", lambda name, *args: made.append((name, [a for a in args if type(a) is int])))
+    monkeypatch.setattr(scored, "Workspace", _Workspace)
+    return made
+
+
+class _Workspace:
+    """Takes the place of a workspace; `before` is called once as one is made: what another thread does meanwhile."""
+    before = None
+
+    def __init__(self, *args, nbytes=None):
+        _Workspace.before, then = None, _Workspace.before
+        if then:
+            then()
+        self.nbytes = self.bytes_for() if nbytes is None else nbytes
+        self.buf = types.SimpleNamespace(ptr=AT)
+
+    @staticmethod
+    def bytes_for(*_):
+        return 1000
+
+    shared_bytes_for = bytes_for
+
+
+def _interrupt(monkeypatch, then):
+    """`then` runs once, as a call has no output yet and is about to make one (the allocation lets other threads run)."""
+    output = scored._output
+
+    def interrupted(*args):
+        monkeypatch.setattr(scored, "_output", output)
+        then()
+        return output(*args)
+
+    monkeypatch.setattr(scored, "_output", interrupted)
 
 
 @pytest.mark.parametrize("d", [64, 256])
@@ -42,3 +82,59 @@ def test_a_shared_step_refuses_queries_of_another_head_size_than_the_caches(call
     q, new = _tensor(2, 4, 1, 128), _tensor(2, 2, 1, 128)
     scored.inplace_kv_sdpa_eval_shared(q, new, new, *prefix, caches[:2], caches[2:], workspace=ws, out=_tensor(2, 4, 1, 128))
     assert calls == ["trocm_inplace_kv_sdpa_eval_shared"]
+
+
+def _out(*shape):
+    """An output of a shape that is right and a type that is equal but not the same object: looked at by `_output`, and allocates nothing."""
+    t = _tensor(*shape)
+    t.dtype = np.dtype(F16, copy=True)
+    assert t.dtype is not F16
+    return t
+
+
+def test_norms_of_two_threads_keep_their_own_sizes(sizes, monkeypatch):
+    op = scored.QkNormRope()
+
+    def norm(n):
+        q, k, c = _tensor(1, 4, n, 64), _tensor(1, 2, n, 64), _tensor(1, 1, n, 64)
+        op.eval(q, k, None, None, c, c, q_out=_out(1, 4, n, 64), k_out=_tensor(1, 2, n, 64))
+
+    norm(3)
+    _interrupt(monkeypatch, lambda: norm(7000))
+    norm(3)
+    _interrupt(monkeypatch, lambda: norm(9))
+    norm(5)
+    assert [s[s.index(64) - 1] for _, s in sizes] == [3, 7000, 3, 9, 5]
+
+
+def test_shared_prefixes_of_two_threads_keep_their_own_sizes(sizes, monkeypatch):
+    op = scored.SharedPrefixSdpa()
+
+    def attend(n):
+        q, p, k = _tensor(n, 4, 1, 64), _tensor(1, 2, 11, 64), _tensor(n, 2, 5, 64)
+        op.eval(q, p, p, k, k, [1] * n, out=_out(n, 4, 1, 64))
+
+    attend(2)
+    _interrupt(monkeypatch, lambda: attend(300))
+    attend(2)
+    assert [s[1] for _, s in sizes] == [2, 300, 2]
+    other = scored.SharedPrefixSdpa()      # a first workspace that cannot be had leaves nothing behind
+    _Workspace.before = lambda: (_ for _ in ()).throw(TractRocmError("no memory"))
+    q, p, k = _tensor(2, 4, 1, 64), _tensor(1, 2, 11, 64), _tensor(2, 2, 5, 64)
+    with pytest.raises(TractRocmError, match="no memory"):
+        other.eval(q, p, p, k, k, [1, 1], out=_tensor(2, 4, 1, 64))
+    other.eval(q, p, p, k, k, [1, 1], out=_tensor(2, 4, 1, 64))
+    assert sizes[-1][1][1] == 2
+
+
+def test_scored_attention_of_two_threads_keeps_its_own_sizes(sizes, monkeypatch):
+    op = scored.ScoredSdpa(softcap=5.0)
+
+    def attend(n):
+        q, k = _tensor(1, 4, n, 64), _tensor(1, 2, n, 64)
+        op.eval(q, k, k, out=_out(1, 4, n, 64))
+
+    attend(2)
+    _interrupt(monkeypatch, lambda: attend(300))
+    attend(2)
+    assert [s[s.index(64) - 1] for _, s in sizes] == [2, 300, 2]

@@ -42,7 +42,7 @@ class QkNormRope:
 
     def __init__(self, eps: float = 1e-6):
         self.eps = float(eps)
-        self._key = self._sizes = None
+        self._last = (None, None)
 
     def name(self) -> str:
         return "QkNormRope"
@@ -63,7 +63,8 @@ class QkNormRope:
         # (A decode step's call takes the device 3.4 us: shapes and types are looked into where they are not the last call's.)
         key = (shape, k_shape, cos.shape, sin.shape, q_strides and tuple(q_strides), k_strides and tuple(k_strides), dtype, k.dtype, cos.dtype, sin.dtype,
                q_weight is None or (q_weight.shape, q_weight.dtype), k_weight is None or (k_weight.shape, k_weight.dtype))
-        if key != self._key:
+        last_key, sizes = self._last   # (a pair, read once: another thread's call may put its own there)
+        if key != last_key:
             for t in (k, q_weight, k_weight, cos, sin):
                 if t is not None and not _same(t.dtype, dtype):
                     raise TractRocmError("Q, K, weights, cos and sin must share a datum type")
@@ -72,13 +73,14 @@ class QkNormRope:
             b, hq, n, d = shape
             cb = _cos_sin_batch(cos, sin, b, n, d)
             _check_norm_weights(q_weight, k_weight, d)
-            self._key, self._sizes = key, (0 if cb == 1 else n * d, _code(dtype), b, hq, k_shape[1], n, d, _strides4(q_strides), _strides4(k_strides))
+            sizes = 0 if cb == 1 else n * d, _code(dtype), b, hq, k_shape[1], n, d, _strides4(q_strides), _strides4(k_strides)
+            self._last = key, sizes
         if q_out is None or q_out.shape != shape or q_out.dtype is not dtype:
             q_out = _output(q_out, shape, dtype)
         if k_out is None or k_out.shape != k_shape or k_out.dtype is not dtype:
             k_out = _output(k_out, k_shape, dtype)
         call("trocm_qk_norm_rope", q.ptr, k.ptr, None if q_weight is None else q_weight.ptr, None if k_weight is None else k_weight.ptr, self.eps,
-             cos.ptr, sin.ptr, *self._sizes, q_out.ptr, k_out.ptr, None if stream is None else _sh(stream))
+             cos.ptr, sin.ptr, *sizes, q_out.ptr, k_out.ptr, None if stream is None else _sh(stream))
         return q_out, k_out
 
 
@@ -87,13 +89,13 @@ class SharedPrefixSdpa:
 
     def __init__(self, scale=None, is_causal: bool = True):
         self.scale, self.is_causal = scale, bool(is_causal)
-        self._ws = self._key = self._sizes = None
+        self._ws, self._last = None, (None, None, None)
 
     def _workspace(self, n, hq, sq, d, stream):
-        need = Workspace.shared_bytes_for(n, hq, sq, d)
-        if self._ws is None or self._ws.nbytes < need:
-            self._ws = Workspace(n, hq, sq, d, stream, nbytes=need)
-        return self._ws
+        need, ws = Workspace.shared_bytes_for(n, hq, sq, d), self._ws
+        if ws is None or ws.nbytes < need:
+            ws = self._ws = Workspace(n, hq, sq, d, stream, nbytes=need)
+        return ws
 
     def eval(self, q, prefix_k, prefix_v, k, v, lens, stream=None, out=None, prefix_len=None) -> DeviceTensor:
         """Q [n_seq, q_heads, q_len, head_dim]; prefix K and V [1, kv_heads, room, head_dim] of which `prefix_len` tokens (None:
@@ -102,7 +104,8 @@ class SharedPrefixSdpa:
             q, prefix_k, prefix_v, k, v = (_as_device(t, stream) for t in (q, prefix_k, prefix_v, k, v))
         dtype, shape = q.dtype, q.shape
         key = (shape, k.shape, v.shape, prefix_k.shape, prefix_v.shape, prefix_len, dtype, k.dtype, v.dtype, prefix_k.dtype, prefix_v.dtype)
-        if key != self._key:   # (the last call's need no second look)
+        last_key, sizes, ws = self._last   # (read once: another thread's call may put its own there)
+        if key != last_key:                # (the last call's need no second look)
             for t in (prefix_k, prefix_v, k, v):
                 if not _same(t.dtype, dtype):
                     raise TractRocmError("Q, K and V must share a datum type")
@@ -114,17 +117,15 @@ class SharedPrefixSdpa:
             p = p_room if prefix_len is None else int(prefix_len)
             if k.shape != (n, hkv, room, d) or prefix_k.shape != (1, hkv, p_room, d) or not 0 <= p <= p_room:
                 raise TractRocmError(f"shared prefix: Q {shape}, prefix {prefix_k.shape} and K {k.shape} do not match")
-            self._key = key
-            self._sizes = (_code(dtype), n, hq, hkv, sq, d), p, (C.c_int64 * 2)(p_room * d, d), _I64x3(hkv * room * d, room * d, d)
-            self._workspace(n, hq, sq, d, stream)
-        sizes, p, prefix_strides, strides = self._sizes
+            sizes, ws = ((_code(dtype), n, hq, hkv, sq, d), p, (C.c_int64 * 2)(p_room * d, d), _I64x3(hkv * room * d, room * d, d)), self._workspace(n, hq, sq, d, stream)
+            self._last = key, sizes, ws
+        sizes, p, prefix_strides, strides = sizes
         n, room = shape[0], k.shape[2]
         lens = array("q", lens)
         if len(lens) != n or (n and max(lens) > room):   # (negative ones are refused below)
             raise TractRocmError(f"shared prefix: lens must be {n} lengths of 0..={room}")
         if out is None or out.shape != shape or out.dtype is not dtype:
             out = _output(out, shape, dtype)
-        ws = self._ws
         call("trocm_sdpa_shared_prefix", q.ptr, *sizes, prefix_k.ptr, prefix_v.ptr, p, prefix_strides, k.ptr, v.ptr, strides,
              _PI64.from_buffer(lens) if n else _I64x3(0, 0, 0), out.ptr, _scale_arg(self.scale), int(self.is_causal), ws.buf.ptr, ws.nbytes,
              None if stream is None else _sh(stream))
@@ -169,15 +170,17 @@ class ScoredSdpa:
 
     def __init__(self, scale=None, softcap: float = 0.0, is_causal: bool = True):
         self.scale, self.softcap, self.is_causal = scale, float(softcap), bool(is_causal)
-        self._ws = self._ws_key = self._key = self._sizes = None
+        self._ws, self._last = (None, None), (None, None)
 
     def name(self) -> str:
         return "ScoredSdpa"
 
     def _workspace(self, b, hq, sq, d, stream):
-        if self._ws is None or self._ws_key != (b, hq, d) or self._ws.nbytes < Workspace.bytes_for(b, hq, sq, d):
-            self._ws, self._ws_key = Workspace(b, hq, sq, d, stream), (b, hq, d)
-        return self._ws
+        ws, ws_key = self._ws
+        if ws_key != (b, hq, d) or ws.nbytes < Workspace.bytes_for(b, hq, sq, d):
+            ws = Workspace(b, hq, sq, d, stream)
+            self._ws = ws, (b, hq, d)
+        return ws
 
     @staticmethod
     def _rules(slopes, documents, prefix_lens, b, hq, sk, stream):
@@ -196,15 +199,16 @@ class ScoredSdpa:
             q, k, v = (_as_device(t, stream) for t in (q, k, v))
         dtype, shape = q.dtype, q.shape
         key = (shape, k.shape, v.shape, dtype, k.dtype, v.dtype)
-        if key != self._key:   # (the last call's need no second look)
+        last_key, sizes = self._last   # (read once: another thread's call may put its own there)
+        if key != last_key:            # (the last call's need no second look)
             if not (_same(k.dtype, dtype) and _same(v.dtype, dtype)):
                 raise TractRocmError("Q, K and V must share a datum type")
             b, hq, sq, d = _canon4(shape)
             _, hkv, sk, _ = _canon4(k.shape)
             if _canon4(k.shape) != (b, hkv, sk, d) or k.shape != v.shape:
                 raise TractRocmError("K/V shape mismatch")
-            self._key, self._sizes = key, (_code(dtype), b, hq, hkv, sq, sk, d)
-        sizes = self._sizes
+            sizes = _code(dtype), b, hq, hkv, sq, sk, d
+            self._last = key, sizes
         _, b, hq, _, sq, sk, d = sizes
         if slopes is not None or documents is not None or prefix_lens is not None:
             slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, sk, stream)
