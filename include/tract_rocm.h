@@ -529,7 +529,7 @@ int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const vo
  *   slopes      : [q_heads] f32, device memory, or NULL; any sign, at most 1e30 in size
  *   documents   : [batch, kv_len] int32, device memory, or NULL; ids in any order, negative ones are padding that nothing sees
  *                 and whose K and V rows may hold anything; needs kv_len >= q_len
- *   prefix_lens : [batch] int32, device memory, or NULL; values past kv_len mean all of it; read only when causal
+ *   prefix_lens : [batch] int32, device memory, or NULL; values past kv_len mean all of it, negative ones none; read only when causal
  * A row that sees nothing is zeros.  All K and V rows but those of padding must be finite, seen or not: a weight of zero times an
  * infinite value is NaN.  out may not overlap q, k or v.  k, v, strides, scale and workspace as for trocm_sdpa. */
 int trocm_sdpa_scored(const void *q, const void *k, const void *v, void *out, int dtype, int64_t batch, int64_t q_heads,

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kAnyThreads) void sdpa_rows_any_kernel(RowsCall cal
     for (int d = tid; d < D; d += kAnyThreads) lds_q[d] = widen(q[d]);
     const int at = i + own.len - p.Sq;
     int lim = p.causal ? at : own.len - 1;
-    if (p.prefix_lens) lim = max(lim, p.prefix_lens[b] - 1);
+    if (p.prefix_lens) lim = max(lim, max(p.prefix_lens[b], 0) - 1);
     lim = min(lim, own.len - 1);
     const float slope = p.slopes ? p.slopes[qh] : 0.0f;
     const int *docs = p.docs ? p.docs + (int64_t)b * p.Sk : nullptr;
@@ -322,7 +322,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
     const int64_t out_row = place.at;
     const int at = place.i + n_keys - p.Sq;
     int lim = n_keys - 1, doc = 0;
-    if (own && p.causal) lim = min(lim, SCORED && p.prefix_lens ? max(at, p.prefix_lens[wk.b] - 1) : at);
+    if (own && p.causal) lim = min(lim, SCORED && p.prefix_lens ? max(at, max(p.prefix_lens[wk.b], 0) - 1) : at);   // (of any value: a negative one is no prefix)
     float slope = 0.0f;
     const int *docs = nullptr;
     int n_tiles = wk.part < wk.parts ? wk.tiles : 0;   // of all parts; with documents those that are listed

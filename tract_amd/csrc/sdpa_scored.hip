@@ -80,12 +80,12 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
     const int64_t out_row = ((int64_t)b * p.Hq + kvh * p.G + g) * p.Sq + i;
     const int at = i + off;
     int lim = p.Sk - 1, n_vis = p.Sk;
+    const int pre = p.prefix_lens ? max(p.prefix_lens[b], 0) : 0;   // (of any value: a negative one is no prefix)
     if (p.causal) {
-        const int pre = p.prefix_lens ? p.prefix_lens[b] : 0;
         lim = min(lim, max(at, pre - 1));
         n_vis = max(0, min(p.Sk, max(p.by_g.by(min(row0 + kRows, seq_rows) - 1) + off + 1, pre)));
     }
-    const int wave_lim = __builtin_amdgcn_readfirstlane(p.causal ? max(p.by_g.by(min(row0 + 32 * w + 32, seq_rows) - 1) + off, p.prefix_lens ? p.prefix_lens[b] - 1 : -1) : p.Sk - 1);
+    const int wave_lim = __builtin_amdgcn_readfirstlane(p.causal ? max(p.by_g.by(min(row0 + 32 * w + 32, seq_rows) - 1) + off, pre - 1) : p.Sk - 1);
     const bool wave_has_rows = row0 + 32 * w < seq_rows;
     const int t_end = (n_vis + kTile - 1) / kTile;
     int n_tiles = t_end;
