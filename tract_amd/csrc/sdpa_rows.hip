@@ -113,6 +113,12 @@ __device__ __forceinline__ float fast_tanh(float x) {
     return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.0f * kLog2e)) + 1.0f);
 }
 
+// a - b of scores as they are rounded: a product fused into it would differ from `b`, which is one of them, by up to half its last place.
+__device__ __forceinline__ float less(float a, float b) {
+#pragma clang fp contract(off)
+    return a - b;
+}
+
 // ---- any head size, any alignment: a workgroup per query row -------------------------------------------------------
 
 constexpr int kAnyThreads = 256, kAnyMaxD = kRowsMaxD;
@@ -524,7 +530,8 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 #pragma unroll
         for (int d = R; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
         // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
-        const bool moved = top > m_run + (H16 ? 8.0f : 0.0f);
+        // (the difference: m_run + 8 is m_run + 16 or m_run where a step of 32 bits is 16)
+        const bool moved = less(top, m_run) > (H16 ? 8.0f : 0.0f);
         const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
         const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
         m_run = m_new;
@@ -532,7 +539,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
         float sum = 0.0f;
 #pragma unroll
         for (int x = 0; x < NS; x++) {
-            float e = __builtin_amdgcn_exp2f(s[x] - ref);
+            float e = __builtin_amdgcn_exp2f(less(s[x], ref));
             if constexpr (H16) {   // the product with V takes f16 weights, and the row's sum the same ones
                 pf[x >> 3][x & 7] = (_Float16)e;
                 e = (float)pf[x >> 3][x & 7];
@@ -670,7 +677,7 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
             *reinterpret_cast<u32x4 *>(lds_v + buf * V_TILE + (key0 + j * RPI) * VROW + ch * 8) = vpre[j];
         }
     };
-    float m_run = -INFINITY, l_run = 0.0f;
+    float m_run = -INFINITY, from = __builtin_nanf(""), s_ref = 0.0f, l_run = 0.0f;   // (a reference as sdpa_scored.hip has it)
     float16_t o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -712,20 +719,20 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
             // look at the maximum: the reference moves where that is more than 8 above it.
             half8_t pf[4];
             float sum;
-            auto weights = [&]() __attribute__((always_inline)) {
+            auto weights = [&](float from) __attribute__((always_inline)) {
                 const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
                 sum = 0.0f;
 #pragma unroll
                 for (int st = 0; st < 4; st++) {
 #pragma unroll
-                    for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, -m_run));
+                    for (int x = 0; x < 8; x++) pf[st][x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + x], to_log2, from));
 #pragma unroll
                     for (int x = 0; x < 4; x++) sum = __builtin_amdgcn_fdot2(half2_t{pf[st][2 * x], pf[st][2 * x + 1]}, ones, sum, false);   // the same rounded weights
                 }
             };
             bool look = n == 0;
             if (!look) {
-                weights();
+                weights(from);
                 look = __builtin_amdgcn_ballot_w64(!(sum < 32768.0f)) != 0;
             }
             if (look) {
@@ -734,16 +741,27 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
                 for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb][x]);
-                top = fmaxf(top, __shfl_xor(top, 32, 64)) * to_log2;   // (scale > 0: the maximum commutes with it)
-                const bool moved = top > m_run + 8.0f;
-                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                const float s_top = fmaxf(top, __shfl_xor(top, 32, 64));
+                top = s_top * to_log2;   // (scale > 0: the maximum commutes with it)
+                const bool far = from != from && m_run != -INFINITY, moved = top > m_run + 8.0f || (far && s_top > s_ref);
+                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(far ? (s_ref - s_top) * to_log2 : m_run - m_new) : 1.0f;
                 m_run = m_new;
+                if (moved) s_ref = s_top, from = fabsf(m_new) < 0x1p20f ? -m_new : __builtin_nanf("");
                 l_run *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) o[db][x] *= keep;
-                weights();
+                float f = from;
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(from != from) != 0, 0)) {
+                    const float less = from != from ? s_ref : 0.0f;   // (rows of ordinary scores stay as they are)
+#pragma unroll
+                    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                        for (int x = 0; x < 16; x++) s[kb][x] -= less;
+                    f = from != from ? 0.0f : from;
+                }
+                weights(f);
             }
             l_run += sum;
             const _Float16 *vsrc = lds_v + buf * V_TILE + (4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);

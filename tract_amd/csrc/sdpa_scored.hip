@@ -206,7 +206,10 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
         }
     };
 
-    float m_run = kNone, l_run = 0.0f;
+    // A row's reference: s_ref among the scores, m_run in the log2 domain.  What the rounding of m_run left out is a factor that all weights
+    // taken from it share, unless it is an exponent that f16 does not have: from 2^20 on every tile of the row gets a look (of it `from` is
+    // NaN), which takes weights from s_ref and moves it to whatever is larger.
+    float m_run = kNone, from = base - kNone, s_ref = 0.0f, l_run = 0.0f;
     float16_t o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -281,9 +284,8 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
             // look at the maximum: the reference moves where that is more than 8 above it.
             half8_t pf[4];
             float sum;
-            auto weights = [&]() __attribute__((always_inline)) {
+            auto weights = [&](float from) __attribute__((always_inline)) {
                 const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
-                const float from = base - m_run;
                 sum = 0.0f;
 #pragma unroll
                 for (int st = 0; st < 4; st++) {
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
             };
             bool look = !DOCS && n == kg;   // (documents: weights against no reference come to infinity; asked for by place, the first tile spills scalar registers)
             if (!look) {
-                weights();
+                weights(from);
                 look = __builtin_amdgcn_ballot_w64(!(sum < 32768.0f)) != 0;
             }
             if (look) {
@@ -304,17 +306,27 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
                 for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) top = CAP ? fminf(top, s[kb2][x]) : fmaxf(top, s[kb2][x]);
-                const float other = __shfl_xor(top, 32, 64);
-                top = __builtin_fmaf(CAP ? fminf(top, other) : fmaxf(top, other), to_log2, base);
-                const bool moved = top > m_run + 8.0f;
-                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+                const float other = __shfl_xor(top, 32, 64), s_top = CAP ? fminf(top, other) : fmaxf(top, other);
+                top = __builtin_fmaf(s_top, to_log2, base);
+                const bool far = from != from, moved = top > m_run + 8.0f || (far && (CAP ? s_top < s_ref : s_top > s_ref));
+                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(far ? (s_ref - s_top) * to_log2 : m_run - m_new) : 1.0f;
                 m_run = m_new;
+                if (moved) s_ref = s_top, from = fabsf(m_new) < 0x1p20f ? base - m_new : __builtin_nanf("");
                 l_run *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) o[db][x] *= keep;
-                weights();
+                float f = from;
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(from != from) != 0, 0)) {
+                    const float less = from != from ? s_ref : 0.0f;   // (rows of ordinary scores stay as they are)
+#pragma unroll
+                    for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+                        for (int x = 0; x < 16; x++) s[kb2][x] -= less;
+                    f = from != from ? 0.0f : from;
+                }
+                weights(f);
             }
             l_run += sum;
             const _Float16 *vsrc = &lds_v[buf][(4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
@@ -412,6 +424,8 @@ void launch_of(const ScoredDev &p, hipStream_t s) {
 int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s) {
     if (a.dtype != TROCM_F16 || (a.D != 64 && a.D != 128) || a.P || a.lens || a.seqs || a.Sk == 0 || a.softcap > kFastTanhCap) return 2;
     if (a.softcap > 0.0f ? a.softcap < 1e-6f : !(a.scale > 1e-6f)) return 2;   // (slopes are divided by it, and the largest product stands for the largest score)
+    const double per = a.softcap > 0.0f ? 2.0 * a.softcap : a.scale;   // (slopes of up to 1e30 times a distance, so divided, and as they are, stay inside f32)
+    if (a.slopes && (double)(a.Sk + a.Sq) > 1e8 * (per < 1.0 ? per : 1.0)) return 2;
     auto aligned = [](const void *x) { return (uintptr_t)x % 16 == 0; };
     const int64_t G = a.Hq / a.Hkv, rows = a.Sq * G;
     if (!aligned(a.q) || !aligned(a.out) || !aligned(a.k) || !aligned(a.v) || a.stride_b % 8 || a.stride_h % 8 || a.stride_t % 8 || a.stride_t * 2 > (1 << 25)) return 2;
