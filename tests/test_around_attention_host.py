@@ -138,3 +138,30 @@ def test_scored_attention_of_two_threads_keeps_its_own_sizes(sizes, monkeypatch)
     _interrupt(monkeypatch, lambda: attend(300))
     attend(2)
     assert [s[s.index(64) - 1] for _, s in sizes] == [2, 300, 2]
+
+
+@pytest.mark.parametrize("make", [scored.SharedPrefixSdpa, scored.ScoredSdpa])
+def test_a_workspace_that_was_outgrown_stays(sizes, monkeypatch, make):
+    """A recorded graph goes on using the workspace of the call that it recorded, by address; a call's share is that of its shape."""
+    op, made, alive = make(), [], set()
+
+    class Counted(_Workspace):
+        bytes_for = shared_bytes_for = staticmethod(lambda b, hq, sq, d: 100 * b * sq)
+
+        def __init__(self, *args, **kw):
+            super().__init__(*args, **kw)
+            made.append(self.nbytes)
+            alive.add(self.nbytes)
+
+        def __del__(self):
+            alive.discard(getattr(self, "nbytes", None))
+
+    monkeypatch.setattr(scored, "Workspace", Counted)
+    for n in (2, 40, 2, 30, 41, 7, 500, 3):
+        q, p, k = _tensor(n, 4, 1, 64), _tensor(1, 2, 11, 64), _tensor(n, 2, 5, 64)
+        if make is scored.ScoredSdpa:
+            op.eval(q, k, k, out=_tensor(n, 4, 1, 64))
+        else:
+            op.eval(q, p, p, k, k, [1] * n, out=_tensor(n, 4, 1, 64))
+        assert sizes[-1][1][-1] == 100 * n
+    assert alive == set(made) and len(made) <= 4 and sum(made) <= 2 * made[-1]

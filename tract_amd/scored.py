@@ -7,7 +7,8 @@
 * ``ScoredSdpa``        Sdpa (transformers/src/ops/sdpa.rs:83-89) whose scores are capped by a tanh, fall with the distance,
   stay inside documents or see a prefix
 
-An object keeps its workspace from call to call: its calls follow each other on one stream.
+An object keeps its workspace from call to call: its calls follow each other on one stream.  A graph that recorded a call uses
+that workspace: the object has to live as long as the graph, and later calls of other shapes leave it be.
 """
 from __future__ import annotations
 
@@ -35,6 +36,20 @@ def _output(out, shape, dtype):
     if out.shape != shape or not _same(out.dtype, dtype):
         raise TractRocmError("out must have Q's shape and datum type")
     return out
+
+
+class _Scratch:
+    """An operator's workspace.  It grows; what it outgrew is kept, since recorded graphs go on using it (at most as much again)."""
+
+    def __init__(self):
+        self._all = []
+
+    def holding(self, need: int, stream) -> Workspace:
+        ws = self._all[-1] if self._all else None
+        if ws is None or ws.nbytes < need:
+            ws = Workspace(0, 0, 0, 0, stream, nbytes=need if ws is None else max(need, 2 * ws.nbytes))
+            self._all.append(ws)
+        return ws
 
 
 class QkNormRope:
@@ -89,13 +104,7 @@ class SharedPrefixSdpa:
 
     def __init__(self, scale=None, is_causal: bool = True):
         self.scale, self.is_causal = scale, bool(is_causal)
-        self._ws, self._last = None, (None, None, None)
-
-    def _workspace(self, n, hq, sq, d, stream):
-        need, ws = Workspace.shared_bytes_for(n, hq, sq, d), self._ws
-        if ws is None or ws.nbytes < need:
-            ws = self._ws = Workspace(n, hq, sq, d, stream, nbytes=need)
-        return ws
+        self._scratch, self._last = _Scratch(), (None, None, None)
 
     def eval(self, q, prefix_k, prefix_v, k, v, lens, stream=None, out=None, prefix_len=None) -> DeviceTensor:
         """Q [n_seq, q_heads, q_len, head_dim]; prefix K and V [1, kv_heads, room, head_dim] of which `prefix_len` tokens (None:
@@ -117,9 +126,10 @@ class SharedPrefixSdpa:
             p = p_room if prefix_len is None else int(prefix_len)
             if k.shape != (n, hkv, room, d) or prefix_k.shape != (1, hkv, p_room, d) or not 0 <= p <= p_room:
                 raise TractRocmError(f"shared prefix: Q {shape}, prefix {prefix_k.shape} and K {k.shape} do not match")
-            sizes, ws = ((_code(dtype), n, hq, hkv, sq, d), p, (C.c_int64 * 2)(p_room * d, d), _I64x3(hkv * room * d, room * d, d)), self._workspace(n, hq, sq, d, stream)
+            need = Workspace.shared_bytes_for(n, hq, sq, d)
+            sizes, ws = ((_code(dtype), n, hq, hkv, sq, d), p, (C.c_int64 * 2)(p_room * d, d), _I64x3(hkv * room * d, room * d, d), need), self._scratch.holding(need, stream)
             self._last = key, sizes, ws
-        sizes, p, prefix_strides, strides = sizes
+        sizes, p, prefix_strides, strides, need = sizes
         n, room = shape[0], k.shape[2]
         lens = array("q", lens)
         if len(lens) != n or (n and max(lens) > room):   # (negative ones are refused below)
@@ -127,7 +137,7 @@ class SharedPrefixSdpa:
         if out is None or out.shape != shape or out.dtype is not dtype:
             out = _output(out, shape, dtype)
         call("trocm_sdpa_shared_prefix", q.ptr, *sizes, prefix_k.ptr, prefix_v.ptr, p, prefix_strides, k.ptr, v.ptr, strides,
-             _PI64.from_buffer(lens) if n else _I64x3(0, 0, 0), out.ptr, _scale_arg(self.scale), int(self.is_causal), ws.buf.ptr, ws.nbytes,
+             _PI64.from_buffer(lens) if n else _I64x3(0, 0, 0), out.ptr, _scale_arg(self.scale), int(self.is_causal), ws.buf.ptr, need,
              None if stream is None else _sh(stream))
         return out
 
@@ -170,17 +180,10 @@ class ScoredSdpa:
 
     def __init__(self, scale=None, softcap: float = 0.0, is_causal: bool = True):
         self.scale, self.softcap, self.is_causal = scale, float(softcap), bool(is_causal)
-        self._ws, self._last = (None, None), (None, None)
+        self._scratch, self._last = _Scratch(), (None, None)
 
     def name(self) -> str:
         return "ScoredSdpa"
-
-    def _workspace(self, b, hq, sq, d, stream):
-        ws, ws_key = self._ws
-        if ws_key != (b, hq, d) or ws.nbytes < Workspace.bytes_for(b, hq, sq, d):
-            ws = Workspace(b, hq, sq, d, stream)
-            self._ws = ws, (b, hq, d)
-        return ws
 
     @staticmethod
     def _rules(slopes, documents, prefix_lens, b, hq, sk, stream):
@@ -214,9 +217,10 @@ class ScoredSdpa:
             slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, sk, stream)
         if out is None or out.shape != shape or out.dtype is not dtype:
             out = _output(out, shape, dtype)
-        ws = self._workspace(b, hq, sq, d, stream)
+        need = Workspace.bytes_for(b, hq, sq, d)
+        ws = self._scratch.holding(need, stream)
         call("trocm_sdpa_scored", q.ptr, k.ptr, v.ptr, out.ptr, *sizes, None, _scale_arg(self.scale), self.softcap, _optr(slopes), _optr(documents),
-             _optr(prefix_lens), int(self.is_causal), ws.buf.ptr, ws.nbytes, None if stream is None else _sh(stream))
+             _optr(prefix_lens), int(self.is_causal), ws.buf.ptr, need, None if stream is None else _sh(stream))
         return out
 
     def eval_cached(self, q: DeviceTensor, k_cache, v_cache, slopes=None, documents=None, prefix_lens=None, stream=None, out=None) -> DeviceTensor:
@@ -229,7 +233,8 @@ class ScoredSdpa:
             raise TractRocmError(f"Q {q.shape} does not match the cache's {k_cache._shape}")
         slopes, documents, prefix_lens = self._rules(slopes, documents, prefix_lens, b, hq, k_cache.len(), stream)
         out = _output(out, q.shape, q.dtype)
-        ws = self._workspace(b, hq, sq, d, stream)
+        need = Workspace.bytes_for(b, hq, sq, d)
+        ws = self._scratch.holding(need, stream)
         call("trocm_sdpa_cached_scored", q.ptr, _code(q.dtype), hq, sq, k_cache.handle, v_cache.handle, out.ptr, _scale_arg(self.scale), self.softcap,
-             _optr(slopes), _optr(documents), _optr(prefix_lens), int(self.is_causal), ws.ptr, ws.nbytes, _sh(stream))
+             _optr(slopes), _optr(documents), _optr(prefix_lens), int(self.is_causal), ws.ptr, need, _sh(stream))
         return out
