@@ -94,3 +94,23 @@ def test_products_a_step_of_32_bits_apart(rt, kind, d):
     else:
         got = ta.ScoredSdpa(is_causal=False).eval(q, k, v).to_numpy()
     assert np.isfinite(got).all() and got.min() >= 1.0 - 2.0**-11 and got.max() <= 2.0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("cap,scale", [(1e-30, 1e9), (1e-30, -1e30), (1e-6, 1e34), (2.0, 3e38)])
+@pytest.mark.parametrize("shape", [(1, 32, 8, 1000, 1000, 128), (1, 8, 2, 1, 900, 64), (1, 2, 1, 5, 40, 48)], ids=str)
+def test_scales_far_above_the_cap(rt, dtype, cap, scale, shape):
+    """A scale that f32 cannot hold once divided by the cap: a product of zero is still a score of zero, any other the cap or its opposite."""
+    b, hq, hkv, n, t, d = shape
+    if dtype == F32 and n == 1000:
+        b, hq, hkv, n, t, d = 1, 4, 2, 300, 300, 128
+    rng = np.random.default_rng(65)
+    q = np.zeros((b, hq, n, d), dtype)
+    q[:, ::2, :, 0] = 1.0
+    k = _rows(rng, (b, hkv, t, d), dtype)
+    k[..., 0] = rng.choice([-2.0, 2.0], (b, hkv, t))
+    v = _rows(rng, (b, hkv, t, d), dtype)
+    got = ta.ScoredSdpa(scale, cap).eval(q, k, v).to_numpy()
+    signs = np.sign(scale) * np.sign(k)
+    want = scored(q, signs.astype(dtype), v, scale=cap)    # the score: cap times the product's sign
+    assert_within(got, want[0], want[1] + 1e-6 * np.abs(v).max())

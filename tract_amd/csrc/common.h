@@ -287,6 +287,8 @@ int launch_sdpa_rows(const SdpaRowsArgs &a, hipStream_t s);
 constexpr int kRowsMaxD = 2048;   // the largest head size that it takes
 // tanh as 1 - 2 / (e^2x + 1) is off by about 1e-7, times the cap: up to this cap less than a f16 weight's own rounding.
 constexpr float kFastTanhCap = 512.0f;
+// A scale over a cap where f32 does not hold it: its largest, so that a product of zero stays zero and any other is past all caps.
+__host__ __device__ inline float within_f32(float x) { return fminf(fmaxf(x, -3.4028234e38f), 3.4028234e38f); }
 // f16 prompts of scored attention (sdpa_scored.hip); 2 = not covered.
 int launch_sdpa_scored_prompt(const SdpaRowsArgs &a, hipStream_t s);
 size_t sdpa_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Sq, int64_t D);

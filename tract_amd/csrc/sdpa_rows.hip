@@ -394,7 +394,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 #pragma unroll
         for (int j = 0; j < NI; j++) vpre[j] = load16<ONCE>(tv, (uint32_t)min(j * RPI + kr, most) * (uint32_t)wk.st + ch * 16);
     };
-    const float to_log2 = p.scale * kLog2e, cap_log2 = p.cap * kLog2e, to_cap = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
+    const float to_log2 = p.scale * kLog2e, cap_log2 = p.cap * kLog2e, to_cap = p.cap > 0.0f ? within_f32(p.scale / p.cap) : 0.0f;
     // key of score x of this lane, from the tile's first: groups of four consecutive ones
     auto key_of = [](int x) { return R == 16 ? 16 * (x >> 2) + (x & 3) : 8 * (x >> 2) + (x & 3); };   // + 4 grp
 

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
 
     // A score in the log2 domain is base + to_log2 s, of s the product with the key or, capped, 1 / (e^2x + 1) with x = scale q.k / cap:
     // cap log2e tanh(x) = A - 2 A / (e^2x + 1).  The largest score is the smallest s there.  Only weights take the whole sum.
-    const float base = CAP ? p.cap * kLog2e : 0.0f, to_log2 = CAP ? -2.0f * base : p.scale * kLog2e, cap_k = CAP ? p.scale / p.cap * (2.0f * kLog2e) : 0.0f;
+    const float base = CAP ? p.cap * kLog2e : 0.0f, to_log2 = CAP ? -2.0f * base : p.scale * kLog2e, cap_k = CAP ? within_f32(p.scale / p.cap * (2.0f * kLog2e)) : 0.0f;
     const float hidden = CAP ? INFINITY : -INFINITY, slope = SLOPES ? -kLog2e / to_log2 * p.slopes[kvh * p.G + g] : 0.0f;
     if (DOCS && doc < 0) lim = -1;   // padding sees nothing
     bool listed = false;
