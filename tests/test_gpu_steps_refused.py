@@ -66,3 +66,24 @@ def test_head_sizes_that_steps_with_norms_do_not_take(rt, dtype, n):
     with pytest.raises(ta.TractRocmError, match="head_dim 514"):
         op.eval_into(q, new, new)
     assert _state([op.k, op.v]) == before
+
+
+def test_a_scratch_over_the_inputs_of_a_step_with_norms(rt):
+    """Rows of normed queries and keys would lie over what is still to be read: refused before the caches grow."""
+    rng, d, n = np.random.default_rng(54), 64, 40
+    kc, vc = (_pushed(rng, (1, 2, 3, d), F16) for _ in range(2))
+    before = _state([kc, vc])
+    q, new = (ta.DeviceTensor.from_numpy(np.ones((1, h, n, d), F16)) for h in (4, 2))
+    cs, out = ta.DeviceTensor.from_numpy(np.ones((1, 1, n, d), F16)), ta.DeviceTensor((1, 4, n, d), F16)
+    room = ta.DeviceTensor((8 * n * d,), F16)
+    ws = ta.Workspace(1, 4, n, d)
+    at = room.ptr.value
+    for over in (dict(q=at + 256), dict(k=at), dict(cos=at + 512), dict(sin=at), dict(wq=at + 4 * n * d * 2)):
+        a = dict(q=q.ptr, k=new.ptr, wq=None, cos=cs.ptr, sin=cs.ptr) | over
+        with pytest.raises(ta.TractRocmError, match="overlap"):
+            ta._lib.call("trocm_inplace_kv_sdpa_eval_norm_rope", a["q"], a["k"], new.ptr, a["wq"], None, 1e-6, a["cos"], a["sin"], 0, 1, 4, n, None, None, None,
+                         kc.handle, vc.handle, out.ptr, float("nan"), 1, ws.ptr, ws.nbytes, room.ptr, room.nbytes, None)
+        assert _state([kc, vc]) == before, list(over)
+    ta._lib.call("trocm_inplace_kv_sdpa_eval_norm_rope", q.ptr, new.ptr, new.ptr, None, None, 1e-6, cs.ptr, cs.ptr, 0, 1, 4, n, None, None, None,
+                 kc.handle, vc.handle, out.ptr, float("nan"), 1, ws.ptr, ws.nbytes, room.ptr, room.nbytes, None)
+    assert kc.len() == vc.len() == 3 + n

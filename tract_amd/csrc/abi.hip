@@ -1698,15 +1698,12 @@ static int norm_rope_check(const char *what, const void *q, const void *k, float
     return 0;
 }
 
-int trocm_qk_norm_rope(const void *q, const void *k, const void *q_weight, const void *k_weight, float eps, const void *cos,
-                       const void *sin, int64_t cos_sin_batch_stride, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
-                       int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides, void *q_out, void *k_out,
-                       void *stream) {
-    if (norm_rope_check("qk_norm_rope", q, k, eps, cos, sin, cos_sin_batch_stride, dtype, batch, q_heads, kv_heads, n, head_dim, q_strides, k_strides)) return 1;
-    if (batch * n * head_dim == 0 || q_heads + kv_heads == 0) return 0;
+// The launch's arguments, behind norm_rope_check; refuses outputs over what other workgroups read.
+static int norm_rope_args(QkNormRopeArgs &a, const void *q, const void *k, const void *q_weight, const void *k_weight, float eps, const void *cos,
+                          const void *sin, int64_t cos_sin_batch_stride, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                          int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides, void *q_out, void *k_out) {
     TROCM_REQUIRE(q_out != nullptr || q_heads == 0, "unexpected null pointer argument: q_out");
     TROCM_REQUIRE(k_out != nullptr || kv_heads == 0, "unexpected null pointer argument: k_out");
-    QkNormRopeArgs a;
     a.x[0] = q, a.x[1] = k, a.w[0] = q_weight, a.w[1] = k_weight, a.y[0] = q_out, a.y[1] = k_out;
     a.H[0] = q_heads, a.H[1] = kv_heads;
     a.cos = cos, a.sin = sin, a.cs_stride_b = cos_sin_batch_stride, a.dtype = dtype;
@@ -1733,6 +1730,18 @@ int trocm_qk_norm_rope(const void *q, const void *k, const void *q_weight, const
             TROCM_REQUIRE(!other || !ranges_meet(a.y[i], out[i], other, (size_t)head_dim * es), "qk_norm_rope: an output overlaps a weight");
     }
     TROCM_REQUIRE(!out[0] || !out[1] || !ranges_meet(q_out, out[0], k_out, out[1]), "qk_norm_rope: q_out and k_out overlap");
+    return 0;
+}
+
+int trocm_qk_norm_rope(const void *q, const void *k, const void *q_weight, const void *k_weight, float eps, const void *cos,
+                       const void *sin, int64_t cos_sin_batch_stride, int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                       int64_t n, int64_t head_dim, const int64_t *q_strides, const int64_t *k_strides, void *q_out, void *k_out,
+                       void *stream) {
+    if (norm_rope_check("qk_norm_rope", q, k, eps, cos, sin, cos_sin_batch_stride, dtype, batch, q_heads, kv_heads, n, head_dim, q_strides, k_strides)) return 1;
+    if (batch * n * head_dim == 0 || q_heads + kv_heads == 0) return 0;
+    QkNormRopeArgs a;
+    if (norm_rope_args(a, q, k, q_weight, k_weight, eps, cos, sin, cos_sin_batch_stride, dtype, batch, q_heads, kv_heads, n, head_dim, q_strides, k_strides,
+                       q_out, k_out)) return 1;
     hipStream_t s;
     if (resolve_stream(stream, &s)) return 1;
     return launch_qk_norm_rope(a, s);
@@ -1768,10 +1777,12 @@ int trocm_inplace_kv_sdpa_eval_norm_rope(const void *q, const void *k_new, const
                                 "%s: rot_scratch overlaps v_new", what);
     else TROCM_REQUIRE(!ranges_meet(rot_scratch, q_room + k_bytes, v_new, k_bytes), "%s: rot_scratch overlaps v_new", what);
     TROCM_REQUIRE(!ranges_meet(rot_scratch, q_room + k_bytes, out, q_bytes), "%s: rot_scratch overlaps out", what);
+    QkNormRopeArgs a;
+    if (norm_rope_args(a, q, k_new, q_weight, k_weight, eps, cos, sin, cos_sin_batch_stride, dtype, kc->B, q_heads, kc->H, n_new, kc->D, q_strides, k_strides,
+                       q_rot, k_rot)) return 1;
     // room for the new tokens first: a call that finds no memory has changed nothing
     if (equalise_capacities(kc, vc, s) || append_prepare(kc, k_rot, dtype, dense, n_new, s) || append_prepare(vc, v_new, dtype, vs, n_new, s)) return 1;
-    if (trocm_qk_norm_rope(q, k_new, q_weight, k_weight, eps, cos, sin, cos_sin_batch_stride, dtype, kc->B, q_heads, kc->H, n_new, kc->D, q_strides,
-                           k_strides, q_rot, k_rot, stream)) return 1;
+    if (launch_qk_norm_rope(a, s)) return 1;
     if (v_dense)
         return trocm_inplace_kv_sdpa_eval(q_rot, k_rot, v_new, dtype, q_heads, n_new, nullptr, kc, vc, out, scale, causal, workspace, workspace_bytes, stream);
     if (trocm_kv_append(kc, k_rot, dtype, dense, n_new, stream) || trocm_kv_append(vc, v_new, dtype, vs, n_new, stream)) return 1;
