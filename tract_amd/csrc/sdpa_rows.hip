@@ -362,7 +362,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 #pragma unroll
         for (int r = 0; r < NA; r++) o[db][r] = 0.0f;
 
-    T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: R == 32)
+    T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: KL)
     const int kr = lane / LPRW, ch = lane % LPRW;
     constexpr int NK = !KL ? 2 * KS : NI;
     u32x4 kpre[NK], vpre[NI];
@@ -435,7 +435,7 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
                 }
 #pragma unroll
             for (int x = 0; x < NS; x++) s[x] = acc[x >> 2][x & 3];
-        } else if constexpr (R == 16) {
+        } else if constexpr (!KL) {
             float4_t acc[2];
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
@@ -444,14 +444,10 @@ __device__ __forceinline__ void rows_body(const RowsDev &p, const RowsWork &wk, 
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++) {
-                    if constexpr (H16) {
-                        acc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kpre[kb * KS + ks]), __builtin_bit_cast(half8_t, qf[ks]), acc[kb], 0, 0, 0);
-                    } else {   // (one feature of each group's four at a time)
-                        const float4_t a = __builtin_bit_cast(float4_t, kpre[kb * KS + ks]), c = __builtin_bit_cast(float4_t, qf[ks]);
+                for (int kb = 0; kb < 2; kb++) {   // (f32; one feature of each group's four at a time)
+                    const float4_t a = __builtin_bit_cast(float4_t, kpre[kb * KS + ks]), c = __builtin_bit_cast(float4_t, qf[ks]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[kb], 0, 0, 0);
-                    }
+                    for (int e = 0; e < 4; e++) acc[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[kb], 0, 0, 0);
                 }
 #pragma unroll
             for (int x = 0; x < NS; x++) s[x] = acc[x >> 2][x & 3];
