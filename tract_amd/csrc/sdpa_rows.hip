@@ -673,7 +673,7 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
             *reinterpret_cast<u32x4 *>(lds_v + buf * V_TILE + (key0 + j * RPI) * VROW + ch * 8) = vpre[j];
         }
     };
-    float m_run = -INFINITY, from = __builtin_nanf(""), s_ref = 0.0f, l_run = 0.0f;   // (a reference as sdpa_scored.hip has it)
+    float m_run = -INFINITY, s_ref = 0.0f, l_run = 0.0f;   // (a reference as sdpa_scored.hip has it: NaN from 2^20 on)
     float16_t o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -728,7 +728,7 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
             };
             bool look = n == 0;
             if (!look) {
-                weights(from);
+                weights(-m_run);
                 look = __builtin_amdgcn_ballot_w64(!(sum < 32768.0f)) != 0;
             }
             if (look) {
@@ -739,25 +739,24 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
                     for (int x = 0; x < 16; x++) top = fmaxf(top, s[kb][x]);
                 const float s_top = fmaxf(top, __shfl_xor(top, 32, 64));
                 top = s_top * to_log2;   // (scale > 0: the maximum commutes with it)
-                const bool far = from != from && m_run != -INFINITY, moved = top > m_run + 8.0f || (far && s_top > s_ref);
-                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(far ? (s_ref - s_top) * to_log2 : m_run - m_new) : 1.0f;
-                m_run = m_new;
-                if (moved) s_ref = s_top, from = fabsf(m_new) < 0x1p20f ? -m_new : __builtin_nanf("");
+                const bool far = m_run != m_run, moved = top > m_run + 8.0f || (far && s_top > s_ref);
+                const float keep = moved ? __builtin_amdgcn_exp2f(far ? (s_ref - s_top) * to_log2 : m_run - top) : 1.0f;
+                if (moved) s_ref = s_top, m_run = fabsf(top) < 0x1p20f ? top : __builtin_nanf("");
                 l_run *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) o[db][x] *= keep;
-                float f = from;
-                if (__builtin_expect(__builtin_amdgcn_ballot_w64(from != from) != 0, 0)) {
-                    const float less = from != from ? s_ref : 0.0f;   // (rows of ordinary scores stay as they are)
+                float from = -m_run;
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(m_run != m_run) != 0, 0)) {
+                    const float less = m_run != m_run ? s_ref : 0.0f;   // (rows of ordinary scores stay as they are)
 #pragma unroll
                     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                         for (int x = 0; x < 16; x++) s[kb][x] -= less;
-                    f = from != from ? 0.0f : from;
+                    if (m_run != m_run) from = 0.0f;
                 }
-                weights(f);
+                weights(from);
             }
             l_run += sum;
             const _Float16 *vsrc = lds_v + buf * V_TILE + (4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -775,6 +774,7 @@ __device__ __forceinline__ void tall_body(const RowsDev &p, const RowsWork &wk, 
         }
     }
     l_run += __shfl_xor(l_run, 32, 64);
+    if (m_run != m_run) m_run = s_ref * to_log2;
     if (my_row < wk.row_end) p.part_ml[((int64_t)wk.split * 2 + hb) * p.part_rows + out_row] = hb ? l_run : m_run;
     // rows to their places in whole lines, through a corner of LDS of the wave's own
     constexpr int CROW = D + 4, LPR = D / 4, RPS = 64 / LPR;

@@ -207,9 +207,9 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
     };
 
     // A row's reference: s_ref among the scores, m_run in the log2 domain.  What the rounding of m_run left out is a factor that all weights
-    // taken from it share, unless it is an exponent that f16 does not have: from 2^20 on every tile of the row gets a look (of it `from` is
-    // NaN), which takes weights from s_ref and moves it to whatever is larger.
-    float m_run = kNone, from = base - kNone, s_ref = 0.0f, l_run = 0.0f;
+    // taken from it share, unless it is an exponent that f16 does not have: from 2^20 on m_run is NaN up to the end, so that every tile of
+    // the row gets a look, which takes weights from s_ref and moves it to whatever is larger.
+    float m_run = kNone, s_ref = 0.0f, l_run = 0.0f;
     float16_t o[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
             };
             bool look = !DOCS && n == kg;   // (documents: weights against no reference come to infinity; asked for by place, the first tile spills scalar registers)
             if (!look) {
-                weights(from);
+                weights(base - m_run);
                 look = __builtin_amdgcn_ballot_w64(!(sum < 32768.0f)) != 0;
             }
             if (look) {
@@ -308,25 +308,24 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
                     for (int x = 0; x < 16; x++) top = CAP ? fminf(top, s[kb2][x]) : fmaxf(top, s[kb2][x]);
                 const float other = __shfl_xor(top, 32, 64), s_top = CAP ? fminf(top, other) : fmaxf(top, other);
                 top = __builtin_fmaf(s_top, to_log2, base);
-                const bool far = from != from, moved = top > m_run + 8.0f || (far && (CAP ? s_top < s_ref : s_top > s_ref));
-                const float m_new = moved ? top : m_run, keep = moved ? __builtin_amdgcn_exp2f(far ? (s_ref - s_top) * to_log2 : m_run - m_new) : 1.0f;
-                m_run = m_new;
-                if (moved) s_ref = s_top, from = fabsf(m_new) < 0x1p20f ? base - m_new : __builtin_nanf("");
+                const bool far = m_run != m_run, moved = top > m_run + 8.0f || (far && (CAP ? s_top < s_ref : s_top > s_ref));
+                const float keep = moved ? __builtin_amdgcn_exp2f(far ? (s_ref - s_top) * to_log2 : m_run - top) : 1.0f;
+                if (moved) s_ref = s_top, m_run = fabsf(top) < 0x1p20f ? top : __builtin_nanf("");
                 l_run *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int x = 0; x < 16; x++) o[db][x] *= keep;
-                float f = from;
-                if (__builtin_expect(__builtin_amdgcn_ballot_w64(from != from) != 0, 0)) {
-                    const float less = from != from ? s_ref : 0.0f;   // (rows of ordinary scores stay as they are)
+                float from = base - m_run;
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(m_run != m_run) != 0, 0)) {
+                    const float less = m_run != m_run ? s_ref : 0.0f;   // (rows of ordinary scores stay as they are)
 #pragma unroll
                     for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
                         for (int x = 0; x < 16; x++) s[kb2][x] -= less;
-                    f = from != from ? 0.0f : from;
+                    if (m_run != m_run) from = 0.0f;
                 }
-                weights(f);
+                weights(from);
             }
             l_run += sum;
             const _Float16 *vsrc = &lds_v[buf][(4 * hb + ((lane & 15) >> 2)) * VROW + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
@@ -344,6 +343,7 @@ __global__ __launch_bounds__(256 * NK, D == 128 || NK == 2 ? 2 : 3) void sdpa_sc
         }
     }
     l_run += __shfl_xor(l_run, 32, 64);
+    if (NK == 2 && m_run != m_run) m_run = __builtin_fmaf(s_ref, to_log2, base);
 
     if constexpr (NK == 2) {   // the second group's rows join the first's, through the tiles' LDS
         float *comb = reinterpret_cast<float *>(&lds_all[0][0]) + w * 32 * JROW, *comb_ml = reinterpret_cast<float *>(&lds_all[0][0]) + kWaves * 32 * JROW + w * 64;
