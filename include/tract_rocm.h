@@ -526,7 +526,7 @@ int trocm_inplace_kv_sdpa_eval_shared(const void *q, const void *k_new, const vo
  *   (not causal, or j <= i + (kv_len - q_len), or j < prefix_lens[b])
  *   and, with documents, both tokens are of one document: documents[b][j] == documents[b][i + kv_len - q_len] >= 0.
  *   softcap     : 0 (none) or 1e-30..1e30
- *   slopes      : [q_heads] f32, device memory, or NULL; any sign, at most 1e30 in size (1e38 times the longest distance)
+ *   slopes      : [q_heads] f32, device memory, or NULL; any sign, at most 1e30 in size, the longest distance multiplied in at most 1e38
  *   documents   : [batch, kv_len] int32, device memory, or NULL; ids in any order, negative ones are padding that nothing sees
  *                 and whose K and V rows may hold anything; needs kv_len >= q_len
  *   prefix_lens : [batch] int32, device memory, or NULL; values past kv_len mean all of it, negative ones none; read only when causal

@@ -9,11 +9,16 @@
 // at the end.  Two workgroups (head size 64: three) share a compute unit without knowing of each
 // other, so that one's softmax runs beside the other's MFMAs.
 //
-// What bounds it: the sum of a SIMD's vector and matrix streams, which take turns.  4096 queries of 32 heads over 8, 128 features, capped: 188 us
-// (731 TFLOP/s of visible products; a large product alone reaches 1176), vector instructions 53 % of the cycles and matrix instructions 35 %.  Per
+// What bounds it: the sum of a SIMD's vector and matrix streams, which take turns.  4096 queries of 32 heads over 8, 128 features, capped: 187 to 194 us
+// from card to card (709 to 735 TFLOP/s of visible products; a large product alone reaches 1176), vector instructions 53 % of the cycles and matrix
+// instructions 34 %.  Per
 // 64 scores the cap takes two of the three exponentials and reciprocals (8 cycles each) and two of the four other instructions (4).
-// 64 heads of 64 features 221 us.  Two batches of 4096 in 9 documents, 14 heads over 2, 64 features, with slopes: 49 us; there the compute
-// units have unlike shares (on average 27 tiles, 49 at most); in 40 documents, where a workgroup's start and end are most of it, 22.5 us.
+// 64 heads of 64 features 221 us.  Two batches of 4096 in 9 documents, 14 heads over 2, 64 features, with slopes: 50 us; there the compute
+// units have unlike shares (on average 27 tiles, 49 at most); in 40 documents, where a workgroup's start and end are most of it, 23 us.
+//
+// Weights are rounded to f16, half a step each, since the product with V takes f16 operands: what is left of them would be a second product, and
+// the matrix stream is a third of the time.  The row's sum takes the rounded weights, so that a row of equal values stays that value.  Against 64
+// bits outputs are off by 2.3e-4 (2-norm, relative), of which the rounding of the result is 2.1e-4.  All else is f32.
 #include <hip/hip_fp16.h>
 #include <limits.h>
 #include <string.h>
