@@ -543,6 +543,90 @@ int trocm_sdpa_cached_scored(const void *q, int q_dtype, int64_t q_heads, int64_
                              const int32_t *documents, const int32_t *prefix_lens, int causal, void *workspace,
                              size_t workspace_bytes, void *stream);
 
+/* ---- pages: sequences whose keys and values lie in pages of one pool ---------------------------------------------
+ * Where the caches above hold a sequence's tokens in planes of its own, these entry points take pages of `page_size` tokens,
+ * K and V each a tensor [n_pages, kv_heads, page_size, head_dim] (element strides page_strides[3] for page, head and token, the
+ * same for both; NULL: dense), one pair per layer, and one table for all layers: table[i][p] is the page that holds tokens
+ * p * page_size .. of sequence i.  Lengths, tables, the stack of free pages and the counts of holders are int32 device memory of the
+ * caller's, read and written by kernels only, so that a recorded step can be replayed.  No counterpart in the reference, whose caches
+ * are a tensor per sequence (gpu/src/ops/dyn_kv_cache.rs:58-113).  F32 and F16.
+ *
+ * Every id that comes from device memory is checked there: a page outside 0 .. n_pages - 1 is a hole (its keys are not seen, rows for
+ * it are not stored), and a length outside 0 .. table_width * page_size is taken as the nearest of those for attention and refused by
+ * the plan.  n_pages * page_size, and a table's row of tokens, at most 2^30; page_size at most 2^20 and page_size * head_dim at most
+ * 2^29; plan and reorder take up to 4096 sequences. */
+
+/* Pages for the tokens that a step adds, and where each token goes.  Sequence i holds lens[i] tokens and gets n_new[i] more (0: none),
+ * which are rows starts[i] .. of the step's n_tokens packed rows (sequences one behind the other, in order).
+ *   table          : [n_seq, table_width]; the pages that the step adds are written behind the ceil(lens / page_size) held ones
+ *   free_pages     : [n_pages], of which the first *free_count are free; pages are taken from the end, in the sequences' order
+ *   refs           : [n_pages] or NULL; 1 for every page taken
+ *   lens_out       : [n_seq]; starts: [n_seq + 1] or NULL; free_count_out, refused: one each
+ *   slots          : [n_tokens], page * page_size + place, -1 for rows that go nowhere; positions: [n_tokens] or NULL, -1 likewise
+ * A sequence is refused (no pages, no slots, its length stays; counted in *refused) where the free pages, the table's row or the packed
+ * rows do not suffice for it, or its length or addition is negative.  Where the free pages do not suffice for one, they do not for any
+ * later one that needs some.  Outputs may not overlap inputs or each other (sums of additions stop at 2^30). */
+int trocm_paged_plan(const int32_t *lens, const int32_t *n_new, int64_t n_seq, int64_t page_size, int32_t *table,
+                     int64_t table_width, const int32_t *free_pages, const int32_t *free_count, int64_t n_pages, int32_t *refs,
+                     int64_t n_tokens, int32_t *lens_out, int32_t *starts, int32_t *slots, int32_t *positions,
+                     int32_t *free_count_out, int32_t *refused, void *stream);
+
+/* Rows of K and V into their pages: row t of k_new and v_new ([n_tokens, kv_heads, head_dim], element strides k_strides[2] and
+ * v_strides[2] for token and head; NULL: dense) goes to slots[t].  Slots outside 0 .. n_pages * page_size - 1 store nothing; of rows
+ * with the same slot any may stay, piece by piece. */
+int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t n_tokens, int64_t kv_heads, int64_t head_dim,
+                       const int64_t *k_strides, const int64_t *v_strides, const int32_t *slots, void *k_pages, void *v_pages,
+                       int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream);
+
+/* Attention of q_len new tokens of every sequence over its pages: out = softmax(scale q k^T) v over the first lens[i] tokens, which
+ * count the new ones; causal: query r sees tokens up to lens[i] - q_len + r.  A row that sees nothing is zeros.  What lies behind a
+ * sequence's last token, in pages that are not its own and in holes may hold anything; tokens that are hidden by causality alone must be finite.
+ *   q, out    : [n_seq, q_heads, q_len, head_dim] dense, not overlapping; q_heads a multiple of kv_heads
+ *   workspace : trocm_sdpa_paged_workspace_bytes, initialised by trocm_sdpa_workspace_init and shared like any other; with a smaller
+ *               one or NULL a slow kernel runs
+ * Fast kernels: head_dim 64 and 128, page_size a multiple of 16, bases and strides multiples of 16 bytes, q_heads / kv_heads * q_len rows
+ * of a kv head as tiles of 16; anything else up to head_dim 2048 is correct and slow. */
+int trocm_sdpa_paged_workspace_bytes(int64_t n_seq, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t head_dim,
+                                     size_t *bytes);
+int trocm_sdpa_paged(const void *q, int dtype, int64_t n_seq, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t head_dim,
+                     const void *k_pages, const void *v_pages, int64_t n_pages, int64_t page_size, const int64_t *page_strides,
+                     const int32_t *table, int64_t table_width, const int32_t *lens, void *out, float scale, int causal,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
+/* Sequences that go on from other sequences (beams): sequence j takes the length and pages of sequence parents[j] (outside of
+ * 0 .. n_seq - 1: it is empty).  Full pages are shared; the partial last page stays with the first of a parent's children (if refs says
+ * that the parent alone holds it) and every other child gets a free page for a copy of it.  refs counts a page's holders; pages that
+ * nobody holds any more go onto the stack, in ascending order.
+ *   table_out      : like table, -1 behind a sequence's pages; lens_out, refs_out, free_pages_out (-1 behind the free ones), free_count_out
+ *   copies         : [n_seq, 3]: source page, destination page and tokens for trocm_paged_copy, (-1, -1, 0) where nothing is copied
+ *   missing        : 0, or how many free pages were missing for the copies: then all outputs are as the inputs, and nothing is copied
+ * Outputs may not overlap inputs or each other. */
+int trocm_paged_reorder(const int32_t *parents, int64_t n_seq, int64_t page_size, const int32_t *table, int64_t table_width,
+                        const int32_t *lens, const int32_t *refs, const int32_t *free_pages, const int32_t *free_count,
+                        int64_t n_pages, int32_t *table_out, int32_t *lens_out, int32_t *refs_out, int32_t *free_pages_out,
+                        int32_t *free_count_out, int32_t *copies, int32_t *missing, void *stream);
+
+/* The first `tokens` rows of every head from the source page to the destination page of each of n_copies entries, in each of n_pools
+ * pools (a HOST array of device pointers: the K and the V pages of all layers, all of one shape and page_strides).  Entries with a page
+ * outside of the pool are skipped; no destination may be another entry's source or destination. */
+int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools, int64_t n_pools, int dtype, int64_t kv_heads,
+                     int64_t head_dim, int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream);
+
+/* Beam search's choice.  For every request: of all c = scores[b] + logits[b][v] - log(sum over u of exp(logits[b][u])) over its `beams`
+ * beams and the vocabulary the `keep` largest, largest first, equal ones by ascending beam * vocab + token; c is compared in 64 bits.
+ *   logits     : rows of `vocab` for batch * beams beams, row_stride elements apart (0: dense)
+ *   scores     : [batch, beams] f32; one that is infinite or NaN leaves its beam only candidates of -inf, and so do logits without a finite largest one
+ *   ended      : [batch, beams] int32 or NULL: a beam with one that is not 0 has a single candidate, its score as it is with token `eos`
+ *   eos        : -1 (none; `ended` must be NULL) or a token
+ *   outputs    : [batch, keep]: scores_out f32, parents (rows of the batch: request * beams + beam), tokens, ended_out (or NULL: 1 where the token
+ *                is eos or the parent had ended).  May not overlap inputs
+ *   workspace  : trocm_beam_select_workspace_bytes, needs no initialisation
+ * A NaN among the logits counts as -inf.  keep and beams up to 64, keep at most beams * vocab, vocab up to 2^30, beams * vocab below 2^31. */
+int trocm_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep, size_t *bytes);
+int trocm_beam_select(const void *logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,
+                      const float *scores, const int32_t *ended, int32_t eos, int64_t keep, float *scores_out, int32_t *parents,
+                      int32_t *tokens, int32_t *ended_out, void *workspace, size_t workspace_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

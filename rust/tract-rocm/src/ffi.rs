@@ -119,6 +119,14 @@ extern "C" {
     pub fn trocm_inplace_kv_sdpa_eval_shared(q: *const c_void, k_new: *const c_void, v_new: *const c_void, dtype: c_int, q_heads: i64, n_seq: i64, n_new: i64, prefix_k_cache: *const trocm_kv_cache, prefix_v_cache: *const trocm_kv_cache, k_caches: *const *mut trocm_kv_cache, v_caches: *const *mut trocm_kv_cache, out: *mut c_void, scale: f32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn trocm_sdpa_scored(q: *const c_void, k: *const c_void, v: *const c_void, out: *mut c_void, dtype: c_int, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, kv_strides: *const i64, scale: f32, softcap: f32, slopes: *const f32, documents: *const i32, prefix_lens: *const i32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn trocm_sdpa_cached_scored(q: *const c_void, q_dtype: c_int, q_heads: i64, q_len: i64, k_cache: *const trocm_kv_cache, v_cache: *const trocm_kv_cache, out: *mut c_void, scale: f32, softcap: f32, slopes: *const f32, documents: *const i32, prefix_lens: *const i32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn trocm_paged_plan(lens: *const i32, n_new: *const i32, n_seq: i64, page_size: i64, table: *mut i32, table_width: i64, free_pages: *const i32, free_count: *const i32, n_pages: i64, refs: *mut i32, n_tokens: i64, lens_out: *mut i32, starts: *mut i32, slots: *mut i32, positions: *mut i32, free_count_out: *mut i32, refused: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn trocm_paged_append(k_new: *const c_void, v_new: *const c_void, dtype: c_int, n_tokens: i64, kv_heads: i64, head_dim: i64, k_strides: *const i64, v_strides: *const i64, slots: *const i32, k_pages: *mut c_void, v_pages: *mut c_void, n_pages: i64, page_size: i64, page_strides: *const i64, stream: *mut c_void) -> c_int;
+    pub fn trocm_sdpa_paged_workspace_bytes(n_seq: i64, q_heads: i64, kv_heads: i64, q_len: i64, head_dim: i64, bytes: *mut usize) -> c_int;
+    pub fn trocm_sdpa_paged(q: *const c_void, dtype: c_int, n_seq: i64, q_heads: i64, kv_heads: i64, q_len: i64, head_dim: i64, k_pages: *const c_void, v_pages: *const c_void, n_pages: i64, page_size: i64, page_strides: *const i64, table: *const i32, table_width: i64, lens: *const i32, out: *mut c_void, scale: f32, causal: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn trocm_paged_reorder(parents: *const i32, n_seq: i64, page_size: i64, table: *const i32, table_width: i64, lens: *const i32, refs: *const i32, free_pages: *const i32, free_count: *const i32, n_pages: i64, table_out: *mut i32, lens_out: *mut i32, refs_out: *mut i32, free_pages_out: *mut i32, free_count_out: *mut i32, copies: *mut i32, missing: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn trocm_paged_copy(copies: *const i32, n_copies: i64, pools: *const *mut c_void, n_pools: i64, dtype: c_int, kv_heads: i64, head_dim: i64, n_pages: i64, page_size: i64, page_strides: *const i64, stream: *mut c_void) -> c_int;
+    pub fn trocm_beam_select_workspace_bytes(batch: i64, beams: i64, vocab: i64, keep: i64, bytes: *mut usize) -> c_int;
+    pub fn trocm_beam_select(logits: *const c_void, dtype: c_int, batch: i64, beams: i64, vocab: i64, row_stride: i64, scores: *const f32, ended: *const i32, eos: i32, keep: i64, scores_out: *mut f32, parents: *mut i32, tokens: *mut i32, ended_out: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
 }
 
 /// KO -> an error that carries the library's message.

@@ -1,0 +1,373 @@
+"""Tables, appends, reordering and attention over pages against plain restatements (tests/paged_ref.py)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import tract_amd as ta
+from tests import paged_ref as ref
+from tests.attention_ref import assert_within
+from tests.gpu_util import rt  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+F16, F32, I32 = np.float16, np.float32, np.int32
+up = ta.DeviceTensor.from_numpy
+
+
+def ints(x):
+    return up(np.asarray(x, I32))
+
+
+# ---- plan --------------------------------------------------------------------------------------------------
+
+
+def _tables(rng, lens, page, width, n_pages):
+    order = rng.permutation(n_pages).astype(I32)
+    table, at = np.full((len(lens), width), -1, I32), 0
+    for i, n in enumerate(lens):
+        held = min(-(-max(int(n), 0) // page), width)
+        table[i, :held] = order[at:at + held]
+        at += held
+    free = np.full(n_pages, -1, I32)
+    free[:n_pages - at] = order[at:]
+    return table, free, n_pages - at
+
+
+def _check_plan(lens, new, page, width, n_pages, tokens, count=None, seed=0, with_refs=True):
+    rng = np.random.default_rng(seed)
+    table, free, there = _tables(rng, lens, page, width, n_pages)
+    count = there if count is None else count
+    refs = np.zeros(n_pages, I32)
+    want = ref.plan(lens, new, table, free, count, n_pages, page, tokens, refs if with_refs else None)
+    d_table, d_refs = up(table), up(refs) if with_refs else None
+    got = ta.PagedPlan(page).eval(ints(lens), ints(new), d_table, up(free), ints([count]), tokens, refs=d_refs)
+    for name in ("lens", "starts", "slots", "positions", "free_count", "refused"):
+        np.testing.assert_array_equal(got[name].to_numpy(), want[name], err_msg=name)
+    np.testing.assert_array_equal(d_table.to_numpy(), want["table"])
+    if with_refs:
+        np.testing.assert_array_equal(d_refs.to_numpy(), want["refs"])
+    return want
+
+
+@pytest.mark.parametrize("n,longest,most,page", [(1, 0, 1, 16), (1, 100, 1, 1), (3, 40, 5, 7), (64, 500, 1, 16), (257, 300, 9, 32), (1500, 90, 3, 16), (4096, 40, 2, 5), (70, 2000, 300, 64)])
+def test_plan(rt, n, longest, most, page):
+    rng = np.random.default_rng(n)
+    lens, new = rng.integers(0, longest, n, endpoint=True), rng.integers(0, most, n, endpoint=True)
+    width = -(-(longest + most) // page) + 1
+    n_pages = int(sum(-(-(a + b) // page) for a, b in zip(lens, new))) + 3
+    for tokens in {int(new.sum()), int(new.sum()) + 11}:
+        assert _check_plan(lens, new, page, width, n_pages, tokens, seed=n)["refused"][0] == 0
+    _check_plan(lens, new, page, width, n_pages, int(new.sum()), seed=n, with_refs=False)
+
+
+def test_plan_refuses_what_does_not_fit(rt):
+    page, width = 4, 3
+    lens, new = [3, 12, 4, 11, -1, 5, 5, 0, 8], [2, 1, 0, 1, 3, -2, 2, 9, 4]
+    for count in (0, 1, 2, 4, 5, 6, 100, -3):
+        for tokens in (0, 3, 8, 9, 18, 30):
+            _check_plan(lens, new, page, width, 40, tokens, count=min(count, 20))
+    assert _check_plan(lens, new, page, width, 40, 30)["refused"][0] == 3
+    big = 1 << 30
+    _check_plan([5, big, 2 ** 31 - 1, 7], [2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 1], page, width, 40, 30)      # (sums that would leave 32 bits)
+    _check_plan([5, 2, 7], [big, 1, 1], page, width, 40, 30)
+
+
+def test_plan_without_sequences_or_tokens(rt):
+    _check_plan([], [], 16, 4, 8, 5)
+    _check_plan([3, 4], [0, 0], 16, 4, 8, 0)
+    _check_plan([0, 0], [0, 0], 16, 0, 0, 0)
+
+
+def test_plan_over_holes_and_ids_that_are_no_pages(rt):
+    """A partial page that is a hole gets no slots; free ids outside of the pool are handed out as they are, and stored for nobody."""
+    page = 4
+    table, free = np.array([[-1, -1, -1], [7, 99, -1]], I32), np.array([5, 400, -2, 6], I32)
+    want = ref.plan([2, 6], [4, 4], table, free, 4, 10, page, 8, np.zeros(10, I32))
+    free10 = np.full(10, -1, I32)
+    free10[:4] = free
+    d_table, refs = up(table), up(np.zeros(10, I32))
+    got = ta.PagedPlan(page).eval(ints([2, 6]), ints([4, 4]), d_table, up(free10), ints([4]), 8, refs=refs)
+    np.testing.assert_array_equal(got["slots"].to_numpy(), want["slots"])
+    np.testing.assert_array_equal(d_table.to_numpy(), want["table"])
+    np.testing.assert_array_equal(refs.to_numpy(), want["refs"])
+    assert (want["slots"][:2] == -1).all() and want["slots"][2] == 6 * 4
+
+
+# ---- append ----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("tokens,heads,d,page", [(1, 1, 64, 16), (5, 2, 128, 16), (33, 3, 7, 5), (700, 8, 128, 32), (64, 2, 63, 16), (9, 70, 2, 1), (3, 1, 2050, 4)])
+def test_append(rt, dtype, tokens, heads, d, page):
+    rng = np.random.default_rng(tokens)
+    n_pages = tokens // page + 3
+    pools = [rng.standard_normal((n_pages, heads, page, d)).astype(dtype) for _ in range(2)]
+    rows = [rng.standard_normal((tokens, heads, d)).astype(dtype) for _ in range(2)]
+    slots = rng.permutation(n_pages * page)[:tokens].astype(I32)
+    slots[::7] = [-1, n_pages * page, 2 ** 31 - 1, -2 ** 31][tokens % 4]      # (nowhere)
+    dk, dv = (up(p) for p in pools)
+    ta.PagedAppend().eval(up(rows[0]), up(rows[1]), up(slots), dk, dv)
+    for got, r, p in ((dk, rows[0], pools[0]), (dv, rows[1], pools[1])):
+        assert got.to_numpy().tobytes() == ref.append(r, p, slots).tobytes()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,skew", [(128, 0), (64, 1), (66, 0), (64, 8)])
+def test_append_of_views_into_pools_of_other_orders(rt, dtype, d, skew):
+    """Rows of a fused projection, and pages laid out [n_pages, page, heads, head_dim] behind an offset."""
+    rng, tokens, heads, page, n_pages = np.random.default_rng(5), 21, 3, 8, 6
+    fused = rng.standard_normal((tokens, 9 * d + skew)).astype(dtype)
+    size = fused.itemsize
+    pools = [rng.standard_normal((n_pages, page, heads, d)).astype(dtype) for _ in range(2)]
+    slots = rng.permutation(n_pages * page)[:tokens].astype(I32)
+    base, dk, dv = up(fused), up(pools[0]), up(pools[1])
+    view = lambda at: ta.DeviceTensor((tokens, heads, d), dtype, ptr=base.ptr.value + at * size, owner=base)  # noqa: E731
+    shaped = lambda t: ta.DeviceTensor((n_pages, heads, page, d), dtype, ptr=t.ptr.value, owner=t)  # noqa: E731
+    ta.PagedAppend().eval(view(3 * d), view(6 * d + skew), up(slots), shaped(dk), shaped(dv), k_strides=(9 * d + skew, d), v_strides=(9 * d + skew, d),
+                          page_strides=(page * heads * d, d, heads * d))
+    for got, at, p in ((dk, 3 * d, pools[0]), (dv, 6 * d + skew, pools[1])):
+        rows = fused[:, at:at + 3 * d].reshape(tokens, heads, d)
+        assert got.to_numpy().tobytes() == ref.append(rows, p.transpose(0, 2, 1, 3), slots).transpose(0, 2, 1, 3).tobytes()
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------
+
+
+def _attend(rng, lens, hq, hkv, sq, d, page, dtype, width=None, garbage=True, holes=0.0, page_order="heads", scale=None, causal=True, spare=3, offset=0):
+    lens = np.asarray(lens, I32)
+    held = np.array([-(-max(int(n), 0) // page) for n in lens])
+    width = int(held.max(initial=0)) if width is None else width
+    n_pages = int(np.minimum(held, width).sum()) + spare
+    order = rng.permutation(n_pages).astype(I32)
+    table, at = rng.integers(-5, n_pages + 5, (len(lens), width)).astype(I32), 0      # (anything behind a sequence's pages)
+    k, v = (rng.standard_normal((n_pages, hkv, page, d)).astype(dtype) for _ in range(2))
+    used = np.zeros((n_pages, page), bool)
+    for i, n in enumerate(lens):
+        h = min(held[i], width)
+        table[i, :h] = order[at:at + h]
+        at += h
+        for p in range(h):
+            used[table[i, p], :max(0, int(n) - p * page)] = True
+    if garbage:   # what belongs to no sequence may hold anything
+        for pool in (k, v):
+            pool.transpose(0, 2, 1, 3)[~used] = np.array([np.nan, np.inf, -np.inf])[rng.integers(0, 3, (int((~used).sum()), hkv, d))].astype(dtype)
+    if holes:
+        cut = rng.random(table.shape) < holes
+        table[cut] = rng.choice([-1, n_pages, 2 ** 31 - 1, -2 ** 31], int(cut.sum()))
+    q = (rng.standard_normal((len(lens), hq, sq, d)) * 2).astype(dtype)
+    want, bound = ref.attend(q, k, v, table, lens, scale=scale, causal=causal)
+
+    def pool(x):
+        if page_order == "tokens":
+            x = np.ascontiguousarray(x.transpose(0, 2, 1, 3))
+        base = up(np.concatenate([np.zeros(offset, dtype), x.reshape(-1)]))
+        return ta.DeviceTensor((n_pages, hkv, page, d), dtype, ptr=base.ptr.value + offset * x.itemsize, owner=base)
+
+    strides = (hkv * page * d, d, hkv * d) if page_order == "tokens" else None
+    out = up(np.full(q.shape, np.nan, dtype))
+    got = ta.PagedSdpa(scale, is_causal=causal).eval(up(q), pool(k), pool(v), up(table.reshape(len(lens), width)), up(lens), out=out, page_strides=strides).to_numpy()
+    assert_within(got, want, bound, f"{lens.tolist()[:6]} {hq}/{hkv} {sq} {d} {page} {np.dtype(dtype).name}")
+
+
+HEADS = [(1, 1), (2, 1), (4, 1), (14, 2), (8, 8), (32, 2), (6, 2)]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("page", [16, 32, 48, 128])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_lengths(rt, dtype, page, d):
+    """Every length around a tile and a page, one after the other, and none."""
+    rng = np.random.default_rng(page + d)
+    _attend(rng, [1], 4, 2, 1, d, page, dtype)
+    _attend(rng, [0], 4, 2, 1, d, page, dtype)
+    _attend(rng, [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 0, 127, 128, 129, 130, 255, 256, 257], 4, 2, 1, d, page, dtype)
+    _attend(rng, [2000, 0, 3, 777, 1, 1300], 8, 2, 1, d, page, dtype, width=2100 // page + 4)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_attend_heads(rt, dtype, hq, hkv):
+    rng = np.random.default_rng(hq)
+    for d in (64, 128):
+        _attend(rng, [300, 17, 0, 129], hq, hkv, 1, d, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("sq", [2, 3, 5, 16, 17, 40])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_several_queries(rt, dtype, sq, causal):
+    """Sequences that hold fewer tokens than they have queries leave rows empty."""
+    rng = np.random.default_rng(sq)
+    _attend(rng, [sq, 300, sq - 1, 1, 0, 64, 65 + sq], 8, 2, sq, 128, 16, dtype, causal=causal, garbage=True)
+    _attend(rng, [200, 1000], 14, 2, sq, 64, 32, dtype, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,page,offset", [(80, 16, 0), (128, 1, 0), (128, 7, 0), (64, 24, 0), (128, 16, 1), (64, 16, 4), (2, 3, 0), (2048, 4, 0), (1, 16, 0)])
+def test_attend_any_size(rt, dtype, d, page, offset):
+    rng = np.random.default_rng(d)
+    _attend(rng, [0, 1, 40, 97], 4, 2, 1, d, page, dtype, offset=offset)
+    _attend(rng, [5, 40], 4, 1, 3, d, page, dtype, offset=offset)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("sq", [1, 4])
+@pytest.mark.parametrize("page", [16, 32, 64, 5])
+def test_attend_over_holes(rt, dtype, sq, page):
+    """Entries that are no pages hide their tokens; a sequence of holes alone is zeros."""
+    rng = np.random.default_rng(page)
+    _attend(rng, [500, 64, 33, 700, 1, 16], 8, 2, sq, 128, page, dtype, holes=0.4)
+    _attend(rng, [500, 64, 1200], 8, 2, sq, 64, page, dtype, holes=0.95)
+    _attend(rng, [500, 64], 8, 2, sq, 64, page, dtype, holes=1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_pages_in_token_order(rt, dtype):
+    rng = np.random.default_rng(3)
+    for d, page in ((128, 16), (64, 64), (64, 9)):
+        _attend(rng, [300, 0, 1, 95, 600], 8, 2, 1, d, page, dtype, page_order="tokens")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_many_sequences(rt, dtype):
+    rng = np.random.default_rng(4)
+    _attend(rng, rng.integers(0, 90, 400), 8, 2, 1, 64, 16, dtype)
+    _attend(rng, rng.integers(0, 20, 3000), 2, 1, 1, 64, 16, dtype)
+    _attend(rng, [0] * 300 + [3] + [0] * 300, 4, 2, 1, 64, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_long(rt, dtype):
+    rng = np.random.default_rng(6)
+    _attend(rng, [20011], 4, 2, 1, 128, 16, dtype)
+    _attend(rng, [9000, 1, 12000, 0, 8000], 4, 1, 2, 64, 64, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_lengths_that_the_table_has_no_pages_for(rt, dtype):
+    """Taken as the nearest that it has."""
+    rng = np.random.default_rng(7)
+    _attend(rng, [100, -5, 2 ** 31 - 1, 64, -2 ** 31], 4, 2, 1, 64, 16, dtype, width=4)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_scales_and_sizes_of_scores(rt, dtype):
+    rng = np.random.default_rng(8)
+    _attend(rng, [300, 40], 4, 2, 1, 128, 16, dtype, scale=3.0)
+    _attend(rng, [300, 40], 4, 2, 1, 64, 16, dtype, scale=0.0)
+    _attend(rng, [300, 40], 4, 2, 1, 64, 16, dtype, scale=-1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128, 40])
+def test_rows_that_are_not_numbers_stay_so(rt, dtype, d):
+    """A query of NaN is the row that shows it; a value of NaN that is seen shows in every row that sees it."""
+    rng = np.random.default_rng(9)
+    lens, page = [3000, 40], 16
+    n_pages = 188 + 3
+    table = np.full((2, 188), -1, I32)
+    table[0], table[1, :3] = np.arange(188), [188, 189, 190]
+    q, k, v = (rng.standard_normal(s).astype(dtype) for s in ((2, 4, 1, d), (n_pages, 2, page, d), (n_pages, 2, page, d)))
+    clean = ta.PagedSdpa().eval(up(q), up(k), up(v), up(table), ints(lens)).to_numpy()
+    q[0, 1, 0, 3] = np.nan
+    v[189, 1, 5, 7] = np.nan
+    got = ta.PagedSdpa().eval(up(q), up(k), up(v), up(table), ints(lens)).to_numpy()
+    assert np.isnan(got[0, 1]).all() and np.isnan(got[1, 2:, 0, 7]).all()
+    for at in (np.s_[0, 0], np.s_[0, 2:], np.s_[1, :2]):
+        assert got[at].tobytes() == clean[at].tobytes()
+
+
+# ---- sequences that go on from others -----------------------------------------------------------------------------------
+
+
+def _check_reorder(parents, table, lens, refs, free, count, page):
+    want = ref.reorder(parents, table, lens, refs, free, count, page)
+    got = ta.PagedReorder(page).eval(ints(parents), up(table), up(lens), up(refs), up(free), ints([count]))
+    for name, w in want.items():
+        np.testing.assert_array_equal(got[name].to_numpy(), w, err_msg=name)
+    return want
+
+
+@pytest.mark.parametrize("n,longest,page,spare", [(1, 20, 16, 2), (4, 100, 16, 10), (9, 50, 4, 9), (64, 300, 16, 70), (257, 60, 7, 300), (3000, 30, 8, 3000), (12, 9000, 1, 40000)])
+def test_reorder(rt, n, longest, page, spare):
+    """Several steps one after the other, each from what the last one left; places without a parent among them."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, longest, n, endpoint=True).astype(I32)
+    width, n_pages = -(-longest // page) + 1, int((-(-lens // page)).sum()) + spare
+    table, free, count = _tables(rng, lens, page, width, n_pages)
+    refs = np.zeros(n_pages, I32)
+    refs[table[table >= 0]] = 1
+    for step in range(4):
+        parents = rng.integers(-1 if step % 2 else 0, n, n)
+        if step == 2:
+            parents = np.arange(n)
+        w = _check_reorder(parents, table, lens, refs, free, count, page)
+        assert w["missing"][0] == 0
+        table, lens, refs, free, count = w["table"], w["lens"], w["refs"], w["free_pages"], int(w["free_count"][0])
+        held = np.bincount(table[table >= 0], minlength=n_pages)
+        np.testing.assert_array_equal(held, refs)          # every page is held, or free, exactly once
+        assert sorted(free[:count]) == list(np.flatnonzero(held == 0))
+
+
+def test_reorder_without_enough_free_pages_changes_nothing(rt):
+    rng = np.random.default_rng(1)
+    lens = np.array([5, 9, 3], I32)
+    table, free, count = _tables(rng, lens, 4, 4, 8)
+    refs = np.zeros(8, I32)
+    refs[table[table >= 0]] = 1
+    w = _check_reorder([0, 0, 0], table, lens, refs, free, 1, 4)
+    assert w["missing"][0] == 1
+    _check_reorder([0, 0, 0], table, lens, refs, free, 2, 4)
+    _check_reorder([7, -1, -9], table, lens, refs, free, 2, 4)
+
+
+def test_reorder_of_pages_that_others_hold_and_of_holes(rt):
+    """A partial page that has another holder is copied for all children; holes and ids that are no pages stay where they are."""
+    table = np.array([[0, 1, 2, -1], [0, 1, 3, -1], [5, -1, 4, -1], [6, 99, -1, -1]], I32)
+    lens, refs = np.array([10, 11, 9, 7], I32), np.array([2, 2, 2, 1, 1, 1, 1, 0, 0, 0, 0, 0], I32)
+    free = np.array([7, 8, 9, 10, 11] + [-1] * 7, I32)
+    for parents in ([0, 0, 1, 2], [3, 3, 2, 0], [0, 1, 2, 3], [-1, -1, -1, -1], [2, 2, 2, 2]):
+        _check_reorder(parents, table, lens, refs, free, 5, 4)
+
+
+def test_reorder_of_nothing(rt):
+    empty, none = np.zeros((0, 3), I32), np.zeros(0, I32)
+    _check_reorder([], empty, none, np.ones(5, I32), np.full(5, -1, I32), 0, 4)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("heads,d,page,pools", [(1, 64, 16, 1), (8, 128, 16, 4), (3, 7, 5, 2), (70, 2, 4, 2), (2, 64, 16, 300)])
+def test_copy(rt, dtype, heads, d, page, pools):
+    rng, n_pages = np.random.default_rng(page), 12
+    host = [rng.standard_normal((n_pages, heads, page, d)).astype(dtype) for _ in range(pools)]
+    copies = np.array([[0, 1, 3], [0, 2, page], [4, 3, 1], [-1, -1, 0], [5, n_pages, 2], [n_pages, 6, 2], [7, 8, 0], [9, 10, page + 5]], I32)
+    device = [up(h) for h in host]
+    ta.PagedCopy().eval(up(copies), device)
+    for got, h in zip(device, host):
+        assert got.to_numpy().tobytes() == ref.copy(h, copies).tobytes()
+    ta.PagedCopy().eval(up(copies[:0]), device)
+    ta.PagedCopy().eval(up(copies), [])
+
+
+# ---- arguments that the Python side looks at ---------------------------------------------------------------------------------
+
+
+def test_shapes_and_types_are_refused(rt):
+    q, k, t, n = up(np.zeros((2, 4, 1, 64), F16)), up(np.zeros((5, 2, 16, 64), F16)), ints(np.zeros((2, 3))), ints([1, 1])
+    op = ta.PagedSdpa()
+    for bad in ((up(np.zeros((2, 4, 64), F16)), k, k, t, n), (q, k, up(np.zeros((5, 2, 16, 32), F16)), t, n), (up(np.zeros((2, 4, 1, 32), F16)), k, k, t, n), (up(np.zeros((2, 4, 1, 64), F32)), k, k, t, n),
+                (q, k, k, ints(np.zeros((3, 3))), n), (q, k, k, t, ints([1])), (q, k, k, up(np.zeros((2, 3), F32)), n), (up(np.zeros((2, 3, 1, 64), F16)), k, k, t, n)):
+        with pytest.raises(ta.TractRocmError):
+            op.eval(*bad)
+    with pytest.raises(ta.TractRocmError):
+        op.eval(q, k, k, t, n, out=up(np.zeros((2, 4, 1, 64), F32)))
+    with pytest.raises(ta.TractRocmError):
+        ta.PagedPlan(16).eval(n, ints([1]), t, ints([0] * 5), ints([5]), 2)
+    with pytest.raises(ta.TractRocmError):
+        ta.PagedPlan(16).eval(n, n, t, ints([0] * 5), ints([5]), 2, out={"slots": ints([0, 0, 0])})
+    with pytest.raises(ta.TractRocmError):
+        ta.PagedAppend().eval(up(np.zeros((3, 2, 32), F16)), up(np.zeros((3, 2, 32), F16)), ints([0, 1, 2]), k, k)
+    with pytest.raises(ta.TractRocmError):
+        ta.PagedCopy().eval(ints([[0, 1, 2]]), [k, up(np.zeros((5, 2, 16, 64), F32))])
+    with pytest.raises(ta.TractRocmError):
+        ta.PagedReorder(16).eval(n, t, n, ints([0] * 5), ints([0] * 4), ints([5]))

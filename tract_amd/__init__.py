@@ -13,5 +13,6 @@ from .ops import (ApplyRope, BlockQuant, Cast, GgmlGemm, Q40Weights, RotateHalf,
                   InPlaceKvSdpa, InPlaceKvSdpaState, Sdpa, StreamedSdpaOp, WindowKvCache, WindowKvSdpa, WindowKvSdpaState, Q4_0_FORMAT, Q8_0_FORMAT, inplace_kv_sdpa_eval_ragged, inplace_kv_sdpa_eval_ragged_rope,
                   sdpa_decode_ragged)
 from .scored import QkNormRope, ScoredSdpa, SharedPrefixSdpa, inplace_kv_sdpa_eval_shared  # noqa: F401
+from .paged import BeamSelect, PagedAppend, PagedCopy, PagedKvCache, PagedPlan, PagedReorder, PagedSdpa  # noqa: F401
 from .kivi import (KiviCache, QuantizedDynKeyValueCache, QuantizedDynKvCacheState, QuantizedKvSdpa,  # noqa: F401
                    QuantizedKvSdpaState, KIVI_BLOCK_CHANNEL, KIVI_PER_TOKEN, KIVI_RUNNING_CHANNEL)

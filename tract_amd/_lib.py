@@ -114,6 +114,14 @@ SIGNATURES = {
                                           _sz, _vp],
     "trocm_sdpa_scored": [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _f, _f, _vp, _vp, _vp, _i, _vp, _sz, _vp],
     "trocm_sdpa_cached_scored": [_vp, _i, _i64, _i64, _vp, _vp, _vp, _f, _f, _vp, _vp, _vp, _i, _vp, _sz, _vp],
+    "trocm_paged_plan": [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "trocm_paged_append": [_vp, _vp, _i, _i64, _i64, _i64, _pi64, _pi64, _vp, _vp, _vp, _i64, _i64, _pi64, _vp],
+    "trocm_sdpa_paged_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, C.POINTER(_sz)],
+    "trocm_sdpa_paged": [_vp, _i, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _pi64, _vp, _i64, _vp, _vp, _f, _i, _vp, _sz, _vp],
+    "trocm_paged_reorder": [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "trocm_paged_copy": [_vp, _i64, C.POINTER(_vp), _i64, _i, _i64, _i64, _i64, _i64, _pi64, _vp],
+    "trocm_beam_select_workspace_bytes": [_i64, _i64, _i64, _i64, C.POINTER(_sz)],
+    "trocm_beam_select": [_vp, _i, _i64, _i64, _i64, _i64, _vp, _vp, C.c_int32, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
 }
 _RESTYPES = {"trocm_last_error": C.c_char_p}
 

@@ -29,7 +29,8 @@ COMMON = [
 EXTRA = {"kv_quant.hip": ["-ffp-contract=off"], "elementwise.hip": ["-ffp-contract=off"], "kivi.hip": ["-ffp-contract=off"]}
 SOURCES = ["abi.hip", "copy.hip", "kv_quant.hip", "sdpa_generic.hip", "sdpa_decode.hip", "sdpa_decode_quant.hip", "sdpa_decode_f32.hip",
            "sdpa_prefill.hip", "sdpa_prefill_pp.hip", "sdpa_prefill_f32.hip", "elementwise.hip", "dat_format.hip", "q4_matvec.hip", "q4_matvec_mfma.hip", "q4_matmul.hip", "q4_matmul_f32.hip", "q4_matmul_waves.hip", "q4_tiled.hip", "sdpa_decode_mfma.hip", "kivi.hip",
-           "qk_norm_rope.hip", "sdpa_rows.hip", "sdpa_scored.hip"]
+           "qk_norm_rope.hip", "sdpa_rows.hip", "sdpa_scored.hip",
+           "abi_paged.hip", "paged.hip", "sdpa_paged.hip", "beam_select.hip"]
 
 
 def _newer(target: str, deps: list[str]) -> bool:

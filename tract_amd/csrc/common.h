@@ -295,6 +295,71 @@ size_t sdpa_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Sq, int64_t D)
 // k_new, v_new dense [B, Hkv, Sq, D] behind the rows of `seqs` (whose lengths do not count them yet).
 int launch_append_rows(const SdpaRowsArgs &a, const void *k_new, const void *v_new, hipStream_t s);
 
+// Pages of keys and values (paged.hip).  Ids, lengths and counts are device memory unless a line says otherwise.
+constexpr int kPagedMaxSeqs = 4096;    // sequences of a call that builds tables (their prefix sums are in LDS)
+constexpr int kPagedMaxPools = 256;    // pools of a launch that copies pages (in its arguments)
+struct PagedPlanArgs {
+    const int32_t *lens, *n_new, *free_pages, *free_count;
+    int32_t *table, *refs, *lens_out, *starts, *slots, *positions, *free_count_out, *refused;   // refs, starts, positions: or NULL
+    int64_t n_seq, page_size, table_width, n_pages, n_tokens;
+};
+int launch_paged_plan(const PagedPlanArgs &a, hipStream_t s);
+struct PagedAppendArgs {   // strides in elements
+    const void *src[2];
+    void *dst[2];
+    int dtype;
+    int64_t n_tokens, kv_heads, D, n_pages, page_size;
+    int64_t src_strides[2][2], page_strides[3];
+    const int32_t *slots;
+};
+int launch_paged_append(const PagedAppendArgs &a, hipStream_t s);
+struct PagedReorderArgs {
+    const int32_t *parents, *table, *lens, *refs, *free_pages, *free_count;
+    int32_t *table_out, *lens_out, *refs_out, *free_pages_out, *free_count_out, *copies, *missing;
+    int64_t n_seq, page_size, table_width, n_pages;
+};
+int launch_paged_reorder(const PagedReorderArgs &a, hipStream_t s);
+struct PagedCopyArgs {
+    const int32_t *copies;
+    void *const *pools;    // host array
+    int dtype;
+    int64_t n_copies, n_pools, kv_heads, D, n_pages, page_size, page_strides[3];
+};
+int launch_paged_copy(const PagedCopyArgs &a, hipStream_t s);
+// Attention over pages (sdpa_paged.hip).  Strides in elements, head_dim contiguous.
+struct SdpaPagedArgs {
+    const void *q;         // [B, Hq, Sq, D] dense
+    void *out;
+    int dtype;
+    int64_t B, Hq, Hkv, Sq, D;
+    const void *k, *v;
+    int64_t n_pages, page_size, stride_page, stride_h, stride_t;
+    const int32_t *table, *lens;
+    int64_t table_width;
+    float scale;
+    int causal;
+    void *workspace;
+    size_t workspace_bytes;
+};
+int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s);
+size_t sdpa_paged_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D);
+// The best continuations of beams (beam_select.hip).
+constexpr int kBeamMaxKeep = 64, kBeamMaxBeams = 64;
+struct BeamSelectArgs {
+    const void *logits;
+    int dtype;
+    int64_t batch, beams, vocab, row_stride, keep;
+    const float *scores;
+    const int32_t *ended;   // or NULL
+    int32_t eos;
+    float *scores_out;
+    int32_t *parents, *tokens, *ended_out;
+    void *workspace;
+    size_t workspace_bytes;
+};
+int launch_beam_select(const BeamSelectArgs &a, hipStream_t s);
+size_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep);
+
 // Workspace layout: [arrival counters][partials ...]; a ragged launch keeps its plan (work items and
 // per-sequence slot ranges) between the two, so that the counters stay zero for whichever launch comes next:
 // [arrival counters][plan][partials ...].
