@@ -1,5 +1,13 @@
 // Attention over pages of keys and values: o = softmax(scale q k^T) v for one or a few new tokens of every sequence, whose keys lie in
 // pages anywhere, found through a table, and whose lengths are read from device memory.  f16 and f32.
+//
+// The query rows of a kv head (heads of the group, queries) are rows of matrix tiles, S^T = K Q^T and O^T = V^T P^T, so that every softmax
+// scalar of a row sits in one lane.  A tile is 32 keys: two halves of 16 that lie in a page each (pages are multiples of 16 tokens).
+//
+// The host does not know the lengths, so the work is shared out on the device: all units (sequence, kv head, 16 rows) one behind the other
+// are a line of tiles, and every workgroup takes a stretch of it, all of the same length.  A unit inside of a stretch goes straight to the
+// output; one that a stretch's end cuts goes to the workspace in parts (unnormalised O, maximum, sum, f32), which the last workgroup to
+// arrive joins, always in the same order.
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
@@ -9,7 +17,15 @@
 namespace trocm {
 namespace {
 
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kTile = 32, kRows = 16;
 
 struct PagedDev {
     const char *q, *k, *v;
@@ -20,6 +36,11 @@ struct PagedDev {
     float scale;
     int causal;
     FastDiv by_page;
+    // tiles of 16 rows
+    int row_tiles;              // of a kv head
+    int *counters;
+    float *parts;
+    FastDiv by_g, by_row_tiles;
 };
 
 __device__ __forceinline__ float widen(float x) { return x; }
@@ -93,9 +114,474 @@ __global__ __launch_bounds__(kAnyThreads) void sdpa_paged_any_kernel(PagedDev p)
     }
 }
 
+// ---- head sizes 64 and 128, pages of multiples of 16 tokens: matrix tiles ---------------------------------------------------
+
+// 16 bytes of device memory; ONCE: past the caches.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load16(const char *base, uint32_t off) {
+    const auto *at = (const __attribute__((address_space(1))) u32x4 *)(base + off);
+    return ONCE ? __builtin_nontemporal_load(at) : *at;
+}
+
+// Transposing 64-bit LDS load of 16-bit elements: in each block of 16 lanes, lane i receives
+// element i%4 of the four 8-byte rows addressed by lanes i/4, i/4+4, i/4+8, i/4+12.
+__device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *lds_ptr) {
+    typedef __attribute__((address_space(3))) short4_t *lds_v4_ptr;
+    short4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_ptr)(uintptr_t)(uint32_t)(uintptr_t)lds_ptr);
+    return __builtin_bit_cast(half4_t, r);
+}
+
+// Orders a wave's LDS accesses across its lanes (no instruction: the LDS serves a wave in order).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Partial results for whichever workgroup joins them: written through to where every compute unit sees them once they complete.
+__device__ __forceinline__ void put(float *at, float x) { __hip_atomic_store(at, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get(const float *at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put2(float *at, float2_t x) { __hip_atomic_store(reinterpret_cast<uint64_t *>(at), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float2_t get2(const float *at) { return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t *>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)); }
+
+// a - b of scores as they are rounded: a product fused into it would differ from `b`, which is one of them, by up to half its last place.
+__device__ __forceinline__ float less(float a, float b) {
+#pragma clang fp contract(off)
+    return a - b;
+}
+
+// Where row r of a kv head lies among the q and output rows, and which query it is.
+struct RowPlace { int64_t at; int i; };
+__device__ __forceinline__ RowPlace q_row(const PagedDev &p, int b, int kvh, int r) {
+    const int i = p.by_g.by(r);
+    return {((int64_t)b * p.Hq + kvh * p.G + r - i * p.G) * p.Sq + i, i};
+}
+
+constexpr int kLinePart(int D) { return kRows * D + 2 * kRows; }   // floats of a part: rows of O, their maxima, their sums
+
+// Tiles [first, end) of a unit; `part`: where its partial rows go (NULL: it is the whole unit, rows go to the output).
+struct Stretch {
+    int b, kvh, row0, rows, len, first, end;
+    float *part;
+};
+
+template <typename T, int D, bool ONCE>
+__device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u, unsigned char *lds) {
+    constexpr bool H16 = sizeof(T) == 2;
+    constexpr int DB = D / 16;                    // feature blocks of the output
+    constexpr int KROW = D + 8, VROW = H16 ? D + 16 : D + 4;   // elements per row in LDS: rows of a read in different banks
+    constexpr int PRIV = kTile * (VROW + (H16 ? KROW : 0)) * (int)sizeof(T);   // a wave's tile
+    constexpr int CROW = D + 4;                   // floats per row where waves are joined
+    constexpr int LPRW = D * (int)sizeof(T) / 16, RPI = 64 / LPRW, NI = kTile / RPI;   // lanes per key row, rows per load, loads per tile and tensor
+    constexpr int KS = D * (int)sizeof(T) / 64;   // 16-byte pieces of a lane's share of a row
+    constexpr int NK = H16 ? NI : 2 * KS;
+    static_assert(kWaves * kRows * CROW * 4 + kWaves * 2 * kRows * 4 <= kWaves * PRIV, "waves are joined where the tiles were");
+
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane / 16, lr = lane % 16;
+    const RowPlace place = q_row(p, u.b, u.kvh, u.row0 + min(lr, u.rows - 1));
+    const int lim = p.causal ? min(u.len - 1, u.len - p.Sq + place.i) : u.len - 1;
+    const int last_key = u.len - 1;
+    const char *kb = p.k + u.kvh * p.stride_h, *vb = p.v + u.kvh * p.stride_h;
+    const int *pages = p.table + u.b * p.table_width;
+    const uint32_t st = (uint32_t)p.stride_t;     // (below 2^27: checked by the host)
+    const int n_mine = (u.end - u.first - w + kWaves - 1) / kWaves;   // this wave takes every fourth tile
+
+    // Where the halves of 32 of this wave's tiles lie: lane 2 i + h has tile i's half h, as bytes from the pool's beginning (-1: a hole, or
+    // behind the last key).
+    auto ask_pages = [&](int i0) __attribute__((always_inline)) {
+        const int key = (u.first + w + kWaves * (i0 + (lane >> 1))) * kTile + 16 * (lane & 1);
+        return key <= last_key && i0 + (lane >> 1) < n_mine ? pages[p.by_page.by(key)] : -1;
+    };
+    auto bytes_at = [&](int id, int i0) __attribute__((always_inline)) {
+        const int key = (u.first + w + kWaves * (i0 + (lane >> 1))) * kTile + 16 * (lane & 1);
+        const int in_page = key - p.by_page.by(key) * (int)p.by_page.d;
+        return (unsigned)id < (unsigned)p.n_pages ? id * p.stride_page + (int64_t)in_page * p.stride_t : (int64_t)-1;
+    };
+    int64_t at = -1;
+    int ids_next = -1;
+
+    float m_run = -INFINITY, l_run = 0.0f;
+    float4_t o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++) o[db] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+    T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: f16)
+    const int kr = lane / LPRW, ch = lane % LPRW;
+    u32x4 kpre[NK], vpre[NI];
+    struct Halves { int64_t at[2]; } now, next;   // of the tile whose rows are in flight
+    auto halves_of = [&](int i) __attribute__((always_inline)) {
+        Halves r;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int from = 2 * (i & 31) + h;
+            r.at[h] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint64_t)at, from) | ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)((uint64_t)at >> 32), from) << 32));
+        }
+        return r;
+    };
+    // (halves that are not there read the other one's rows, or the pool's first: they weigh nothing; rows behind the last key repeat it)
+    auto row_base = [&](const Halves &x, int h) __attribute__((always_inline)) { return x.at[h] >= 0 ? x.at[h] : x.at[1 - h] >= 0 ? x.at[1 - h] : 0; };
+    auto rows_of = [&](int i, const Halves &x, int h) __attribute__((always_inline)) {   // the last row of a half that may be read
+        const int most = last_key - (u.first + w + kWaves * i) * kTile;
+        if (x.at[0] < 0 && x.at[1] < 0) return 0;
+        const int there = x.at[h] >= 0 ? h : 1 - h;
+        return min(most - 16 * there, 15);
+    };
+    auto prefetch_k = [&](int i, const Halves &x) __attribute__((always_inline)) {
+        if constexpr (H16) {
+#pragma unroll
+            for (int j = 0; j < NI; j++) {
+                const int h = j * RPI / 16;
+                kpre[j] = load16<ONCE>(kb + row_base(x, h), (uint32_t)min(j * RPI % 16 + kr, rows_of(i, x, h)) * st + ch * 16);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const char *base = kb + row_base(x, h);
+                const uint32_t off = (uint32_t)min(lr, rows_of(i, x, h)) * st + grp * 16;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) kpre[h * KS + ks] = load16<false>(base, off + ks * 64);   // (64 bytes of a row at a time: the caches join them)
+            }
+        }
+    };
+    auto prefetch_v = [&](int i, const Halves &x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NI; j++) {
+            const int h = j * RPI / 16;
+            vpre[j] = load16<ONCE>(vb + row_base(x, h), (uint32_t)min(j * RPI % 16 + kr, rows_of(i, x, h)) * st + ch * 16);
+        }
+    };
+    const float to_log2 = p.scale * kLog2e;
+    // key of score x of this lane, from the tile's first: two groups of four consecutive ones
+    auto key_of = [](int x) { return 16 * (x >> 2) + (x & 3); };   // + 4 grp
+
+    if (n_mine > 0) {
+        const int ids = ask_pages(0);
+        ids_next = ask_pages(32);
+        at = bytes_at(ids, 0);
+        now = halves_of(0);
+        prefetch_k(0, now), prefetch_v(0, now);
+    }
+    u32x4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = load16<false>(p.q + place.at * (D * (int)sizeof(T)), ks * 64 + grp * 16);
+    for (int i = 0; i < n_mine; i++) {
+        const int k_lo = (u.first + w + kWaves * i) * kTile;
+        const bool more = i + 1 < n_mine;
+        if (more) {
+            if (((i + 1) & 31) == 0) at = bytes_at(ids_next, i + 1), ids_next = ask_pages(i + 33);
+            next = halves_of(i + 1);
+        }
+        const bool odd = now.at[0] < 0 || now.at[1] < 0 || k_lo + kTile > u.len;   // a hole, or the last key inside
+
+        // ---- S^T = K Q^T --------------------------------------------------------------------------------------
+        float4_t acc[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) acc[h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (H16) {
+#pragma unroll
+            for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_k + (j * RPI + kr) * KROW + ch * 8) = kpre[j];
+            if (more) prefetch_k(i + 1, next);
+            wave_sync();
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4 *>(lds_k + (16 * h + lr) * KROW + ks * 32 + grp * 8);
+                    acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kf), __builtin_bit_cast(half8_t, qf[ks]), acc[h], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {   // (one feature of each group's four at a time)
+                    const float4_t a = __builtin_bit_cast(float4_t, kpre[h * KS + ks]), c = __builtin_bit_cast(float4_t, qf[ks]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[h], 0, 0, 0);
+                }
+            if (more) prefetch_k(i + 1, next);
+        }
+        float s[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) s[x] = acc[x >> 2][x & 3] * to_log2;
+        if (odd) {   // rows that are not the sequence's may hold anything
+#pragma unroll
+            for (int j = 0; j < NI; j++) {
+                const int r = j * RPI + kr;
+                if (now.at[j * RPI / 16] < 0 || k_lo + r > last_key) vpre[j] = u32x4{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_v + (j * RPI + kr) * VROW + ch * (16 / (int)sizeof(T))) = vpre[j];
+        if (more) prefetch_v(i + 1, next);
+
+        // ---- softmax of this lane's row over its keys k_lo + 4 grp + key_of(x) -----------------------------------
+        const int last = lim - k_lo - 4 * grp;
+        if (odd || __builtin_amdgcn_ballot_w64(last < 28) != 0) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) s[x] = key_of(x) <= last && now.at[x >> 2] >= 0 ? s[x] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int x = 1; x < 8; x++) top = fmaxf(top, s[x]);
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
+        const bool moved = less(top, m_run) > (H16 ? 8.0f : 0.0f);
+        const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
+        m_run = m_new;
+        half8_t pf;
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            float e = __builtin_amdgcn_exp2f(less(s[x], ref));
+            // The product with V takes f16 operands: weights are rounded, half a step each, and the row's sum takes the same ones, so that a row
+            // of equal values stays that value.
+            if constexpr (H16) {
+                pf[x] = (_Float16)e;
+                e = (float)pf[x];
+            }
+            s[x] = e;
+            sum += e;
+        }
+        l_run = l_run * keep + sum;
+        if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+            for (int db = 0; db < DB; db++) o[db] *= keep;
+        }
+
+        // ---- O^T += V^T P^T --------------------------------------------------------------------------------
+        wave_sync();
+        if constexpr (H16) {
+            // this lane as a source of the transposing loads: key (lane%16)/4 of a group of four, features 4 (lane%4) of a block of 16
+            const _Float16 *vsrc = reinterpret_cast<const _Float16 *>(lds_v) + (4 * grp + ((lane & 15) >> 2)) * VROW + 4 * (lane & 3);
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const half4_t lo = lds_read_tr16(vsrc + 16 * db), hi = lds_read_tr16(vsrc + 16 * VROW + 16 * db);
+                o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf, o[db], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+#pragma unroll
+                for (int db = 0; db < DB; db++) o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(lds_v[(key_of(x) + 4 * grp) * VROW + 16 * db + lr], s[x], o[db], 0, 0, 0);
+        }
+        wave_sync();   // (the next tile goes where this one was)
+        now = next;
+    }
+
+    // ---- the four waves' results joined ------------------------------------------------------------------------
+    float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + kWaves * kRows * CROW;
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) l_run += __shfl_xor(l_run, d, 64);
+    __syncthreads();   // the tiles are done with
+#pragma unroll
+    for (int db = 0; db < DB; db++) *reinterpret_cast<float4_t *>(comb + (w * kRows + lr) * CROW + 16 * db + 4 * grp) = o[db];
+    if (grp < 2) comb_ml[(w * 2 + grp) * kRows + lr] = grp ? l_run : m_run;
+    __syncthreads();
+    constexpr int TPR = kThreads / kRows, PER = D / TPR;   // threads per row, features per thread
+    const int row = tid / TPR;
+    if (row < u.rows) {
+        float mm = -INFINITY, l = 0.0f, f[kWaves];
+#pragma unroll
+        for (int x = 0; x < kWaves; x++) mm = fmaxf(mm, comb_ml[x * 2 * kRows + row]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+        for (int x = 0; x < kWaves; x++) {
+            f[x] = __builtin_amdgcn_exp2f(comb_ml[x * 2 * kRows + row] - ref);
+            l += f[x] * comb_ml[(x * 2 + 1) * kRows + row];
+        }
+        const int64_t orow = q_row(p, u.b, u.kvh, u.row0 + row).at;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+            const int d = (tid % TPR) * 2 + e * TPR;   // (8 bytes per thread, threads of a row side by side: a store covers whole lines)
+            float2_t sum = {0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < kWaves; x++) {
+                const float2_t v = *reinterpret_cast<const float2_t *>(comb + (x * kRows + row) * CROW + d);
+#pragma unroll
+                for (int y = 0; y < 2; y++) sum[y] = __builtin_fmaf(f[x], v[y], sum[y]);
+            }
+            if (!u.part) {
+                struct alignas(2 * sizeof(T)) Two { T e[2]; } two;
+                two.e[0] = (T)(sum[0] * inv), two.e[1] = (T)(sum[1] * inv);
+                *reinterpret_cast<Two *>(reinterpret_cast<T *>(p.out) + orow * D + d) = two;
+            } else {
+                put2(u.part + row * D + d, sum);
+            }
+        }
+        if (u.part && tid % TPR == 0) put(u.part + kRows * D + row, mm), put(u.part + kRows * D + kRows + row, l);
+    }
+    __syncthreads();   // (the next stretch's tiles go where these rows were)
+}
+
+// The parts of a unit -> its output.  Part x of [0, n) is at part_of(x).  Sixteen lanes take a row; where there are few rows, several groups
+// of lanes share a row's parts and are joined through LDS.
+template <typename T, int D, typename PartOf>
+__device__ __forceinline__ void join_unit(const PagedDev &p, const Stretch &u, int n, PartOf part_of, unsigned char *lds) {
+    constexpr int PER = D / 16, BATCH = 4, CROW = D + 4;
+    const int tid = threadIdx.x, t = tid % 16, who = tid / 16;
+    int live = 1;
+    while (live < u.rows) live *= 2;
+    const int row = who & (live - 1), group = who / live, groups = 16 / live, at_row = min(row, u.rows - 1);
+    float m_run = -INFINITY, l_run = 0.0f;
+    float2_t acc[PER / 2];
+#pragma unroll
+    for (int e = 0; e < PER / 2; e++) acc[e] = float2_t{0.0f, 0.0f};
+    for (int x0 = group; x0 < n; x0 += groups * BATCH) {
+        float m[BATCH], l[BATCH];
+        float2_t v[BATCH][PER / 2];
+#pragma unroll
+        for (int y = 0; y < BATCH; y++) {
+            const float *part = part_of(min(x0 + y * groups, n - 1));
+            m[y] = get(part + kRows * D + at_row), l[y] = get(part + kRows * D + kRows + at_row);
+#pragma unroll
+            for (int e = 0; e < PER / 2; e++) v[y][e] = get2(part + at_row * D + 2 * t + 32 * e);
+        }
+#pragma unroll
+        for (int y = 0; y < BATCH; y++) {
+            // (without keys: a maximum of -inf and a sum of 0; scores that are all NaN raise no maximum either, but their sum is NaN)
+            const bool has = x0 + y * groups < n && (m[y] != -INFINITY || l[y] != 0.0f);
+            const float mm = has ? fmaxf(m_run, m[y]) : m_run, ref = mm == -INFINITY ? 0.0f : mm;
+            const float keep = __builtin_amdgcn_exp2f(m_run - ref), f = has ? __builtin_amdgcn_exp2f(m[y] - ref) : 0.0f;
+            const float was = m_run == -INFINITY && l_run == 0.0f ? 0.0f : keep;
+            l_run = l_run * was + (has ? f * l[y] : 0.0f);
+#pragma unroll
+            for (int e = 0; e < PER / 2; e++)
+#pragma unroll
+                for (int z = 0; z < 2; z++) acc[e][z] = acc[e][z] * was + (has ? f * v[y][e][z] : 0.0f);
+            m_run = mm;
+        }
+    }
+    float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + 16 * CROW;
+#pragma unroll
+    for (int e = 0; e < PER / 2; e++) *reinterpret_cast<float2_t *>(comb + who * CROW + 2 * t + 32 * e) = acc[e];
+    if (t == 0) comb_ml[2 * who] = m_run, comb_ml[2 * who + 1] = l_run;
+    __syncthreads();
+    if (who < u.rows) {   // (who == row of group 0)
+        float mm = -INFINITY, l = 0.0f;
+        for (int g = 0; g < groups; g++) mm = fmaxf(mm, comb_ml[2 * (g * live + who)]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float2_t sum[PER / 2];
+#pragma unroll
+        for (int e = 0; e < PER / 2; e++) sum[e] = float2_t{0.0f, 0.0f};
+        for (int g = 0; g < groups; g++) {
+            const int from = g * live + who;
+            const float m = comb_ml[2 * from], lg = comb_ml[2 * from + 1];
+            const bool has = m != -INFINITY || lg != 0.0f;
+            const float f = has ? __builtin_amdgcn_exp2f(m - ref) : 0.0f;
+            l += has ? f * lg : 0.0f;
+#pragma unroll
+            for (int e = 0; e < PER / 2; e++) {
+                const float2_t v = *reinterpret_cast<const float2_t *>(comb + from * CROW + 2 * t + 32 * e);
+#pragma unroll
+                for (int z = 0; z < 2; z++) sum[e][z] = has ? __builtin_fmaf(f, v[z], sum[e][z]) : sum[e][z];
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T *out = reinterpret_cast<T *>(p.out) + q_row(p, u.b, u.kvh, u.row0 + who).at * D;
+#pragma unroll
+        for (int e = 0; e < PER / 2; e++) {
+            struct alignas(2 * sizeof(T)) Two { T e[2]; } two;
+            two.e[0] = (T)(sum[e][0] * inv), two.e[1] = (T)(sum[e][1] * inv);
+            *reinterpret_cast<Two *>(out + 2 * t + 32 * e) = two;
+        }
+    }
+    __syncthreads();
+}
+
+constexpr int line_lds(int es, int D) { return kWaves * kTile * (es == 2 ? 2 * D + 24 : D + 4) * es; }
+constexpr int kLeast = 8;   // tiles of a stretch at least: two a wave
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev p) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
+    __shared__ int64_t s_sums[kWaves], s_start;
+    __shared__ int s_b, s_last;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    const int units = p.Hkv * p.row_tiles;   // of a sequence
+    auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
+    auto tiles_of = [&](int b) { return b < p.B ? max((len_of(b) + kTile - 1) / kTile, 1) : 0; };   // (one for nothing: its rows are zeros)
+
+    // the line's length, and this workgroup's stretch
+    int64_t sum = 0;
+    for (int b = tid; b < p.B; b += kThreads) sum += tiles_of(b);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((long long)sum, d, 64);
+    if (lane == 0) s_sums[w] = sum;
+    __syncthreads();
+    const int64_t total = (s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3]) * units;
+    const int64_t per = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, kLeast);
+    const int64_t begin = blockIdx.x * per, end = std::min<int64_t>(begin + per, total);
+    if (begin >= end) return;
+    // the sequence where it begins
+    int64_t carry = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+        const int b = b0 + tid, mine = tiles_of(b);
+        int64_t up = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t y = __shfl_up((long long)up, d, 64);
+            if (lane >= d) up += y;
+        }
+        __syncthreads();
+        if (lane == 63) s_sums[w] = up;
+        __syncthreads();
+        int64_t before = carry;
+        for (int x = 0; x < w; x++) before += s_sums[x];
+        const int64_t from = (before + up - mine) * units;
+        if (b < p.B && from <= begin && begin < from + (int64_t)mine * units) s_b = b, s_start = from;
+        carry += s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3];
+        if (carry * units > begin) break;
+    }
+    __syncthreads();
+
+    Stretch u;
+    u.b = s_b, u.len = len_of(u.b);
+    int tiles = tiles_of(u.b);
+    int unit = (int)((begin - s_start) / tiles);
+    u.first = (int)(begin - s_start - (int64_t)unit * tiles);
+    for (int64_t t = begin; t < end;) {
+        u.kvh = p.by_row_tiles.by(unit);
+        u.row0 = (unit - u.kvh * p.row_tiles) * kRows, u.rows = min(kRows, p.Sq * p.G - u.row0);
+        u.end = (int)std::min<int64_t>(tiles, u.first + (end - t));
+        const bool whole = u.first == 0 && u.end == tiles;
+        u.part = whole ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * kLinePart(D);
+        stretch_body<T, D, false>(p, u, lds);
+        if (!whole) {
+            const int64_t unit_at = t - u.first;
+            const int first = (int)(unit_at / per), n = (int)((unit_at + tiles - 1) / per) - first + 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
+            __syncthreads();                                     // ... and so have the whole workgroup's
+            if (tid == 0) {
+                int *counter = p.counters + first;   // (a workgroup cuts one unit at most at its end)
+                s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+                if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (s_last) join_unit<T, D>(p, u, n, [&](int x) { return p.parts + (2 * (int64_t)(first + x) + (x == 0)) * kLinePart(D); }, lds);
+        }
+        t += u.end - u.first;
+        u.first = 0;
+        if (++unit == units && t < end) unit = 0, u.b++, u.len = len_of(u.b), tiles = tiles_of(u.b);
+    }
+}
+
+template <typename T, int D>
+int launch_line(const PagedDev &p, int workgroups, hipStream_t s) {
+    sdpa_paged_kernel<T, D><<<dim3((unsigned)workgroups), kThreads, 0, s>>>(p);
+    TROCM_HIP(hipGetLastError());
+    return 0;
+}
+
+int line_workgroups() { return 2 * num_compute_units(); }
+
 }  // namespace
 
-size_t sdpa_paged_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return kWsCounterBytes; }
+size_t sdpa_paged_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t D) {
+    return kWsCounterBytes + (D == 64 || D == 128 ? (size_t)2 * line_workgroups() * kLinePart((int)D) * 4 : 0);
+}
 
 int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
     if (a.B == 0 || a.Hq == 0 || a.Sq == 0 || a.D == 0) return 0;
@@ -107,6 +593,15 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
     p.B = (int)a.B, p.Hq = (int)a.Hq, p.Hkv = (int)a.Hkv, p.Sq = (int)a.Sq, p.G = (int)(a.Hq / a.Hkv), p.D = (int)a.D;
     p.n_pages = (int)a.n_pages, p.most = (int)std::min<int64_t>(a.table_width * a.page_size, 1 << 30);
     p.scale = a.scale, p.causal = a.causal, p.by_page = fast_div(a.page_size);
+    const uint64_t bits = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.out | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)p.stride_page | (uint64_t)p.stride_h | (uint64_t)p.stride_t;
+    if ((a.D == 64 || a.D == 128) && a.page_size % 16 == 0 && bits % 16 == 0 && a.n_pages > 0 && p.stride_t < (1 << 27) && a.workspace &&
+        a.workspace_bytes >= sdpa_paged_workspace_bytes(a.B, a.Hq, a.Hkv, a.Sq, a.D)) {
+        p.row_tiles = (int)((a.Hq / a.Hkv * a.Sq + kRows - 1) / kRows);
+        p.by_g = fast_div(p.G), p.by_row_tiles = fast_div(p.row_tiles);
+        p.counters = (int *)a.workspace, p.parts = (float *)((char *)a.workspace + kWsCounterBytes);
+        if (a.dtype == TROCM_F16) return a.D == 64 ? launch_line<_Float16, 64>(p, line_workgroups(), s) : launch_line<_Float16, 128>(p, line_workgroups(), s);
+        return a.D == 64 ? launch_line<float, 64>(p, line_workgroups(), s) : launch_line<float, 128>(p, line_workgroups(), s);
+    }
     TROCM_REQUIRE(a.D <= kRowsMaxD, "sdpa_paged: head_dim %lld is more than %d", (long long)a.D, kRowsMaxD);
     const dim3 grid((unsigned)(a.Hq * a.Sq), (unsigned)std::min<int64_t>(a.B, 32768));
     if (a.dtype == TROCM_F16) sdpa_paged_any_kernel<_Float16><<<grid, kAnyThreads, 0, s>>>(p);
