@@ -21,7 +21,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kPiece = 8;                     // consecutive values of a lane
-constexpr int kWaveList = 256;                // values above the bound that a wave lists; ties up to `keep` come on top
+constexpr int kWaveList = 128;                // values above the bound that a wave lists (at least kBeamMaxKeep); ties up to `keep` come on top
 constexpr uint32_t kLowest = 0x007fffffu;     // key_of(-inf); 0 is below all values: nothing there
 
 struct Candidate { float x; int token; };     // token < 0: none
@@ -59,90 +59,136 @@ __device__ __forceinline__ uint32_t bound_of_lanes(uint32_t key, int count) {
     return t;
 }
 
-template <typename T> struct alignas(sizeof(T)) Piece { T x[kPiece]; };   // (rows begin where they begin: whole pieces are loaded from any element)
+template <typename T> using Eight = T __attribute__((ext_vector_type(kPiece)));
 
-// A part of a row: kThreads * kPiece * C values.
+// A part of a row: kThreads * kPiece * C values, all of them asked for before the first is looked at.
 template <typename T, int C>
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
-    constexpr int E = C * kPiece, kPart = kThreads * E;
-    __shared__ Candidate s_list[kWaves * (kWaveList + kBeamMaxKeep)];
+    constexpr int kPart = kThreads * kPiece * C, kList = kWaveList + kBeamMaxKeep;
+    __shared__ Candidate s_list[kWaves * kList];
     __shared__ int s_count[kWaves];
+    __shared__ uint32_t s_bound[kWaves];
     __shared__ float s_max[kWaves];
     __shared__ double s_sum[kWaves];
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int row = p.by_parts.by(blockIdx.x), part = blockIdx.x - row * p.parts;
-    const T *x = reinterpret_cast<const T *>(p.logits + row * p.row_bytes);
+    const T *from = reinterpret_cast<const T *>(p.logits + row * p.row_bytes);
     const int i0 = part * kPart + tid * kPiece;
-    uint32_t key[E];
+    // (rows begin where they begin: pieces are loaded from any element on; what is behind the row's end is -inf)
+    Eight<T> x[C];
+    if (part * kPart + kPart <= p.vocab) {
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-        const int i = i0 + c * kThreads * kPiece;
-        if (i + kPiece <= p.vocab) {
-            Piece<T> piece;
-            __builtin_memcpy(&piece, x + i, sizeof(piece));
+        for (int c = 0; c < C; c++) __builtin_memcpy(&x[c], from + i0 + c * kThreads * kPiece, sizeof(x[c]));
+    } else {
 #pragma unroll
-            for (int e = 0; e < kPiece; e++) key[c * kPiece + e] = key_of((float)piece.x[e]);
-        } else {
+        for (int c = 0; c < C; c++) {
+            const int i = i0 + c * kThreads * kPiece;
+            if (i <= p.vocab - kPiece) {
+                __builtin_memcpy(&x[c], from + i, sizeof(x[c]));
+            } else {
 #pragma unroll
-            for (int e = 0; e < kPiece; e++) key[c * kPiece + e] = i + e < p.vocab ? key_of((float)x[i + e]) : 0;
+                for (int e = 0; e < kPiece; e++) x[c][e] = i + e < p.vocab ? from[i + e] : (T)-INFINITY;
+            }
         }
     }
-    uint32_t top = 0;
+    Eight<T> top8 = (T)-INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; e++) top = max(top, key[e]);
+    for (int c = 0; c < C; c++) {
+        x[c] = __builtin_elementwise_max(x[c], (Eight<T>)(T)-INFINITY);   // (the number of the two: NaN counts as -inf)
+        top8 = __builtin_elementwise_max(top8, x[c]);
+    }
+    float top = (float)top8[0];
+#pragma unroll
+    for (int e = 1; e < kPiece; e++) top = fmaxf(top, (float)top8[e]);
 
-    // maximum and sum; a wave without values has the sum 0 at -inf
-    uint32_t wave_top = top;
+    // at least `keep` values of a wave reach its bound, so the largest bound will do for the workgroup
+    const uint32_t wave_bound = bound_of_lanes(key_of(top), p.keep);
+    float m = top;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) wave_top = max(wave_top, (uint32_t)__shfl_xor((int)wave_top, d, 64));
-    const float m = value_of(max(wave_top, kLowest)), ref = m == -INFINITY ? 0.0f : m;
-    // (f32 for the values of a piece, f64 from there on: beam_join_kernel's s_err says what that may be off by)
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (lane == 0) s_bound[w] = max(wave_bound, kLowest);
+    // maximum and sum: f32 for the values of a piece, f64 from there on (beam_join_kernel's s_err says what that may be off by)
+    const float ref = m == -INFINITY ? 0.0f : m;
     double all = 0.0;
 #pragma unroll
     for (int c = 0; c < C; c++) {
+        asm("" : "+v"(x[c]));
         float sum = 0.0f;
 #pragma unroll
-        for (int e = c * kPiece; e < (c + 1) * kPiece; e++) sum += key[e] ? __builtin_amdgcn_exp2f((value_of(key[e]) - ref) * kLog2e) : 0.0f;
+        for (int e = 0; e < kPiece; e++) sum += __builtin_amdgcn_exp2f(((float)x[c][e] - ref) * kLog2e);
         all += (double)sum;
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
     if (lane == 0) s_max[w] = m, s_sum[w] = all;
+    __syncthreads();
 
-    // the wave's largest values
-    Candidate *list = s_list + w * (kWaveList + kBeamMaxKeep);
-    uint32_t bound = bound_of_lanes(top, p.keep);
-    int above = 0;
+    // the values above the bound
+    uint32_t bound_key = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
+    float bound = value_of(bound_key);
+    Candidate *list = s_list + w * kList;
+    // (Each look at the values begins with what was loaded: kept in 32 bits from one look to the next, halves would take twice the registers.)
+    auto again = [&](int c) __attribute__((always_inline)) { asm("" : "+v"(x[c])); };
+    auto pieces = [&](auto &&with) __attribute__((always_inline)) {   // pieces with values above the bound
 #pragma unroll
-    for (int e = 0; e < E; e++) above += __popcll(__builtin_amdgcn_ballot_w64(key[e] > bound));
-    if (above > kWaveList) {
-        bound = 0;
+        for (int c = 0; c < C; c++) {
+            again(c);
+            T t = x[c][0];
+#pragma unroll
+            for (int e = 1; e < kPiece; e++) t = __builtin_elementwise_max(t, x[c][e]);
+            if (__builtin_amdgcn_ballot_w64((float)t > bound)) with(c);
+        }
+    };
+    int n = 0;
+    if (__builtin_amdgcn_ballot_w64(top > bound))
+        pieces([&](int c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < kPiece; e++) {
+                const float v = (float)x[c][e];
+                const uint64_t in = __builtin_amdgcn_ballot_w64(v > bound);
+                if (in) {
+                    const int at = n + lanes_below(in);
+                    if (v > bound && at < kWaveList) list[at] = Candidate{v, i0 + c * kThreads * kPiece + e};
+                    n += __popcll(in);
+                }
+            }
+        });
+    if (n > kWaveList) {   // too many in few lanes: the bound of all values, above which there are fewer than `keep`
+        bound_key = 0;
 #pragma unroll 1
         for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-            int n = 0;
+            int reach = 0;
 #pragma unroll
-            for (int e = 0; e < E; e++) n += __popcll(__builtin_amdgcn_ballot_w64(key[e] >= (bound | bit)));
-            if (n >= p.keep) bound |= bit;
-        }
-    }
-    int n = 0;
+            for (int c = 0; c < C; c++) {
+                again(c);
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const uint64_t in = __builtin_amdgcn_ballot_w64(key[e] > bound);
-        if (in) {
-            if (key[e] > bound) list[n + lanes_below(in)] = Candidate{value_of(key[e]), i0 + (e / kPiece) * kThreads * kPiece + e % kPiece};
-            n += __popcll(in);
+                for (int e = 0; e < kPiece; e++) reach += __popcll(__builtin_amdgcn_ballot_w64(key_of((float)x[c][e]) >= (bound_key | bit)));
+            }
+            if (reach >= p.keep) bound_key |= bit;
         }
+        bound = value_of(bound_key), n = 0;
+        pieces([&](int c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < kPiece; e++) {
+                const float v = (float)x[c][e];
+                const uint64_t in = __builtin_amdgcn_ballot_w64(v > bound);
+                if (v > bound) list[n + lanes_below(in)] = Candidate{v, i0 + c * kThreads * kPiece + e};
+                n += __popcll(in);
+            }
+        });
     }
-    // and those that equal the bound, in their order: pieces, lanes, values of a piece
-    if (bound) {
-        const int most = max(n, p.keep);
+    // and those that equal the bound, as many as could be among the best, in their order: pieces, lanes, values of a piece
+    const int most = max(n, p.keep);
+    if (n < most && __builtin_amdgcn_ballot_w64(top >= bound)) {
 #pragma unroll
         for (int c = 0; c < C; c++) {
             uint32_t ties = 0;
+            again(c);
 #pragma unroll
-            for (int e = 0; e < kPiece; e++) ties |= (key[c * kPiece + e] == bound ? 1u : 0u) << e;
+            for (int e = 0; e < kPiece; e++) ties |= ((float)x[c][e] == bound ? 1u : 0u) << e;
             if (n < most && __builtin_amdgcn_ballot_w64(ties != 0)) {
+                const int i = i0 + c * kThreads * kPiece;
+                ties &= i < p.vocab - kPiece ? 0xffu : i < p.vocab ? (1u << (p.vocab - i)) - 1 : 0u;   // (-inf behind the row's end is nothing)
                 const int mine = __popc(ties);
                 int at = n, here = 0;
 #pragma unroll
@@ -150,8 +196,7 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
                     const uint64_t lanes = __builtin_amdgcn_ballot_w64((mine >> bit) & 1);
                     at += lanes_below(lanes) << bit, here += __popcll(lanes) << bit;
                 }
-                for (uint32_t left = ties; left && at < most; left &= left - 1, at++)
-                    list[at] = Candidate{value_of(bound), i0 + c * kThreads * kPiece + __ffs(left) - 1};
+                for (uint32_t left = ties; left && at < most; left &= left - 1, at++) list[at] = Candidate{bound, i + __ffs(left) - 1};
                 n = min(n + here, most);
             }
         }
@@ -165,13 +210,14 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
     for (int y = 0; y < kWaves; y++) counts[y] = s_count[y], total += counts[y];
     Candidate *best = p.part_best + (int64_t)blockIdx.x * p.keep;
     for (int j = tid; j < total; j += kThreads) {
-        int from = j, y = 0;
-        while (from >= counts[y]) from -= counts[y++];
-        const Candidate c = s_list[y * (kWaveList + kBeamMaxKeep) + from];
+        int at = j, y = 0;
+        while (at >= counts[y]) at -= counts[y++];
+        const Candidate c = s_list[y * kList + at];
         int rank = 0;
         for (int o = 0; o < kWaves; o++)
+#pragma unroll 4
             for (int z = 0; z < counts[o]; z++) {
-                const Candidate d = s_list[o * (kWaveList + kBeamMaxKeep) + z];
+                const Candidate d = s_list[o * kList + z];
                 rank += d.x > c.x || (d.x == c.x && d.token < c.token);
             }
         if (rank < p.keep) best[rank] = c;
@@ -200,25 +246,10 @@ template <typename T>
 __device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint64_t *lds_sums) {
     const int shift = 61 - (32 - __clz(vocab)), tid = threadIdx.x;
     uint64_t sum = 0;
-    auto add = [&](float v) { sum += v == v ? (uint64_t)(ldexp(exp((double)v - (double)m), shift) + 0.5) : 0; };
-    constexpr int kDeep = 4, kStep = kDeep * kThreads * kPiece;
-    for (int i0 = 0; i0 < vocab; i0 += min(kStep, vocab - i0)) {
-        Piece<T> piece[kDeep];
-#pragma unroll
-        for (int y = 0; y < kDeep; y++) {
-            const int i = i0 + (y * kThreads + tid) * kPiece;
-            if (i <= vocab - kPiece) __builtin_memcpy(&piece[y], x + i, sizeof(piece[y]));
-        }
-#pragma unroll
-        for (int y = 0; y < kDeep; y++) {
-            const int i = i0 + (y * kThreads + tid) * kPiece;
-            if (i <= vocab - kPiece) {
-#pragma unroll 1
-                for (int e = 0; e < kPiece; e++) add((float)piece[y].x[e]);
-            } else {
-                for (int e = i; e < vocab; e++) add((float)x[e]);
-            }
-        }
+#pragma unroll 8
+    for (int i = tid; i < vocab; i += kThreads) {
+        const float v = (float)x[i];
+        sum += v == v ? (uint64_t)(ldexp(exp((double)v - (double)m), shift) + 0.5) : 0;
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += (uint64_t)__shfl_xor((unsigned long long)sum, d, 64);
@@ -236,24 +267,26 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
     __shared__ float s_max[kBeamMaxBeams];
     __shared__ int s_kind[kBeamMaxBeams], s_ended[kBeamMaxBeams];   // kind 0: goes on, 1: stays at the token of the ended, 2: has no candidates but of -inf
     __shared__ int s_again[kBeamMaxBeams], s_any;
-    __shared__ double s_c[kJoinList], s_best_c[kWaves];
-    __shared__ int s_place[kJoinList], s_count, s_best_place[kWaves], s_best_beam[kWaves];
+    __shared__ Choice s_list[kJoinList];
+    __shared__ double s_best_c[kWaves];
+    __shared__ int s_count, s_best_place[kWaves], s_best_beam[kWaves];
     __shared__ uint64_t s_sums[kWaves];
-    __shared__ uint8_t s_beam[kJoinList];
+    __shared__ uint32_t s_bound[kWaves];
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, request = blockIdx.x;
-    for (int beam = w; beam < p.beams; beam += kWaves) {
+    constexpr int kLanes = 16;   // of a beam
+    for (int beam = tid / kLanes; beam < p.beams; beam += kThreads / kLanes) {
         const int64_t row = (int64_t)request * p.beams + beam;
         const float *pm = p.part_max + row * p.parts;
         const double *ps = p.part_sum + row * p.parts;
         float m = -INFINITY;
-        for (int i = lane; i < p.parts; i += 64) m = fmaxf(m, pm[i]);
+        for (int i = tid % kLanes; i < p.parts; i += kLanes) m = fmaxf(m, pm[i]);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        for (int d = 1; d < kLanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
         double l = 0.0;
-        for (int i = lane; i < p.parts; i += 64) l += pm[i] == -INFINITY ? 0.0 : ps[i] * exp((double)pm[i] - (double)m);
+        for (int i = tid % kLanes; i < p.parts; i += kLanes) l += pm[i] == -INFINITY ? 0.0 : ps[i] * exp((double)pm[i] - (double)m);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-        if (lane == 0) {
+        for (int d = 1; d < kLanes; d <<= 1) l += __shfl_xor(l, d, 64);
+        if (tid % kLanes == 0) {
             const float score = p.scores[row];
             const bool dead = !(fabsf(score) < INFINITY);
             s_score[beam] = dead ? -INFINITY : (double)score;
@@ -304,10 +337,13 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
             const Choice r = candidate(j);
             if (r.place >= 0) top = max(top, key_of((float)r.c));
         }
-        const float bound = value_of(max(bound_of_lanes(top, p.keep), kLowest));
-        const double from = (double)bound - 0x1p-23 * fabs((double)bound) - 0x1p-149 - 2.0 * err;   // (-inf stays that)
+        const uint32_t wave_bound = bound_of_lanes(top, p.keep);
+        __syncthreads();   // (what the last turn has listed is done with)
+        if (lane == 0) s_bound[w] = wave_bound;
         if (tid == 0) s_count = 0;
         __syncthreads();
+        const float bound = value_of(max(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])), kLowest));
+        const double from = (double)bound - 0x1p-23 * fabs((double)bound) - 0x1p-149 - 2.0 * err;   // (-inf stays that)
         for (int j0 = 0; j0 < n; j0 += kThreads) {
             const int j = j0 + tid;
             Choice r = {-INFINITY, -1, 0};
@@ -318,31 +354,42 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
                 int at = 0;
                 if (lane == 0) at = atomicAdd(&s_count, __popcll(lanes));
                 at = __builtin_amdgcn_readfirstlane(at) + lanes_below(lanes);
-                if (in && at < kJoinList) s_c[at] = r.c, s_place[at] = r.place, s_beam[at] = (uint8_t)r.beam;
+                if (in && at < kJoinList) s_list[at] = r;
             }
         }
         __syncthreads();
         const int listed = min(s_count, kJoinList);
         const bool whole = s_count <= kJoinList;
-        if (again == 0) {   // beams whose values are too near for sums of 32-bit terms
-            if (!whole) {
-                for (int beam = tid; beam < p.beams; beam += kThreads) s_again[beam] = s_kind[beam] == 0;
-                if (tid == 0) s_any = 1;
+        // Every listed value counts those before it; a value that is nearer to another beam's than sums of 32-bit terms tell apart asks for
+        // both beams' sums to be made again.
+        constexpr int kMine = kJoinList / kThreads;
+        int rank[kMine];
+#pragma unroll
+        for (int y = 0; y < kMine; y++) {
+            const int j = tid + y * kThreads;
+            rank[y] = p.keep;
+            if (!whole || j >= listed) continue;
+            const Choice c = s_list[j];
+            int r = 0, near = 0;
+#pragma unroll 4
+            for (int o = 0; o < listed; o++) {
+                const Choice d = s_list[o];
+                r += before(d.c, d.place, c.c, c.place);
+                near |= d.beam != c.beam && fabs(d.c - c.c) <= 2.0 * err ? 1 : 0;
             }
-            for (int j = tid; whole && j < listed; j += kThreads) {
-                const double c = s_c[j];
-                const int place = s_place[j], beam = s_beam[j];
-                int rank = 0, near = 0;
+            rank[y] = r;
+            if (again == 0 && near && r < p.keep) {
                 for (int o = 0; o < listed; o++) {
-                    rank += before(s_c[o], s_place[o], c, place);
-                    near |= s_beam[o] != beam && fabs(s_c[o] - c) <= s_err[beam] + s_err[s_beam[o]] ? 1 : 0;
+                    const Choice d = s_list[o];
+                    const double off = s_err[c.beam] + s_err[d.beam];
+                    if (d.beam != c.beam && off > 0.0 && fabs(d.c - c.c) <= off) s_again[c.beam] = s_again[d.beam] = 1, s_any = 1;
                 }
-                if (near && rank < p.keep) {
-                    for (int o = 0; o < listed; o++) {
-                        const int other = s_beam[o];
-                        if (other != beam && s_err[beam] + s_err[other] > 0.0 && fabs(s_c[o] - c) <= s_err[beam] + s_err[other]) s_again[beam] = s_again[other] = 1, s_any = 1;
-                    }
-                }
+            }
+        }
+        if (again == 0) {
+            if (!whole) {
+                for (int beam = tid; beam < p.beams; beam += kThreads) s_again[beam] = 1;
+                if (tid == 0) s_any = 1;
             }
             __syncthreads();
             if (s_any) {
@@ -356,13 +403,12 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
             }
         }
         if (whole) {
-            for (int j = tid; j < listed; j += kThreads) {
-                const double c = s_c[j];
-                const int place = s_place[j];
-                int rank = 0;
-                for (int o = 0; o < listed; o++) rank += before(s_c[o], s_place[o], c, place);
-                if (rank < p.keep) put(rank, c, place, s_beam[j]);
-            }
+#pragma unroll
+            for (int y = 0; y < kMine; y++)
+                if (rank[y] < p.keep) {
+                    const Choice c = s_list[tid + y * kThreads];
+                    put(rank[y], c.c, c.place, c.beam);
+                }
             return;
         }
         break;
@@ -393,21 +439,33 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
     }
 }
 
-// Values of a row that a workgroup takes.
-int64_t part_of(int64_t rows, int64_t vocab) { return rows * ((vocab + 8191) / 8192) >= 256 ? 8192 : 2048; }
+// Pieces of 8 values that a thread takes: few where rows are few, so that there are workgroups for the compute units; of at most 256 bytes,
+// what its registers hold.
+int pieces_of(int64_t rows, int64_t vocab, int dtype) {
+    const int most = dtype == TROCM_F16 ? 16 : 8;
+    for (int c = most; c > 1; c /= 4)
+        if (rows * ((vocab + kThreads * kPiece * c - 1) / (kThreads * kPiece * c)) >= 2 * num_compute_units()) return c;
+    return dtype == TROCM_F16 ? 1 : 2;
+}
 
 size_t bytes_for(int64_t rows, int64_t parts, int64_t keep) { return (size_t)(rows * parts) * (sizeof(double) + sizeof(float) + sizeof(Candidate) * (size_t)keep) + 64; }
 
 }  // namespace
 
-size_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep) {
-    const int64_t rows = batch * beams, part = part_of(rows, vocab);
-    return bytes_for(rows, (vocab + part - 1) / part, keep);
+size_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep) {   // (of either type)
+    const int64_t rows = batch * beams;
+    size_t most = 0;
+    for (int dtype : {TROCM_F16, TROCM_F32}) {
+        const int64_t part = (int64_t)kThreads * kPiece * pieces_of(rows, vocab, dtype);
+        most = std::max(most, bytes_for(rows, (vocab + part - 1) / part, keep));
+    }
+    return most;
 }
 
 int launch_beam_select(const BeamSelectArgs &a, hipStream_t s) {
     if (a.batch == 0) return 0;
-    const int64_t rows = a.batch * a.beams, part = part_of(rows, a.vocab), parts = (a.vocab + part - 1) / part;
+    const int pieces = pieces_of(a.batch * a.beams, a.vocab, a.dtype);
+    const int64_t rows = a.batch * a.beams, part = (int64_t)kThreads * kPiece * pieces, parts = (a.vocab + part - 1) / part;
     TROCM_REQUIRE(a.workspace && a.workspace_bytes >= bytes_for(rows, parts, a.keep), "beam_select: the workspace must hold %zu bytes", bytes_for(rows, parts, a.keep));
     TROCM_REQUIRE(rows * parts < (1ll << 31) && a.beams * parts * a.keep < (1ll << 31), "beam_select: tensor too large");
     SelectDev p;
@@ -420,11 +478,12 @@ int launch_beam_select(const BeamSelectArgs &a, hipStream_t s) {
     p.by_parts = fast_div(parts), p.by_row_candidates = fast_div(parts * a.keep);
     const dim3 grid((unsigned)(rows * parts));
     if (a.dtype == TROCM_F16) {
-        if (part == 8192) beam_scan_kernel<_Float16, 4><<<grid, kThreads, 0, s>>>(p);
+        if (pieces == 16) beam_scan_kernel<_Float16, 16><<<grid, kThreads, 0, s>>>(p);
+        else if (pieces == 4) beam_scan_kernel<_Float16, 4><<<grid, kThreads, 0, s>>>(p);
         else beam_scan_kernel<_Float16, 1><<<grid, kThreads, 0, s>>>(p);
     } else {
-        if (part == 8192) beam_scan_kernel<float, 4><<<grid, kThreads, 0, s>>>(p);
-        else beam_scan_kernel<float, 1><<<grid, kThreads, 0, s>>>(p);
+        if (pieces == 8) beam_scan_kernel<float, 8><<<grid, kThreads, 0, s>>>(p);
+        else beam_scan_kernel<float, 2><<<grid, kThreads, 0, s>>>(p);
     }
     TROCM_HIP(hipGetLastError());
     if (a.dtype == TROCM_F16) beam_join_kernel<_Float16><<<dim3((unsigned)a.batch), kThreads, 0, s>>>(p);
