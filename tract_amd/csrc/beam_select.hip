@@ -12,6 +12,7 @@
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 #include "common.h"
 #include "fast_div.h"
 
@@ -21,7 +22,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kPiece = 8;                     // consecutive values of a lane
-constexpr int kWaveList = 128;                // values above the bound that a wave lists (at least kBeamMaxKeep); ties up to `keep` come on top
+constexpr int kWaveList = 512;                // values that a wave lists
 constexpr uint32_t kLowest = 0x007fffffu;     // key_of(-inf); 0 is below all values: nothing there
 
 struct Candidate { float x; int token; };     // token < 0: none
@@ -64,9 +65,10 @@ template <typename T> using Eight = T __attribute__((ext_vector_type(kPiece)));
 // A part of a row: kThreads * kPiece * C values, all of them asked for before the first is looked at.
 template <typename T, int C>
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
-    constexpr int kPart = kThreads * kPiece * C, kList = kWaveList + kBeamMaxKeep;
-    __shared__ Candidate s_list[kWaves * kList];
-    __shared__ int s_count[kWaves];
+    constexpr int kPart = kThreads * kPiece * C, kStep = kThreads * kPiece, kAtOnce = C < 4 ? C : 4;
+    __shared__ int s_list[kWaves * kWaveList];        // tokens
+    __shared__ Candidate s_all[kWaves * kWaveList];
+    __shared__ int s_total;
     __shared__ uint32_t s_bound[kWaves];
     __shared__ float s_max[kWaves];
     __shared__ double s_sum[kWaves];
@@ -75,151 +77,183 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
     const T *from = reinterpret_cast<const T *>(p.logits + row * p.row_bytes);
     const int i0 = part * kPart + tid * kPiece;
     // (rows begin where they begin: pieces are loaded from any element on; what is behind the row's end is -inf)
-    Eight<T> x[C];
-    if (part * kPart + kPart <= p.vocab) {
+    auto piece_at = [&](int i) __attribute__((always_inline)) {
+        Eight<T> v;
+        if (i <= p.vocab - kPiece) {
+            __builtin_memcpy(&v, from + i, sizeof(v));
+        } else {
 #pragma unroll
-        for (int c = 0; c < C; c++) __builtin_memcpy(&x[c], from + i0 + c * kThreads * kPiece, sizeof(x[c]));
+            for (int e = 0; e < kPiece; e++) v[e] = i + e < p.vocab ? from[i + e] : (T)-INFINITY;
+        }
+        return v;
+    };
+    Eight<T> x[C];
+    if (part * kPart <= p.vocab - kPart) {
+#pragma unroll
+        for (int c = 0; c < C; c++) __builtin_memcpy(&x[c], from + i0 + c * kStep, sizeof(x[c]));
     } else {
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int i = i0 + c * kThreads * kPiece;
-            if (i <= p.vocab - kPiece) {
-                __builtin_memcpy(&x[c], from + i, sizeof(x[c]));
-            } else {
-#pragma unroll
-                for (int e = 0; e < kPiece; e++) x[c][e] = i + e < p.vocab ? from[i + e] : (T)-INFINITY;
-            }
-        }
+        for (int c = 0; c < C; c++) x[c] = piece_at(i0 + c * kStep);
     }
-    Eight<T> top8 = (T)-INFINITY;
+    // (Each look at the values begins with what was loaded: kept in 32 bits from one look to the next, halves would take twice the registers.)
+    auto again = [&](int c) __attribute__((always_inline)) { asm("" : "+v"(x[c])); };
+    T most[C];   // of a piece; NaN only where all are
+    T top_t = (T)-INFINITY;
 #pragma unroll
     for (int c = 0; c < C; c++) {
-        x[c] = __builtin_elementwise_max(x[c], (Eight<T>)(T)-INFINITY);   // (the number of the two: NaN counts as -inf)
-        top8 = __builtin_elementwise_max(top8, x[c]);
+        auto v4 = __builtin_elementwise_max(__builtin_shufflevector(x[c], x[c], 0, 1, 2, 3), __builtin_shufflevector(x[c], x[c], 4, 5, 6, 7));
+        auto v2 = __builtin_elementwise_max(__builtin_shufflevector(v4, v4, 0, 1), __builtin_shufflevector(v4, v4, 2, 3));
+        most[c] = __builtin_elementwise_max(v2[0], v2[1]);
+        top_t = __builtin_elementwise_max(top_t, most[c]);
     }
-    float top = (float)top8[0];
-#pragma unroll
-    for (int e = 1; e < kPiece; e++) top = fmaxf(top, (float)top8[e]);
+    const float top = (float)top_t;
 
     // at least `keep` values of a wave reach its bound, so the largest bound will do for the workgroup
-    const uint32_t wave_bound = bound_of_lanes(key_of(top), p.keep);
+    const uint32_t wave_bound = max(bound_of_lanes(key_of(top), p.keep), kLowest);
     float m = top;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    if (lane == 0) s_bound[w] = max(wave_bound, kLowest);
-    // maximum and sum: f32 for the values of a piece, f64 from there on (beam_join_kernel's s_err says what that may be off by)
-    const float ref = m == -INFINITY ? 0.0f : m;
+    if (lane == 0) s_bound[w] = wave_bound;
+    if (tid == 0) s_total = 0;
+
+    // Maximum and sum: f32 for the values of a piece, f64 from there on.  A weight is 2^(x a - c) in one step, a = log2 e as f32 has it, c = m a
+    // rounded; what c is off by is put right at the end, what a is off by counts for x - m alone (beam_join_kernel's s_err has both).
+    const float c_m = m == -INFINITY ? 0.0f : m * kLog2e;
     double all = 0.0;
 #pragma unroll
     for (int c = 0; c < C; c++) {
-        asm("" : "+v"(x[c]));
+        again(c);
         float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kPiece; e++) sum += __builtin_amdgcn_exp2f(((float)x[c][e] - ref) * kLog2e);
+        for (int e = 0; e < kPiece; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf((float)x[c][e], kLog2e, -c_m));
         all += (double)sum;
     }
+    if (__builtin_amdgcn_ballot_w64(all != all)) {   // a NaN counts as -inf
+        all = 0.0;
+#pragma unroll 1
+        for (int i = i0; i < min(part * kPart + kPart, p.vocab); i += kStep) {
+            const Eight<T> v = piece_at(i);
+#pragma unroll
+            for (int e = 0; e < kPiece; e++) {
+                const float t = __builtin_amdgcn_exp2f(__builtin_fmaf((float)v[e], kLog2e, -c_m));
+                all += t == t ? (double)t : 0.0;
+            }
+        }
+    }
+    if (m != -INFINITY) all += all * (((double)c_m - (double)m * (double)kLog2e) * 0.6931471805599453);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
     if (lane == 0) s_max[w] = m, s_sum[w] = all;
     __syncthreads();
 
-    // the values above the bound
-    uint32_t bound_key = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
-    float bound = value_of(bound_key);
-    Candidate *list = s_list + w * kList;
-    // (Each look at the values begins with what was loaded: kept in 32 bits from one look to the next, halves would take twice the registers.)
-    auto again = [&](int c) __attribute__((always_inline)) { asm("" : "+v"(x[c])); };
-    auto pieces = [&](auto &&with) __attribute__((always_inline)) {   // pieces with values above the bound
+    // the values that reach the bound
+    const float least = value_of(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])));
+    int *list = s_list + w * kWaveList;
+    int n = 0;
+    auto list_four = [&](auto first) __attribute__((always_inline)) {   // pieces first .. of kAtOnce
+        constexpr int c0 = decltype(first)::value;
+        uint32_t hits = 0;   // bit 8 c + e
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            again(c);
-            T t = x[c][0];
+        for (int c = 0; c < kAtOnce; c++) {
+            if (__builtin_amdgcn_ballot_w64((float)most[c0 + c] >= least)) {
+                again(c0 + c);
 #pragma unroll
-            for (int e = 1; e < kPiece; e++) t = __builtin_elementwise_max(t, x[c][e]);
-            if (__builtin_amdgcn_ballot_w64((float)t > bound)) with(c);
+                for (int e = 0; e < kPiece; e++) hits |= x[c0 + c][e] >= (T)least ? 1u << (c * kPiece + e) : 0u;
+            }
+        }
+        while (const uint64_t in = __builtin_amdgcn_ballot_w64(hits != 0)) {
+            const int b = __ffs(hits) - 1, at = n + lanes_below(in);
+            if (hits && at < kWaveList) list[at] = i0 + (c0 + b / kPiece) * kStep + b % kPiece;
+            hits &= hits - 1;
+            n += __popcll(in);
         }
     };
-    int n = 0;
-    if (__builtin_amdgcn_ballot_w64(top > bound))
-        pieces([&](int c) __attribute__((always_inline)) {
-#pragma unroll
-            for (int e = 0; e < kPiece; e++) {
-                const float v = (float)x[c][e];
-                const uint64_t in = __builtin_amdgcn_ballot_w64(v > bound);
-                if (in) {
-                    const int at = n + lanes_below(in);
-                    if (v > bound && at < kWaveList) list[at] = Candidate{v, i0 + c * kThreads * kPiece + e};
-                    n += __popcll(in);
-                }
-            }
-        });
-    if (n > kWaveList) {   // too many in few lanes: the bound of all values, above which there are fewer than `keep`
-        bound_key = 0;
-#pragma unroll 1
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-            int reach = 0;
+    if (__builtin_amdgcn_ballot_w64(!(top < least))) {   // (a lane of NaN too: they tie at -inf)
+        list_four(std::integral_constant<int, 0>{});
+        if constexpr (C > 4) list_four(std::integral_constant<int, 4>{});
+        if constexpr (C > 8) list_four(std::integral_constant<int, 8>{}), list_four(std::integral_constant<int, 12>{});
+    }
+    // -inf is the bound of waves that have little else, and what lies behind the row's end has it too; and where more values reach the
+    // bound than the list holds, equal ones above all, only so many of them are wanted as could be among the best: both in the values' order,
+    // pieces, lanes, values of a piece.
+    if (n > kWaveList || (least == -INFINITY && __builtin_amdgcn_ballot_w64(!(top < least)))) {
+        uint32_t bound_key = key_of(least);
+        int above = 0;
+        auto count = [&](float reach) __attribute__((always_inline)) {
+            int k = 0;
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 again(c);
 #pragma unroll
-                for (int e = 0; e < kPiece; e++) reach += __popcll(__builtin_amdgcn_ballot_w64(key_of((float)x[c][e]) >= (bound_key | bit)));
+                for (int e = 0; e < kPiece; e++) k += __popcll(__builtin_amdgcn_ballot_w64((float)x[c][e] >= reach));
             }
-            if (reach >= p.keep) bound_key |= bit;
+            return k;
+        };
+        if (__builtin_amdgcn_ballot_w64(top > least)) above = count(value_of(bound_key + 1));
+        if (above > kWaveList - kBeamMaxKeep) {   // the bound of all values, above which there are fewer than `keep`
+            bound_key = 0;
+#pragma unroll 1
+            for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+                if ((bound_key | bit) <= kLowest || ((bound_key | bit) <= 0xff800000u && count(value_of(bound_key | bit)) >= p.keep)) bound_key |= bit;
+            bound_key = max(bound_key, kLowest);
+            above = kWaveList;
         }
-        bound = value_of(bound_key), n = 0;
-        pieces([&](int c) __attribute__((always_inline)) {
+        const float bound = value_of(bound_key);
+        n = 0;
+        int equal = 0;
+#pragma unroll 1
+        for (int c = 0; c < C && (above > 0 || equal < p.keep); c++) {
+            const int i = i0 + c * kStep;
+            const Eight<T> v = piece_at(i);
+            uint32_t hits = 0, ties = 0;
 #pragma unroll
             for (int e = 0; e < kPiece; e++) {
-                const float v = (float)x[c][e];
-                const uint64_t in = __builtin_amdgcn_ballot_w64(v > bound);
-                if (v > bound) list[n + lanes_below(in)] = Candidate{v, i0 + c * kThreads * kPiece + e};
+                const float f = (float)v[e] == (float)v[e] ? (float)v[e] : -INFINITY;
+                hits |= (f > bound ? 1u : 0u) << e, ties |= (f == bound && i + e < p.vocab ? 1u : 0u) << e;
+            }
+            while (const uint64_t in = __builtin_amdgcn_ballot_w64(hits != 0)) {
+                if (hits) list[n + lanes_below(in)] = i + __ffs(hits) - 1;
+                hits &= hits - 1;
                 n += __popcll(in);
             }
-        });
-    }
-    // and those that equal the bound, as many as could be among the best, in their order: pieces, lanes, values of a piece
-    const int most = max(n, p.keep);
-    if (n < most && __builtin_amdgcn_ballot_w64(top >= bound)) {
+            if (equal >= p.keep) continue;
+            const int mine = __popc(ties);
+            int before = equal, here = 0;
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            uint32_t ties = 0;
-            again(c);
-#pragma unroll
-            for (int e = 0; e < kPiece; e++) ties |= ((float)x[c][e] == bound ? 1u : 0u) << e;
-            if (n < most && __builtin_amdgcn_ballot_w64(ties != 0)) {
-                const int i = i0 + c * kThreads * kPiece;
-                ties &= i < p.vocab - kPiece ? 0xffu : i < p.vocab ? (1u << (p.vocab - i)) - 1 : 0u;   // (-inf behind the row's end is nothing)
-                const int mine = __popc(ties);
-                int at = n, here = 0;
-#pragma unroll
-                for (int bit = 0; bit < 4; bit++) {
-                    const uint64_t lanes = __builtin_amdgcn_ballot_w64((mine >> bit) & 1);
-                    at += lanes_below(lanes) << bit, here += __popcll(lanes) << bit;
-                }
-                for (uint32_t left = ties; left && at < most; left &= left - 1, at++) list[at] = Candidate{bound, i + __ffs(left) - 1};
-                n = min(n + here, most);
+            for (int bit = 0; bit < 4; bit++) {
+                const uint64_t lanes = __builtin_amdgcn_ballot_w64((mine >> bit) & 1);
+                before += lanes_below(lanes) << bit, here += __popcll(lanes) << bit;
             }
+            for (int at = n + before - equal; ties && before < p.keep; ties &= ties - 1, at++, before++) list[at] = i + __ffs(ties) - 1;
+            n += min(here, p.keep - equal), equal = min(equal + here, p.keep);
         }
     }
-    if (lane == 0) s_count[w] = n;
-    __syncthreads();
 
     // the workgroup's: every listed value counts those before it
-    int counts[kWaves], total = 0;
-#pragma unroll
-    for (int y = 0; y < kWaves; y++) counts[y] = s_count[y], total += counts[y];
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        Candidate c = {-INFINITY, -1};
+        if (j0 + lane < n) {
+            c.token = list[j0 + lane];
+            const float v = (float)from[c.token];
+            c.x = v == v ? v : -INFINITY;
+        }
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(c.token >= 0);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s_total, __popcll(lanes));
+        at = __builtin_amdgcn_readfirstlane(at) + lanes_below(lanes);
+        if (c.token >= 0) s_all[at] = c;
+    }
+    __syncthreads();
+    const int total = s_total;
     Candidate *best = p.part_best + (int64_t)blockIdx.x * p.keep;
     for (int j = tid; j < total; j += kThreads) {
-        int at = j, y = 0;
-        while (at >= counts[y]) at -= counts[y++];
-        const Candidate c = s_list[y * kList + at];
+        const Candidate c = s_all[j];
         int rank = 0;
-        for (int o = 0; o < kWaves; o++)
 #pragma unroll 4
-            for (int z = 0; z < counts[o]; z++) {
-                const Candidate d = s_list[o * kList + z];
-                rank += d.x > c.x || (d.x == c.x && d.token < c.token);
-            }
+        for (int z = 0; z < total; z++) {
+            const Candidate d = s_all[z];
+            rank += d.x > c.x || (d.x == c.x && d.token < c.token);
+        }
         if (rank < p.keep) best[rank] = c;
     }
     for (int j = total + tid; j < p.keep; j += kThreads) best[j] = Candidate{-INFINITY, -1};
@@ -294,9 +328,10 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
             s_max[beam] = m;
             s_ended[beam] = p.ended && p.ended[row] != 0;
             s_kind[beam] = dead ? 2 : s_ended[beam] ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
-            // What the sum may be off by, relatively, is what its logarithm is: exponents d by two half steps of f32, weighted by the weights at
-            // most ln(vocab / l) of them (their entropy is d + ln l on average), the exponential's two, a piece's seven additions; f64 from there on.
-            s_err[beam] = s_kind[beam] == 0 ? (2.0 * fmax(log((double)p.vocab / l), 0.0) + 10.0) * 0x1p-24 : 0.0;
+            // What the sum may be off by, relatively, is what its logarithm is: exponents d by a half step of f32 and a quarter for log2 e, weighted
+            // by the weights at most ln(vocab / l) of them (their entropy is d + ln l on average); another for the part's maximum, to which d
+            // counts from there; the exponential's two, a piece's seven additions; f64 from there on.
+            s_err[beam] = s_kind[beam] == 0 ? (1.5 * fmax(log((double)p.vocab / l), 0.0) + 10.0) * 0x1p-24 : 0.0;
             s_again[beam] = 0;
         }
     }
@@ -442,8 +477,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
 // Pieces of 8 values that a thread takes: few where rows are few, so that there are workgroups for the compute units; of at most 256 bytes,
 // what its registers hold.
 int pieces_of(int64_t rows, int64_t vocab, int dtype) {
-    const int most = dtype == TROCM_F16 ? 16 : 8;
-    for (int c = most; c > 1; c /= 4)
+    for (int c = dtype == TROCM_F16 ? 16 : 8; c > 1; c /= 4)
         if (rows * ((vocab + kThreads * kPiece * c - 1) / (kThreads * kPiece * c)) >= 2 * num_compute_units()) return c;
     return dtype == TROCM_F16 ? 1 : 2;
 }
