@@ -620,7 +620,7 @@ int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools
  *   eos        : -1 (none; `ended` must be NULL) or a token
  *   outputs    : [batch, keep]: scores_out f32, parents (rows of the batch: request * beams + beam), tokens, ended_out (or NULL: 1 where the token
  *                is eos or the parent had ended).  May not overlap inputs
- *   workspace  : trocm_beam_select_workspace_bytes, needs no initialisation
+ *   workspace  : trocm_beam_select_workspace_bytes, initialised by trocm_sdpa_workspace_init and shared like any other
  * A NaN among the logits counts as -inf.  keep and beams up to 64, keep at most beams * vocab, vocab up to 2^30, beams * vocab below 2^31. */
 int trocm_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep, size_t *bytes);
 int trocm_beam_select(const void *logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,

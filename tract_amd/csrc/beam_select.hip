@@ -2,17 +2,15 @@
 // ties to the lowest (beam, token).
 //
 // Within a beam the order of c is the order of the logits, which is exact; only between beams does c itself count.  So the vocabulary is
-// read once: a workgroup holds a part of a row in registers, makes its maximum and sum (f32 for eight values, then f64) and keeps its `keep`
-// largest logits; a second launch puts the parts together in f64, one workgroup per request.  Where values of two beams are nearer than those
-// sums can be told apart, the beams' sums are made again, exactly.
+// read once: a workgroup streams a part of a row through registers, makes its maximum and sum (f32 for eight values, then f64) and keeps its
+// `keep` largest logits; the last workgroup of a request to arrive puts the parts together in f64.  Where values of two beams are nearer than
+// those sums can be told apart, the beams' sums are made again, exactly.
 //
-// The largest of a wave's values: the K-th largest of the 64 lanes' maxima is found by bisection over the bits of an order-preserving
-// integer (a ballot and a count per bit); at least K values are not below it, and few more than that, which are compacted into LDS and
-// ranked by counting.  Where more values than the list holds pass, the bisection is over all values instead of the lanes' maxima.
+// The largest of a wave's values: the K-th largest of its lanes' maxima is found by bisection over the bits of an order-preserving integer
+// (ballots and counts); at least K values reach it, and few more than that, which are listed in LDS and ranked by counting.
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
-#include <type_traits>
 #include "common.h"
 #include "fast_div.h"
 
@@ -25,12 +23,13 @@ constexpr int kPiece = 8;                     // consecutive values of a lane
 constexpr int kWaveList = 512;                // values that a wave lists
 constexpr uint32_t kLowest = 0x007fffffu;     // key_of(-inf); 0 is below all values: nothing there
 
-struct Candidate { float x; int token; };     // token < 0: none
+struct alignas(8) Candidate { float x; int token; };     // token < 0: none
 
 struct SelectDev {
     const char *logits;
     int64_t row_bytes;
-    int vocab, parts, keep, beams, eos;
+    int vocab, parts, turns, keep, beams, eos, row0;   // row0: of this launch's first row, for parents
+    int *counters;              // of a request: how many of its parts are there
     float *part_max;
     double *part_sum;
     Candidate *part_best;       // [row][part][keep], best first
@@ -38,7 +37,7 @@ struct SelectDev {
     const int *ended;
     float *scores_out;
     int *parents, *tokens, *ended_out;
-    FastDiv by_parts, by_row_candidates;
+    FastDiv by_parts, by_row_candidates, by_beams;
 };
 
 // Integers in the order of the numbers; both zeros are one number and NaN counts as -inf.
@@ -51,31 +50,78 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cas
 
 __device__ __forceinline__ int lanes_below(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
 
-// The largest t that at least `count` of the wave's keys (one per lane) reach; 0 if there are fewer.
+// The largest t that at least `count` of the wave's keys (one per lane) reach; 0 if there are fewer.  Two bits a step.  Halves as 32 bits have
+// LOW = 13 low bits alike, zeros, or ones in the key of a negative number: left out, and given back as the sign has them.
+template <int LOW>
 __device__ __forceinline__ uint32_t bound_of_lanes(uint32_t key, int count) {
+    auto reach = [&](uint32_t t) __attribute__((always_inline)) { return __popcll(__builtin_amdgcn_ballot_w64(key >= t)) >= count; };
     uint32_t t = 0;
 #pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-        if (__popcll(__builtin_amdgcn_ballot_w64(key >= (t | bit))) >= count) t |= bit;
-    return t;
+    for (int at = 30; at >= LOW - 1 && at >= 0; at -= 2) {
+        const bool one = reach(t | 1u << at), two = reach(t | 2u << at), three = reach(t | 3u << at);
+        t |= three ? 3u << at : two ? 2u << at : one ? 1u << at : 0u;
+    }
+    return t == 0 || t >> 31 ? t : t | ((1u << LOW) - 1);
+}
+
+// A wave's largest value and its sum, everywhere: along the rows of 16 lanes, then over the rows; the last lane has it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int none, int x) { return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float larger(float x) {
+    return fmaxf(x, __builtin_bit_cast(float, moved<CTRL, ROWS>(__builtin_bit_cast(int, -INFINITY), __builtin_bit_cast(int, x))));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double plus(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)moved<CTRL, ROWS>(0, (int)(uint32_t)b), hi = (uint32_t)moved<CTRL, ROWS>(0, (int)(uint32_t)(b >> 32));
+    return x + __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+}
+constexpr int kShift = 0x110, kRow15 = 0x142, kRow31 = 0x143;   // lanes up within a row by n; lane 15 of a row to the next row; lane 31 to the upper half
+__device__ __forceinline__ float wave_most(float x) {
+    x = fmaxf(x, -INFINITY);
+    x = larger<kShift + 1, 0xf>(x), x = larger<kShift + 2, 0xf>(x), x = larger<kShift + 4, 0xf>(x), x = larger<kShift + 8, 0xf>(x);
+    x = larger<kRow15, 0xa>(x), x = larger<kRow31, 0xc>(x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ double wave_sum(double x) {
+    x = plus<kShift + 1, 0xf>(x), x = plus<kShift + 2, 0xf>(x), x = plus<kShift + 4, 0xf>(x), x = plus<kShift + 8, 0xf>(x);
+    x = plus<kRow15, 0xa>(x), x = plus<kRow31, 0xc>(x);
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63) << 32);
+}
+
+// What a workgroup leaves for the one that puts a request together: written through to where every compute unit sees it once it completes.
+template <typename X>
+__device__ __forceinline__ void put(X *at, X x) {
+    static_assert(sizeof(X) == 8 || sizeof(X) == 4, "one store");
+    if constexpr (sizeof(X) == 8) __hip_atomic_store(reinterpret_cast<uint64_t *>(at), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else __hip_atomic_store(reinterpret_cast<uint32_t *>(at), __builtin_bit_cast(uint32_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename X>
+__device__ __forceinline__ X get(const X *at) {
+    if constexpr (sizeof(X) == 8) return __builtin_bit_cast(X, __hip_atomic_load(reinterpret_cast<const uint64_t *>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    else return __builtin_bit_cast(X, __hip_atomic_load(reinterpret_cast<const uint32_t *>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 template <typename T> using Eight = T __attribute__((ext_vector_type(kPiece)));
 
-// A part of a row: kThreads * kPiece * C values, all of them asked for before the first is looked at.
+struct ScanLds {
+    int list[kWaves][kWaveList];      // tokens
+    Candidate all[kWaves * kWaveList];
+    double sum[kWaves];
+    float max[kWaves];
+    uint32_t bound[kWaves];
+    int total;
+};
+
+// A part of a row: `turns` tiles of kThreads * kPiece * C values, the next one in flight while one is looked at.
 template <typename T, int C>
-__global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
-    constexpr int kPart = kThreads * kPiece * C, kStep = kThreads * kPiece, kAtOnce = C < 4 ? C : 4;
-    __shared__ int s_list[kWaves * kWaveList];        // tokens
-    __shared__ Candidate s_all[kWaves * kWaveList];
-    __shared__ int s_total;
-    __shared__ uint32_t s_bound[kWaves];
-    __shared__ float s_max[kWaves];
-    __shared__ double s_sum[kWaves];
+__device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part, ScanLds &lds) {
+    constexpr int kTile = kThreads * kPiece * C, kStep = kThreads * kPiece, LOW = sizeof(T) == 2 ? 13 : 0;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-    const int row = p.by_parts.by(blockIdx.x), part = blockIdx.x - row * p.parts;
     const T *from = reinterpret_cast<const T *>(p.logits + row * p.row_bytes);
-    const int i0 = part * kPart + tid * kPiece;
+    const int begin = part * p.turns * kTile, turns = min(p.turns, (p.vocab - begin + kTile - 1) / kTile), mine = begin + tid * kPiece;
     // (rows begin where they begin: pieces are loaded from any element on; what is behind the row's end is -inf)
     auto piece_at = [&](int i) __attribute__((always_inline)) {
         Eight<T> v;
@@ -87,123 +133,125 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
         }
         return v;
     };
-    Eight<T> x[C];
-    if (part * kPart <= p.vocab - kPart) {
+    Eight<T> x[C], coming[C];
+    auto load = [&](int turn) __attribute__((always_inline)) {
+        const int i = mine + turn * kTile;
+        if (begin + turn * kTile <= p.vocab - kTile) {
 #pragma unroll
-        for (int c = 0; c < C; c++) __builtin_memcpy(&x[c], from + i0 + c * kStep, sizeof(x[c]));
-    } else {
+            for (int c = 0; c < C; c++) __builtin_memcpy(&coming[c], from + i + c * kStep, sizeof(coming[c]));
+        } else {
 #pragma unroll
-        for (int c = 0; c < C; c++) x[c] = piece_at(i0 + c * kStep);
-    }
-    // (Each look at the values begins with what was loaded: kept in 32 bits from one look to the next, halves would take twice the registers.)
-    auto again = [&](int c) __attribute__((always_inline)) { asm("" : "+v"(x[c])); };
-    T most[C];   // of a piece; NaN only where all are
-    T top_t = (T)-INFINITY;
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-        auto v4 = __builtin_elementwise_max(__builtin_shufflevector(x[c], x[c], 0, 1, 2, 3), __builtin_shufflevector(x[c], x[c], 4, 5, 6, 7));
-        auto v2 = __builtin_elementwise_max(__builtin_shufflevector(v4, v4, 0, 1), __builtin_shufflevector(v4, v4, 2, 3));
-        most[c] = __builtin_elementwise_max(v2[0], v2[1]);
-        top_t = __builtin_elementwise_max(top_t, most[c]);
-    }
-    const float top = (float)top_t;
-
-    // at least `keep` values of a wave reach its bound, so the largest bound will do for the workgroup
-    const uint32_t wave_bound = max(bound_of_lanes(key_of(top), p.keep), kLowest);
-    float m = top;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    if (lane == 0) s_bound[w] = wave_bound;
-    if (tid == 0) s_total = 0;
-
-    // Maximum and sum: f32 for the values of a piece, f64 from there on.  A weight is 2^(x a - c) in one step, a = log2 e as f32 has it, c = m a
-    // rounded; what c is off by is put right at the end, what a is off by counts for x - m alone (beam_join_kernel's s_err has both).
-    const float c_m = m == -INFINITY ? 0.0f : m * kLog2e;
-    double all = 0.0;
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-        again(c);
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < kPiece; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf((float)x[c][e], kLog2e, -c_m));
-        all += (double)sum;
-    }
-    if (__builtin_amdgcn_ballot_w64(all != all)) {   // a NaN counts as -inf
-        all = 0.0;
-#pragma unroll 1
-        for (int i = i0; i < min(part * kPart + kPart, p.vocab); i += kStep) {
-            const Eight<T> v = piece_at(i);
-#pragma unroll
-            for (int e = 0; e < kPiece; e++) {
-                const float t = __builtin_amdgcn_exp2f(__builtin_fmaf((float)v[e], kLog2e, -c_m));
-                all += t == t ? (double)t : 0.0;
-            }
-        }
-    }
-    if (m != -INFINITY) all += all * (((double)c_m - (double)m * (double)kLog2e) * 0.6931471805599453);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
-    if (lane == 0) s_max[w] = m, s_sum[w] = all;
-    __syncthreads();
-
-    // the values that reach the bound
-    const float least = value_of(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])));
-    int *list = s_list + w * kWaveList;
-    int n = 0;
-    auto list_four = [&](auto first) __attribute__((always_inline)) {   // pieces first .. of kAtOnce
-        constexpr int c0 = decltype(first)::value;
-        uint32_t hits = 0;   // bit 8 c + e
-#pragma unroll
-        for (int c = 0; c < kAtOnce; c++) {
-            if (__builtin_amdgcn_ballot_w64((float)most[c0 + c] >= least)) {
-                again(c0 + c);
-#pragma unroll
-                for (int e = 0; e < kPiece; e++) hits |= x[c0 + c][e] >= (T)least ? 1u << (c * kPiece + e) : 0u;
-            }
-        }
-        while (const uint64_t in = __builtin_amdgcn_ballot_w64(hits != 0)) {
-            const int b = __ffs(hits) - 1, at = n + lanes_below(in);
-            if (hits && at < kWaveList) list[at] = i0 + (c0 + b / kPiece) * kStep + b % kPiece;
-            hits &= hits - 1;
-            n += __popcll(in);
+            for (int c = 0; c < C; c++) coming[c] = piece_at(i + c * kStep);
         }
     };
-    if (__builtin_amdgcn_ballot_w64(!(top < least))) {   // (a lane of NaN too: they tie at -inf)
-        list_four(std::integral_constant<int, 0>{});
-        if constexpr (C > 4) list_four(std::integral_constant<int, 4>{});
-        if constexpr (C > 8) list_four(std::integral_constant<int, 8>{}), list_four(std::integral_constant<int, 12>{});
+    int *list = lds.list[w];
+    int n = 0;
+    uint32_t bound_key = 0;
+    float least = -INFINITY, m = -INFINITY, top = -INFINITY, c_m = 0.0f;
+    double all = 0.0;
+    // A sum against one reference as a sum against another one: both are exact but for f64.
+    auto against = [&](double sum, float c, float ref) { return ref == -INFINITY ? 0.0 : sum * exp((double)c * 0.6931471805599453 - (double)ref * ((double)kLog2e * 0.6931471805599453)); };
+    load(0);
+#pragma unroll 1
+    for (int turn = 0; turn < turns; turn++) {
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c] = coming[c];
+        if (turn + 1 < turns) load(turn + 1);
+        T most[C], top_t = (T)-INFINITY;   // of a piece; NaN only where all are
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            auto v4 = __builtin_elementwise_max(__builtin_shufflevector(x[c], x[c], 0, 1, 2, 3), __builtin_shufflevector(x[c], x[c], 4, 5, 6, 7));
+            auto v2 = __builtin_elementwise_max(__builtin_shufflevector(v4, v4, 0, 1), __builtin_shufflevector(v4, v4, 2, 3));
+            most[c] = __builtin_elementwise_max(v2[0], v2[1]);
+            top_t = __builtin_elementwise_max(top_t, most[c]);
+        }
+        const float now = (float)top_t;
+        top = fmaxf(top, now);
+        // Maximum and sum: f32 for the values of a piece, f64 from there on.  A weight is 2^(x a - c) in one step, a = log2 e as f32 has it,
+        // c = m a rounded; what c is off by is put right with the reference, what a is off by counts for x - m alone (join_request's err has
+        // both).  m is the largest value of the first tile, or of a later one that has one more than 2 above.
+        if (__builtin_amdgcn_ballot_w64(now > m + 2.0f)) {
+            const float was = m, c_was = c_m;
+            m = wave_most(top);
+            c_m = m * kLog2e;
+            all = was == -INFINITY ? 0.0 : all * exp(((double)c_was - (double)c_m) * 0.6931471805599453);
+        }
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kPiece; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf((float)x[c][e], kLog2e, -c_m));
+            all += (double)sum;
+        }
+        if (__builtin_amdgcn_ballot_w64(all != all) && m < INFINITY) {   // a NaN counts as -inf: the sum so far again
+            all = 0.0;
+#pragma unroll 1
+            for (int i = mine; i < min(mine + (turn + 1) * kTile, p.vocab); i += kStep) {
+                const Eight<T> v = piece_at(i);
+#pragma unroll
+                for (int e = 0; e < kPiece; e++) {
+                    const float t = __builtin_amdgcn_exp2f(__builtin_fmaf((float)v[e], kLog2e, -c_m));
+                    all += t == t ? (double)t : 0.0;
+                }
+            }
+        }
+        // The values that could be among the best: of the first tile at least `keep` reach its bound (all but -inf is listed where fewer
+        // lanes have a value); from then on they do of all.
+        if (turn == 0) bound_key = max(bound_of_lanes<LOW>(key_of(top), p.keep), kLowest), least = value_of(bound_key);
+        if (__builtin_amdgcn_ballot_w64(now >= least && now > -INFINITY)) {
+            uint32_t hits = 0;   // bit 8 c + e
+#pragma unroll
+            for (int c = 0; c < C; c++)
+                if (__builtin_amdgcn_ballot_w64((float)most[c] >= least)) {
+                    asm("" : "+v"(x[c]));   // (halves that are kept as 32 bits from the sum to here would take twice the registers)
+#pragma unroll
+                    for (int e = 0; e < kPiece; e++) hits |= x[c][e] >= (T)least && x[c][e] > (T)-INFINITY ? 1u << (c * kPiece + e) : 0u;
+                }
+            while (const uint64_t in = __builtin_amdgcn_ballot_w64(hits != 0)) {
+                const int b = __ffs(hits) - 1, at = n + lanes_below(in);
+                if (hits && at < kWaveList) list[at] = mine + turn * kTile + (b / kPiece) * kStep + b % kPiece;
+                hits &= hits - 1;
+                n += __popcll(in);
+            }
+        }
     }
-    // -inf is the bound of waves that have little else, and what lies behind the row's end has it too; and where more values reach the
-    // bound than the list holds, equal ones above all, only so many of them are wanted as could be among the best: both in the values' order,
-    // pieces, lanes, values of a piece.
-    if (n > kWaveList || (least == -INFINITY && __builtin_amdgcn_ballot_w64(!(top < least)))) {
-        uint32_t bound_key = key_of(least);
-        int above = 0;
-        auto count = [&](float reach) __attribute__((always_inline)) {
+    const uint32_t wave_bound = max(bound_of_lanes<LOW>(key_of(top), p.keep), bound_key);
+    if (lane == 0) lds.bound[w] = wave_bound;
+    if (tid == 0) lds.total = 0;
+    if (m < INFINITY) all = against(all, c_m, m);
+    all = wave_sum(all);
+    if (lane == 0) lds.max[w] = m, lds.sum[w] = all;
+    __syncthreads();
+    bound_key = max(max(lds.bound[0], lds.bound[1]), max(lds.bound[2], lds.bound[3]));   // (at least `keep` values reach the largest of the waves')
+    least = value_of(bound_key);
+
+    // Where the list does not hold what reaches the wave's own bound, equal values above all, or the workgroup's bound is -inf: what is above the
+    // bound, and of what equals it only so many as could be among the best, in their order: tiles, pieces, lanes, values of a piece.
+    if (n > kWaveList || least == -INFINITY) {
+        const int end = min(begin + turns * kTile, p.vocab);
+        auto count = [&](float reach) {
             int k = 0;
+#pragma unroll 1
+            for (int i = mine; i - lane * kPiece < end; i += kStep) {
+                const Eight<T> v = piece_at(i);
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                again(c);
-#pragma unroll
-                for (int e = 0; e < kPiece; e++) k += __popcll(__builtin_amdgcn_ballot_w64((float)x[c][e] >= reach));
+                for (int e = 0; e < kPiece; e++) k += __popcll(__builtin_amdgcn_ballot_w64((float)v[e] >= reach));
             }
             return k;
         };
-        if (__builtin_amdgcn_ballot_w64(top > least)) above = count(value_of(bound_key + 1));
-        if (above > kWaveList - kBeamMaxKeep) {   // the bound of all values, above which there are fewer than `keep`
+        bool above = __builtin_amdgcn_ballot_w64(top > least) != 0;
+        if (above && count(value_of(bound_key + 1)) > kWaveList - kBeamMaxKeep) {   // the bound of all values, above which there are fewer than `keep`
             bound_key = 0;
 #pragma unroll 1
             for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
                 if ((bound_key | bit) <= kLowest || ((bound_key | bit) <= 0xff800000u && count(value_of(bound_key | bit)) >= p.keep)) bound_key |= bit;
             bound_key = max(bound_key, kLowest);
-            above = kWaveList;
         }
         const float bound = value_of(bound_key);
         n = 0;
         int equal = 0;
 #pragma unroll 1
-        for (int c = 0; c < C && (above > 0 || equal < p.keep); c++) {
-            const int i = i0 + c * kStep;
+        for (int i = mine; i - lane * kPiece < end && (above || equal < p.keep); i += kStep) {
             const Eight<T> v = piece_at(i);
             uint32_t hits = 0, ties = 0;
 #pragma unroll
@@ -217,16 +265,16 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
                 n += __popcll(in);
             }
             if (equal >= p.keep) continue;
-            const int mine = __popc(ties);
             int before = equal, here = 0;
 #pragma unroll
             for (int bit = 0; bit < 4; bit++) {
-                const uint64_t lanes = __builtin_amdgcn_ballot_w64((mine >> bit) & 1);
+                const uint64_t lanes = __builtin_amdgcn_ballot_w64((__popc(ties) >> bit) & 1);
                 before += lanes_below(lanes) << bit, here += __popcll(lanes) << bit;
             }
             for (int at = n + before - equal; ties && before < p.keep; ties &= ties - 1, at++, before++) list[at] = i + __ffs(ties) - 1;
             n += min(here, p.keep - equal), equal = min(equal + here, p.keep);
         }
+        least = -INFINITY;   // (all of the list)
     }
 
     // the workgroup's: every listed value counts those before it
@@ -237,54 +285,76 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(SelectDev p) {
             const float v = (float)from[c.token];
             c.x = v == v ? v : -INFINITY;
         }
-        const uint64_t lanes = __builtin_amdgcn_ballot_w64(c.token >= 0);
+        const bool in = c.token >= 0 && c.x >= least;
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
         int at = 0;
-        if (lane == 0) at = atomicAdd(&s_total, __popcll(lanes));
+        if (lane == 0) at = atomicAdd(&lds.total, __popcll(lanes));
         at = __builtin_amdgcn_readfirstlane(at) + lanes_below(lanes);
-        if (c.token >= 0) s_all[at] = c;
+        if (in) lds.all[at] = c;
     }
     __syncthreads();
-    const int total = s_total;
-    Candidate *best = p.part_best + (int64_t)blockIdx.x * p.keep;
+    const int total = lds.total;
+    const int64_t at_part = (int64_t)row * p.parts + part;
+    Candidate *best = p.part_best + at_part * p.keep;
     for (int j = tid; j < total; j += kThreads) {
-        const Candidate c = s_all[j];
+        const Candidate c = lds.all[j];
         int rank = 0;
 #pragma unroll 4
         for (int z = 0; z < total; z++) {
-            const Candidate d = s_all[z];
+            const Candidate d = lds.all[z];
             rank += d.x > c.x || (d.x == c.x && d.token < c.token);
         }
-        if (rank < p.keep) best[rank] = c;
+        if (rank < p.keep) put(best + rank, c);
     }
-    for (int j = total + tid; j < p.keep; j += kThreads) best[j] = Candidate{-INFINITY, -1};
-    if (tid == 0) {
-        float mm = s_max[0];
-        for (int y = 1; y < kWaves; y++) mm = fmaxf(mm, s_max[y]);
-        double l = 0.0;
-        for (int y = 0; y < kWaves; y++) l += s_max[y] == -INFINITY ? 0.0 : s_sum[y] * exp((double)s_max[y] - (double)mm);
-        p.part_max[blockIdx.x] = mm, p.part_sum[blockIdx.x] = l;
+    for (int j = total + tid; j < p.keep; j += kThreads) put(best + j, Candidate{-INFINITY, -1});
+    if (w == 0) {   // (a lane per wave's sum)
+        const float mine_m = lds.max[lane & 3], mm = fmaxf(fmaxf(lds.max[0], lds.max[1]), fmaxf(lds.max[2], lds.max[3]));
+        double l = mine_m == -INFINITY ? 0.0 : lds.sum[lane & 3] * exp((double)mine_m - (double)mm);
+        l += __shfl_xor(l, 1, 64);
+        l += __shfl_xor(l, 2, 64);
+        if (lane == 0) put(p.part_max + at_part, mm), put(p.part_sum + at_part, l);
     }
 }
 
-// ---- parts and beams put together: a workgroup per request ------------------------------------------------------------------
+// ---- parts and beams put together: the last workgroup of a request ----------------------------------------------------------
 
 constexpr int kJoinList = 1024;
 struct Choice { double c; int place, beam; };   // place: beam * vocab + token (below 2^31, checked by the host); < 0: none
 
 __device__ __forceinline__ bool before(double c, int place, double d, int other) { return c > d || (c == d && place < other); }
 
+// 2^t for t <= 0 times 2^shift, in f64: the exponential's series for the fraction, of at most a half (the twelfth term is 6e-15).
+__device__ __forceinline__ double exp2_scaled(double t, int shift) {
+    const double n = __builtin_rint(t), r = (t - n) * 0.6931471805599453;
+    double y = 1.0 / 39916800.0;
+    constexpr double kInverse[11] = {1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+#pragma unroll
+    for (int i = 0; i < 11; i++) y = __builtin_fma(y, r, kInverse[i]);
+    return __builtin_ldexp(y, (int)fmax(n, -2000.0) + shift);
+}
+
 // log sum exp of a row whose largest value is m, the same for the same values in any order: terms of 64 bits, rounded to whole multiples of
-// 2^-shift of the largest and added as integers.  All threads; only where two beams are nearer than their 32-bit sums tell apart (about
-// one launch in twenty of 32 requests of 8 beams over 128256 tokens).
+// 2^-shift of the largest and added as integers.  All threads; only where two beams are nearer than their 32-bit sums tell apart.
 template <typename T>
 __device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint64_t *lds_sums) {
     const int shift = 61 - (32 - __clz(vocab)), tid = threadIdx.x;
     uint64_t sum = 0;
-#pragma unroll 8
-    for (int i = tid; i < vocab; i += kThreads) {
-        const float v = (float)x[i];
-        sum += v == v ? (uint64_t)(ldexp(exp((double)v - (double)m), shift) + 0.5) : 0;
+    auto add = [&](float v) { sum += v == v ? (uint64_t)(exp2_scaled(((double)v - (double)m) * 1.4426950408889634, shift) + 0.5) : 0; };
+    constexpr int kStep = kThreads * kPiece;
+    const int whole = vocab / kPiece * kPiece;
+    Eight<T> coming[2];
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+        if (tid * kPiece + y * kStep < whole) __builtin_memcpy(&coming[y], x + tid * kPiece + y * kStep, sizeof(coming[y]));
+#pragma unroll 1
+    for (int i = tid * kPiece; i < whole; i += kStep) {
+        const Eight<T> now = coming[0];
+        coming[0] = coming[1];
+        if (i + 2 * kStep < whole) __builtin_memcpy(&coming[1], x + i + 2 * kStep, sizeof(coming[1]));
+#pragma unroll
+        for (int e = 0; e < kPiece; e++) add((float)now[e]);
     }
+    if (whole + tid < vocab) add((float)x[whole + tid]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += (uint64_t)__shfl_xor((unsigned long long)sum, d, 64);
     __syncthreads();
@@ -295,47 +365,56 @@ __device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint
     return (double)m + log(ldexp((double)sum, -shift));
 }
 
+struct JoinLds {
+    Choice list[kJoinList];
+    double lse[kBeamMaxBeams], score[kBeamMaxBeams], err[kBeamMaxBeams], best_c[kWaves];
+    uint64_t sums[kWaves];
+    float max[kBeamMaxBeams];
+    int kind[kBeamMaxBeams], ended[kBeamMaxBeams];   // kind 0: goes on, 1: stays at the token of the ended, 2: has no candidates but of -inf
+    int again[kBeamMaxBeams], any, count, best_place[kWaves], best_beam[kWaves];
+    uint32_t bound[kWaves];
+};
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
-    __shared__ double s_lse[kBeamMaxBeams], s_score[kBeamMaxBeams], s_err[kBeamMaxBeams];
-    __shared__ float s_max[kBeamMaxBeams];
-    __shared__ int s_kind[kBeamMaxBeams], s_ended[kBeamMaxBeams];   // kind 0: goes on, 1: stays at the token of the ended, 2: has no candidates but of -inf
-    __shared__ int s_again[kBeamMaxBeams], s_any;
-    __shared__ Choice s_list[kJoinList];
-    __shared__ double s_best_c[kWaves];
-    __shared__ int s_count, s_best_place[kWaves], s_best_beam[kWaves];
-    __shared__ uint64_t s_sums[kWaves];
-    __shared__ uint32_t s_bound[kWaves];
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, request = blockIdx.x;
+__device__ __forceinline__ void join_request(const SelectDev &p, int request, JoinLds &lds) {
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     constexpr int kLanes = 16;   // of a beam
     for (int beam = tid / kLanes; beam < p.beams; beam += kThreads / kLanes) {
         const int64_t row = (int64_t)request * p.beams + beam;
         const float *pm = p.part_max + row * p.parts;
         const double *ps = p.part_sum + row * p.parts;
-        float m = -INFINITY;
-        for (int i = tid % kLanes; i < p.parts; i += kLanes) m = fmaxf(m, pm[i]);
+        const Candidate *first = p.part_best + row * p.parts * p.keep;   // of every part its best
+        float m = -INFINITY, top = -INFINITY, over = 0.0f;               // the largest reference, the largest value, how far one is above its part's reference
+        for (int i = tid % kLanes; i < p.parts; i += kLanes) {
+            const float ref = get(pm + i), most = get(first + i * (int64_t)p.keep).x;
+            m = fmaxf(m, ref), top = fmaxf(top, most), over = fmaxf(over, most - ref);   // (NaN where both are infinite: no number)
+        }
 #pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        for (int d = 1; d < kLanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64)), top = fmaxf(top, __shfl_xor(top, d, 64)), over = fmaxf(over, __shfl_xor(over, d, 64));
         double l = 0.0;
-        for (int i = tid % kLanes; i < p.parts; i += kLanes) l += pm[i] == -INFINITY ? 0.0 : ps[i] * exp((double)pm[i] - (double)m);
+        for (int i = tid % kLanes; i < p.parts; i += kLanes) {
+            const float ref = get(pm + i);
+            l += ref == -INFINITY ? 0.0 : get(ps + i) * exp((double)ref - (double)m);
+        }
 #pragma unroll
         for (int d = 1; d < kLanes; d <<= 1) l += __shfl_xor(l, d, 64);
         if (tid % kLanes == 0) {
             const float score = p.scores[row];
             const bool dead = !(fabsf(score) < INFINITY);
-            s_score[beam] = dead ? -INFINITY : (double)score;
-            s_lse[beam] = (double)m + log(l);
-            s_max[beam] = m;
-            s_ended[beam] = p.ended && p.ended[row] != 0;
-            s_kind[beam] = dead ? 2 : s_ended[beam] ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
-            // What the sum may be off by, relatively, is what its logarithm is: exponents d by a half step of f32 and a quarter for log2 e, weighted
-            // by the weights at most ln(vocab / l) of them (their entropy is d + ln l on average); another for the part's maximum, to which d
-            // counts from there; the exponential's two, a piece's seven additions; f64 from there on.
-            s_err[beam] = s_kind[beam] == 0 ? (1.5 * fmax(log((double)p.vocab / l), 0.0) + 10.0) * 0x1p-24 : 0.0;
-            s_again[beam] = 0;
+            lds.score[beam] = dead ? -INFINITY : (double)score;
+            lds.lse[beam] = (double)m + log(l);
+            lds.max[beam] = top;
+            lds.ended[beam] = p.ended && p.ended[row] != 0;
+            lds.kind[beam] = dead ? 2 : lds.ended[beam] ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
+            // What the sum may be off by, relatively, is what its logarithm is: exponents x - ref by a half step of f32 and a quarter for log2 e,
+            // weighted by the weights at most ln(vocab / l) of them (their entropy is ref - x + ln l on average) and twice what lies above the
+            // reference, which is at most `over` and what a wave's may be below its part's, 2; the exponential's two, a piece's seven additions;
+            // f64 from there on.
+            lds.err[beam] = lds.kind[beam] == 0 ? (1.5 * (fmax(log((double)p.vocab / l), 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 : 0.0;
+            lds.again[beam] = 0;
         }
     }
-    if (tid == 0) s_any = 0;
+    if (tid == 0) lds.any = 0;
     __syncthreads();
 
     const int per_row = p.parts * p.keep, n = p.beams * per_row;
@@ -343,58 +422,66 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
     auto candidate = [&](int j) {
         const int beam = p.by_row_candidates.by(j), k = j - beam * per_row;
         Choice r = {-INFINITY, -1, beam};
-        if (s_kind[beam] == 0) {
-            const Candidate c = all[j];
-            if (c.token >= 0) r.c = s_score[beam] + ((double)c.x - s_lse[beam]), r.place = beam * p.vocab + c.token;
+        if (lds.kind[beam] == 0) {
+            const Candidate c = get(all + j);
+            if (c.token >= 0) r.c = lds.score[beam] + ((double)c.x - lds.lse[beam]), r.place = beam * p.vocab + c.token;
         } else if (k < p.keep) {   // the token that an ended beam stays at, and then, as in a beam without values, tokens in their order
-            const bool stays = s_kind[beam] == 1 && k == 0;
-            const int token = s_kind[beam] == 1 ? (stays ? p.eos : k - 1 < p.eos ? k - 1 : k) : k;
-            if (stays) r.c = s_score[beam];
+            const bool stays = lds.kind[beam] == 1 && k == 0;
+            const int token = lds.kind[beam] == 1 ? (stays ? p.eos : k - 1 < p.eos ? k - 1 : k) : k;
+            if (stays) r.c = lds.score[beam];
             if (token < p.vocab) r.place = beam * p.vocab + token;
         }
         return r;
     };
-    auto put = [&](int rank, double c, int place, int beam) {
+    auto chosen = [&](int rank, double c, int place, int beam) {
         const int token = place - beam * p.vocab;
         const int64_t at = (int64_t)request * p.keep + rank;
         p.scores_out[at] = (float)c;
-        p.parents[at] = request * p.beams + beam;
+        p.parents[at] = p.row0 + request * p.beams + beam;
         p.tokens[at] = token;
-        if (p.ended_out) p.ended_out[at] = token == p.eos || s_ended[beam];
+        if (p.ended_out) p.ended_out[at] = token == p.eos || lds.ended[beam];
     };
     double err = 0.0;
-    for (int beam = 0; beam < p.beams; beam++) err = fmax(err, s_err[beam]);
+    for (int beam = 0; beam < p.beams; beam++) err = fmax(err, lds.err[beam]);
+    constexpr int kHeld = 4;   // candidates that a thread keeps from the first look at them to the second
     for (int again = 0;; again++) {
-        // at least `keep` of a wave's candidates reach its bound (of f32, whose order is that of f64 but for ties); all that could be among the
-        // best are listed
+        // at least `keep` of a wave's candidates reach its bound (of f32, whose order is that of f64 but for ties), so the largest bound will
+        // do; all that could be among the best are listed
+        Choice held[kHeld];
         uint32_t top = 0;
-        for (int j = tid; j < n; j += kThreads) {
+#pragma unroll
+        for (int y = 0; y < kHeld; y++) {
+            const int j = tid + y * kThreads;
+            held[y] = j < n ? candidate(j) : Choice{-INFINITY, -1, 0};
+            if (held[y].place >= 0) top = max(top, key_of((float)held[y].c));
+        }
+        for (int j = tid + kHeld * kThreads; j < n; j += kThreads) {
             const Choice r = candidate(j);
             if (r.place >= 0) top = max(top, key_of((float)r.c));
         }
-        const uint32_t wave_bound = bound_of_lanes(top, p.keep);
+        const uint32_t wave_bound = bound_of_lanes<0>(top, p.keep);
         __syncthreads();   // (what the last turn has listed is done with)
-        if (lane == 0) s_bound[w] = wave_bound;
-        if (tid == 0) s_count = 0;
+        if (lane == 0) lds.bound[w] = wave_bound;
+        if (tid == 0) lds.count = 0;
         __syncthreads();
-        const float bound = value_of(max(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])), kLowest));
+        const float bound = value_of(max(max(max(lds.bound[0], lds.bound[1]), max(lds.bound[2], lds.bound[3])), kLowest));
         const double from = (double)bound - 0x1p-23 * fabs((double)bound) - 0x1p-149 - 2.0 * err;   // (-inf stays that)
-        for (int j0 = 0; j0 < n; j0 += kThreads) {
-            const int j = j0 + tid;
-            Choice r = {-INFINITY, -1, 0};
-            if (j < n) r = candidate(j);
+        auto add = [&](const Choice &r) __attribute__((always_inline)) {
             const bool in = r.place >= 0 && (r.c >= from || bound == -INFINITY);
             const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
             if (lanes) {
                 int at = 0;
-                if (lane == 0) at = atomicAdd(&s_count, __popcll(lanes));
+                if (lane == 0) at = atomicAdd(&lds.count, __popcll(lanes));
                 at = __builtin_amdgcn_readfirstlane(at) + lanes_below(lanes);
-                if (in && at < kJoinList) s_list[at] = r;
+                if (in && at < kJoinList) lds.list[at] = r;
             }
-        }
+        };
+#pragma unroll
+        for (int y = 0; y < kHeld; y++) add(held[y]);
+        for (int j0 = kHeld * kThreads; j0 < n; j0 += kThreads) add(j0 + tid < n ? candidate(j0 + tid) : Choice{-INFINITY, -1, 0});
         __syncthreads();
-        const int listed = min(s_count, kJoinList);
-        const bool whole = s_count <= kJoinList;
+        const int listed = min(lds.count, kJoinList);
+        const bool whole = lds.count <= kJoinList;
         // Every listed value counts those before it; a value that is nearer to another beam's than sums of 32-bit terms tell apart asks for
         // both beams' sums to be made again.
         constexpr int kMine = kJoinList / kThreads;
@@ -404,34 +491,34 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
             const int j = tid + y * kThreads;
             rank[y] = p.keep;
             if (!whole || j >= listed) continue;
-            const Choice c = s_list[j];
+            const Choice c = lds.list[j];
             int r = 0, near = 0;
 #pragma unroll 4
             for (int o = 0; o < listed; o++) {
-                const Choice d = s_list[o];
+                const Choice d = lds.list[o];
                 r += before(d.c, d.place, c.c, c.place);
                 near |= d.beam != c.beam && fabs(d.c - c.c) <= 2.0 * err ? 1 : 0;
             }
             rank[y] = r;
             if (again == 0 && near && r < p.keep) {
                 for (int o = 0; o < listed; o++) {
-                    const Choice d = s_list[o];
-                    const double off = s_err[c.beam] + s_err[d.beam];
-                    if (d.beam != c.beam && off > 0.0 && fabs(d.c - c.c) <= off) s_again[c.beam] = s_again[d.beam] = 1, s_any = 1;
+                    const Choice d = lds.list[o];
+                    const double off = lds.err[c.beam] + lds.err[d.beam];
+                    if (d.beam != c.beam && off > 0.0 && fabs(d.c - c.c) <= off) lds.again[c.beam] = lds.again[d.beam] = 1, lds.any = 1;
                 }
             }
         }
         if (again == 0) {
             if (!whole) {
-                for (int beam = tid; beam < p.beams; beam += kThreads) s_again[beam] = 1;
-                if (tid == 0) s_any = 1;
+                for (int beam = tid; beam < p.beams; beam += kThreads) lds.again[beam] = 1;
+                if (tid == 0) lds.any = 1;
             }
             __syncthreads();
-            if (s_any) {
+            if (lds.any) {
                 for (int beam = 0; beam < p.beams; beam++)
-                    if (s_again[beam] && s_kind[beam] == 0) {
-                        const double lse = exact_lse(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, s_max[beam], s_sums);
-                        if (tid == 0) s_lse[beam] = lse;
+                    if (lds.again[beam] && lds.kind[beam] == 0) {
+                        const double lse = exact_lse(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, lds.max[beam], lds.sums);
+                        if (tid == 0) lds.lse[beam] = lse;
                     }
                 __syncthreads();
                 continue;
@@ -441,8 +528,8 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
 #pragma unroll
             for (int y = 0; y < kMine; y++)
                 if (rank[y] < p.keep) {
-                    const Choice c = s_list[tid + y * kThreads];
-                    put(rank[y], c.c, c.place, c.beam);
+                    const Choice c = lds.list[tid + y * kThreads];
+                    chosen(rank[y], c.c, c.place, c.beam);
                 }
             return;
         }
@@ -463,66 +550,87 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectDev p) {
             const int place = __shfl_xor(best.place, d, 64), beam = __shfl_xor(best.beam, d, 64);
             if (place >= 0 && (best.place < 0 || before(c, place, best.c, best.place))) best = {c, place, beam};
         }
-        if (lane == 0) s_best_c[w] = best.c, s_best_place[w] = best.place, s_best_beam[w] = best.beam;
+        if (lane == 0) lds.best_c[w] = best.c, lds.best_place[w] = best.place, lds.best_beam[w] = best.beam;
         __syncthreads();
         best = {-INFINITY, -1, 0};
         for (int y = 0; y < kWaves; y++)
-            if (s_best_place[y] >= 0 && (best.place < 0 || before(s_best_c[y], s_best_place[y], best.c, best.place))) best = {s_best_c[y], s_best_place[y], s_best_beam[y]};
-        if (tid == 0 && best.place >= 0) put(rank, best.c, best.place, best.beam);
+            if (lds.best_place[y] >= 0 && (best.place < 0 || before(lds.best_c[y], lds.best_place[y], best.c, best.place))) best = {lds.best_c[y], lds.best_place[y], lds.best_beam[y]};
+        if (tid == 0 && best.place >= 0) chosen(rank, best.c, best.place, best.beam);
         last_c = best.c, last_place = best.place;
         __syncthreads();
     }
 }
 
-// Pieces of 8 values that a thread takes: few where rows are few, so that there are workgroups for the compute units; of at most 256 bytes,
-// what its registers hold.
-int pieces_of(int64_t rows, int64_t vocab, int dtype) {
-    for (int c = dtype == TROCM_F16 ? 16 : 8; c > 1; c /= 4)
-        if (rows * ((vocab + kThreads * kPiece * c - 1) / (kThreads * kPiece * c)) >= 2 * num_compute_units()) return c;
-    return dtype == TROCM_F16 ? 1 : 2;
+template <typename T, int C>
+__global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
+    __shared__ union Lds { ScanLds scan; JoinLds join; __device__ Lds() {} } lds;
+    __shared__ int s_last;
+    const int row = p.by_parts.by(blockIdx.x), part = blockIdx.x - row * p.parts, request = p.by_beams.by(row);
+    scan_part<T, C>(p, row, part, lds.scan);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what this thread leaves has completed
+    __syncthreads();                                     // ... and what the whole workgroup does
+    if (threadIdx.x == 0) {
+        s_last = __hip_atomic_fetch_add(p.counters + request, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.parts * p.beams - 1;
+        if (s_last) __hip_atomic_store(p.counters + request, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s_last) join_request<T>(p, request, lds.join);
 }
 
-size_t bytes_for(int64_t rows, int64_t parts, int64_t keep) { return (size_t)(rows * parts) * (sizeof(double) + sizeof(float) + sizeof(Candidate) * (size_t)keep) + 64; }
+// How rows are cut into parts: tiles of 4 pieces of 8 values a thread, or of 1 where that leaves compute units without a workgroup; and as many
+// tiles one after the other as leave each compute unit kPerUnit workgroups.
+constexpr int kPerUnit = 4;
+struct Cut { int pieces; int64_t parts, turns; };
+Cut cut_of(int64_t rows, int64_t vocab) {
+    Cut c;
+    auto tiles = [&](int pieces) { return (vocab + kThreads * kPiece * pieces - 1) / (kThreads * kPiece * pieces); };
+    c.pieces = rows * tiles(4) >= 2 * num_compute_units() ? 4 : 1;
+    const int64_t all = tiles(c.pieces);
+    c.parts = std::min(all, std::max<int64_t>(1, ((int64_t)kPerUnit * num_compute_units() + rows - 1) / rows));
+    c.turns = (all + c.parts - 1) / c.parts;
+    c.parts = (all + c.turns - 1) / c.turns;
+    return c;
+}
+
+constexpr int64_t kCounters = kWsCounterBytes / 4;   // requests of a launch, at most
+size_t bytes_for(int64_t rows, int64_t parts, int64_t keep) { return kWsCounterBytes + (size_t)(rows * parts) * (sizeof(double) + sizeof(float) + sizeof(Candidate) * (size_t)keep); }
 
 }  // namespace
 
-size_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep) {   // (of either type)
-    const int64_t rows = batch * beams;
-    size_t most = 0;
-    for (int dtype : {TROCM_F16, TROCM_F32}) {
-        const int64_t part = (int64_t)kThreads * kPiece * pieces_of(rows, vocab, dtype);
-        most = std::max(most, bytes_for(rows, (vocab + part - 1) / part, keep));
-    }
-    return most;
+size_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep) {
+    return bytes_for(batch * beams, cut_of(batch * beams, vocab).parts, keep);
 }
 
 int launch_beam_select(const BeamSelectArgs &a, hipStream_t s) {
     if (a.batch == 0) return 0;
-    const int pieces = pieces_of(a.batch * a.beams, a.vocab, a.dtype);
-    const int64_t rows = a.batch * a.beams, part = (int64_t)kThreads * kPiece * pieces, parts = (a.vocab + part - 1) / part;
-    TROCM_REQUIRE(a.workspace && a.workspace_bytes >= bytes_for(rows, parts, a.keep), "beam_select: the workspace must hold %zu bytes", bytes_for(rows, parts, a.keep));
-    TROCM_REQUIRE(rows * parts < (1ll << 31) && a.beams * parts * a.keep < (1ll << 31), "beam_select: tensor too large");
-    SelectDev p;
-    p.logits = (const char *)a.logits, p.row_bytes = a.row_stride * (int64_t)elem_bytes(a.dtype);
-    p.vocab = (int)a.vocab, p.parts = (int)parts, p.keep = (int)a.keep, p.beams = (int)a.beams, p.eos = a.eos;
-    p.part_sum = (double *)(((uintptr_t)a.workspace + 15) & ~(uintptr_t)15);
-    p.part_best = (Candidate *)(p.part_sum + rows * parts);
-    p.part_max = (float *)(p.part_best + rows * parts * a.keep);
-    p.scores = a.scores, p.ended = a.ended, p.scores_out = a.scores_out, p.parents = a.parents, p.tokens = a.tokens, p.ended_out = a.ended_out;
-    p.by_parts = fast_div(parts), p.by_row_candidates = fast_div(parts * a.keep);
-    const dim3 grid((unsigned)(rows * parts));
-    if (a.dtype == TROCM_F16) {
-        if (pieces == 16) beam_scan_kernel<_Float16, 16><<<grid, kThreads, 0, s>>>(p);
-        else if (pieces == 4) beam_scan_kernel<_Float16, 4><<<grid, kThreads, 0, s>>>(p);
-        else beam_scan_kernel<_Float16, 1><<<grid, kThreads, 0, s>>>(p);
-    } else {
-        if (pieces == 8) beam_scan_kernel<float, 8><<<grid, kThreads, 0, s>>>(p);
-        else beam_scan_kernel<float, 2><<<grid, kThreads, 0, s>>>(p);
+    const int64_t rows = a.batch * a.beams, es = (int64_t)elem_bytes(a.dtype);
+    const Cut cut = cut_of(rows, a.vocab);
+    TROCM_REQUIRE(a.workspace && a.workspace_bytes >= bytes_for(rows, cut.parts, a.keep), "beam_select: the workspace must hold %zu bytes", bytes_for(rows, cut.parts, a.keep));
+    TROCM_REQUIRE(kCounters * a.beams * cut.parts < (1ll << 31) && a.beams * cut.parts * a.keep < (1ll << 31), "beam_select: tensor too large");
+    for (int64_t first = 0; first < a.batch; first += kCounters) {
+        const int64_t batch = std::min(a.batch - first, kCounters), row0 = first * a.beams;
+        SelectDev p;
+        p.logits = (const char *)a.logits + row0 * a.row_stride * es, p.row_bytes = a.row_stride * es;
+        p.vocab = (int)a.vocab, p.parts = (int)cut.parts, p.turns = (int)cut.turns, p.keep = (int)a.keep, p.beams = (int)a.beams, p.eos = a.eos;
+        p.counters = (int *)a.workspace;
+        p.part_sum = (double *)((char *)a.workspace + kWsCounterBytes);
+        p.part_best = (Candidate *)(p.part_sum + rows * cut.parts);
+        p.part_max = (float *)(p.part_best + rows * cut.parts * a.keep);
+        p.scores = a.scores + row0, p.ended = a.ended ? a.ended + row0 : nullptr;
+        p.scores_out = a.scores_out + first * a.keep, p.parents = a.parents + first * a.keep, p.tokens = a.tokens + first * a.keep;
+        p.ended_out = a.ended_out ? a.ended_out + first * a.keep : nullptr;
+        p.row0 = (int)row0;
+        p.by_parts = fast_div(cut.parts), p.by_row_candidates = fast_div(cut.parts * a.keep), p.by_beams = fast_div(a.beams);
+        const dim3 grid((unsigned)(batch * a.beams * cut.parts));
+        if (a.dtype == TROCM_F16) {
+            if (cut.pieces == 4) beam_select_kernel<_Float16, 4><<<grid, kThreads, 0, s>>>(p);
+            else beam_select_kernel<_Float16, 1><<<grid, kThreads, 0, s>>>(p);
+        } else {
+            if (cut.pieces == 4) beam_select_kernel<float, 4><<<grid, kThreads, 0, s>>>(p);
+            else beam_select_kernel<float, 1><<<grid, kThreads, 0, s>>>(p);
+        }
+        TROCM_HIP(hipGetLastError());
     }
-    TROCM_HIP(hipGetLastError());
-    if (a.dtype == TROCM_F16) beam_join_kernel<_Float16><<<dim3((unsigned)a.batch), kThreads, 0, s>>>(p);
-    else beam_join_kernel<float><<<dim3((unsigned)a.batch), kThreads, 0, s>>>(p);
-    TROCM_HIP(hipGetLastError());
     return 0;
 }
 

@@ -262,7 +262,7 @@ class BeamSelect:
                 _ints("ended", ended, scores.shape)
             batch, beams, vocab = logits.shape
             need = _beam_bytes(batch, beams, vocab, self.keep)
-            sizes, ws = ((_code(logits.dtype), batch, beams, vocab), (batch, self.keep), need), self._scratch.holding(max(need, 1 << 16), stream)
+            sizes, ws = ((_code(logits.dtype), batch, beams, vocab), (batch, self.keep), need), self._scratch.holding(need, stream)
             self._last = key, sizes, ws
         sizes, shape, need = sizes
         if out is None or (scores_out := out.get("scores")) is None or scores_out.shape != shape or not _same(scores_out.dtype, _F32) or any(
