@@ -6,8 +6,8 @@
 // `keep` largest logits; the last workgroup of a request to arrive puts the parts together in f64.  Where values of two beams are nearer than
 // those sums can be told apart, the beams' sums are made again, exactly.
 //
-// The largest of a wave's values: the K-th largest of its lanes' maxima is found by bisection over the bits of an order-preserving integer
-// (ballots and counts); at least K values reach it, and few more than that, which are listed in LDS and ranked by counting.
+// The largest of a wave's values: the K-th largest of its lanes' maxima is found, nearly, by bisection over the upper bits of an order-preserving
+// integer (ballots and counts); at least K values reach it, and few more than that, which are listed in LDS and ranked by counting.
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
@@ -50,18 +50,17 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cas
 
 __device__ __forceinline__ int lanes_below(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
 
-// The largest t that at least `count` of the wave's keys (one per lane) reach; 0 if there are fewer.  Two bits a step.  Halves as 32 bits have
-// LOW = 13 low bits alike, zeros, or ones in the key of a negative number: left out, and given back as the sign has them.
-template <int LOW>
+// A t that at least `count` of the wave's keys (one per lane) reach, and few more: the largest one of 20 bits and zeros; 0 if there are fewer
+// keys.  Two bits a step.
 __device__ __forceinline__ uint32_t bound_of_lanes(uint32_t key, int count) {
     auto reach = [&](uint32_t t) __attribute__((always_inline)) { return __popcll(__builtin_amdgcn_ballot_w64(key >= t)) >= count; };
     uint32_t t = 0;
 #pragma unroll 1
-    for (int at = 30; at >= LOW - 1 && at >= 0; at -= 2) {
+    for (int at = 30; at >= 12; at -= 2) {
         const bool one = reach(t | 1u << at), two = reach(t | 2u << at), three = reach(t | 3u << at);
         t |= three ? 3u << at : two ? 2u << at : one ? 1u << at : 0u;
     }
-    return t == 0 || t >> 31 ? t : t | ((1u << LOW) - 1);
+    return t;
 }
 
 // A wave's largest value and its sum, everywhere: along the rows of 16 lanes, then over the rows; the last lane has it.
@@ -108,7 +107,7 @@ template <typename T> using Eight = T __attribute__((ext_vector_type(kPiece)));
 
 struct ScanLds {
     int list[kWaves][kWaveList];      // tokens
-    Candidate all[kWaves * kWaveList];
+    uint64_t all[kWaves * kWaveList];   // values' keys above what their tokens lack of 2^32: the order of the choice
     double sum[kWaves];
     float max[kWaves];
     uint32_t bound[kWaves];
@@ -118,7 +117,7 @@ struct ScanLds {
 // A part of a row: `turns` tiles of kThreads * kPiece * C values, the next one in flight while one is looked at.
 template <typename T, int C>
 __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part, ScanLds &lds) {
-    constexpr int kTile = kThreads * kPiece * C, kStep = kThreads * kPiece, LOW = sizeof(T) == 2 ? 13 : 0;
+    constexpr int kTile = kThreads * kPiece * C, kStep = kThreads * kPiece;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const T *from = reinterpret_cast<const T *>(p.logits + row * p.row_bytes);
     const int begin = part * p.turns * kTile, turns = min(p.turns, (p.vocab - begin + kTile - 1) / kTile), mine = begin + tid * kPiece;
@@ -197,7 +196,7 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
         }
         // The values that could be among the best: of the first tile at least `keep` reach its bound (all but -inf is listed where fewer
         // lanes have a value); from then on they do of all.
-        if (turn == 0) bound_key = max(bound_of_lanes<LOW>(key_of(top), p.keep), kLowest), least = value_of(bound_key);
+        if (turn == 0) bound_key = max(bound_of_lanes(key_of(top), p.keep), kLowest), least = value_of(bound_key);
         if (__builtin_amdgcn_ballot_w64(now >= least && now > -INFINITY)) {
             uint32_t hits = 0;   // bit 8 c + e
 #pragma unroll
@@ -205,7 +204,7 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
                 if (__builtin_amdgcn_ballot_w64((float)most[c] >= least)) {
                     asm("" : "+v"(x[c]));   // (halves that are kept as 32 bits from the sum to here would take twice the registers)
 #pragma unroll
-                    for (int e = 0; e < kPiece; e++) hits |= x[c][e] >= (T)least && x[c][e] > (T)-INFINITY ? 1u << (c * kPiece + e) : 0u;
+                    for (int e = 0; e < kPiece; e++) hits |= (float)x[c][e] >= least && (float)x[c][e] > -INFINITY ? 1u << (c * kPiece + e) : 0u;
                 }
             while (const uint64_t in = __builtin_amdgcn_ballot_w64(hits != 0)) {
                 const int b = __ffs(hits) - 1, at = n + lanes_below(in);
@@ -215,7 +214,16 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
             }
         }
     }
-    const uint32_t wave_bound = max(bound_of_lanes<LOW>(key_of(top), p.keep), bound_key);
+    // (the first values of the list are asked for ahead of what does not need them)
+    constexpr int kAhead = 2;
+    int token[kAhead];
+    float value[kAhead];
+#pragma unroll
+    for (int y = 0; y < kAhead; y++) {
+        token[y] = lane + 64 * y < min(n, kWaveList) ? list[lane + 64 * y] : -1;
+        value[y] = token[y] >= 0 ? (float)from[token[y]] : -INFINITY;
+    }
+    const uint32_t wave_bound = max(bound_of_lanes(key_of(top), p.keep), bound_key);
     if (lane == 0) lds.bound[w] = wave_bound;
     if (tid == 0) lds.total = 0;
     if (m < INFINITY) all = against(all, c_m, m);
@@ -275,36 +283,39 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
             n += min(here, p.keep - equal), equal = min(equal + here, p.keep);
         }
         least = -INFINITY;   // (all of the list)
+#pragma unroll
+        for (int y = 0; y < kAhead; y++) {
+            token[y] = lane + 64 * y < n ? list[lane + 64 * y] : -1;
+            value[y] = token[y] >= 0 ? (float)from[token[y]] : -INFINITY;
+        }
     }
 
     // the workgroup's: every listed value counts those before it
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        Candidate c = {-INFINITY, -1};
-        if (j0 + lane < n) {
-            c.token = list[j0 + lane];
-            const float v = (float)from[c.token];
-            c.x = v == v ? v : -INFINITY;
-        }
-        const bool in = c.token >= 0 && c.x >= least;
+    auto add = [&](int t, float v) __attribute__((always_inline)) {
+        const bool in = t >= 0 && !(v < least);   // (NaN: -inf, where that is looked for)
         const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
+        if (!lanes) return;
         int at = 0;
         if (lane == 0) at = atomicAdd(&lds.total, __popcll(lanes));
         at = __builtin_amdgcn_readfirstlane(at) + lanes_below(lanes);
-        if (in) lds.all[at] = c;
+        if (in) lds.all[at] = (uint64_t)key_of(v) << 32 | (uint32_t)~t;
+    };
+#pragma unroll
+    for (int y = 0; y < kAhead; y++) add(token[y], value[y]);
+    for (int j0 = 64 * kAhead; j0 < n; j0 += 64) {
+        const int t = j0 + lane < n ? list[j0 + lane] : -1;
+        add(t, t >= 0 ? (float)from[t] : -INFINITY);
     }
     __syncthreads();
     const int total = lds.total;
     const int64_t at_part = (int64_t)row * p.parts + part;
     Candidate *best = p.part_best + at_part * p.keep;
     for (int j = tid; j < total; j += kThreads) {
-        const Candidate c = lds.all[j];
+        const uint64_t c = lds.all[j];
         int rank = 0;
-#pragma unroll 4
-        for (int z = 0; z < total; z++) {
-            const Candidate d = lds.all[z];
-            rank += d.x > c.x || (d.x == c.x && d.token < c.token);
-        }
-        if (rank < p.keep) put(best + rank, c);
+#pragma unroll 8
+        for (int z = 0; z < total; z++) rank += lds.all[z] > c ? 1 : 0;
+        if (rank < p.keep) put(best + rank, Candidate{value_of((uint32_t)(c >> 32)), (int)~(uint32_t)c});
     }
     for (int j = total + tid; j < p.keep; j += kThreads) put(best + j, Candidate{-INFINITY, -1});
     if (w == 0) {   // (a lane per wave's sum)
@@ -319,7 +330,7 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
 // ---- parts and beams put together: the last workgroup of a request ----------------------------------------------------------
 
 constexpr int kJoinList = 1024;
-struct Choice { double c; int place, beam; };   // place: beam * vocab + token (below 2^31, checked by the host); < 0: none
+struct alignas(16) Choice { double c; int place, beam; };   // place: beam * vocab + token (below 2^31, checked by the host); < 0: none
 
 __device__ __forceinline__ bool before(double c, int place, double d, int other) { return c > d || (c == d && place < other); }
 
@@ -366,7 +377,8 @@ __device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint
 }
 
 struct JoinLds {
-    Choice list[kJoinList];
+    double c[kJoinList];
+    int2 at[kJoinList];   // place, beam
     double lse[kBeamMaxBeams], score[kBeamMaxBeams], err[kBeamMaxBeams], best_c[kWaves];
     uint64_t sums[kWaves];
     float max[kBeamMaxBeams];
@@ -378,52 +390,59 @@ struct JoinLds {
 template <typename T>
 __device__ __forceinline__ void join_request(const SelectDev &p, int request, JoinLds &lds) {
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    const int per_row = p.parts * p.keep, n = p.beams * per_row;
+    const Candidate *all = p.part_best + (int64_t)request * n;
+    constexpr int kHeld = 4;   // candidates that a thread asks for ahead of all, and keeps
+    Candidate first_of[kHeld];
+#pragma unroll
+    for (int y = 0; y < kHeld; y++) first_of[y] = tid + y * kThreads < n ? get(all + tid + y * kThreads) : Candidate{-INFINITY, -1};
     constexpr int kLanes = 16;   // of a beam
     for (int beam = tid / kLanes; beam < p.beams; beam += kThreads / kLanes) {
         const int64_t row = (int64_t)request * p.beams + beam;
         const float *pm = p.part_max + row * p.parts;
         const double *ps = p.part_sum + row * p.parts;
-        const Candidate *first = p.part_best + row * p.parts * p.keep;   // of every part its best
-        float m = -INFINITY, top = -INFINITY, over = 0.0f;               // the largest reference, the largest value, how far one is above its part's reference
-        for (int i = tid % kLanes; i < p.parts; i += kLanes) {
-            const float ref = get(pm + i), most = get(first + i * (int64_t)p.keep).x;
-            m = fmaxf(m, ref), top = fmaxf(top, most), over = fmaxf(over, most - ref);   // (NaN where both are infinite: no number)
-        }
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64)), top = fmaxf(top, __shfl_xor(top, d, 64)), over = fmaxf(over, __shfl_xor(over, d, 64));
+        const Candidate *first = all + beam * per_row;     // of every part its best
+        const float score = p.scores[row];
+        const bool ended = p.ended && p.ended[row] != 0;
+        // (the largest reference, the largest value, how far one is above its part's reference; sums against the largest so far)
+        float m = -INFINITY, top = -INFINITY, over = 0.0f;
         double l = 0.0;
         for (int i = tid % kLanes; i < p.parts; i += kLanes) {
-            const float ref = get(pm + i);
-            l += ref == -INFINITY ? 0.0 : get(ps + i) * exp((double)ref - (double)m);
+            const float ref = get(pm + i), most = get(first + i * (int64_t)p.keep).x;
+            const double sum = get(ps + i);
+            const float was = m;
+            m = fmaxf(m, ref), top = fmaxf(top, most), over = fmaxf(over, most - ref);   // (NaN where both are infinite: no number)
+            l = (was == -INFINITY ? 0.0 : l * exp((double)was - (double)m)) + (ref == -INFINITY ? 0.0 : sum * exp((double)ref - (double)m));
         }
+        const float mine = m;
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64)), top = fmaxf(top, __shfl_xor(top, d, 64)), over = fmaxf(over, __shfl_xor(over, d, 64));
+        l = mine == -INFINITY ? 0.0 : l * exp((double)mine - (double)m);
 #pragma unroll
         for (int d = 1; d < kLanes; d <<= 1) l += __shfl_xor(l, d, 64);
         if (tid % kLanes == 0) {
-            const float score = p.scores[row];
             const bool dead = !(fabsf(score) < INFINITY);
+            const double log_l = log(l);
             lds.score[beam] = dead ? -INFINITY : (double)score;
-            lds.lse[beam] = (double)m + log(l);
+            lds.lse[beam] = (double)m + log_l;
             lds.max[beam] = top;
-            lds.ended[beam] = p.ended && p.ended[row] != 0;
-            lds.kind[beam] = dead ? 2 : lds.ended[beam] ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
+            lds.ended[beam] = ended;
+            lds.kind[beam] = dead ? 2 : ended ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
             // What the sum may be off by, relatively, is what its logarithm is: exponents x - ref by a half step of f32 and a quarter for log2 e,
-            // weighted by the weights at most ln(vocab / l) of them (their entropy is ref - x + ln l on average) and twice what lies above the
+            // weighted by the weights at most ln vocab - ln l of them (their entropy is ref - x + ln l on average) and twice what lies above the
             // reference, which is at most `over` and what a wave's may be below its part's, 2; the exponential's two, a piece's seven additions;
-            // f64 from there on.
-            lds.err[beam] = lds.kind[beam] == 0 ? (1.5 * (fmax(log((double)p.vocab / l), 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 : 0.0;
+            // f64 from there on.  (ln vocab is at most 0.6932 times the bits of it.)
+            lds.err[beam] = lds.kind[beam] == 0 ? (1.5 * (fmax(0.6932 * (32 - __clz(p.vocab)) - log_l, 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 : 0.0;
             lds.again[beam] = 0;
         }
     }
     if (tid == 0) lds.any = 0;
     __syncthreads();
 
-    const int per_row = p.parts * p.keep, n = p.beams * per_row;
-    const Candidate *all = p.part_best + (int64_t)request * n;
-    auto candidate = [&](int j) {
+    auto choice = [&](int j, const Candidate &c) {
         const int beam = p.by_row_candidates.by(j), k = j - beam * per_row;
         Choice r = {-INFINITY, -1, beam};
         if (lds.kind[beam] == 0) {
-            const Candidate c = get(all + j);
             if (c.token >= 0) r.c = lds.score[beam] + ((double)c.x - lds.lse[beam]), r.place = beam * p.vocab + c.token;
         } else if (k < p.keep) {   // the token that an ended beam stays at, and then, as in a beam without values, tokens in their order
             const bool stays = lds.kind[beam] == 1 && k == 0;
@@ -433,6 +452,7 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
         }
         return r;
     };
+    auto candidate = [&](int j) { return choice(j, get(all + j)); };
     auto chosen = [&](int rank, double c, int place, int beam) {
         const int token = place - beam * p.vocab;
         const int64_t at = (int64_t)request * p.keep + rank;
@@ -443,7 +463,6 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
     };
     double err = 0.0;
     for (int beam = 0; beam < p.beams; beam++) err = fmax(err, lds.err[beam]);
-    constexpr int kHeld = 4;   // candidates that a thread keeps from the first look at them to the second
     for (int again = 0;; again++) {
         // at least `keep` of a wave's candidates reach its bound (of f32, whose order is that of f64 but for ties), so the largest bound will
         // do; all that could be among the best are listed
@@ -452,14 +471,14 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
 #pragma unroll
         for (int y = 0; y < kHeld; y++) {
             const int j = tid + y * kThreads;
-            held[y] = j < n ? candidate(j) : Choice{-INFINITY, -1, 0};
+            held[y] = j < n ? choice(j, first_of[y]) : Choice{-INFINITY, -1, 0};
             if (held[y].place >= 0) top = max(top, key_of((float)held[y].c));
         }
         for (int j = tid + kHeld * kThreads; j < n; j += kThreads) {
             const Choice r = candidate(j);
             if (r.place >= 0) top = max(top, key_of((float)r.c));
         }
-        const uint32_t wave_bound = bound_of_lanes<0>(top, p.keep);
+        const uint32_t wave_bound = bound_of_lanes(top, p.keep);
         __syncthreads();   // (what the last turn has listed is done with)
         if (lane == 0) lds.bound[w] = wave_bound;
         if (tid == 0) lds.count = 0;
@@ -473,7 +492,7 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
                 int at = 0;
                 if (lane == 0) at = atomicAdd(&lds.count, __popcll(lanes));
                 at = __builtin_amdgcn_readfirstlane(at) + lanes_below(lanes);
-                if (in && at < kJoinList) lds.list[at] = r;
+                if (in && at < kJoinList) lds.c[at] = r.c, lds.at[at] = make_int2(r.place, r.beam);
             }
         };
 #pragma unroll
@@ -491,22 +510,24 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
             const int j = tid + y * kThreads;
             rank[y] = p.keep;
             if (!whole || j >= listed) continue;
-            const Choice c = lds.list[j];
+            const double c = lds.c[j];
             int r = 0, near = 0;
-#pragma unroll 4
+#pragma unroll 8
             for (int o = 0; o < listed; o++) {
-                const Choice d = lds.list[o];
-                r += before(d.c, d.place, c.c, c.place);
-                near |= d.beam != c.beam && fabs(d.c - c.c) <= 2.0 * err ? 1 : 0;
+                const double d = lds.c[o];
+                r += d > c ? 1 : 0;
+                near += !(fabs(d - c) > 2.0 * err) ? 1 : 0;   // (itself, and two of -inf)
             }
-            rank[y] = r;
-            if (again == 0 && near && r < p.keep) {
+            if (near > 1 && r < p.keep) {
+                const int2 mine = lds.at[j];
                 for (int o = 0; o < listed; o++) {
-                    const Choice d = lds.list[o];
-                    const double off = lds.err[c.beam] + lds.err[d.beam];
-                    if (d.beam != c.beam && off > 0.0 && fabs(d.c - c.c) <= off) lds.again[c.beam] = lds.again[d.beam] = 1, lds.any = 1;
+                    const int2 other = lds.at[o];
+                    const double d = lds.c[o], off = lds.err[mine.y] + lds.err[other.y];
+                    r += d == c && other.x < mine.x ? 1 : 0;
+                    if (again == 0 && other.y != mine.y && off > 0.0 && fabs(d - c) <= off) lds.again[mine.y] = lds.again[other.y] = 1, lds.any = 1;
                 }
             }
+            rank[y] = r;
         }
         if (again == 0) {
             if (!whole) {
@@ -528,8 +549,8 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
 #pragma unroll
             for (int y = 0; y < kMine; y++)
                 if (rank[y] < p.keep) {
-                    const Choice c = lds.list[tid + y * kThreads];
-                    chosen(rank[y], c.c, c.place, c.beam);
+                    const int2 at = lds.at[tid + y * kThreads];
+                    chosen(rank[y], lds.c[tid + y * kThreads], at.x, at.y);
                 }
             return;
         }
