@@ -15,25 +15,37 @@ constexpr int kSumTop = 1 << 30;   // where sums of lengths stay (adding never w
 
 __device__ __forceinline__ int add_up_to_top(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)kSumTop); }   // (both of 0 ..= kSumTop)
 
-// Exclusive prefix sums of a value per thread over the workgroup; `total` is the sum.  All threads.
+// Lane l's value to lane l + n of a row of 16, lane 15's of a row to the next row, lane 31's to the upper half; 0 where none comes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+constexpr int kUp = 0x110, kRow15 = 0x142, kRow31 = 0x143;
+__device__ __forceinline__ int row_sums(int x) {   // of a row's lanes up to this one
+    x = add_up_to_top(x, moved<kUp + 1, 0xf>(x)), x = add_up_to_top(x, moved<kUp + 2, 0xf>(x));
+    x = add_up_to_top(x, moved<kUp + 4, 0xf>(x)), x = add_up_to_top(x, moved<kUp + 8, 0xf>(x));
+    return x;
+}
+__device__ __forceinline__ int wave_sums(int x) {   // of a wave's
+    x = row_sums(x);
+    x = add_up_to_top(x, moved<kRow15, 0xa>(x));
+    return add_up_to_top(x, moved<kRow31, 0xc>(x));
+}
+__device__ __forceinline__ int wave_most(int x) {   // of values that are not negative
+    x = max(x, moved<kUp + 1, 0xf>(x)), x = max(x, moved<kUp + 2, 0xf>(x)), x = max(x, moved<kUp + 4, 0xf>(x)), x = max(x, moved<kUp + 8, 0xf>(x));
+    x = max(x, moved<kRow15, 0xa>(x)), x = max(x, moved<kRow31, 0xc>(x));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Exclusive prefix sums of a value per thread over the workgroup; `total` is the sum.  All threads; lds_waves[16] may be used again after the
+// next barrier.
 __device__ __forceinline__ int block_scan(int x, int *lds_waves, int &total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    int up = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(up, d, 64);
-        if (lane >= d) up = add_up_to_top(up, y);
-    }
-    __syncthreads();   // (lds_waves may still be read from the scan before)
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int up = wave_sums(x);
     if (lane == 63) lds_waves[w] = up;
     __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < waves; i++) {
-        if (i == w) before = total;
-        total = add_up_to_top(total, lds_waves[i]);
-    }
-    const int left = __shfl_up(up, 1, 64);
+    const int sums = row_sums(lane < waves ? lds_waves[lane] : 0);   // (at most 16 waves)
+    total = __builtin_amdgcn_readlane(sums, 15);
+    const int before = w ? __builtin_amdgcn_readlane(sums, w - 1) : 0;
+    const int left = __shfl_up(up, 1, 64);   // (not up - x: sums stop at the top)
     return add_up_to_top(before, lane ? left : 0);
 }
 
@@ -59,67 +71,71 @@ struct PlanDev {
 // Pages of the step and where its tokens go.  Every workgroup makes the prefix sums over the sequences itself (at most four a thread)
 // and takes its share of the tokens and pages, so that no workgroup waits for another.
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanDev p) {
-    __shared__ int s_ends[kPagedMaxSeqs], s_offs[kPagedMaxSeqs + 1], s_waves[kPlanWaves];
-    const int tid = threadIdx.x, page = (int)p.by_page.d;
-    const int per = (p.n_seq + blockDim.x - 1) / blockDim.x, i0 = min(tid * per, p.n_seq), i1 = min(i0 + per, p.n_seq);
+    __shared__ int s_ends[kPagedMaxSeqs], s_offs[kPagedMaxSeqs + 1], s_lens[kPagedMaxSeqs];   // s_lens: -1 of a sequence that is refused
+    __shared__ int s_waves[2][kPlanWaves], s_taken, s_refused;
+    constexpr int kMine = kPagedMaxSeqs / kPlanThreads;
+    const int tid = threadIdx.x, lane = tid & 63, page = (int)p.by_page.d;
+    const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * per, p.n_seq), mine = min(per, p.n_seq - i0);
     const int count = min(max(p.free_count[0], 0), p.n_pages);
-    auto pages_of = [&](int tokens) { return p.by_page.by(tokens + page - 1); };
-    // (tokens + page - 1 stays below 2^31: `most` is at most 2^30 and a page at most 2^20 tokens)
-    auto fits = [&](int len, int add, int end) { return len >= 0 && add >= 0 && len <= p.most && add <= p.most - len && end <= p.n_tokens; };
+    auto pages_of = [&](int tokens) { return p.by_page.by(tokens + page - 1); };   // (below 2^31: `most` is at most 2^30 and a page at most 2^20 tokens)
+    int len[kMine], add[kMine], need[kMine];
+#pragma unroll
+    for (int y = 0; y < kMine; y++) len[y] = y < mine ? p.lens[i0 + y] : 0, add[y] = y < mine ? p.n_new[i0 + y] : 0;
+    if (tid == 0) s_taken = 0, s_refused = 0;
 
-    int sum = 0, total;
-    for (int i = i0; i < i1; i++) sum = add_up_to_top(sum, min(max(p.n_new[i], 0), kSumTop));
-    int at = block_scan(sum, s_waves, total);
+    int sum = 0, total, all_needs;
+#pragma unroll
+    for (int y = 0; y < kMine; y++) sum = add_up_to_top(sum, min(max(add[y], 0), kSumTop));
+    int at = block_scan(sum, s_waves[0], total);
     int needs = 0;
-    const int start = at;
-    for (int i = i0; i < i1; i++) {
-        const int len = p.lens[i], add = p.n_new[i];
-        if (blockIdx.x == 0 && p.starts) p.starts[i] = at;
-        at = add_up_to_top(at, min(max(add, 0), kSumTop));
-        s_ends[i] = at;
-        if (fits(len, add, at)) needs = add_up_to_top(needs, pages_of(len + add) - pages_of(len));
+    uint32_t fits = 0;
+#pragma unroll
+    for (int y = 0; y < kMine; y++) {
+        if (y < mine && blockIdx.x == 0 && p.starts) p.starts[i0 + y] = at;
+        at = add_up_to_top(at, min(max(add[y], 0), kSumTop));
+        if (y < mine) s_ends[i0 + y] = at;
+        const bool fit = y < mine && len[y] >= 0 && add[y] >= 0 && len[y] <= p.most && add[y] <= p.most - len[y] && at <= p.n_tokens;
+        fits |= (fit ? 1u : 0u) << y;
+        need[y] = fit ? pages_of(len[y] + add[y]) - pages_of(len[y]) : 0;
+        needs = add_up_to_top(needs, need[y]);
     }
     if (blockIdx.x == 0 && p.starts && tid == 0) p.starts[p.n_seq] = total;
-    int all_needs;
-    int off = block_scan(needs, s_waves, all_needs);
-    at = start;
-    int refused = 0, taken = 0;
-    for (int i = i0; i < i1; i++) {
-        const int len = p.lens[i], add = p.n_new[i];
-        at = add_up_to_top(at, min(max(add, 0), kSumTop));
-        const bool fit = fits(len, add, at);
-        const int need = fit ? pages_of(len + add) - pages_of(len) : 0;
-        s_offs[i] = off;
-        off = add_up_to_top(off, need);
-        const bool in = fit && (need == 0 || off <= count);
+    int off = block_scan(needs, s_waves[1], all_needs);
+    int refused = 0, taken = 0;   // (what is taken ends where the last sequence that gets pages ends)
+#pragma unroll
+    for (int y = 0; y < kMine; y++) {
+        if (y >= mine) continue;
+        s_offs[i0 + y] = off;
+        off = add_up_to_top(off, need[y]);
+        const bool in = ((fits >> y) & 1) && (need[y] == 0 || off <= count);
         refused += !in;
-        if (in) taken += need;
-        if (blockIdx.x == 0) p.lens_out[i] = in ? len + add : len;
+        if (in && need[y]) taken = off;
+        s_lens[i0 + y] = in ? len[y] : -1;
+        if (blockIdx.x == 0) p.lens_out[i0 + y] = in ? len[y] + add[y] : len[y];
     }
     if (tid == 0) s_offs[p.n_seq] = all_needs;
-    int all_taken, all_refused;
-    block_scan(taken, s_waves, all_taken);
-    block_scan(refused, s_waves, all_refused);   // (and what the threads wrote to LDS can be read)
-    if (blockIdx.x == 0 && tid == 0) p.free_count_out[0] = count - all_taken, p.refused[0] = all_refused;
+    taken = wave_most(taken), refused = __builtin_amdgcn_readlane(wave_sums(refused), 63);
+    if (lane == 0 && taken) atomicMax(&s_taken, taken);
+    if (lane == 0 && refused) atomicAdd(&s_refused, refused);
+    __syncthreads();
+    const int all_taken = s_taken;
+    if (blockIdx.x == 0 && tid == 0) p.free_count_out[0] = count - all_taken, p.refused[0] = s_refused;
 
     // the pages taken, in the sequences' order, from the end of the stack
-    for (int o = blockIdx.x * blockDim.x + tid; o < all_taken; o += gridDim.x * blockDim.x) {
-        const int i = first_above(s_offs, p.n_seq + 1, o) - 1, id = p.free_pages[count - 1 - o];
-        p.table[i * p.table_width + pages_of(p.lens[i]) + o - s_offs[i]] = id;
+    for (int o = blockIdx.x * kPlanThreads + tid; o < all_taken; o += gridDim.x * kPlanThreads) {
+        const int id = p.free_pages[count - 1 - o], i = first_above(s_offs, p.n_seq + 1, o) - 1;
+        p.table[i * p.table_width + pages_of(s_lens[i]) + o - s_offs[i]] = id;
         if (p.refs && (unsigned)id < (unsigned)p.n_pages) p.refs[id] = 1;
     }
     // where the tokens go
-    for (int t = blockIdx.x * blockDim.x + tid; t < p.n_tokens; t += gridDim.x * blockDim.x) {
-        const int i = first_above(s_ends, p.n_seq, t);
+    for (int t = blockIdx.x * kPlanThreads + tid; t < p.n_tokens; t += gridDim.x * kPlanThreads) {
+        const int i = first_above(s_ends, p.n_seq, t), held = i < p.n_seq ? s_lens[i] : -1;
         int slot = -1, pos = -1;
-        if (i < p.n_seq) {
-            const int len = p.lens[i], add = p.n_new[i], need = s_offs[i + 1] - s_offs[i];
-            if (fits(len, add, s_ends[i]) && (need == 0 || s_offs[i + 1] <= count)) {
-                pos = len + t - (s_ends[i] - add);
-                const int pi = p.by_page.by(pos), have = pages_of(len);
-                const int id = pi < have ? p.table[i * p.table_width + pi] : p.free_pages[count - 1 - (s_offs[i] + pi - have)];
-                if ((unsigned)id < (unsigned)p.n_pages) slot = id * page + (pos - pi * page);
-            }
+        if (held >= 0) {
+            pos = held + t - (i ? s_ends[i - 1] : 0);
+            const int pi = p.by_page.by(pos), have = pages_of(held);
+            const int id = pi < have ? p.table[i * p.table_width + pi] : p.free_pages[count - 1 - (s_offs[i] + pi - have)];
+            if ((unsigned)id < (unsigned)p.n_pages) slot = id * page + (pos - pi * page);
         }
         p.slots[t] = slot;
         if (p.positions) p.positions[t] = pos;
@@ -163,18 +179,65 @@ struct ReorderDev {
     int *table_out, *lens_out, *refs_out, *free_pages_out, *free_count_out, *copies, *missing;
     int64_t table_width;
     int n_seq, n_pages, most;
-    FastDiv by_page;
+    FastDiv by_page, by_width;
 };
 
-// What sequence s holds: full pages and the tokens of the partial one (0: none).  Lengths outside of the table hold nothing.
-__device__ __forceinline__ int2 held_pages(const ReorderDev &p, int s) {
-    const int len = p.lens[s];
+// What a sequence of so many tokens holds: full pages and the tokens of the partial one (0: none).  Lengths outside of the table hold nothing.
+__device__ __forceinline__ int2 held_by(const ReorderDev &p, int len) {
     if (len < 0 || len > p.most) return make_int2(0, 0);
     const int full = p.by_page.by(len);
     return make_int2(full, len - full * (int)p.by_page.d);
 }
+__device__ __forceinline__ int2 held_pages(const ReorderDev &p, int s) { return held_by(p, p.lens[s]); }
 
-// First launch.  Workgroup 0: who needs a copy of the partial page and which free page takes it; the others: counts of holders as they were.
+// Who needs a copy of the partial page, and which free page takes it.  All threads of a workgroup of kPlanThreads, which take sequences j0 .. of
+// `mine`; s_first[n_seq] is left with the destination of every sequence's copy (-1: none).
+constexpr int kMine = kPagedMaxSeqs / kPlanThreads;
+struct Begun { int copies, total; bool enough; };   // of this thread, of all
+__device__ __forceinline__ Begun begin_reorder(const ReorderDev &p, int j0, int mine, int count, int *s_first, int *s_lens, int *s_waves) {
+    int from[kMine], partial[kMine];
+    int2 held[kMine];
+#pragma unroll
+    for (int y = 0; y < kMine; y++) {
+        from[y] = y < mine ? p.parents[j0 + y] : -1;
+        if (y < mine) s_first[j0 + y] = p.n_seq, s_lens[j0 + y] = p.lens[j0 + y];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < kMine; y++) {
+        if ((unsigned)from[y] >= (unsigned)p.n_seq) from[y] = -1;
+        if (from[y] >= 0) atomicMin(&s_first[from[y]], j0 + y);
+        held[y] = from[y] >= 0 ? held_by(p, s_lens[from[y]]) : make_int2(0, 0);
+        partial[y] = held[y].y ? p.table[from[y] * p.table_width + held[y].x] : -1;
+    }
+    __syncthreads();
+    Begun r = {0, 0, false};
+    uint32_t copied = 0;   // (bits: with -1 put into partial[y] where there is none, this compiler left the first one as it was)
+#pragma unroll
+    for (int y = 0; y < kMine; y++) {
+        bool need = (unsigned)partial[y] < (unsigned)p.n_pages;
+        if (need) need = !(s_first[from[y]] == j0 + y && p.refs[partial[y]] == 1);
+        copied |= (need ? 1u : 0u) << y;
+    }
+    r.copies = __popc(copied);
+    int at = block_scan(r.copies, s_waves, r.total);
+    r.enough = r.total <= count;
+    if (threadIdx.x == 0) p.missing[0] = r.enough ? 0 : r.total - count;
+#pragma unroll
+    for (int y = 0; y < kMine; y++) {
+        if (y >= mine) continue;
+        int *out = p.copies + 3 * (j0 + y);
+        const bool need = (copied >> y) & 1, go = r.enough && need;
+        const int dst = go ? p.free_pages[count - 1 - at] : -1;
+        at += need;
+        out[0] = go ? partial[y] : -1, out[1] = dst, out[2] = go ? held[y].y : 0;
+        p.lens_out[j0 + y] = !r.enough ? s_lens[j0 + y] : from[y] >= 0 ? s_lens[from[y]] : 0;
+        s_first[j0 + y] = dst;   // (the firsts have been looked at)
+    }
+    return r;
+}
+
+// First launch.  Workgroup 0: the copies; the others: counts of holders as they were.
 __global__ __launch_bounds__(kPlanThreads) void paged_reorder_begin_kernel(ReorderDev p) {
     const int tid = threadIdx.x;
     if (blockIdx.x > 0) {
@@ -182,40 +245,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_reorder_begin_kernel(Reord
         if (x < p.n_pages) p.refs_out[x] = p.refs[x];
         return;
     }
-    __shared__ int s_first[kPagedMaxSeqs], s_waves[kPlanWaves];
-    for (int s = tid; s < p.n_seq; s += kPlanThreads) s_first[s] = p.n_seq;
-    __syncthreads();
-    for (int j = tid; j < p.n_seq; j += kPlanThreads) {
-        const int from = p.parents[j];
-        if ((unsigned)from < (unsigned)p.n_seq) atomicMin(&s_first[from], j);
-    }
-    __syncthreads();
-    const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads, j0 = min(tid * per, p.n_seq), j1 = min(j0 + per, p.n_seq);
-    const int count = min(max(p.free_count[0], 0), p.n_pages);
-    // (partial page, its tokens) where sequence j needs a copy of it, else (-1, 0)
-    auto copied = [&](int j) {
-        const int from = p.parents[j];
-        if ((unsigned)from >= (unsigned)p.n_seq) return make_int2(-1, 0);
-        const int2 held = held_pages(p, from);
-        if (held.y == 0) return make_int2(-1, 0);
-        const int id = p.table[from * p.table_width + held.x];
-        if ((unsigned)id >= (unsigned)p.n_pages || (s_first[from] == j && p.refs[id] == 1)) return make_int2(-1, 0);
-        return make_int2(id, held.y);
-    };
-    int mine = 0, total;
-    for (int j = j0; j < j1; j++) mine += copied(j).x >= 0;
-    int at = block_scan(mine, s_waves, total);
-    const bool enough = total <= count;
-    for (int j = j0; j < j1; j++) {
-        const int2 c = copied(j);
-        int *out = p.copies + 3 * j;
-        const bool go = enough && c.x >= 0;
-        out[0] = go ? c.x : -1, out[1] = go ? p.free_pages[count - 1 - at] : -1, out[2] = go ? c.y : 0;
-        at += c.x >= 0;
-        const int from = p.parents[j];
-        p.lens_out[j] = !enough ? p.lens[j] : (unsigned)from < (unsigned)p.n_seq ? p.lens[from] : 0;
-    }
-    if (tid == 0) p.missing[0] = enough ? 0 : total - count;
+    __shared__ int s_first[kPagedMaxSeqs], s_lens[kPagedMaxSeqs], s_waves[kPlanWaves];
+    const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads, j0 = min(tid * per, p.n_seq);
+    begin_reorder(p, j0, min(per, p.n_seq - j0), min(max(p.free_count[0], 0), p.n_pages), s_first, s_lens, s_waves);
 }
 
 // Second launch, a workgroup per sequence: its new row of the table, and what its old row's pages lose or gain: a holder for every child
@@ -262,34 +294,161 @@ __global__ __launch_bounds__(256) void paged_reorder_tables_kernel(ReorderDev p)
 // Third launch: pages that nobody holds any more go onto the stack, in ascending order behind what is left of it.  A workgroup takes
 // kReclaim pages and counts the freed ones of all others itself, so that none waits for another.
 constexpr int kReclaim = 16 * kPlanThreads;
+struct Reclaim { int left, freed; };   // free pages that are left, and how many come back
+
+// Sixteen consecutive numbers of [0, n) from x0 on, `none` behind the end: whole loads and stores where they are whole, and all of them at once.
+struct Sixteen { int v[16]; };
+__device__ __forceinline__ Sixteen load_sixteen(const int *from, int x0, int n, int none) {
+    Sixteen r;
+    if (x0 <= n - 16) {
+        __builtin_memcpy(&r, from + x0, sizeof(r));
+    } else {
+#pragma unroll
+        for (int x = 0; x < 16; x++) r.v[x] = x0 + x < n ? from[x0 + x] : none;
+    }
+    return r;
+}
+__device__ __forceinline__ void store_sixteen(int *to, int x0, int n, const Sixteen &r) {
+    if (x0 <= n - 16) {
+        __builtin_memcpy(to + x0, &r, sizeof(r));
+    } else {
+#pragma unroll
+        for (int x = 0; x < 16; x++)
+            if (x0 + x < n) to[x0 + x] = r.v[x];
+    }
+}
+
+// was, now: holders of this thread's pages, block * kReclaim + tid * 16 .., free: that part of the stack; `taken`: this thread's share of the
+// copies.  now_of(x0): holders of 16 other pages.  All threads.
+template <typename NowOf>
+__device__ __forceinline__ Reclaim reclaim_pages(const ReorderDev &p, int block, int count, int taken, const Sixteen &was, const Sixteen &now, Sixteen free, NowOf now_of,
+                                                 int *lds_waves, int *lds_sums) {
+    const int tid = threadIdx.x, my0 = block * kReclaim + tid * 16;
+    auto freed_of = [&](const Sixteen &w, const Sixteen &n) {   // a bit for each page that somebody held and nobody does any more
+        uint32_t bits = 0;
+#pragma unroll
+        for (int x = 0; x < 16; x++) bits |= (n.v[x] <= 0 && w.v[x] > 0 ? 1u : 0u) << x;
+        return bits;
+    };
+    const uint32_t mine = freed_of(was, now);
+    int before = 0, others = 0;
+    if (p.n_pages > kReclaim) {
+        if (tid < 2) lds_sums[tid] = 0;
+        __syncthreads();
+        for (int b = 0; b * kReclaim < p.n_pages; b++) {
+            if (b == block) continue;
+            const int x0 = b * kReclaim + tid * 16, n = __popc(freed_of(load_sixteen(p.refs, x0, p.n_pages, 0), now_of(x0)));
+            others += n;
+            if (b < block) before += n;
+        }
+        before = __builtin_amdgcn_readlane(wave_sums(before), 63), others = __builtin_amdgcn_readlane(wave_sums(others), 63);
+        if ((tid & 63) == 0) atomicAdd(&lds_sums[0], before), atomicAdd(&lds_sums[1], others);
+    }
+    // (both sums of a scan in one word: 16 pages a thread, and at most four sequences)
+    int total;
+    const int scan = block_scan(__popc(mine) | taken << 16, lds_waves, total);
+    if (p.n_pages > kReclaim) before = lds_sums[0], others = lds_sums[1];
+    const int left = count - (total >> 16), freed = others + (total & 0xffff);
+    int at = left + before + (scan & 0xffff);
+    for (uint32_t bits = mine; bits; bits &= bits - 1, at++)   // (more free pages than there are pages: counts that were not kept)
+        if (at < p.n_pages) p.free_pages_out[at] = my0 + __ffs(bits) - 1;
+    bool whole = true;
+#pragma unroll
+    for (int x = 0; x < 16; x++) {
+        if (my0 + x >= left + freed) free.v[x] = -1;
+        else if (my0 + x >= left) whole = false;
+    }
+    if (whole) {
+        store_sixteen(p.free_pages_out, my0, p.n_pages, free);
+    } else {
+#pragma unroll
+        for (int x = 0; x < 16; x++)
+            if (my0 + x < p.n_pages && (my0 + x < left || my0 + x >= left + freed)) p.free_pages_out[my0 + x] = free.v[x];
+    }
+    return {left, freed};
+}
+
 __global__ __launch_bounds__(kPlanThreads) void paged_reclaim_kernel(ReorderDev p) {
-    __shared__ int s_waves[kPlanWaves];
-    const int tid = threadIdx.x;
-    int taken = 0, n;
-    for (int j = tid; j < p.n_seq; j += kPlanThreads) taken += p.copies[3 * j] >= 0;
-    block_scan(taken, s_waves, n);
-    const int left = min(max(p.free_count[0], 0), p.n_pages) - n;
-    auto freed = [&](int x) { return x < p.n_pages && p.refs_out[x] <= 0 && p.refs[x] > 0; };
-    int before = 0, all = 0, mine = 0;
-    const int my0 = blockIdx.x * kReclaim + tid * 16;
-    for (int x0 = 0; x0 < p.n_pages; x0 += kReclaim) {
-        int here = 0;
-        for (int x = 0; x < 16; x++) here += freed(x0 + tid * 16 + x);
-        if (x0 < (int)blockIdx.x * kReclaim) before += here;
-        if (x0 == (int)blockIdx.x * kReclaim) mine = here;
-        all += here;
+    __shared__ int s_waves[kPlanWaves], s_sums[2];
+    const int x0 = blockIdx.x * kReclaim + threadIdx.x * 16, count = min(max(p.free_count[0], 0), p.n_pages);
+    const Sixteen was = load_sixteen(p.refs, x0, p.n_pages, 0), now = load_sixteen(p.refs_out, x0, p.n_pages, 0), free = load_sixteen(p.free_pages, x0, p.n_pages, -1);
+    int taken = 0;
+#pragma unroll
+    for (int y = 0; y < kPagedMaxSeqs / kPlanThreads; y++) {
+        const int j = threadIdx.x + y * kPlanThreads;
+        taken += j < p.n_seq && p.copies[3 * j] >= 0;
     }
-    int sum_before, sum_all, unused;
-    block_scan(before, s_waves, sum_before);
-    block_scan(all, s_waves, sum_all);
-    int at = left + sum_before + block_scan(mine, s_waves, unused);
-    for (int x = my0; x < my0 + 16; x++)
-        if (freed(x) && at < p.n_pages) p.free_pages_out[at++] = x;   // (more free pages than there are pages: counts that were not kept)
-    for (int x = blockIdx.x * kReclaim + tid; x < min(p.n_pages, ((int)blockIdx.x + 1) * kReclaim); x += kPlanThreads) {
-        if (x < left) p.free_pages_out[x] = p.free_pages[x];
-        else if (x >= left + sum_all) p.free_pages_out[x] = -1;
+    const Reclaim r = reclaim_pages(p, blockIdx.x, count, taken, was, now, free, [&](int x) { return load_sixteen(p.refs_out, x, p.n_pages, 0); }, s_waves, s_sums);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.free_count_out[0] = min(r.left + r.freed, p.n_pages);
+}
+
+// All of it by one workgroup, with the counts of holders in LDS, where pages and tables are few: three launches and their memory accesses
+// cost more than the one compute unit takes (one | three launches, with the copies that follow: 64 sequences of 46 entries 12.7 | 15.0 to 17.8 us,
+// 128 14.8 | 14.9 to 17.8, 256, in eight layers, 29.2 | 25.7).
+constexpr int kSmallPages = kReclaim, kSmallEntries = 6144;
+__global__ __launch_bounds__(kPlanThreads) void paged_reorder_kernel(ReorderDev p) {
+    __shared__ int s_refs[kSmallPages + kSmallPages / 16], s_first[kPagedMaxSeqs], s_children[kPagedMaxSeqs], s_lens[kPagedMaxSeqs], s_from[kPagedMaxSeqs], s_waves[2][kPlanWaves];
+    auto page_at = [](int x) { return x + (x >> 4); };   // (threads that take 16 pages each are in different banks)
+    const int tid = threadIdx.x, width = (int)p.table_width, per = (p.n_seq + kPlanThreads - 1) / kPlanThreads, j0 = min(tid * per, p.n_seq), mine = min(per, p.n_seq - j0);
+    const Sixteen was = load_sixteen(p.refs, tid * 16, p.n_pages, 0), free = load_sixteen(p.free_pages, tid * 16, p.n_pages, -1);
+    const int count = min(max(p.free_count[0], 0), p.n_pages);
+#pragma unroll
+    for (int y = 0; y < kMine; y++)
+        if (y < mine) {
+            const int from = p.parents[j0 + y];
+            s_from[j0 + y] = (unsigned)from < (unsigned)p.n_seq ? from : -1, s_children[j0 + y] = 0;
+        }
+#pragma unroll
+    for (int x = 0; x < 16; x++)
+        if (tid * 16 + x < p.n_pages) s_refs[page_at(tid * 16 + x)] = was.v[x];
+    const Begun begun = begin_reorder(p, j0, mine, count, s_first, s_lens, s_waves[0]);
+    const bool enough = begun.enough;
+#pragma unroll
+    for (int y = 0; y < kMine; y++)
+        if (y < mine && s_from[j0 + y] >= 0) atomicAdd(&s_children[s_from[j0 + y]], 1);
+    __syncthreads();
+    // the tables, a thread per entry, several entries' loads at once; what old rows' pages lose or gain
+    const FastDiv by_width = p.by_width;
+    constexpr int kDeep = 4;
+    for (int x0 = tid; x0 < p.n_seq * width; x0 += kDeep * kPlanThreads) {
+        int mine_id[kDeep], new_id[kDeep];
+#pragma unroll
+        for (int y = 0; y < kDeep; y++) {
+            const int x = min(x0 + y * kPlanThreads, p.n_seq * width - 1), j = by_width.by(x), src = s_from[j];
+            mine_id[y] = p.table[x];
+            new_id[y] = src >= 0 ? p.table[src * p.table_width + x - j * width] : -1;
+        }
+#pragma unroll
+        for (int y = 0; y < kDeep; y++) {
+            const int x = x0 + y * kPlanThreads;
+            if (x >= p.n_seq * width) continue;
+            const int j = by_width.by(x), pi = x - j * width, src = s_from[j], dst = s_first[j], children = s_children[j], old = mine_id[y];
+            if (!enough) {
+                p.table_out[x] = old;
+                continue;
+            }
+            int2 h = src >= 0 ? held_by(p, s_lens[src]) : make_int2(0, 0);
+            int id = pi < h.x + (h.y > 0) ? new_id[y] : -1;
+            if (h.y && pi == h.x && dst >= 0) {
+                id = dst;
+                if (dst < p.n_pages) atomicAdd(&s_refs[page_at(dst)], 1);
+            }
+            p.table_out[x] = id;
+            h = held_by(p, s_lens[j]);
+            if (pi < h.x + (h.y > 0) && (unsigned)old < (unsigned)p.n_pages) {
+                // (the partial page stays with the first child, if nobody else holds it)
+                const int change = pi < h.x ? children - 1 : children > 0 && p.refs[old] == 1 ? 0 : -1;
+                if (change) atomicAdd(&s_refs[page_at(old)], change);
+            }
+        }
     }
-    if (blockIdx.x == 0 && tid == 0) p.free_count_out[0] = min(left + sum_all, p.n_pages);
+    __syncthreads();
+    Sixteen now;
+#pragma unroll
+    for (int x = 0; x < 16; x++) now.v[x] = tid * 16 + x < p.n_pages ? s_refs[page_at(tid * 16 + x)] : 0;
+    store_sixteen(p.refs_out, tid * 16, p.n_pages, now);
+    const Reclaim r = reclaim_pages(p, 0, count, enough ? begun.copies : 0, was, now, free, [&](int) { return now; }, s_waves[1], nullptr);
+    if (tid == 0) p.free_count_out[0] = min(r.left + r.freed, p.n_pages);
 }
 
 // ---- copies of pages ------------------------------------------------------------------------------------------------------
@@ -302,7 +461,7 @@ struct CopyDev {
     FastDiv by_words_per_row;
 };
 
-// A workgroup per copy, pool and head group.
+// A workgroup per copy and pool: threads side by side along a head's rows, which lie side by side where tokens do, and heads in turn.
 template <typename W>
 __global__ __launch_bounds__(256) void paged_copy_kernel(CopyDev p) {
     const int *c = p.copies + 3 * (int64_t)blockIdx.x;
@@ -313,13 +472,16 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(CopyDev p) {
     char *pool = reinterpret_cast<char *>(reinterpret_cast<Words>(reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr()))[blockIdx.y]);
     const char *src = pool + from * p.page_stride;
     char *dst = pool + to * p.page_stride;
-    const int words_per_head = tokens * p.words_per_row;
-    for (int h = blockIdx.z; h < p.heads; h += gridDim.z)
-        for (int x = threadIdx.x; x < words_per_head; x += 256) {
-            const int r = p.by_words_per_row.by(x), w = x - r * p.words_per_row;
-            const int64_t at = h * p.head_stride + r * p.token_stride + (int64_t)w * (int64_t)sizeof(W);
-            *reinterpret_cast<W *>(dst + at) = *reinterpret_cast<const W *>(src + at);
-        }
+    const int words = tokens * p.words_per_row;   // of a head
+    int wide = 256;                               // threads of a head
+    while (wide > 16 && wide / 2 >= words) wide /= 2;
+    const int h0 = threadIdx.x / wide, step = 256 / wide;
+    for (int x = threadIdx.x % wide; x < words; x += wide) {
+        const int r = p.by_words_per_row.by(x);
+        const int64_t at = r * p.token_stride + (int64_t)(x - r * p.words_per_row) * (int64_t)sizeof(W);
+#pragma unroll 4
+        for (int h = h0; h < p.heads; h += step) *reinterpret_cast<W *>(dst + at + h * p.head_stride) = *reinterpret_cast<const W *>(src + at + h * p.head_stride);
+    }
 }
 
 }  // namespace
@@ -374,6 +536,12 @@ int launch_paged_reorder(const PagedReorderArgs &a, hipStream_t s) {
     p.table_width = a.table_width, p.n_seq = (int)a.n_seq, p.n_pages = (int)a.n_pages;
     p.most = (int)std::min<int64_t>(a.table_width * a.page_size, kSumTop);
     p.by_page = fast_div(a.page_size);
+    p.by_width = fast_div(a.table_width);
+    if (a.n_pages <= kSmallPages && a.n_seq * a.table_width <= kSmallEntries) {
+        paged_reorder_kernel<<<dim3(1), kPlanThreads, 0, s>>>(p);
+        TROCM_HIP(hipGetLastError());
+        return 0;
+    }
     paged_reorder_begin_kernel<<<dim3((unsigned)(1 + (a.n_pages + kPlanThreads - 1) / kPlanThreads)), kPlanThreads, 0, s>>>(p);
     TROCM_HIP(hipGetLastError());
     if (a.n_seq) paged_reorder_tables_kernel<<<dim3((unsigned)a.n_seq), 256, 0, s>>>(p);
@@ -400,7 +568,7 @@ int launch_paged_copy(const PagedCopyArgs &a, hipStream_t s) {
         const int word = word_of(bits);
         p.n_pages = (int)a.n_pages, p.page = (int)a.page_size, p.heads = (int)a.kv_heads, p.words_per_row = (int)(a.D * es / word);
         p.by_words_per_row = fast_div(p.words_per_row);
-        const dim3 grid((unsigned)a.n_copies, (unsigned)n, (unsigned)std::min<int64_t>(a.kv_heads, 64));
+        const dim3 grid((unsigned)a.n_copies, (unsigned)n);
         if (word == 16) paged_copy_kernel<uint4><<<grid, 256, 0, s>>>(p);
         else if (word == 4) paged_copy_kernel<uint32_t><<<grid, 256, 0, s>>>(p);
         else paged_copy_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
