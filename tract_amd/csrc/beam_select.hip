@@ -353,15 +353,12 @@ __device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint
     auto add = [&](float v) { sum += v == v ? (uint64_t)(exp2_scaled(((double)v - (double)m) * 1.4426950408889634, shift) + 0.5) : 0; };
     constexpr int kStep = kThreads * kPiece;
     const int whole = vocab / kPiece * kPiece;
-    Eight<T> coming[2];
-#pragma unroll
-    for (int y = 0; y < 2; y++)
-        if (tid * kPiece + y * kStep < whole) __builtin_memcpy(&coming[y], x + tid * kPiece + y * kStep, sizeof(coming[y]));
+    Eight<T> coming;
+    if (tid * kPiece < whole) __builtin_memcpy(&coming, x + tid * kPiece, sizeof(coming));
 #pragma unroll 1
     for (int i = tid * kPiece; i < whole; i += kStep) {
-        const Eight<T> now = coming[0];
-        coming[0] = coming[1];
-        if (i + 2 * kStep < whole) __builtin_memcpy(&coming[1], x + i + 2 * kStep, sizeof(coming[1]));
+        const Eight<T> now = coming;
+        if (i + kStep < whole) __builtin_memcpy(&coming, x + i + kStep, sizeof(coming));
 #pragma unroll
         for (int e = 0; e < kPiece; e++) add((float)now[e]);
     }
@@ -388,11 +385,12 @@ struct JoinLds {
 };
 
 template <typename T>
-__device__ __forceinline__ void join_request(const SelectDev &p, int request, JoinLds &lds) {
+__device__ __forceinline__ void join_request(const __attribute__((address_space(4))) SelectDev &p, int request, JoinLds &lds) {
+    const FastDiv by_row_candidates = {p.by_row_candidates.d, p.by_row_candidates.mul, p.by_row_candidates.shift};
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int per_row = p.parts * p.keep, n = p.beams * per_row;
     const Candidate *all = p.part_best + (int64_t)request * n;
-    constexpr int kHeld = 4;   // candidates that a thread asks for ahead of all, and keeps
+    constexpr int kHeld = 2;   // candidates that a thread asks for ahead of all, and keeps
     Candidate first_of[kHeld];
 #pragma unroll
     for (int y = 0; y < kHeld; y++) first_of[y] = tid + y * kThreads < n ? get(all + tid + y * kThreads) : Candidate{-INFINITY, -1};
@@ -440,7 +438,7 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
     __syncthreads();
 
     auto choice = [&](int j, const Candidate &c) {
-        const int beam = p.by_row_candidates.by(j), k = j - beam * per_row;
+        const int beam = by_row_candidates.by(j), k = j - beam * per_row;
         Choice r = {-INFINITY, -1, beam};
         if (lds.kind[beam] == 0) {
             if (c.token >= 0) r.c = lds.score[beam] + ((double)c.x - lds.lse[beam]), r.place = beam * p.vocab + c.token;
@@ -582,6 +580,15 @@ __device__ __forceinline__ void join_request(const SelectDev &p, int request, Jo
     }
 }
 
+// A kernel's one argument where it lies, as loads from here on: kept from the beginning, what only the end looks at would leave too few scalar
+// registers for what is between.
+template <typename Args>
+__device__ __forceinline__ const __attribute__((address_space(4))) Args &arguments_again() {
+    auto at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(at));
+    return *reinterpret_cast<const __attribute__((address_space(4))) Args *>(at);
+}
+
 template <typename T, int C>
 __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
     __shared__ union Lds { ScanLds scan; JoinLds join; __device__ Lds() {} } lds;
@@ -595,7 +602,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
         if (s_last) __hip_atomic_store(p.counters + request, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (s_last) join_request<T>(p, request, lds.join);
+    if (s_last) join_request<T>(arguments_again<SelectDev>(), request, lds.join);
 }
 
 // How rows are cut into parts: tiles of 4 pieces of 8 values a thread, or of 1 where that leaves compute units without a workgroup; and as many

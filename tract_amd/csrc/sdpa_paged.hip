@@ -150,14 +150,27 @@ __device__ __forceinline__ float less(float a, float b) {
     return a - b;
 }
 
+// A kernel's one argument where it lies, as loads from here on: kept from the beginning, what only some places look at would leave the loop too
+// few scalar registers.
+typedef const __attribute__((address_space(4))) PagedDev &Arguments;
+__device__ __forceinline__ Arguments arguments_again() {
+    auto at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(at));
+    return *reinterpret_cast<const __attribute__((address_space(4))) PagedDev *>(at);
+}
+__device__ __forceinline__ int divided(const __attribute__((address_space(4))) FastDiv &by, int n) { return FastDiv{by.d, by.mul, by.shift}.by(n); }
+
 // Where row r of a kv head lies among the q and output rows, and which query it is.
 struct RowPlace { int64_t at; int i; };
-__device__ __forceinline__ RowPlace q_row(const PagedDev &p, int b, int kvh, int r) {
-    const int i = p.by_g.by(r);
+__device__ __forceinline__ RowPlace q_row(Arguments p, int b, int kvh, int r) {
+    const int i = divided(p.by_g, r);
     return {((int64_t)b * p.Hq + kvh * p.G + r - i * p.G) * p.Sq + i, i};
 }
 
 constexpr int kLinePart(int D) { return kRows * D + 2 * kRows; }   // floats of a part: rows of O, their maxima, their sums
+
+constexpr int in_lds(int es, int D) { return es == 4 && D == 128 ? kRows * D * es : 0; }   // bytes of queries
+constexpr int line_lds(int es, int D) { return kWaves * kTile * (es == 2 ? 2 * D + 24 : D + 4) * es + in_lds(es, D); }
 
 // Tiles [first, end) of a unit; `part`: where its partial rows go (NULL: it is the whole unit, rows go to the output).
 struct Stretch {
@@ -166,7 +179,7 @@ struct Stretch {
 };
 
 template <typename T, int D, bool ONCE>
-__device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u, unsigned char *lds) {
+__device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *lds) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int DB = D / 16;                    // feature blocks of the output
     constexpr int KROW = D + 8, VROW = H16 ? D + 16 : D + 4;   // elements per row in LDS: rows of a read in different banks
@@ -178,23 +191,26 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
     static_assert(kWaves * kRows * CROW * 4 + kWaves * 2 * kRows * 4 <= kWaves * PRIV, "waves are joined where the tiles were");
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane / 16, lr = lane % 16;
+    Arguments p = arguments_again();
     const RowPlace place = q_row(p, u.b, u.kvh, u.row0 + min(lr, u.rows - 1));
     const int lim = p.causal ? min(u.len - 1, u.len - p.Sq + place.i) : u.len - 1;
     const int last_key = u.len - 1;
     const char *kb = p.k + u.kvh * p.stride_h, *vb = p.v + u.kvh * p.stride_h;
-    const int *pages = p.table + u.b * p.table_width;
     const uint32_t st = (uint32_t)p.stride_t;     // (below 2^27: checked by the host)
+    const float to_log2 = p.scale * kLog2e;
     const int n_mine = (u.end - u.first - w + kWaves - 1) / kWaves;   // this wave takes every fourth tile
 
     // Where the halves of 32 of this wave's tiles lie: lane 2 i + h has tile i's half h, as bytes from the pool's beginning (-1: a hole, or
     // behind the last key).
     auto ask_pages = [&](int i0) __attribute__((always_inline)) {
+        Arguments p = arguments_again();
         const int key = (u.first + w + kWaves * (i0 + (lane >> 1))) * kTile + 16 * (lane & 1);
-        return key <= last_key && i0 + (lane >> 1) < n_mine ? pages[p.by_page.by(key)] : -1;
+        return key <= last_key && i0 + (lane >> 1) < n_mine ? p.table[u.b * p.table_width + divided(p.by_page, key)] : -1;
     };
     auto bytes_at = [&](int id, int i0) __attribute__((always_inline)) {
+        Arguments p = arguments_again();
         const int key = (u.first + w + kWaves * (i0 + (lane >> 1))) * kTile + 16 * (lane & 1);
-        const int in_page = key - p.by_page.by(key) * (int)p.by_page.d;
+        const int in_page = key - divided(p.by_page, key) * (int)p.by_page.d;
         return (unsigned)id < (unsigned)p.n_pages ? id * p.stride_page + (int64_t)in_page * p.stride_t : (int64_t)-1;
     };
     int64_t at = -1;
@@ -208,7 +224,8 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
     T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: f16)
     const int kr = lane / LPRW, ch = lane % LPRW;
     u32x4 kpre[NK], vpre[NI];
-    struct Halves { int64_t at[2]; } now, next;   // of the tile whose rows are in flight
+    struct Halves { int64_t at[2]; };   // (of the tile whose rows are in flight)
+    int there = 0, there_next = 0;      // bits: which halves are
     auto halves_of = [&](int i) __attribute__((always_inline)) {
         Halves r;
 #pragma unroll
@@ -223,8 +240,7 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
     auto rows_of = [&](int i, const Halves &x, int h) __attribute__((always_inline)) {   // the last row of a half that may be read
         const int most = last_key - (u.first + w + kWaves * i) * kTile;
         if (x.at[0] < 0 && x.at[1] < 0) return 0;
-        const int there = x.at[h] >= 0 ? h : 1 - h;
-        return min(most - 16 * there, 15);
+        return min(most - 16 * (x.at[h] >= 0 ? h : 1 - h), 15);
     };
     auto prefetch_k = [&](int i, const Halves &x) __attribute__((always_inline)) {
         if constexpr (H16) {
@@ -250,7 +266,6 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
             vpre[j] = load16<ONCE>(vb + row_base(x, h), (uint32_t)min(j * RPI % 16 + kr, rows_of(i, x, h)) * st + ch * 16);
         }
     };
-    const float to_log2 = p.scale * kLog2e;
     // key of score x of this lane, from the tile's first: two groups of four consecutive ones
     auto key_of = [](int x) { return 16 * (x >> 2) + (x & 3); };   // + 4 grp
 
@@ -258,20 +273,30 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
         const int ids = ask_pages(0);
         ids_next = ask_pages(32);
         at = bytes_at(ids, 0);
-        now = halves_of(0);
-        prefetch_k(0, now), prefetch_v(0, now);
+        const Halves first = halves_of(0);
+        there = (first.at[0] >= 0) + 2 * (first.at[1] >= 0);
+        prefetch_k(0, first), prefetch_v(0, first);
     }
-    u32x4 qf[KS];
+    // queries: in registers, or, where those are all taken, in LDS
+    constexpr bool QL = in_lds(sizeof(T), D) > 0;
+    u32x4 qf[QL ? 1 : KS], *lds_q = reinterpret_cast<u32x4 *>(lds + kWaves * PRIV);
+    if constexpr (QL) {
+        for (int ks = w; ks < KS; ks += kWaves) lds_q[ks * 64 + lane] = load16<false>(p.q + place.at * (D * (int)sizeof(T)), ks * 64 + grp * 16);
+        __syncthreads();
+    } else {
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) qf[ks] = load16<false>(p.q + place.at * (D * (int)sizeof(T)), ks * 64 + grp * 16);
+        for (int ks = 0; ks < KS; ks++) qf[ks] = load16<false>(p.q + place.at * (D * (int)sizeof(T)), ks * 64 + grp * 16);
+    }
     for (int i = 0; i < n_mine; i++) {
         const int k_lo = (u.first + w + kWaves * i) * kTile;
         const bool more = i + 1 < n_mine;
+        Halves next = {-1, -1};
         if (more) {
             if (((i + 1) & 31) == 0) at = bytes_at(ids_next, i + 1), ids_next = ask_pages(i + 33);
             next = halves_of(i + 1);
+            there_next = (next.at[0] >= 0) + 2 * (next.at[1] >= 0);
         }
-        const bool odd = now.at[0] < 0 || now.at[1] < 0 || k_lo + kTile > u.len;   // a hole, or the last key inside
+        const bool odd = there != 3 || k_lo + kTile > u.len;   // a hole, or the last key inside
 
         // ---- S^T = K Q^T --------------------------------------------------------------------------------------
         float4_t acc[2];
@@ -291,13 +316,15 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
                 }
         } else {
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
+            for (int ks = 0; ks < KS; ks++) {
+                const float4_t c = __builtin_bit_cast(float4_t, QL ? lds_q[ks * 64 + lane] : qf[QL ? 0 : ks]);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {   // (one feature of each group's four at a time)
-                    const float4_t a = __builtin_bit_cast(float4_t, kpre[h * KS + ks]), c = __builtin_bit_cast(float4_t, qf[ks]);
+                    const float4_t a = __builtin_bit_cast(float4_t, kpre[h * KS + ks]);
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[h], 0, 0, 0);
                 }
+            }
             if (more) prefetch_k(i + 1, next);
         }
         float s[8];
@@ -307,7 +334,7 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
 #pragma unroll
             for (int j = 0; j < NI; j++) {
                 const int r = j * RPI + kr;
-                if (now.at[j * RPI / 16] < 0 || k_lo + r > last_key) vpre[j] = u32x4{0, 0, 0, 0};
+                if (!((there >> (j * RPI / 16)) & 1) || k_lo + r > last_key) vpre[j] = u32x4{0, 0, 0, 0};
             }
         }
 #pragma unroll
@@ -318,7 +345,7 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
         const int last = lim - k_lo - 4 * grp;
         if (odd || __builtin_amdgcn_ballot_w64(last < 28) != 0) {
 #pragma unroll
-            for (int x = 0; x < 8; x++) s[x] = key_of(x) <= last && now.at[x >> 2] >= 0 ? s[x] : -INFINITY;
+            for (int x = 0; x < 8; x++) s[x] = key_of(x) <= last && ((there >> (x >> 2)) & 1) ? s[x] : -INFINITY;
         }
         float top = s[0];
 #pragma unroll
@@ -367,7 +394,7 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
                 for (int db = 0; db < DB; db++) o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(lds_v[(key_of(x) + 4 * grp) * VROW + 16 * db + lr], s[x], o[db], 0, 0, 0);
         }
         wave_sync();   // (the next tile goes where this one was)
-        now = next;
+        there = there_next;
     }
 
     // ---- the four waves' results joined ------------------------------------------------------------------------
@@ -391,6 +418,7 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
             f[x] = __builtin_amdgcn_exp2f(comb_ml[x * 2 * kRows + row] - ref);
             l += f[x] * comb_ml[(x * 2 + 1) * kRows + row];
         }
+        Arguments p = arguments_again();
         const int64_t orow = q_row(p, u.b, u.kvh, u.row0 + row).at;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -419,7 +447,7 @@ __device__ __forceinline__ void stretch_body(const PagedDev &p, const Stretch &u
 // The parts of a unit -> its output.  Part x of [0, n) is at part_of(x).  Sixteen lanes take a row; where there are few rows, several groups
 // of lanes share a row's parts and are joined through LDS.
 template <typename T, int D, typename PartOf>
-__device__ __forceinline__ void join_unit(const PagedDev &p, const Stretch &u, int n, PartOf part_of, unsigned char *lds) {
+__device__ __forceinline__ void join_unit(const Stretch &u, int n, PartOf part_of, unsigned char *lds) {
     constexpr int PER = D / 16, BATCH = 4, CROW = D + 4;
     const int tid = threadIdx.x, t = tid % 16, who = tid / 16;
     int live = 1;
@@ -480,6 +508,7 @@ __device__ __forceinline__ void join_unit(const PagedDev &p, const Stretch &u, i
             }
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        Arguments p = arguments_again();
         T *out = reinterpret_cast<T *>(p.out) + q_row(p, u.b, u.kvh, u.row0 + who).at * D;
 #pragma unroll
         for (int e = 0; e < PER / 2; e++) {
@@ -491,67 +520,92 @@ __device__ __forceinline__ void join_unit(const PagedDev &p, const Stretch &u, i
     __syncthreads();
 }
 
-constexpr int line_lds(int es, int D) { return kWaves * kTile * (es == 2 ? 2 * D + 24 : D + 4) * es; }
-constexpr int kLeast = 8;   // tiles of a stretch at least: two a wave
+constexpr int kLeast = 4;   // tiles of a stretch at least: one a wave (8: 10.4 for 9.9 us of one token behind 777, 16: 12.6)
+
+// Whether a sequence begins with its neighbour's page, as beams of a request do.  Pages that one workgroup reads go past the caches (64 sequences
+// of 64 to 8192 keys 195 us, through them 217; 8 x 1000 13.0 | 13.5), those that several do through them (32 requests of 8 beams over 700 common
+// keys 64 us, past them 86; 8 of 8 over 4000 67 | 76).
+__device__ __forceinline__ bool shares_pages(Arguments p, int b) {
+    if (p.table_width == 0) return false;
+    const int mine = p.table[b * p.table_width], left = p.table[max(b - 1, 0) * p.table_width], right = p.table[min(b + 1, p.B - 1) * p.table_width];
+    return (b > 0 && left == mine) || (b + 1 < p.B && right == mine);
+}
+
+// A wave-uniform value out of LDS.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)((uint64_t)(uint32_t)uniform((int)(uint64_t)x) | (uint64_t)(uint32_t)uniform((int)((uint64_t)x >> 32)) << 32); }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev p) {
+__global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
-    __shared__ int64_t s_sums[kWaves], s_start;
-    __shared__ int s_b, s_last;
+    __shared__ int64_t s_sums[kWaves];
+    // (what is looked at between stretches alone is in LDS: the loop needs the scalar registers)
+    __shared__ struct { int64_t per, at, end; int b, unit, len, tiles, first, once; } s_line;
+    __shared__ int s_last;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-    const int units = p.Hkv * p.row_tiles;   // of a sequence
-    auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
-    auto tiles_of = [&](int b) { return b < p.B ? max((len_of(b) + kTile - 1) / kTile, 1) : 0; };   // (one for nothing: its rows are zeros)
+    {
+        Arguments p = arguments_again();
+        const int units = p.Hkv * p.row_tiles;   // of a sequence
+        auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
+        auto tiles_of = [&](int b) { return b < p.B ? max((len_of(b) + kTile - 1) / kTile, 1) : 0; };   // (one for nothing: its rows are zeros)
 
-    // the line's length, and this workgroup's stretch
-    int64_t sum = 0;
-    for (int b = tid; b < p.B; b += kThreads) sum += tiles_of(b);
+        // the line's length, and this workgroup's stretch
+        int64_t sum = 0;
+        bool shares = tid < p.B && shares_pages(p, tid);
+        for (int b = tid; b < p.B; b += kThreads) sum += tiles_of(b);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((long long)sum, d, 64);
-    if (lane == 0) s_sums[w] = sum;
-    __syncthreads();
-    const int64_t total = (s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3]) * units;
-    const int64_t per = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, kLeast);
-    const int64_t begin = blockIdx.x * per, end = std::min<int64_t>(begin + per, total);
-    if (begin >= end) return;
-    // the sequence where it begins
-    int64_t carry = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-        const int b = b0 + tid, mine = tiles_of(b);
-        int64_t up = mine;
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((long long)sum, d, 64);
+        if (lane == 0) s_sums[w] = sum;
+        __syncthreads();
+        const int64_t total = (s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3]) * units;
+        const int64_t per = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, kLeast);
+        const int64_t begin = blockIdx.x * per, end = std::min<int64_t>(begin + per, total);
+        if (begin >= end) return;
+        // the sequence where it begins
+        int64_t carry = 0;
+        for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+            const int b = b0 + tid, mine = tiles_of(b);
+            if (b0 > 0) shares = b < p.B && shares_pages(p, b);
+            int64_t up = mine;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t y = __shfl_up((long long)up, d, 64);
-            if (lane >= d) up += y;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int64_t y = __shfl_up((long long)up, d, 64);
+                if (lane >= d) up += y;
+            }
+            __syncthreads();
+            if (lane == 63) s_sums[w] = up;
+            __syncthreads();
+            int64_t before = carry;
+            for (int x = 0; x < w; x++) before += s_sums[x];
+            const int64_t from = (before + up - mine) * units;
+            if (b < p.B && from <= begin && begin < from + (int64_t)mine * units) {
+                s_line.b = b, s_line.len = len_of(b), s_line.tiles = mine;
+                s_line.unit = (int)((begin - from) / mine), s_line.first = (int)((begin - from) % mine);
+                s_line.once = p.row_tiles == 1 && !shares;
+            }
+            carry += s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3];
+            if (carry * units > begin) break;
         }
+        if (tid == 0) s_line.per = per, s_line.at = begin, s_line.end = end;
         __syncthreads();
-        if (lane == 63) s_sums[w] = up;
-        __syncthreads();
-        int64_t before = carry;
-        for (int x = 0; x < w; x++) before += s_sums[x];
-        const int64_t from = (before + up - mine) * units;
-        if (b < p.B && from <= begin && begin < from + (int64_t)mine * units) s_b = b, s_start = from;
-        carry += s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3];
-        if (carry * units > begin) break;
     }
-    __syncthreads();
-
-    Stretch u;
-    u.b = s_b, u.len = len_of(u.b);
-    int tiles = tiles_of(u.b);
-    int unit = (int)((begin - s_start) / tiles);
-    u.first = (int)(begin - s_start - (int64_t)unit * tiles);
-    for (int64_t t = begin; t < end;) {
-        u.kvh = p.by_row_tiles.by(unit);
-        u.row0 = (unit - u.kvh * p.row_tiles) * kRows, u.rows = min(kRows, p.Sq * p.G - u.row0);
-        u.end = (int)std::min<int64_t>(tiles, u.first + (end - t));
-        const bool whole = u.first == 0 && u.end == tiles;
-        u.part = whole ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * kLinePart(D);
-        stretch_body<T, D, false>(p, u, lds);
-        if (!whole) {
-            const int64_t unit_at = t - u.first;
-            const int first = (int)(unit_at / per), n = (int)((unit_at + tiles - 1) / per) - first + 1;
+    for (;;) {
+        Stretch u;
+        {
+            Arguments p = arguments_again();
+            const int unit = uniform(s_line.unit), tiles = uniform(s_line.tiles);
+            u.b = uniform(s_line.b), u.len = uniform(s_line.len), u.first = uniform(s_line.first);
+            u.kvh = divided(p.by_row_tiles, unit);
+            u.row0 = (unit - u.kvh * p.row_tiles) * kRows, u.rows = min(kRows, p.Sq * p.G - u.row0);
+            u.end = (int)std::min<int64_t>(tiles, u.first + uniform(s_line.end) - uniform(s_line.at));
+            u.part = u.first == 0 && u.end == tiles ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * kLinePart(D);
+        }
+        if (uniform(s_line.once)) stretch_body<T, D, true>(u, lds);
+        else stretch_body<T, D, false>(u, lds);
+        if (u.part) {
+            Arguments p = arguments_again();
+            const int64_t per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
+            const int first = (int)(unit_at / per), n = (int)((unit_at + uniform(s_line.tiles) - 1) / per) - first + 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
             __syncthreads();                                     // ... and so have the whole workgroup's
             if (tid == 0) {
@@ -560,11 +614,21 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev p) {
                 if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
-            if (s_last) join_unit<T, D>(p, u, n, [&](int x) { return p.parts + (2 * (int64_t)(first + x) + (x == 0)) * kLinePart(D); }, lds);
+            float *parts = p.parts;
+            if (s_last) join_unit<T, D>(u, n, [&](int x) { return parts + (2 * (int64_t)(first + x) + (x == 0)) * kLinePart(D); }, lds);
         }
-        t += u.end - u.first;
-        u.first = 0;
-        if (++unit == units && t < end) unit = 0, u.b++, u.len = len_of(u.b), tiles = tiles_of(u.b);
+        __syncthreads();   // (everybody has read where the line stands)
+        if (tid == 0) {
+            Arguments p = arguments_again();
+            s_line.at += u.end - u.first, s_line.first = 0;
+            if (++s_line.unit == p.Hkv * p.row_tiles && s_line.at < s_line.end) {
+                const int len = min(max(p.lens[u.b + 1], 0), p.most);
+                s_line.once = p.row_tiles == 1 && !shares_pages(p, u.b + 1);
+                s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.tiles = max((len + kTile - 1) / kTile, 1);
+            }
+        }
+        __syncthreads();
+        if (s_line.at >= s_line.end) return;
     }
 }
 
