@@ -40,7 +40,7 @@ struct PagedDev {
     int row_tiles;              // of a kv head
     int *counters;
     float *parts;
-    FastDiv by_g, by_row_tiles;
+    FastDiv by_g, by_row_tiles, by_workgroups;
 };
 
 __device__ __forceinline__ float widen(float x) { return x; }
@@ -533,58 +533,62 @@ __device__ __forceinline__ bool shares_pages(Arguments p, int b) {
 
 // A wave-uniform value out of LDS.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)((uint64_t)(uint32_t)uniform((int)(uint64_t)x) | (uint64_t)(uint32_t)uniform((int)((uint64_t)x >> 32)) << 32); }
+
+// Sums of a wave's lanes up to each one: along the rows of 16 lanes, then over the rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_sums(int x) {
+    constexpr int kUp = 0x110, kRow15 = 0x142, kRow31 = 0x143;
+    x += moved<kUp + 1, 0xf>(x), x += moved<kUp + 2, 0xf>(x), x += moved<kUp + 4, 0xf>(x), x += moved<kUp + 8, 0xf>(x);
+    x += moved<kRow15, 0xa>(x), x += moved<kRow31, 0xc>(x);
+    return x;
+}
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
-    __shared__ int64_t s_sums[kWaves];
+    __shared__ int s_sums[kWaves], s_totals[kWaves];
     // (what is looked at between stretches alone is in LDS: the loop needs the scalar registers)
-    __shared__ struct { int64_t per, at, end; int b, unit, len, tiles, first, once; } s_line;
+    __shared__ struct { int per, at, end, b, unit, len, tiles, first, once; } s_line;
     __shared__ int s_last;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     {
         Arguments p = arguments_again();
         const int units = p.Hkv * p.row_tiles;   // of a sequence
         auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
-        auto tiles_of = [&](int b) { return b < p.B ? max((len_of(b) + kTile - 1) / kTile, 1) : 0; };   // (one for nothing: its rows are zeros)
+        auto tiles_of = [&](int len) { return max((len + kTile - 1) / kTile, 1); };   // (one for nothing: its rows are zeros)
 
-        // the line's length, and this workgroup's stretch
-        int64_t sum = 0;
+        // the line's length (below 2^30: checked by the host), and this workgroup's stretch
+        int len = tid < p.B ? len_of(tid) : 0, mine = tid < p.B ? tiles_of(len) : 0, all = mine;
         bool shares = tid < p.B && shares_pages(p, tid);
-        for (int b = tid; b < p.B; b += kThreads) sum += tiles_of(b);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor((long long)sum, d, 64);
-        if (lane == 0) s_sums[w] = sum;
+        for (int b = tid + kThreads; b < p.B; b += kThreads) all += tiles_of(len_of(b));
+        int up = wave_sums(mine);
+        const int sum = p.B > kThreads ? wave_sums(all) : up;
+        if (lane == 63) s_sums[w] = up, s_totals[w] = sum;
         __syncthreads();
-        const int64_t total = (s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3]) * units;
-        const int64_t per = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, kLeast);
-        const int64_t begin = blockIdx.x * per, end = std::min<int64_t>(begin + per, total);
+        const int total = (s_totals[0] + s_totals[1] + s_totals[2] + s_totals[3]) * units;
+        const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), kLeast);
+        const int begin = blockIdx.x * per, end = min(begin + per, total);
         if (begin >= end) return;
         // the sequence where it begins
-        int64_t carry = 0;
-        for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-            const int b = b0 + tid, mine = tiles_of(b);
-            if (b0 > 0) shares = b < p.B && shares_pages(p, b);
-            int64_t up = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int64_t y = __shfl_up((long long)up, d, 64);
-                if (lane >= d) up += y;
-            }
-            __syncthreads();
-            if (lane == 63) s_sums[w] = up;
-            __syncthreads();
-            int64_t before = carry;
+        for (int b0 = 0, carry = 0;;) {
+            int before = carry;
             for (int x = 0; x < w; x++) before += s_sums[x];
-            const int64_t from = (before + up - mine) * units;
-            if (b < p.B && from <= begin && begin < from + (int64_t)mine * units) {
-                s_line.b = b, s_line.len = len_of(b), s_line.tiles = mine;
-                s_line.unit = (int)((begin - from) / mine), s_line.first = (int)((begin - from) % mine);
+            const int from = (before + up - mine) * units;
+            if (b0 + tid < p.B && from <= begin && begin < from + mine * units) {
+                s_line.b = b0 + tid, s_line.len = len, s_line.tiles = mine;
+                s_line.unit = (unsigned)(begin - from) / (unsigned)mine, s_line.first = (unsigned)(begin - from) % (unsigned)mine;
                 s_line.once = p.row_tiles == 1 && !shares;
             }
             carry += s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3];
-            if (carry * units > begin) break;
+            b0 += kThreads;
+            if (b0 >= p.B || carry * units > begin) break;
+            len = b0 + tid < p.B ? len_of(b0 + tid) : 0, mine = b0 + tid < p.B ? tiles_of(len) : 0;
+            shares = b0 + tid < p.B && shares_pages(p, b0 + tid);
+            up = wave_sums(mine);
+            __syncthreads();
+            if (lane == 63) s_sums[w] = up;
+            __syncthreads();
         }
         if (tid == 0) s_line.per = per, s_line.at = begin, s_line.end = end;
         __syncthreads();
@@ -597,14 +601,14 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             u.b = uniform(s_line.b), u.len = uniform(s_line.len), u.first = uniform(s_line.first);
             u.kvh = divided(p.by_row_tiles, unit);
             u.row0 = (unit - u.kvh * p.row_tiles) * kRows, u.rows = min(kRows, p.Sq * p.G - u.row0);
-            u.end = (int)std::min<int64_t>(tiles, u.first + uniform(s_line.end) - uniform(s_line.at));
+            u.end = min(tiles, u.first + uniform(s_line.end) - uniform(s_line.at));
             u.part = u.first == 0 && u.end == tiles ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * kLinePart(D);
         }
         if (uniform(s_line.once)) stretch_body<T, D, true>(u, lds);
         else stretch_body<T, D, false>(u, lds);
         if (u.part) {
             Arguments p = arguments_again();
-            const int64_t per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
+            const unsigned per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
             const int first = (int)(unit_at / per), n = (int)((unit_at + uniform(s_line.tiles) - 1) / per) - first + 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
             __syncthreads();                                     // ... and so have the whole workgroup's
@@ -617,18 +621,18 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             float *parts = p.parts;
             if (s_last) join_unit<T, D>(u, n, [&](int x) { return parts + (2 * (int64_t)(first + x) + (x == 0)) * kLinePart(D); }, lds);
         }
+        if (uniform(s_line.at) + u.end - u.first >= uniform(s_line.end)) return;
         __syncthreads();   // (everybody has read where the line stands)
         if (tid == 0) {
             Arguments p = arguments_again();
             s_line.at += u.end - u.first, s_line.first = 0;
-            if (++s_line.unit == p.Hkv * p.row_tiles && s_line.at < s_line.end) {
+            if (++s_line.unit == p.Hkv * p.row_tiles) {
                 const int len = min(max(p.lens[u.b + 1], 0), p.most);
                 s_line.once = p.row_tiles == 1 && !shares_pages(p, u.b + 1);
                 s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.tiles = max((len + kTile - 1) / kTile, 1);
             }
         }
         __syncthreads();
-        if (s_line.at >= s_line.end) return;
     }
 }
 
@@ -661,10 +665,23 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
     if ((a.D == 64 || a.D == 128) && a.page_size % 16 == 0 && bits % 16 == 0 && a.n_pages > 0 && p.stride_t < (1 << 27) && a.workspace &&
         a.workspace_bytes >= sdpa_paged_workspace_bytes(a.B, a.Hq, a.Hkv, a.Sq, a.D)) {
         p.row_tiles = (int)((a.Hq / a.Hkv * a.Sq + kRows - 1) / kRows);
-        p.by_g = fast_div(p.G), p.by_row_tiles = fast_div(p.row_tiles);
+        p.by_g = fast_div(p.G), p.by_row_tiles = fast_div(p.row_tiles), p.by_workgroups = fast_div(line_workgroups());
         p.counters = (int *)a.workspace, p.parts = (float *)((char *)a.workspace + kWsCounterBytes);
-        if (a.dtype == TROCM_F16) return a.D == 64 ? launch_line<_Float16, 64>(p, line_workgroups(), s) : launch_line<_Float16, 128>(p, line_workgroups(), s);
-        return a.D == 64 ? launch_line<float, 64>(p, line_workgroups(), s) : launch_line<float, 128>(p, line_workgroups(), s);
+        // a line of tiles is counted in 31 bits: as many sequences in a launch as cannot be more
+        const int64_t most_tiles = std::max<int64_t>((p.most + kTile - 1) / kTile, 1) * a.Hkv * p.row_tiles, seqs = (1 << 30) / most_tiles;
+        if (seqs > 0) {
+            for (int64_t b0 = 0; b0 < a.B; b0 += seqs) {
+                PagedDev part = p;
+                part.B = (int)std::min(seqs, a.B - b0);
+                part.q += b0 * a.Hq * a.Sq * a.D * es, part.out += b0 * a.Hq * a.Sq * a.D * es;
+                part.table += b0 * a.table_width, part.lens += b0;
+                const int rc = a.dtype == TROCM_F16 ? a.D == 64 ? launch_line<_Float16, 64>(part, line_workgroups(), s) : launch_line<_Float16, 128>(part, line_workgroups(), s)
+                               : a.D == 64          ? launch_line<float, 64>(part, line_workgroups(), s)
+                                                    : launch_line<float, 128>(part, line_workgroups(), s);
+                if (rc) return rc;
+            }
+            return 0;
+        }
     }
     TROCM_REQUIRE(a.D <= kRowsMaxD, "sdpa_paged: head_dim %lld is more than %d", (long long)a.D, kRowsMaxD);
     const dim3 grid((unsigned)(a.Hq * a.Sq), (unsigned)std::min<int64_t>(a.B, 32768));
