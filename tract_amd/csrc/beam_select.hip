@@ -90,6 +90,17 @@ __device__ __forceinline__ double wave_sum(double x) {
     return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63) << 32);
 }
 
+// The same among a row's 16 lanes, everywhere in the row: rotations by 8, 4, 2, 1.
+constexpr int kRotate = 0x120;
+__device__ __forceinline__ float row_most(float x) {
+    x = larger<kRotate + 8, 0xf>(x), x = larger<kRotate + 4, 0xf>(x), x = larger<kRotate + 2, 0xf>(x);
+    return larger<kRotate + 1, 0xf>(x);
+}
+__device__ __forceinline__ double row_sum(double x) {
+    x = plus<kRotate + 8, 0xf>(x), x = plus<kRotate + 4, 0xf>(x), x = plus<kRotate + 2, 0xf>(x);
+    return plus<kRotate + 1, 0xf>(x);
+}
+
 // What a workgroup leaves for the one that puts a request together: written through to where every compute unit sees it once it completes.
 template <typename X>
 __device__ __forceinline__ void put(X *at, X x) {
@@ -408,16 +419,18 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         for (int i = tid % kLanes; i < p.parts; i += kLanes) {
             const float ref = get(pm + i), most = get(first + i * (int64_t)p.keep).x;
             const double sum = get(ps + i);
-            const float was = m;
-            m = fmaxf(m, ref), top = fmaxf(top, most), over = fmaxf(over, most - ref);   // (NaN where both are infinite: no number)
-            l = (was == -INFINITY ? 0.0 : l * exp((double)was - (double)m)) + (ref == -INFINITY ? 0.0 : sum * exp((double)ref - (double)m));
+            top = fmaxf(top, most), over = fmaxf(over, most - ref);   // (NaN where both are infinite: no number)
+            if (l == 0.0) {
+                l = ref == -INFINITY ? 0.0 : sum, m = ref;
+            } else if (ref != -INFINITY) {
+                const double step = exp(-fabs((double)ref - (double)m));
+                l = ref > m ? l * step + sum : l + sum * step;
+                m = fmaxf(m, ref);
+            }
         }
         const float mine = m;
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64)), top = fmaxf(top, __shfl_xor(top, d, 64)), over = fmaxf(over, __shfl_xor(over, d, 64));
-        l = mine == -INFINITY ? 0.0 : l * exp((double)mine - (double)m);
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) l += __shfl_xor(l, d, 64);
+        m = row_most(m), top = row_most(top), over = row_most(over);
+        l = row_sum(mine == -INFINITY ? 0.0 : l * exp((double)mine - (double)m));
         if (tid % kLanes == 0) {
             const bool dead = !(fabsf(score) < INFINITY);
             const double log_l = log(l);
