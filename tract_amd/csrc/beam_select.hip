@@ -619,8 +619,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
 }
 
 // How rows are cut into parts: tiles of 4 pieces of 8 values a thread, or of 1 where that leaves compute units without a workgroup; and as many
-// tiles one after the other as leave each compute unit kPerUnit workgroups.
-constexpr int kPerUnit = 4;
+// tiles one after the other as leave each compute unit kPerUnit workgroups.  (Three for each run at once with what they hold, so nothing waits
+// for a second round; us with 2, 3 and 4: 32 x 8 rows of 128256, f16 35.1, 33.0, 35.6 and f32 33.5, 34.4, 37.2; 64 x 4 of 32000, f16 15.6, 15.6,
+// 17.5; 16 x 4 of 32000, f32 16.5, 16.5, 22.5.)
+constexpr int kPerUnit = 3;
 struct Cut { int pieces; int64_t parts, turns; };
 Cut cut_of(int64_t rows, int64_t vocab) {
     Cut c;
