@@ -554,7 +554,7 @@ int trocm_sdpa_cached_scored(const void *q, int q_dtype, int64_t q_heads, int64_
  * Every id that comes from device memory is checked there: a page outside 0 .. n_pages - 1 is a hole (its keys are not seen, rows for
  * it are not stored), and a length outside 0 .. table_width * page_size is taken as the nearest of those for attention and refused by
  * the plan.  n_pages * page_size, and a table's row of tokens, at most 2^30; page_size at most 2^20 and page_size * head_dim at most
- * 2^29; plan and reorder take up to 4096 sequences. */
+ * 2^29; plan and reorder take up to 4096 sequences, reorder up to 2^24 pages. */
 
 /* Pages for the tokens that a step adds, and where each token goes.  Sequence i holds lens[i] tokens and gets n_new[i] more (0: none),
  * which are rows starts[i] .. of the step's n_tokens packed rows (sequences one behind the other, in order).
@@ -582,8 +582,8 @@ int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t 
  * count the new ones; causal: query r sees tokens up to lens[i] - q_len + r.  A row that sees nothing is zeros.  What lies behind a
  * sequence's last token, in pages that are not its own and in holes may hold anything; tokens that are hidden by causality alone must be finite.
  *   q, out    : [n_seq, q_heads, q_len, head_dim] dense, not overlapping; q_heads a multiple of kv_heads
- *   workspace : trocm_sdpa_paged_workspace_bytes, initialised by trocm_sdpa_workspace_init and shared like any other; with a smaller
- *               one or NULL a slow kernel runs
+ *   workspace : trocm_sdpa_paged_workspace_bytes, 16-byte aligned, initialised by trocm_sdpa_workspace_init and shared like any other;
+ *               with a smaller one or NULL a slow kernel runs
  * Fast kernels: head_dim 64 and 128, page_size a multiple of 16, bases and strides multiples of 16 bytes, q_heads / kv_heads * q_len rows
  * of a kv head as tiles of 16; anything else up to head_dim 2048 is correct and slow. */
 int trocm_sdpa_paged_workspace_bytes(int64_t n_seq, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t head_dim,
@@ -608,7 +608,7 @@ int trocm_paged_reorder(const int32_t *parents, int64_t n_seq, int64_t page_size
 
 /* The first `tokens` rows of every head from the source page to the destination page of each of n_copies entries, in each of n_pools
  * pools (a HOST array of device pointers: the K and the V pages of all layers, all of one shape and page_strides).  Entries with a page
- * outside of the pool are skipped; no destination may be another entry's source or destination. */
+ * outside of the pool are skipped; no destination may be another entry's source or destination.  n_copies up to 2^22. */
 int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools, int64_t n_pools, int dtype, int64_t kv_heads,
                      int64_t head_dim, int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream);
 
@@ -620,7 +620,7 @@ int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools
  *   eos        : -1 (none; `ended` must be NULL) or a token
  *   outputs    : [batch, keep]: scores_out f32, parents (rows of the batch: request * beams + beam), tokens, ended_out (or NULL: 1 where the token
  *                is eos or the parent had ended).  May not overlap inputs
- *   workspace  : trocm_beam_select_workspace_bytes, initialised by trocm_sdpa_workspace_init and shared like any other
+ *   workspace  : trocm_beam_select_workspace_bytes, 16-byte aligned, initialised by trocm_sdpa_workspace_init and shared like any other
  * A NaN among the logits counts as -inf.  keep and beams up to 64, keep at most beams * vocab, vocab up to 2^30, beams * vocab below 2^31. */
 int trocm_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep, size_t *bytes);
 int trocm_beam_select(const void *logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,

@@ -141,3 +141,22 @@ def test_shapes_and_types_are_refused(rt):
         ta.BeamSelect(2).eval(x, s, out={"scores": up(np.zeros((2, 3), F32))})
     with pytest.raises(ta.TractRocmError):
         ta.BeamSelect(200).eval(x, s)
+
+
+def test_more_requests_than_a_launch_counts(rt):
+    """16384 requests have a counter each in a launch; parents of the ones behind them are rows of the whole batch."""
+    rng = np.random.default_rng(6)
+    logits = (rng.standard_normal((16400, 2, 9)) * 2).astype(F32)
+    got = _check(logits, (-rng.random((16400, 2))).astype(F32), 3)
+    assert got["parents"].max() >= 2 * 16399
+
+
+def test_keep_that_changes_from_call_to_call(rt):
+    rng = np.random.default_rng(7)
+    logits, scores = (rng.standard_normal((2, 3, 500))).astype(F16), (-rng.random((2, 3))).astype(F32)
+    op = ta.BeamSelect(2)
+    for keep in (2, 60, 5):
+        op.keep = keep
+        got, want = op.eval(up(logits), up(scores)), ref.select(logits, scores, keep)
+        for name in ("parents", "tokens"):
+            np.testing.assert_array_equal(got[name].to_numpy(), want[name])

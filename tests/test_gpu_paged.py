@@ -371,3 +371,93 @@ def test_shapes_and_types_are_refused(rt):
         ta.PagedCopy().eval(ints([[0, 1, 2]]), [k, up(np.zeros((5, 2, 16, 64), F32))])
     with pytest.raises(ta.TractRocmError):
         ta.PagedReorder(16).eval(n, t, n, ints([0] * 5), ints([0] * 4), ints([5]))
+    refs = ints([0] * 5)
+    plan = ta.PagedPlan(16)
+    plan.eval(n, n, t, ints([0] * 5), ints([5]), 2, refs=refs)
+    with pytest.raises(ta.TractRocmError):   # (a type that changes from call to call)
+        plan.eval(n, n, t, ints([0] * 5), ints([5]), 2, refs=up(np.zeros(5, np.int64)))
+
+
+# ---- the far ends of what the calls allow -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_tables_of_so_many_tokens_that_a_launch_takes_one_sequence(rt, dtype, d):
+    """Rows of the table for 2^30 tokens, 32 kv heads: a line of tiles counted in 31 bits has room for one sequence, whatever its length.
+    Pages of 2^20 tokens of which 100 are used: heads lie 128 rows apart, inside of one another's pages."""
+    rng, page, width, heads, lens = np.random.default_rng(d), 1 << 20, 1 << 10, 32, [100, 0, 33]
+    apart = 128
+    strides = (heads * apart * d, apart * d, d)
+    size = 2 * strides[0] + (heads - 1) * strides[1] + page * d
+    n_pages = 3
+    used = [rng.standard_normal((n_pages, heads, apart, d)).astype(dtype) for _ in range(2)]
+    pools = []
+    for u in used:
+        flat = np.zeros(size, dtype)
+        flat[:u.size] = u.reshape(-1)
+        base = up(flat)
+        pools.append((base, ta.DeviceTensor((n_pages, heads, page, d), dtype, ptr=base.ptr.value, owner=base)))
+    table = np.full((3, width), -1, I32)
+    table[:, 0] = [2, 0, 1]
+    q = (rng.standard_normal((3, heads, 1, d)) * 2).astype(dtype)
+    got = ta.PagedSdpa().eval(up(q), pools[0][1], pools[1][1], up(table), ints(lens), page_strides=strides).to_numpy()
+    want, bound = ref.attend(q, *used, table[:, :1], np.array(lens, I32))
+    assert_within(got, want, bound, f"{d} {np.dtype(dtype).name}")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attend_more_rows_than_a_launch_has_workgroups(rt, dtype):
+    """5120000 query rows of an odd size, a workgroup each: sequences of one token repeat its value, empty ones are zeros."""
+    rng, n, heads, sq, d, page = np.random.default_rng(9), 5000, 8, 128, 2, 3
+    k, v = (rng.standard_normal((n, 2, page, d)).astype(dtype) for _ in range(2))
+    lens = rng.integers(0, 2, n).astype(I32)
+    got = ta.PagedSdpa(is_causal=False).eval(up(np.zeros((n, heads, sq, d), dtype)), up(k), up(v), up(np.arange(n, dtype=I32)[:, None]), up(lens)).to_numpy()
+    want = np.where(lens[:, None, None, None] > 0, np.repeat(v[:, :, 0], heads // 2, axis=1)[:, :, None, :], dtype(0))
+    np.testing.assert_array_equal(got, np.broadcast_to(want, got.shape))
+
+
+def test_append_more_tokens_than_a_launch_has_workgroups(rt):
+    """4194304 workgroups of a token each, and 7 tokens more; most go nowhere.  Rows begin 8 elements apart."""
+    tokens, heads, d, n_pages, page = (1 << 22) + 7, 8, 1024, 3, 4
+    rng = np.random.default_rng(3)
+    flat = rng.integers(0, 1 << 15, (tokens - 1) * 8 + heads * d, dtype=np.uint16).view(F16)
+    slots = np.full(tokens, -1, I32)
+    goes = [0, 5, (1 << 22) - 1, 1 << 22, (1 << 22) + 1, tokens - 1]
+    slots[goes] = [3, 11, 0, 7, 4, 8]
+    base, pools = up(flat), [up(np.zeros((n_pages, heads, page, d), F16)) for _ in range(2)]
+    rows = ta.DeviceTensor((tokens, heads, d), F16, ptr=base.ptr.value, owner=base)
+    ta.PagedAppend().eval(rows, rows, up(slots), *pools, k_strides=(8, d), v_strides=(8, d))
+    want = np.zeros((n_pages, heads, page, d), F16)
+    for t in goes:
+        want[slots[t] // page, :, slots[t] % page] = flat[t * 8:t * 8 + heads * d].reshape(heads, d)
+    for pool in pools:
+        assert pool.to_numpy().tobytes() == want.tobytes()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_the_same_pages_many_times(rt, causal):
+    """Sequences that are one another's copies, and a page that comes twice in a row of the table."""
+    rng, d, page = np.random.default_rng(4), 128, 16
+    k, v = (rng.standard_normal((4, 2, page, d)).astype(F16) for _ in range(2))
+    table = np.array([[0, 1, 0, 2], [0, 1, 0, 2], [3, 3, 3, 3], [0, 1, 0, 2], [2, 2, 1, 1]], I32)
+    lens = np.array([64, 64, 50, 1, 33], I32)
+    q = (rng.standard_normal((5, 8, 3, d)) * 2).astype(F16)
+    got = ta.PagedSdpa(is_causal=causal).eval(up(q), up(k), up(v), up(table), up(lens)).to_numpy()
+    want, bound = ref.attend(q, k, v, table, lens, causal=causal)
+    assert_within(got, want, bound, "shared")
+    if not causal:
+        one = ta.PagedSdpa(is_causal=False).eval(up(np.repeat(q[:1], 5, axis=0)), up(k), up(v), up(table), up(lens)).to_numpy()
+        assert_within(one[1], one[0].astype(np.float64), 2 * bound[0], "copies")
+
+
+@pytest.mark.parametrize("n_pages,page", [(20000, 1), (100000, 2), (1 << 20, 1)])
+def test_reorder_of_large_pools(rt, n_pages, page):
+    """More pages than a workgroup takes: the stack of the free ones is put together from several shares."""
+    rng, n, longest = np.random.default_rng(n_pages), 40, min(n_pages // 50 * page, 8000)
+    lens = rng.integers(0, longest, n).astype(I32)
+    width = -(-longest // page)
+    table, free, count = _tables(rng, lens, page, width, n_pages)
+    refs = np.zeros(n_pages, I32)
+    np.add.at(refs, table[table >= 0], 1)
+    _check_reorder(rng.integers(-2, n + 2, n).astype(I32), table, lens, refs, free, count, page)

@@ -115,3 +115,19 @@ def _select(**kw):
     (dict(tokens=at(4) + 8), "overlaps parents"), (dict(ws=at(1)), "workspace overlaps logits"), (dict(logits=at(1) + 1), "aligned"), (dict(batch=1 << 24), "too large")])
 def test_select(kw, says):
     assert says in _select(**kw)
+
+
+@pytest.mark.parametrize("ps", [I3(1 << 39, 64, 64), I3(1, 1 << 39, 64), I3(1, 64, 1 << 39)])
+def test_strides_that_no_memory_has_room_for(ps):
+    """(each below 2^40, but products with pages, heads or tokens that would leave 64 bits or any address space)"""
+    assert "page strides too large" in _append(ps=ps, pages=1 << 10, page=1 << 12, heads=1 << 12)
+    assert "page strides too large" in _sdpa(ps=ps, pages=1 << 10, page=1 << 12, hkv=1 << 12, hq=1 << 12)
+    assert "page strides too large" in _copy(ps=ps, pages=1 << 10, page=1 << 12, heads=1 << 12)
+    assert "row_stride" in _select(stride=1 << 40, batch=1 << 8)
+
+
+@pytest.mark.parametrize("call,kw,says", [
+    (_sdpa, dict(ws=at(7) + 8, wsb=1 << 16), "16-byte aligned"), (_sdpa, dict(ws=at(6), wsb=1 << 16), "workspace overlaps out"), (_sdpa, dict(ws=at(2), wsb=1 << 16), "workspace overlaps k_pages"),
+    (_select, dict(ws=at(7) + 8), "16-byte aligned"), (_reorder, dict(pages=(1 << 24) + 1, page=1), "2^24"), (_copy, dict(n=(1 << 22) + 1), "2^22")])
+def test_workspaces_and_what_would_take_too_long(call, kw, says):
+    assert says in call(**kw)

@@ -1,6 +1,7 @@
 // Entry points over pages of keys and values, and beam search's choice: checks of arguments, in the manner of abi.hip.
 #include <math.h>
 #include <string.h>
+#include <algorithm>
 #include <initializer_list>
 #include "common.h"
 
@@ -8,7 +9,11 @@ using namespace trocm;
 
 namespace {
 
-constexpr int64_t kMostTokens = 1ll << 30, kMostPage = 1ll << 20;
+constexpr int64_t kMostTokens = 1ll << 30, kMostPage = 1ll << 20, kMostReclaimed = 1ll << 24;
+
+// (far more than there is memory, and sums of a few such products stay inside of 64 bits)
+constexpr double kReach = 281474976710656.0;
+bool within_reach(int64_t rows, int64_t stride) { return (double)rows * (double)stride < kReach; }
 
 struct Range { const void *at; size_t bytes; const char *name; };
 
@@ -43,7 +48,7 @@ int table_check(const char *what, int64_t n_seq, int64_t table_width, int64_t pa
 }
 
 // Strides of the pools, checked; dense ones where none are given.
-int page_strides_check(const char *what, int dtype, int64_t kv_heads, int64_t head_dim, int64_t page_size, const int64_t *given, int64_t *st) {
+int page_strides_check(const char *what, int dtype, int64_t n_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size, const int64_t *given, int64_t *st) {
     TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "%s: dtype must be F32 or F16", what);
     TROCM_REQUIRE(kv_heads >= 0 && head_dim >= 0, "%s: negative dimension", what);
     TROCM_REQUIRE(head_dim < (1 << 24) && kv_heads <= 65535 && head_dim * page_size <= (1 << 29) && head_dim * kv_heads < (1 << 29), "%s: tensor too large", what);
@@ -54,6 +59,7 @@ int page_strides_check(const char *what, int dtype, int64_t kv_heads, int64_t he
         TROCM_REQUIRE(given[i] < (1ll << 40), "%s: page strides too large", what);
         st[i] = given[i];
     }
+    TROCM_REQUIRE(within_reach(n_pages, st[0]) && (double)kv_heads * st[1] + (double)page_size * st[2] < kReach, "%s: page strides too large", what);
     return 0;
 }
 
@@ -103,7 +109,7 @@ int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t 
                        int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream) {
     PagedAppendArgs a;
     if (pages_check("paged_append", n_pages, page_size)) return 1;
-    if (page_strides_check("paged_append", dtype, kv_heads, head_dim, page_size, page_strides, a.page_strides)) return 1;
+    if (page_strides_check("paged_append", dtype, n_pages, kv_heads, head_dim, page_size, page_strides, a.page_strides)) return 1;
     TROCM_REQUIRE(n_tokens >= 0, "paged_append: negative dimension");
     TROCM_REQUIRE(n_tokens <= kMostTokens, "paged_append: tensor too large");
     if (n_tokens == 0 || kv_heads == 0 || head_dim == 0 || n_pages == 0) return 0;
@@ -149,7 +155,7 @@ int trocm_sdpa_paged(const void *q, int dtype, int64_t n_seq, int64_t q_heads, i
     int64_t st[3];
     if (pages_check("sdpa_paged", n_pages, page_size) || table_check("sdpa_paged", n_seq, table_width, page_size, (1 << 24) - 1)) return 1;
     TROCM_REQUIRE(q_heads >= 0 && kv_heads >= 1 && q_len >= 0, "sdpa_paged: negative dimension");
-    if (page_strides_check("sdpa_paged", dtype, kv_heads, head_dim, page_size, page_strides, st)) return 1;
+    if (page_strides_check("sdpa_paged", dtype, n_pages, kv_heads, head_dim, page_size, page_strides, st)) return 1;
     TROCM_REQUIRE(q_heads % kv_heads == 0, "Q heads (%lld) must be a multiple of K/V heads (%lld)", (long long)q_heads, (long long)kv_heads);
     TROCM_REQUIRE(q_heads < (1 << 24) && q_len < (1 << 24) && q_heads * q_len < (1ll << 30) && n_seq * q_heads * q_len < (1ll << 31), "sdpa_paged: tensor too large");
     if (n_seq == 0 || q_heads == 0 || q_len == 0 || head_dim == 0) return 0;
@@ -162,10 +168,11 @@ int trocm_sdpa_paged(const void *q, int dtype, int64_t n_seq, int64_t q_heads, i
     }
     if (table_width) TROCM_NOT_NULL(table);
     const size_t q_bytes = (size_t)(n_seq * q_heads * q_len * head_dim) * elem_bytes(dtype), pool = pool_bytes(n_pages, kv_heads, page_size, head_dim, st, dtype);
-    if (apart("sdpa_paged", {{out, q_bytes, "out"}}, {{q, q_bytes, "q"}, {k_pages, pool, "k_pages"}, {v_pages, pool, "v_pages"},
+    if (apart("sdpa_paged", {{out, q_bytes, "out"}, {workspace, workspace_bytes, "workspace"}}, {{q, q_bytes, "q"}, {k_pages, pool, "k_pages"}, {v_pages, pool, "v_pages"},
                                                      {table, (size_t)n_seq * (size_t)table_width * 4, "table"}, {lens, (size_t)n_seq * 4, "lens"}})) return 1;
     if (aligned("sdpa_paged", {{q, 0, "q"}, {out, 0, "out"}, {k_pages, 0, "k_pages"}, {v_pages, 0, "v_pages"}}, elem_bytes(dtype))) return 1;
     if (aligned("sdpa_paged", {{table, 0, "table"}, {lens, 0, "lens"}}, 4)) return 1;
+    TROCM_REQUIRE((uintptr_t)workspace % 16 == 0, "sdpa_paged: workspace must be 16-byte aligned");
     hipStream_t s;
     if (resolve_stream(stream, &s)) return 1;
     SdpaPagedArgs a;
@@ -182,6 +189,7 @@ int trocm_paged_reorder(const int32_t *parents, int64_t n_seq, int64_t page_size
                         int32_t *lens_out, int32_t *refs_out, int32_t *free_pages_out, int32_t *free_count_out, int32_t *copies,
                         int32_t *missing, void *stream) {
     if (pages_check("paged_reorder", n_pages, page_size) || table_check("paged_reorder", n_seq, table_width, page_size, kPagedMaxSeqs)) return 1;
+    TROCM_REQUIRE(n_pages <= kMostReclaimed, "paged_reorder: %lld pages are more than 2^24", (long long)n_pages);   // (every 16384 of them count all others')
     if (n_seq) {
         TROCM_NOT_NULL(parents);
         TROCM_NOT_NULL(lens);
@@ -218,9 +226,9 @@ int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools
                      int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream) {
     PagedCopyArgs a;
     if (pages_check("paged_copy", n_pages, page_size)) return 1;
-    if (page_strides_check("paged_copy", dtype, kv_heads, head_dim, page_size, page_strides, a.page_strides)) return 1;
+    if (page_strides_check("paged_copy", dtype, n_pages, kv_heads, head_dim, page_size, page_strides, a.page_strides)) return 1;
     TROCM_REQUIRE(n_copies >= 0 && n_pools >= 0, "paged_copy: negative dimension");
-    TROCM_REQUIRE(n_copies <= kMostTokens, "paged_copy: tensor too large");
+    TROCM_REQUIRE(n_copies <= (1 << 22), "paged_copy: %lld entries are more than 2^22", (long long)n_copies);
     if (n_copies == 0 || n_pools == 0 || n_pages == 0) return 0;
     TROCM_NOT_NULL(copies);
     TROCM_NOT_NULL(pools);
@@ -260,7 +268,7 @@ int trocm_beam_select(const void *logits, int dtype, int64_t batch, int64_t beam
     TROCM_REQUIRE(dtype == TROCM_F32 || dtype == TROCM_F16, "beam_select: dtype must be F32 or F16");
     if (beam_check(batch, beams, vocab, keep)) return 1;
     if (row_stride == 0) row_stride = vocab;
-    TROCM_REQUIRE(row_stride >= vocab && row_stride < (1ll << 40), "beam_select: row_stride %lld does not hold a row of %lld", (long long)row_stride, (long long)vocab);
+    TROCM_REQUIRE(row_stride >= vocab && within_reach(std::max<int64_t>(batch * beams, 1), row_stride), "beam_select: row_stride %lld does not hold a row of %lld", (long long)row_stride, (long long)vocab);
     TROCM_REQUIRE(eos >= -1 && eos < vocab, "beam_select: eos must be -1 or a token (got %d)", eos);
     TROCM_REQUIRE(!ended || eos >= 0, "beam_select: beams that have ended need eos");
     if (batch == 0) return 0;
@@ -275,6 +283,7 @@ int trocm_beam_select(const void *logits, int dtype, int64_t batch, int64_t beam
               {{logits, (size_t)((batch * beams - 1) * row_stride + vocab) * es, "logits"}, {scores, in, "scores"}, {ended, in, "ended"}})) return 1;
     if (aligned("beam_select", {{logits, 0, "logits"}}, es)) return 1;
     if (aligned("beam_select", {{scores, 0, "scores"}, {ended, 0, "ended"}, {scores_out, 0, "scores_out"}, {parents, 0, "parents"}, {tokens, 0, "tokens"}, {ended_out, 0, "ended_out"}}, 4)) return 1;
+    TROCM_REQUIRE((uintptr_t)workspace % 16 == 0, "beam_select: workspace must be 16-byte aligned");
     hipStream_t s;
     if (resolve_stream(stream, &s)) return 1;
     BeamSelectArgs a;

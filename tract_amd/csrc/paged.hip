@@ -404,7 +404,17 @@ __global__ __launch_bounds__(kPlanThreads) void paged_reclaim_kernel(ReorderDev 
 // cost more than the one compute unit takes (one | three launches, with the copies that follow: 64 sequences of 46 entries 12.7 | 15.0 to 17.8 us,
 // 128 14.8 | 14.9 to 17.8, 256, in eight layers, 29.2 | 25.7).
 constexpr int kSmallPages = kReclaim, kSmallEntries = 6144;
-__global__ __launch_bounds__(kPlanThreads) void paged_reorder_kernel(ReorderDev p) {
+// The argument where it lies, as loads from here on: kept from the beginning, it would not leave enough scalar registers.
+__device__ __forceinline__ ReorderDev arguments_again() {
+    auto at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(at));
+    struct Words { uint64_t w[sizeof(ReorderDev) / 8]; } r;
+#pragma unroll
+    for (size_t i = 0; i < sizeof(ReorderDev) / 8; i++) r.w[i] = reinterpret_cast<const __attribute__((address_space(4))) uint64_t *>(at)[i];
+    return __builtin_bit_cast(ReorderDev, r);
+}
+__global__ __launch_bounds__(kPlanThreads) void paged_reorder_kernel(ReorderDev) {
+    ReorderDev p = arguments_again();
     __shared__ int s_refs[kSmallPages + kSmallPages / 16], s_first[kPagedMaxSeqs], s_children[kPagedMaxSeqs], s_lens[kPagedMaxSeqs], s_from[kPagedMaxSeqs], s_waves[2][kPlanWaves];
     auto page_at = [](int x) { return x + (x >> 4); };   // (threads that take 16 pages each are in different banks)
     const int tid = threadIdx.x, width = (int)p.table_width, per = (p.n_seq + kPlanThreads - 1) / kPlanThreads, j0 = min(tid * per, p.n_seq), mine = min(per, p.n_seq - j0);
@@ -425,6 +435,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_reorder_kernel(ReorderDev 
     for (int y = 0; y < kMine; y++)
         if (y < mine && s_from[j0 + y] >= 0) atomicAdd(&s_children[s_from[j0 + y]], 1);
     __syncthreads();
+    p = arguments_again();
     // the tables, a thread per entry, several entries' loads at once; what old rows' pages lose or gain
     const FastDiv by_width = p.by_width;
     constexpr int kDeep = 4;
@@ -461,6 +472,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_reorder_kernel(ReorderDev 
         }
     }
     __syncthreads();
+    p = arguments_again();
     Sixteen now;
 #pragma unroll
     for (int x = 0; x < 16; x++) now.v[x] = tid * 16 + x < p.n_pages ? s_refs[page_at(tid * 16 + x)] : 0;
@@ -540,15 +552,22 @@ int launch_paged_append(const PagedAppendArgs &a, hipStream_t s) {
     p.dst_page = a.page_strides[0] * es, p.dst_head = a.page_strides[1] * es, p.dst_token = a.page_strides[2] * es;
     bits |= (uint64_t)p.dst_page | (uint64_t)p.dst_head | (uint64_t)p.dst_token;
     const int word = word_of(bits);
-    p.slots = a.slots, p.n_tokens = (int)a.n_tokens, p.n_slots = (int)(a.n_pages * a.page_size);
+    p.slots = a.slots, p.n_slots = (int)(a.n_pages * a.page_size);
     p.words_per_token = (int)(a.kv_heads * a.D * es / word);
     p.tokens_per_block = std::max(1, 256 * kTurns / p.words_per_token);
     p.by_words_per_token = fast_div(p.words_per_token), p.by_words_per_row = fast_div(a.D * es / word), p.by_page = fast_div(a.page_size);
-    const dim3 grid((unsigned)((a.n_tokens + p.tokens_per_block - 1) / p.tokens_per_block));
-    if (word == 16) paged_append_kernel<Quad><<<grid, 256, 0, s>>>(p);
-    else if (word == 4) paged_append_kernel<uint32_t><<<grid, 256, 0, s>>>(p);
-    else paged_append_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
-    TROCM_HIP(hipGetLastError());
+    // (a launch counts threads in 32 bits)
+    const int64_t turn = std::min<int64_t>((int64_t)p.tokens_per_block << 22, 1 << 30);
+    for (int64_t first = 0; first < a.n_tokens; first += turn) {
+        p.n_tokens = (int)std::min(turn, a.n_tokens - first);
+        const dim3 grid((unsigned)((p.n_tokens + p.tokens_per_block - 1) / p.tokens_per_block));
+        if (word == 16) paged_append_kernel<Quad><<<grid, 256, 0, s>>>(p);
+        else if (word == 4) paged_append_kernel<uint32_t><<<grid, 256, 0, s>>>(p);
+        else paged_append_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
+        TROCM_HIP(hipGetLastError());
+        p.slots += turn;
+        for (int y = 0; y < 2; y++) p.src[y] += turn * p.src_token[y];
+    }
     return 0;
 }
 

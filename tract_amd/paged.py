@@ -76,7 +76,7 @@ class PagedPlan:
         lens [n_seq], starts [n_seq + 1], slots and positions [tokens], free_count [1], refused [1]; none of them may be an input."""
         if not isinstance(lens, DeviceTensor) or not isinstance(n_new, DeviceTensor):
             lens, n_new = _as_device(lens, stream), _as_device(n_new, stream)
-        key = (lens.shape, n_new.shape, table.shape, free_pages.shape, free_count.shape, tokens, refs is None or refs.shape,
+        key = (lens.shape, n_new.shape, table.shape, free_pages.shape, free_count.shape, tokens, refs is None or (refs.shape, refs.dtype),
                *(t.dtype for t in (lens, n_new, table, free_pages, free_count)))
         last_key, sizes = self._last   # (a pair, read once: another thread's call may put its own there)
         if key != last_key:
@@ -253,7 +253,7 @@ class BeamSelect:
             logits, scores = _as_device(logits, stream), _as_device(scores, stream)
         if ended is not None and not isinstance(ended, DeviceTensor):
             ended = _as_device(ended, stream)
-        key = (logits.shape, scores.shape, logits.dtype, scores.dtype, ended is None or (ended.shape, ended.dtype))
+        key = (self.keep, logits.shape, scores.shape, logits.dtype, scores.dtype, ended is None or (ended.shape, ended.dtype))
         last_key, sizes, ws = self._last
         if key != last_key:
             if len(logits.shape) != 3 or scores.shape != logits.shape[:2] or not _same(scores.dtype, _F32):
