@@ -26,6 +26,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kTile = 32, kRows = 16;
+constexpr int kStep = kTile * kWaves;   // keys of a step: a tile for each wave
 
 struct PagedDev {
     const char *q, *k, *v;
@@ -178,13 +179,14 @@ constexpr int kLinePart(int D) { return kRows * D + 2 * kRows; }   // floats of 
 constexpr int in_lds(int es, int D) { return es == 4 && D == 128 ? kRows * D * es : 0; }   // bytes of queries
 constexpr int line_lds(int es, int D) { return kWaves * kTile * (es == 2 ? 2 * D + 24 : D + 4) * es + in_lds(es, D); }
 
-// Tiles [first, end) of a unit; `part`: where its partial rows go (NULL: it is the whole unit, rows go to the output).
+// Steps [first, end) of a unit; `part`: where its partial rows go, a row tile's behind the other's (NULL: it is the whole unit, rows go to the
+// output).
 struct Stretch {
     int b, kvh, row0, rows, len, first, end;
     float *part;
 };
 
-template <typename T, int D, bool ONCE>
+template <typename T, int D, int RT, bool ONCE>
 __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *lds) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int DB = D / 16;                    // feature blocks of the output
@@ -198,34 +200,43 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane / 16, lr = lane % 16;
     Arguments p = arguments_again();
-    const RowPlace place = q_row(p, u.b, u.kvh, u.row0 + min(lr, u.rows - 1));
-    const int lim = p.causal ? min(u.len - 1, u.len - p.Sq + place.i) : u.len - 1;
+    int64_t q_at[RT];
+    int lim[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const RowPlace place = q_row(p, u.b, u.kvh, u.row0 + min(16 * t + lr, u.rows - 1));
+        q_at[t] = place.at, lim[t] = p.causal ? min(u.len - 1, u.len - p.Sq + place.i) : u.len - 1;
+    }
     const int last_key = u.len - 1;
     const char *kb = p.k + u.kvh * p.stride_h, *vb = p.v + u.kvh * p.stride_h;
     const uint32_t st = (uint32_t)p.stride_t;     // (below 2^27: checked by the host)
     const float to_log2 = p.scale * kLog2e;
-    const int n_mine = (u.end - u.first - w + kWaves - 1) / kWaves;   // this wave takes every fourth tile
+    const int n_mine = min(u.end - u.first, (last_key / kTile - u.first * kWaves - w + kWaves) / kWaves);   // this wave takes a tile of every step
 
     // Where the halves of 32 of this wave's tiles lie: lane 2 i + h has tile i's half h, as bytes from the pool's beginning (-1: a hole, or
     // behind the last key).
     auto ask_pages = [&](int i0) __attribute__((always_inline)) {
         Arguments p = arguments_again();
-        const int key = (u.first + w + kWaves * (i0 + (lane >> 1))) * kTile + 16 * (lane & 1);
+        const int key = ((u.first + i0 + (lane >> 1)) * kWaves + w) * kTile + 16 * (lane & 1);
         return key <= last_key && i0 + (lane >> 1) < n_mine ? p.table[u.b * p.table_width + divided(p.by_page, key)] : -1;
     };
     auto bytes_at = [&](int id, int i0) __attribute__((always_inline)) {
         Arguments p = arguments_again();
-        const int key = (u.first + w + kWaves * (i0 + (lane >> 1))) * kTile + 16 * (lane & 1);
+        const int key = ((u.first + i0 + (lane >> 1)) * kWaves + w) * kTile + 16 * (lane & 1);
         const int in_page = key - divided(p.by_page, key) * (int)p.by_page.d;
         return (unsigned)id < (unsigned)p.n_pages ? id * p.stride_page + (int64_t)in_page * p.stride_t : (int64_t)-1;
     };
     int64_t at = -1;
     int ids_next = -1;
 
-    float m_run = -INFINITY, l_run = 0.0f;
-    float4_t o[DB];
+    float m_run[RT], l_run[RT];
+    float4_t o[RT][DB];
 #pragma unroll
-    for (int db = 0; db < DB; db++) o[db] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < RT; t++) {
+        m_run[t] = -INFINITY, l_run[t] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; db++) o[t][db] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     T *lds_v = reinterpret_cast<T *>(lds + w * PRIV), *lds_k = lds_v + kTile * VROW;   // (lds_k: f16)
     const int kr = lane / LPRW, ch = lane % LPRW;
@@ -244,7 +255,7 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
     // (halves that are not there read the other one's rows, or the pool's first: they weigh nothing; rows behind the last key repeat it)
     auto row_base = [&](const Halves &x, int h) __attribute__((always_inline)) { return x.at[h] >= 0 ? x.at[h] : x.at[1 - h] >= 0 ? x.at[1 - h] : 0; };
     auto rows_of = [&](int i, const Halves &x, int h) __attribute__((always_inline)) {   // the last row of a half that may be read
-        const int most = last_key - (u.first + w + kWaves * i) * kTile;
+        const int most = last_key - ((u.first + i) * kWaves + w) * kTile;
         if (x.at[0] < 0 && x.at[1] < 0) return 0;
         return min(most - 16 * (x.at[h] >= 0 ? h : 1 - h), 15);
     };
@@ -285,16 +296,19 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
     }
     // queries: in registers, or, where those are all taken, in LDS
     constexpr bool QL = in_lds(sizeof(T), D) > 0;
-    u32x4 qf[QL ? 1 : KS], *lds_q = reinterpret_cast<u32x4 *>(lds + kWaves * PRIV);
+    static_assert(!QL || RT == 1, "one row tile's");
+    u32x4 qf[RT][QL ? 1 : KS], *lds_q = reinterpret_cast<u32x4 *>(lds + kWaves * PRIV);
     if constexpr (QL) {
-        for (int ks = w; ks < KS; ks += kWaves) lds_q[ks * 64 + lane] = load16<false>(p.q + place.at * (D * (int)sizeof(T)), ks * 64 + grp * 16);
+        for (int ks = w; ks < KS; ks += kWaves) lds_q[ks * 64 + lane] = load16<false>(p.q + q_at[0] * (D * (int)sizeof(T)), ks * 64 + grp * 16);
         __syncthreads();
     } else {
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) qf[ks] = load16<false>(p.q + place.at * (D * (int)sizeof(T)), ks * 64 + grp * 16);
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) qf[t][ks] = load16<false>(p.q + q_at[t] * (D * (int)sizeof(T)), ks * 64 + grp * 16);
     }
     for (int i = 0; i < n_mine; i++) {
-        const int k_lo = (u.first + w + kWaves * i) * kTile;
+        const int k_lo = ((u.first + i) * kWaves + w) * kTile;
         const bool more = i + 1 < n_mine;
         Halves next = {-1, -1};
         if (more) {
@@ -305,9 +319,11 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
         const bool odd = there != 3 || k_lo + kTile > u.len;   // a hole, or the last key inside
 
         // ---- S^T = K Q^T --------------------------------------------------------------------------------------
-        float4_t acc[2];
+        float4_t acc[RT][2];
 #pragma unroll
-        for (int h = 0; h < 2; h++) acc[h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) acc[t][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
         if constexpr (H16) {
 #pragma unroll
             for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_k + (j * RPI + kr) * KROW + ch * 8) = kpre[j];
@@ -317,25 +333,25 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4 *>(lds_k + (16 * h + lr) * KROW + ks * 32 + grp * 8);
-                    acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, kf), __builtin_bit_cast(half8_t, qf[ks]), acc[h], 0, 0, 0);
+                    const half8_t kf = __builtin_bit_cast(half8_t, *reinterpret_cast<const u32x4 *>(lds_k + (16 * h + lr) * KROW + ks * 32 + grp * 8));
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(half8_t, qf[t][ks]), acc[t][h], 0, 0, 0);
                 }
         } else {
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const float4_t c = __builtin_bit_cast(float4_t, QL ? lds_q[ks * 64 + lane] : qf[QL ? 0 : ks]);
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {   // (one feature of each group's four at a time)
-                    const float4_t a = __builtin_bit_cast(float4_t, kpre[h * KS + ks]);
+                for (int t = 0; t < RT; t++) {
+                    const float4_t c = __builtin_bit_cast(float4_t, QL ? lds_q[ks * 64 + lane] : qf[t][QL ? 0 : ks]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[h], 0, 0, 0);
+                    for (int h = 0; h < 2; h++) {   // (one feature of each group's four at a time)
+                        const float4_t a = __builtin_bit_cast(float4_t, kpre[h * KS + ks]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[t][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], acc[t][h], 0, 0, 0);
+                    }
                 }
-            }
             if (more) prefetch_k(i + 1, next);
         }
-        float s[8];
-#pragma unroll
-        for (int x = 0; x < 8; x++) s[x] = acc[x >> 2][x & 3] * to_log2;
         if (odd) {   // rows that are not the sequence's may hold anything
 #pragma unroll
             for (int j = 0; j < NI; j++) {
@@ -347,40 +363,46 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
         for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_v + (j * RPI + kr) * VROW + ch * (16 / (int)sizeof(T))) = vpre[j];
         if (more) prefetch_v(i + 1, next);
 
-        // ---- softmax of this lane's row over its keys k_lo + 4 grp + key_of(x) -----------------------------------
-        const int last = lim - k_lo - 4 * grp;
-        if (odd || __builtin_amdgcn_ballot_w64(last < 28) != 0) {
+        // ---- softmax of this lane's rows over their keys k_lo + 4 grp + key_of(x) --------------------------------
+        half8_t pf[RT];        // weights: f16
+        float e[RT][8];        // ... and f32
 #pragma unroll
-            for (int x = 0; x < 8; x++) s[x] = key_of(x) <= last && ((there >> (x >> 2)) & 1) ? s[x] : -INFINITY;
-        }
-        float top = s[0];
+        for (int t = 0; t < RT; t++) {
+            float s[8];
 #pragma unroll
-        for (int x = 1; x < 8; x++) top = fmaxf(top, s[x]);
+            for (int x = 0; x < 8; x++) s[x] = acc[t][x >> 2][x & 3] * to_log2;
+            const int last = lim[t] - k_lo - 4 * grp;
+            if (odd || __builtin_amdgcn_ballot_w64(last < 28) != 0) {
 #pragma unroll
-        for (int d = 16; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
-        const bool moved = less(top, m_run) > (H16 ? 8.0f : 0.0f);
-        const float m_new = moved ? top : m_run, ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float keep = moved ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
-        m_run = m_new;
-        half8_t pf;
-        float sum = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 8; x++) {
-            float e = __builtin_amdgcn_exp2f(less(s[x], ref));
-            // The product with V takes f16 operands: weights are rounded, half a step each, and the row's sum takes the same ones, so that a row
-            // of equal values stays that value.
-            if constexpr (H16) {
-                pf[x] = (_Float16)e;
-                e = (float)pf[x];
+                for (int x = 0; x < 8; x++) s[x] = key_of(x) <= last && ((there >> (x >> 2)) & 1) ? s[x] : -INFINITY;
             }
-            s[x] = e;
-            sum += e;
-        }
-        l_run = l_run * keep + sum;
-        if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+            float top = s[0];
 #pragma unroll
-            for (int db = 0; db < DB; db++) o[db] *= keep;
+            for (int x = 1; x < 8; x++) top = fmaxf(top, s[x]);
+#pragma unroll
+            for (int d = 16; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
+            const bool moved = less(top, m_run[t]) > (H16 ? 8.0f : 0.0f);
+            const float m_new = moved ? top : m_run[t], ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float keep = moved ? __builtin_amdgcn_exp2f(m_run[t] - ref) : 1.0f;
+            m_run[t] = m_new;
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                e[t][x] = __builtin_amdgcn_exp2f(less(s[x], ref));
+                // The product with V takes f16 operands: weights are rounded, half a step each, and the row's sum takes the same ones, so that
+                // a row of equal values stays that value.
+                if constexpr (H16) {
+                    pf[t][x] = (_Float16)e[t][x];
+                    e[t][x] = (float)pf[t][x];
+                }
+                sum += e[t][x];
+            }
+            l_run[t] = l_run[t] * keep + sum;
+            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+                for (int db = 0; db < DB; db++) o[t][db] *= keep;
+            }
         }
 
         // ---- O^T += V^T P^T --------------------------------------------------------------------------------
@@ -391,13 +413,18 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
 #pragma unroll
             for (int db = 0; db < DB; db++) {
                 const half4_t lo = lds_read_tr16(vsrc + 16 * db), hi = lds_read_tr16(vsrc + 16 * VROW + 16 * db);
-                o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf, o[db], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < RT; t++) o[t][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[t], o[t][db], 0, 0, 0);
             }
         } else {
 #pragma unroll
             for (int x = 0; x < 8; x++)
 #pragma unroll
-                for (int db = 0; db < DB; db++) o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(lds_v[(key_of(x) + 4 * grp) * VROW + 16 * db + lr], s[x], o[db], 0, 0, 0);
+                for (int db = 0; db < DB; db++) {
+                    const float v = lds_v[(key_of(x) + 4 * grp) * VROW + 16 * db + lr];
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, e[t][x], o[t][db], 0, 0, 0);
+                }
         }
         wave_sync();   // (the next tile goes where this one was)
         there = there_next;
@@ -405,47 +432,51 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
 
     // ---- the four waves' results joined ------------------------------------------------------------------------
     float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + kWaves * kRows * CROW;
-#pragma unroll
-    for (int d = 16; d < 64; d <<= 1) l_run += __shfl_xor(l_run, d, 64);
-    __syncthreads();   // the tiles are done with
-#pragma unroll
-    for (int db = 0; db < DB; db++) *reinterpret_cast<float4_t *>(comb + (w * kRows + lr) * CROW + 16 * db + 4 * grp) = o[db];
-    if (grp < 2) comb_ml[(w * 2 + grp) * kRows + lr] = grp ? l_run : m_run;
-    __syncthreads();
     constexpr int TPR = kThreads / kRows, PER = D / TPR;   // threads per row, features per thread
     const int row = tid / TPR;
-    if (row < u.rows) {
-        float mm = -INFINITY, l = 0.0f, f[kWaves];
 #pragma unroll
-        for (int x = 0; x < kWaves; x++) mm = fmaxf(mm, comb_ml[x * 2 * kRows + row]);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
+    for (int t = 0; t < RT; t++) {
 #pragma unroll
-        for (int x = 0; x < kWaves; x++) {
-            f[x] = __builtin_amdgcn_exp2f(comb_ml[x * 2 * kRows + row] - ref);
-            l += f[x] * comb_ml[(x * 2 + 1) * kRows + row];
-        }
-        Arguments p = arguments_again();
-        const int64_t orow = q_row(p, u.b, u.kvh, u.row0 + row).at;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int d = 16; d < 64; d <<= 1) l_run[t] += __shfl_xor(l_run[t], d, 64);
+        __syncthreads();   // the tiles, or the last rows, are done with
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) {
-            const int d = (tid % TPR) * 2 + e * TPR;   // (8 bytes per thread, threads of a row side by side: a store covers whole lines)
-            float2_t sum = {0.0f, 0.0f};
+        for (int db = 0; db < DB; db++) *reinterpret_cast<float4_t *>(comb + (w * kRows + lr) * CROW + 16 * db + 4 * grp) = o[t][db];
+        if (grp < 2) comb_ml[(w * 2 + grp) * kRows + lr] = grp ? l_run[t] : m_run[t];
+        __syncthreads();
+        if (16 * t + row < u.rows) {
+            float mm = -INFINITY, l = 0.0f, f[kWaves];
+#pragma unroll
+            for (int x = 0; x < kWaves; x++) mm = fmaxf(mm, comb_ml[x * 2 * kRows + row]);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
             for (int x = 0; x < kWaves; x++) {
-                const float2_t v = *reinterpret_cast<const float2_t *>(comb + (x * kRows + row) * CROW + d);
+                f[x] = __builtin_amdgcn_exp2f(comb_ml[x * 2 * kRows + row] - ref);
+                l += f[x] * comb_ml[(x * 2 + 1) * kRows + row];
+            }
+            Arguments p = arguments_again();
+            float *part = u.part + t * kLinePart(D);
+            const int64_t orow = q_row(p, u.b, u.kvh, u.row0 + 16 * t + row).at;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-                for (int y = 0; y < 2; y++) sum[y] = __builtin_fmaf(f[x], v[y], sum[y]);
+            for (int e = 0; e < PER; e += 2) {
+                const int d = (tid % TPR) * 2 + e * TPR;   // (8 bytes per thread, threads of a row side by side: a store covers whole lines)
+                float2_t sum = {0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < kWaves; x++) {
+                    const float2_t v = *reinterpret_cast<const float2_t *>(comb + (x * kRows + row) * CROW + d);
+#pragma unroll
+                    for (int y = 0; y < 2; y++) sum[y] = __builtin_fmaf(f[x], v[y], sum[y]);
+                }
+                if (!u.part) {
+                    struct alignas(2 * sizeof(T)) Two { T e[2]; } two;
+                    two.e[0] = (T)(sum[0] * inv), two.e[1] = (T)(sum[1] * inv);
+                    *reinterpret_cast<Two *>(reinterpret_cast<T *>(p.out) + orow * D + d) = two;
+                } else {
+                    put2(part + row * D + d, sum);
+                }
             }
-            if (!u.part) {
-                struct alignas(2 * sizeof(T)) Two { T e[2]; } two;
-                two.e[0] = (T)(sum[0] * inv), two.e[1] = (T)(sum[1] * inv);
-                *reinterpret_cast<Two *>(reinterpret_cast<T *>(p.out) + orow * D + d) = two;
-            } else {
-                put2(u.part + row * D + d, sum);
-            }
+            if (u.part && tid % TPR == 0) put(part + kRows * D + row, mm), put(part + kRows * D + kRows + row, l);
         }
-        if (u.part && tid % TPR == 0) put(u.part + kRows * D + row, mm), put(u.part + kRows * D + kRows + row, l);
     }
     __syncthreads();   // (the next stretch's tiles go where these rows were)
 }
@@ -453,12 +484,13 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
 // The parts of a unit -> its output.  Part x of [0, n) is at part_of(x).  Sixteen lanes take a row; where there are few rows, several groups
 // of lanes share a row's parts and are joined through LDS.
 template <typename T, int D, typename PartOf>
-__device__ __forceinline__ void join_unit(const Stretch &u, int n, PartOf part_of, unsigned char *lds) {
+__device__ __forceinline__ void join_unit(const Stretch &u, int tile, int n, PartOf part_of, unsigned char *lds) {
     constexpr int PER = D / 16, BATCH = 4, CROW = D + 4;
     const int tid = threadIdx.x, t = tid % 16, who = tid / 16;
+    const int rows = min(u.rows - 16 * tile, kRows);   // of this row tile
     int live = 1;
-    while (live < u.rows) live *= 2;
-    const int row = who & (live - 1), group = who / live, groups = 16 / live, at_row = min(row, u.rows - 1);
+    while (live < rows) live *= 2;
+    const int row = who & (live - 1), group = who / live, groups = 16 / live, at_row = min(row, rows - 1);
     float m_run = -INFINITY, l_run = 0.0f;
     float2_t acc[PER / 2];
 #pragma unroll
@@ -493,7 +525,7 @@ __device__ __forceinline__ void join_unit(const Stretch &u, int n, PartOf part_o
     for (int e = 0; e < PER / 2; e++) *reinterpret_cast<float2_t *>(comb + who * CROW + 2 * t + 32 * e) = acc[e];
     if (t == 0) comb_ml[2 * who] = m_run, comb_ml[2 * who + 1] = l_run;
     __syncthreads();
-    if (who < u.rows) {   // (who == row of group 0)
+    if (who < rows) {   // (who == row of group 0)
         float mm = -INFINITY, l = 0.0f;
         for (int g = 0; g < groups; g++) mm = fmaxf(mm, comb_ml[2 * (g * live + who)]);
         const float ref = mm == -INFINITY ? 0.0f : mm;
@@ -515,7 +547,7 @@ __device__ __forceinline__ void join_unit(const Stretch &u, int n, PartOf part_o
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         Arguments p = arguments_again();
-        T *out = reinterpret_cast<T *>(p.out) + q_row(p, u.b, u.kvh, u.row0 + who).at * D;
+        T *out = reinterpret_cast<T *>(p.out) + q_row(p, u.b, u.kvh, u.row0 + 16 * tile + who).at * D;
 #pragma unroll
         for (int e = 0; e < PER / 2; e++) {
             struct alignas(2 * sizeof(T)) Two { T e[2]; } two;
@@ -525,8 +557,6 @@ __device__ __forceinline__ void join_unit(const Stretch &u, int n, PartOf part_o
     }
     __syncthreads();
 }
-
-constexpr int kLeast = 4;   // tiles of a stretch at least: one a wave (8: 10.4 for 9.9 us of one token behind 777, 16: 12.6)
 
 // Whether a sequence begins with its neighbour's page, as beams of a request do.  Pages that one workgroup reads go past the caches (64 sequences
 // of 64 to 8192 keys 195 us, through them 217; 8 x 1000 13.0 | 13.5), those that several do through them (32 requests of 8 beams over 700 common
@@ -550,30 +580,30 @@ __device__ __forceinline__ int wave_sums(int x) {
     return x;
 }
 
-template <typename T, int D>
+template <typename T, int D, int RT>
 __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
     __shared__ int s_sums[kWaves], s_totals[kWaves];
     // (what is looked at between stretches alone is in LDS: the loop needs the scalar registers)
-    __shared__ struct { int per, at, end, b, unit, len, tiles, first, once; } s_line;
+    __shared__ struct { int per, at, end, b, unit, len, steps, first, once; } s_line;
     __shared__ int s_last;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     {
         Arguments p = arguments_again();
         const int units = p.Hkv * p.row_tiles;   // of a sequence
         auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
-        auto tiles_of = [&](int len) { return max((len + kTile - 1) / kTile, 1); };   // (one for nothing: its rows are zeros)
+        auto steps_of = [&](int len) { return max((len + kStep - 1) / kStep, 1); };   // (one for nothing: its rows are zeros)
 
-        // the line's length (below 2^30: checked by the host), and this workgroup's stretch
-        int len = tid < p.B ? len_of(tid) : 0, mine = tid < p.B ? tiles_of(len) : 0, all = mine;
+        // the line's length (below 2^28: checked by the host), and this workgroup's stretch
+        int len = tid < p.B ? len_of(tid) : 0, mine = tid < p.B ? steps_of(len) : 0, all = mine;
         bool shares = tid < p.B && shares_pages(p, tid);
-        for (int b = tid + kThreads; b < p.B; b += kThreads) all += tiles_of(len_of(b));
+        for (int b = tid + kThreads; b < p.B; b += kThreads) all += steps_of(len_of(b));
         int up = wave_sums(mine);
         const int sum = p.B > kThreads ? wave_sums(all) : up;
         if (lane == 63) s_sums[w] = up, s_totals[w] = sum;
         __syncthreads();
         const int total = (s_totals[0] + s_totals[1] + s_totals[2] + s_totals[3]) * units;
-        const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), kLeast);
+        const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), 1);
         const int begin = blockIdx.x * per, end = min(begin + per, total);
         if (begin >= end) return;
         // the sequence where it begins
@@ -582,14 +612,14 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             for (int x = 0; x < w; x++) before += s_sums[x];
             const int from = (before + up - mine) * units;
             if (b0 + tid < p.B && from <= begin && begin < from + mine * units) {
-                s_line.b = b0 + tid, s_line.len = len, s_line.tiles = mine;
+                s_line.b = b0 + tid, s_line.len = len, s_line.steps = mine;
                 s_line.unit = (unsigned)(begin - from) / (unsigned)mine, s_line.first = (unsigned)(begin - from) % (unsigned)mine;
                 s_line.once = p.row_tiles == 1 && !shares;
             }
             carry += s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3];
             b0 += kThreads;
             if (b0 >= p.B || carry * units > begin) break;
-            len = b0 + tid < p.B ? len_of(b0 + tid) : 0, mine = b0 + tid < p.B ? tiles_of(len) : 0;
+            len = b0 + tid < p.B ? len_of(b0 + tid) : 0, mine = b0 + tid < p.B ? steps_of(len) : 0;
             shares = b0 + tid < p.B && shares_pages(p, b0 + tid);
             up = wave_sums(mine);
             __syncthreads();
@@ -603,19 +633,19 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         Stretch u;
         {
             Arguments p = arguments_again();
-            const int unit = uniform(s_line.unit), tiles = uniform(s_line.tiles);
+            const int unit = uniform(s_line.unit), steps = uniform(s_line.steps);
             u.b = uniform(s_line.b), u.len = uniform(s_line.len), u.first = uniform(s_line.first);
             u.kvh = divided(p.by_row_tiles, unit);
-            u.row0 = (unit - u.kvh * p.row_tiles) * kRows, u.rows = min(kRows, p.Sq * p.G - u.row0);
-            u.end = min(tiles, u.first + uniform(s_line.end) - uniform(s_line.at));
-            u.part = u.first == 0 && u.end == tiles ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * kLinePart(D);
+            u.row0 = (unit - u.kvh * p.row_tiles) * RT * kRows, u.rows = min(RT * kRows, p.Sq * p.G - u.row0);
+            u.end = min(steps, u.first + uniform(s_line.end) - uniform(s_line.at));
+            u.part = u.first == 0 && u.end == steps ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * (RT * kLinePart(D));
         }
-        if (uniform(s_line.once)) stretch_body<T, D, true>(u, lds);
-        else stretch_body<T, D, false>(u, lds);
+        if (uniform(s_line.once)) stretch_body<T, D, RT, true>(u, lds);
+        else stretch_body<T, D, RT, false>(u, lds);
         if (u.part) {
             Arguments p = arguments_again();
             const unsigned per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
-            const int first = (int)(unit_at / per), n = (int)((unit_at + uniform(s_line.tiles) - 1) / per) - first + 1;
+            const int first = (int)(unit_at / per), n = (int)((unit_at + uniform(s_line.steps) - 1) / per) - first + 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
             __syncthreads();                                     // ... and so have the whole workgroup's
             if (tid == 0) {
@@ -625,7 +655,9 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             }
             __syncthreads();
             float *parts = p.parts;
-            if (s_last) join_unit<T, D>(u, n, [&](int x) { return parts + (2 * (int64_t)(first + x) + (x == 0)) * kLinePart(D); }, lds);
+            if (s_last)
+                for (int y = 0; y < RT && 16 * y < u.rows; y++)
+                    join_unit<T, D>(u, y, n, [&](int x) { return parts + ((2 * (int64_t)(first + x) + (x == 0)) * RT + y) * kLinePart(D); }, lds);
         }
         if (uniform(s_line.at) + u.end - u.first >= uniform(s_line.end)) return;
         __syncthreads();   // (everybody has read where the line stands)
@@ -635,16 +667,16 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             if (++s_line.unit == p.Hkv * p.row_tiles) {
                 const int len = min(max(p.lens[u.b + 1], 0), p.most);
                 s_line.once = p.row_tiles == 1 && !shares_pages(p, u.b + 1);
-                s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.tiles = max((len + kTile - 1) / kTile, 1);
+                s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.steps = max((len + kStep - 1) / kStep, 1);
             }
         }
         __syncthreads();
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int RT>
 int launch_line(const PagedDev &p, int workgroups, hipStream_t s) {
-    sdpa_paged_kernel<T, D><<<dim3((unsigned)workgroups), kThreads, 0, s>>>(p);
+    sdpa_paged_kernel<T, D, RT><<<dim3((unsigned)workgroups), kThreads, 0, s>>>(p);
     TROCM_HIP(hipGetLastError());
     return 0;
 }
@@ -653,8 +685,11 @@ int line_workgroups() { return 2 * num_compute_units(); }
 
 }  // namespace
 
-size_t sdpa_paged_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t D) {
-    return kWsCounterBytes + (D == 64 || D == 128 ? (size_t)2 * line_workgroups() * kLinePart((int)D) * 4 : 0);
+// Row tiles of a unit: two share the keys that a workgroup reads.
+static int row_tiles_of_unit(int64_t rows, int64_t es, int64_t D) { return rows > kRows && !in_lds((int)es, (int)D) ? 2 : 1; }
+
+size_t sdpa_paged_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
+    return kWsCounterBytes + (D == 64 || D == 128 ? (size_t)2 * line_workgroups() * row_tiles_of_unit(Hq / Hkv * Sq, 2, D) * kLinePart((int)D) * 4 : 0);
 }
 
 int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
@@ -670,20 +705,29 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
     const uint64_t bits = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.out | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)p.stride_page | (uint64_t)p.stride_h | (uint64_t)p.stride_t;
     if ((a.D == 64 || a.D == 128) && a.page_size % 16 == 0 && bits % 16 == 0 && a.n_pages > 0 && p.stride_t < (1 << 27) && a.workspace &&
         a.workspace_bytes >= sdpa_paged_workspace_bytes(a.B, a.Hq, a.Hkv, a.Sq, a.D)) {
-        p.row_tiles = (int)((a.Hq / a.Hkv * a.Sq + kRows - 1) / kRows);
+        const int64_t rows = a.Hq / a.Hkv * a.Sq;
+        const int rt = row_tiles_of_unit(rows, es, a.D);
+        p.row_tiles = (int)((rows + rt * kRows - 1) / (rt * kRows));
         p.by_g = fast_div(p.G), p.by_row_tiles = fast_div(p.row_tiles), p.by_workgroups = fast_div(line_workgroups());
         p.counters = (int *)a.workspace, p.parts = (float *)((char *)a.workspace + kWsCounterBytes);
-        // a line of tiles is counted in 31 bits: as many sequences in a launch as cannot be more
-        const int64_t most_tiles = std::max<int64_t>((p.most + kTile - 1) / kTile, 1) * a.Hkv * p.row_tiles, seqs = (1 << 30) / most_tiles;
+        // a line's tiles are counted in 31 bits: as many sequences in a launch as cannot be more
+        const int64_t most_steps = std::max<int64_t>((p.most + kStep - 1) / kStep, 1) * a.Hkv * p.row_tiles, seqs = (1 << 28) / most_steps;
         if (seqs > 0) {
             for (int64_t b0 = 0; b0 < a.B; b0 += seqs) {
                 PagedDev part = p;
                 part.B = (int)std::min(seqs, a.B - b0);
                 part.q += b0 * a.Hq * a.Sq * a.D * es, part.out += b0 * a.Hq * a.Sq * a.D * es;
                 part.table += b0 * a.table_width, part.lens += b0;
-                const int rc = a.dtype == TROCM_F16 ? a.D == 64 ? launch_line<_Float16, 64>(part, line_workgroups(), s) : launch_line<_Float16, 128>(part, line_workgroups(), s)
-                               : a.D == 64          ? launch_line<float, 64>(part, line_workgroups(), s)
-                                                    : launch_line<float, 128>(part, line_workgroups(), s);
+                const int n = line_workgroups();
+                int rc;
+                if (a.dtype == TROCM_F16) {
+                    if (rt == 1) rc = a.D == 64 ? launch_line<_Float16, 64, 1>(part, n, s) : launch_line<_Float16, 128, 1>(part, n, s);
+                    else rc = a.D == 64 ? launch_line<_Float16, 64, 2>(part, n, s) : launch_line<_Float16, 128, 2>(part, n, s);
+                } else if (a.D == 64) {
+                    rc = rt == 1 ? launch_line<float, 64, 1>(part, n, s) : launch_line<float, 64, 2>(part, n, s);
+                } else {
+                    rc = launch_line<float, 128, 1>(part, n, s);
+                }
                 if (rc) return rc;
             }
             return 0;
