@@ -378,6 +378,17 @@ def test_shapes_and_types_are_refused(rt):
         plan.eval(n, n, t, ints([0] * 5), ints([5]), 2, refs=up(np.zeros(5, np.int64)))
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,hq,hkv,sq,causal", [(70, 16, 8, 9, True), (40, 24, 8, 14, True), (70, 24, 8, 12, False), (70, 16, 8, 40, True)])
+def test_attend_several_tiles_of_rows(rt, dtype, d, n, hq, hkv, sq, causal):
+    """17 to 32, 33 to 64 and more rows of a kv head, in so many sequences that units of the most row tiles, or half as many, fill the workgroups."""
+    rng = np.random.default_rng(n + sq)
+    lens = rng.integers(0, 60, n)
+    lens[:3] = 300, 0, 129
+    _attend(rng, lens, hq, hkv, sq, d, 16, dtype, causal=causal, holes=0.05)
+
+
 # ---- the far ends of what the calls allow -------------------------------------------------------------------------------------
 
 

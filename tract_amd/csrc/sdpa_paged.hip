@@ -38,10 +38,10 @@ struct PagedDev {
     int causal;
     FastDiv by_page;
     // tiles of 16 rows
-    int row_tiles;              // of a kv head
     int *counters;
     float *parts;
-    FastDiv by_g, by_row_tiles, by_workgroups;
+    FastDiv by_g, by_workgroups;
+    FastDiv row_units[3];       // by the units of a kv head's rows, where they take one, two and four tiles
 };
 
 __device__ __forceinline__ float widen(float x) { return x; }
@@ -580,17 +580,71 @@ __device__ __forceinline__ int wave_sums(int x) {
     return x;
 }
 
+// Where a workgroup stands on the line: what is looked at between stretches alone is in LDS, since the loop needs the scalar registers.
+struct Line { int per, at, end, b, unit, len, steps, first, once, last; };
+
+// A workgroup's stretch, unit by unit.
+template <typename T, int D, int RT, bool MAY_ONCE>
+__device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
+    const int tid = threadIdx.x;
+    for (;;) {
+        Stretch u;
+        {
+            Arguments p = arguments_again();
+            const int unit = uniform(s_line.unit), steps = uniform(s_line.steps);
+            u.b = uniform(s_line.b), u.len = uniform(s_line.len), u.first = uniform(s_line.first);
+            const auto &row_units = p.row_units[RT >> 1];
+            u.kvh = divided(row_units, unit);
+            u.row0 = (unit - u.kvh * (int)row_units.d) * RT * kRows, u.rows = min(RT * kRows, p.Sq * p.G - u.row0);
+            u.end = min(steps, u.first + uniform(s_line.end) - uniform(s_line.at));
+            u.part = u.first == 0 && u.end == steps ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * (RT * kLinePart(D));
+        }
+        if (MAY_ONCE && uniform(s_line.once)) stretch_body<T, D, RT, MAY_ONCE>(u, lds);
+        else stretch_body<T, D, RT, false>(u, lds);
+        if (u.part) {
+            Arguments p = arguments_again();
+            const unsigned per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
+            const int first = (int)(unit_at / per), n = (int)((unit_at + uniform(s_line.steps) - 1) / per) - first + 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
+            __syncthreads();                                     // ... and so have the whole workgroup's
+            if (tid == 0) {
+                int *counter = p.counters + first;   // (a workgroup cuts one unit at most at its end)
+                s_line.last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+                if (s_line.last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            float *parts = p.parts;
+            if (s_line.last)
+                for (int y = 0; y < RT && 16 * y < u.rows; y++)
+                    join_unit<T, D>(u, y, n, [&](int x) { return parts + ((2 * (int64_t)(first + x) + (x == 0)) * RT + y) * kLinePart(D); }, lds);
+        }
+        if (uniform(s_line.at) + u.end - u.first >= uniform(s_line.end)) return;
+        __syncthreads();   // (everybody has read where the line stands)
+        if (tid == 0) {
+            Arguments p = arguments_again();
+            s_line.at += u.end - u.first, s_line.first = 0;
+            if (++s_line.unit == p.Hkv * (int)p.row_units[RT >> 1].d) {
+                const int len = min(max(p.lens[u.b + 1], 0), p.most);
+                s_line.once = p.row_units[RT >> 1].d == 1 && !shares_pages(p, u.b + 1);
+                s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.steps = max((len + kStep - 1) / kStep, 1);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// RT: row tiles of a unit, which share the keys that it reads.  Where that leaves no more steps than workgroups, units take half as many, and
+// again: what a workgroup does for one tile after the other is then what takes the time (2 sequences of up to 300 keys, 7 heads' 5 queries
+// 12.9 us with four tiles, 7.8 with one).
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
     __shared__ int s_sums[kWaves], s_totals[kWaves];
-    // (what is looked at between stretches alone is in LDS: the loop needs the scalar registers)
-    __shared__ struct { int per, at, end, b, unit, len, steps, first, once; } s_line;
-    __shared__ int s_last;
+    __shared__ Line s_line;
+    int rt = RT;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     {
         Arguments p = arguments_again();
-        const int units = p.Hkv * p.row_tiles;   // of a sequence
         auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
         auto steps_of = [&](int len) { return max((len + kStep - 1) / kStep, 1); };   // (one for nothing: its rows are zeros)
 
@@ -602,7 +656,10 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         const int sum = p.B > kThreads ? wave_sums(all) : up;
         if (lane == 63) s_sums[w] = up, s_totals[w] = sum;
         __syncthreads();
-        const int total = (s_totals[0] + s_totals[1] + s_totals[2] + s_totals[3]) * units;
+        const int all_steps = s_totals[0] + s_totals[1] + s_totals[2] + s_totals[3];   // of one unit of every sequence
+        auto units_of = [&](int rt) { return p.Hkv * (int)p.row_units[rt >> 1].d; };   // of a sequence
+        while (rt > 1 && all_steps * units_of(rt) <= (int)gridDim.x) rt >>= 1;
+        const int units = units_of(rt), total = all_steps * units;
         const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), 1);
         const int begin = blockIdx.x * per, end = min(begin + per, total);
         if (begin >= end) return;
@@ -614,7 +671,7 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             if (b0 + tid < p.B && from <= begin && begin < from + mine * units) {
                 s_line.b = b0 + tid, s_line.len = len, s_line.steps = mine;
                 s_line.unit = (unsigned)(begin - from) / (unsigned)mine, s_line.first = (unsigned)(begin - from) % (unsigned)mine;
-                s_line.once = p.row_tiles == 1 && !shares;
+                s_line.once = units == p.Hkv && !shares;
             }
             carry += s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3];
             b0 += kThreads;
@@ -629,49 +686,10 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         if (tid == 0) s_line.per = per, s_line.at = begin, s_line.end = end;
         __syncthreads();
     }
-    for (;;) {
-        Stretch u;
-        {
-            Arguments p = arguments_again();
-            const int unit = uniform(s_line.unit), steps = uniform(s_line.steps);
-            u.b = uniform(s_line.b), u.len = uniform(s_line.len), u.first = uniform(s_line.first);
-            u.kvh = divided(p.by_row_tiles, unit);
-            u.row0 = (unit - u.kvh * p.row_tiles) * RT * kRows, u.rows = min(RT * kRows, p.Sq * p.G - u.row0);
-            u.end = min(steps, u.first + uniform(s_line.end) - uniform(s_line.at));
-            u.part = u.first == 0 && u.end == steps ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * (RT * kLinePart(D));
-        }
-        if (uniform(s_line.once)) stretch_body<T, D, RT, true>(u, lds);
-        else stretch_body<T, D, RT, false>(u, lds);
-        if (u.part) {
-            Arguments p = arguments_again();
-            const unsigned per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
-            const int first = (int)(unit_at / per), n = (int)((unit_at + uniform(s_line.steps) - 1) / per) - first + 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this thread's parts have completed
-            __syncthreads();                                     // ... and so have the whole workgroup's
-            if (tid == 0) {
-                int *counter = p.counters + first;   // (a workgroup cuts one unit at most at its end)
-                s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-                if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            __syncthreads();
-            float *parts = p.parts;
-            if (s_last)
-                for (int y = 0; y < RT && 16 * y < u.rows; y++)
-                    join_unit<T, D>(u, y, n, [&](int x) { return parts + ((2 * (int64_t)(first + x) + (x == 0)) * RT + y) * kLinePart(D); }, lds);
-        }
-        if (uniform(s_line.at) + u.end - u.first >= uniform(s_line.end)) return;
-        __syncthreads();   // (everybody has read where the line stands)
-        if (tid == 0) {
-            Arguments p = arguments_again();
-            s_line.at += u.end - u.first, s_line.first = 0;
-            if (++s_line.unit == p.Hkv * p.row_tiles) {
-                const int len = min(max(p.lens[u.b + 1], 0), p.most);
-                s_line.once = p.row_tiles == 1 && !shares_pages(p, u.b + 1);
-                s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.steps = max((len + kStep - 1) / kStep, 1);
-            }
-        }
-        __syncthreads();
-    }
+    if (rt == RT) return walk_line<T, D, RT, true>(s_line, lds);
+    if constexpr (RT > 2)
+        if (rt == 2) return walk_line<T, D, 2, false>(s_line, lds);
+    if constexpr (RT > 1) walk_line<T, D, 1, false>(s_line, lds);
 }
 
 template <typename T, int D, int RT>
@@ -685,8 +703,12 @@ int line_workgroups() { return 2 * num_compute_units(); }
 
 }  // namespace
 
-// Row tiles of a unit: two share the keys that a workgroup reads.
-static int row_tiles_of_unit(int64_t rows, int64_t es, int64_t D) { return rows > kRows && !in_lds((int)es, (int)D) ? 2 : 1; }
+// Row tiles of a unit, at most: as many as a lane's registers hold (f32 of head size 128 has no place for two rows' queries in LDS either).  91
+// sequences of 2880 to 5761 keys: 8 heads' 5 queries of head size 64 in four tiles 172 us, in two 300; 4 heads' 5 of 128 in two 275, in one 561.
+static int row_tiles_of_unit(int64_t rows, int64_t es, int64_t D) {
+    if (rows <= kRows || in_lds((int)es, (int)D)) return 1;
+    return rows > 2 * kRows && es == 2 && D == 64 ? 4 : 2;
+}
 
 size_t sdpa_paged_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
     return kWsCounterBytes + (D == 64 || D == 128 ? (size_t)2 * line_workgroups() * row_tiles_of_unit(Hq / Hkv * Sq, 2, D) * kLinePart((int)D) * 4 : 0);
@@ -707,11 +729,11 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
         a.workspace_bytes >= sdpa_paged_workspace_bytes(a.B, a.Hq, a.Hkv, a.Sq, a.D)) {
         const int64_t rows = a.Hq / a.Hkv * a.Sq;
         const int rt = row_tiles_of_unit(rows, es, a.D);
-        p.row_tiles = (int)((rows + rt * kRows - 1) / (rt * kRows));
-        p.by_g = fast_div(p.G), p.by_row_tiles = fast_div(p.row_tiles), p.by_workgroups = fast_div(line_workgroups());
+        for (int i = 0; i < 3; i++) p.row_units[i] = fast_div((rows + (kRows << i) - 1) / (kRows << i));
+        p.by_g = fast_div(p.G), p.by_workgroups = fast_div(line_workgroups());
         p.counters = (int *)a.workspace, p.parts = (float *)((char *)a.workspace + kWsCounterBytes);
         // a line's tiles are counted in 31 bits: as many sequences in a launch as cannot be more
-        const int64_t most_steps = std::max<int64_t>((p.most + kStep - 1) / kStep, 1) * a.Hkv * p.row_tiles, seqs = (1 << 28) / most_steps;
+        const int64_t most_steps = std::max<int64_t>((p.most + kStep - 1) / kStep, 1) * a.Hkv * p.row_units[rt >> 1].d, seqs = (1 << 28) / most_steps;
         if (seqs > 0) {
             for (int64_t b0 = 0; b0 < a.B; b0 += seqs) {
                 PagedDev part = p;
@@ -721,7 +743,8 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
                 const int n = line_workgroups();
                 int rc;
                 if (a.dtype == TROCM_F16) {
-                    if (rt == 1) rc = a.D == 64 ? launch_line<_Float16, 64, 1>(part, n, s) : launch_line<_Float16, 128, 1>(part, n, s);
+                    if (rt == 4) rc = launch_line<_Float16, 64, 4>(part, n, s);
+                    else if (rt == 1) rc = a.D == 64 ? launch_line<_Float16, 64, 1>(part, n, s) : launch_line<_Float16, 128, 1>(part, n, s);
                     else rc = a.D == 64 ? launch_line<_Float16, 64, 2>(part, n, s) : launch_line<_Float16, 128, 2>(part, n, s);
                 } else if (a.D == 64) {
                     rc = rt == 1 ? launch_line<float, 64, 1>(part, n, s) : launch_line<float, 64, 2>(part, n, s);
