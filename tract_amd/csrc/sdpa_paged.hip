@@ -2,12 +2,20 @@
 // pages anywhere, found through a table, and whose lengths are read from device memory.  f16 and f32.
 //
 // The query rows of a kv head (heads of the group, queries) are rows of matrix tiles, S^T = K Q^T and O^T = V^T P^T, so that every softmax
-// scalar of a row sits in one lane.  A tile is 32 keys: two halves of 16 that lie in a page each (pages are multiples of 16 tokens).
+// scalar of a row sits in one lane.  A tile is 32 keys: two halves of 16 that lie in a page each (pages are multiples of 16 tokens).  One
+// pass over the keys, with the running maximum m and sum l of every row: o <- o 2^(m - m') + 2^(s - m') v, f32.
 //
-// The host does not know the lengths, so the work is shared out on the device: all units (sequence, kv head, 16 rows) one behind the other
-// are a line of tiles, and every workgroup takes a stretch of it, all of the same length.  A unit inside of a stretch goes straight to the
-// output; one that a stretch's end cuts goes to the workspace in parts (unnormalised O, maximum, sum, f32), which the last workgroup to
-// arrive joins, always in the same order.
+// The host does not know the lengths, so the work is shared out on the device: all units (sequence, kv head, up to four tiles of 16 rows) one
+// behind the other are a line of steps of 128 keys, a tile for each of a workgroup's waves, and every workgroup takes a stretch of the line,
+// all of the same length.  A unit inside of a stretch goes straight to the output; one that a stretch's end cuts goes to the workspace in
+// parts (unnormalised O, maximum, sum, f32), which the last workgroup to arrive joins, always in the same order.  Two workgroups a compute
+// unit, whose rows of the next tile are on their way while one is worked on (1, 3, 4 and 8 were slower).  A line counted in tiles, whose
+// stretches began anywhere, left waves of a step without a tile and put short sequences behind one another (64 sequences of up to 8192 keys
+// 195 us for 190.5, one token behind 777 10.4 for 7.6, 9 sequences of up to 120 in f32 23.9 for 10.2).
+//
+// What bounds it: the pages' bytes where there are many (64 sequences of 64 to 8192 keys of 8 x 128, f16, 1.18 GB: 190.5 us, 6.2 TB/s; 3
+// queries behind 90000 and 100001 keys 137.6 us, 5.7 TB/s; 16 sequences of up to 3000 keys of 32 x 64, f32, 80.9 us, 5.2 TB/s), matrix
+// instructions busy for 4 to 34 % of the SIMDs' cycles; the chain lengths - table - keys - join where there are few (7.6 us).
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
