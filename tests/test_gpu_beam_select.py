@@ -160,3 +160,26 @@ def test_keep_that_changes_from_call_to_call(rt):
         got, want = op.eval(up(logits), up(scores)), ref.select(logits, scores, keep)
         for name in ("parents", "tokens"):
             np.testing.assert_array_equal(got[name].to_numpy(), want[name])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("batch,beams,vocab,keep", [(1, 8, 40000, 16), (1, 2, 128256, 64), (2, 64, 9000, 64), (1, 40, 16385, 3), (3, 8, 50257, 16)])
+def test_more_candidates_than_a_workgroup_holds(rt, dtype, batch, beams, vocab, keep):
+    """Parts of a request whose candidates are looked at by their best ones first: scores alike, far apart (one beam has all of the choice), of beams
+    that have ended or are gone, and rows sorted both ways, equal throughout or with few numbers."""
+    rng = np.random.default_rng(vocab + keep)
+    logits = (rng.standard_normal((batch, beams, vocab)) * 3).astype(dtype)
+    near, far = (-rng.random((batch, beams))).astype(F32), (-200.0 * rng.random((batch, beams))).astype(F32)
+    _check(logits, near, keep)
+    _check(logits, far, keep)
+    ended = (rng.random((batch, beams)) < 0.5).astype(I32)
+    gone = near.copy()
+    gone[:, 1] = -np.inf
+    _check(logits, gone, keep, ended, vocab - 1)
+    _check(np.sort(logits, axis=-1), near, keep)
+    _check(-np.sort(logits, axis=-1), far, keep)
+    _check(np.zeros_like(logits), near, keep)
+    _check(np.zeros_like(logits), np.zeros_like(near), keep)
+    few = np.full_like(logits, -np.inf)
+    few[..., ::vocab // 3] = logits[..., ::vocab // 3]
+    _check(few, near, keep)

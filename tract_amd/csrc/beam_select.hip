@@ -9,9 +9,9 @@
 // The largest of a wave's values: the K-th largest of its lanes' maxima is found, nearly, by bisection over the upper bits of an order-preserving
 // integer (ballots and counts); at least K values reach it, and few more than that, which are listed in LDS and ranked by counting.
 //
-// What bounds it: one request (4 beams of 32000, f32) is a chain of stages, 10.1 us; 32 requests of 8 beams of 128256 in f16 take 33 us, of
+// What bounds it: one request (4 beams of 32000, f32) is a chain of stages, 10.1 us; 32 requests of 8 beams of 128256 in f16 take 30.6 us, of
 // which the stream of the rows takes 13.4 (4.9 TB/s; the vector ALUs are busy for half of it, exponentials for most), what a workgroup does
-// behind its stream 4.6 and the last workgroups' joins 6, with nothing left to overlap them with.
+// behind its stream 4.6 and the last workgroups' joins 5, with nothing left to overlap them with.
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
@@ -41,7 +41,7 @@ struct SelectDev {
     const int *ended;
     float *scores_out;
     int *parents, *tokens, *ended_out;
-    FastDiv by_parts, by_row_candidates, by_beams;
+    FastDiv by_parts, by_row_candidates, by_keep, by_beams;
 };
 
 // Integers in the order of the numbers; both zeros are one number and NaN counts as -inf.
@@ -344,7 +344,7 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
 
 // ---- parts and beams put together: the last workgroup of a request ----------------------------------------------------------
 
-constexpr int kJoinList = 1024;
+constexpr int kJoinList = 1024, kJoinParts = 1024;   // parts of a request: checked by the host
 struct alignas(16) Choice { double c; int place, beam; };   // place: beam * vocab + token (below 2^31, checked by the host); < 0: none
 
 __device__ __forceinline__ bool before(double c, int place, double d, int other) { return c > d || (c == d && place < other); }
@@ -395,20 +395,40 @@ struct JoinLds {
     uint64_t sums[kWaves];
     float max[kBeamMaxBeams];
     int kind[kBeamMaxBeams], ended[kBeamMaxBeams];   // kind 0: goes on, 1: stays at the token of the ended, 2: has no candidates but of -inf
+    int part[kJoinParts], parts;
     int again[kBeamMaxBeams], any, count, best_place[kWaves], best_beam[kWaves];
     uint32_t bound[kWaves];
 };
 
+// A kernel's one argument where it lies, as loads from here on: kept from the beginning, what only the end looks at would leave too few scalar
+// registers for what is between.
+template <typename Args>
+__device__ __forceinline__ const __attribute__((address_space(4))) Args &arguments_again() {
+    auto at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(at));
+    return *reinterpret_cast<const __attribute__((address_space(4))) Args *>(at);
+}
+
 template <typename T>
 __device__ __forceinline__ void join_request(const __attribute__((address_space(4))) SelectDev &p, int request, JoinLds &lds) {
-    const FastDiv by_row_candidates = {p.by_row_candidates.d, p.by_row_candidates.mul, p.by_row_candidates.shift};
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int per_row = p.parts * p.keep, n = p.beams * per_row;
     const Candidate *all = p.part_best + (int64_t)request * n;
-    constexpr int kHeld = 2;   // candidates that a thread asks for ahead of all, and keeps
+    // What a thread asks for ahead of all, and keeps: candidates, or, where those are more, the best one of every part; of those parts that reach
+    // the bound the others are looked at later (8 beams of 128256, f16, in 63 parts each of which 16 are kept: 21.5 us, 48.5 with all 8064 looked
+    // at twice).
+    constexpr int kHeld = 2;
+    const bool few = n <= kHeld * kThreads;
+    // (the argument is read again wherever it is looked at: kept, it takes scalar registers that are not there)
+    auto beam_of = [](const __attribute__((address_space(4))) SelectDev &p, int j) { return FastDiv{p.by_row_candidates.d, p.by_row_candidates.mul, p.by_row_candidates.shift}.by(j); };
     Candidate first_of[kHeld];
+    int held_beam[kHeld], held_k[kHeld];   // beam < 0: none
 #pragma unroll
-    for (int y = 0; y < kHeld; y++) first_of[y] = tid + y * kThreads < n ? get(all + tid + y * kThreads) : Candidate{-INFINITY, -1};
+    for (int y = 0; y < kHeld; y++) {
+        const int i = tid + y * kThreads, j = i * (few ? 1 : p.keep);
+        first_of[y] = j < n ? get(all + j) : Candidate{-INFINITY, -1};
+        held_beam[y] = j < n ? beam_of(p, j) : -1, held_k[y] = j - held_beam[y] * per_row;
+    }
     constexpr int kLanes = 16;   // of a beam
     for (int beam = tid / kLanes; beam < p.beams; beam += kThreads / kLanes) {
         const int64_t row = (int64_t)request * p.beams + beam;
@@ -454,8 +474,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
     if (tid == 0) lds.any = 0;
     __syncthreads();
 
-    auto choice = [&](int j, const Candidate &c) {
-        const int beam = by_row_candidates.by(j), k = j - beam * per_row;
+    auto choice = [&](int beam, int k, const Candidate &c) {   // k: which one of the beam
         Choice r = {-INFINITY, -1, beam};
         if (lds.kind[beam] == 0) {
             if (c.token >= 0) r.c = lds.score[beam] + ((double)c.x - lds.lse[beam]), r.place = beam * p.vocab + c.token;
@@ -467,8 +486,13 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         }
         return r;
     };
-    auto candidate = [&](int j) { return choice(j, get(all + j)); };
+    auto candidate = [&](int j) {
+        const auto &p = arguments_again<SelectDev>();
+        const int beam = beam_of(p, j);
+        return choice(beam, j - beam * (p.parts * p.keep), get(p.part_best + (int64_t)request * (p.beams * p.parts * p.keep) + j));
+    };
     auto chosen = [&](int rank, double c, int place, int beam) {
+        const auto &p = arguments_again<SelectDev>();
         const int token = place - beam * p.vocab;
         const int64_t at = (int64_t)request * p.keep + rank;
         p.scores_out[at] = (float)c;
@@ -481,27 +505,33 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
     for (int again = 0;; again++) {
         // at least `keep` of a wave's candidates reach its bound (of f32, whose order is that of f64 but for ties), so the largest bound will
         // do; all that could be among the best are listed
+        int tid = threadIdx.x;
+        asm("" : "+v"(tid));   // (comparisons again: kept, they take scalar registers)
+        const int lane = tid & 63;
         Choice held[kHeld];
         uint32_t top = 0;
 #pragma unroll
         for (int y = 0; y < kHeld; y++) {
-            const int j = tid + y * kThreads;
-            held[y] = j < n ? choice(j, first_of[y]) : Choice{-INFINITY, -1, 0};
+            held[y] = held_beam[y] >= 0 ? choice(held_beam[y], held_k[y], first_of[y]) : Choice{-INFINITY, -1, 0};
             if (held[y].place >= 0) top = max(top, key_of((float)held[y].c));
         }
-        for (int j = tid + kHeld * kThreads; j < n; j += kThreads) {
-            const Choice r = candidate(j);
+        const int bests = few ? 0 : p.beams * p.parts;
+        for (int i = tid + kHeld * kThreads; i < bests; i += kThreads) {
+            const Choice r = candidate(i * p.keep);
             if (r.place >= 0) top = max(top, key_of((float)r.c));
         }
         const uint32_t wave_bound = bound_of_lanes(top, p.keep);
         __syncthreads();   // (what the last turn has listed is done with)
         if (lane == 0) lds.bound[w] = wave_bound;
-        if (tid == 0) lds.count = 0;
+        if (tid == 0) lds.count = lds.parts = 0;
         __syncthreads();
-        const float bound = value_of(max(max(max(lds.bound[0], lds.bound[1]), max(lds.bound[2], lds.bound[3])), kLowest));
-        const double from = (double)bound - 0x1p-23 * fabs((double)bound) - 0x1p-149 - 2.0 * err;   // (-inf stays that)
+        auto bound_of_waves = [&] { return value_of(max(max(max(lds.bound[0], lds.bound[1]), max(lds.bound[2], lds.bound[3])), kLowest)); };
+        auto from_of = [&](float b) { return (double)b - 0x1p-23 * fabs((double)b) - 0x1p-149 - 2.0 * err; };   // (-inf stays that)
+        float bound = bound_of_waves();
+        double from = from_of(bound);
+        auto reaches = [&](const Choice &r) { return r.place >= 0 && (r.c >= from || bound == -INFINITY); };
         auto add = [&](const Choice &r) __attribute__((always_inline)) {
-            const bool in = r.place >= 0 && (r.c >= from || bound == -INFINITY);
+            const bool in = reaches(r);
             const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
             if (lanes) {
                 int at = 0;
@@ -510,14 +540,53 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
                 if (in && at < kJoinList) lds.c[at] = r.c, lds.at[at] = make_int2(r.place, r.beam);
             }
         };
+        if (few) {
 #pragma unroll
-        for (int y = 0; y < kHeld; y++) add(held[y]);
-        for (int j0 = kHeld * kThreads; j0 < n; j0 += kThreads) add(j0 + tid < n ? candidate(j0 + tid) : Choice{-INFINITY, -1, 0});
+            for (int y = 0; y < kHeld; y++) add(held[y]);
+        } else {
+#pragma unroll
+            for (int y = 0; y < kHeld; y++)
+                if (reaches(held[y])) lds.part[atomicAdd(&lds.parts, 1)] = tid + y * kThreads;
+            for (int i = tid + kHeld * kThreads; i < bests; i += kThreads)
+                if (reaches(candidate(i * p.keep))) lds.part[atomicAdd(&lds.parts, 1)] = i;
+            __syncthreads();
+            constexpr int kDeep = 4;
+            const auto &p = arguments_again<SelectDev>();
+            const FastDiv by_keep = {p.by_keep.d, p.by_keep.mul, p.by_keep.shift};
+            const int there = lds.parts * p.keep;
+            for (int x0 = 0; x0 < there; x0 += kDeep * kThreads) {
+                int j[kDeep];
+                Candidate c[kDeep];
+#pragma unroll
+                for (int y = 0; y < kDeep; y++) {
+                    const int x = x0 + y * kThreads + tid, i = by_keep.by(min(x, there - 1));
+                    j[y] = x < there ? lds.part[i] * p.keep + x - i * p.keep : -1;
+                    c[y] = get(p.part_best + (int64_t)request * (p.beams * p.parts * p.keep) + max(j[y], 0));
+                }
+                // (best ones alone make a low bound where one beam has most of what is chosen: again, of these)
+                Choice r[kDeep];
+                uint32_t top = 0;
+#pragma unroll
+                for (int y = 0; y < kDeep; y++) {
+                    const int beam = beam_of(p, max(j[y], 0));
+                    r[y] = j[y] >= 0 ? choice(beam, j[y] - beam * (p.parts * p.keep), c[y]) : Choice{-INFINITY, -1, 0};
+                    if (r[y].place >= 0) top = max(top, key_of((float)r[y].c));
+                }
+                const uint32_t wave_bound = bound_of_lanes(top, p.keep);
+                if (lane == 0) lds.bound[w] = wave_bound;
+                __syncthreads();
+                bound = fmaxf(bound, bound_of_waves()), from = from_of(bound);
+#pragma unroll
+                for (int y = 0; y < kDeep; y++) add(r[y]);
+                __syncthreads();
+            }
+        }
         __syncthreads();
         const int listed = min(lds.count, kJoinList);
         const bool whole = lds.count <= kJoinList;
         // Every listed value counts those before it; a value that is nearer to another beam's than sums of 32-bit terms tell apart asks for
-        // both beams' sums to be made again.
+        // both beams' sums to be made again.  Equal values are common (f16: steps of 2^-7 at 10): up to two near ones are looked at without
+        // another pass over the list (32 x 8 beams of 128256 32.8 us with one, 30.6 without).
         constexpr int kMine = kJoinList / kThreads;
         int rank[kMine];
 #pragma unroll
@@ -526,20 +595,27 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             rank[y] = p.keep;
             if (!whole || j >= listed) continue;
             const double c = lds.c[j];
-            int r = 0, near = 0;
-#pragma unroll 8
+            int r = 0, near = 0, one = j, two = j;   // near: others; the last two of them
+#pragma unroll 4
             for (int o = 0; o < listed; o++) {
                 const double d = lds.c[o];
+                const bool is_near = !(fabs(d - c) > 2.0 * err) && o != j;   // (two of -inf are)
                 r += d > c ? 1 : 0;
-                near += !(fabs(d - c) > 2.0 * err) ? 1 : 0;   // (itself, and two of -inf)
+                near += is_near ? 1 : 0;
+                two = is_near ? one : two, one = is_near ? o : one;
             }
-            if (near > 1 && r < p.keep) {
+            if (near > 0 && r < p.keep) {
                 const int2 mine = lds.at[j];
-                for (int o = 0; o < listed; o++) {
+                auto look = [&](int o) {
                     const int2 other = lds.at[o];
                     const double d = lds.c[o], off = lds.err[mine.y] + lds.err[other.y];
                     r += d == c && other.x < mine.x ? 1 : 0;
                     if (again == 0 && other.y != mine.y && off > 0.0 && fabs(d - c) <= off) lds.again[mine.y] = lds.again[other.y] = 1, lds.any = 1;
+                };
+                if (near <= 2) {   // (itself in place of one that is not there)
+                    look(one), look(two);
+                } else {
+                    for (int o = 0; o < listed; o++) look(o);
                 }
             }
             rank[y] = r;
@@ -553,6 +629,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             if (lds.any) {
                 for (int beam = 0; beam < p.beams; beam++)
                     if (lds.again[beam] && lds.kind[beam] == 0) {
+                        const auto &p = arguments_again<SelectDev>();
                         const double lse = exact_lse(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, lds.max[beam], lds.sums);
                         if (tid == 0) lds.lse[beam] = lse;
                     }
@@ -572,11 +649,13 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         break;
     }
     // more than the list holds (equal values above all): one after the other
+    const auto &q = arguments_again<SelectDev>();
+    const int all_there = q.beams * q.parts * q.keep;
     double last_c = INFINITY;
     int last_place = -1;
-    for (int rank = 0; rank < p.keep; rank++) {
+    for (int rank = 0; rank < q.keep; rank++) {
         Choice best = {-INFINITY, -1, 0};
-        for (int j = tid; j < n; j += kThreads) {
+        for (int j = tid; j < all_there; j += kThreads) {
             const Choice r = candidate(j);
             if (r.place >= 0 && before(last_c, last_place, r.c, r.place) && (best.place < 0 || before(r.c, r.place, best.c, best.place))) best = r;
         }
@@ -597,15 +676,6 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
     }
 }
 
-// A kernel's one argument where it lies, as loads from here on: kept from the beginning, what only the end looks at would leave too few scalar
-// registers for what is between.
-template <typename Args>
-__device__ __forceinline__ const __attribute__((address_space(4))) Args &arguments_again() {
-    auto at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
-    asm volatile("" : "+s"(at));
-    return *reinterpret_cast<const __attribute__((address_space(4))) Args *>(at);
-}
-
 template <typename T, int C>
 __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
     __shared__ union Lds { ScanLds scan; JoinLds join; __device__ Lds() {} } lds;
@@ -622,18 +692,21 @@ __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
     if (s_last) join_request<T>(arguments_again<SelectDev>(), request, lds.join);
 }
 
-// How rows are cut into parts: tiles of 4 pieces of 8 values a thread, or of 1 where that leaves compute units without a workgroup; and as many
-// tiles one after the other as leave each compute unit kPerUnit workgroups.  (Three for each run at once with what they hold, so nothing waits
-// for a second round; us with 2, 3 and 4: 32 x 8 rows of 128256, f16 35.1, 33.0, 35.6 and f32 33.5, 34.4, 37.2; 64 x 4 of 32000, f16 15.6, 15.6,
-// 17.5; 16 x 4 of 32000, f32 16.5, 16.5, 22.5.)
+// How rows are cut into parts: tiles of 4 pieces of 8 values a thread, or of 1 where there are fewer than an eighth as many tiles as compute
+// units (us of 1 and 4 pieces: 1 x 4 rows of 32000 in 16 tiles 10.2, 10.9; 8 x 3 of 5000 in 24 10.2, 11.4; 3 x 4 of 32000 in 48 13.0, 11.5; 1 x 8 of
+// 128256 in 128, 16 kept, 22.3, 18.0); and as many tiles one after the other as leave each compute unit kPerUnit workgroups.  (Three for each
+// run at once with what they hold, so nothing waits for a second round; us with 2, 3 and 4: 32 x 8 rows of 128256, f16 32.5, 30.7, 34.2 and f32
+// 33.9, 34.9, 37.5; 64 x 4 of 32000, f16 16.2, 16.2, 18.1.  Parts of the same length end their streams at the same time: 34.2 for 33.0.)
 constexpr int kPerUnit = 3;
 struct Cut { int pieces; int64_t parts, turns; };
-Cut cut_of(int64_t rows, int64_t vocab) {
+Cut cut_of(int64_t batch, int64_t beams, int64_t vocab) {
+    const int64_t rows = batch * beams;
     Cut c;
     auto tiles = [&](int pieces) { return (vocab + kThreads * kPiece * pieces - 1) / (kThreads * kPiece * pieces); };
-    c.pieces = rows * tiles(4) >= 2 * num_compute_units() ? 4 : 1;
+    c.pieces = 8 * rows * tiles(4) >= num_compute_units() ? 4 : 1;
     const int64_t all = tiles(c.pieces);
     c.parts = std::min(all, std::max<int64_t>(1, ((int64_t)kPerUnit * num_compute_units() + rows - 1) / rows));
+    c.parts = std::min(c.parts, kJoinParts / beams);
     c.turns = (all + c.parts - 1) / c.parts;
     c.parts = (all + c.turns - 1) / c.turns;
     return c;
@@ -645,13 +718,13 @@ size_t bytes_for(int64_t rows, int64_t parts, int64_t keep) { return kWsCounterB
 }  // namespace
 
 size_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep) {
-    return bytes_for(batch * beams, cut_of(batch * beams, vocab).parts, keep);
+    return bytes_for(batch * beams, cut_of(batch, beams, vocab).parts, keep);
 }
 
 int launch_beam_select(const BeamSelectArgs &a, hipStream_t s) {
     if (a.batch == 0) return 0;
     const int64_t rows = a.batch * a.beams, es = (int64_t)elem_bytes(a.dtype);
-    const Cut cut = cut_of(rows, a.vocab);
+    const Cut cut = cut_of(a.batch, a.beams, a.vocab);
     TROCM_REQUIRE(a.workspace && a.workspace_bytes >= bytes_for(rows, cut.parts, a.keep), "beam_select: the workspace must hold %zu bytes", bytes_for(rows, cut.parts, a.keep));
     TROCM_REQUIRE(kCounters * a.beams * cut.parts < (1ll << 31) && a.beams * cut.parts * a.keep < (1ll << 31), "beam_select: tensor too large");
     for (int64_t first = 0; first < a.batch; first += kCounters) {
@@ -667,7 +740,7 @@ int launch_beam_select(const BeamSelectArgs &a, hipStream_t s) {
         p.scores_out = a.scores_out + first * a.keep, p.parents = a.parents + first * a.keep, p.tokens = a.tokens + first * a.keep;
         p.ended_out = a.ended_out ? a.ended_out + first * a.keep : nullptr;
         p.row0 = (int)row0;
-        p.by_parts = fast_div(cut.parts), p.by_row_candidates = fast_div(cut.parts * a.keep), p.by_beams = fast_div(a.beams);
+        p.by_parts = fast_div(cut.parts), p.by_row_candidates = fast_div(cut.parts * a.keep), p.by_keep = fast_div(a.keep), p.by_beams = fast_div(a.beams);
         const dim3 grid((unsigned)(batch * a.beams * cut.parts));
         if (a.dtype == TROCM_F16) {
             if (cut.pieces == 4) beam_select_kernel<_Float16, 4><<<grid, kThreads, 0, s>>>(p);
