@@ -579,8 +579,8 @@ int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t 
                        int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream);
 
 /* Attention of q_len new tokens of every sequence over its pages: out = softmax(scale q k^T) v over the first lens[i] tokens, which
- * count the new ones; causal: query r sees tokens up to lens[i] - q_len + r.  A row that sees nothing is zeros.  What lies behind a
- * sequence's last token, in pages that are not its own and in holes may hold anything; tokens that are hidden by causality alone must be finite.
+ * count the new ones; causal: query r sees tokens up to lens[i] - q_len + r.  A row that sees nothing is zeros.  What a row does not
+ * see may hold anything: what lies behind a sequence's last token, in pages that are not its own, in holes, and the later ones of a call's tokens.
  *   q, out    : [n_seq, q_heads, q_len, head_dim] dense, not overlapping; q_heads a multiple of kv_heads
  *   workspace : trocm_sdpa_paged_workspace_bytes, 16-byte aligned, initialised by trocm_sdpa_workspace_init and shared like any other;
  *               with a smaller one or NULL a slow kernel runs

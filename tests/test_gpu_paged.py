@@ -389,6 +389,45 @@ def test_attend_several_tiles_of_rows(rt, dtype, d, n, hq, hkv, sq, causal):
     _attend(rng, lens, hq, hkv, sq, d, 16, dtype, causal=causal, holes=0.05)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("hq,hkv,sq,page", [(8, 8, 2, 16), (4, 1, 3, 32), (16, 2, 3, 16), (8, 2, 9, 16), (14, 2, 6, 64), (6, 3, 70, 16)])
+def test_attend_later_tokens_that_are_not_numbers(rt, dtype, d, hq, hkv, sq, page):
+    """An infinity or a NaN among the values of a call's own tokens is seen by the queries from its token on alone, and in its feature; a
+    NaN among the keys makes those rows NaN.  Lengths of one step, of several parts, of fewer tokens than queries."""
+    rng = np.random.default_rng(d + sq)
+    lens = np.array([sq, 3, 150, 700, 127 + sq // 2, 2600, 20, 128], I32)
+    n, width = len(lens), -(-2600 // page)
+    held = -(-lens // page)
+    n_pages = int(held.sum())
+    order, table, at = rng.permutation(n_pages).astype(I32), np.full((n, width), -1, I32), 0
+    for i in range(n):
+        table[i, :held[i]] = order[at:at + held[i]]
+        at += held[i]
+    k, v = (rng.standard_normal((n_pages, hkv, page, d)).astype(dtype) for _ in range(2))
+    q = rng.standard_normal((n, hq, sq, d)).astype(dtype)
+    bad_k, bad_v, zero_k, zero_v = k.copy(), v.copy(), k.copy(), v.copy()
+    seen, token = np.array([np.nan, np.inf, -np.inf]), np.full(n, -1)
+    for i in range(n):
+        token[i] = int(rng.integers(max(0, lens[i] - sq + 1), lens[i]))
+        place = (table[i, token[i] // page], slice(None), token[i] % page)
+        bad_v[place][:, 1:4], zero_v[place][:, 1:4] = seen.astype(dtype), 0
+        bad_k[place][:, d - 1], zero_k[place] = np.nan, 0
+    sees = (lens[:, None] - sq + np.arange(sq)[None, :] >= token[:, None])[:, None, :, None]
+    run = lambda kk, vv: ta.PagedSdpa().eval(up(q), up(kk), up(vv), up(table), up(lens)).to_numpy()  # noqa: E731
+    want, bound = ref.attend(q, k, zero_v, table, lens)
+    got = run(k, bad_v)
+    hit = np.broadcast_to(sees, got.shape).copy()
+    hit[..., 0], hit[..., 4:] = False, False
+    np.testing.assert_array_equal(got[hit], np.broadcast_to(np.concatenate([[0], seen, np.zeros(d - 4)]), got.shape)[hit].astype(dtype))
+    assert_within(np.where(hit, want, got), want, bound, "values")
+    want, bound = ref.attend(q, zero_k, zero_v, table, lens)
+    got = run(bad_k, bad_v)
+    hit = np.broadcast_to(sees, got.shape)
+    assert np.isnan(got[hit]).all()
+    assert_within(np.where(hit, want, got), want, bound, "keys")
+
+
 # ---- the far ends of what the calls allow -------------------------------------------------------------------------------------
 
 

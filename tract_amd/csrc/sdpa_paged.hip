@@ -194,8 +194,27 @@ struct Stretch {
     float *part;
 };
 
+// A wave-uniform value out of LDS.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// The sum of the values of features d and d + 1 that are not finite, over the keys of a stretch that row r sees and not all rows do.
+template <typename T, int D>
+__device__ __forceinline__ float2_t not_finite(const Stretch &u, int r, int d) {
+    Arguments p = arguments_again();
+    const int seen = u.len - p.Sq + q_row(p, u.b, u.kvh, r).i, end = min(min(u.end * kStep, u.len) - 1, seen);
+    float2_t sum = {0.0f, 0.0f};
+    for (int key = max(u.len - p.Sq + 1, u.first * kStep); key <= end; key++) {
+        const int pi = divided(p.by_page, key), id = p.table[u.b * p.table_width + pi];
+        if ((unsigned)id >= (unsigned)p.n_pages) continue;
+        const T *v = reinterpret_cast<const T *>(p.v + id * p.stride_page + u.kvh * p.stride_h + (key - pi * (int)p.by_page.d) * p.stride_t) + d;
+#pragma unroll
+        for (int y = 0; y < 2; y++) sum[y] += fabsf(widen(v[y])) < INFINITY ? 0.0f : widen(v[y]);
+    }
+    return sum;
+}
+
 template <typename T, int D, int RT, bool ONCE>
-__device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *lds) {
+__device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, unsigned char *lds) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int DB = D / 16;                    // feature blocks of the output
     constexpr int KROW = D + 8, VROW = H16 ? D + 16 : D + 4;   // elements per row in LDS: rows of a read in different banks
@@ -216,6 +235,9 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
         q_at[t] = place.at, lim[t] = p.causal ? min(u.len - 1, u.len - p.Sq + place.i) : u.len - 1;
     }
     const int last_key = u.len - 1;
+    // From here on keys that not all rows see.  A weight of zero does not take an infinity or a NaN out of a product: values from here on that are
+    // not finite are zeros in the tiles, and are added where waves are joined, to the rows that see them.
+    const int some_see = p.causal ? max(u.len - p.Sq + 1, 0) : u.len;
     const char *kb = p.k + u.kvh * p.stride_h, *vb = p.v + u.kvh * p.stride_h;
     const uint32_t st = (uint32_t)p.stride_t;     // (below 2^27: checked by the host)
     const float to_log2 = p.scale * kLog2e;
@@ -370,7 +392,6 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
 #pragma unroll
         for (int j = 0; j < NI; j++) *reinterpret_cast<u32x4 *>(lds_v + (j * RPI + kr) * VROW + ch * (16 / (int)sizeof(T))) = vpre[j];
         if (more) prefetch_v(i + 1, next);
-
         // ---- softmax of this lane's rows over their keys k_lo + 4 grp + key_of(x) --------------------------------
         half8_t pf[RT];        // weights: f16
         float e[RT][8];        // ... and f32
@@ -413,6 +434,21 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
             }
         }
 
+        if (k_lo + kTile > some_see && some_see <= last_key) {
+            wave_sync();
+            uint32_t found = 0;
+            for (int r = max(some_see - k_lo, 0) + kr; r <= min(last_key - k_lo, kTile - 1); r += RPI) {
+                u32x4 &piece = *reinterpret_cast<u32x4 *>(lds_v + r * VROW + ch * (16 / (int)sizeof(T))), x = piece;
+#pragma unroll
+                for (int y = 0; y < 4; y++) {   // a one for every exponent of all ones: in bits 0 and 16, or 0
+                    const uint32_t ones = H16 ? ((x[y] & 0x7fff7fffu) + 0x04000400u) >> 15 & 0x00010001u : ((x[y] & 0x7fffffffu) + 0x00800000u) >> 31;
+                    x[y] &= H16 ? ~(ones * 0xffffu) : ones - 1, found |= ones;
+                }
+                piece = x;
+            }
+            if (found) s_poison = 1;
+        }
+
         // ---- O^T += V^T P^T --------------------------------------------------------------------------------
         wave_sync();
         if constexpr (H16) {
@@ -442,15 +478,18 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
     float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + kWaves * kRows * CROW;
     constexpr int TPR = kThreads / kRows, PER = D / TPR;   // threads per row, features per thread
     const int row = tid / TPR;
+    int poison = 0;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
 #pragma unroll
         for (int d = 16; d < 64; d <<= 1) l_run[t] += __shfl_xor(l_run[t], d, 64);
         __syncthreads();   // the tiles, or the last rows, are done with
+        if (t == 0) poison = s_poison;
 #pragma unroll
         for (int db = 0; db < DB; db++) *reinterpret_cast<float4_t *>(comb + (w * kRows + lr) * CROW + 16 * db + 4 * grp) = o[t][db];
         if (grp < 2) comb_ml[(w * 2 + grp) * kRows + lr] = grp ? l_run[t] : m_run[t];
         __syncthreads();
+        if (t == 0 && tid == 0) s_poison = 0;   // (everybody has seen it)
         if (16 * t + row < u.rows) {
             float mm = -INFINITY, l = 0.0f, f[kWaves];
 #pragma unroll
@@ -484,6 +523,26 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, unsigned char *ld
                 }
             }
             if (u.part && tid % TPR == 0) put(part + kRows * D + row, mm), put(part + kRows * D + kRows + row, l);
+        }
+    }
+    if (uniform(poison)) {   // (every thread to what it has written)
+        int tid = threadIdx.x;
+        asm("" : "+v"(tid));   // (or what is made of it waits in registers all the time)
+        const int row = tid / TPR;
+#pragma unroll 1
+        for (int x = 0; x < RT * PER / 2; x++) {
+            const int r = 16 * (x / (PER / 2)) + row, d = (tid % TPR) * 2 + x % (PER / 2) * 2 * TPR;
+            if (r >= u.rows) continue;
+            const float2_t add = not_finite<T, D>(u, u.row0 + r, d);
+            if (u.part) {
+                float *at = u.part + r / 16 * kLinePart(D) + (r & 15) * D + d;
+                put2(at, get2(at) + add);
+            } else {
+                Arguments p = arguments_again();
+                T *at = reinterpret_cast<T *>(p.out) + q_row(p, u.b, u.kvh, u.row0 + r).at * D + d;
+#pragma unroll
+                for (int y = 0; y < 2; y++) at[y] = (T)(widen(at[y]) + add[y]);
+            }
         }
     }
     __syncthreads();   // (the next stretch's tiles go where these rows were)
@@ -575,9 +634,6 @@ __device__ __forceinline__ bool shares_pages(Arguments p, int b) {
     return (b > 0 && left == mine) || (b + 1 < p.B && right == mine);
 }
 
-// A wave-uniform value out of LDS.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
 // Sums of a wave's lanes up to each one: along the rows of 16 lanes, then over the rows.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
@@ -589,7 +645,7 @@ __device__ __forceinline__ int wave_sums(int x) {
 }
 
 // Where a workgroup stands on the line: what is looked at between stretches alone is in LDS, since the loop needs the scalar registers.
-struct Line { int per, at, end, b, unit, len, steps, first, once, last; };
+struct Line { int per, at, end, b, unit, len, steps, first, once, last, poison; };
 
 // A workgroup's stretch, unit by unit.
 template <typename T, int D, int RT, bool MAY_ONCE>
@@ -607,8 +663,8 @@ __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
             u.end = min(steps, u.first + uniform(s_line.end) - uniform(s_line.at));
             u.part = u.first == 0 && u.end == steps ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * (RT * kLinePart(D));
         }
-        if (MAY_ONCE && uniform(s_line.once)) stretch_body<T, D, RT, MAY_ONCE>(u, lds);
-        else stretch_body<T, D, RT, false>(u, lds);
+        if (MAY_ONCE && uniform(s_line.once)) stretch_body<T, D, RT, MAY_ONCE>(u, s_line.poison, lds);
+        else stretch_body<T, D, RT, false>(u, s_line.poison, lds);
         if (u.part) {
             Arguments p = arguments_again();
             const unsigned per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
@@ -691,7 +747,7 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
             if (lane == 63) s_sums[w] = up;
             __syncthreads();
         }
-        if (tid == 0) s_line.per = per, s_line.at = begin, s_line.end = end;
+        if (tid == 0) s_line.per = per, s_line.at = begin, s_line.end = end, s_line.poison = 0;
         __syncthreads();
     }
     if (rt == RT) return walk_line<T, D, RT, true>(s_line, lds);
