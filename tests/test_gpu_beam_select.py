@@ -183,3 +183,16 @@ def test_more_candidates_than_a_workgroup_holds(rt, dtype, batch, beams, vocab, 
     few = np.full_like(logits, -np.inf)
     few[..., ::vocab // 3] = logits[..., ::vocab // 3]
     _check(few, near, keep)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_rows_behind_four_gibibytes(rt, dtype):
+    """Rows 2^29 elements apart, of which nine hold logits: put there as rows of pages, whose strides say where."""
+    rng, b, w, vocab, apart = np.random.default_rng(13), 3, 3, 5003, 1 << 29
+    logits = (rng.standard_normal((b, w, vocab)) * 3).astype(dtype)
+    rows, size = up(logits.reshape(b * w, 1, vocab)), (b * w - 1) * apart + vocab
+    far, other = ta.DeviceTensor((size,), dtype), ta.DeviceTensor((size,), dtype)
+    pages = lambda t: ta.DeviceTensor((b * w, 1, 1, vocab), dtype, ptr=t.ptr.value, owner=t)  # noqa: E731
+    ta.PagedAppend().eval(rows, rows, up(np.arange(b * w, dtype=I32)), pages(far), pages(other), page_strides=(apart, vocab, vocab))
+    view = ta.DeviceTensor((b, w, vocab), dtype, ptr=far.ptr.value, owner=far)
+    _check(logits, (-rng.random((b, w))).astype(F32), 6, row_stride=apart, device_logits=view)

@@ -511,3 +511,36 @@ def test_reorder_of_large_pools(rt, n_pages, page):
     refs = np.zeros(n_pages, I32)
     np.add.at(refs, table[table >= 0], 1)
     _check_reorder(rng.integers(-2, n + 2, n).astype(I32), table, lens, refs, free, count, page)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("order", ["heads", "tokens"])
+def test_pages_behind_eight_gibibytes(rt, dtype, order):
+    """Byte and element offsets that pass 32 bits: the append, the copy and the attention over pages at both ends of a pool and around its middle."""
+    rng, heads, d, page = np.random.default_rng(12), 8, 128, 16
+    n_pages = (1 << 33) // (heads * d * page * np.dtype(dtype).itemsize) + 7
+    pools = [ta.DeviceTensor((n_pages, heads, page, d), dtype) for _ in range(2)]
+    strides = (heads * page * d, d, heads * d) if order == "tokens" else None
+    ids = np.array([n_pages - 1, 0, n_pages // 2, n_pages // 2 - 1, n_pages - 3, n_pages // 4], I32)
+    lens = np.array([40, 33], I32)
+    table = ids.reshape(2, 3)
+    rows = [rng.standard_normal((73, heads, d)).astype(dtype) for _ in range(2)]
+    slots = np.concatenate([table[i, np.arange(n) // page] * page + np.arange(n) % page for i, n in enumerate(lens)]).astype(I32)
+    ta.PagedAppend().eval(up(rows[0]), up(rows[1]), up(slots), *pools, page_strides=strides)
+
+    q = (rng.standard_normal((2, 32, 1, d)) * 2).astype(dtype)
+    small = [np.zeros((6, heads, page, d), dtype) for _ in range(2)]
+    for x in range(2):
+        for t, slot in enumerate(slots):
+            small[x][int(np.flatnonzero(ids == slot // page)[0]), :, slot % page] = rows[x][t]
+    want, bound = ref.attend(q, *small, np.arange(6, dtype=I32).reshape(2, 3), lens)
+    got = ta.PagedSdpa().eval(up(q), *pools, up(table), up(lens), page_strides=strides).to_numpy()
+    assert_within(got, want, bound, f"{order} {np.dtype(dtype).name}")
+
+    copies = np.array([[n_pages - 1, n_pages - 2, page], [0, n_pages // 2 + 1, 9]], I32)
+    ta.PagedCopy().eval(up(copies), pools, page_strides=strides)
+    got = ta.PagedSdpa().eval(up(q), *pools, ints([[n_pages - 2, 0, n_pages // 2], [n_pages // 2 - 1, n_pages - 3, n_pages // 4]]), up(lens), page_strides=strides).to_numpy()
+    assert_within(got, want, bound, f"copied, {order} {np.dtype(dtype).name}")
+    one = ints([9, 9])
+    got = ta.PagedSdpa().eval(up(q), *pools, ints([[n_pages // 2 + 1], [0]]), one, page_strides=strides).to_numpy()
+    assert got[0].tobytes() == ta.PagedSdpa().eval(up(q[[0, 0]]), *pools, ints([[0], [0]]), one, page_strides=strides).to_numpy()[0].tobytes()
