@@ -389,15 +389,8 @@ def test_attend_several_tiles_of_rows(rt, dtype, d, n, hq, hkv, sq, causal):
     _attend(rng, lens, hq, hkv, sq, d, 16, dtype, causal=causal, holes=0.05)
 
 
-@pytest.mark.parametrize("dtype", [F16, F32])
-@pytest.mark.parametrize("d", [64, 128, 40])
-@pytest.mark.parametrize("hq,hkv,sq,page", [(8, 8, 2, 16), (4, 1, 3, 32), (16, 2, 3, 16), (8, 2, 9, 16), (14, 2, 6, 64), (6, 3, 70, 16)])
-def test_attend_later_tokens_that_are_not_numbers(rt, dtype, d, hq, hkv, sq, page):
-    """An infinity or a NaN among the values of a call's own tokens is seen by the queries from its token on alone, and in its feature; a
-    NaN among the keys makes those rows NaN.  Lengths of one step, of several parts, of fewer tokens than queries."""
-    rng = np.random.default_rng(d + sq)
-    lens = np.array([sq, 3, 150, 700, 127 + sq // 2, 2600, 20, 128], I32)
-    n, width = len(lens), -(-2600 // page)
+def _later_tokens(rng, lens, hq, hkv, sq, d, page, dtype):
+    n, width = len(lens), -(-int(lens.max()) // page)
     held = -(-lens // page)
     n_pages = int(held.sum())
     order, table, at = rng.permutation(n_pages).astype(I32), np.full((n, width), -1, I32), 0
@@ -426,6 +419,27 @@ def test_attend_later_tokens_that_are_not_numbers(rt, dtype, d, hq, hkv, sq, pag
     hit = np.broadcast_to(sees, got.shape)
     assert np.isnan(got[hit]).all()
     assert_within(np.where(hit, want, got), want, bound, "keys")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("hq,hkv,sq,page", [(8, 8, 2, 16), (4, 1, 3, 32), (16, 2, 3, 16), (8, 2, 9, 16), (14, 2, 6, 64), (6, 3, 70, 16)])
+def test_attend_later_tokens_that_are_not_numbers(rt, dtype, d, hq, hkv, sq, page):
+    """An infinity or a NaN among the values of a call's own tokens is seen by the queries from its token on alone, and in its feature; a
+    NaN among the keys makes those rows NaN.  Lengths of one step, of several parts, of fewer tokens than queries."""
+    rng = np.random.default_rng(d + sq)
+    lens = np.array([sq, 3, 150, 700, 127 + sq // 2, 2600, 20, 128], I32)
+    _later_tokens(rng, lens, hq, hkv, sq, d, page, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,hq,hkv,sq", [(64, 16, 8, 20), (64, 16, 8, 9), (128, 16, 8, 9)])
+def test_attend_later_tokens_that_are_not_numbers_in_many_sequences(rt, dtype, d, hq, hkv, sq):
+    """The same in units of several row tiles."""
+    rng = np.random.default_rng(d * sq)
+    lens = rng.integers(1, 50, 300).astype(I32)
+    lens[:3] = 400, 129, 1
+    _later_tokens(rng, lens, hq, hkv, sq, d, 16, dtype)
 
 
 # ---- the far ends of what the calls allow -------------------------------------------------------------------------------------
@@ -544,3 +558,14 @@ def test_pages_behind_eight_gibibytes(rt, dtype, order):
     one = ints([9, 9])
     got = ta.PagedSdpa().eval(up(q), *pools, ints([[n_pages // 2 + 1], [0]]), one, page_strides=strides).to_numpy()
     assert got[0].tobytes() == ta.PagedSdpa().eval(up(q[[0, 0]]), *pools, ints([[0], [0]]), one, page_strides=strides).to_numpy()[0].tobytes()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,hq,hkv,sq,causal", [(300, 16, 8, 20, True), (300, 8, 8, 30, False), (160, 16, 8, 9, True)])
+def test_attend_tiles_of_rows_in_many_sequences(rt, dtype, d, n, hq, hkv, sq, causal):
+    """So many steps that no unit takes fewer row tiles than it can, or half as many."""
+    rng = np.random.default_rng(n + sq)
+    lens = rng.integers(0, 40, n)
+    lens[:4] = 300, 0, 129, sq
+    _attend(rng, lens, hq, hkv, sq, d, 16, dtype, causal=causal, holes=0.05)

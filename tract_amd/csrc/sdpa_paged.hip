@@ -697,9 +697,10 @@ __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
     }
 }
 
-// RT: row tiles of a unit, which share the keys that it reads.  Where that leaves no more steps than workgroups, units take half as many, and
-// again: what a workgroup does for one tile after the other is then what takes the time (2 sequences of up to 300 keys, 7 heads' 5 queries
-// 12.9 us with four tiles, 7.8 with one).
+// RT: row tiles of a unit, which share the keys that it reads.  Where that leaves no more than a step or two per workgroup and tile, units take
+// half as many, and again: what a workgroup does for one tile after the other is then what takes the time.  In us, more tiles and half as many: 2
+// sequences of up to 300 keys, 7 heads' 5 queries 12.9 (four), 9.8, 7.8; 4 of 3000 to 6000, 8 heads' 6 queries 35.3 (four), 26.3; 20 of up to 900, 8
+// heads' 4 queries 20.0 (two), 16.2; beyond the rule 40 of 500 to 900, 4 heads' 5 queries of 128 37.0 (two), 45.2.
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
@@ -722,7 +723,7 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         __syncthreads();
         const int all_steps = s_totals[0] + s_totals[1] + s_totals[2] + s_totals[3];   // of one unit of every sequence
         auto units_of = [&](int rt) { return p.Hkv * (int)p.row_units[rt >> 1].d; };   // of a sequence
-        while (rt > 1 && all_steps * units_of(rt) <= (int)gridDim.x) rt >>= 1;
+        while (rt > 1 && all_steps * units_of(rt) <= rt * (int)gridDim.x) rt >>= 1;
         const int units = units_of(rt), total = all_steps * units;
         const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), 1);
         const int begin = blockIdx.x * per, end = min(begin + per, total);
