@@ -196,3 +196,13 @@ def test_rows_behind_four_gibibytes(rt, dtype):
     ta.PagedAppend().eval(rows, rows, up(np.arange(b * w, dtype=I32)), pages(far), pages(other), page_strides=(apart, vocab, vocab))
     view = ta.DeviceTensor((b, w, vocab), dtype, ptr=far.ptr.value, owner=far)
     _check(logits, (-rng.random((b, w))).astype(F32), 6, row_stride=apart, device_logits=view)
+
+
+def test_arrays_of_the_host_are_taken_too(rt):
+    rng = np.random.default_rng(8)
+    logits, scores = rng.standard_normal((2, 3, 300)).astype(F32), (-rng.random((2, 3))).astype(F32)
+    want = ref.select(logits, scores, 4)
+    for x, s in ((logits, scores), (up(logits), scores), (logits, up(scores))):
+        got = ta.BeamSelect(4).eval(x, s)
+        for name in ("parents", "tokens"):
+            np.testing.assert_array_equal(got[name].to_numpy(), want[name])

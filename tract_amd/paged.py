@@ -46,6 +46,17 @@ def _outputs(out, shapes):
     return out
 
 
+def _holds(out, shapes) -> bool:
+    """Whether `out` has all of the named int32 outputs (a loop: this runs with every call)."""
+    if out is None:
+        return False
+    for name, shape in shapes.items():
+        t = out.get(name)
+        if t is None or t.shape != shape or t.dtype is not _I32:
+            return False
+    return True
+
+
 def _strides(given, kind, n):
     if given is None:
         return None
@@ -77,7 +88,7 @@ class PagedPlan:
         if not isinstance(lens, DeviceTensor) or not isinstance(n_new, DeviceTensor):
             lens, n_new = _as_device(lens, stream), _as_device(n_new, stream)
         key = (lens.shape, n_new.shape, table.shape, free_pages.shape, free_count.shape, tokens, refs is None or (refs.shape, refs.dtype),
-               *(t.dtype for t in (lens, n_new, table, free_pages, free_count)))
+               lens.dtype, n_new.dtype, table.dtype, free_pages.dtype, free_count.dtype)
         last_key, sizes = self._last   # (a pair, read once: another thread's call may put its own there)
         if key != last_key:
             if len(table.shape) != 2 or len(free_pages.shape) != 1 or tokens < 0:
@@ -91,7 +102,7 @@ class PagedPlan:
             sizes = n, width, free_pages.shape[0], {"lens": (n,), "starts": (n + 1,), "slots": (tokens,), "positions": (tokens,), "free_count": (1,), "refused": (1,)}
             self._last = key, sizes
         n, width, n_pages, shapes = sizes
-        if out is None or any((t := out.get(name)) is None or t.shape != shape or t.dtype is not _I32 for name, shape in shapes.items()):
+        if not _holds(out, shapes):
             out = _outputs(out, shapes)
         call("trocm_paged_plan", lens.ptr, n_new.ptr, n, self.page_size, table.ptr, width, free_pages.ptr, free_count.ptr, n_pages, None if refs is None else refs.ptr,
              tokens, out["lens"].ptr, out["starts"].ptr, out["slots"].ptr, out["positions"].ptr, out["free_count"].ptr, out["refused"].ptr, None if stream is None else _sh(stream))
@@ -110,7 +121,7 @@ class PagedAppend:
     def eval(self, k, v, slots, k_pages, v_pages, stream=None, k_strides=None, v_strides=None, page_strides=None) -> None:
         """K and V [tokens, kv_heads, head_dim], strides of views for token and head in elements (None: dense); slots [tokens];
         pages [n_pages, kv_heads, page_size, head_dim], strides for page, head and token (None: dense)."""
-        if not isinstance(k, DeviceTensor):
+        if not isinstance(k, DeviceTensor) or not isinstance(v, DeviceTensor):
             k, v = _as_device(k, stream), _as_device(v, stream)
         key = (k.shape, v.shape, slots.shape, k_pages.shape, v_pages.shape, k.dtype, v.dtype, slots.dtype, k_pages.dtype, v_pages.dtype,
                k_strides and tuple(k_strides), v_strides and tuple(v_strides), page_strides and tuple(page_strides))
@@ -186,7 +197,8 @@ class PagedReorder:
         free_pages, free_count, copies [n_seq, 3] for PagedCopy and missing [1] (not 0: nothing has changed); none of them may be an input."""
         if not isinstance(parents, DeviceTensor):
             parents = _as_device(parents, stream)
-        key = (parents.shape, table.shape, lens.shape, refs.shape, free_pages.shape, free_count.shape, *(t.dtype for t in (parents, table, lens, refs, free_pages, free_count)))
+        key = (parents.shape, table.shape, lens.shape, refs.shape, free_pages.shape, free_count.shape,
+               parents.dtype, table.dtype, lens.dtype, refs.dtype, free_pages.dtype, free_count.dtype)
         last_key, sizes = self._last
         if key != last_key:
             if len(table.shape) != 2 or len(refs.shape) != 1:
@@ -198,7 +210,7 @@ class PagedReorder:
             sizes = n, width, n_pages, {"table": (n, width), "lens": (n,), "refs": (n_pages,), "free_pages": (n_pages,), "free_count": (1,), "copies": (n, 3), "missing": (1,)}
             self._last = key, sizes
         n, width, n_pages, shapes = sizes
-        if out is None or any((t := out.get(name)) is None or t.shape != shape or t.dtype is not _I32 for name, shape in shapes.items()):
+        if not _holds(out, shapes):
             out = _outputs(out, shapes)
         call("trocm_paged_reorder", parents.ptr, n, self.page_size, table.ptr, width, lens.ptr, refs.ptr, free_pages.ptr, free_count.ptr, n_pages, out["table"].ptr,
              out["lens"].ptr, out["refs"].ptr, out["free_pages"].ptr, out["free_count"].ptr, out["copies"].ptr, out["missing"].ptr, None if stream is None else _sh(stream))
@@ -249,7 +261,7 @@ class BeamSelect:
         """logits [batch, beams, vocab], rows `row_stride` elements apart (0: dense); scores f32 [batch, beams]; ended int32
         [batch, beams] or None.  Returns (into `out`, where given) scores f32, parents (rows: request * beams + beam), tokens and ended
         int32, all [batch, keep], best first."""
-        if not isinstance(logits, DeviceTensor):
+        if not isinstance(logits, DeviceTensor) or not isinstance(scores, DeviceTensor):
             logits, scores = _as_device(logits, stream), _as_device(scores, stream)
         if ended is not None and not isinstance(ended, DeviceTensor):
             ended = _as_device(ended, stream)
@@ -262,17 +274,17 @@ class BeamSelect:
                 _ints("ended", ended, scores.shape)
             batch, beams, vocab = logits.shape
             need = _beam_bytes(batch, beams, vocab, self.keep)
-            sizes, ws = ((_code(logits.dtype), batch, beams, vocab), (batch, self.keep), need), self._scratch.holding(need, stream)
+            shape = batch, self.keep
+            sizes, ws = ((_code(logits.dtype), batch, beams, vocab), shape, {"parents": shape, "tokens": shape, "ended": shape}, need), self._scratch.holding(need, stream)
             self._last = key, sizes, ws
-        sizes, shape, need = sizes
-        if out is None or (scores_out := out.get("scores")) is None or scores_out.shape != shape or not _same(scores_out.dtype, _F32) or any(
-                (t := out.get(name)) is None or t.shape != shape or t.dtype is not _I32 for name in ("parents", "tokens", "ended")):
-            scores_out = (out or {}).get("scores")
+        sizes, shape, shapes, need = sizes
+        scores_out = None if out is None else out.get("scores")
+        if scores_out is None or scores_out.shape != shape or scores_out.dtype is not _F32 or not _holds(out, shapes):
             if scores_out is None:
                 scores_out = DeviceTensor(shape, _F32)
             elif scores_out.shape != shape or not _same(scores_out.dtype, _F32):
                 raise TractRocmError(f"scores must be f32 of shape {list(shape)}")
-            out = _outputs(out, {"parents": shape, "tokens": shape, "ended": shape})
+            out = _outputs(out, shapes)
             out["scores"] = scores_out
         call("trocm_beam_select", logits.ptr, *sizes, row_stride, scores.ptr, _optr(ended), self.eos, self.keep, scores_out.ptr, out["parents"].ptr, out["tokens"].ptr,
              out["ended"].ptr, ws.buf.ptr, need, None if stream is None else _sh(stream))
