@@ -4,9 +4,9 @@
 // All state (lengths, tables, counts of holders, the stack of free pages) is read and written by kernels alone, so a step can be
 // recorded once and replayed.  Every id that comes from device memory is checked before it becomes an address.
 //
-// Tables are kilobytes: what bounds plan and reorder is the chain of dependent accesses and barriers (a plan of 256 sequences 5.5 us, 4.4 of
-// them the kernel's; 4 beams reordered 12 us in two launches with the copy, 256 beams in eight layers 24.4 in four).  Prefix sums go along the
-// lanes (shuffles through LDS: 6.9 us for the plan's 5.5).  The append and the copies are bound by their bytes.
+// Tables are kilobytes: what bounds plan and reorder is the chain of dependent accesses and barriers (a plan of 256 sequences 5.1 us, 4.4 of
+// them the kernel's; 4 beams reordered 11 us in two launches with the copy, 256 beams in eight layers 25 in four).  Prefix sums go along the
+// lanes (shuffles through LDS: 6.9 us for the plan, then 5.5).  The append and the copies are bound by their bytes.
 #include <algorithm>
 #include "common.h"
 #include "fast_div.h"

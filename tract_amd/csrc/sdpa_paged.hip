@@ -11,11 +11,11 @@
 // parts (unnormalised O, maximum, sum, f32), which the last workgroup to arrive joins, always in the same order.  Two workgroups a compute
 // unit, whose rows of the next tile are on their way while one is worked on (1, 3, 4 and 8 were slower).  A line counted in tiles, whose
 // stretches began anywhere, left waves of a step without a tile and put short sequences behind one another (64 sequences of up to 8192 keys
-// 195 us for 190.5, one token behind 777 10.4 for 7.6, 9 sequences of up to 120 in f32 23.9 for 10.2).
+// 195 us for 190.5, one token behind 777 10.4 for 7.7, 9 sequences of up to 120 in f32 23.9 for 10.2).
 //
 // What bounds it: the pages' bytes where there are many (64 sequences of 64 to 8192 keys of 8 x 128, f16, 1.18 GB: 190.5 us, 6.2 TB/s; 3
-// queries behind 90000 and 100001 keys 137.6 us, 5.7 TB/s; 16 sequences of up to 3000 keys of 32 x 64, f32, 80.9 us, 5.2 TB/s), matrix
-// instructions busy for 4 to 34 % of the SIMDs' cycles; the chain lengths - table - keys - join where there are few (7.6 us).
+// queries behind 90000 and 100001 keys 137 us, 5.8 TB/s; 16 sequences of up to 3000 keys of 32 x 64, f32, 82 us, 5.2 TB/s), matrix
+// instructions busy for 4 to 34 % of the SIMDs' cycles; the chain lengths - table - keys - join where there are few (7.7 us).
 #include <hip/hip_fp16.h>
 #include <math.h>
 #include <algorithm>
@@ -769,7 +769,7 @@ int line_workgroups() { return 2 * num_compute_units(); }
 }  // namespace
 
 // Row tiles of a unit, at most: as many as a lane's registers hold (f32 of head size 128 has no place for two rows' queries in LDS either).  91
-// sequences of 2880 to 5761 keys: 8 heads' 5 queries of head size 64 in four tiles 172 us, in two 300; 4 heads' 5 of 128 in two 275, in one 561.
+// sequences of 2880 to 5761 keys: 8 heads' 5 queries of head size 64 in four tiles 175 us, in two 300; 4 heads' 5 of 128 in two 275, in one 561.
 static int row_tiles_of_unit(int64_t rows, int64_t es, int64_t D) {
     if (rows <= kRows || in_lds((int)es, (int)D)) return 1;
     return rows > 2 * kRows && es == 2 && D == 64 ? 4 : 2;
