@@ -613,7 +613,9 @@ int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools
                      int64_t head_dim, int64_t n_pages, int64_t page_size, const int64_t *page_strides, void *stream);
 
 /* Beam search's choice.  For every request: of all c = scores[b] + logits[b][v] - log(sum over u of exp(logits[b][u])) over its `beams`
- * beams and the vocabulary the `keep` largest, largest first, equal ones by ascending beam * vocab + token; c is compared in 64 bits.
+ * beams and the vocabulary the `keep` largest, largest first, equal ones by ascending beam * vocab + token; c is compared in
+ * 64 bits, as scores[b] + ((logits[b][v] - max) - log(sum exp(logits[b] - max))) with sums right to 2^-51 + vocab * 2^-62: values of
+ * different beams that are nearer than that come in either order, but for beams with the same differences of logits, whose sums are the same.
  *   logits     : rows of `vocab` for batch * beams beams, row_stride elements apart (0: dense)
  *   scores     : [batch, beams] f32; one that is infinite or NaN leaves its beam only candidates of -inf, and so do logits without a finite largest one
  *   ended      : [batch, beams] int32 or NULL: a beam with one that is not 0 has a single candidate, its score as it is with token `eos`

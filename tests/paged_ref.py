@@ -152,7 +152,7 @@ def select(logits, scores, keep, ended=None, eos=-1):
             x = np.where(np.isnan(x), -np.inf, x)
             top = x.max()
             if np.isfinite(top):
-                c[j] = s + (x - (top + math.log(math.fsum(np.exp(x - top)))))
+                c[j] = s + ((x - top) - math.log(math.fsum(np.exp(x - top))))
         order = np.argsort(-c.reshape(-1), kind="stable")[:keep]
         out["scores"][i], out["parents"][i], out["tokens"][i] = c.reshape(-1)[order], i * w + order // n, order % n
         out["ended"][i] = (order % n == eos) | (False if ended is None else ended[i][order // n] != 0)

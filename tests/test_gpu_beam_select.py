@@ -206,3 +206,28 @@ def test_arrays_of_the_host_are_taken_too(rt):
         got = ta.BeamSelect(4).eval(x, s)
         for name in ("parents", "tokens"):
             np.testing.assert_array_equal(got[name].to_numpy(), want[name])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("vocab", [2, 3, 17, 3000])
+def test_rows_that_are_others_shifted_tie(rt, dtype, vocab):
+    """Logits of one beam plus a whole number are the same continuation probabilities: equal values, to the lowest beam."""
+    rng = np.random.default_rng(vocab)
+    base, by = rng.integers(-4, 5, (5, 1, vocab)), rng.integers(-9, 10, (5, 6, 1))
+    keep = min(12, 6 * vocab)
+    _check((base + by).astype(dtype), np.zeros((5, 6), F32), keep)
+    _check((rng.permuted(np.repeat(base, 6, axis=1), axis=2) + by).astype(dtype), np.full((5, 6), -3.25, F32), keep)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_sums_that_differ_in_the_last_places(rt, dtype):
+    """Beams that differ in one logit of 28 to 33 below the largest: their sums, in parts of 7e-13 to 5e-15, and what is chosen with them, in an order
+    that is not that of the beams.  (The terms that the rows share are off by the same; 5e-15 is 20 steps of 64 bits.)"""
+    rng = np.random.default_rng(11)
+    row = (-12 + rng.standard_normal(20001)).astype(dtype)
+    logits = np.repeat(row[None, None], 6, axis=1).repeat(2, axis=0)
+    logits[..., 777] = 0
+    logits[0, :, 5000] = -28 - np.arange(6)
+    logits[1, :, 19999] = -28 - np.array([2, 0, 5, 1, 4, 3])
+    got = _check(logits, np.zeros((2, 6), F32), 12)
+    assert got["parents"][0, :6].tolist() == [5, 4, 3, 2, 1, 0] and (got["parents"][1, :6] - 6).tolist() == [2, 4, 5, 0, 3, 1]

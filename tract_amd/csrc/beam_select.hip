@@ -4,7 +4,8 @@
 // Within a beam the order of c is the order of the logits, which is exact; only between beams does c itself count.  So the vocabulary is
 // read once: a workgroup streams a part of a row through registers, makes its maximum and sum (f32 for eight values, then f64) and keeps its
 // `keep` largest logits; the last workgroup of a request to arrive puts the parts together in f64.  Where values of two beams are nearer than
-// those sums can be told apart, the beams' sums are made again, exactly.
+// those sums can be told apart, the beams' sums are made again, exactly, against the beams' own largest values: rows that are others shifted, or in
+// another order, tie exactly.
 //
 // The largest of a wave's values: the K-th largest of its lanes' maxima is found, nearly, by bisection over the upper bits of an order-preserving
 // integer (ballots and counts); at least K values reach it, and few more than that, which are listed in LDS and ranked by counting.
@@ -349,23 +350,25 @@ struct alignas(16) Choice { double c; int place, beam; };   // place: beam * voc
 
 __device__ __forceinline__ bool before(double c, int place, double d, int other) { return c > d || (c == d && place < other); }
 
-// 2^t for t <= 0 times 2^shift, in f64: the exponential's series for the fraction, of at most a half (the twelfth term is 6e-15).
+// 2^t for t <= 0 times 2^shift, in f64: the exponential's series for the fraction, of at most a half (the term behind the last is 1e-19).
 __device__ __forceinline__ double exp2_scaled(double t, int shift) {
     const double n = __builtin_rint(t), r = (t - n) * 0.6931471805599453;
-    double y = 1.0 / 39916800.0;
-    constexpr double kInverse[11] = {1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+    double y = 1.0 / 87178291200.0;
+    constexpr double kInverse[14] = {1.0 / 6227020800.0, 1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
 #pragma unroll
-    for (int i = 0; i < 11; i++) y = __builtin_fma(y, r, kInverse[i]);
+    for (int i = 0; i < 14; i++) y = __builtin_fma(y, r, kInverse[i]);
     return __builtin_ldexp(y, (int)fmax(n, -2000.0) + shift);
 }
 
-// log sum exp of a row whose largest value is m, the same for the same values in any order: terms of 64 bits, rounded to whole multiples of
-// 2^-shift of the largest and added as integers.  All threads; only where two beams are nearer than their 32-bit sums tell apart.
+// log sum exp(x - m) of a row whose largest value is m, the same for the same differences in any order: terms of 64 bits, rounded to whole multiples of
+// 2^-61 of the largest and added as integers of 128: off by 2^-51 and 2^-62 a term.  All threads; only where two beams are nearer than their 32-bit sums tell apart.
 template <typename T>
-__device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint64_t *lds_sums) {
-    const int shift = 61 - (32 - __clz(vocab)), tid = threadIdx.x;
-    uint64_t sum = 0;
-    auto add = [&](float v) { sum += v == v ? (uint64_t)(exp2_scaled(((double)v - (double)m) * 1.4426950408889634, shift) + 0.5) : 0; };
+__device__ __forceinline__ double exact_log_sum(const T *x, int vocab, float m, uint64_t *lds_sums) {
+    constexpr int kShift = 61;
+    const int tid = threadIdx.x;
+    uint64_t sum = 0, high = 0;
+    auto plus = [&](uint64_t low, uint64_t upper) { sum += low, high += upper + (sum < low ? 1 : 0); };
+    auto add = [&](float v) { plus(v == v ? (uint64_t)(exp2_scaled(((double)v - (double)m) * 1.4426950408889634, kShift) + 0.5) : 0, 0); };
     constexpr int kStep = kThreads * kPiece;
     const int whole = vocab / kPiece * kPiece;
     Eight<T> coming;
@@ -379,21 +382,24 @@ __device__ __forceinline__ double exact_lse(const T *x, int vocab, float m, uint
     }
     if (whole + tid < vocab) add((float)x[whole + tid]);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += (uint64_t)__shfl_xor((unsigned long long)sum, d, 64);
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t low = (uint64_t)__shfl_xor((unsigned long long)sum, d, 64), upper = (uint64_t)__shfl_xor((unsigned long long)high, d, 64);
+        plus(low, upper);
+    }
     __syncthreads();
-    if ((tid & 63) == 0) lds_sums[tid >> 6] = sum;
+    if ((tid & 63) == 0) lds_sums[2 * (tid >> 6)] = sum, lds_sums[2 * (tid >> 6) + 1] = high;
     __syncthreads();
-    sum = 0;
-    for (int y = 0; y < kWaves; y++) sum += lds_sums[y];
-    return (double)m + log(ldexp((double)sum, -shift));
+    sum = high = 0;
+    for (int y = 0; y < kWaves; y++) plus(lds_sums[2 * y], lds_sums[2 * y + 1]);
+    return log(ldexp((double)high, 64 - kShift) + ldexp((double)sum, -kShift));
 }
 
 struct JoinLds {
     double c[kJoinList];
     int2 at[kJoinList];   // place, beam
-    double lse[kBeamMaxBeams], score[kBeamMaxBeams], err[kBeamMaxBeams], best_c[kWaves];
-    uint64_t sums[kWaves];
-    float max[kBeamMaxBeams];
+    double log_sum[kBeamMaxBeams], score[kBeamMaxBeams], err[kBeamMaxBeams], best_c[kWaves];
+    uint64_t sums[2 * kWaves];
+    float max[kBeamMaxBeams], ref[kBeamMaxBeams];   // the largest value; what the sum is against
     int kind[kBeamMaxBeams], ended[kBeamMaxBeams];   // kind 0: goes on, 1: stays at the token of the ended, 2: has no candidates but of -inf
     int part[kJoinParts], parts;
     int again[kBeamMaxBeams], any, count, best_place[kWaves], best_beam[kWaves];
@@ -459,7 +465,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             const bool dead = !(fabsf(score) < INFINITY);
             const double log_l = log(l);
             lds.score[beam] = dead ? -INFINITY : (double)score;
-            lds.lse[beam] = (double)m + log_l;
+            lds.log_sum[beam] = log_l, lds.ref[beam] = m;
             lds.max[beam] = top;
             lds.ended[beam] = ended;
             lds.kind[beam] = dead ? 2 : ended ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
@@ -477,7 +483,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
     auto choice = [&](int beam, int k, const Candidate &c) {   // k: which one of the beam
         Choice r = {-INFINITY, -1, beam};
         if (lds.kind[beam] == 0) {
-            if (c.token >= 0) r.c = lds.score[beam] + ((double)c.x - lds.lse[beam]), r.place = beam * p.vocab + c.token;
+            if (c.token >= 0) r.c = lds.score[beam] + (((double)c.x - (double)lds.ref[beam]) - lds.log_sum[beam]), r.place = beam * p.vocab + c.token;
         } else if (k < p.keep) {   // the token that an ended beam stays at, and then, as in a beam without values, tokens in their order
             const bool stays = lds.kind[beam] == 1 && k == 0;
             const int token = lds.kind[beam] == 1 ? (stays ? p.eos : k - 1 < p.eos ? k - 1 : k) : k;
@@ -630,8 +636,8 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
                 for (int beam = 0; beam < p.beams; beam++)
                     if (lds.again[beam] && lds.kind[beam] == 0) {
                         const auto &p = arguments_again<SelectDev>();
-                        const double lse = exact_lse(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, lds.max[beam], lds.sums);
-                        if (tid == 0) lds.lse[beam] = lse;
+                        const double log_sum = exact_log_sum(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, lds.max[beam], lds.sums);
+                        if (tid == 0) lds.log_sum[beam] = log_sum, lds.ref[beam] = lds.max[beam];
                     }
                 __syncthreads();
                 continue;
