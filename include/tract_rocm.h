@@ -583,7 +583,7 @@ int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t 
  * see may hold anything: what lies behind a sequence's last token, in pages that are not its own, in holes, and the later ones of a call's tokens.
  *   q, out    : [n_seq, q_heads, q_len, head_dim] dense, not overlapping; q_heads a multiple of kv_heads
  *   workspace : trocm_sdpa_paged_workspace_bytes, 16-byte aligned, initialised by trocm_sdpa_workspace_init and shared like any other;
- *               with a smaller one or NULL a slow kernel runs
+ *               with one that does for q_len 1 more is read, with a smaller one or NULL a slow kernel runs
  * Fast kernels: head_dim 64 and 128, page_size a multiple of 16, bases and strides multiples of 16 bytes, q_heads / kv_heads * q_len rows
  * of a kv head as tiles of 16; anything else up to head_dim 2048 is correct and slow. */
 int trocm_sdpa_paged_workspace_bytes(int64_t n_seq, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t head_dim,

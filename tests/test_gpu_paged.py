@@ -569,3 +569,35 @@ def test_attend_tiles_of_rows_in_many_sequences(rt, dtype, d, n, hq, hkv, sq, ca
     lens = rng.integers(0, 40, n)
     lens[:4] = 300, 0, 129, sq
     _attend(rng, lens, hq, hkv, sq, d, 16, dtype, causal=causal, holes=0.05)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_with_workspaces_of_every_size(rt, dtype, d):
+    """That of the call, of fewer queries, a byte less than any, and none: all within the bounds, and nothing behind the workspace is written."""
+    rng, n, hq, hkv, sq, page = np.random.default_rng(d), 300, 16, 8, 20, 16
+    lens = rng.integers(0, 40, n).astype(I32)
+    lens[:2] = 500, 129
+    held = -(-lens // page)
+    table, at = np.full((n, held.max()), -1, I32), 0
+    for i in range(n):
+        table[i, :held[i]] = np.arange(at, at + held[i])
+        at += held[i]
+    k, v = (rng.standard_normal((at, hkv, page, d)).astype(dtype) for _ in range(2))
+    q = rng.standard_normal((n, hq, sq, d)).astype(dtype)
+    want, bound = ref.attend(q, k, v, table, lens)
+    sizes = []
+    for queries in (20, 16, 9, 1):
+        b = C.c_size_t()
+        ta._lib.call("trocm_sdpa_paged_workspace_bytes", n, hq, hkv, queries, d, C.byref(b))
+        sizes.append(b.value)
+    assert sizes[0] >= sizes[1] >= sizes[2] >= sizes[3]
+    dq, dk, dv, dt, dl = up(q), up(k), up(v), up(table), up(lens)
+    for size in [*sizes, sizes[-1] - 1, 0]:
+        ws, out = up(np.full(size + 4096, 0xA5, np.uint8)), up(np.full(q.shape, np.nan, dtype))
+        if size:
+            ta._lib.call("trocm_sdpa_workspace_init", ws.ptr, size, None)
+        ta._lib.call("trocm_sdpa_paged", dq.ptr, 1 if dtype is F16 else 0, n, hq, hkv, sq, d, dk.ptr, dv.ptr, at, page, None, dt.ptr, table.shape[1], dl.ptr, out.ptr,
+                     float("nan"), 1, ws.ptr if size else None, size, None)
+        assert_within(out.to_numpy(), want, bound, f"{size} bytes")
+        assert (ws.to_numpy()[size:] == 0xA5).all()

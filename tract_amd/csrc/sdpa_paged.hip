@@ -775,8 +775,10 @@ static int row_tiles_of_unit(int64_t rows, int64_t es, int64_t D) {
     return rows > 2 * kRows && es == 2 && D == 64 ? 4 : 2;
 }
 
+static size_t bytes_for(int64_t row_tiles, int64_t D) { return kWsCounterBytes + (size_t)(2 * line_workgroups() * row_tiles * kLinePart((int)D)) * 4; }
+
 size_t sdpa_paged_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
-    return kWsCounterBytes + (D == 64 || D == 128 ? (size_t)2 * line_workgroups() * row_tiles_of_unit(Hq / Hkv * Sq, 2, D) * kLinePart((int)D) * 4 : 0);
+    return D == 64 || D == 128 ? bytes_for(row_tiles_of_unit(Hq / Hkv * Sq, 2, D), D) : kWsCounterBytes;
 }
 
 int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
@@ -791,9 +793,10 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
     p.scale = a.scale, p.causal = a.causal, p.by_page = fast_div(a.page_size);
     const uint64_t bits = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.out | (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.v | (uint64_t)p.stride_page | (uint64_t)p.stride_h | (uint64_t)p.stride_t;
     if ((a.D == 64 || a.D == 128) && a.page_size % 16 == 0 && bits % 16 == 0 && a.n_pages > 0 && p.stride_t < (1 << 27) && a.workspace &&
-        a.workspace_bytes >= sdpa_paged_workspace_bytes(a.B, a.Hq, a.Hkv, a.Sq, a.D)) {
+        a.workspace_bytes >= bytes_for(1, a.D)) {
         const int64_t rows = a.Hq / a.Hkv * a.Sq;
-        const int rt = row_tiles_of_unit(rows, es, a.D);
+        int rt = row_tiles_of_unit(rows, es, a.D);
+        while (rt > 1 && a.workspace_bytes < bytes_for(rt, a.D)) rt /= 2;
         for (int i = 0; i < 3; i++) p.row_units[i] = fast_div((rows + (kRows << i) - 1) / (kRows << i));
         p.by_g = fast_div(p.G), p.by_workgroups = fast_div(line_workgroups());
         p.counters = (int *)a.workspace, p.parts = (float *)((char *)a.workspace + kWsCounterBytes);
