@@ -601,3 +601,22 @@ def test_attend_with_workspaces_of_every_size(rt, dtype, d):
                      float("nan"), 1, ws.ptr if size else None, size, None)
         assert_within(out.to_numpy(), want, bound, f"{size} bytes")
         assert (ws.to_numpy()[size:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,hq,hkv,sq,page,causal", [(400, 8, 8, 1, 16, True), (400, 6, 3, 1, 32, True), (300, 8, 8, 3, 16, False), (500, 9, 3, 5, 16, True), (200, 32, 16, 1, 48, True)])
+def test_attend_many_short_sequences(rt, dtype, d, n, hq, hkv, sq, page, causal):
+    """More units of a step than workgroups: a wave each where sequences have up to 64 keys, beside longer ones and empty ones."""
+    rng = np.random.default_rng(n + hq + sq)
+    lens = rng.integers(0, 70, n)
+    lens[rng.random(n) < 0.1] = 0
+    lens[:4] = 64, 65, 32, 200
+    _attend(rng, lens, hq, hkv, sq, d, page, dtype, causal=causal, holes=0.1)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_later_tokens_that_are_not_numbers_in_short_sequences(rt, dtype, d):
+    rng = np.random.default_rng(d)
+    _later_tokens(rng, rng.integers(1, 64, 400, endpoint=True).astype(I32), 8, 4, 5, d, 16, dtype)

@@ -213,7 +213,8 @@ __device__ __forceinline__ float2_t not_finite(const Stretch &u, int r, int d) {
     return sum;
 }
 
-template <typename T, int D, int RT, bool ONCE>
+// SOLO: a unit of this wave alone, in tiles one after the other.
+template <typename T, int D, int RT, bool ONCE, bool SOLO>
 __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, unsigned char *lds) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int DB = D / 16;                    // feature blocks of the output
@@ -241,18 +242,19 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
     const char *kb = p.k + u.kvh * p.stride_h, *vb = p.v + u.kvh * p.stride_h;
     const uint32_t st = (uint32_t)p.stride_t;     // (below 2^27: checked by the host)
     const float to_log2 = p.scale * kLog2e;
-    const int n_mine = min(u.end - u.first, (last_key / kTile - u.first * kWaves - w + kWaves) / kWaves);   // this wave takes a tile of every step
+    auto tile_at = [&](int i) { return SOLO ? i : (u.first + i) * kWaves + w; };   // this wave takes a tile of every step
+    const int n_mine = SOLO ? last_key / kTile + 1 : min(u.end - u.first, (last_key / kTile - u.first * kWaves - w + kWaves) / kWaves);
 
     // Where the halves of 32 of this wave's tiles lie: lane 2 i + h has tile i's half h, as bytes from the pool's beginning (-1: a hole, or
     // behind the last key).
     auto ask_pages = [&](int i0) __attribute__((always_inline)) {
         Arguments p = arguments_again();
-        const int key = ((u.first + i0 + (lane >> 1)) * kWaves + w) * kTile + 16 * (lane & 1);
+        const int key = tile_at(i0 + (lane >> 1)) * kTile + 16 * (lane & 1);
         return key <= last_key && i0 + (lane >> 1) < n_mine ? p.table[u.b * p.table_width + divided(p.by_page, key)] : -1;
     };
     auto bytes_at = [&](int id, int i0) __attribute__((always_inline)) {
         Arguments p = arguments_again();
-        const int key = ((u.first + i0 + (lane >> 1)) * kWaves + w) * kTile + 16 * (lane & 1);
+        const int key = tile_at(i0 + (lane >> 1)) * kTile + 16 * (lane & 1);
         const int in_page = key - divided(p.by_page, key) * (int)p.by_page.d;
         return (unsigned)id < (unsigned)p.n_pages ? id * p.stride_page + (int64_t)in_page * p.stride_t : (int64_t)-1;
     };
@@ -285,7 +287,7 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
     // (halves that are not there read the other one's rows, or the pool's first: they weigh nothing; rows behind the last key repeat it)
     auto row_base = [&](const Halves &x, int h) __attribute__((always_inline)) { return x.at[h] >= 0 ? x.at[h] : x.at[1 - h] >= 0 ? x.at[1 - h] : 0; };
     auto rows_of = [&](int i, const Halves &x, int h) __attribute__((always_inline)) {   // the last row of a half that may be read
-        const int most = last_key - ((u.first + i) * kWaves + w) * kTile;
+        const int most = last_key - tile_at(i) * kTile;
         if (x.at[0] < 0 && x.at[1] < 0) return 0;
         return min(most - 16 * (x.at[h] >= 0 ? h : 1 - h), 15);
     };
@@ -325,20 +327,21 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
         prefetch_k(0, first), prefetch_v(0, first);
     }
     // queries: in registers, or, where those are all taken, in LDS
-    constexpr bool QL = in_lds(sizeof(T), D) > 0;
+    constexpr bool QL = in_lds(sizeof(T), D) > 0 && !SOLO, QT = in_lds(sizeof(T), D) > 0 && SOLO;   // QT: a few at a time, with every tile again
     static_assert(!QL || RT == 1, "one row tile's");
-    u32x4 qf[RT][QL ? 1 : KS], *lds_q = reinterpret_cast<u32x4 *>(lds + kWaves * PRIV);
+    u32x4 qf[RT][QL || QT ? 1 : KS], *lds_q = reinterpret_cast<u32x4 *>(lds + kWaves * PRIV);
     if constexpr (QL) {
         for (int ks = w; ks < KS; ks += kWaves) lds_q[ks * 64 + lane] = load16<false>(p.q + q_at[0] * (D * (int)sizeof(T)), ks * 64 + grp * 16);
         __syncthreads();
-    } else {
+    } else if constexpr (!QT) {
 #pragma unroll
         for (int t = 0; t < RT; t++)
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) qf[t][ks] = load16<false>(p.q + q_at[t] * (D * (int)sizeof(T)), ks * 64 + grp * 16);
     }
+    bool poisoned = false;   // SOLO
     for (int i = 0; i < n_mine; i++) {
-        const int k_lo = ((u.first + i) * kWaves + w) * kTile;
+        const int k_lo = tile_at(i) * kTile;
         const bool more = i + 1 < n_mine;
         Halves next = {-1, -1};
         if (more) {
@@ -372,7 +375,7 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    const float4_t c = __builtin_bit_cast(float4_t, QL ? lds_q[ks * 64 + lane] : qf[t][QL ? 0 : ks]);
+                    const float4_t c = __builtin_bit_cast(float4_t, QT ? load16<false>(p.q + q_at[t] * (D * (int)sizeof(T)), ks * 64 + grp * 16) : QL ? lds_q[ks * 64 + lane] : qf[t][QL ? 0 : ks]);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {   // (one feature of each group's four at a time)
                         const float4_t a = __builtin_bit_cast(float4_t, kpre[h * KS + ks]);
@@ -446,7 +449,8 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
                 }
                 piece = x;
             }
-            if (found) s_poison = 1;
+            if constexpr (SOLO) poisoned |= __builtin_amdgcn_ballot_w64(found != 0) != 0;
+            else if (found) s_poison = 1;
         }
 
         // ---- O^T += V^T P^T --------------------------------------------------------------------------------
@@ -474,6 +478,33 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
         there = there_next;
     }
 
+    if constexpr (SOLO) {
+        static_assert(RT == 1, "one row tile");
+        float l = l_run[0];
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (lr < u.rows) {
+            Arguments p = arguments_again();
+            T *out = reinterpret_cast<T *>(p.out) + q_row(p, u.b, u.kvh, u.row0 + lr).at * D + 4 * grp;
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
+#pragma unroll
+                for (int y = 0; y < 4; y++) four.e[y] = (T)(o[0][db][y] * inv);
+                *reinterpret_cast<Four *>(out + 16 * db) = four;
+            }
+            if (poisoned)
+#pragma unroll 1
+                for (int x = 0; x < 2 * DB; x++) {
+                    T *at = out + 16 * (x >> 1) + 2 * (x & 1);
+                    const float2_t add = not_finite<T, D>(u, u.row0 + lr, 16 * (x >> 1) + 4 * grp + 2 * (x & 1));
+#pragma unroll
+                    for (int y = 0; y < 2; y++) at[y] = (T)(widen(at[y]) + add[y]);
+                }
+        }
+        return;
+    }
     // ---- the four waves' results joined ------------------------------------------------------------------------
     float *comb = reinterpret_cast<float *>(lds), *comb_ml = comb + kWaves * kRows * CROW;
     constexpr int TPR = kThreads / kRows, PER = D / TPR;   // threads per row, features per thread
@@ -647,7 +678,8 @@ __device__ __forceinline__ int wave_sums(int x) {
 // Where a workgroup stands on the line: what is looked at between stretches alone is in LDS, since the loop needs the scalar registers.
 struct Line { int per, at, end, b, unit, len, steps, first, once, last, poison; };
 
-// A workgroup's stretch, unit by unit.
+// A workgroup's stretch, unit by unit; units of a step a wave each, side by side (200 sequences of 30 keys of 32 heads, f16, 24.7 us, one after the
+// other 50.3; of 64 38.9 | 55.3, of 100 61.1 | 67.2; of 30 to 60, f32, 84.6 | 122).
 template <typename T, int D, int RT, bool MAY_ONCE>
 __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
     const int tid = threadIdx.x;
@@ -663,8 +695,25 @@ __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
             u.end = min(steps, u.first + uniform(s_line.end) - uniform(s_line.at));
             u.part = u.first == 0 && u.end == steps ? nullptr : p.parts + (2 * (int64_t)blockIdx.x + (u.first == 0)) * (RT * kLinePart(D));
         }
-        if (MAY_ONCE && uniform(s_line.once)) stretch_body<T, D, RT, MAY_ONCE>(u, s_line.poison, lds);
-        else stretch_body<T, D, RT, false>(u, s_line.poison, lds);
+        int done = 1;   // units, where they are short
+        if constexpr (RT == 1) {
+            Arguments p = arguments_again();
+            if (u.len <= kStep) done = min(min(kWaves, p.Hkv * (int)p.row_units[0].d - uniform(s_line.unit)), uniform(s_line.end) - uniform(s_line.at));
+        }
+        if (RT == 1 && done > 1) {
+            if constexpr (RT == 1) {
+                const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+                if (w < done) {
+                    Arguments p = arguments_again();
+                    const int unit = uniform(s_line.unit) + w;
+                    u.kvh = divided(p.row_units[0], unit);
+                    u.row0 = (unit - u.kvh * (int)p.row_units[0].d) * kRows, u.rows = min(kRows, p.Sq * p.G - u.row0);
+                    if (MAY_ONCE && uniform(s_line.once)) stretch_body<T, D, 1, MAY_ONCE, true>(u, s_line.poison, lds);
+                    else stretch_body<T, D, 1, false, true>(u, s_line.poison, lds);
+                }
+            }
+        } else if (MAY_ONCE && uniform(s_line.once)) stretch_body<T, D, RT, MAY_ONCE, false>(u, s_line.poison, lds);
+        else stretch_body<T, D, RT, false, false>(u, s_line.poison, lds);
         if (u.part) {
             Arguments p = arguments_again();
             const unsigned per = uniform(s_line.per), unit_at = uniform(s_line.at) - u.first;
@@ -682,12 +731,13 @@ __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
                 for (int y = 0; y < RT && 16 * y < u.rows; y++)
                     join_unit<T, D>(u, y, n, [&](int x) { return parts + ((2 * (int64_t)(first + x) + (x == 0)) * RT + y) * kLinePart(D); }, lds);
         }
-        if (uniform(s_line.at) + u.end - u.first >= uniform(s_line.end)) return;
+        const int steps_done = done > 1 ? done : u.end - u.first;
+        if (uniform(s_line.at) + steps_done >= uniform(s_line.end)) return;
         __syncthreads();   // (everybody has read where the line stands)
         if (tid == 0) {
             Arguments p = arguments_again();
-            s_line.at += u.end - u.first, s_line.first = 0;
-            if (++s_line.unit == p.Hkv * (int)p.row_units[RT >> 1].d) {
+            s_line.at += steps_done, s_line.unit += done, s_line.first = 0;
+            if (s_line.unit == p.Hkv * (int)p.row_units[RT >> 1].d) {
                 const int len = min(max(p.lens[u.b + 1], 0), p.most);
                 s_line.once = p.row_units[RT >> 1].d == 1 && !shares_pages(p, u.b + 1);
                 s_line.unit = 0, s_line.b = u.b + 1, s_line.len = len, s_line.steps = max((len + kStep - 1) / kStep, 1);
@@ -700,7 +750,9 @@ __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
 // RT: row tiles of a unit, which share the keys that it reads.  Where that leaves no more than a step or two per workgroup and tile, units take
 // half as many, and again: what a workgroup does for one tile after the other is then what takes the time.  In us, more tiles and half as many: 2
 // sequences of up to 300 keys, 7 heads' 5 queries 12.9 (four), 9.8, 7.8; 4 of 3000 to 6000, 8 heads' 6 queries 35.3 (four), 26.3; 20 of up to 900, 8
-// heads' 4 queries 20.0 (two), 16.2; beyond the rule 40 of 500 to 900, 4 heads' 5 queries of 128 37.0 (two), 45.2.
+// heads' 4 queries 20.0 (two), 16.2; beyond the rule 40 of 500 to 900, 4 heads' 5 queries of 128 37.0 (two), 45.2.  Where sequences are of two steps
+// on average, or fewer, one tile: a unit of a step is then a wave's (150 of up to 60, 8 heads' 4 queries 17.9 with two tiles, 12.4; 200 of 60 to 200, 4
+// heads' 5 queries of 128 46.5, 43.5).
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[line_lds(sizeof(T), D)];
@@ -713,7 +765,7 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.most); };
         auto steps_of = [&](int len) { return max((len + kStep - 1) / kStep, 1); };   // (one for nothing: its rows are zeros)
 
-        // the line's length (below 2^28: checked by the host), and this workgroup's stretch
+        // the line's length (below 2^28 of units of RT tiles: checked by the host; below 2^30 of any), and this workgroup's stretch
         int len = tid < p.B ? len_of(tid) : 0, mine = tid < p.B ? steps_of(len) : 0, all = mine;
         bool shares = tid < p.B && shares_pages(p, tid);
         for (int b = tid + kThreads; b < p.B; b += kThreads) all += steps_of(len_of(b));
@@ -723,7 +775,7 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         __syncthreads();
         const int all_steps = s_totals[0] + s_totals[1] + s_totals[2] + s_totals[3];   // of one unit of every sequence
         auto units_of = [&](int rt) { return p.Hkv * (int)p.row_units[rt >> 1].d; };   // of a sequence
-        while (rt > 1 && all_steps * units_of(rt) <= rt * (int)gridDim.x) rt >>= 1;
+        while (rt > 1 && (all_steps * units_of(rt) <= rt * (int)gridDim.x || all_steps <= 2 * p.B)) rt >>= 1;
         const int units = units_of(rt), total = all_steps * units;
         const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), 1);
         const int begin = blockIdx.x * per, end = min(begin + per, total);
