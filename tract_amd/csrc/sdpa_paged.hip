@@ -49,6 +49,7 @@ struct PagedDev {
     int *counters;
     float *parts;
     FastDiv by_g, by_workgroups;
+    float part_cost;            // kPartCost, of the rows, for the average of the sequences
     FastDiv row_units[3];       // by the units of a kv head's rows, where they take one, two and four tiles
 };
 
@@ -747,6 +748,12 @@ __device__ __forceinline__ void walk_line(Line &s_line, unsigned char *lds) {
     }
 }
 
+// A unit of s steps in stretches of n is joined out of s / n parts by one workgroup: n + (s / n) c is least at n = sqrt(s c), and c, what a part
+// costs there against a step, goes with its rows (s: of the sequences on average).  Without, with 0.01, 0.02 and 0.04 a row, us: 100000 keys of one kv head
+// with 8 rows 57.7, 34.0, 36.7, 41.9; 2 x 27741 of two with 7 22.8, 20.9, 19.8, 19.8; 5264 of eight with 8, f32, 25.9, 25.8, 22.2, 25.1; 4000 of two with 12
+// 16.2, 16.4, 14.5, 17.3.
+constexpr float kPartCost = 0.02f;
+
 // RT: row tiles of a unit, which share the keys that it reads.  Where that leaves no more than a step or two per workgroup and tile, units take
 // half as many, and again: what a workgroup does for one tile after the other is then what takes the time.  In us, more tiles and half as many: 2
 // sequences of up to 300 keys, 7 heads' 5 queries 12.9 (four), 9.8, 7.8; 4 of 3000 to 6000, 8 heads' 6 queries 35.3 (four), 26.3; 20 of up to 900, 8
@@ -777,7 +784,7 @@ __global__ __launch_bounds__(kThreads, 2) void sdpa_paged_kernel(PagedDev) {
         auto units_of = [&](int rt) { return p.Hkv * (int)p.row_units[rt >> 1].d; };   // of a sequence
         while (rt > 1 && (all_steps * units_of(rt) <= rt * (int)gridDim.x || all_steps <= 2 * p.B)) rt >>= 1;
         const int units = units_of(rt), total = all_steps * units;
-        const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), 1);
+        const int per = max(divided(p.by_workgroups, total + (int)gridDim.x - 1), max((int)__builtin_amdgcn_sqrtf((float)all_steps * p.part_cost), 1));
         const int begin = blockIdx.x * per, end = min(begin + per, total);
         if (begin >= end) return;
         // the sequence where it begins
@@ -857,7 +864,7 @@ int launch_sdpa_paged(const SdpaPagedArgs &a, hipStream_t s) {
         if (seqs > 0) {
             for (int64_t b0 = 0; b0 < a.B; b0 += seqs) {
                 PagedDev part = p;
-                part.B = (int)std::min(seqs, a.B - b0);
+                part.B = (int)std::min(seqs, a.B - b0), part.part_cost = kPartCost * (float)std::min<int64_t>(rows, kRows) / (float)part.B;
                 part.q += b0 * a.Hq * a.Sq * a.D * es, part.out += b0 * a.Hq * a.Sq * a.D * es;
                 part.table += b0 * a.table_width, part.lens += b0;
                 const int n = line_workgroups();
