@@ -1,0 +1,87 @@
+"""Beam search's choice over masked vocabularies: rows whose values are finite and far from zero, and sums made again over rows with -inf."""
+import numpy as np
+import pytest
+
+import tract_amd as ta
+from tests import paged_ref as ref
+from tests.gpu_util import rt  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+F16, F32, I32 = np.float16, np.float32, np.int32
+up = ta.DeviceTensor.from_numpy
+MASKS = [-1e9, -1e10, -1e12, -1e15, -1e18, -1e25, -1e30, -1e38, float(np.finfo(F32).min)]
+
+
+def _check(logits, scores, keep, ended=None, eos=-1):
+    """The choice into buffers that hold something else; the bound on scores as tests/test_gpu_beam_select.py derives it, with a weight's exponent off by
+    three half steps of itself: 3 * 21.5 + 2 + 7 half steps of the sum, and the score's own."""
+    want = ref.select(logits, scores, keep, ended, eos)
+    shape = (logits.shape[0], keep)
+    out = {"scores": up(np.full(shape, 77.0, F32)), **{name: up(np.full(shape, -777, I32)) for name in ("parents", "tokens", "ended")}}
+    got = ta.BeamSelect(keep, eos).eval(up(logits), up(scores), ended=None if ended is None else up(ended), out=out)
+    got = {name: t.to_numpy() for name, t in got.items()}
+    w, g = want["scores"], got["scores"].astype(np.float64)
+    for name in ("parents", "tokens", "ended"):
+        np.testing.assert_array_equal(got[name], want[name], err_msg=name)
+    sure = np.abs(w) < np.finfo(F32).max     # (f32 has no others; those become infinities)
+    assert np.isneginf(g[~sure]).all()
+    assert (np.abs(g[sure] - w[sure]) <= 2.0 ** -24 * np.abs(w[sure]) + 74 * 2.0 ** -24).all(), np.abs(g[sure] - w[sure]).max()
+    return got
+
+
+def _masked(rng, beams, vocab, mask, allowed):
+    """`allowed` tokens of every beam have a logit, the others the mask."""
+    logits = np.full((2, beams, vocab), mask, F32)
+    for i in range(2):
+        for b in range(beams):
+            at = rng.choice(vocab, allowed, replace=False)
+            logits[i, b, at] = rng.standard_normal(allowed) * 3
+    return logits
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("vocab", [70, 3001, 40000])
+def test_few_tokens_are_allowed(rt, mask, vocab):
+    """All that most waves see is the mask."""
+    rng = np.random.default_rng(vocab)
+    for beams, allowed, keep in ((1, 20, 4), (4, 20, 8), (4, 3, 12), (4, 1, 4)):
+        _check(_masked(rng, beams, vocab, mask, allowed), (-rng.random((2, beams))).astype(F32), keep)
+
+
+@pytest.mark.parametrize("value", MASKS + [1e10, 1e20, 3e38])
+@pytest.mark.parametrize("vocab", [9, 3001, 40000])
+def test_rows_of_one_far_value(rt, value, vocab):
+    """A row that is the mask throughout leaves every token score - log(vocab): alone, in all beams, and beside ordinary beams that it wins and loses against."""
+    rng, keep = np.random.default_rng(3), 6
+    row = np.full(vocab, value, F32)
+    _check(row[None, None], np.array([[-1.5]], F32), keep)
+    _check(np.tile(row, (2, 4, 1)), (-rng.random((2, 4))).astype(F32), keep)
+    _check(np.tile(row, (1, 4, 1)), np.zeros((1, 4), F32), keep)
+    mixed = (rng.standard_normal((3, 4, vocab)) * 3).astype(F32)
+    mixed[0, 2], mixed[1, 0], mixed[2, 1:3] = row, row, row
+    for lead in (0.0, 8.0, 30.0):
+        scores = (-rng.random((3, 4))).astype(F32)
+        scores[0, 2] += lead
+        scores[1, 0] += lead
+        scores[2, 1:3] += lead
+        _check(mixed, scores, keep)
+
+
+@pytest.mark.parametrize("far", [1e6, 1e8, 1e10])
+def test_a_largest_value_far_above(rt, far):
+    """One token has nearly all of the weight, and what is below it is far away, too."""
+    rng = np.random.default_rng(5)
+    logits = (rng.standard_normal((2, 3, 9000)) * 3).astype(F32)
+    logits[0, :, 4321] = far
+    logits[1, 1, [7, 8999]] = far
+    _check(logits, np.array([[-1.0, -2.0, -3.0], [-0.5, -0.25, -0.75]], F32), 7)
+
+
+@pytest.mark.parametrize("by", [2.0 ** 20, 2.0 ** 23])
+def test_rows_far_from_zero(rt, by):
+    """Ordinary differences around a value whose last place is 2^-3 or 1: the sum is as good as that of rows around zero."""
+    rng = np.random.default_rng(6)
+    logits = (rng.integers(-12, 1, (2, 4, 20001)) + by).astype(F32)
+    logits[:, :, 777] = by + np.array([3, 4, 5, 6])
+    _check(logits, (-rng.random((2, 4))).astype(F32), 4)
+    _check(-logits, (-rng.random((2, 4))).astype(F32), 4)

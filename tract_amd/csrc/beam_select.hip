@@ -162,10 +162,16 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
     int *list = lds.list[w];
     int n = 0;
     uint32_t bound_key = 0;
-    float least = -INFINITY, m = -INFINITY, top = -INFINITY, c_m = 0.0f;
+    float least = -INFINITY, m = -INFINITY, top = -INFINITY;
     double all = 0.0;
-    // A sum against one reference as a sum against another one: both are exact but for f64.
-    auto against = [&](double sum, float c, float ref) { return ref == -INFINITY ? 0.0 : sum * exp((double)c * 0.6931471805599453 - (double)ref * ((double)kLog2e * 0.6931471805599453)); };
+    // Weights against a reference c, a = log2 e as f32 has it (what a is off by counts for x - m alone: join_request's err has it).  f16: 2^(x a - c)
+    // in one step, c = m a rounded, and what that is off by, 2^-8 at most, is put right with the whole sum.  f32: 2^((x - c) a), c = m itself:
+    // beyond 2^24, where masks are, m a would be off by 1 and more, and from 1e10 on by more than f32 has exponents.
+    constexpr bool kProduct = sizeof(T) == 2;
+    float c_m = 0.0f;
+    auto reference = [&] { return kProduct ? m * kLog2e : m; };
+    auto weight = [&](T v) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(kProduct ? __builtin_fmaf((float)v, kLog2e, -c_m) : ((float)v - c_m) * kLog2e); };
+    auto step = [&](double to) { return exp(kProduct ? to * 0.6931471805599453 : to); };   // of references
     load(0);
 #pragma unroll 1
     for (int turn = 0; turn < turns; turn++) {
@@ -182,20 +188,19 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
         }
         const float now = (float)top_t;
         top = fmaxf(top, now);
-        // Maximum and sum: f32 for the values of a piece, f64 from there on.  A weight is 2^(x a - c) in one step, a = log2 e as f32 has it,
-        // c = m a rounded; what c is off by is put right with the reference, what a is off by counts for x - m alone (join_request's err has
-        // both).  m is the largest value of the first tile, or of a later one that has one more than 2 above.
-        if (__builtin_amdgcn_ballot_w64(now > m + 2.0f)) {
+        // Maximum and sum: f32 for the values of a piece, f64 from there on.  m is the largest value of the first tile, or of a later one that has
+        // one more than 2 above.
+        if (__builtin_amdgcn_ballot_w64(now - m > 2.0f)) {
             const float was = m, c_was = c_m;
             m = wave_most(top);
-            c_m = m * kLog2e;
-            all = was == -INFINITY ? 0.0 : all * exp(((double)c_was - (double)c_m) * 0.6931471805599453);
+            c_m = reference();
+            all = was == -INFINITY ? 0.0 : all * step((double)c_was - (double)c_m);
         }
 #pragma unroll
         for (int c = 0; c < C; c++) {
             float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < kPiece; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf((float)x[c][e], kLog2e, -c_m));
+            for (int e = 0; e < kPiece; e++) sum += weight(x[c][e]);
             all += (double)sum;
         }
         if (__builtin_amdgcn_ballot_w64(all != all) && m < INFINITY) {   // a NaN counts as -inf: the sum so far again
@@ -205,7 +210,7 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
                 const Eight<T> v = piece_at(i);
 #pragma unroll
                 for (int e = 0; e < kPiece; e++) {
-                    const float t = __builtin_amdgcn_exp2f(__builtin_fmaf((float)v[e], kLog2e, -c_m));
+                    const float t = weight(v[e]);
                     all += t == t ? (double)t : 0.0;
                 }
             }
@@ -242,7 +247,7 @@ __device__ __forceinline__ void scan_part(const SelectDev &p, int row, int part,
     const uint32_t wave_bound = max(bound_of_lanes(key_of(top), p.keep), bound_key);
     if (lane == 0) lds.bound[w] = wave_bound;
     if (tid == 0) lds.total = 0;
-    if (m < INFINITY) all = against(all, c_m, m);
+    if (kProduct && m < INFINITY) all = m == -INFINITY ? 0.0 : all * step((double)c_m - (double)m * (double)kLog2e);   // against m (exact but for f64)
     all = wave_sum(all);
     if (lane == 0) lds.max[w] = m, lds.sum[w] = all;
     __syncthreads();
@@ -469,11 +474,12 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             lds.max[beam] = top;
             lds.ended[beam] = ended;
             lds.kind[beam] = dead ? 2 : ended ? 1 : !(fabsf(m) < INFINITY) ? 2 : 0;
-            // What the sum may be off by, relatively, is what its logarithm is: exponents x - ref by a half step of f32 and a quarter for log2 e,
-            // weighted by the weights at most ln vocab - ln l of them (their entropy is ref - x + ln l on average) and twice what lies above the
-            // reference, which is at most `over` and what a wave's may be below its part's, 2; the exponential's two, a piece's seven additions;
-            // f64 from there on.  (ln vocab is at most 0.6932 times the bits of it.)
-            lds.err[beam] = lds.kind[beam] == 0 ? (1.5 * (fmax(0.6932 * (32 - __clz(p.vocab)) - log_l, 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 : 0.0;
+            // What the sum may be off by, relatively, is what its logarithm is: exponents x - ref by a half step of f32, f32's by one more for the
+            // product, and a quarter for log2 e, weighted by the weights at most ln vocab - ln l of them (their entropy is ref - x + ln l on
+            // average) and twice what lies above the reference, which is at most `over` and what a wave's may be below its part's, 2; the
+            // exponential's two, a piece's seven additions; f64 from there on.  (ln vocab is at most 0.6932 times the bits of it.)  The
+            // reference's own weight is 1, so the sum is no less, and no c is NaN: ranks by comparison are a permutation.
+            lds.err[beam] = lds.kind[beam] == 0 ? ((sizeof(T) == 2 ? 1.5 : 2.5) * (fmax(0.6932 * (32 - __clz(p.vocab)) - log_l, 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 : 0.0;
             lds.again[beam] = 0;
         }
     }
