@@ -23,7 +23,7 @@ def _check(logits, scores, keep, ended=None, eos=-1):
     w, g = want["scores"], got["scores"].astype(np.float64)
     for name in ("parents", "tokens", "ended"):
         np.testing.assert_array_equal(got[name], want[name], err_msg=name)
-    sure = np.abs(w) < np.finfo(F32).max     # (f32 has no others; those become infinities)
+    sure = np.abs(w) < float(np.finfo(F32).max) + 2.0 ** 103     # (f32 rounds others to infinities: its last step, halved, is 2^103)
     assert np.isneginf(g[~sure]).all()
     assert (np.abs(g[sure] - w[sure]) <= 2.0 ** -24 * np.abs(w[sure]) + 74 * 2.0 ** -24).all(), np.abs(g[sure] - w[sure]).max()
     return got
@@ -85,3 +85,20 @@ def test_rows_far_from_zero(rt, by):
     logits[:, :, 777] = by + np.array([3, 4, 5, 6])
     _check(logits, (-rng.random((2, 4))).astype(F32), 4)
     _check(-logits, (-rng.random((2, 4))).astype(F32), 4)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("vocab", [13, 3001, 40000])
+def test_sums_made_again_over_masked_rows(rt, dtype, vocab):
+    """Beams that are copies of one another, or others shifted, whose vocabulary is mostly masked: values so near that the exact sums decide, over terms of
+    -inf, of the type's lowest value and NaN."""
+    rng = np.random.default_rng(vocab)
+    base = rng.integers(-4, 5, (3, 1, vocab)).astype(dtype)
+    for mask in (-np.inf, np.finfo(dtype).min, np.nan):
+        hidden = rng.random(base.shape) < 0.7
+        hidden[..., 5] = False
+        same = np.where(hidden, dtype(mask), base).repeat(5, axis=1)
+        zero = np.zeros((3, 5), F32)
+        _check(same, zero, 11)
+        _check(np.where(hidden, dtype(mask), base + rng.integers(-9, 10, (3, 5, 1)).astype(dtype)), zero, 11)
+        _check(rng.permuted(same, axis=2), zero - 3.25, 11)

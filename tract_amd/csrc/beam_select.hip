@@ -355,14 +355,16 @@ struct alignas(16) Choice { double c; int place, beam; };   // place: beam * voc
 
 __device__ __forceinline__ bool before(double c, int place, double d, int other) { return c > d || (c == d && place < other); }
 
-// 2^t for t <= 0 times 2^shift, in f64: the exponential's series for the fraction, of at most a half (the term behind the last is 1e-19).
+// 2^t for t <= 0 times 2^shift, in f64: the exponential's series for the fraction, of at most a half (the term behind the last is 1e-19).  Zero
+// from 2^-2000 on, -inf among them (of which the fraction would be no number).
 __device__ __forceinline__ double exp2_scaled(double t, int shift) {
+    t = fmax(t, -2000.0);
     const double n = __builtin_rint(t), r = (t - n) * 0.6931471805599453;
     double y = 1.0 / 87178291200.0;
     constexpr double kInverse[14] = {1.0 / 6227020800.0, 1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
 #pragma unroll
     for (int i = 0; i < 14; i++) y = __builtin_fma(y, r, kInverse[i]);
-    return __builtin_ldexp(y, (int)fmax(n, -2000.0) + shift);
+    return __builtin_ldexp(y, (int)n + shift);
 }
 
 // log sum exp(x - m) of a row whose largest value is m, the same for the same differences in any order: terms of 64 bits, rounded to whole multiples of
