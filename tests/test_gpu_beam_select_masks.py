@@ -67,7 +67,7 @@ def test_rows_of_one_far_value(rt, value, vocab):
         _check(mixed, scores, keep)
 
 
-@pytest.mark.parametrize("far", [1e6, 1e8, 1e10])
+@pytest.mark.parametrize("far", [1e6, 1e8, 1e10, 1e30, 3e38])
 def test_a_largest_value_far_above(rt, far):
     """One token has nearly all of the weight, and what is below it is far away, too."""
     rng = np.random.default_rng(5)
@@ -102,3 +102,34 @@ def test_sums_made_again_over_masked_rows(rt, dtype, vocab):
         _check(same, zero, 11)
         _check(np.where(hidden, dtype(mask), base + rng.integers(-9, 10, (3, 5, 1)).astype(dtype)), zero, 11)
         _check(rng.permuted(same, axis=2), zero - 3.25, 11)
+
+
+@pytest.mark.parametrize("vocab", [7, 3001, 40000])
+@pytest.mark.parametrize("keep", [1, 5, 64])
+def test_logits_that_one_value_stands_for(rt, vocab, keep):
+    """Where 64 bits hold the same score + log softmax for logits that differ, the lowest places are chosen, not the largest logits: logits next to nothing
+    (alone, among others, beside a far one), and scores that take all of them in."""
+    rng = np.random.default_rng(vocab + keep)
+    keep = min(keep, 3 * vocab)
+    score = np.zeros((2, 3), F32)
+    tiny = (rng.standard_normal((2, 3, vocab)) * 1e-20).astype(F32)
+    _check(tiny, score, keep)
+    _check(tiny, (-rng.random((2, 3))).astype(F32), keep)
+    some = np.where(rng.random(tiny.shape) < 0.5, tiny, F32(-1)).astype(F32)
+    some[:, :, vocab // 2] = [3, 2, 2]
+    _check(some, score, keep)
+    far = (rng.standard_normal((2, 3, vocab)) * 3).astype(F32)
+    far[..., vocab // 3] = 1e25
+    _check(far, score, keep)
+    for dtype, large in ((F32, -1e17), (F32, 1e30), (F16, -3e16), (F16, 1e9)):
+        logits = (rng.standard_normal((2, 3, vocab)) * (3 if abs(large) > 1e10 else 1e-7)).astype(dtype)
+        _check(logits, np.full((2, 3), large, F32), keep)
+        _check(logits, np.array([[large, large, 1.0], [large, -1.0, large]], F32), keep, np.array([[0, 1, 0], [1, 0, 0]], I32), vocab - 2)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_more_of_them_than_are_listed(rt, dtype):
+    """Candidates of equal value beyond what the join lists: 64 beams of 64 candidates each in every part."""
+    rng = np.random.default_rng(9)
+    tiny = (rng.integers(-9, 10, (1, 64, 2500)) * (1e-20 if dtype == F32 else 6e-8)).astype(dtype)
+    _check(tiny, np.full((1, 64), 0.0 if dtype == F32 else 1e9, F32), 64)

@@ -514,6 +514,49 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         p.tokens[at] = token;
         if (p.ended_out) p.ended_out[at] = token == p.eos || lds.ended[beam];
     };
+    // Values that equal the last one chosen go by their places, and of those a part holds the ones of its largest logits alone.  Where 64 bits hold one
+    // c for logits that differ, that is not the same: the value below x is x 2^-25 or more away (f16's 2^-24 at least), and the three roundings of c
+    // are 2^-50 of the sizes that it is made of, so only logits that are next to nothing beside those can do that.
+    auto one_for_several = [&](double cut) {
+        const auto &p = arguments_again<SelectDev>();
+        bool may = false;
+        if (lane < p.beams && lds.kind[lane] == 0 && cut > -INFINITY) {
+            const double score = lds.score[lane], ref = lds.ref[lane], log_sum = lds.log_sum[lane], x = ((cut - score) + log_sum) + ref;
+            const double size = fabs(score) + fabs(x) + fabs(ref) + fabs(log_sum);
+            may = !(fabs(x) > 0x1p-24 * size) && (sizeof(T) == 4 || size >= 0x1p24);
+        }
+        return __builtin_amdgcn_ballot_w64(may) != 0;
+    };
+    // Then a wave looks for all that equal it, in the order of their places, for the ranks from `rank` on.
+    auto choose_equal = [&](double cut, int rank) {
+        const auto &p = arguments_again<SelectDev>();
+        constexpr int kLook = 8;
+        for (int beam = 0; beam < p.beams && rank < p.keep; beam++) {
+            const int kind = lds.kind[beam];
+            const double score = lds.score[beam], ref = lds.ref[beam], log_sum = lds.log_sum[beam];
+            if (kind == 1 && score == cut) {
+                if (lane == 0) chosen(rank, cut, beam * p.vocab + p.eos, beam);
+                rank++;
+            }
+            if (kind != 0) continue;
+            const T *row = reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes);
+            for (int i0 = lane; i0 - lane < p.vocab && rank < p.keep; i0 += kLook * 64) {
+                uint32_t is = 0;
+#pragma unroll
+                for (int e = 0; e < kLook; e++) {
+                    const int i = i0 + e * 64;
+                    is |= i < p.vocab && score + (((double)(float)row[min(i, p.vocab - 1)] - ref) - log_sum) == cut ? 1u << e : 0u;
+                }
+#pragma unroll 1
+                for (int e = 0; __builtin_amdgcn_ballot_w64(is >> e) != 0; e++) {
+                    const uint64_t lanes = __builtin_amdgcn_ballot_w64((is >> e) & 1);
+                    const int at = rank + lanes_below(lanes);
+                    if (((is >> e) & 1) && at < p.keep) chosen(at, cut, beam * p.vocab + i0 + e * 64, beam);
+                    rank += __popcll(lanes);
+                }
+            }
+        }
+    };
     double err = 0.0;
     for (int beam = 0; beam < p.beams; beam++) err = fmax(err, lds.err[beam]);
     for (int again = 0;; again++) {
@@ -658,6 +701,18 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
                     const int2 at = lds.at[tid + y * kThreads];
                     chosen(rank[y], lds.c[tid + y * kThreads], at.x, at.y);
                 }
+            int last = -1;   // where the last one is listed: in the wave that has it
+#pragma unroll
+            for (int y = 0; y < kMine; y++)
+                if (const uint64_t lanes = __builtin_amdgcn_ballot_w64(rank[y] == p.keep - 1)) last = (w + y * kWaves) * 64 + __builtin_ctzll(lanes);
+            const bool several = last >= 0 && one_for_several(lds.c[last]);
+            __syncthreads();   // (all have been put where they go)
+            if (several) {
+                const double cut = lds.c[last];
+                int above = 0;
+                for (int o = 0; o < listed; o++) above += lds.c[o] > cut ? 1 : 0;
+                choose_equal(cut, above);
+            }
             return;
         }
         break;
@@ -666,7 +721,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
     const auto &q = arguments_again<SelectDev>();
     const int all_there = q.beams * q.parts * q.keep;
     double last_c = INFINITY;
-    int last_place = -1;
+    int last_place = -1, above = 0;   // above: ranks of values larger than the last
     for (int rank = 0; rank < q.keep; rank++) {
         Choice best = {-INFINITY, -1, 0};
         for (int j = tid; j < all_there; j += kThreads) {
@@ -685,9 +740,11 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         for (int y = 0; y < kWaves; y++)
             if (lds.best_place[y] >= 0 && (best.place < 0 || before(lds.best_c[y], lds.best_place[y], best.c, best.place))) best = {lds.best_c[y], lds.best_place[y], lds.best_beam[y]};
         if (tid == 0 && best.place >= 0) chosen(rank, best.c, best.place, best.beam);
+        if (best.c < last_c) above = rank;
         last_c = best.c, last_place = best.place;
         __syncthreads();
     }
+    if (w == 0 && one_for_several(last_c)) choose_equal(last_c, above);
 }
 
 template <typename T, int C>
