@@ -411,6 +411,8 @@ struct JoinLds {
     int part[kJoinParts], parts;
     int again[kBeamMaxBeams], any, count, best_place[kWaves], best_beam[kWaves];
     uint32_t bound[kWaves];
+    double cut;   // the last value chosen
+    int above;    // how many are larger, where they were chosen one after the other
 };
 
 // A kernel's one argument where it lies, as loads from here on: kept from the beginning, what only the end looks at would leave too few scalar
@@ -422,6 +424,69 @@ __device__ __forceinline__ const __attribute__((address_space(4))) Args &argumen
     return *reinterpret_cast<const __attribute__((address_space(4))) Args *>(at);
 }
 
+__device__ __forceinline__ void put_chosen(const __attribute__((address_space(4))) SelectDev &p, int request, const JoinLds &lds, int rank, double c, int place, int beam) {
+    const int token = place - beam * p.vocab;
+    const int64_t at = (int64_t)request * p.keep + rank;
+    p.scores_out[at] = (float)c;
+    p.parents[at] = p.row0 + request * p.beams + beam;
+    p.tokens[at] = token;
+    if (p.ended_out) p.ended_out[at] = token == p.eos || lds.ended[beam];
+}
+
+// Values that equal the last one chosen go by their places, and of those a part holds the ones of its largest logits alone.  Where 64 bits hold one c
+// for logits that differ, that is not the same: the value below x is x 2^-25 or more away (f16's 2^-24 at least), and the three roundings of c are
+// 2^-50 of the sizes that it is made of, so only logits that are next to nothing beside those can do that.  A wave's lanes.
+template <typename T>
+__device__ __forceinline__ bool one_for_several(const __attribute__((address_space(4))) SelectDev &p, const JoinLds &lds) {
+    const int lane = threadIdx.x & 63;
+    const double cut = lds.cut;
+    bool may = false;
+    if (lane < p.beams && lds.kind[lane] == 0 && cut > -INFINITY) {
+        const double score = lds.score[lane], ref = lds.ref[lane], log_sum = lds.log_sum[lane], x = ((cut - score) + log_sum) + ref;
+        const double size = fabs(score) + fabs(x) + fabs(ref) + fabs(log_sum);
+        may = !(fabs(x) > 0x1p-24 * size) && (sizeof(T) == 4 || size >= 0x1p24);
+    }
+    return __builtin_amdgcn_ballot_w64(may) != 0;
+}
+
+// Then a wave looks for all that equal it, in the order of their places, for the ranks behind those of larger values.
+template <typename T>
+__device__ __forceinline__ void choose_equal(const __attribute__((address_space(4))) SelectDev &p, int request, const JoinLds &lds) {
+    constexpr int kLook = 8;
+    const int lane = threadIdx.x & 63;
+    const double cut = lds.cut;
+    int rank = 0;
+    if (lds.count > kJoinList) rank = lds.above;
+    else
+        for (int o = 0; o < lds.count; o++) rank += lds.c[o] > cut ? 1 : 0;
+    for (int beam = 0; beam < p.beams && rank < p.keep; beam++) {
+        const int kind = lds.kind[beam];
+        const double score = lds.score[beam], ref = lds.ref[beam], log_sum = lds.log_sum[beam];
+        if (kind == 1 && score == cut) {
+            if (lane == 0) put_chosen(p, request, lds, rank, cut, beam * p.vocab + p.eos, beam);
+            rank++;
+        }
+        if (kind != 0) continue;
+        const T *row = reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes);
+        for (int i0 = lane; i0 - lane < p.vocab && rank < p.keep; i0 += kLook * 64) {
+            uint32_t is = 0;
+#pragma unroll
+            for (int e = 0; e < kLook; e++) {
+                const int i = i0 + e * 64;
+                is |= i < p.vocab && score + (((double)(float)row[min(i, p.vocab - 1)] - ref) - log_sum) == cut ? 1u << e : 0u;
+            }
+#pragma unroll 1
+            for (int e = 0; __builtin_amdgcn_ballot_w64(is >> e) != 0; e++) {
+                const uint64_t lanes = __builtin_amdgcn_ballot_w64((is >> e) & 1);
+                const int at = rank + lanes_below(lanes);
+                if (((is >> e) & 1) && at < p.keep) put_chosen(p, request, lds, at, cut, beam * p.vocab + i0 + e * 64, beam);
+                rank += __popcll(lanes);
+            }
+        }
+    }
+}
+
+// What is chosen, best first.
 template <typename T>
 __device__ __forceinline__ void join_request(const __attribute__((address_space(4))) SelectDev &p, int request, JoinLds &lds) {
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
@@ -505,58 +570,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         const int beam = beam_of(p, j);
         return choice(beam, j - beam * (p.parts * p.keep), get(p.part_best + (int64_t)request * (p.beams * p.parts * p.keep) + j));
     };
-    auto chosen = [&](int rank, double c, int place, int beam) {
-        const auto &p = arguments_again<SelectDev>();
-        const int token = place - beam * p.vocab;
-        const int64_t at = (int64_t)request * p.keep + rank;
-        p.scores_out[at] = (float)c;
-        p.parents[at] = p.row0 + request * p.beams + beam;
-        p.tokens[at] = token;
-        if (p.ended_out) p.ended_out[at] = token == p.eos || lds.ended[beam];
-    };
-    // Values that equal the last one chosen go by their places, and of those a part holds the ones of its largest logits alone.  Where 64 bits hold one
-    // c for logits that differ, that is not the same: the value below x is x 2^-25 or more away (f16's 2^-24 at least), and the three roundings of c
-    // are 2^-50 of the sizes that it is made of, so only logits that are next to nothing beside those can do that.
-    auto one_for_several = [&](double cut) {
-        const auto &p = arguments_again<SelectDev>();
-        bool may = false;
-        if (lane < p.beams && lds.kind[lane] == 0 && cut > -INFINITY) {
-            const double score = lds.score[lane], ref = lds.ref[lane], log_sum = lds.log_sum[lane], x = ((cut - score) + log_sum) + ref;
-            const double size = fabs(score) + fabs(x) + fabs(ref) + fabs(log_sum);
-            may = !(fabs(x) > 0x1p-24 * size) && (sizeof(T) == 4 || size >= 0x1p24);
-        }
-        return __builtin_amdgcn_ballot_w64(may) != 0;
-    };
-    // Then a wave looks for all that equal it, in the order of their places, for the ranks from `rank` on.
-    auto choose_equal = [&](double cut, int rank) {
-        const auto &p = arguments_again<SelectDev>();
-        constexpr int kLook = 8;
-        for (int beam = 0; beam < p.beams && rank < p.keep; beam++) {
-            const int kind = lds.kind[beam];
-            const double score = lds.score[beam], ref = lds.ref[beam], log_sum = lds.log_sum[beam];
-            if (kind == 1 && score == cut) {
-                if (lane == 0) chosen(rank, cut, beam * p.vocab + p.eos, beam);
-                rank++;
-            }
-            if (kind != 0) continue;
-            const T *row = reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes);
-            for (int i0 = lane; i0 - lane < p.vocab && rank < p.keep; i0 += kLook * 64) {
-                uint32_t is = 0;
-#pragma unroll
-                for (int e = 0; e < kLook; e++) {
-                    const int i = i0 + e * 64;
-                    is |= i < p.vocab && score + (((double)(float)row[min(i, p.vocab - 1)] - ref) - log_sum) == cut ? 1u << e : 0u;
-                }
-#pragma unroll 1
-                for (int e = 0; __builtin_amdgcn_ballot_w64(is >> e) != 0; e++) {
-                    const uint64_t lanes = __builtin_amdgcn_ballot_w64((is >> e) & 1);
-                    const int at = rank + lanes_below(lanes);
-                    if (((is >> e) & 1) && at < p.keep) chosen(at, cut, beam * p.vocab + i0 + e * 64, beam);
-                    rank += __popcll(lanes);
-                }
-            }
-        }
-    };
+    auto chosen = [&](int rank, double c, int place, int beam) { put_chosen(arguments_again<SelectDev>(), request, lds, rank, c, place, beam); };
     double err = 0.0;
     for (int beam = 0; beam < p.beams; beam++) err = fmax(err, lds.err[beam]);
     for (int again = 0;; again++) {
@@ -569,7 +583,9 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         uint32_t top = 0;
 #pragma unroll
         for (int y = 0; y < kHeld; y++) {
-            held[y] = held_beam[y] >= 0 ? choice(held_beam[y], held_k[y], first_of[y]) : Choice{-INFINITY, -1, 0};
+            int beam = held_beam[y], k = held_k[y];
+            asm("" : "+v"(beam), "+v"(k));   // (likewise)
+            held[y] = beam >= 0 ? choice(beam, k, first_of[y]) : Choice{-INFINITY, -1, 0};
             if (held[y].place >= 0) top = max(top, key_of((float)held[y].c));
         }
         const int bests = few ? 0 : p.beams * p.parts;
@@ -697,22 +713,14 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         if (whole) {
 #pragma unroll
             for (int y = 0; y < kMine; y++)
+                if (rank[y] == p.keep - 1) lds.cut = lds.c[tid + y * kThreads];
+            __syncthreads();
+#pragma unroll
+            for (int y = 0; y < kMine; y++)
                 if (rank[y] < p.keep) {
                     const int2 at = lds.at[tid + y * kThreads];
                     chosen(rank[y], lds.c[tid + y * kThreads], at.x, at.y);
                 }
-            int last = -1;   // where the last one is listed: in the wave that has it
-#pragma unroll
-            for (int y = 0; y < kMine; y++)
-                if (const uint64_t lanes = __builtin_amdgcn_ballot_w64(rank[y] == p.keep - 1)) last = (w + y * kWaves) * 64 + __builtin_ctzll(lanes);
-            const bool several = last >= 0 && one_for_several(lds.c[last]);
-            __syncthreads();   // (all have been put where they go)
-            if (several) {
-                const double cut = lds.c[last];
-                int above = 0;
-                for (int o = 0; o < listed; o++) above += lds.c[o] > cut ? 1 : 0;
-                choose_equal(cut, above);
-            }
             return;
         }
         break;
@@ -721,7 +729,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
     const auto &q = arguments_again<SelectDev>();
     const int all_there = q.beams * q.parts * q.keep;
     double last_c = INFINITY;
-    int last_place = -1, above = 0;   // above: ranks of values larger than the last
+    int last_place = -1;
     for (int rank = 0; rank < q.keep; rank++) {
         Choice best = {-INFINITY, -1, 0};
         for (int j = tid; j < all_there; j += kThreads) {
@@ -740,11 +748,11 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         for (int y = 0; y < kWaves; y++)
             if (lds.best_place[y] >= 0 && (best.place < 0 || before(lds.best_c[y], lds.best_place[y], best.c, best.place))) best = {lds.best_c[y], lds.best_place[y], lds.best_beam[y]};
         if (tid == 0 && best.place >= 0) chosen(rank, best.c, best.place, best.beam);
-        if (best.c < last_c) above = rank;
+        if (tid == 0 && best.c < last_c) lds.above = rank;
         last_c = best.c, last_place = best.place;
+        if (tid == 0) lds.cut = last_c;
         __syncthreads();
     }
-    if (w == 0 && one_for_several(last_c)) choose_equal(last_c, above);
 }
 
 template <typename T, int C>
@@ -760,7 +768,12 @@ __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
         if (s_last) __hip_atomic_store(p.counters + request, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (s_last) join_request<T>(arguments_again<SelectDev>(), request, lds.join);
+    if (!s_last) return;
+    join_request<T>(arguments_again<SelectDev>(), request, lds.join);
+    const auto &q = arguments_again<SelectDev>();
+    if (!one_for_several<T>(q, lds.join)) return;
+    __syncthreads();   // (all have been put where they go)
+    if (threadIdx.x < 64) choose_equal<T>(q, FastDiv{q.by_beams.d, q.by_beams.mul, q.by_beams.shift}.by(FastDiv{q.by_parts.d, q.by_parts.mul, q.by_parts.shift}.by(blockIdx.x)), lds.join);
 }
 
 // How rows are cut into parts: tiles of 4 pieces of 8 values a thread, or of 1 where there are fewer than an eighth as many tiles as compute
