@@ -581,6 +581,8 @@ int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t 
 /* Attention of q_len new tokens of every sequence over its pages: out = softmax(scale q k^T) v over the first lens[i] tokens, which
  * count the new ones; causal: query r sees tokens up to lens[i] - q_len + r.  A row that sees nothing is zeros.  What a row does not
  * see may hold anything: what lies behind a sequence's last token, in pages that are not its own, in holes, and the later ones of a call's tokens.
+ * The fast kernels round f16's weights to f16 (half a step, 2^-11) before they meet the values, and divide by the sum of the rounded ones; weights of
+ * less than 2^-28 of a row's largest keep fewer bits, below 2^-39 none.  All other sums, weights and maxima are f32.
  *   q, out    : [n_seq, q_heads, q_len, head_dim] dense, not overlapping; q_heads a multiple of kv_heads
  *   workspace : trocm_sdpa_paged_workspace_bytes, 16-byte aligned, initialised by trocm_sdpa_workspace_init and shared like any other;
  *               with one that does for q_len 1 more is read, with a smaller one or NULL a slow kernel runs

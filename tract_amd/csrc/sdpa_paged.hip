@@ -225,6 +225,7 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
     constexpr int LPRW = D * (int)sizeof(T) / 16, RPI = 64 / LPRW, NI = kTile / RPI;   // lanes per key row, rows per load, loads per tile and tensor
     constexpr int KS = D * (int)sizeof(T) / 64;   // 16-byte pieces of a lane's share of a row
     constexpr int NK = H16 ? NI : 2 * KS;
+    constexpr float kMost = H16 ? 15.0f : 0.0f;   // weights are 2^kMost at most
     static_assert(kWaves * kRows * CROW * 4 + kWaves * 2 * kRows * 4 <= kWaves * PRIV, "waves are joined where the tiles were");
 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, grp = lane / 16, lr = lane % 16;
@@ -386,6 +387,8 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
                 }
             if (more) prefetch_k(i + 1, next);
         }
+        int kr = lane / LPRW;
+        asm("" : "+v"(kr));   // (or what is made of it waits in registers, which four row tiles do not have)
         if (odd) {   // rows that are not the sequence's may hold anything
 #pragma unroll
             for (int j = 0; j < NI; j++) {
@@ -414,11 +417,21 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
             for (int x = 1; x < 8; x++) top = fmaxf(top, s[x]);
 #pragma unroll
             for (int d = 16; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-            // f16: the reference moves only when the maximum exceeds it by more than 8 (weights reach 2^8 at most, far inside f16)
-            const bool moved = less(top, m_run[t]) > (H16 ? 8.0f : 0.0f);
-            const float m_new = moved ? top : m_run[t], ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float keep = moved ? __builtin_amdgcn_exp2f(m_run[t] - ref) : 1.0f;
-            m_run[t] = m_new;
+            // f16: weights are f16 numbers of 2^15 at most, which keep all their bits down to 2^-14 and are gone below 2^-25, so the reference is 14
+            // below the maximum where it moves, and moves when the maximum is more than 15 above: 2^-28 of the largest weight is whole, 2^-39 is
+            // something.  (Beside one key with nearly all of the weight, and a value of next to nothing, those are the result.)  Maxima beyond
+            // 2^25, from which 14 may round to 16, are references themselves.
+            const bool moved = less(top, m_run[t]) > kMost;
+            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+                float m_new = H16 ? less(top, kMost - 1.0f) : top;
+                if (H16) m_new = less(top, m_new) > kMost ? top : m_new;
+                const float keep = moved ? __builtin_amdgcn_exp2f(m_run[t] - m_new) : 1.0f;
+                m_run[t] = moved ? m_new : m_run[t];
+                l_run[t] *= keep;
+#pragma unroll
+                for (int db = 0; db < DB; db++) o[t][db] *= keep;
+            }
+            const float ref = m_run[t] == -INFINITY ? 0.0f : m_run[t];
             float sum = 0.0f;
 #pragma unroll
             for (int x = 0; x < 8; x++) {
@@ -431,11 +444,7 @@ __device__ __forceinline__ void stretch_body(const Stretch &u, int &s_poison, un
                 }
                 sum += e[t][x];
             }
-            l_run[t] = l_run[t] * keep + sum;
-            if (__builtin_amdgcn_ballot_w64(moved) != 0) {
-#pragma unroll
-                for (int db = 0; db < DB; db++) o[t][db] *= keep;
-            }
+            l_run[t] += sum;
         }
 
         if (k_lo + kTile > some_see && some_see <= last_key) {
