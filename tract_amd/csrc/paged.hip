@@ -96,9 +96,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanDev p) {
 #pragma unroll
     for (int y = 0; y < kMine; y++) {
         if (y < mine && blockIdx.x == 0 && p.starts) p.starts[i0 + y] = at;
+        const int rows = p.n_tokens - at;   // that are left (not by where it ends: sums stop at 2^30, which may be n_tokens)
         at = add_up_to_top(at, min(max(add[y], 0), kSumTop));
         if (y < mine) s_ends[i0 + y] = at;
-        const bool fit = y < mine && len[y] >= 0 && add[y] >= 0 && len[y] <= p.most && add[y] <= p.most - len[y] && at <= p.n_tokens;
+        const bool fit = y < mine && len[y] >= 0 && add[y] >= 0 && len[y] <= p.most && add[y] <= p.most - len[y] && add[y] <= rows;
         fits |= (fit ? 1u : 0u) << y;
         need[y] = fit ? pages_of(len[y] + add[y]) - pages_of(len[y]) : 0;
         needs = add_up_to_top(needs, need[y]);
