@@ -546,8 +546,8 @@ int trocm_sdpa_cached_scored(const void *q, int q_dtype, int64_t q_heads, int64_
 /* ---- pages: sequences whose keys and values lie in pages of one pool ---------------------------------------------
  * Where the caches above hold a sequence's tokens in planes of its own, these entry points take pages of `page_size` tokens,
  * K and V each a tensor [n_pages, kv_heads, page_size, head_dim] (element strides page_strides[3] for page, head and token, the
- * same for both; NULL: dense), one pair per layer, and one table for all layers: table[i][p] is the page that holds tokens
- * p * page_size .. of sequence i.  Lengths, tables, the stack of free pages and the counts of holders are int32 device memory of the
+ * same for both; NULL: dense; K and V may lie in one another's gaps, as the halves of one tensor), one pair per layer, and one table for
+ * all layers: table[i][p] is the page that holds tokens p * page_size .. of sequence i.  Lengths, tables, the stack of free pages and the counts of holders are int32 device memory of the
  * caller's, read and written by kernels only, so that a recorded step can be replayed.  No counterpart in the reference, whose caches
  * are a tensor per sequence (gpu/src/ops/dyn_kv_cache.rs:58-113).  F32 and F16.
  *

@@ -3,6 +3,7 @@
 #include <string.h>
 #include <algorithm>
 #include <initializer_list>
+#include <numeric>
 #include "common.h"
 
 using namespace trocm;
@@ -68,6 +69,23 @@ size_t pool_bytes(int64_t n_pages, int64_t kv_heads, int64_t page_size, int64_t 
     return (size_t)((n_pages - 1) * st[0] + (kv_heads - 1) * st[1] + (page_size - 1) * st[2] + head_dim) * elem_bytes(dtype);
 }
 
+// Whether two pools of these sizes and strides, `by` bytes apart, lie in one another's gaps (K and V halves of one tensor): with the largest strides
+// outside, whose combinations are multiples of g bytes, and the others inside, which reach over e, what is at least e past a multiple of g and ends
+// before the next one meets nothing.
+bool interleaved(uint64_t by, int64_t n_pages, int64_t kv_heads, int64_t page_size, int64_t head_dim, const int64_t *st, int dtype) {
+    struct Axis { int64_t n, stride; } axes[3] = {{n_pages, st[0]}, {kv_heads, st[1]}, {page_size, st[2]}};
+    std::sort(axes, axes + 3, [](const Axis &a, const Axis &b) { return a.stride > b.stride; });
+    uint64_t g = 0;
+    for (int outer = 1; outer <= 3; outer++) {
+        if (axes[outer - 1].n > 1) g = std::gcd(g, (uint64_t)axes[outer - 1].stride * elem_bytes(dtype));
+        uint64_t e = (uint64_t)head_dim;
+        for (int i = outer; i < 3; i++) e += (uint64_t)(axes[i].n - 1) * (uint64_t)axes[i].stride;
+        e *= elem_bytes(dtype);
+        if (g && by % g >= e && by % g + e <= g) return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -130,7 +148,11 @@ int trocm_paged_append(const void *k_new, const void *v_new, int dtype, int64_t 
         rows[y] = (size_t)((n_tokens - 1) * a.src_strides[y][0] + (kv_heads - 1) * a.src_strides[y][1] + head_dim) * elem_bytes(dtype);
     }
     const size_t pool = pool_bytes(n_pages, kv_heads, page_size, head_dim, a.page_strides, dtype), t = (size_t)n_tokens * 4;
-    if (apart("paged_append", {{k_pages, pool, "k_pages"}, {v_pages, pool, "v_pages"}}, {{k_new, rows[0], "k_new"}, {v_new, rows[1], "v_new"}, {slots, t, "slots"}})) return 1;
+    const std::initializer_list<Range> ins = {{k_new, rows[0], "k_new"}, {v_new, rows[1], "v_new"}, {slots, t, "slots"}};
+    if (apart("paged_append", {{k_pages, pool, "k_pages"}}, ins) || apart("paged_append", {{v_pages, pool, "v_pages"}}, ins)) return 1;
+    const uintptr_t at[2] = {(uintptr_t)k_pages, (uintptr_t)v_pages};
+    TROCM_REQUIRE(!ranges_meet(k_pages, pool, v_pages, pool) || interleaved(std::max(at[0], at[1]) - std::min(at[0], at[1]), n_pages, kv_heads, page_size, head_dim, a.page_strides, dtype),
+                  "paged_append: v_pages overlaps k_pages");
     if (aligned("paged_append", {{k_new, 0, "k_new"}, {v_new, 0, "v_new"}, {k_pages, 0, "k_pages"}, {v_pages, 0, "v_pages"}}, elem_bytes(dtype))) return 1;
     if (aligned("paged_append", {{slots, t, "slots"}}, 4)) return 1;
     hipStream_t s;
