@@ -133,3 +133,19 @@ def test_more_of_them_than_are_listed(rt, dtype):
     rng = np.random.default_rng(9)
     tiny = (rng.integers(-9, 10, (1, 64, 2500)) * (1e-20 if dtype == F32 else 6e-8)).astype(dtype)
     _check(tiny, np.full((1, 64), 0.0 if dtype == F32 else 1e9, F32), 64)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("score", [2.0 ** 51, 2.0 ** 52, 1e15, 3e12])
+def test_values_that_their_own_rounding_decides(rt, dtype, score):
+    """Scores whose last place is about the steps of the logits, which lie half way between two values of 64 bits as often as not: the least that a sum is
+    off by turns them the other way, and with them equal ones and their order, in one beam and between beams that have the same score."""
+    rng, vocab = np.random.default_rng(12), 10481
+    logits = (rng.integers(-400, 401, (2, 5, vocab)) / 4).astype(dtype)
+    logits[..., 5000] = 60000
+    scores = np.full((2, 5), -score, F32)
+    for keep in (1, 7, 50):
+        _check(logits, scores, keep)
+        _check(np.ascontiguousarray(logits[:, :1]), np.ascontiguousarray(scores[:, :1]), keep)
+    scores[1, 1:4] *= F32(0.75)
+    _check(logits, scores, 50)

@@ -433,23 +433,24 @@ __device__ __forceinline__ void put_chosen(const __attribute__((address_space(4)
     if (p.ended_out) p.ended_out[at] = token == p.eos || lds.ended[beam];
 }
 
-// Values that equal the last one chosen go by their places, and of those a part holds the ones of its largest logits alone.  Where 64 bits hold one c
-// for logits that differ, that is not the same: the value below x is x 2^-25 or more away (f16's 2^-24 at least), and the three roundings of c are
-// 2^-50 of the sizes that it is made of, so only logits that are next to nothing beside those can do that.  A wave's lanes.
+// Whether 64 bits may hold one c for logits of a beam that differ: the logit below x is x 2^-25 or more away (f16's 2^-24 at least), and the three
+// roundings of c are 2^-50 of the sizes that it is made of, so only logits that are next to nothing beside those can do that.
 template <typename T>
-__device__ __forceinline__ bool one_for_several(const __attribute__((address_space(4))) SelectDev &p, const JoinLds &lds) {
-    const int lane = threadIdx.x & 63;
-    const double cut = lds.cut;
-    bool may = false;
-    if (lane < p.beams && lds.kind[lane] == 0 && cut > -INFINITY) {
-        const double score = lds.score[lane], ref = lds.ref[lane], log_sum = lds.log_sum[lane], x = ((cut - score) + log_sum) + ref;
-        const double size = fabs(score) + fabs(x) + fabs(ref) + fabs(log_sum);
-        may = !(fabs(x) > 0x1p-24 * size) && (sizeof(T) == 4 || size >= 0x1p24);
-    }
-    return __builtin_amdgcn_ballot_w64(may) != 0;
+__device__ __forceinline__ bool one_for_several(const JoinLds &lds, int beam, double c) {
+    const double score = lds.score[beam], ref = lds.ref[beam], log_sum = lds.log_sum[beam], x = ((c - score) + log_sum) + ref;
+    const bool next_to_nothing = !(fabs(x) > 0x1p-24 * (fabs(score) + fabs(x) + fabs(ref) + fabs(log_sum)));
+    return next_to_nothing & (lds.kind[beam] == 0) & (c > -INFINITY) & (sizeof(T) == 4 || fabs(score) >= 0x1p23);   // (no branches: all loads at once)
 }
 
-// Then a wave looks for all that equal it, in the order of their places, for the ranks behind those of larger values.
+// Values that equal the last one chosen go by their places, and of those a part holds the ones of its largest logits alone: where one value may stand
+// for several logits, all of them have to be looked at, with exact sums.  A wave's lanes.
+template <typename T>
+__device__ __forceinline__ bool more_may_equal(const __attribute__((address_space(4))) SelectDev &p, const JoinLds &lds) {
+    const int lane = threadIdx.x & 63;
+    return __builtin_amdgcn_ballot_w64(one_for_several<T>(lds, lane, lds.cut) & (lane < p.beams)) != 0;
+}
+
+// A wave looks for all that equal the last one chosen, in the order of their places, for the ranks behind those of larger values.
 template <typename T>
 __device__ __forceinline__ void choose_equal(const __attribute__((address_space(4))) SelectDev &p, int request, const JoinLds &lds) {
     constexpr int kLook = 8;
@@ -486,8 +487,8 @@ __device__ __forceinline__ void choose_equal(const __attribute__((address_space(
     }
 }
 
-// What is chosen, best first.
-template <typename T>
+// What is chosen, best first.  EXACT: behind a join, with exact sums for all beams.
+template <typename T, bool EXACT>
 __device__ __forceinline__ void join_request(const __attribute__((address_space(4))) SelectDev &p, int request, JoinLds &lds) {
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int per_row = p.parts * p.keep, n = p.beams * per_row;
@@ -508,7 +509,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         held_beam[y] = j < n ? beam_of(p, j) : -1, held_k[y] = j - held_beam[y] * per_row;
     }
     constexpr int kLanes = 16;   // of a beam
-    for (int beam = tid / kLanes; beam < p.beams; beam += kThreads / kLanes) {
+    for (int beam = EXACT ? p.beams : tid / kLanes; beam < p.beams; beam += kThreads / kLanes) {
         const int64_t row = (int64_t)request * p.beams + beam;
         const float *pm = p.part_max + row * p.parts;
         const double *ps = p.part_sum + row * p.parts;
@@ -545,8 +546,9 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             // product, and a quarter for log2 e, weighted by the weights at most ln vocab - ln l of them (their entropy is ref - x + ln l on
             // average) and twice what lies above the reference, which is at most `over` and what a wave's may be below its part's, 2; the
             // exponential's two, a piece's seven additions; f64 from there on.  (ln vocab is at most 0.6932 times the bits of it.)  The
-            // reference's own weight is 1, so the sum is no less, and no c is NaN: ranks by comparison are a permutation.
-            lds.err[beam] = lds.kind[beam] == 0 ? ((sizeof(T) == 2 ? 1.5 : 2.5) * (fmax(0.6932 * (32 - __clz(p.vocab)) - log_l, 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 : 0.0;
+            // reference's own weight is 1, so the sum is no less, and no c is NaN: ranks by comparison are a permutation.  c's own three roundings,
+            // which a sum that is off may turn the other way, are of 2^-50 of the score and of c at most (c's where it is looked at).
+            lds.err[beam] = lds.kind[beam] == 0 ? ((sizeof(T) == 2 ? 1.5 : 2.5) * (fmax(0.6932 * (32 - __clz(p.vocab)) - log_l, 0.0) + 2.0 * over + 4.0) + 10.0) * 0x1p-24 + 0x1p-50 * fabs((double)score) : 0.0;
             lds.again[beam] = 0;
         }
     }
@@ -571,9 +573,19 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
         return choice(beam, j - beam * (p.parts * p.keep), get(p.part_best + (int64_t)request * (p.beams * p.parts * p.keep) + j));
     };
     auto chosen = [&](int rank, double c, int place, int beam) { put_chosen(arguments_again<SelectDev>(), request, lds, rank, c, place, beam); };
+    auto make_exact = [&](int which) {   // the sums of the beams that are marked so
+        for (int beam = 0; beam < p.beams; beam++)
+            if (lds.again[beam] == which && lds.kind[beam] == 0) {
+                const auto &p = arguments_again<SelectDev>();
+                const double log_sum = exact_log_sum(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, lds.max[beam], lds.sums);
+                if (tid == 0) lds.log_sum[beam] = log_sum, lds.ref[beam] = lds.max[beam], lds.again[beam] = 1;
+            }
+        __syncthreads();
+    };
+    if constexpr (EXACT) make_exact(0);
     double err = 0.0;
     for (int beam = 0; beam < p.beams; beam++) err = fmax(err, lds.err[beam]);
-    for (int again = 0;; again++) {
+    for (int again = EXACT;; again++) {
         // at least `keep` of a wave's candidates reach its bound (of f32, whose order is that of f64 but for ties), so the largest bound will
         // do; all that could be among the best are listed
         int tid = threadIdx.x;
@@ -667,12 +679,12 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             const int j = tid + y * kThreads;
             rank[y] = p.keep;
             if (!whole || j >= listed) continue;
-            const double c = lds.c[j];
+            const double c = lds.c[j], own = c > -INFINITY ? 0x1p-50 * fabs(c) : 0.0;
             int r = 0, near = 0, one = j, two = j;   // near: others; the last two of them
 #pragma unroll 4
             for (int o = 0; o < listed; o++) {
                 const double d = lds.c[o];
-                const bool is_near = !(fabs(d - c) > 2.0 * err) && o != j;   // (two of -inf are)
+                const bool is_near = !(fabs(d - c) > 2.0 * err + own) && o != j;   // (two of -inf are)
                 r += d > c ? 1 : 0;
                 near += is_near ? 1 : 0;
                 two = is_near ? one : two, one = is_near ? o : one;
@@ -683,7 +695,7 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
                     const int2 other = lds.at[o];
                     const double d = lds.c[o], off = lds.err[mine.y] + lds.err[other.y];
                     r += d == c && other.x < mine.x ? 1 : 0;
-                    if (again == 0 && other.y != mine.y && off > 0.0 && fabs(d - c) <= off) lds.again[mine.y] = lds.again[other.y] = 1, lds.any = 1;
+                    if (again == 0 && off > 0.0 && fabs(d - c) <= off + own && (other.y != mine.y || (o != j && one_for_several<T>(lds, mine.y, c)))) lds.again[mine.y] = lds.again[other.y] = 1, lds.any = 1;
                 };
                 if (near <= 2) {   // (itself in place of one that is not there)
                     look(one), look(two);
@@ -693,37 +705,26 @@ __device__ __forceinline__ void join_request(const __attribute__((address_space(
             }
             rank[y] = r;
         }
-        if (again == 0) {
-            if (!whole) {
-                for (int beam = tid; beam < p.beams; beam += kThreads) lds.again[beam] = 1;
-                if (tid == 0) lds.any = 1;
-            }
-            __syncthreads();
-            if (lds.any) {
-                for (int beam = 0; beam < p.beams; beam++)
-                    if (lds.again[beam] && lds.kind[beam] == 0) {
-                        const auto &p = arguments_again<SelectDev>();
-                        const double log_sum = exact_log_sum(reinterpret_cast<const T *>(p.logits + ((int64_t)request * p.beams + beam) * p.row_bytes), p.vocab, lds.max[beam], lds.sums);
-                        if (tid == 0) lds.log_sum[beam] = log_sum, lds.ref[beam] = lds.max[beam];
-                    }
-                __syncthreads();
-                continue;
-            }
+        if (!whole) {
+            if (tid < p.beams) lds.again[tid] = 1;
+            if (tid == 0) lds.any = 1;
         }
-        if (whole) {
 #pragma unroll
-            for (int y = 0; y < kMine; y++)
-                if (rank[y] == p.keep - 1) lds.cut = lds.c[tid + y * kThreads];
-            __syncthreads();
-#pragma unroll
-            for (int y = 0; y < kMine; y++)
-                if (rank[y] < p.keep) {
-                    const int2 at = lds.at[tid + y * kThreads];
-                    chosen(rank[y], lds.c[tid + y * kThreads], at.x, at.y);
-                }
-            return;
+        for (int y = 0; y < kMine; y++)
+            if (rank[y] == p.keep - 1) lds.cut = lds.c[tid + y * kThreads];
+        __syncthreads();
+        if (!EXACT && again == 0 && lds.any) {
+            make_exact(1);
+            continue;
         }
-        break;
+        if (!whole) break;
+#pragma unroll
+        for (int y = 0; y < kMine; y++)
+            if (rank[y] < p.keep) {
+                const int2 at = lds.at[tid + y * kThreads];
+                chosen(rank[y], lds.c[tid + y * kThreads], at.x, at.y);
+            }
+        return;
     }
     // more than the list holds (equal values above all): one after the other
     const auto &q = arguments_again<SelectDev>();
@@ -769,10 +770,13 @@ __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
     }
     __syncthreads();
     if (!s_last) return;
-    join_request<T>(arguments_again<SelectDev>(), request, lds.join);
-    const auto &q = arguments_again<SelectDev>();
-    if (!one_for_several<T>(q, lds.join)) return;
+    join_request<T, false>(arguments_again<SelectDev>(), request, lds.join);
+    if (!more_may_equal<T>(arguments_again<SelectDev>(), lds.join)) return;
     __syncthreads();   // (all have been put where they go)
+    join_request<T, true>(arguments_again<SelectDev>(), request, lds.join);
+    if (!more_may_equal<T>(arguments_again<SelectDev>(), lds.join)) return;
+    __syncthreads();
+    const auto &q = arguments_again<SelectDev>();
     if (threadIdx.x < 64) choose_equal<T>(q, FastDiv{q.by_beams.d, q.by_beams.mul, q.by_beams.shift}.by(FastDiv{q.by_parts.d, q.by_parts.mul, q.by_parts.shift}.by(blockIdx.x)), lds.join);
 }
 
