@@ -618,6 +618,7 @@ int trocm_paged_copy(const int32_t *copies, int64_t n_copies, void *const *pools
  * beams and the vocabulary the `keep` largest, largest first, equal ones by ascending beam * vocab + token; c is compared in
  * 64 bits, as scores[b] + ((logits[b][v] - max) - log(sum exp(logits[b] - max))) with sums right to 2^-51 + vocab * 2^-62: values of
  * different beams that are nearer than that come in either order, but for beams with the same differences of logits, whose sums are the same.
+ * scores_out is c rounded, or, where no two values were near enough to ask for sums of 64 bits, c of sums of weights of 32: 2^-18 at most beside its half step.
  *   logits     : rows of `vocab` for batch * beams beams, row_stride elements apart (0: dense)
  *   scores     : [batch, beams] f32; one that is infinite or NaN leaves its beam only candidates of -inf, and so do logits without a finite largest one
  *   ended      : [batch, beams] int32 or NULL: a beam with one that is not 0 has a single candidate, its score as it is with token `eos`

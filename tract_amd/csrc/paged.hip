@@ -406,8 +406,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_reclaim_kernel(ReorderDev 
 }
 
 // All of it by one workgroup, with the counts of holders in LDS, where pages and tables are few: three launches and their memory accesses
-// cost more than the one compute unit takes (one | three launches, with the copies that follow: 64 sequences of 46 entries 12.7 | 15.0 to 17.8 us,
-// 128 14.8 | 14.9 to 17.8, 256, in eight layers, 29.2 | 25.7).
+// cost more than the one compute unit takes (one | three launches, with the copies that follow, by entries: 8 a sequence 1536 11.4 | 17.7 us, 6144
+// 16.7 | 17.6, 12288 23.5 | 20.0; 46 a sequence 2944 12.1 | 17.7, 5888 14.8 | 17.7, 11776 20.3 | 17.8; 256 a sequence 1536 11.0 | 17.7, 6144 15.3 | 17.8,
+// 12288 20.2 | 17.9).
 constexpr int kSmallPages = kReclaim, kSmallEntries = 6144;
 // The argument where it lies, as loads from here on: kept from the beginning, it would not leave enough scalar registers.
 __device__ __forceinline__ ReorderDev arguments_again() {
