@@ -779,10 +779,14 @@ __global__ __launch_bounds__(kThreads, 4) void beam_select_kernel(SelectDev p) {
     if (!s_last) return;
     join_request<T, false>(arguments_again<SelectDev>(), request, lds.join);
     if (!more_may_equal<T>(arguments_again<SelectDev>(), lds.join)) return;
+    const int beam = threadIdx.x & 63;
+    const bool inexact = __builtin_amdgcn_ballot_w64(beam < arguments_again<SelectDev>().beams && lds.join.kind[beam] == 0 && !lds.join.again[beam]) != 0;
     __syncthreads();   // (all have been put where they go)
-    join_request<T, true>(arguments_again<SelectDev>(), request, lds.join);
-    if (!more_may_equal<T>(arguments_again<SelectDev>(), lds.join)) return;
-    __syncthreads();
+    if (inexact) {
+        join_request<T, true>(arguments_again<SelectDev>(), request, lds.join);
+        if (!more_may_equal<T>(arguments_again<SelectDev>(), lds.join)) return;
+        __syncthreads();
+    }
     const auto &q = arguments_again<SelectDev>();
     if (threadIdx.x < 64) choose_equal<T>(q, FastDiv{q.by_beams.d, q.by_beams.mul, q.by_beams.shift}.by(FastDiv{q.by_parts.d, q.by_parts.mul, q.by_parts.shift}.by(blockIdx.x)), lds.join);
 }
